@@ -558,6 +558,95 @@ int unblend_lstm_recurrence_bf16(const float* xp, const float* whh_t, float* h_o
 /* Device flag set when a bounded wait of unblend_lstm_recurrence_bf16 gives up (0 = none). Synchronous. */
 int unblend_lstm_error_flag(int* out_host, int clear);
 
+/*
+ * Training operators: layer norm, attention and dropout-add with their gradients, for fine-tuning the
+ * transformers of the separation models (the pre-norm block x + LayerScale * dropout(attention(layer_norm(x))),
+ * unblend/transformer.py:290-301, 328-359, unblend/roformer.py:478-511). Element types are named by UnblendDtype; sums,
+ * statistics and softmax are fp32. Results do not depend on scheduling: no floating-point atomics. Outputs are
+ * contiguous unless strides are given; inputs may have any strides with a unit last one.
+ */
+enum UnblendDtype { UNBLEND_F32 = 0, UNBLEND_BF16 = 1, UNBLEND_F16 = 2 };
+
+/*
+ * y = (x - mean) * rstd * gamma + beta over rows of `cols` elements, stats[row] = (mean, rstd) (float2) for the
+ * backward pass. Row (o, i) of x starts at x + o * x_so + i * x_si, i < inner, o < outer (fewer than 2^31 rows); y is
+ * contiguous. gamma / beta may be NULL; their type w_dtype is fp32 or x's (the gradients' too).
+ */
+int unblend_layer_norm_forward(const void* x, long long x_so, long long x_si, void* y, float* stats,
+                               const void* gamma, const void* beta, float eps, long long outer, long long inner,
+                               int cols, int dtype, int w_dtype, void* stream);
+
+/* dx (contiguous), and dgamma / dbeta [cols] (both or neither) from dy, x and the forward's stats. work:
+ * unblend_layer_norm_grad_workspace bytes, 16-byte aligned (not needed without dgamma). */
+int unblend_layer_norm_backward(const void* dy, long long dy_so, long long dy_si, const void* x, long long x_so,
+                                long long x_si, const float* stats, const void* gamma, void* dx, void* dgamma,
+                                void* dbeta, float* work, long long outer, long long inner, int cols, int dtype,
+                                int w_dtype, void* stream);
+int unblend_layer_norm_grad_workspace(long long rows, int cols, long long* bytes);
+
+/*
+ * y = residual + scale[c] * keep * x / (1 - p): dropout of a residual branch with its LayerScale
+ * (unblend/transformer.py:290-301, 328-359). Element e = row * cols + c is kept when word e % 4 of Philox-4x32-10 with
+ * key seed and counter (e / 4, offset) is >= round(p 2^32); rng is a device array of (seed, offset), two 64-bit
+ * integers. The mask is never stored: the backward pass draws it again. x and dx have type dtype, residual, y and
+ * dy r_dtype (fp32 or dtype), scale and dscale w_dtype (fp32 or dtype); residual and scale may be NULL. Row
+ * addressing as in unblend_layer_norm_forward, y and dx contiguous.
+ */
+int unblend_dropout_add_forward(const void* x, long long x_so, long long x_si, const void* residual, long long r_so,
+                                long long r_si, const void* scale, void* y, double p, const void* rng,
+                                long long outer, long long inner, int cols, int dtype, int r_dtype, int w_dtype,
+                                void* stream);
+
+/* dx = scale[c] * keep * dy / (1 - p) and, when dscale is set, dscale[c] = sum_rows keep * x * dy / (1 - p) (x is
+ * read only for it). work: unblend_dropout_add_grad_workspace bytes (not needed without dscale). */
+int unblend_dropout_add_backward(const void* dy, long long dy_so, long long dy_si, const void* x, long long x_so,
+                                 long long x_si, const void* scale, void* dx, void* dscale, float* work, double p,
+                                 const void* rng, long long outer, long long inner, int cols, int dtype,
+                                 int dy_dtype, int w_dtype, void* stream);
+int unblend_dropout_add_grad_workspace(long long rows, int cols, long long* bytes);
+
+/*
+ * Multi-head attention with gradients. Sequence (o, i), row r, head h, dim d of a tensor is at
+ * base + o * outer + i * inner + r * row + h * head + d (strides in elements). Query head h reads key/value head
+ * h / (heads / kv_heads).
+ *
+ *   score[i, j] = scale * q_i . k_j for the keys j that query i sees, P = softmax, out = P V,
+ *   lse[sequence, head, i] = log sum_j exp(score[i, j])  (float, [outer * inner, heads, lq])
+ *
+ * q_lens / k_lens (device, [outer * inner], may be NULL; clamped to [0, lq] / [0, lk]) give each sequence's
+ * own lengths in a padded batch. With causal, query i sees keys j <= i + k_len - q_len: the last query sees every
+ * key. A query that sees no key, and rows behind q_len, have out = 0 and lse = -inf and add nothing to any
+ * gradient; rows of dk and dv behind k_len are 0. What lies in rows behind the lengths, NaN included, is not used;
+ * NaN or infinities within them may reach any output of their sequence.
+ */
+typedef struct {
+  long long outer, inner, row, head;
+} UnblendHeadStrides;
+
+typedef struct {
+  int dtype; /* UnblendDtype of q, k, v, out, dout, dq, dk, dv */
+  int outer, inner, heads, kv_heads, lq, lk, hd; /* hd <= 128 */
+  int causal;
+  float scale;
+  const int* q_lens;
+  const int* k_lens;
+  UnblendHeadStrides q, k, v, out;
+  UnblendHeadStrides dout, dq, dk, dv; /* backward only */
+} UnblendAttnTrainParams;
+
+/* Workspace bytes of a call (0: none needed, work may be NULL). */
+int unblend_attention_workspace(const UnblendAttnTrainParams* p, int backward, long long* bytes);
+
+int unblend_attention_forward(const void* q, const void* k, const void* v, void* out, float* lse, void* work,
+                              long long work_bytes, const UnblendAttnTrainParams* p, void* stream);
+
+/* dv = P^T dout, dS = P * (dout V^T - rowsum(dout * out)), dq = scale dS K, dk = scale dS^T Q; dk and dv are summed
+ * over the query heads that share a key/value head. P is computed again from q, k and lse. */
+int unblend_attention_backward(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                               const float* lse, void* dq, void* dk, void* dv, void* work, long long work_bytes,
+                               const UnblendAttnTrainParams* p, void* stream);
+
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,7 @@ c_void_p = ctypes.c_void_p
 ACT_NONE, ACT_GELU, ACT_GLU, ACT_TANH, ACT_SWISH = 0, 1, 2, 3, 4
 PRO_NONE, PRO_GN_GELU, PRO_ADD = 0, 1, 2
 GEMM_MAX_GROUPS = 64
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 
 
 class ConvParams(ctypes.Structure):
@@ -78,6 +79,24 @@ class GemmParams(ctypes.Structure):
         ("groups", c_int), ("group", ctypes.POINTER(GemmGroup)), ("bias", c_void_p), ("act", c_int),
         ("res", c_void_p), ("ldr", c_ll), ("out", c_void_p), ("ldo", c_ll), ("out_bf16", c_int),
         ("rope", c_void_p), ("rope_cols", c_int), ("rope_hd", c_int), ("rope_div", c_int), ("rope_mod", c_int),
+    ]
+
+
+class HeadStrides(ctypes.Structure):
+    """Mirror of ``UnblendHeadStrides``."""
+
+    _fields_ = [("outer", c_ll), ("inner", c_ll), ("row", c_ll), ("head", c_ll)]
+
+
+class AttnTrainParams(ctypes.Structure):
+    """Mirror of ``UnblendAttnTrainParams``."""
+
+    _fields_ = [
+        ("dtype", c_int), ("outer", c_int), ("inner", c_int), ("heads", c_int), ("kv_heads", c_int),
+        ("lq", c_int), ("lk", c_int), ("hd", c_int), ("causal", c_int), ("scale", c_float),
+        ("q_lens", c_void_p), ("k_lens", c_void_p),
+        ("q", HeadStrides), ("k", HeadStrides), ("v", HeadStrides), ("out", HeadStrides),
+        ("dout", HeadStrides), ("dq", HeadStrides), ("dk", HeadStrides), ("dv", HeadStrides),
     ]
 
 
@@ -152,6 +171,18 @@ _SIGNATURES = {
     "unblend_lstm_error_flag": [c_void_p, c_int],
     "unblend_istft_masked": [c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                              c_int, c_int, c_int, c_int, c_void_p],
+    "unblend_layer_norm_forward": [c_void_p, c_ll, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_ll, c_ll,
+                                   c_int, c_int, c_int, c_void_p],
+    "unblend_layer_norm_backward": [c_void_p, c_ll, c_ll, c_void_p, c_ll, c_ll, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_ll, c_ll, c_int, c_int, c_int, c_void_p],
+    "unblend_dropout_add_forward": [c_void_p, c_ll, c_ll, c_void_p, c_ll, c_ll, c_void_p, c_void_p, c_double, c_void_p,
+                                    c_ll, c_ll, c_int, c_int, c_int, c_int, c_void_p],
+    "unblend_dropout_add_backward": [c_void_p, c_ll, c_ll, c_void_p, c_ll, c_ll, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_double, c_void_p, c_ll, c_ll, c_int, c_int, c_int, c_int, c_void_p],
+    "unblend_attention_forward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll,
+                                  ctypes.POINTER(AttnTrainParams), c_void_p],
+    "unblend_attention_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_ll, ctypes.POINTER(AttnTrainParams), c_void_p],
 }
 
 # Entry points without a stream argument.
@@ -161,6 +192,9 @@ _HOST_SIGNATURES = {
     "unblend_gemm_error_flag": [ctypes.POINTER(c_int), c_int],
     "unblend_attention_bf16_error_flag": [ctypes.POINTER(c_int), c_int],
     "unblend_dconv_error_flag": [ctypes.POINTER(c_int), c_int],
+    "unblend_layer_norm_grad_workspace": [c_ll, c_int, ctypes.POINTER(c_ll)],
+    "unblend_dropout_add_grad_workspace": [c_ll, c_int, ctypes.POINTER(c_ll)],
+    "unblend_attention_workspace": [ctypes.POINTER(AttnTrainParams), c_int, ctypes.POINTER(c_ll)],
 }
 
 # Tensor-core convolution modes (unblend_conv2d_tc): 3-pass TF32, bf16, 3-pass bf16,
@@ -247,7 +281,10 @@ def check(name: str, rc: int) -> None:
 
 
 # Kernels launched by one call of each entry point (1 unless listed).
-KERNELS_PER_CALL = {"unblend_mean_std": 3, "unblend_istft_output": 2, "unblend_istft_masked": 2}
+# The joins of split attention calls depend on the sizes and are not counted.
+KERNELS_PER_CALL = {"unblend_mean_std": 3, "unblend_istft_output": 2, "unblend_istft_masked": 2,
+                    "unblend_layer_norm_backward": 2, "unblend_dropout_add_backward": 2,
+                    "unblend_attention_backward": 2}
 
 # Launch accounting: total kernels launched through this binding.
 counters = {"launches": 0}

@@ -1,0 +1,605 @@
+// Attention with gradients: entry points, and the fp32 CUDA-core kernels.
+//
+//   S = scale Q K^T (masked),  lse = log sum_j exp S,  P = exp(S - lse),  O = P V
+//   D = rowsum(dO * O),  dV = P^T dO,  dS = P * (dO V^T - D),  dQ = scale dS K,  dK = scale dS^T Q
+//
+// Nothing of size lq x lk is stored: the forward pass keeps a running maximum and sum per query and leaves lse, the
+// backward pass computes P again from it. The backward pass is two kernels, one walking the keys for a tile of
+// queries (dQ, and D on the way), one walking the queries of all heads of a group for a tile of keys (dK, dV); each
+// output element belongs to one CTA, so nothing is added by atomics and the result is the same on every run, for two
+// products more than the five that one kernel with atomics would need.
+// When the tiles are too few to fill the GPU the walked axis is split and the parts joined in order by another kernel.
+//
+// The kernels here take every type, stride and alignment, and are the path of fp32: 64 x 64 score tiles on 256
+// threads, 4 x 4 scores per thread, operands in shared memory as fp32 (transposed where the head axis is summed).
+#include "attention_train.cuh"
+
+namespace {
+
+using namespace ub::train;
+
+constexpr int TILE = 64;
+constexpr int NT = 256;
+constexpr int LD = TILE + 4;  // row pitch of [dim][row] tiles: 16-byte rows, 4-bank shift per dim
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+// Rows [r0, r0 + 64) of a head into shared memory: transposed [dim][LD] and / or as rows [row][HDP + 4]. Rows from
+// `valid` on and dims from hd up to a multiple of 4 become 0. Lane = row, so the transposed stores do not conflict.
+template <typename T, int HDP, bool TRANS, bool ROWS>
+__device__ __forceinline__ void load_tile(const T* base, long long row_stride, int r0, int valid, int hd, bool vec,
+                                          float* trans, float* rows) {
+  const int row = threadIdx.x & 63, part = threadIdx.x >> 6;
+  const bool in = r0 + row < valid;
+  const T* p = base + (long long)(r0 + row) * row_stride;
+  for (int d = part * 4; d < hd; d += 16) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (in) {
+      if (vec) {
+        load_vec<T, 4>(p + d, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < hd) v[e] = to_f(p[d + e]);
+      }
+    }
+    if constexpr (TRANS) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) trans[(d + e) * LD + row] = v[e];
+    }
+    if constexpr (ROWS) *reinterpret_cast<float4*>(rows + row * (HDP + 4) + d) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+
+// acc[r][c] = sum_d A[d][4 ty + r] * B[d][4 tx + c]
+__device__ __forceinline__ void mm_nt(float2 (&acc)[4][2], const float* A, const float* B, int hd, int ty, int tx) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) acc[r][0] = acc[r][1] = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int d = 0; d < hd; ++d) {
+    const float4 a = *reinterpret_cast<const float4*>(A + d * LD + 4 * ty);
+    const float4 b = *reinterpret_cast<const float4*>(B + d * LD + 4 * tx);
+    const float ar[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float2 rr = make_float2(ar[r], ar[r]);
+      acc[r][0] = ub::fma2(rr, make_float2(b.x, b.y), acc[r][0]);
+      acc[r][1] = ub::fma2(rr, make_float2(b.z, b.w), acc[r][1]);
+    }
+  }
+}
+
+// acc[r][g] += sum_j W[j][4 ty + r] * B[j][64 g + 4 tx ..]
+template <int HDP>
+__device__ __forceinline__ void mm_wn(float2 (&acc)[4][HDP / 64][2], const float* W, const float* B, int ty, int tx) {
+#pragma unroll 4
+  for (int j = 0; j < TILE; ++j) {
+    const float4 w = *reinterpret_cast<const float4*>(W + j * LD + 4 * ty);
+    const float wr[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int g = 0; g < HDP / 64; ++g) {
+      const float4 b = *reinterpret_cast<const float4*>(B + j * (HDP + 4) + 64 * g + 4 * tx);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float2 rr = make_float2(wr[r], wr[r]);
+        acc[r][g][0] = ub::fma2(rr, make_float2(b.x, b.y), acc[r][g][0]);
+        acc[r][g][1] = ub::fma2(rr, make_float2(b.z, b.w), acc[r][g][1]);
+      }
+    }
+  }
+}
+
+template <int HDP>
+__device__ __forceinline__ void zero(float2 (&acc)[4][HDP / 64][2]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int g = 0; g < HDP / 64; ++g) acc[r][g][0] = acc[r][g][1] = make_float2(0.f, 0.f);
+}
+
+// One accumulator row (64 g + 4 tx + e over all tx, g) times mul to out[d] (T) or to a fp32 part row.
+template <typename T, int HDP>
+__device__ __forceinline__ void store_row(const float2 (&acc)[HDP / 64][2], float mul, T* out, int hd, int tx) {
+#pragma unroll
+  for (int g = 0; g < HDP / 64; ++g) {
+    const float v[4] = {acc[g][0].x * mul, acc[g][0].y * mul, acc[g][1].x * mul, acc[g][1].y * mul};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 64 * g + 4 * tx + e;
+      if (d < hd) out[d] = from_f<T>(v[e]);
+    }
+  }
+}
+
+// Over the 16 lanes (tx) that share a row.
+__device__ __forceinline__ float row_max16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float row_sum16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+struct Unit {
+  int seq, h, tile, split;
+};
+
+__device__ __forceinline__ Unit unit_of(int tiles, int heads, int splits) {
+  unsigned u = blockIdx.x;
+  Unit r;
+  r.split = u % splits;
+  u /= splits;
+  r.tile = u % tiles;
+  u /= tiles;
+  r.h = u % heads;
+  r.seq = u / heads;
+  return r;
+}
+
+template <typename T, int HDP>
+__global__ void __launch_bounds__(NT) attention_fwd_kernel(const __grid_constant__ AttnArgs a, int vec) {
+  extern __shared__ float smem[];
+  float* sQ = smem;                      // [HDP][LD]
+  float* sK = sQ + HDP * LD;             // [HDP][LD]
+  float* sV = sK + HDP * LD;             // [64][HDP + 4]
+  float* sP = sV + TILE * (HDP + 4);     // [64 keys][LD]
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const Unit u = unit_of((a.lq + TILE - 1) / TILE, a.heads, a.splits);
+  const Bounds b = bounds_of(a, u.seq);
+  const int i0 = u.tile * TILE;
+  const T* q = static_cast<const T*>(a.q) + head_offset(a.q_s, a, u.seq, u.h);
+  const T* k = static_cast<const T*>(a.k) + head_offset(a.k_s, a, u.seq, u.h / a.group);
+  const T* v = static_cast<const T*>(a.v) + head_offset(a.v_s, a, u.seq, u.h / a.group);
+  const int tiles = (key_end(a, b, i0, TILE) + TILE - 1) / TILE;
+  const int t0 = (int)((long long)tiles * u.split / a.splits), t1 = (int)((long long)tiles * (u.split + 1) / a.splits);
+  float2 o[4][HDP / 64][2];
+  zero<HDP>(o);
+  float m[4], l[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) m[r] = -INFINITY, l[r] = 0.f;
+  const float c = a.scale * LOG2E;
+  const int hd = a.hd;
+  if (t0 < t1) load_tile<T, HDP, true, false>(q, a.q_s.row, i0, b.ql, hd, vec, sQ, nullptr);
+  for (int t = t0; t < t1; ++t) {
+    const int j0 = t * TILE;
+    __syncthreads();
+    load_tile<T, HDP, true, false>(k, a.k_s.row, j0, b.kl, hd, vec, sK, nullptr);
+    load_tile<T, HDP, false, true>(v, a.v_s.row, j0, b.kl, hd, vec, nullptr, sV);
+    __syncthreads();
+    float2 s[4][2];
+    mm_nt(s, sQ, sK, hd, ty, tx);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x[4] = {s[r][0].x * c, s[r][0].y * c, s[r][1].x * c, s[r][1].y * c};
+      float top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (!sees(a, b, i0 + 4 * ty + r, j0 + 4 * tx + e)) x[e] = -INFINITY;
+        top = fmaxf(top, x[e]);
+      }
+      top = fmaxf(row_max16(top), m[r]);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float corr = exp2f(m[r] - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = exp2f(x[e] - base);
+        sum += p;
+        sP[(4 * tx + e) * LD + 4 * ty + r] = p;
+      }
+      l[r] = l[r] * corr + row_sum16(sum);
+      m[r] = top;
+#pragma unroll
+      for (int g = 0; g < HDP / 64; ++g)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) o[r][g][e].x *= corr, o[r][g][e].y *= corr;
+    }
+    __syncthreads();
+    mm_wn<HDP>(o, sP, sV, ty, tx);
+  }
+  const long long rows = (long long)a.seqs * a.heads * a.lq;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = i0 + 4 * ty + r;
+    if (i >= a.lq) continue;
+    const long long row = ((long long)u.seq * a.heads + u.h) * a.lq + i;
+    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+    const float lse = m[r] == -INFINITY ? -INFINITY : (m[r] + log2f(l[r])) * LN2;
+    if (a.splits > 1) {
+      store_row<float, HDP>(o[r], inv, a.part + (u.split * rows + row) * hd, hd, tx);
+      if (tx == 0) a.part_lse[u.split * rows + row] = lse;
+    } else {
+      store_row<T, HDP>(o[r], inv,
+                        static_cast<T*>(a.out) + head_offset(a.out_s, a, u.seq, u.h) + (long long)i * a.out_s.row, hd,
+                        tx);
+      if (tx == 0 && a.lse) a.lse[row] = lse;
+    }
+  }
+}
+
+// dQ of 64 queries of one head; D = rowsum(dO * O) on the way (its first split leaves it for the dk / dv kernel).
+template <typename T, int HDP>
+__global__ void __launch_bounds__(NT) attention_dq_kernel(const __grid_constant__ AttnArgs a, int vec) {
+  extern __shared__ float smem[];
+  float* sQ = smem;                       // [HDP][LD]
+  float* sO = sQ + HDP * LD;              // [HDP][LD] dO
+  float* sV = sO + HDP * LD;              // [HDP][LD]
+  float* sK = sV + HDP * LD;              // [HDP][LD]
+  float* sKr = sK + HDP * LD;             // [64][HDP + 4]
+  float* sS = sKr + TILE * (HDP + 4);     // [64 keys][LD]
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const Unit u = unit_of((a.lq + TILE - 1) / TILE, a.heads, a.splits);
+  const Bounds b = bounds_of(a, u.seq);
+  const int i0 = u.tile * TILE;
+  const T* q = static_cast<const T*>(a.q) + head_offset(a.q_s, a, u.seq, u.h);
+  const T* dout = static_cast<const T*>(a.dout) + head_offset(a.dout_s, a, u.seq, u.h);
+  const T* out = static_cast<const T*>(a.out_in) + head_offset(a.out_s, a, u.seq, u.h);
+  const T* k = static_cast<const T*>(a.k) + head_offset(a.k_s, a, u.seq, u.h / a.group);
+  const T* v = static_cast<const T*>(a.v) + head_offset(a.v_s, a, u.seq, u.h / a.group);
+  const long long row0 = ((long long)u.seq * a.heads + u.h) * a.lq;
+  const int tiles = (key_end(a, b, i0, TILE) + TILE - 1) / TILE;
+  const int t0 = (int)((long long)tiles * u.split / a.splits), t1 = (int)((long long)tiles * (u.split + 1) / a.splits);
+  const int hd = a.hd;
+  float D[4], lse[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = i0 + 4 * ty + r;
+    float s = 0.f;
+    lse[r] = -INFINITY;
+    if (i < b.ql) {
+      lse[r] = a.lse[row0 + i];
+      if (lse[r] != -INFINITY)
+        for (int d = tx; d < hd; d += 16)
+          s = fmaf(to_f(dout[i * a.dout_s.row + d]), to_f(out[i * a.out_s.row + d]), s);
+    }
+    D[r] = row_sum16(s);
+    if (i < a.lq && tx == 0 && u.split == 0) a.dsum[row0 + i] = D[r];
+  }
+  float2 acc[4][HDP / 64][2];
+  zero<HDP>(acc);
+  const float c = a.scale * LOG2E;
+  if (t0 < t1) {
+    load_tile<T, HDP, true, false>(q, a.q_s.row, i0, b.ql, hd, vec, sQ, nullptr);
+    load_tile<T, HDP, true, false>(dout, a.dout_s.row, i0, b.ql, hd, vec, sO, nullptr);
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int j0 = t * TILE;
+    __syncthreads();
+    load_tile<T, HDP, true, true>(k, a.k_s.row, j0, b.kl, hd, vec, sK, sKr);
+    load_tile<T, HDP, true, false>(v, a.v_s.row, j0, b.kl, hd, vec, sV, nullptr);
+    __syncthreads();
+    float2 s[4][2], dp[4][2];
+    mm_nt(s, sQ, sK, hd, ty, tx);
+    mm_nt(dp, sO, sV, hd, ty, tx);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float x[4] = {s[r][0].x, s[r][0].y, s[r][1].x, s[r][1].y};
+      const float g[4] = {dp[r][0].x, dp[r][0].y, dp[r][1].x, dp[r][1].y};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float ds = 0.f;
+        if (sees(a, b, i0 + 4 * ty + r, j0 + 4 * tx + e)) ds = exp2f(x[e] * c - lse[r] * LOG2E) * (g[e] - D[r]);
+        sS[(4 * tx + e) * LD + 4 * ty + r] = ds;
+      }
+    }
+    __syncthreads();
+    mm_wn<HDP>(acc, sS, sKr, ty, tx);
+  }
+  const long long rows = (long long)a.seqs * a.heads * a.lq;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = i0 + 4 * ty + r;
+    if (i >= a.lq) continue;
+    if (a.splits > 1)
+      store_row<float, HDP>(acc[r], a.scale, a.part + (u.split * rows + row0 + i) * hd, hd, tx);
+    else
+      store_row<T, HDP>(acc[r], a.scale,
+                        static_cast<T*>(a.dq) + head_offset(a.dq_s, a, u.seq, u.h) + (long long)i * a.dq_s.row, hd,
+                        tx);
+  }
+}
+
+// dK and dV of 64 keys of one key/value head: walks the (query head of the group, query tile) pairs.
+template <typename T, int HDP>
+__global__ void __launch_bounds__(NT) attention_dkv_kernel(const __grid_constant__ AttnArgs a, int vec) {
+  extern __shared__ float smem[];
+  float* sK = smem;                       // [HDP][LD]
+  float* sV = sK + HDP * LD;              // [HDP][LD]
+  float* sQ = sV + HDP * LD;              // [HDP][LD]
+  float* sO = sQ + HDP * LD;              // [HDP][LD] dO
+  float* sQr = sO + HDP * LD;             // [64][HDP + 4]
+  float* sOr = sQr + TILE * (HDP + 4);    // [64][HDP + 4]
+  float* sS = sOr + TILE * (HDP + 4);     // [64 queries][LD]: P^T, then dS^T
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const Unit u = unit_of((a.lk + TILE - 1) / TILE, a.kv_heads, a.splits);
+  const Bounds b = bounds_of(a, u.seq);
+  const int j0 = u.tile * TILE;
+  const T* k = static_cast<const T*>(a.k) + head_offset(a.k_s, a, u.seq, u.h);
+  const T* v = static_cast<const T*>(a.v) + head_offset(a.v_s, a, u.seq, u.h);
+  const int begin = query_begin(a, b, j0) / TILE;
+  const int per_head = j0 < b.kl ? max(0, (b.ql + TILE - 1) / TILE - begin) : 0;
+  const int total = per_head * a.group;
+  const int t0 = (int)((long long)total * u.split / a.splits), t1 = (int)((long long)total * (u.split + 1) / a.splits);
+  const int hd = a.hd;
+  const float c = a.scale * LOG2E;
+  float2 dk[4][HDP / 64][2], dv[4][HDP / 64][2];
+  zero<HDP>(dk);
+  zero<HDP>(dv);
+  if (t0 < t1) {
+    load_tile<T, HDP, true, false>(k, a.k_s.row, j0, b.kl, hd, vec, sK, nullptr);
+    load_tile<T, HDP, true, false>(v, a.v_s.row, j0, b.kl, hd, vec, sV, nullptr);
+  }
+  // Rows that see no key have P = 0 whatever they hold: cut away, so that NaN in them stays out of the sums.
+  const int first = a.causal ? max(0, -b.off) : 0;
+  for (int t = t0; t < t1; ++t) {
+    const int h = u.h * a.group + t / per_head;
+    const int i0 = (begin + t % per_head) * TILE;
+    const T* q = static_cast<const T*>(a.q) + head_offset(a.q_s, a, u.seq, h);
+    const T* dout = static_cast<const T*>(a.dout) + head_offset(a.dout_s, a, u.seq, h);
+    const long long row0 = ((long long)u.seq * a.heads + h) * a.lq;
+    __syncthreads();
+    load_tile<T, HDP, true, true>(q, a.q_s.row, i0, b.ql, hd, vec, sQ, sQr);
+    load_tile<T, HDP, true, true>(dout, a.dout_s.row, i0, b.ql, hd, vec, sO, sOr);
+    __syncthreads();
+    if (i0 < first) {
+      for (int e = threadIdx.x; e < (first - i0 < TILE ? first - i0 : TILE) * (HDP + 4); e += NT) sQr[e] = sOr[e] = 0.f;
+      __syncthreads();
+    }
+    float2 s[4][2], dp[4][2];
+    mm_nt(s, sK, sQ, hd, ty, tx);
+    mm_nt(dp, sV, sO, hd, ty, tx);
+    float ds[4][4];
+    float lse[4], D[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + 4 * tx + e;
+      lse[e] = i < b.ql ? a.lse[row0 + i] * LOG2E : 0.f;
+      D[e] = i < b.ql ? a.dsum[row0 + i] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float x[4] = {s[r][0].x, s[r][0].y, s[r][1].x, s[r][1].y};
+      const float g[4] = {dp[r][0].x, dp[r][0].y, dp[r][1].x, dp[r][1].y};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool on = sees(a, b, i0 + 4 * tx + e, j0 + 4 * ty + r);
+        const float p = on ? exp2f(x[e] * c - lse[e]) : 0.f;
+        ds[r][e] = on ? p * (g[e] - D[e]) : 0.f;
+        sS[(4 * tx + e) * LD + 4 * ty + r] = p;
+      }
+    }
+    __syncthreads();
+    mm_wn<HDP>(dv, sS, sOr, ty, tx);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sS[(4 * tx + e) * LD + 4 * ty + r] = ds[r][e];
+    __syncthreads();
+    mm_wn<HDP>(dk, sS, sQr, ty, tx);
+  }
+  const long long rows = (long long)a.seqs * a.kv_heads * a.lk;
+  const long long row0 = ((long long)u.seq * a.kv_heads + u.h) * a.lk;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int j = j0 + 4 * ty + r;
+    if (j >= a.lk) continue;
+    if (a.splits > 1) {
+      store_row<float, HDP>(dk[r], a.scale, a.part + (u.split * rows + row0 + j) * hd, hd, tx);
+      store_row<float, HDP>(dv[r], 1.f, a.part + ((a.splits + u.split) * rows + row0 + j) * hd, hd, tx);
+    } else {
+      store_row<T, HDP>(dk[r], a.scale,
+                        static_cast<T*>(a.dk) + head_offset(a.dk_s, a, u.seq, u.h) + (long long)j * a.dk_s.row, hd,
+                        tx);
+      store_row<T, HDP>(dv[r], 1.f,
+                        static_cast<T*>(a.dv) + head_offset(a.dv_s, a, u.seq, u.h) + (long long)j * a.dv_s.row, hd,
+                        tx);
+    }
+  }
+}
+
+constexpr int fwd_smem(int hdp) { return 4 * (2 * hdp * LD + TILE * (hdp + 4) + TILE * LD); }
+constexpr int dq_smem(int hdp) { return 4 * (4 * hdp * LD + TILE * (hdp + 4) + TILE * LD); }
+constexpr int dkv_smem(int hdp) { return 4 * (4 * hdp * LD + 2 * TILE * (hdp + 4) + TILE * LD); }
+static_assert(dkv_smem(128) <= 227 * 1024 && dq_smem(128) <= 227 * 1024, "shared memory of one CTA");
+
+// Parts of the walked axis (`tiles` long): enough CTAs for the GPU, never an empty part of a full-length sequence.
+int split_count(long long units, long long tiles, long long want) {
+  if (units >= want || tiles <= 1) return 1;
+  long long n = (want + units - 1) / units;
+  if (n > tiles) n = tiles;
+  return (int)(n < 32 ? n : 32);
+}
+
+long long div_up(long long a, long long b) { return (a + b - 1) / b; }
+
+struct Plan {
+  int fwd_splits, dq_splits, dkv_splits;
+  long long q_rows, k_rows;
+  long long fwd_floats() const { return fwd_splits > 1 ? fwd_splits * q_rows : 0; }
+};
+
+Plan plan_of(const UnblendAttnTrainParams& p) {
+  Plan n;
+  const long long seqs = (long long)p.outer * p.inner;
+  const long long qt = div_up(p.lq, TILE), kt = div_up(p.lk, TILE);
+  const long long want = 2LL * ub::kNumSMs;
+  n.q_rows = seqs * p.heads * p.lq;
+  n.k_rows = seqs * p.kv_heads * p.lk;
+  n.fwd_splits = split_count(seqs * p.heads * qt, kt, want);
+  n.dq_splits = n.fwd_splits;
+  n.dkv_splits = split_count(seqs * p.kv_heads * kt, qt * (p.heads / p.kv_heads), want);
+  return n;
+}
+
+// Workspace: forward [parts][q_rows][hd] and [parts][q_rows] lse; backward D [q_rows], then the larger of the two
+// kernels' parts (they run one after the other).
+long long round4(long long n) { return (n + 3) / 4 * 4; }
+
+long long workspace_floats(const UnblendAttnTrainParams& p, bool backward) {
+  const Plan n = plan_of(p);
+  if (!backward) return n.fwd_splits > 1 ? n.fwd_splits * n.q_rows * (p.hd + 1LL) : 0;
+  const long long dq = n.dq_splits > 1 ? n.dq_splits * n.q_rows * p.hd : 0;
+  const long long dkv = n.dkv_splits > 1 ? 2 * n.dkv_splits * n.k_rows * p.hd : 0;
+  return round4(n.q_rows) + (dq > dkv ? dq : dkv);
+}
+
+bool params_ok(const UnblendAttnTrainParams* p) {
+  if (!p || !known_type(p->dtype)) return false;
+  if (p->outer <= 0 || p->inner <= 0 || p->heads <= 0 || p->kv_heads <= 0 || p->lq <= 0 || p->lk <= 0) return false;
+  if (p->hd <= 0 || p->hd > 128 || p->heads % p->kv_heads != 0) return false;
+  if (p->lq >= (1 << 30) || p->lk >= (1 << 30)) return false;
+  const long long seqs = (long long)p->outer * p->inner;
+  if (seqs >= (1LL << 31)) return false;
+  // CTAs of each kernel, splits included (at most 32).
+  const long long qt = div_up(p->lq, TILE), kt = div_up(p->lk, TILE);
+  return seqs <= (1LL << 31) / p->heads / qt / 32 && seqs <= (1LL << 31) / p->kv_heads / kt / 32;
+}
+
+bool vec4_ok(const void* p, const UnblendHeadStrides& s, const UnblendAttnTrainParams& a) {
+  const int w = 4 * elem_size(a.dtype);
+  auto fits = [&](long long st, int n) { return n <= 1 || st % 4 == 0; };
+  return reinterpret_cast<uintptr_t>(p) % w == 0 && fits(s.outer, a.outer) && fits(s.inner, a.inner) && s.row % 4 == 0 &&
+         s.head % 4 == 0;
+}
+
+AttnArgs args_of(const UnblendAttnTrainParams& p) {
+  AttnArgs a{};
+  a.q_s = p.q;
+  a.k_s = p.k;
+  a.v_s = p.v;
+  a.out_s = p.out;
+  a.dout_s = p.dout;
+  a.dq_s = p.dq;
+  a.dk_s = p.dk;
+  a.dv_s = p.dv;
+  a.q_lens = p.q_lens;
+  a.k_lens = p.k_lens;
+  a.seqs = p.outer * p.inner;
+  a.inner = p.inner;
+  a.heads = p.heads;
+  a.kv_heads = p.kv_heads;
+  a.group = p.heads / p.kv_heads;
+  a.lq = p.lq;
+  a.lk = p.lk;
+  a.hd = p.hd;
+  a.causal = p.causal ? 1 : 0;
+  a.scale = p.scale;
+  a.splits = 1;
+  return a;
+}
+
+template <typename T, int HDP>
+int forward_simt(AttnArgs a, const Plan& n, bool vec, cudaStream_t st) {
+  const long long units = (long long)a.seqs * a.heads * div_up(a.lq, TILE) * a.splits;
+  cudaFuncSetAttribute(attention_fwd_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem(HDP));
+  attention_fwd_kernel<T, HDP><<<(unsigned)units, NT, fwd_smem(HDP), st>>>(a, vec);
+  UB_CHECK_LAUNCH();
+  if (a.splits > 1) {
+    attention_join_kernel<T><<<(unsigned)div_up(n.q_rows, 8), 256, 0, st>>>(a);
+    UB_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+template <typename T, int HDP>
+int backward_simt(AttnArgs a, const Plan& n, float* parts, bool vec, cudaStream_t st) {
+  a.splits = n.dq_splits;
+  a.part = a.splits > 1 ? parts : nullptr;
+  long long units = (long long)a.seqs * a.heads * div_up(a.lq, TILE) * a.splits;
+  cudaFuncSetAttribute(attention_dq_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, dq_smem(HDP));
+  attention_dq_kernel<T, HDP><<<(unsigned)units, NT, dq_smem(HDP), st>>>(a, vec);
+  UB_CHECK_LAUNCH();
+  if (a.splits > 1) {
+    attention_sum_kernel<T><<<(unsigned)div_up(n.q_rows, 8), 256, 0, st>>>(a, parts, a.splits, a.heads, a.lq, a.dq,
+                                                                         a.dq_s);
+    UB_CHECK_LAUNCH();
+  }
+  a.splits = n.dkv_splits;
+  a.part = a.splits > 1 ? parts : nullptr;
+  units = (long long)a.seqs * a.kv_heads * div_up(a.lk, TILE) * a.splits;
+  cudaFuncSetAttribute(attention_dkv_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, dkv_smem(HDP));
+  attention_dkv_kernel<T, HDP><<<(unsigned)units, NT, dkv_smem(HDP), st>>>(a, vec);
+  UB_CHECK_LAUNCH();
+  if (a.splits > 1) {
+    const unsigned grid = (unsigned)div_up(n.k_rows, 8);
+    attention_sum_kernel<T><<<grid, 256, 0, st>>>(a, parts, a.splits, a.kv_heads, a.lk, a.dk, a.dk_s);
+    UB_CHECK_LAUNCH();
+    attention_sum_kernel<T><<<grid, 256, 0, st>>>(a, parts + a.splits * n.k_rows * a.hd, a.splits, a.kv_heads, a.lk,
+                                                  a.dv, a.dv_s);
+    UB_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+template <typename T>
+int forward_types(const AttnArgs& a, const Plan& n, bool vec, cudaStream_t st) {
+  return a.hd <= 64 ? forward_simt<T, 64>(a, n, vec, st) : forward_simt<T, 128>(a, n, vec, st);
+}
+
+template <typename T>
+int backward_types(const AttnArgs& a, const Plan& n, float* parts, bool vec, cudaStream_t st) {
+  return a.hd <= 64 ? backward_simt<T, 64>(a, n, parts, vec, st) : backward_simt<T, 128>(a, n, parts, vec, st);
+}
+
+}  // namespace
+
+extern "C" int unblend_attention_workspace(const UnblendAttnTrainParams* p, int backward, long long* bytes) {
+  UB_REQUIRE(params_ok(p) && bytes);
+  *bytes = 4 * workspace_floats(*p, backward != 0);
+  return 0;
+}
+
+extern "C" int unblend_attention_forward(const void* q, const void* k, const void* v, void* out, float* lse,
+                                         void* work, long long work_bytes, const UnblendAttnTrainParams* p,
+                                         void* stream) {
+  UB_REQUIRE(q && k && v && out && params_ok(p));
+  const long long need = 4 * workspace_floats(*p, false);
+  UB_REQUIRE(need == 0 || (aligned16(work) && work && work_bytes >= need));
+  const Plan n = plan_of(*p);
+  AttnArgs a = args_of(*p);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.lse = lse;
+  a.splits = n.fwd_splits;
+  if (a.splits > 1) {
+    a.part = static_cast<float*>(work);
+    a.part_lse = a.part + a.splits * n.q_rows * p->hd;
+  }
+  cudaStream_t st = ub::as_stream(stream);
+  const bool vec = p->hd % 4 == 0 && vec4_ok(q, p->q, *p) && vec4_ok(k, p->k, *p) && vec4_ok(v, p->v, *p);
+  if (p->dtype == UNBLEND_F32) return forward_types<float>(a, n, vec, st);
+  if (p->dtype == UNBLEND_BF16) return forward_types<__nv_bfloat16>(a, n, vec, st);
+  return forward_types<__half>(a, n, vec, st);
+}
+
+extern "C" int unblend_attention_backward(const void* dout, const void* q, const void* k, const void* v,
+                                          const void* out, const float* lse, void* dq, void* dk, void* dv, void* work,
+                                          long long work_bytes, const UnblendAttnTrainParams* p, void* stream) {
+  UB_REQUIRE(dout && q && k && v && out && lse && dq && dk && dv && params_ok(p));
+  UB_REQUIRE(work && aligned16(work) && work_bytes >= 4 * workspace_floats(*p, true));
+  const Plan n = plan_of(*p);
+  AttnArgs a = args_of(*p);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.dout = dout;
+  a.out_in = out;
+  a.lse = const_cast<float*>(lse);
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.dsum = static_cast<float*>(work);
+  float* parts = a.dsum + round4(n.q_rows);
+  cudaStream_t st = ub::as_stream(stream);
+  const bool vec = p->hd % 4 == 0 && vec4_ok(q, p->q, *p) && vec4_ok(k, p->k, *p) && vec4_ok(v, p->v, *p) &&
+                   vec4_ok(dout, p->dout, *p);
+  if (p->dtype == UNBLEND_F32) return backward_types<float>(a, n, parts, vec, st);
+  if (p->dtype == UNBLEND_BF16) return backward_types<__nv_bfloat16>(a, n, parts, vec, st);
+  return backward_types<__half>(a, n, parts, vec, st);
+}

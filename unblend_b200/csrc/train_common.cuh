@@ -1,0 +1,140 @@
+// Shared helpers of the training operators (layer norm, dropout-add, attention with gradients): element types,
+// vector loads into fp32 registers, two-level row addressing and the fixed-order join of column sums.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace ub {
+namespace train {
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+// VEC consecutive elements as fp32. VEC * sizeof(T) is the access width (2, 4, 8, 16 or 32 bytes; p is aligned to
+// it, 32 bytes as two 16-byte halves).
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
+  constexpr int BYTES = VEC * (int)sizeof(T);
+  if constexpr (VEC == 1) {
+    v[0] = to_f(*p);
+  } else {
+    alignas(16) T raw[VEC];
+    if constexpr (BYTES == 8)
+      *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
+    else {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i)
+        reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = to_f(raw[i]);
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
+  constexpr int BYTES = VEC * (int)sizeof(T);
+  if constexpr (VEC == 1) {
+    *p = from_f<T>(v[0]);
+  } else {
+    alignas(16) T raw[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) raw[i] = from_f<T>(v[i]);
+    if constexpr (BYTES == 8)
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(raw);
+    else {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i)
+        reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(raw)[i];
+    }
+  }
+}
+
+// Rows of a tensor whose leading axes are (outer, inner): row r starts at (r / inner) * so + (r % inner) * si.
+struct RowMap {
+  long long so, si;
+  unsigned inner;
+};
+
+__device__ __forceinline__ long long row_offset(const RowMap& m, unsigned r) {
+  const unsigned o = r / m.inner;
+  return (long long)o * m.so + (long long)(r - o * m.inner) * m.si;
+}
+
+inline RowMap row_map(long long so, long long si, long long inner) { return RowMap{so, si, (unsigned)inner}; }
+
+inline bool known_type(int t) { return t == UNBLEND_F32 || t == UNBLEND_BF16 || t == UNBLEND_F16; }
+inline int elem_size(int t) { return t == UNBLEND_F32 ? 4 : 2; }
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+inline bool rows_ok(long long outer, long long inner, int cols) {
+  return outer > 0 && inner > 0 && cols > 0 && outer < (1LL << 31) && inner < (1LL << 31) &&
+         outer * inner < (1LL << 31);
+}
+
+// True when every row of `m` starts on a `bytes` boundary.
+inline bool rows_aligned(const void* p, const RowMap& m, long long outer, int elem, int bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (m.inner <= 1 || m.si * elem % bytes == 0) &&
+         (outer <= 1 || m.so * elem % bytes == 0);
+}
+
+// Column sums out[c] = sum_p part[p][c] of n_part partial rows, always added in the same order (each of 16 threads
+// takes every 16th row, then the 16 sums in sequence), so the result does not depend on scheduling. The columns are
+// `sums` runs of `cols` values, run i going to out_i.
+constexpr int COLSUM_Y = 16;
+
+template <typename TO>
+__global__ void __launch_bounds__(32 * COLSUM_Y)
+    column_sums_kernel(const float* __restrict__ part, int n_part, int cols, int sums, TO* out0, TO* out1) {
+  __shared__ float red[COLSUM_Y][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const long long width = (long long)cols * sums;
+  const long long c = blockIdx.x * 32LL + tx;
+  float s = 0.f;
+  if (c < width) {
+#pragma unroll 4
+    for (int p = ty; p < n_part; p += COLSUM_Y) s += part[p * width + c];
+  }
+  red[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < width) {
+#pragma unroll
+    for (int y = 1; y < COLSUM_Y; ++y) s += red[y][tx];
+    if (c < cols)
+      out0[c] = from_f<TO>(s);
+    else
+      out1[c - cols] = from_f<TO>(s);
+  }
+}
+
+template <typename TO>
+inline int launch_column_sums(const float* part, int n_part, int cols, int sums, void* out0, void* out1,
+                              cudaStream_t st) {
+  const long long width = (long long)cols * sums;
+  column_sums_kernel<TO><<<(unsigned)((width + 31) / 32), 32 * COLSUM_Y, 0, st>>>(
+      part, n_part, cols, sums, static_cast<TO*>(out0), static_cast<TO*>(out1));
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
+}  // namespace train
+}  // namespace ub
