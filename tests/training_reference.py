@@ -18,6 +18,11 @@ def half(t: torch.dtype) -> float:
     return torch.finfo(t).eps / 2
 
 
+def floor(t: torch.dtype) -> float:
+    """Half of the smallest step of type t: what one rounding costs below its normal range (fp16: under 2^-14)."""
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
 def acc(n: int) -> float:
     return 4 * (n + 16) * U
 
@@ -38,7 +43,7 @@ def assert_within(name: str, got: torch.Tensor, want: torch.Tensor, tol: torch.T
 def norm_reference(x, gamma, beta, eps, dy):
     """{name: (value, bound)} of y, dx, dgamma, dbeta; x and dy as rows."""
     t = x.dtype
-    x, dy = x.double().flatten(0, -2), dy.double().flatten(0, -2)
+    x, dy = (a.double().reshape(-1, a.shape[-1]) for a in (x, dy))
     n, c = x.shape
     g = torch.ones(c, device=x.device, dtype=torch.float64) if gamma is None else gamma.double()
     b = torch.zeros_like(g) if beta is None else beta.double()
@@ -66,7 +71,8 @@ def norm_reference(x, gamma, beta, eps, dy):
     dg, db = (dy * xhat).sum(0), dy.sum(0)
     e_dg = half(tw) * dg.abs() + acc(n) * (dy * xhat).abs().sum(0) + (dy.abs() * e_xhat).sum(0)
     e_db = half(tw) * db.abs() + acc(n) * dy.abs().sum(0)
-    return {"y": (y, e_y), "dx": (dx, e_dx), "dgamma": (dg, e_dg), "dbeta": (db, e_db)}
+    f, fw = floor(t), floor(tw)
+    return {"y": (y, e_y + f), "dx": (dx, e_dx + f), "dgamma": (dg, e_dg + fw), "dbeta": (db, e_db + fw)}
 
 
 # ------------------------------------------------------------------------------------------- attention
@@ -107,35 +113,33 @@ def attention_reference(q, k, v, dout, scale=None, causal=False, q_lens=None, k_
     dq, dk, dv = ds @ k * scale, ds.transpose(-1, -2) @ q * scale, p.transpose(-1, -2) @ dout
     # Bounds. A score is off by acc(hd) of its magnitude sum, and P relatively by twice that (its sum too); its
     # exponential by 2^-20 (approximations of 2^x and of the sum's reciprocal, and the score's own rounding). 16-bit
-    # kernels round P and dS to the type before the second product.
-    ht = half(t)
+    # kernels round P and dS to the type before the second product: half a step, of the smallest one below the type's
+    # normal range (P relative to its row's maximum or sum, so a floor on P itself).
+    ht, fl = half(t), floor(t)
     mag = q.abs() @ k.abs().transpose(-1, -2) * abs(scale)
     es = acc(hd) * mag
     top = torch.where(see, es + 2 * U * z.abs().nan_to_num(0, 0, 0), 0.0)
     worst = top.amax(-1, keepdim=True)
     ep = (top + worst + 2.0**-20 + acc(lk)) * p  # of P in fp32
-    e_out = ht * out.abs() + (ht * p + ep) @ v.abs() + acc(lk) * (p @ v.abs())
+    e_out = ht * out.abs() + (ht * p + fl * see + ep) @ v.abs() + acc(lk) * (p @ v.abs())
     e_lse = worst[..., 0] + 2.0**-20 + acc(lk) + 4 * U * lse.abs().nan_to_num(0, 0, 0)
     e_dp = acc(hd) * (dout.abs() @ v.abs().transpose(-1, -2))
     e_D = (dout.abs() * (e_out + acc(hd) * out.abs())).sum(-1, keepdim=True)
-    e_ds = ht * ds.abs() + ep * (dp - D).abs() + p * (e_dp + e_D + 4 * U * (dp.abs() + D.abs()))
+    e_ds = ht * ds.abs() + fl * see + ep * (dp - D).abs() + p * (e_dp + e_D + 4 * U * (dp.abs() + D.abs()))
     w = abs(scale)
     e_dq = ht * dq.abs() + w * (e_ds @ k.abs()) + acc(lk) * w * (ds.abs() @ k.abs())
     e_dk = w * (e_ds.transpose(-1, -2) @ q.abs()) + acc(lq * rep) * w * (ds.abs().transpose(-1, -2) @ q.abs())
-    e_dv = (ht * p + ep).transpose(-1, -2) @ dout.abs() + acc(lq * rep) * (p.transpose(-1, -2) @ dout.abs())
+    e_dv = (ht * p + fl * see + ep).transpose(-1, -2) @ dout.abs() + acc(lq * rep) * (p.transpose(-1, -2) @ dout.abs())
 
     def shared(x):
         return x.unflatten(1, (hk, rep)).sum(2)
 
     dk, dv, e_dk, e_dv = shared(dk), shared(dv), shared(e_dk), shared(e_dv)
     e_dk, e_dv = e_dk + ht * dk.abs(), e_dv + ht * dv.abs()
-    # Results below the type's normal range are off by its smallest step instead.
-    tiny = torch.finfo(t).smallest_normal * torch.finfo(t).eps
-
     def tokens(x):
         return x.transpose(1, 2).reshape(*lead, x.shape[2], x.shape[1], hd)
 
-    res = {m: (tokens(a), tokens(e) + tiny)
+    res = {m: (tokens(a), tokens(e) + fl)
            for m, a, e in (("out", out, e_out), ("dq", dq, e_dq), ("dk", dk, e_dk), ("dv", dv, e_dv))}
     res["lse"] = (lse, e_lse)
     return res

@@ -192,6 +192,7 @@ _HOST_SIGNATURES = {
     "unblend_gemm_error_flag": [ctypes.POINTER(c_int), c_int],
     "unblend_attention_bf16_error_flag": [ctypes.POINTER(c_int), c_int],
     "unblend_dconv_error_flag": [ctypes.POINTER(c_int), c_int],
+    "unblend_attention_train_error_flag": [ctypes.POINTER(c_int), c_int],
     "unblend_layer_norm_grad_workspace": [c_ll, c_int, ctypes.POINTER(c_ll)],
     "unblend_dropout_add_grad_workspace": [c_ll, c_int, ctypes.POINTER(c_ll)],
     "unblend_attention_workspace": [ctypes.POINTER(AttnTrainParams), c_int, ctypes.POINTER(c_ll)],
@@ -249,7 +250,8 @@ def error_flag(clear: bool = True) -> int:
     """Read (and by default clear) the device flag that bounded waits set on timeout."""
     total = 0
     for name in ("unblend_error_flag", "unblend_attention_error_flag", "unblend_gemm_error_flag",
-                 "unblend_attention_bf16_error_flag", "unblend_dconv_error_flag", "unblend_lstm_error_flag"):
+                 "unblend_attention_bf16_error_flag", "unblend_dconv_error_flag", "unblend_lstm_error_flag",
+                 "unblend_attention_train_error_flag"):
         v = c_int(0)
         check(name, getattr(load(), name)(ctypes.byref(v), 1 if clear else 0))
         total |= v.value

@@ -406,7 +406,7 @@ constexpr int dq_smem(int hdp) { return 4 * (4 * hdp * LD + TILE * (hdp + 4) + T
 constexpr int dkv_smem(int hdp) { return 4 * (4 * hdp * LD + 2 * TILE * (hdp + 4) + TILE * LD); }
 static_assert(dkv_smem(128) <= 227 * 1024 && dq_smem(128) <= 227 * 1024, "shared memory of one CTA");
 
-// Parts of the walked axis (`tiles` long): enough CTAs for the GPU, never an empty part of a full-length sequence.
+// Parts of the walked axis (`tiles` long) for at least `want` CTAs, at most one part per tile.
 int split_count(long long units, long long tiles, long long want) {
   if (units >= want || tiles <= 1) return 1;
   long long n = (want + units - 1) / units;
@@ -415,36 +415,49 @@ int split_count(long long units, long long tiles, long long want) {
 }
 
 long long div_up(long long a, long long b) { return (a + b - 1) / b; }
+long long round4(long long n) { return (n + 3) / 4 * 4; }
 
+// Work division of a call on the CUDA cores (tc false) or the tensor cores.
 struct Plan {
+  int fwd_rows;  // queries per CTA of the forward kernel
   int fwd_splits, dq_splits, dkv_splits;
   long long q_rows, k_rows;
-  long long fwd_floats() const { return fwd_splits > 1 ? fwd_splits * q_rows : 0; }
 };
 
-Plan plan_of(const UnblendAttnTrainParams& p) {
+Plan plan_of(const UnblendAttnTrainParams& p, bool tc) {
   Plan n;
-  const long long seqs = (long long)p.outer * p.inner;
-  const long long qt = div_up(p.lq, TILE), kt = div_up(p.lk, TILE);
-  const long long want = 2LL * ub::kNumSMs;
-  n.q_rows = seqs * p.heads * p.lq;
-  n.k_rows = seqs * p.kv_heads * p.lk;
-  n.fwd_splits = split_count(seqs * p.heads * qt, kt, want);
-  n.dq_splits = n.fwd_splits;
-  n.dkv_splits = split_count(seqs * p.kv_heads * kt, qt * (p.heads / p.kv_heads), want);
+  const long long seqs = (long long)p.outer * p.inner, qh = seqs * p.heads, kh = seqs * p.kv_heads;
+  const long long tile = tc ? 128 : TILE;
+  const long long qt = div_up(p.lq, tile), kt = div_up(p.lk, tile);
+  const long long sms = ub::kNumSMs, group = p.heads / p.kv_heads;
+  n.q_rows = qh * p.lq;
+  n.k_rows = kh * p.lk;
+  n.fwd_rows = (int)tile;
+  if (tc && qh * div_up(p.lq, 256) >= sms && p.lq > 128) n.fwd_rows = 256;
+  n.fwd_splits = n.fwd_rows == 256 ? 1 : split_count(qh * qt, kt, 2 * sms);
+  n.dq_splits = split_count(qh * qt, kt, tc ? sms : 2 * sms);
+  n.dkv_splits = split_count(kh * kt, qt * group, tc ? sms : 2 * sms);
   return n;
 }
 
 // Workspace: forward [parts][q_rows][hd] and [parts][q_rows] lse; backward D [q_rows], then the larger of the two
-// kernels' parts (they run one after the other).
-long long round4(long long n) { return (n + 3) / 4 * 4; }
-
+// kernels' parts (they run one after the other). Room for either kind of kernels: which of them runs depends on the
+// pointers too.
 long long workspace_floats(const UnblendAttnTrainParams& p, bool backward) {
-  const Plan n = plan_of(p);
-  if (!backward) return n.fwd_splits > 1 ? n.fwd_splits * n.q_rows * (p.hd + 1LL) : 0;
-  const long long dq = n.dq_splits > 1 ? n.dq_splits * n.q_rows * p.hd : 0;
-  const long long dkv = n.dkv_splits > 1 ? 2 * n.dkv_splits * n.k_rows * p.hd : 0;
-  return round4(n.q_rows) + (dq > dkv ? dq : dkv);
+  long long most = 0;
+  for (int tc = 0; tc < 2; ++tc) {
+    const Plan n = plan_of(p, tc != 0);
+    long long need;
+    if (!backward) {
+      need = n.fwd_splits > 1 ? n.fwd_splits * n.q_rows * (p.hd + 1LL) : 0;
+    } else {
+      const long long dq = n.dq_splits > 1 ? n.dq_splits * n.q_rows * p.hd : 0;
+      const long long dkv = n.dkv_splits > 1 ? 2 * n.dkv_splits * n.k_rows * p.hd : 0;
+      need = round4(n.q_rows) + (dq > dkv ? dq : dkv);
+    }
+    most = need > most ? need : most;
+  }
+  return most;
 }
 
 bool params_ok(const UnblendAttnTrainParams* p) {
@@ -493,56 +506,77 @@ AttnArgs args_of(const UnblendAttnTrainParams& p) {
 }
 
 template <typename T, int HDP>
-int forward_simt(AttnArgs a, const Plan& n, bool vec, cudaStream_t st) {
+int simt_forward(const AttnArgs& a, bool vec, cudaStream_t st) {
   const long long units = (long long)a.seqs * a.heads * div_up(a.lq, TILE) * a.splits;
   cudaFuncSetAttribute(attention_fwd_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem(HDP));
   attention_fwd_kernel<T, HDP><<<(unsigned)units, NT, fwd_smem(HDP), st>>>(a, vec);
   UB_CHECK_LAUNCH();
-  if (a.splits > 1) {
-    attention_join_kernel<T><<<(unsigned)div_up(n.q_rows, 8), 256, 0, st>>>(a);
-    UB_CHECK_LAUNCH();
-  }
   return 0;
 }
 
 template <typename T, int HDP>
-int backward_simt(AttnArgs a, const Plan& n, float* parts, bool vec, cudaStream_t st) {
-  a.splits = n.dq_splits;
-  a.part = a.splits > 1 ? parts : nullptr;
-  long long units = (long long)a.seqs * a.heads * div_up(a.lq, TILE) * a.splits;
+int simt_dq(AttnArgs a, int splits, float* parts, bool vec, cudaStream_t st) {
+  a.splits = splits;
+  a.part = parts;
+  const long long units = (long long)a.seqs * a.heads * div_up(a.lq, TILE) * splits;
   cudaFuncSetAttribute(attention_dq_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, dq_smem(HDP));
   attention_dq_kernel<T, HDP><<<(unsigned)units, NT, dq_smem(HDP), st>>>(a, vec);
   UB_CHECK_LAUNCH();
-  if (a.splits > 1) {
-    attention_sum_kernel<T><<<(unsigned)div_up(n.q_rows, 8), 256, 0, st>>>(a, parts, a.splits, a.heads, a.lq, a.dq,
-                                                                         a.dq_s);
-    UB_CHECK_LAUNCH();
-  }
-  a.splits = n.dkv_splits;
-  a.part = a.splits > 1 ? parts : nullptr;
-  units = (long long)a.seqs * a.kv_heads * div_up(a.lk, TILE) * a.splits;
+  return 0;
+}
+
+template <typename T, int HDP>
+int simt_dkv(AttnArgs a, int splits, float* parts, bool vec, cudaStream_t st) {
+  a.splits = splits;
+  a.part = parts;
+  const long long units = (long long)a.seqs * a.kv_heads * div_up(a.lk, TILE) * splits;
   cudaFuncSetAttribute(attention_dkv_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, dkv_smem(HDP));
   attention_dkv_kernel<T, HDP><<<(unsigned)units, NT, dkv_smem(HDP), st>>>(a, vec);
   UB_CHECK_LAUNCH();
-  if (a.splits > 1) {
-    const unsigned grid = (unsigned)div_up(n.k_rows, 8);
-    attention_sum_kernel<T><<<grid, 256, 0, st>>>(a, parts, a.splits, a.kv_heads, a.lk, a.dk, a.dk_s);
-    UB_CHECK_LAUNCH();
-    attention_sum_kernel<T><<<grid, 256, 0, st>>>(a, parts + a.splits * n.k_rows * a.hd, a.splits, a.kv_heads, a.lk,
-                                                  a.dv, a.dv_s);
-    UB_CHECK_LAUNCH();
-  }
   return 0;
 }
 
 template <typename T>
-int forward_types(const AttnArgs& a, const Plan& n, bool vec, cudaStream_t st) {
-  return a.hd <= 64 ? forward_simt<T, 64>(a, n, vec, st) : forward_simt<T, 128>(a, n, vec, st);
+int forward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Plan& n, bool tc, bool vec,
+                  cudaStream_t st) {
+  int rc;
+  if (tc)
+    rc = attention_fwd_tc(a, p, n.fwd_rows, st);
+  else
+    rc = a.hd <= 64 ? simt_forward<T, 64>(a, vec, st) : simt_forward<T, 128>(a, vec, st);
+  if (rc || a.splits == 1) return rc;
+  attention_join_kernel<T><<<(unsigned)div_up(n.q_rows, 8), 256, 0, st>>>(a);
+  UB_CHECK_LAUNCH();
+  return 0;
 }
 
 template <typename T>
-int backward_types(const AttnArgs& a, const Plan& n, float* parts, bool vec, cudaStream_t st) {
-  return a.hd <= 64 ? backward_simt<T, 64>(a, n, parts, vec, st) : backward_simt<T, 128>(a, n, parts, vec, st);
+int backward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Plan& n, float* parts, bool tc, bool vec,
+                   cudaStream_t st) {
+  int rc;
+  if (tc)
+    rc = attention_dq_tc(a, p, n.dq_splits, parts, st);
+  else
+    rc = a.hd <= 64 ? simt_dq<T, 64>(a, n.dq_splits, parts, vec, st) : simt_dq<T, 128>(a, n.dq_splits, parts, vec, st);
+  if (rc) return rc;
+  if (n.dq_splits > 1) {
+    attention_sum_kernel<T><<<(unsigned)div_up(n.q_rows, 8), 256, 0, st>>>(a, parts, n.dq_splits, a.heads, a.lq, a.dq,
+                                                                         a.dq_s);
+    UB_CHECK_LAUNCH();
+  }
+  if (tc)
+    rc = attention_dkv_tc(a, p, n.dkv_splits, parts, st);
+  else
+    rc = a.hd <= 64 ? simt_dkv<T, 64>(a, n.dkv_splits, parts, vec, st)
+                    : simt_dkv<T, 128>(a, n.dkv_splits, parts, vec, st);
+  if (rc || n.dkv_splits == 1) return rc;
+  const unsigned grid = (unsigned)div_up(n.k_rows, 8);
+  attention_sum_kernel<T><<<grid, 256, 0, st>>>(a, parts, n.dkv_splits, a.kv_heads, a.lk, a.dk, a.dk_s);
+  UB_CHECK_LAUNCH();
+  attention_sum_kernel<T><<<grid, 256, 0, st>>>(a, parts + n.dkv_splits * n.k_rows * a.hd, n.dkv_splits, a.kv_heads,
+                                                a.lk, a.dv, a.dv_s);
+  UB_CHECK_LAUNCH();
+  return 0;
 }
 
 }  // namespace
@@ -559,7 +593,11 @@ extern "C" int unblend_attention_forward(const void* q, const void* k, const voi
   UB_REQUIRE(q && k && v && out && params_ok(p));
   const long long need = 4 * workspace_floats(*p, false);
   UB_REQUIRE(need == 0 || (aligned16(work) && work && work_bytes >= need));
-  const Plan n = plan_of(*p);
+  const void* ptrs[] = {q, k, v, out};
+  const UnblendHeadStrides strides[] = {p->q, p->k, p->v, p->out};
+  const int heads[] = {p->heads, p->kv_heads, p->kv_heads, p->heads}, rows[] = {p->lq, p->lk, p->lk, p->lq};
+  const bool tc = attention_tc_fits(*p, ptrs, strides, heads, rows, 4);
+  const Plan n = plan_of(*p, tc);
   AttnArgs a = args_of(*p);
   a.q = q;
   a.k = k;
@@ -573,9 +611,9 @@ extern "C" int unblend_attention_forward(const void* q, const void* k, const voi
   }
   cudaStream_t st = ub::as_stream(stream);
   const bool vec = p->hd % 4 == 0 && vec4_ok(q, p->q, *p) && vec4_ok(k, p->k, *p) && vec4_ok(v, p->v, *p);
-  if (p->dtype == UNBLEND_F32) return forward_types<float>(a, n, vec, st);
-  if (p->dtype == UNBLEND_BF16) return forward_types<__nv_bfloat16>(a, n, vec, st);
-  return forward_types<__half>(a, n, vec, st);
+  if (p->dtype == UNBLEND_F32) return forward_types<float>(a, *p, n, tc, vec, st);
+  if (p->dtype == UNBLEND_BF16) return forward_types<__nv_bfloat16>(a, *p, n, tc, vec, st);
+  return forward_types<__half>(a, *p, n, tc, vec, st);
 }
 
 extern "C" int unblend_attention_backward(const void* dout, const void* q, const void* k, const void* v,
@@ -583,7 +621,13 @@ extern "C" int unblend_attention_backward(const void* dout, const void* q, const
                                           long long work_bytes, const UnblendAttnTrainParams* p, void* stream) {
   UB_REQUIRE(dout && q && k && v && out && lse && dq && dk && dv && params_ok(p));
   UB_REQUIRE(work && aligned16(work) && work_bytes >= 4 * workspace_floats(*p, true));
-  const Plan n = plan_of(*p);
+  const void* ptrs[] = {q, k, v, out, dout, dq, dk, dv};
+  const UnblendHeadStrides strides[] = {p->q, p->k, p->v, p->out, p->dout, p->dq, p->dk, p->dv};
+  const int hq = p->heads, hk = p->kv_heads;
+  const int heads[] = {hq, hk, hk, hq, hq, hq, hk, hk};
+  const int rows[] = {p->lq, p->lk, p->lk, p->lq, p->lq, p->lq, p->lk, p->lk};
+  const bool tc = attention_tc_fits(*p, ptrs, strides, heads, rows, 8);
+  const Plan n = plan_of(*p, tc);
   AttnArgs a = args_of(*p);
   a.q = q;
   a.k = k;
@@ -599,7 +643,7 @@ extern "C" int unblend_attention_backward(const void* dout, const void* q, const
   cudaStream_t st = ub::as_stream(stream);
   const bool vec = p->hd % 4 == 0 && vec4_ok(q, p->q, *p) && vec4_ok(k, p->k, *p) && vec4_ok(v, p->v, *p) &&
                    vec4_ok(dout, p->dout, *p);
-  if (p->dtype == UNBLEND_F32) return backward_types<float>(a, n, parts, vec, st);
-  if (p->dtype == UNBLEND_BF16) return backward_types<__nv_bfloat16>(a, n, parts, vec, st);
-  return backward_types<__half>(a, n, parts, vec, st);
+  if (p->dtype == UNBLEND_F32) return backward_types<float>(a, *p, n, parts, tc, vec, st);
+  if (p->dtype == UNBLEND_BF16) return backward_types<__nv_bfloat16>(a, *p, n, parts, tc, vec, st);
+  return backward_types<__half>(a, *p, n, parts, tc, vec, st);
 }

@@ -116,5 +116,12 @@ __global__ void __launch_bounds__(256)
 }
 
 
+// The tensor-core kernels (attention_train_tc.cu). `fits`: whether they can address the n tensors of a call.
+bool attention_tc_fits(const UnblendAttnTrainParams& p, const void* const* ptrs, const UnblendHeadStrides* strides,
+                       const int* heads, const int* rows, int n);
+int attention_fwd_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int rows_per_cta, cudaStream_t st);
+int attention_dq_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st);
+int attention_dkv_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st);
+
 }  // namespace train
 }  // namespace ub

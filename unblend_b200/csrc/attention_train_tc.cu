@@ -1,0 +1,1351 @@
+// Attention with gradients on the tcgen05 tensor cores: bf16 and fp16, head dims that are multiples of 8.
+//
+// All products take the form D[128 rows x N] += A[128 x K] B[N x K]^T with fp32 accumulators in TMEM. Operand tiles
+// are rows of 64 elements (128 bytes, 128-byte swizzle) written by TMA, two such column blocks for head dims over 64;
+// columns past the head dim and rows past the tensor read as 0. The same tile serves as a K-major operand (summed
+// over the head dim: S, dP) and as an MN-major one (summed over its rows: O, dQ, dK, dV): nothing is transposed in
+// shared memory. P and dS go from registers to TMEM as 16-bit A operands, over the scores that they came from.
+//
+//   forward   rows = queries: S = Q K^T (Q resident, K streamed), O += P V
+//   dq        rows = queries: S = Q K^T, dP = dO V^T, dQ += dS K
+//   dk / dv   rows = keys:    S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//
+// P and dS are rounded to the inputs' type, as the tensor cores take both operands in one 16-bit type; softmax, its
+// statistics and all sums are fp32. 2^x is the hardware approximation (2 ulp).
+//
+// A thread owns a row (or half a row), so row maxima and sums need no shuffles. One warp issues TMA, one the MMAs;
+// every barrier wait gives up after two seconds and sets the error flag.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cudaTypedefs.h>
+
+#include "attention_train.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+using namespace ub::tc;
+using namespace ub::train;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int ROWS = 128;                  // rows of a tile: TMEM lanes
+constexpr float RESCALE_THRESHOLD = 8.f;   // log2 units by which the maximum may grow before O is rescaled
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// 32 lanes x 32 columns without waiting for the data (tmem_wait_ld does).
+__device__ __forceinline__ void tmem_ld32_async(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Instruction descriptor of kind::f16, M = 128, fp32 accumulate. fmt: 0 fp16, 1 bf16; b_mn: B is MN-major.
+__device__ __forceinline__ uint32_t idesc_of(uint32_t fmt, uint32_t n, uint32_t b_mn) {
+  return instr_desc(fmt, n) | (b_mn << 16);
+}
+
+// MN-major operand: rows (K) of 64 elements (MN), 8-row swizzle atoms back to back; the next 64 elements of MN lie
+// `block_bytes` on.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, int block_bytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFF);
+  d |= (uint64_t)((block_bytes >> 4) & 0x3FFF) << 16;  // leading byte offset: next 64 elements of MN
+  d |= (uint64_t)(1024 >> 4) << 32;                    // stride byte offset: next 8 rows
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;  // 128-byte swizzle
+  return d;
+}
+
+// D = A B^T over the head dim: A [128 x hd] and B [n x hd] as K-major tiles of a_rows / b_rows rows.
+__device__ __forceinline__ void mma_heads(uint32_t d, uint32_t a, uint32_t b, int a_rows, int b_rows, int ksteps,
+                                          uint32_t idesc) {
+  for (int ks = 0; ks < ksteps; ++ks)
+    umma_bf16(d, smem_desc(a + (ks >> 2) * a_rows * 128 + (ks & 3) * 32, 128),
+              smem_desc(b + (ks >> 2) * b_rows * 128 + (ks & 3) * 32, 128), idesc, ks > 0 ? 1u : 0u);
+}
+
+// Rows r with r0 + r outside [lo, hi) of a tile become 0 (thread = row; the tile's products over the head dim are
+// complete). 0 * NaN in a masked row would otherwise reach the sums over rows.
+__device__ __forceinline__ void clear_row(uint8_t* tile, int rows, int blocks, int r) {
+  for (int b = 0; b < blocks; ++b) {
+    uint4* p = reinterpret_cast<uint4*>(tile + b * rows * 128 + r * 128);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+struct TcArgs {
+  AttnArgs a;
+  int row_tiles, units;  // units of the kernel's rows
+  int ksteps, n_hd;      // head dim / 16 rounded up, and * 16
+  uint32_t fmt;
+};
+
+struct TcUnit {
+  int seq, h, tile, split;
+};
+
+// Unit number -> work. Causal units are ordered by row tile across all heads, the longest first (`heavy_last`: the
+// last row tile is the longest); others by head, so that CTAs at work together share the streamed operand in L2.
+__device__ __forceinline__ TcUnit tc_unit(const TcArgs& t, int heads, int u, bool last_is_long) {
+  TcUnit r;
+  r.split = u % t.a.splits;
+  u /= t.a.splits;
+  if (t.a.causal) {
+    const int sh = t.a.seqs * heads;
+    const int rank = u / sh;
+    const int rest = u - rank * sh;
+    r.tile = last_is_long ? t.row_tiles - 1 - rank : rank;
+    r.h = rest % heads;
+    r.seq = rest / heads;
+  } else {
+    r.tile = u % t.row_tiles;
+    u /= t.row_tiles;
+    r.h = u % heads;
+    r.seq = u / heads;
+  }
+  return r;
+}
+
+// The k-th unit of this CTA: alternate rounds walk the CTAs in opposite directions, which evens out causal work.
+__device__ __forceinline__ int unit_index(int k) {
+  const int g = gridDim.x, c = blockIdx.x;
+  return k * g + ((k & 1) ? g - 1 - c : c);
+}
+
+__device__ __forceinline__ void tma_head(void* dst, const CUtensorMap* map, uint64_t* bar, int col, int row, int head,
+                                         int seq, int inner) {
+  const int o = seq / inner;
+  tma_load_5d(dst, map, bar, col, row, head, seq - o * inner, o);
+}
+
+// n consecutive values of a row (n a multiple of 8), times mul, to T or fp32.
+template <typename T>
+__device__ __forceinline__ void store_cols(T* out, const uint32_t* v, float mul, int n) {
+#pragma unroll
+  for (int d = 0; d < 32; d += 8) {
+    if (d < n) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = pack2<T>(__uint_as_float(v[d + 2 * e]) * mul, __uint_as_float(v[d + 2 * e + 1]) * mul);
+      *reinterpret_cast<uint4*>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+__device__ __forceinline__ void store_cols_f32(float* out, const uint32_t* v, float mul, int n) {
+#pragma unroll
+  for (int d = 0; d < 32; d += 4)
+    if (d < n)
+      *reinterpret_cast<float4*>(out + d) =
+          make_float4(__uint_as_float(v[d]) * mul, __uint_as_float(v[d + 1]) * mul, __uint_as_float(v[d + 2]) * mul,
+                      __uint_as_float(v[d + 3]) * mul);
+}
+
+// ---------------------------------------------------------------------------------------------- forward
+//
+// A CTA holds NQ tiles of 128 queries of one head (NQ = 2 shares each K / V tile between 256 queries), each with its
+// own softmax warpgroup; while one warpgroup takes exponentials, the tensor cores work for the other.
+
+template <int HD, int NQ>
+struct FwdCfg {
+  static constexpr int BN = 128;                       // keys per tile
+  static constexpr int NB = HD / 64;                   // 64-column blocks
+  static constexpr int TILE_BYTES = 128 * 128 * NB;    // a Q, K or V tile
+  static constexpr int STAGES = NQ == 2 ? (HD == 64 ? 8 : 4) : (HD == 64 ? 4 : 2);  // ring of K and V tiles
+  static constexpr int SMEM = (NQ + STAGES) * TILE_BYTES + 1024 + 512;
+  static constexpr int THREADS = NQ * 128 + 64;
+  static constexpr int TMEM = NQ * 256;
+  static constexpr int S_COL = 0, O_COL = 128;         // per query tile, 256 columns apart
+};
+
+template <typename T, int HD, int NQ>
+__global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
+    attention_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                            const __grid_constant__ CUtensorMap mv, const __grid_constant__ TcArgs ta) {
+  using C = FwdCfg<HD, NQ>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* ring = smem + NQ * C::TILE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::TILE_BYTES);
+  uint64_t* full = bars;                   // [STAGES]
+  uint64_t* empty = full + C::STAGES;      // [STAGES]
+  uint64_t* q_full = empty + C::STAGES;
+  uint64_t* q_free = q_full + 1;
+  uint64_t* s_full = q_free + 1;           // [NQ]
+  uint64_t* p_ready = s_full + NQ;         // [NQ]
+  uint64_t* pv_done = p_ready + NQ;        // [NQ]
+  uint64_t* o_free = pv_done + NQ;         // [NQ]
+  uint32_t* slot = reinterpret_cast<uint32_t*>(o_free + NQ);
+
+  const AttnArgs& a = ta.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_free, 1);
+    for (int h = 0; h < NQ; ++h) {
+      mbar_init(&s_full[h], 1);
+      mbar_init(&p_ready[h], 4);
+      mbar_init(&pv_done[h], 1);
+      mbar_init(&o_free[h], 4);
+    }
+    fence_mbar_init();
+  }
+  if (warp == NQ * 4 + 1) tmem_alloc(slot, C::TMEM);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+
+  // Key tiles of unit u: [t0, t1).
+  auto range = [&](const TcUnit& u, const Bounds& b, int& t0, int& t1) {
+    const int n = (key_end(a, b, u.tile * NQ * ROWS, NQ * ROWS) + C::BN - 1) / C::BN;
+    t0 = (int)((long long)n * u.split / a.splits);
+    t1 = (int)((long long)n * (u.split + 1) / a.splits);
+  };
+
+  if (warp == NQ * 4) {
+    if (lane == 0) {
+      bool ok = true;
+      int it = 0, nq = 0;  // ring tiles and Q loads so far
+      auto load = [&](const CUtensorMap* m, int row, int head, int seq) {
+        const int s = it % C::STAGES, r = it / C::STAGES;
+        if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) return false;
+        mbar_expect_tx(&full[s], C::TILE_BYTES);
+#pragma unroll
+        for (int b = 0; b < C::NB; ++b)
+          tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, seq, a.inner);
+        ++it;
+        return true;
+      };
+      for (int k = 0; ok; ++k) {
+        const int ui = unit_index(k);
+        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+        if (ui >= ta.units) continue;
+        const TcUnit u = tc_unit(ta, a.heads, ui, true);
+        const Bounds b = bounds_of(a, u.seq);
+        int t0, t1;
+        range(u, b, t0, t1);
+        if (t0 >= t1) continue;
+        if (nq > 0 && !mbar_wait(q_free, (nq - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        ++nq;
+        mbar_expect_tx(q_full, NQ * C::TILE_BYTES);
+#pragma unroll
+        for (int h = 0; h < NQ; ++h)
+#pragma unroll
+          for (int c = 0; c < C::NB; ++c)
+            tma_head(sQ + h * C::TILE_BYTES + c * 128 * 128, &mq, q_full, 64 * c, (u.tile * NQ + h) * ROWS, u.h, u.seq,
+                     a.inner);
+        const int hk = u.h / a.group;
+        for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u.seq) && load(&mv, t * C::BN, hk, u.seq);
+      }
+      if (!ok) atomicExch(&g_error_flag, 11);
+    }
+  } else if (warp == NQ * 4 + 1) {
+    if (lane == 0) {
+      const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
+      const uint32_t q0 = smem_u32(sQ), r0 = smem_u32(ring);
+      bool ok = true;
+      int it = 0, nq = 0, g = 0;  // ring tiles, Q loads, key tiles done
+      int units = 0;
+      auto stage = [&](int i) { return r0 + (i % C::STAGES) * C::TILE_BYTES; };
+      for (int k = 0; ok; ++k) {
+        const int ui = unit_index(k);
+        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+        if (ui >= ta.units) continue;
+        const TcUnit u = tc_unit(ta, a.heads, ui, true);
+        const Bounds b = bounds_of(a, u.seq);
+        int t0, t1;
+        range(u, b, t0, t1);
+        if (t0 >= t1) continue;
+        const int n = t1 - t0;
+        // K of tile t is ring tile it + 2 t, V is it + 2 t + 1.
+        if (!mbar_wait(q_full, nq & 1) || !mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1)) {
+          ok = false;
+          break;
+        }
+        ++nq;
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < NQ; ++h) {
+          mma_heads(tmem + h * 256 + C::S_COL, q0 + h * C::TILE_BYTES, stage(it), 128, 128, ta.ksteps, id_s);
+          umma_commit(&s_full[h]);
+        }
+        umma_commit(&empty[it % C::STAGES]);
+        if (n == 1) umma_commit(q_free);
+        for (int t = 0; t < n && ok; ++t) {
+          const int vi = it + 2 * t + 1, ki = vi + 1;
+          const bool more = t + 1 < n;
+          if (!mbar_wait(&full[vi % C::STAGES], (vi / C::STAGES) & 1) ||
+              (more && !mbar_wait(&full[ki % C::STAGES], (ki / C::STAGES) & 1))) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int h = 0; h < NQ; ++h) {
+            if (t == 0 && units > 0 && !mbar_wait(&o_free[h], (units - 1) & 1)) ok = false;
+            if (ok && !mbar_wait(&p_ready[h], g & 1)) ok = false;
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = tmem + h * 256;
+            for (int ks = 0; ks < C::BN / 16; ++ks)
+              umma_bf16_ts(d + C::O_COL, d + C::S_COL + 8 * ks, smem_desc_mn(stage(vi) + ks * 2048, 128 * 128), id_o,
+                           (t > 0 || ks > 0) ? 1u : 0u);
+            umma_commit(&pv_done[h]);
+            if (more) {
+              mma_heads(d + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps, id_s);
+              umma_commit(&s_full[h]);
+            }
+          }
+          if (!ok) break;
+          umma_commit(&empty[vi % C::STAGES]);
+          if (more) {
+            umma_commit(&empty[ki % C::STAGES]);
+            if (t + 2 == n) umma_commit(q_free);
+          }
+          ++g;
+        }
+        it += 2 * n;
+        ++units;
+      }
+      if (!ok) atomicExch(&g_error_flag, 12);
+    }
+  } else {
+    const int h = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = tmem + h * 256 + ((uint32_t)((warp & 3) * 32) << 16);
+    const float c = a.scale * LOG2E;
+    const long long rows = (long long)a.seqs * a.heads * a.lq;
+    bool ok = true;
+    int g = 0, it = 0;
+    for (int k = 0; ok; ++k) {
+      const int ui = unit_index(k);
+      if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+      if (ui >= ta.units) continue;
+      const TcUnit u = tc_unit(ta, a.heads, ui, true);
+      const Bounds b = bounds_of(a, u.seq);
+      int t0, t1;
+      range(u, b, t0, t1);
+      const int i0 = (u.tile * NQ + h) * ROWS, i = i0 + row;
+      const int limit = a.causal ? min(b.kl, i + b.off + 1) : b.kl;  // this row sees keys [0, limit)
+      float m = -INFINITY;
+      float2 sum2 = make_float2(0.f, 0.f);
+      for (int t = t0; t < t1; ++t, ++g) {
+        const int j0 = t * C::BN;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[h], g & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32_async(lanes + C::S_COL + 32 * q, s + 32 * q);
+        tmem_wait_ld();
+        if (j0 + C::BN > b.kl || (a.causal && j0 + C::BN - 1 > i0 + b.off)) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (j0 + e >= limit) s[e] = __float_as_uint(-INFINITY);
+          // V rows behind the length (NaN included) must be 0 before P V. Query tile 0 goes first.
+          if (h == 0 && a.k_lens && j0 + C::BN > b.kl) {
+            const int vi = it + 2 * (t - t0) + 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[vi % C::STAGES], (vi / C::STAGES) & 1))) {
+              ok = false;
+              break;
+            }
+            if (j0 + row >= b.kl) clear_row(ring + (vi % C::STAGES) * C::TILE_BYTES, 128, C::NB, row);
+            fence_proxy_async_smem();
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+        bool rescale = false;
+        float corr = 1.f;
+        if (top > m + RESCALE_THRESHOLD || (m == -INFINITY && top > -INFINITY)) {
+          corr = ex2(m - top);  // 0 on the first tile
+          rescale = t > t0;
+          m = top;
+          sum2.x *= corr, sum2.y *= corr;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        const float2 c2 = make_float2(c, c), mb = make_float2(-base, -base);
+#pragma unroll
+        for (int e = 0; e < 64; ++e) {
+          const float2 x = ub::fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, mb);
+          const float2 p = make_float2(ex2(x.x), ex2(x.y));
+          sum2 = add2(sum2, p);
+          s[e] = pack2<T>(p.x, p.y);
+        }
+        if (__any_sync(0xffffffffu, rescale)) {
+          // O holds the sums up to tile t - 1: they are complete once their product has signalled.
+          if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[h], (g - 1) & 1))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int q = 0; q < HD / 32; ++q) {
+            uint32_t o[32];
+            tmem_ld32(lanes + C::O_COL + 32 * q, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st32(lanes + C::O_COL + 32 * q, o);
+          }
+        }
+        tmem_st32(lanes + C::S_COL, *reinterpret_cast<uint32_t(*)[32]>(s));
+        tmem_st32(lanes + C::S_COL + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[h]);
+      }
+      if (!ok) break;
+      it += 2 * (t1 - t0);
+      const float sum = sum2.x + sum2.y;
+      const bool live = i < b.ql && (m > -INFINITY || sum != sum);  // all scores NaN: no maximum, but a NaN sum
+      const float inv = live ? 1.f / sum : 0.f;
+      const long long orow = ((long long)u.seq * a.heads + u.h) * a.lq + i;
+      if (t0 < t1) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[h], (g - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+      }
+      T* out = static_cast<T*>(a.out) + head_offset(a.out_s, a, u.seq, u.h) + (long long)i * a.out_s.row;
+      float* part = a.splits > 1 ? a.part + (u.split * rows + orow) * a.hd : nullptr;
+#pragma unroll 1
+      for (int q = 0; q < HD / 32; ++q) {
+        uint32_t o[32];
+        if (t0 < t1) tmem_ld32(lanes + C::O_COL + 32 * q, o);
+        if (!live) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+        const int n = a.hd - 32 * q;
+        if (i < a.lq && n > 0) {
+          if (part)
+            store_cols_f32(part + 32 * q, o, inv, n);
+          else
+            store_cols<T>(out + 32 * q, o, inv, n);
+        }
+      }
+      if (t0 < t1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[h]);
+      }
+      if (i < a.lq) {
+        const float lse = live ? (m + log2f(sum)) * LN2 : -INFINITY;
+        if (a.splits > 1)
+          a.part_lse[u.split * rows + orow] = lse;
+        else if (a.lse)
+          a.lse[orow] = lse;
+      }
+    }
+    if (!ok) atomicExch(&g_error_flag, 13);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == NQ * 4 + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM);
+  }
+}
+
+// --------------------------------------------------------------------------------------------------- dq
+//
+// 128 queries of one head per unit, keys streamed 128 at a time; two threads per row, 64 keys each. S is double
+// buffered and dP is read into registers first, so the tensor cores make S and dP of the next tile while this one's
+// exponentials are taken. dS of a thread's 64 keys takes 32 of the 64 columns that its scores came from.
+
+template <int HD>
+struct DqCfg {
+  static constexpr int BN = 128;
+  static constexpr int NB = HD / 64;
+  static constexpr int TILE_BYTES = 128 * 128 * NB;
+  static constexpr int STAGES = HD == 64 ? 8 : 4;
+  static constexpr int SMEM = (2 + STAGES) * TILE_BYTES + 1024 + 512;
+  static constexpr int THREADS = 256 + 64;
+  static constexpr int S_COL = 0, DP_COL = 256, DQ_COL = 384, TMEM = 512;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
+    attention_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mdo,
+                           const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                           const __grid_constant__ TcArgs ta) {
+  using C = DqCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                      // Q, then dO
+  uint8_t* sO = smem + C::TILE_BYTES;
+  uint8_t* ring = smem + 2 * C::TILE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::TILE_BYTES);
+  uint64_t* full = bars;
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* q_full = empty + C::STAGES;
+  uint64_t* q_free = q_full + 1;
+  uint64_t* s_full = q_free + 1;  // [2]
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* dp_free = dp_full + 1;
+  uint64_t* ds_ready = dp_free + 1;
+  uint64_t* dq_done = ds_ready + 1;
+  uint64_t* dq_free = dq_done + 1;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(dq_free + 1);
+
+  const AttnArgs& a = ta.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_free, 1 + 8);  // the MMA warp's commit and the row warps, which read dO for D
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(dp_free, 8);
+    mbar_init(ds_ready, 8);
+    mbar_init(dq_done, 1);
+    mbar_init(dq_free, 8);
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(slot, C::TMEM);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+
+  auto range = [&](const TcUnit& u, const Bounds& b, int& t0, int& t1) {
+    const int n = (key_end(a, b, u.tile * ROWS, ROWS) + C::BN - 1) / C::BN;
+    t0 = (int)((long long)n * u.split / a.splits);
+    t1 = (int)((long long)n * (u.split + 1) / a.splits);
+  };
+
+  if (warp == 8) {
+    if (lane == 0) {
+      bool ok = true;
+      int it = 0, nq = 0;
+      auto load = [&](const CUtensorMap* m, int row, int head, int seq) {
+        const int s = it % C::STAGES, r = it / C::STAGES;
+        if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) return false;
+        mbar_expect_tx(&full[s], C::TILE_BYTES);
+#pragma unroll
+        for (int b = 0; b < C::NB; ++b)
+          tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, seq, a.inner);
+        ++it;
+        return true;
+      };
+      for (int k = 0; ok; ++k) {
+        const int ui = unit_index(k);
+        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+        if (ui >= ta.units) continue;
+        const TcUnit u = tc_unit(ta, a.heads, ui, true);
+        const Bounds b = bounds_of(a, u.seq);
+        int t0, t1;
+        range(u, b, t0, t1);
+        if (t0 >= t1) continue;
+        if (nq > 0 && !mbar_wait(q_free, (nq - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        ++nq;
+        mbar_expect_tx(q_full, 2 * C::TILE_BYTES);
+#pragma unroll
+        for (int c = 0; c < C::NB; ++c) {
+          tma_head(sQ + c * 128 * 128, &mq, q_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+          tma_head(sO + c * 128 * 128, &mdo, q_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+        }
+        const int hk = u.h / a.group;
+        for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u.seq) && load(&mv, t * C::BN, hk, u.seq);
+      }
+      if (!ok) atomicExch(&g_error_flag, 21);
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
+      const uint32_t q0 = smem_u32(sQ), o0 = smem_u32(sO), r0 = smem_u32(ring);
+      bool ok = true;
+      int it = 0, nq = 0, g = 0, units = 0;
+      auto stage = [&](int i) { return r0 + (i % C::STAGES) * C::TILE_BYTES; };
+      auto wait_full = [&](int i) { return mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1); };
+      for (int k = 0; ok; ++k) {
+        const int ui = unit_index(k);
+        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+        if (ui >= ta.units) continue;
+        const TcUnit u = tc_unit(ta, a.heads, ui, true);
+        const Bounds b = bounds_of(a, u.seq);
+        int t0, t1;
+        range(u, b, t0, t1);
+        if (t0 >= t1) continue;
+        const int n = t1 - t0;
+        // Tile g (counted over all units): its K is ring tile it + 2 t, its V it + 2 t + 1; S in buffer g & 1.
+        auto issue_s = [&](int t) {
+          if (!wait_full(it + 2 * t)) return false;
+          tc_fence_after();
+          mma_heads(tmem + C::S_COL + ((g + t) & 1) * 128, q0, stage(it + 2 * t), 128, 128, ta.ksteps, id_s);
+          umma_commit(&s_full[(g + t) & 1]);
+          return true;
+        };
+        auto issue_dp = [&](int t) {
+          if (!wait_full(it + 2 * t + 1)) return false;
+          // dP of the tile before has been read (every tile signals once).
+          if (g + t > 0 && !mbar_wait(dp_free, (g + t - 1) & 1)) return false;
+          tc_fence_after();
+          mma_heads(tmem + C::DP_COL, o0, stage(it + 2 * t + 1), 128, 128, ta.ksteps, id_s);
+          umma_commit(dp_full);
+          umma_commit(&empty[(it + 2 * t + 1) % C::STAGES]);
+          return true;
+        };
+        if (!mbar_wait(q_full, nq & 1) || !issue_s(0) || !issue_dp(0)) {
+          ok = false;
+          break;
+        }
+        ++nq;
+        for (int t = 0; t < n; ++t) {
+          // S of the next tile overwrites dS of tile t - 1, whose product was issued before it.
+          if (t + 1 < n && (!issue_s(t + 1) || !issue_dp(t + 1))) {
+            ok = false;
+            break;
+          }
+          if (t + 1 >= n) umma_commit(q_free);
+          if (t == 0 && units > 0 && !mbar_wait(dq_free, (units - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          if (!mbar_wait(ds_ready, (g + t) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t ds = tmem + C::S_COL + ((g + t) & 1) * 128;
+          for (int ks = 0; ks < C::BN / 16; ++ks)
+            umma_bf16_ts(tmem + C::DQ_COL, ds + (ks >> 2) * 64 + (ks & 3) * 8,
+                         smem_desc_mn(stage(it + 2 * t) + ks * 2048, 128 * 128), id_o, (t > 0 || ks > 0) ? 1u : 0u);
+          umma_commit(&empty[(it + 2 * t) % C::STAGES]);
+        }
+        if (!ok) break;
+        umma_commit(dq_done);
+        g += n;
+        it += 2 * n;
+        ++units;
+      }
+      if (!ok) atomicExch(&g_error_flag, 22);
+    }
+  } else {
+    const int half = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float c = a.scale * LOG2E;
+    const long long rows = (long long)a.seqs * a.heads * a.lq;
+    bool ok = true;
+    int g = 0, it = 0, nq = 0, units = 0;
+    for (int k = 0; ok; ++k) {
+      const int ui = unit_index(k);
+      if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+      if (ui >= ta.units) continue;
+      const TcUnit u = tc_unit(ta, a.heads, ui, true);
+      const Bounds b = bounds_of(a, u.seq);
+      int t0, t1;
+      range(u, b, t0, t1);
+      const int i0 = u.tile * ROWS, i = i0 + row;
+      const int limit = a.causal ? min(b.kl, i + b.off + 1) : b.kl;
+      const long long orow = ((long long)u.seq * a.heads + u.h) * a.lq + i;
+      const bool valid = i < b.ql;
+      float lse = valid ? a.lse[orow] : -INFINITY;
+      const bool live = valid && lse != -INFINITY;
+      float D = 0.f;
+      if (t0 < t1) {
+        // D = rowsum(dO * O), by both threads of the row: dO from shared memory (16-byte chunk j of row r lies at
+        // j ^ (r & 7)), O from global memory, fetched while Q and dO arrive.
+        const T* o = static_cast<const T*>(a.out_in) + head_offset(a.out_s, a, u.seq, u.h) + (long long)i * a.out_s.row;
+        uint4 ov[HD / 8];
+#pragma unroll
+        for (int e = 0; e < HD / 8; ++e)
+          ov[e] = live && 8 * e < a.hd ? *reinterpret_cast<const uint4*>(o + 8 * e) : make_uint4(0, 0, 0, 0);
+        if (!__all_sync(0xffffffffu, mbar_wait(q_full, nq & 1))) {
+          ok = false;
+          break;
+        }
+        ++nq;
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < HD / 8; ++e) {
+            if (8 * e < a.hd) {
+              const uint4 dv = *reinterpret_cast<const uint4*>(sO + (e >> 3) * 128 * 128 + row * 128 +
+                                                               (((e & 7) ^ (row & 7)) << 4));
+              const T* x = reinterpret_cast<const T*>(&dv);
+              const T* y = reinterpret_cast<const T*>(&ov[e]);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) D = fmaf(to_f(x[q]), to_f(y[q]), D);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_free);
+      }
+      // One part leaves D: the one with the first key tile, or the first of a unit without any.
+      const bool writer = t0 < t1 ? t0 == 0 : u.split == 0 && key_end(a, b, i0, ROWS) == 0;
+      if (writer && half == 0 && i < a.lq) a.dsum[orow] = D;
+      const float lse2 = live ? lse * LOG2E : INFINITY;
+      const float2 c2 = make_float2(c, c), l2 = make_float2(-lse2, -lse2), d2 = make_float2(-D, -D);
+      for (int t = t0; t < t1; ++t, ++g) {
+        const int j0 = t * C::BN + half * 64;
+        uint32_t dp[64];
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g & 1], (g >> 1) & 1) && mbar_wait(dp_full, g & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        tmem_ld32_async(lanes + C::DP_COL + half * 64, dp);
+        tmem_ld32_async(lanes + C::DP_COL + half * 64 + 32, dp + 32);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dp_free);
+        const uint32_t scol = lanes + C::S_COL + (g & 1) * 128 + half * 64;
+        uint32_t s[64];
+        tmem_ld32_async(scol, s);
+        tmem_ld32_async(scol + 32, s + 32);
+        tmem_wait_ld();
+        const bool edge = t * C::BN + C::BN > b.kl || (a.causal && t * C::BN + C::BN - 1 > i0 + b.off);
+        if (edge) {
+          // Masked keys: P = exp(-inf) = 0 and dP = D, so dS = 0 whatever the keys hold.
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (j0 + e >= limit) s[e] = __float_as_uint(-INFINITY), dp[e] = __float_as_uint(D);
+          if (a.k_lens && t * C::BN + C::BN > b.kl && half == 0) {
+            if (t * C::BN + row >= b.kl)
+              clear_row(ring + ((it + 2 * (t - t0)) % C::STAGES) * C::TILE_BYTES, 128, C::NB, row);
+            fence_proxy_async_smem();
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float2 x = ub::fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, l2);
+          const float2 p = make_float2(ex2(x.x), ex2(x.y));
+          const float2 d = add2(make_float2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1])), d2);
+          const float2 ds = mul2(p, d);
+          s[e] = pack2<T>(ds.x, ds.y);
+        }
+        tmem_st32(scol, *reinterpret_cast<uint32_t(*)[32]>(s));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+      if (!ok) break;
+      it += 2 * (t1 - t0);
+      if (t0 < t1) {
+        if (!__all_sync(0xffffffffu, mbar_wait(dq_done, units & 1))) {
+          ok = false;
+          break;
+        }
+        ++units;
+        tc_fence_after();
+      }
+      T* dq = static_cast<T*>(a.dq) + head_offset(a.dq_s, a, u.seq, u.h) + (long long)i * a.dq_s.row;
+      float* part = a.splits > 1 ? a.part + (u.split * rows + orow) * a.hd : nullptr;
+#pragma unroll 1
+      for (int q = half * (HD / 64); q < (half + 1) * (HD / 64); ++q) {
+        uint32_t v[32];
+        if (t0 < t1) tmem_ld32(lanes + C::DQ_COL + 32 * q, v);
+        if (!live || t0 >= t1) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0;
+        }
+        const int n = a.hd - 32 * q;
+        if (i < a.lq && n > 0) {
+          if (part)
+            store_cols_f32(part + 32 * q, v, a.scale, n);
+          else
+            store_cols<T>(dq + 32 * q, v, a.scale, n);
+        }
+      }
+      if (t0 < t1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dq_free);
+      }
+    }
+    if (!ok) atomicExch(&g_error_flag, 23);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- dk, dv
+//
+// 128 keys of one key/value head per unit; the queries of all heads of its group are streamed (128 at a time, 64 for
+// head dims over 64, where the two accumulators take half of TMEM). Two threads per key, half of the tile's queries
+// each. lse and D go by column here: a warp brings them to shared memory, and rows that must not count come with
+// lse = +inf, P = 0. P^T and dS^T of a thread share the columns of its scores.
+
+template <int HD>
+struct DkvCfg {
+  static constexpr int BN = HD == 64 ? 128 : 64;
+  static constexpr int NB = HD / 64;
+  static constexpr int KV_BYTES = 128 * 128 * NB;
+  static constexpr int TILE_BYTES = BN * 128 * NB;  // Q or dO: 16 KB
+  static constexpr int STAGES = 4;                  // (Q, dO) pairs
+  static constexpr int STATS = 4;                   // (lse, D) rows
+  static constexpr int SMEM = 2 * KV_BYTES + 2 * STAGES * TILE_BYTES + STATS * BN * 8 + 1024 + 512;
+  static constexpr int THREADS = 256 + 96;
+  static constexpr int HALF = BN / 2;
+  static constexpr int S_COL = 0, DP_COL = 2 * BN, DV_COL = 3 * BN, DK_COL = 3 * BN + HD, TMEM = 512;
+  static_assert(3 * BN + 2 * HD <= 512, "TMEM columns");
+};
+
+// P of fp16 calls is kept times 2^12: probabilities of long rows would sink into fp16's subnormals.
+template <typename T>
+__device__ __forceinline__ constexpr float p_shift() {
+  return 0.f;
+}
+template <>
+__device__ __forceinline__ constexpr float p_shift<__half>() {
+  return 12.f;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
+    attention_dkv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                            const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mdo,
+                            const __grid_constant__ TcArgs ta) {
+  using C = DkvCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = smem + C::KV_BYTES;
+  uint8_t* ring = smem + 2 * C::KV_BYTES;  // [STAGES][Q, dO]
+  float* stats = reinterpret_cast<float*>(ring + 2 * C::STAGES * C::TILE_BYTES);  // [STATS][lse2 BN, -D BN]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stats + C::STATS * 2 * C::BN);
+  uint64_t* full = bars;                  // [STAGES] Q and dO
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* kv_full = empty + C::STAGES;
+  uint64_t* kv_free = kv_full + 1;
+  uint64_t* s_full = kv_free + 1;         // [2]
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* dp_free = dp_full + 1;
+  uint64_t* ps_ready = dp_free + 1;
+  uint64_t* st_full = ps_ready + 1;       // [STATS]
+  uint64_t* st_free = st_full + C::STATS; // [STATS]
+  uint64_t* acc_done = st_free + C::STATS;
+  uint64_t* acc_free = acc_done + 1;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(acc_free + 1);
+
+  const AttnArgs& a = ta.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < C::STATS; ++i) mbar_init(&st_full[i], 32), mbar_init(&st_free[i], 8);
+    mbar_init(kv_full, 1);
+    mbar_init(kv_free, 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(dp_free, 8);
+    mbar_init(ps_ready, 8);
+    mbar_init(acc_done, 1);
+    mbar_init(acc_free, 8);
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(slot, C::TMEM);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+
+  // Tiles of a unit: for each head of the group, query tiles [begin, begin + per); t in [t0, t1) of all of them.
+  auto range = [&](const TcUnit& u, const Bounds& b, int& begin, int& per, int& t0, int& t1) {
+    const int j0 = u.tile * ROWS;
+    begin = query_begin(a, b, j0) / C::BN;
+    per = j0 < b.kl ? max(0, (b.ql + C::BN - 1) / C::BN - begin) : 0;
+    const int total = per * a.group;
+    t0 = (int)((long long)total * u.split / a.splits);
+    t1 = (int)((long long)total * (u.split + 1) / a.splits);
+  };
+
+  if (warp == 8) {
+    if (lane == 0) {
+      bool ok = true;
+      int it = 0, nkv = 0;
+      for (int k = 0; ok; ++k) {
+        const int ui = unit_index(k);
+        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+        if (ui >= ta.units) continue;
+        const TcUnit u = tc_unit(ta, a.kv_heads, ui, false);
+        const Bounds b = bounds_of(a, u.seq);
+        int begin, per, t0, t1;
+        range(u, b, begin, per, t0, t1);
+        if (t0 >= t1) continue;
+        if (nkv > 0 && !mbar_wait(kv_free, (nkv - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        ++nkv;
+        mbar_expect_tx(kv_full, 2 * C::KV_BYTES);
+#pragma unroll
+        for (int c = 0; c < C::NB; ++c) {
+          tma_head(sK + c * 128 * 128, &mk, kv_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+          tma_head(sV + c * 128 * 128, &mv, kv_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+        }
+        for (int t = t0; t < t1; ++t, ++it) {
+          const int h = u.h * a.group + t / per, i0 = (begin + t % per) * C::BN;
+          const int s = it % C::STAGES, r = it / C::STAGES;
+          if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(&full[s], 2 * C::TILE_BYTES);
+          uint8_t* d = ring + 2 * s * C::TILE_BYTES;
+#pragma unroll
+          for (int c = 0; c < C::NB; ++c) {
+            tma_head(d + c * C::BN * 128, &mq, &full[s], 64 * c, i0, h, u.seq, a.inner);
+            tma_head(d + C::TILE_BYTES + c * C::BN * 128, &mdo, &full[s], 64 * c, i0, h, u.seq, a.inner);
+          }
+        }
+      }
+      if (!ok) atomicExch(&g_error_flag, 31);
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
+      const uint32_t k0 = smem_u32(sK), v0 = smem_u32(sV), r0 = smem_u32(ring);
+      bool ok = true;
+      int g = 0, units = 0;  // tiles of all units: ring, S buffers and barriers go by g
+      auto q_tile = [&](int i) { return r0 + 2 * (i % C::STAGES) * C::TILE_BYTES; };
+      auto issue_s = [&](int i) {
+        if (!mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1)) return false;
+        tc_fence_after();
+        mma_heads(tmem + C::S_COL + (i & 1) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
+        umma_commit(&s_full[i & 1]);
+        return true;
+      };
+      auto issue_dp = [&](int i) {
+        if (i > 0 && !mbar_wait(dp_free, (i - 1) & 1)) return false;
+        tc_fence_after();
+        mma_heads(tmem + C::DP_COL, v0, q_tile(i) + C::TILE_BYTES, 128, C::BN, ta.ksteps, id_s);
+        umma_commit(dp_full);
+        return true;
+      };
+      for (int k = 0; ok; ++k) {
+        const int ui = unit_index(k);
+        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+        if (ui >= ta.units) continue;
+        const TcUnit u = tc_unit(ta, a.kv_heads, ui, false);
+        const Bounds b = bounds_of(a, u.seq);
+        int begin, per, t0, t1;
+        range(u, b, begin, per, t0, t1);
+        if (t0 >= t1) continue;
+        const int n = t1 - t0;
+        if (!mbar_wait(kv_full, units & 1) || !issue_s(g) || !issue_dp(g)) {
+          ok = false;
+          break;
+        }
+        for (int t = 0; t < n; ++t) {
+          if (t + 1 < n && (!issue_s(g + t + 1) || !issue_dp(g + t + 1))) {
+            ok = false;
+            break;
+          }
+          if (t + 1 == n) umma_commit(kv_free);
+          if ((t == 0 && units > 0 && !mbar_wait(acc_free, (units - 1) & 1)) || !mbar_wait(ps_ready, (g + t) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t p = tmem + C::S_COL + ((g + t) & 1) * C::BN, q = q_tile(g + t);
+          constexpr int KH = C::HALF / 16;  // K steps per half of the tile's queries
+          for (int ks = 0; ks < 2 * KH; ++ks)
+            umma_bf16_ts(tmem + C::DV_COL, p + (ks / KH) * C::HALF + (ks % KH) * 8,
+                         smem_desc_mn(q + C::TILE_BYTES + ks * 2048, C::BN * 128), id_o,
+                         (t > 0 || ks > 0) ? 1u : 0u);
+          for (int ks = 0; ks < 2 * KH; ++ks)
+            umma_bf16_ts(tmem + C::DK_COL, p + (ks / KH) * C::HALF + C::HALF / 2 + (ks % KH) * 8,
+                         smem_desc_mn(q + ks * 2048, C::BN * 128), id_o, (t > 0 || ks > 0) ? 1u : 0u);
+          umma_commit(&empty[(g + t) % C::STAGES]);
+        }
+        if (!ok) break;
+        umma_commit(acc_done);
+        g += n;
+        ++units;
+      }
+      if (!ok) atomicExch(&g_error_flag, 32);
+    }
+  } else if (warp == 10) {
+    // (lse in log2 units, -D) of each streamed tile; +inf and 0 for rows outside the queries.
+    bool ok = true;
+    int g = 0;
+    for (int k = 0; ok; ++k) {
+      const int ui = unit_index(k);
+      if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+      if (ui >= ta.units) continue;
+      const TcUnit u = tc_unit(ta, a.kv_heads, ui, false);
+      const Bounds b = bounds_of(a, u.seq);
+      int begin, per, t0, t1;
+      range(u, b, begin, per, t0, t1);
+      for (int t = t0; t < t1; ++t, ++g) {
+        const int h = u.h * a.group + t / per, i0 = (begin + t % per) * C::BN;
+        const long long row0 = ((long long)u.seq * a.heads + h) * a.lq + i0;
+        const int sb = g % C::STATS, r = g / C::STATS;
+        float l[C::BN / 32], d[C::BN / 32];
+#pragma unroll
+        for (int e = 0; e < C::BN / 32; ++e) {
+          const int i = 32 * e + lane;
+          const bool in = i0 + i < b.ql;
+          const float x = in ? a.lse[row0 + i] : -INFINITY;
+          l[e] = x == -INFINITY ? INFINITY : x * LOG2E - p_shift<T>();
+          d[e] = in ? -a.dsum[row0 + i] : 0.f;
+        }
+        if (r > 0 && !__all_sync(0xffffffffu, mbar_wait(&st_free[sb], (r - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        float* s = stats + sb * 2 * C::BN;
+#pragma unroll
+        for (int e = 0; e < C::BN / 32; ++e) {
+          s[32 * e + lane] = l[e];
+          s[C::BN + 32 * e + lane] = d[e];
+        }
+        mbar_arrive(&st_full[sb]);
+      }
+    }
+    if (!ok && lane == 0) atomicExch(&g_error_flag, 34);
+  } else {
+    const int half = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float c = a.scale * LOG2E;
+    const float unshift = exp2f(-p_shift<T>());
+    const float2 c2 = make_float2(c, c), un2 = make_float2(unshift, unshift);
+    const long long rows = (long long)a.seqs * a.kv_heads * a.lk;
+    bool ok = true;
+    int g = 0, units = 0;
+    for (int k = 0; ok; ++k) {
+      const int ui = unit_index(k);
+      if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+      if (ui >= ta.units) continue;
+      const TcUnit u = tc_unit(ta, a.kv_heads, ui, false);
+      const Bounds b = bounds_of(a, u.seq);
+      int begin, per, t0, t1;
+      range(u, b, begin, per, t0, t1);
+      const int j0 = u.tile * ROWS, j = j0 + row;
+      const int first = a.causal ? max(0, -b.off) : 0;       // queries before it see no key
+      const int from = a.causal ? max(first, j - b.off) : 0; // this key is seen by queries [from, b.ql)
+      for (int t = t0; t < t1; ++t, ++g) {
+        const int i0 = (begin + t % per) * C::BN;
+        uint32_t dp[C::HALF], s[C::HALF];
+        const int sb = g % C::STATS;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g & 1], (g >> 1) & 1) && mbar_wait(dp_full, g & 1) &&
+                                         mbar_wait(&st_full[sb], (g / C::STATS) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < C::HALF; q += 32) tmem_ld32_async(lanes + C::DP_COL + half * C::HALF + q, dp + q);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dp_free);
+        const uint32_t scol = lanes + C::S_COL + (g & 1) * C::BN + half * C::HALF;
+#pragma unroll
+        for (int q = 0; q < C::HALF; q += 32) tmem_ld32_async(scol + q, s + q);
+        tmem_wait_ld();
+        const float4* l4 = reinterpret_cast<const float4*>(stats + sb * 2 * C::BN + half * C::HALF);
+        const float4* d4 = reinterpret_cast<const float4*>(stats + sb * 2 * C::BN + C::BN + half * C::HALF);
+        if (i0 + C::BN > b.ql || i0 < first || (a.causal && j0 + ROWS - 1 > i0 + b.off)) {
+          const int ib = i0 + half * C::HALF;
+#pragma unroll
+          for (int e = 0; e < C::HALF; ++e)
+            if (ib + e < from || ib + e >= b.ql) s[e] = __float_as_uint(-INFINITY), dp[e] = 0;
+          // Rows of Q and dO that must not count (NaN included) become 0 before they are summed over.
+          if ((a.q_lens && i0 + C::BN > b.ql) || i0 < first) {
+            if (row < C::BN && (i0 + row >= b.ql || i0 + row < first))
+              clear_row(ring + (2 * (g % C::STAGES) + half) * C::TILE_BYTES, C::BN, C::NB, row);
+            fence_proxy_async_smem();
+          }
+        }
+        uint32_t pk[C::HALF / 2];
+#pragma unroll
+        for (int e = 0; e < C::HALF / 4; ++e) {
+          const float4 l = l4[e], d = d4[e];
+          const float2 xa = ub::fma2(make_float2(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1])), c2,
+                                     make_float2(-l.x, -l.y));
+          const float2 xb = ub::fma2(make_float2(__uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3])), c2,
+                                     make_float2(-l.z, -l.w));
+          const float2 pa = make_float2(ex2(xa.x), ex2(xa.y)), pb = make_float2(ex2(xb.x), ex2(xb.y));
+          float2 ga = add2(make_float2(__uint_as_float(dp[4 * e]), __uint_as_float(dp[4 * e + 1])),
+                           make_float2(d.x, d.y));
+          float2 gb = add2(make_float2(__uint_as_float(dp[4 * e + 2]), __uint_as_float(dp[4 * e + 3])),
+                           make_float2(d.z, d.w));
+          if (p_shift<T>() != 0.f) ga = mul2(ga, un2), gb = mul2(gb, un2);
+          ga = mul2(pa, ga);
+          gb = mul2(pb, gb);
+          pk[2 * e] = pack2<T>(pa.x, pa.y);
+          pk[2 * e + 1] = pack2<T>(pb.x, pb.y);
+          s[2 * e] = pack2<T>(ga.x, ga.y);
+          s[2 * e + 1] = pack2<T>(gb.x, gb.y);
+        }
+        if constexpr (C::HALF == 64) {
+          tmem_st32(scol, *reinterpret_cast<uint32_t(*)[32]>(pk));
+          tmem_st32(scol + 32, *reinterpret_cast<uint32_t(*)[32]>(s));
+        } else {
+          tmem_st16(scol, *reinterpret_cast<uint32_t(*)[16]>(pk));
+          tmem_st16(scol + 16, *reinterpret_cast<uint32_t(*)[16]>(s));
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(ps_ready);
+          mbar_arrive(&st_free[sb]);
+        }
+      }
+      if (!ok) break;
+      if (t0 < t1) {
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_done, units & 1))) {
+          ok = false;
+          break;
+        }
+        ++units;
+        tc_fence_after();
+      }
+      const bool live = j < b.kl && t0 < t1;
+      const long long orow = ((long long)u.seq * a.kv_heads + u.h) * a.lk + j;
+      // Threads of half 0 write dV, of half 1 dK.
+      T* out = static_cast<T*>(half ? a.dk : a.dv) + head_offset(half ? a.dk_s : a.dv_s, a, u.seq, u.h) +
+               (long long)j * (half ? a.dk_s.row : a.dv_s.row);
+      float* part = a.splits > 1 ? a.part + ((half ? 0 : a.splits) + u.split) * rows * a.hd + orow * a.hd : nullptr;
+      const float mul = half ? a.scale : unshift;
+#pragma unroll 1
+      for (int q = 0; q < HD / 32; ++q) {
+        uint32_t v[32];
+        if (t0 < t1) tmem_ld32(lanes + (half ? C::DK_COL : C::DV_COL) + 32 * q, v);
+        if (!live) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0;
+        }
+        const int n = a.hd - 32 * q;
+        if (j < a.lk && n > 0) {
+          if (part)
+            store_cols_f32(part + 32 * q, v, mul, n);
+          else
+            store_cols<T>(out + 32 * q, v, mul, n);
+        }
+      }
+      if (t0 < t1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_free);
+      }
+    }
+    if (!ok) atomicExch(&g_error_flag, 33);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- host
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+// (dim, row, head, inner, outer) map of a tensor: boxes of 64 dims x `box_rows` rows of one head.
+bool head_map(CUtensorMap* m, const void* base, const UnblendHeadStrides& s, const UnblendAttnTrainParams& p, int heads,
+              int rows, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  auto legal = [](long long st, int n) { return (cuuint64_t)(n == 1 ? 16 : st * 2); };
+  cuuint64_t dims[5] = {(cuuint64_t)p.hd, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)p.inner,
+                        (cuuint64_t)p.outer};
+  cuuint64_t strides[4] = {legal(s.row, rows), legal(s.head, heads), legal(s.inner, p.inner),
+                           legal(s.outer, p.outer)};
+  cuuint32_t box[5] = {64, (cuuint32_t)box_rows, 1, 1, 1};
+  cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  return fn(m, p.dtype == UNBLEND_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+            const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+TcArgs tc_args(const AttnArgs& a, const UnblendAttnTrainParams& p, int heads, int len, int rows_per_unit, int splits,
+               float* part) {
+  TcArgs t{};
+  t.a = a;
+  t.a.splits = splits;
+  t.a.part = splits > 1 ? part : nullptr;
+  t.row_tiles = (len + rows_per_unit - 1) / rows_per_unit;
+  t.units = (int)((long long)a.seqs * heads * t.row_tiles * splits);
+  t.ksteps = (p.hd + 15) / 16;
+  t.n_hd = 16 * t.ksteps;
+  t.fmt = p.dtype == UNBLEND_BF16 ? 1u : 0u;
+  return t;
+}
+
+int grid_of(int units, int per_sm) { return units < per_sm * ub::kNumSMs ? units : per_sm * ub::kNumSMs; }
+
+template <typename T, int HD, int NQ>
+int launch_fwd(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, cudaStream_t st) {
+  using C = FwdCfg<HD, NQ>;
+  CUtensorMap mq, mk, mv;
+  if (!head_map(&mq, a.q, p.q, p, p.heads, p.lq, 128) || !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, 128) ||
+      !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, 128))
+    return UNBLEND_ERR_INVALID;
+  const TcArgs t = tc_args(a, p, p.heads, p.lq, NQ * ROWS, splits, a.part);
+  auto kern = attention_fwd_tc_kernel<T, HD, NQ>;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  kern<<<grid_of(t.units, NQ == 2 ? 1 : 2), C::THREADS, C::SMEM, st>>>(mq, mk, mv, t);
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, int HD>
+int launch_dq(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st) {
+  using C = DqCfg<HD>;
+  CUtensorMap mq, mdo, mk, mv;
+  if (!head_map(&mq, a.q, p.q, p, p.heads, p.lq, 128) || !head_map(&mdo, a.dout, p.dout, p, p.heads, p.lq, 128) ||
+      !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, 128) || !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, 128))
+    return UNBLEND_ERR_INVALID;
+  const TcArgs t = tc_args(a, p, p.heads, p.lq, ROWS, splits, part);
+  auto kern = attention_dq_tc_kernel<T, HD>;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  kern<<<grid_of(t.units, 1), C::THREADS, C::SMEM, st>>>(mq, mdo, mk, mv, t);
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, int HD>
+int launch_dkv(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st) {
+  using C = DkvCfg<HD>;
+  CUtensorMap mq, mdo, mk, mv;
+  if (!head_map(&mq, a.q, p.q, p, p.heads, p.lq, C::BN) || !head_map(&mdo, a.dout, p.dout, p, p.heads, p.lq, C::BN) ||
+      !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, 128) || !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, 128))
+    return UNBLEND_ERR_INVALID;
+  const TcArgs t = tc_args(a, p, p.kv_heads, p.lk, ROWS, splits, part);
+  auto kern = attention_dkv_tc_kernel<T, HD>;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  kern<<<grid_of(t.units, 1), C::THREADS, C::SMEM, st>>>(mk, mv, mq, mdo, t);
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
+}  // namespace
+
+namespace ub {
+namespace train {
+
+int attention_fwd_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int rows_per_cta, cudaStream_t st) {
+  auto go = [&](auto zero) {
+    using T = decltype(zero);
+    if (rows_per_cta == 256)
+      return p.hd <= 64 ? launch_fwd<T, 64, 2>(a, p, a.splits, st) : launch_fwd<T, 128, 2>(a, p, a.splits, st);
+    return p.hd <= 64 ? launch_fwd<T, 64, 1>(a, p, a.splits, st) : launch_fwd<T, 128, 1>(a, p, a.splits, st);
+  };
+  return p.dtype == UNBLEND_BF16 ? go(__nv_bfloat16()) : go(__half());
+}
+
+int attention_dq_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st) {
+  if (p.dtype == UNBLEND_BF16)
+    return p.hd <= 64 ? launch_dq<__nv_bfloat16, 64>(a, p, splits, part, st)
+                      : launch_dq<__nv_bfloat16, 128>(a, p, splits, part, st);
+  return p.hd <= 64 ? launch_dq<__half, 64>(a, p, splits, part, st) : launch_dq<__half, 128>(a, p, splits, part, st);
+}
+
+int attention_dkv_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st) {
+  if (p.dtype == UNBLEND_BF16)
+    return p.hd <= 64 ? launch_dkv<__nv_bfloat16, 64>(a, p, splits, part, st)
+                      : launch_dkv<__nv_bfloat16, 128>(a, p, splits, part, st);
+  return p.hd <= 64 ? launch_dkv<__half, 64>(a, p, splits, part, st) : launch_dkv<__half, 128>(a, p, splits, part, st);
+}
+
+// What the tensor-core kernels can address: 16-byte rows and strides (TMA, vector stores), a positive scale (the row
+// maximum is taken before the scale).
+bool attention_tc_fits(const UnblendAttnTrainParams& p, const void* const* ptrs, const UnblendHeadStrides* strides,
+                       const int* heads, const int* rows, int n) {
+  if (p.dtype == UNBLEND_F32 || p.hd % 8 != 0 || !(p.scale > 0.f)) return false;
+  for (int i = 0; i < n; ++i) {
+    if (reinterpret_cast<uintptr_t>(ptrs[i]) % 16 != 0) return false;
+    const UnblendHeadStrides& s = strides[i];
+    const long long st[4] = {s.row, s.head, s.inner, s.outer};
+    const int ext[4] = {rows[i], heads[i], p.inner, p.outer};
+    for (int k = 0; k < 4; ++k)
+      if (ext[k] > 1 && (st[k] <= 0 || st[k] % 8 != 0 || st[k] >= (1LL << 38))) return false;
+  }
+  return true;
+}
+
+}  // namespace train
+}  // namespace ub
+
+extern "C" int unblend_attention_train_error_flag(int* out_host, int clear) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_error_flag, sizeof(int));
+  if (e != cudaSuccess) return (int)e;
+  if (out_host) *out_host = v;
+  if (clear) {
+    int z = 0;
+    e = cudaMemcpyToSymbol(g_error_flag, &z, sizeof(int));
+    if (e != cudaSuccess) return (int)e;
+  }
+  return 0;
+}
