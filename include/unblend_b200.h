@@ -577,7 +577,7 @@ int unblend_layer_norm_forward(const void* x, long long x_so, long long x_si, vo
                                int cols, int dtype, int w_dtype, void* stream);
 
 /* dx (contiguous), and dgamma / dbeta [cols] (both or neither) from dy, x and the forward's stats. work:
- * unblend_layer_norm_grad_workspace bytes, 16-byte aligned (not needed without dgamma). */
+ * unblend_layer_norm_grad_workspace bytes (0 for few rows; not needed without dgamma). */
 int unblend_layer_norm_backward(const void* dy, long long dy_so, long long dy_si, const void* x, long long x_so,
                                 long long x_si, const float* stats, const void* gamma, void* dx, void* dgamma,
                                 void* dbeta, float* work, long long outer, long long inner, int cols, int dtype,
@@ -645,6 +645,9 @@ int unblend_attention_forward(const void* q, const void* k, const void* v, void*
 int unblend_attention_backward(const void* dout, const void* q, const void* k, const void* v, const void* out,
                                const float* lse, void* dq, void* dk, void* dv, void* work, long long work_bytes,
                                const UnblendAttnTrainParams* p, void* stream);
+
+/* Device flag set when a bounded wait of the two entry points above gives up (0 = none). Synchronous host call. */
+int unblend_attention_train_error_flag(int* out_host, int clear);
 
 
 #ifdef __cplusplus

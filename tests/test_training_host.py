@@ -129,7 +129,8 @@ def test_workspace_queries_check_their_arguments():
         assert lib.unblend_attention_workspace(ctypes.byref(_params(**bad)), 0, ctypes.byref(n)) == _lib.ERR_INVALID
     assert lib.unblend_attention_workspace(None, 0, ctypes.byref(n)) == _lib.ERR_INVALID
     assert lib.unblend_attention_workspace(ctypes.byref(_params()), 0, None) == _lib.ERR_INVALID
-    assert lib.unblend_layer_norm_grad_workspace(10, 64, ctypes.byref(n)) == 0 and n.value >= 8 * 64
+    assert lib.unblend_layer_norm_grad_workspace(1000, 64, ctypes.byref(n)) == 0 and n.value >= 8 * 64
+    assert lib.unblend_layer_norm_grad_workspace(10, 64, ctypes.byref(n)) == 0 and n.value == 0
     assert lib.unblend_layer_norm_grad_workspace(0, 64, ctypes.byref(n)) == _lib.ERR_INVALID
     assert lib.unblend_dropout_add_grad_workspace(10, 65, ctypes.byref(n)) == 0 and n.value >= 4 * 65
     assert lib.unblend_dropout_add_grad_workspace(1 << 31, 65, ctypes.byref(n)) == _lib.ERR_INVALID
@@ -146,7 +147,7 @@ def test_entry_points_refuse_before_they_launch():
     assert lib.unblend_layer_norm_forward(p, 0, 4, p, p, p, p, 1e-5, 1, 1, 4, 0, 1, None) == bad
     assert lib.unblend_layer_norm_forward(p, 0, 4, p, p, p, p, 1e-5, 1 << 20, 1 << 20, 4, 0, 0, None) == bad
     assert lib.unblend_layer_norm_backward(p, 0, 4, p, 0, 4, p, p, p, p, None, p, 1, 1, 4, 0, 0, None) == bad
-    assert lib.unblend_layer_norm_backward(p, 0, 4, p, 0, 4, p, p, p, p, p, None, 1, 1, 4, 0, 0, None) == bad
+    assert lib.unblend_layer_norm_backward(p, 0, 4, p, 0, 4, p, p, p, p, p, None, 1, 1000, 4, 0, 0, None) == bad
     assert lib.unblend_dropout_add_forward(p, 0, 4, p, 0, 4, p, p, 1.5, p, 1, 1, 4, 0, 0, 0, None) == bad
     assert lib.unblend_dropout_add_forward(p, 0, 4, p, 0, 4, p, p, 0.5, p + 4, 1, 1, 4, 0, 0, 0, None) == bad
     assert lib.unblend_dropout_add_forward(p, 0, 4, p, 0, 4, p, p, 0.5, p, 1, 1, 4, 0, 1, 0, None) == bad

@@ -301,17 +301,17 @@ probe: list | None = None
 def call(name: str, *args, work: float | None = None) -> None:
     """Invoke ``name`` with ``args`` (the trailing stream is appended) and check it."""
     lib = load()
-    cur = torch.cuda.current_stream()
-    stream = c_void_p(cur.cuda_stream)
     if probe is not None:
+        cur = torch.cuda.current_stream()
         start = torch.cuda.Event(enable_timing=True)
         end = torch.cuda.Event(enable_timing=True)
         start.record(cur)
-        rc = getattr(lib, name)(*args, stream)
+        rc = getattr(lib, name)(*args, cur.cuda_stream)
         end.record(cur)
         probe.append((name, start, end, work))
     else:
-        rc = getattr(lib, name)(*args, stream)
+        # The handle alone: building a torch.cuda.Stream object costs more than most launches.
+        rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
     counters["launches"] += KERNELS_PER_CALL.get(name, 1)
     check(name, rc)
 

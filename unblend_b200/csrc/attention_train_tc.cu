@@ -80,6 +80,16 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t addr, uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// Moves a warpgroup's registers per thread; the warpgroups' shares of a CTA add up to what it was launched with.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // Instruction descriptor of kind::f16, M = 128, fp32 accumulate. fmt: 0 fp16, 1 bf16; b_mn: B is MN-major.
 __device__ __forceinline__ uint32_t idesc_of(uint32_t fmt, uint32_t n, uint32_t b_mn) {
   return instr_desc(fmt, n) | (b_mn << 16);
@@ -195,7 +205,9 @@ struct FwdCfg {
   static constexpr int TILE_BYTES = 128 * 128 * NB;    // a Q, K or V tile
   static constexpr int STAGES = NQ == 2 ? (HD == 64 ? 8 : 4) : (HD == 64 ? 4 : 2);  // ring of K and V tiles
   static constexpr int SMEM = (NQ + STAGES) * TILE_BYTES + 1024 + 512;
-  static constexpr int THREADS = NQ * 128 + 64;
+  static constexpr int THREADS = NQ * 128 + 128;       // softmax warpgroups, then one for TMA and MMA issue
+  // Registers: 3 x 168 = 2 x 208 + 88 (NQ = 2, one CTA per SM), 2 x 128 = 200 + 56 (NQ = 1, two).
+  static constexpr int REGS_MORE = NQ == 2 ? 208 : 200, REGS_LESS = NQ == 2 ? 88 : 56;
   static constexpr int TMEM = NQ * 256;
   static constexpr int S_COL = 0, O_COL = 128;         // per query tile, 256 columns apart
 };
@@ -247,116 +259,120 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
     t1 = (int)((long long)n * (u.split + 1) / a.splits);
   };
 
-  if (warp == NQ * 4) {
-    if (lane == 0) {
-      bool ok = true;
-      int it = 0, nq = 0;  // ring tiles and Q loads so far
-      auto load = [&](const CUtensorMap* m, int row, int head, int seq) {
-        const int s = it % C::STAGES, r = it / C::STAGES;
-        if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) return false;
-        mbar_expect_tx(&full[s], C::TILE_BYTES);
+  if (warp >= NQ * 4) {
+    regs_down<C::REGS_LESS>();
+    if (warp == NQ * 4) {
+      if (lane == 0) {
+        bool ok = true;
+        int it = 0, nq = 0;  // ring tiles and Q loads so far
+        auto load = [&](const CUtensorMap* m, int row, int head, int seq) {
+          const int s = it % C::STAGES, r = it / C::STAGES;
+          if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) return false;
+          mbar_expect_tx(&full[s], C::TILE_BYTES);
 #pragma unroll
-        for (int b = 0; b < C::NB; ++b)
-          tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, seq, a.inner);
-        ++it;
-        return true;
-      };
-      for (int k = 0; ok; ++k) {
-        const int ui = unit_index(k);
-        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
-        if (ui >= ta.units) continue;
-        const TcUnit u = tc_unit(ta, a.heads, ui, true);
-        const Bounds b = bounds_of(a, u.seq);
-        int t0, t1;
-        range(u, b, t0, t1);
-        if (t0 >= t1) continue;
-        if (nq > 0 && !mbar_wait(q_free, (nq - 1) & 1)) {
-          ok = false;
-          break;
-        }
-        ++nq;
-        mbar_expect_tx(q_full, NQ * C::TILE_BYTES);
-#pragma unroll
-        for (int h = 0; h < NQ; ++h)
-#pragma unroll
-          for (int c = 0; c < C::NB; ++c)
-            tma_head(sQ + h * C::TILE_BYTES + c * 128 * 128, &mq, q_full, 64 * c, (u.tile * NQ + h) * ROWS, u.h, u.seq,
-                     a.inner);
-        const int hk = u.h / a.group;
-        for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u.seq) && load(&mv, t * C::BN, hk, u.seq);
-      }
-      if (!ok) atomicExch(&g_error_flag, 11);
-    }
-  } else if (warp == NQ * 4 + 1) {
-    if (lane == 0) {
-      const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
-      const uint32_t q0 = smem_u32(sQ), r0 = smem_u32(ring);
-      bool ok = true;
-      int it = 0, nq = 0, g = 0;  // ring tiles, Q loads, key tiles done
-      int units = 0;
-      auto stage = [&](int i) { return r0 + (i % C::STAGES) * C::TILE_BYTES; };
-      for (int k = 0; ok; ++k) {
-        const int ui = unit_index(k);
-        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
-        if (ui >= ta.units) continue;
-        const TcUnit u = tc_unit(ta, a.heads, ui, true);
-        const Bounds b = bounds_of(a, u.seq);
-        int t0, t1;
-        range(u, b, t0, t1);
-        if (t0 >= t1) continue;
-        const int n = t1 - t0;
-        // K of tile t is ring tile it + 2 t, V is it + 2 t + 1.
-        if (!mbar_wait(q_full, nq & 1) || !mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1)) {
-          ok = false;
-          break;
-        }
-        ++nq;
-        tc_fence_after();
-#pragma unroll
-        for (int h = 0; h < NQ; ++h) {
-          mma_heads(tmem + h * 256 + C::S_COL, q0 + h * C::TILE_BYTES, stage(it), 128, 128, ta.ksteps, id_s);
-          umma_commit(&s_full[h]);
-        }
-        umma_commit(&empty[it % C::STAGES]);
-        if (n == 1) umma_commit(q_free);
-        for (int t = 0; t < n && ok; ++t) {
-          const int vi = it + 2 * t + 1, ki = vi + 1;
-          const bool more = t + 1 < n;
-          if (!mbar_wait(&full[vi % C::STAGES], (vi / C::STAGES) & 1) ||
-              (more && !mbar_wait(&full[ki % C::STAGES], (ki / C::STAGES) & 1))) {
+          for (int b = 0; b < C::NB; ++b)
+            tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, seq, a.inner);
+          ++it;
+          return true;
+        };
+        for (int k = 0; ok; ++k) {
+          const int ui = unit_index(k);
+          if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+          if (ui >= ta.units) continue;
+          const TcUnit u = tc_unit(ta, a.heads, ui, true);
+          const Bounds b = bounds_of(a, u.seq);
+          int t0, t1;
+          range(u, b, t0, t1);
+          if (t0 >= t1) continue;
+          if (nq > 0 && !mbar_wait(q_free, (nq - 1) & 1)) {
             ok = false;
             break;
           }
+          ++nq;
+          mbar_expect_tx(q_full, NQ * C::TILE_BYTES);
+#pragma unroll
+          for (int h = 0; h < NQ; ++h)
+#pragma unroll
+            for (int c = 0; c < C::NB; ++c)
+              tma_head(sQ + h * C::TILE_BYTES + c * 128 * 128, &mq, q_full, 64 * c, (u.tile * NQ + h) * ROWS, u.h, u.seq,
+                       a.inner);
+          const int hk = u.h / a.group;
+          for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u.seq) && load(&mv, t * C::BN, hk, u.seq);
+        }
+        if (!ok) atomicExch(&g_error_flag, 11);
+      }
+    } else if (warp == NQ * 4 + 1) {
+      if (lane == 0) {
+        const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
+        const uint32_t q0 = smem_u32(sQ), r0 = smem_u32(ring);
+        bool ok = true;
+        int it = 0, nq = 0, g = 0;  // ring tiles, Q loads, key tiles done
+        int units = 0;
+        auto stage = [&](int i) { return r0 + (i % C::STAGES) * C::TILE_BYTES; };
+        for (int k = 0; ok; ++k) {
+          const int ui = unit_index(k);
+          if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+          if (ui >= ta.units) continue;
+          const TcUnit u = tc_unit(ta, a.heads, ui, true);
+          const Bounds b = bounds_of(a, u.seq);
+          int t0, t1;
+          range(u, b, t0, t1);
+          if (t0 >= t1) continue;
+          const int n = t1 - t0;
+          // K of tile t is ring tile it + 2 t, V is it + 2 t + 1.
+          if (!mbar_wait(q_full, nq & 1) || !mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1)) {
+            ok = false;
+            break;
+          }
+          ++nq;
+          tc_fence_after();
 #pragma unroll
           for (int h = 0; h < NQ; ++h) {
-            if (t == 0 && units > 0 && !mbar_wait(&o_free[h], (units - 1) & 1)) ok = false;
-            if (ok && !mbar_wait(&p_ready[h], g & 1)) ok = false;
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t d = tmem + h * 256;
-            for (int ks = 0; ks < C::BN / 16; ++ks)
-              umma_bf16_ts(d + C::O_COL, d + C::S_COL + 8 * ks, smem_desc_mn(stage(vi) + ks * 2048, 128 * 128), id_o,
-                           (t > 0 || ks > 0) ? 1u : 0u);
-            umma_commit(&pv_done[h]);
-            if (more) {
-              mma_heads(d + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps, id_s);
-              umma_commit(&s_full[h]);
+            mma_heads(tmem + h * 256 + C::S_COL, q0 + h * C::TILE_BYTES, stage(it), 128, 128, ta.ksteps, id_s);
+            umma_commit(&s_full[h]);
+          }
+          umma_commit(&empty[it % C::STAGES]);
+          if (n == 1) umma_commit(q_free);
+          for (int t = 0; t < n && ok; ++t) {
+            const int vi = it + 2 * t + 1, ki = vi + 1;
+            const bool more = t + 1 < n;
+            if (!mbar_wait(&full[vi % C::STAGES], (vi / C::STAGES) & 1) ||
+                (more && !mbar_wait(&full[ki % C::STAGES], (ki / C::STAGES) & 1))) {
+              ok = false;
+              break;
             }
+#pragma unroll
+            for (int h = 0; h < NQ; ++h) {
+              if (t == 0 && units > 0 && !mbar_wait(&o_free[h], (units - 1) & 1)) ok = false;
+              if (ok && !mbar_wait(&p_ready[h], g & 1)) ok = false;
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t d = tmem + h * 256;
+              for (int ks = 0; ks < C::BN / 16; ++ks)
+                umma_bf16_ts(d + C::O_COL, d + C::S_COL + 8 * ks, smem_desc_mn(stage(vi) + ks * 2048, 128 * 128), id_o,
+                             (t > 0 || ks > 0) ? 1u : 0u);
+              umma_commit(&pv_done[h]);
+              if (more) {
+                mma_heads(d + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps, id_s);
+                umma_commit(&s_full[h]);
+              }
+            }
+            if (!ok) break;
+            umma_commit(&empty[vi % C::STAGES]);
+            if (more) {
+              umma_commit(&empty[ki % C::STAGES]);
+              if (t + 2 == n) umma_commit(q_free);
+            }
+            ++g;
           }
-          if (!ok) break;
-          umma_commit(&empty[vi % C::STAGES]);
-          if (more) {
-            umma_commit(&empty[ki % C::STAGES]);
-            if (t + 2 == n) umma_commit(q_free);
-          }
-          ++g;
+          it += 2 * n;
+          ++units;
         }
-        it += 2 * n;
-        ++units;
+        if (!ok) atomicExch(&g_error_flag, 12);
       }
-      if (!ok) atomicExch(&g_error_flag, 12);
     }
   } else {
+    regs_up<C::REGS_MORE>();
     const int h = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = tmem + h * 256 + ((uint32_t)((warp & 3) * 32) << 16);
     const float c = a.scale * LOG2E;
@@ -512,7 +528,8 @@ struct DqCfg {
   static constexpr int TILE_BYTES = 128 * 128 * NB;
   static constexpr int STAGES = HD == 64 ? 8 : 4;
   static constexpr int SMEM = (2 + STAGES) * TILE_BYTES + 1024 + 512;
-  static constexpr int THREADS = 256 + 64;
+  static constexpr int THREADS = 384;  // two warpgroups of rows, one for TMA and MMA issue
+  static constexpr int REGS_MORE = 208, REGS_LESS = 88;  // 2 x 208 + 88 = 3 x 168
   static constexpr int S_COL = 0, DP_COL = 256, DQ_COL = 384, TMEM = 512;
 };
 
@@ -567,117 +584,121 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
     t1 = (int)((long long)n * (u.split + 1) / a.splits);
   };
 
-  if (warp == 8) {
-    if (lane == 0) {
-      bool ok = true;
-      int it = 0, nq = 0;
-      auto load = [&](const CUtensorMap* m, int row, int head, int seq) {
-        const int s = it % C::STAGES, r = it / C::STAGES;
-        if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) return false;
-        mbar_expect_tx(&full[s], C::TILE_BYTES);
+  if (warp >= 8) {
+    regs_down<C::REGS_LESS>();
+    if (warp == 8) {
+      if (lane == 0) {
+        bool ok = true;
+        int it = 0, nq = 0;
+        auto load = [&](const CUtensorMap* m, int row, int head, int seq) {
+          const int s = it % C::STAGES, r = it / C::STAGES;
+          if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) return false;
+          mbar_expect_tx(&full[s], C::TILE_BYTES);
 #pragma unroll
-        for (int b = 0; b < C::NB; ++b)
-          tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, seq, a.inner);
-        ++it;
-        return true;
-      };
-      for (int k = 0; ok; ++k) {
-        const int ui = unit_index(k);
-        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
-        if (ui >= ta.units) continue;
-        const TcUnit u = tc_unit(ta, a.heads, ui, true);
-        const Bounds b = bounds_of(a, u.seq);
-        int t0, t1;
-        range(u, b, t0, t1);
-        if (t0 >= t1) continue;
-        if (nq > 0 && !mbar_wait(q_free, (nq - 1) & 1)) {
-          ok = false;
-          break;
-        }
-        ++nq;
-        mbar_expect_tx(q_full, 2 * C::TILE_BYTES);
-#pragma unroll
-        for (int c = 0; c < C::NB; ++c) {
-          tma_head(sQ + c * 128 * 128, &mq, q_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
-          tma_head(sO + c * 128 * 128, &mdo, q_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
-        }
-        const int hk = u.h / a.group;
-        for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u.seq) && load(&mv, t * C::BN, hk, u.seq);
-      }
-      if (!ok) atomicExch(&g_error_flag, 21);
-    }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
-      const uint32_t q0 = smem_u32(sQ), o0 = smem_u32(sO), r0 = smem_u32(ring);
-      bool ok = true;
-      int it = 0, nq = 0, g = 0, units = 0;
-      auto stage = [&](int i) { return r0 + (i % C::STAGES) * C::TILE_BYTES; };
-      auto wait_full = [&](int i) { return mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1); };
-      for (int k = 0; ok; ++k) {
-        const int ui = unit_index(k);
-        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
-        if (ui >= ta.units) continue;
-        const TcUnit u = tc_unit(ta, a.heads, ui, true);
-        const Bounds b = bounds_of(a, u.seq);
-        int t0, t1;
-        range(u, b, t0, t1);
-        if (t0 >= t1) continue;
-        const int n = t1 - t0;
-        // Tile g (counted over all units): its K is ring tile it + 2 t, its V it + 2 t + 1; S in buffer g & 1.
-        auto issue_s = [&](int t) {
-          if (!wait_full(it + 2 * t)) return false;
-          tc_fence_after();
-          mma_heads(tmem + C::S_COL + ((g + t) & 1) * 128, q0, stage(it + 2 * t), 128, 128, ta.ksteps, id_s);
-          umma_commit(&s_full[(g + t) & 1]);
+          for (int b = 0; b < C::NB; ++b)
+            tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, seq, a.inner);
+          ++it;
           return true;
         };
-        auto issue_dp = [&](int t) {
-          if (!wait_full(it + 2 * t + 1)) return false;
-          // dP of the tile before has been read (every tile signals once).
-          if (g + t > 0 && !mbar_wait(dp_free, (g + t - 1) & 1)) return false;
-          tc_fence_after();
-          mma_heads(tmem + C::DP_COL, o0, stage(it + 2 * t + 1), 128, 128, ta.ksteps, id_s);
-          umma_commit(dp_full);
-          umma_commit(&empty[(it + 2 * t + 1) % C::STAGES]);
-          return true;
-        };
-        if (!mbar_wait(q_full, nq & 1) || !issue_s(0) || !issue_dp(0)) {
-          ok = false;
-          break;
+        for (int k = 0; ok; ++k) {
+          const int ui = unit_index(k);
+          if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+          if (ui >= ta.units) continue;
+          const TcUnit u = tc_unit(ta, a.heads, ui, true);
+          const Bounds b = bounds_of(a, u.seq);
+          int t0, t1;
+          range(u, b, t0, t1);
+          if (t0 >= t1) continue;
+          if (nq > 0 && !mbar_wait(q_free, (nq - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          ++nq;
+          mbar_expect_tx(q_full, 2 * C::TILE_BYTES);
+#pragma unroll
+          for (int c = 0; c < C::NB; ++c) {
+            tma_head(sQ + c * 128 * 128, &mq, q_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+            tma_head(sO + c * 128 * 128, &mdo, q_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+          }
+          const int hk = u.h / a.group;
+          for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u.seq) && load(&mv, t * C::BN, hk, u.seq);
         }
-        ++nq;
-        for (int t = 0; t < n; ++t) {
-          // S of the next tile overwrites dS of tile t - 1, whose product was issued before it.
-          if (t + 1 < n && (!issue_s(t + 1) || !issue_dp(t + 1))) {
-            ok = false;
-            break;
-          }
-          if (t + 1 >= n) umma_commit(q_free);
-          if (t == 0 && units > 0 && !mbar_wait(dq_free, (units - 1) & 1)) {
-            ok = false;
-            break;
-          }
-          if (!mbar_wait(ds_ready, (g + t) & 1)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t ds = tmem + C::S_COL + ((g + t) & 1) * 128;
-          for (int ks = 0; ks < C::BN / 16; ++ks)
-            umma_bf16_ts(tmem + C::DQ_COL, ds + (ks >> 2) * 64 + (ks & 3) * 8,
-                         smem_desc_mn(stage(it + 2 * t) + ks * 2048, 128 * 128), id_o, (t > 0 || ks > 0) ? 1u : 0u);
-          umma_commit(&empty[(it + 2 * t) % C::STAGES]);
-        }
-        if (!ok) break;
-        umma_commit(dq_done);
-        g += n;
-        it += 2 * n;
-        ++units;
+        if (!ok) atomicExch(&g_error_flag, 21);
       }
-      if (!ok) atomicExch(&g_error_flag, 22);
+    } else if (warp == 9) {
+      if (lane == 0) {
+        const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
+        const uint32_t q0 = smem_u32(sQ), o0 = smem_u32(sO), r0 = smem_u32(ring);
+        bool ok = true;
+        int it = 0, nq = 0, g = 0, units = 0;
+        auto stage = [&](int i) { return r0 + (i % C::STAGES) * C::TILE_BYTES; };
+        auto wait_full = [&](int i) { return mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1); };
+        for (int k = 0; ok; ++k) {
+          const int ui = unit_index(k);
+          if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+          if (ui >= ta.units) continue;
+          const TcUnit u = tc_unit(ta, a.heads, ui, true);
+          const Bounds b = bounds_of(a, u.seq);
+          int t0, t1;
+          range(u, b, t0, t1);
+          if (t0 >= t1) continue;
+          const int n = t1 - t0;
+          // Tile g (counted over all units): its K is ring tile it + 2 t, its V it + 2 t + 1; S in buffer g & 1.
+          auto issue_s = [&](int t) {
+            if (!wait_full(it + 2 * t)) return false;
+            tc_fence_after();
+            mma_heads(tmem + C::S_COL + ((g + t) & 1) * 128, q0, stage(it + 2 * t), 128, 128, ta.ksteps, id_s);
+            umma_commit(&s_full[(g + t) & 1]);
+            return true;
+          };
+          auto issue_dp = [&](int t) {
+            if (!wait_full(it + 2 * t + 1)) return false;
+            // dP of the tile before has been read (every tile signals once).
+            if (g + t > 0 && !mbar_wait(dp_free, (g + t - 1) & 1)) return false;
+            tc_fence_after();
+            mma_heads(tmem + C::DP_COL, o0, stage(it + 2 * t + 1), 128, 128, ta.ksteps, id_s);
+            umma_commit(dp_full);
+            umma_commit(&empty[(it + 2 * t + 1) % C::STAGES]);
+            return true;
+          };
+          if (!mbar_wait(q_full, nq & 1) || !issue_s(0) || !issue_dp(0)) {
+            ok = false;
+            break;
+          }
+          ++nq;
+          for (int t = 0; t < n; ++t) {
+            // S of the next tile overwrites dS of tile t - 1, whose product was issued before it.
+            if (t + 1 < n && (!issue_s(t + 1) || !issue_dp(t + 1))) {
+              ok = false;
+              break;
+            }
+            if (t + 1 >= n) umma_commit(q_free);
+            if (t == 0 && units > 0 && !mbar_wait(dq_free, (units - 1) & 1)) {
+              ok = false;
+              break;
+            }
+            if (!mbar_wait(ds_ready, (g + t) & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t ds = tmem + C::S_COL + ((g + t) & 1) * 128;
+            for (int ks = 0; ks < C::BN / 16; ++ks)
+              umma_bf16_ts(tmem + C::DQ_COL, ds + (ks >> 2) * 64 + (ks & 3) * 8,
+                           smem_desc_mn(stage(it + 2 * t) + ks * 2048, 128 * 128), id_o, (t > 0 || ks > 0) ? 1u : 0u);
+            umma_commit(&empty[(it + 2 * t) % C::STAGES]);
+          }
+          if (!ok) break;
+          umma_commit(dq_done);
+          g += n;
+          it += 2 * n;
+          ++units;
+        }
+        if (!ok) atomicExch(&g_error_flag, 22);
+      }
     }
   } else {
+    regs_up<C::REGS_MORE>();
     const int half = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c = a.scale * LOG2E;
@@ -838,7 +859,8 @@ struct DkvCfg {
   static constexpr int STAGES = 4;                  // (Q, dO) pairs
   static constexpr int STATS = 4;                   // (lse, D) rows
   static constexpr int SMEM = 2 * KV_BYTES + 2 * STAGES * TILE_BYTES + STATS * BN * 8 + 1024 + 512;
-  static constexpr int THREADS = 256 + 96;
+  static constexpr int THREADS = 384;  // two warpgroups of keys, one for TMA, MMA issue and lse / D
+  static constexpr int REGS_MORE = 208, REGS_LESS = 88;  // 2 x 208 + 88 = 3 x 168
   static constexpr int HALF = BN / 2;
   static constexpr int S_COL = 0, DP_COL = 2 * BN, DV_COL = 3 * BN, DK_COL = 3 * BN + HD, TMEM = 512;
   static_assert(3 * BN + 2 * HD <= 512, "TMEM columns");
@@ -913,69 +935,118 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
     t1 = (int)((long long)total * (u.split + 1) / a.splits);
   };
 
-  if (warp == 8) {
-    if (lane == 0) {
-      bool ok = true;
-      int it = 0, nkv = 0;
-      for (int k = 0; ok; ++k) {
-        const int ui = unit_index(k);
-        if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
-        if (ui >= ta.units) continue;
-        const TcUnit u = tc_unit(ta, a.kv_heads, ui, false);
-        const Bounds b = bounds_of(a, u.seq);
-        int begin, per, t0, t1;
-        range(u, b, begin, per, t0, t1);
-        if (t0 >= t1) continue;
-        if (nkv > 0 && !mbar_wait(kv_free, (nkv - 1) & 1)) {
-          ok = false;
-          break;
-        }
-        ++nkv;
-        mbar_expect_tx(kv_full, 2 * C::KV_BYTES);
-#pragma unroll
-        for (int c = 0; c < C::NB; ++c) {
-          tma_head(sK + c * 128 * 128, &mk, kv_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
-          tma_head(sV + c * 128 * 128, &mv, kv_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
-        }
-        for (int t = t0; t < t1; ++t, ++it) {
-          const int h = u.h * a.group + t / per, i0 = (begin + t % per) * C::BN;
-          const int s = it % C::STAGES, r = it / C::STAGES;
-          if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) {
+  if (warp >= 8) {
+    regs_down<C::REGS_LESS>();
+    if (warp == 8) {
+      if (lane == 0) {
+        bool ok = true;
+        int it = 0, nkv = 0;
+        for (int k = 0; ok; ++k) {
+          const int ui = unit_index(k);
+          if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+          if (ui >= ta.units) continue;
+          const TcUnit u = tc_unit(ta, a.kv_heads, ui, false);
+          const Bounds b = bounds_of(a, u.seq);
+          int begin, per, t0, t1;
+          range(u, b, begin, per, t0, t1);
+          if (t0 >= t1) continue;
+          if (nkv > 0 && !mbar_wait(kv_free, (nkv - 1) & 1)) {
             ok = false;
             break;
           }
-          mbar_expect_tx(&full[s], 2 * C::TILE_BYTES);
-          uint8_t* d = ring + 2 * s * C::TILE_BYTES;
+          ++nkv;
+          mbar_expect_tx(kv_full, 2 * C::KV_BYTES);
 #pragma unroll
           for (int c = 0; c < C::NB; ++c) {
-            tma_head(d + c * C::BN * 128, &mq, &full[s], 64 * c, i0, h, u.seq, a.inner);
-            tma_head(d + C::TILE_BYTES + c * C::BN * 128, &mdo, &full[s], 64 * c, i0, h, u.seq, a.inner);
+            tma_head(sK + c * 128 * 128, &mk, kv_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+            tma_head(sV + c * 128 * 128, &mv, kv_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+          }
+          for (int t = t0; t < t1; ++t, ++it) {
+            const int h = u.h * a.group + t / per, i0 = (begin + t % per) * C::BN;
+            const int s = it % C::STAGES, r = it / C::STAGES;
+            if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) {
+              ok = false;
+              break;
+            }
+            mbar_expect_tx(&full[s], 2 * C::TILE_BYTES);
+            uint8_t* d = ring + 2 * s * C::TILE_BYTES;
+#pragma unroll
+            for (int c = 0; c < C::NB; ++c) {
+              tma_head(d + c * C::BN * 128, &mq, &full[s], 64 * c, i0, h, u.seq, a.inner);
+              tma_head(d + C::TILE_BYTES + c * C::BN * 128, &mdo, &full[s], 64 * c, i0, h, u.seq, a.inner);
+            }
           }
         }
+        if (!ok) atomicExch(&g_error_flag, 31);
       }
-      if (!ok) atomicExch(&g_error_flag, 31);
-    }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
-      const uint32_t k0 = smem_u32(sK), v0 = smem_u32(sV), r0 = smem_u32(ring);
+    } else if (warp == 9) {
+      if (lane == 0) {
+        const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
+        const uint32_t k0 = smem_u32(sK), v0 = smem_u32(sV), r0 = smem_u32(ring);
+        bool ok = true;
+        int g = 0, units = 0;  // tiles of all units: ring, S buffers and barriers go by g
+        auto q_tile = [&](int i) { return r0 + 2 * (i % C::STAGES) * C::TILE_BYTES; };
+        auto issue_s = [&](int i) {
+          if (!mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1)) return false;
+          tc_fence_after();
+          mma_heads(tmem + C::S_COL + (i & 1) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
+          umma_commit(&s_full[i & 1]);
+          return true;
+        };
+        auto issue_dp = [&](int i) {
+          if (i > 0 && !mbar_wait(dp_free, (i - 1) & 1)) return false;
+          tc_fence_after();
+          mma_heads(tmem + C::DP_COL, v0, q_tile(i) + C::TILE_BYTES, 128, C::BN, ta.ksteps, id_s);
+          umma_commit(dp_full);
+          return true;
+        };
+        for (int k = 0; ok; ++k) {
+          const int ui = unit_index(k);
+          if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+          if (ui >= ta.units) continue;
+          const TcUnit u = tc_unit(ta, a.kv_heads, ui, false);
+          const Bounds b = bounds_of(a, u.seq);
+          int begin, per, t0, t1;
+          range(u, b, begin, per, t0, t1);
+          if (t0 >= t1) continue;
+          const int n = t1 - t0;
+          if (!mbar_wait(kv_full, units & 1) || !issue_s(g) || !issue_dp(g)) {
+            ok = false;
+            break;
+          }
+          for (int t = 0; t < n; ++t) {
+            if (t + 1 < n && (!issue_s(g + t + 1) || !issue_dp(g + t + 1))) {
+              ok = false;
+              break;
+            }
+            if (t + 1 == n) umma_commit(kv_free);
+            if ((t == 0 && units > 0 && !mbar_wait(acc_free, (units - 1) & 1)) || !mbar_wait(ps_ready, (g + t) & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t p = tmem + C::S_COL + ((g + t) & 1) * C::BN, q = q_tile(g + t);
+            constexpr int KH = C::HALF / 16;  // K steps per half of the tile's queries
+            for (int ks = 0; ks < 2 * KH; ++ks)
+              umma_bf16_ts(tmem + C::DV_COL, p + (ks / KH) * C::HALF + (ks % KH) * 8,
+                           smem_desc_mn(q + C::TILE_BYTES + ks * 2048, C::BN * 128), id_o,
+                           (t > 0 || ks > 0) ? 1u : 0u);
+            for (int ks = 0; ks < 2 * KH; ++ks)
+              umma_bf16_ts(tmem + C::DK_COL, p + (ks / KH) * C::HALF + C::HALF / 2 + (ks % KH) * 8,
+                           smem_desc_mn(q + ks * 2048, C::BN * 128), id_o, (t > 0 || ks > 0) ? 1u : 0u);
+            umma_commit(&empty[(g + t) % C::STAGES]);
+          }
+          if (!ok) break;
+          umma_commit(acc_done);
+          g += n;
+          ++units;
+        }
+        if (!ok) atomicExch(&g_error_flag, 32);
+      }
+    } else if (warp == 10) {
+      // (lse in log2 units, -D) of each streamed tile; +inf and 0 for rows outside the queries.
       bool ok = true;
-      int g = 0, units = 0;  // tiles of all units: ring, S buffers and barriers go by g
-      auto q_tile = [&](int i) { return r0 + 2 * (i % C::STAGES) * C::TILE_BYTES; };
-      auto issue_s = [&](int i) {
-        if (!mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1)) return false;
-        tc_fence_after();
-        mma_heads(tmem + C::S_COL + (i & 1) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
-        umma_commit(&s_full[i & 1]);
-        return true;
-      };
-      auto issue_dp = [&](int i) {
-        if (i > 0 && !mbar_wait(dp_free, (i - 1) & 1)) return false;
-        tc_fence_after();
-        mma_heads(tmem + C::DP_COL, v0, q_tile(i) + C::TILE_BYTES, 128, C::BN, ta.ksteps, id_s);
-        umma_commit(dp_full);
-        return true;
-      };
+      int g = 0;
       for (int k = 0; ok; ++k) {
         const int ui = unit_index(k);
         if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
@@ -984,81 +1055,36 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         const Bounds b = bounds_of(a, u.seq);
         int begin, per, t0, t1;
         range(u, b, begin, per, t0, t1);
-        if (t0 >= t1) continue;
-        const int n = t1 - t0;
-        if (!mbar_wait(kv_full, units & 1) || !issue_s(g) || !issue_dp(g)) {
-          ok = false;
-          break;
-        }
-        for (int t = 0; t < n; ++t) {
-          if (t + 1 < n && (!issue_s(g + t + 1) || !issue_dp(g + t + 1))) {
+        for (int t = t0; t < t1; ++t, ++g) {
+          const int h = u.h * a.group + t / per, i0 = (begin + t % per) * C::BN;
+          const long long row0 = ((long long)u.seq * a.heads + h) * a.lq + i0;
+          const int sb = g % C::STATS, r = g / C::STATS;
+          float l[C::BN / 32], d[C::BN / 32];
+#pragma unroll
+          for (int e = 0; e < C::BN / 32; ++e) {
+            const int i = 32 * e + lane;
+            const bool in = i0 + i < b.ql;
+            const float x = in ? a.lse[row0 + i] : -INFINITY;
+            l[e] = x == -INFINITY ? INFINITY : x * LOG2E - p_shift<T>();
+            d[e] = in ? -a.dsum[row0 + i] : 0.f;
+          }
+          if (r > 0 && !__all_sync(0xffffffffu, mbar_wait(&st_free[sb], (r - 1) & 1))) {
             ok = false;
             break;
           }
-          if (t + 1 == n) umma_commit(kv_free);
-          if ((t == 0 && units > 0 && !mbar_wait(acc_free, (units - 1) & 1)) || !mbar_wait(ps_ready, (g + t) & 1)) {
-            ok = false;
-            break;
+          float* s = stats + sb * 2 * C::BN;
+#pragma unroll
+          for (int e = 0; e < C::BN / 32; ++e) {
+            s[32 * e + lane] = l[e];
+            s[C::BN + 32 * e + lane] = d[e];
           }
-          tc_fence_after();
-          const uint32_t p = tmem + C::S_COL + ((g + t) & 1) * C::BN, q = q_tile(g + t);
-          constexpr int KH = C::HALF / 16;  // K steps per half of the tile's queries
-          for (int ks = 0; ks < 2 * KH; ++ks)
-            umma_bf16_ts(tmem + C::DV_COL, p + (ks / KH) * C::HALF + (ks % KH) * 8,
-                         smem_desc_mn(q + C::TILE_BYTES + ks * 2048, C::BN * 128), id_o,
-                         (t > 0 || ks > 0) ? 1u : 0u);
-          for (int ks = 0; ks < 2 * KH; ++ks)
-            umma_bf16_ts(tmem + C::DK_COL, p + (ks / KH) * C::HALF + C::HALF / 2 + (ks % KH) * 8,
-                         smem_desc_mn(q + ks * 2048, C::BN * 128), id_o, (t > 0 || ks > 0) ? 1u : 0u);
-          umma_commit(&empty[(g + t) % C::STAGES]);
+          mbar_arrive(&st_full[sb]);
         }
-        if (!ok) break;
-        umma_commit(acc_done);
-        g += n;
-        ++units;
       }
-      if (!ok) atomicExch(&g_error_flag, 32);
+      if (!ok && lane == 0) atomicExch(&g_error_flag, 34);
     }
-  } else if (warp == 10) {
-    // (lse in log2 units, -D) of each streamed tile; +inf and 0 for rows outside the queries.
-    bool ok = true;
-    int g = 0;
-    for (int k = 0; ok; ++k) {
-      const int ui = unit_index(k);
-      if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
-      if (ui >= ta.units) continue;
-      const TcUnit u = tc_unit(ta, a.kv_heads, ui, false);
-      const Bounds b = bounds_of(a, u.seq);
-      int begin, per, t0, t1;
-      range(u, b, begin, per, t0, t1);
-      for (int t = t0; t < t1; ++t, ++g) {
-        const int h = u.h * a.group + t / per, i0 = (begin + t % per) * C::BN;
-        const long long row0 = ((long long)u.seq * a.heads + h) * a.lq + i0;
-        const int sb = g % C::STATS, r = g / C::STATS;
-        float l[C::BN / 32], d[C::BN / 32];
-#pragma unroll
-        for (int e = 0; e < C::BN / 32; ++e) {
-          const int i = 32 * e + lane;
-          const bool in = i0 + i < b.ql;
-          const float x = in ? a.lse[row0 + i] : -INFINITY;
-          l[e] = x == -INFINITY ? INFINITY : x * LOG2E - p_shift<T>();
-          d[e] = in ? -a.dsum[row0 + i] : 0.f;
-        }
-        if (r > 0 && !__all_sync(0xffffffffu, mbar_wait(&st_free[sb], (r - 1) & 1))) {
-          ok = false;
-          break;
-        }
-        float* s = stats + sb * 2 * C::BN;
-#pragma unroll
-        for (int e = 0; e < C::BN / 32; ++e) {
-          s[32 * e + lane] = l[e];
-          s[C::BN + 32 * e + lane] = d[e];
-        }
-        mbar_arrive(&st_full[sb]);
-      }
-    }
-    if (!ok && lane == 0) atomicExch(&g_error_flag, 34);
   } else {
+    regs_up<C::REGS_MORE>();
     const int half = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c = a.scale * LOG2E;

@@ -97,18 +97,19 @@ inline bool rows_aligned(const void* p, const RowMap& m, long long outer, int el
          (outer <= 1 || m.so * elem % bytes == 0);
 }
 
-// Column sums out[c] = sum_p part[p][c] of n_part partial rows, always added in the same order (each of 16 threads
-// takes every 16th row, then the 16 sums in sequence), so the result does not depend on scheduling. The columns are
-// `sums` runs of `cols` values, run i going to out_i.
-constexpr int COLSUM_Y = 16;
+// Column sums out[c] = sum_p part[p][c] of n_part partial rows, always added in the same order (each of 64 threads
+// takes every 64th row, then the 64 sums in sequence), so the result does not depend on scheduling. The columns are
+// `sums` runs of `cols` values, run i going to out_i. Eight columns (one 32-byte sector) per CTA, so that a few hundred
+// columns already occupy many SMs.
+constexpr int COLSUM_X = 8, COLSUM_Y = 64;
 
 template <typename TO>
-__global__ void __launch_bounds__(32 * COLSUM_Y)
+__global__ void __launch_bounds__(COLSUM_X* COLSUM_Y)
     column_sums_kernel(const float* __restrict__ part, int n_part, int cols, int sums, TO* out0, TO* out1) {
-  __shared__ float red[COLSUM_Y][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  __shared__ float red[COLSUM_Y][COLSUM_X];
+  const int tx = threadIdx.x % COLSUM_X, ty = threadIdx.x / COLSUM_X;
   const long long width = (long long)cols * sums;
-  const long long c = blockIdx.x * 32LL + tx;
+  const long long c = blockIdx.x * (long long)COLSUM_X + tx;
   float s = 0.f;
   if (c < width) {
 #pragma unroll 4
@@ -117,8 +118,8 @@ __global__ void __launch_bounds__(32 * COLSUM_Y)
   red[ty][tx] = s;
   __syncthreads();
   if (ty == 0 && c < width) {
-#pragma unroll
-    for (int y = 1; y < COLSUM_Y; ++y) s += red[y][tx];
+    const int n = n_part < COLSUM_Y ? n_part : COLSUM_Y;
+    for (int y = 1; y < n; ++y) s += red[y][tx];
     if (c < cols)
       out0[c] = from_f<TO>(s);
     else
@@ -130,7 +131,7 @@ template <typename TO>
 inline int launch_column_sums(const float* part, int n_part, int cols, int sums, void* out0, void* out1,
                               cudaStream_t st) {
   const long long width = (long long)cols * sums;
-  column_sums_kernel<TO><<<(unsigned)((width + 31) / 32), 32 * COLSUM_Y, 0, st>>>(
+  column_sums_kernel<TO><<<(unsigned)((width + COLSUM_X - 1) / COLSUM_X), COLSUM_X * COLSUM_Y, 0, st>>>(
       part, n_part, cols, sums, static_cast<TO*>(out0), static_cast<TO*>(out1));
   UB_CHECK_LAUNCH();
   return 0;

@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from contextlib import nullcontext
+from functools import lru_cache
 
 import torch
 
@@ -30,9 +30,17 @@ _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch
 MAX_HEAD_DIM = 128
 
 
-def _on(device: torch.device):
-    """Makes ``device`` current for a launch (the binding launches on the current device's stream)."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _launch(t: torch.Tensor, name: str, *args) -> None:
+    """Calls an entry point on the current stream of ``t``'s device."""
+    if torch.cuda.current_device() == t.get_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(t.get_device()):
+            _lib.call(name, *args)
+
+
+def _empty(like: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _check_tensor(name: str, t, like: torch.Tensor | None = None) -> None:
@@ -99,10 +107,24 @@ def _same_split(a: tuple, b: tuple) -> tuple[tuple, tuple]:
     return _same_split(a, _rows(b[0].contiguous()))
 
 
-def _workspace(name: str, *args, device: torch.device) -> tuple[torch.Tensor | None, int]:
+@lru_cache(maxsize=4096)
+def _workspace_bytes(name: str, rows: int, cols: int) -> int:
     n = ctypes.c_longlong(0)
-    _lib.check(name, getattr(_lib.load(), name)(*args, ctypes.byref(n)))
-    return (torch.empty(n.value, device=device, dtype=torch.uint8) if n.value else None), n.value
+    _lib.check(name, getattr(_lib.load(), name)(rows, cols, ctypes.byref(n)))
+    return n.value
+
+
+@lru_cache(maxsize=4096)
+def _attention_workspace_bytes(backward: int, *sizes) -> int:
+    p = _lib.AttnTrainParams(*sizes)
+    n = ctypes.c_longlong(0)
+    _lib.check("unblend_attention_workspace",
+               _lib.load().unblend_attention_workspace(ctypes.byref(p), backward, ctypes.byref(n)))
+    return n.value
+
+
+def _scratch(t: torch.Tensor, nbytes: int) -> torch.Tensor | None:
+    return t.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def _refuse_capture(what: str) -> None:
@@ -136,19 +158,19 @@ def layer_norm_forward(x: torch.Tensor, gamma: torch.Tensor | None = None, beta:
     """
     _check_norm(x, gamma, beta, eps)
     _check_cuda("x", x)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = _empty(x)
     n = x.numel() // x.shape[-1]
-    stats = torch.empty(n, 2, device=x.device, dtype=torch.float32)
+    stats = x.new_empty((n, 2), dtype=torch.float32)
     if n == 0:
         return y, stats
     w = gamma if gamma is not None else beta
-    gamma, beta = (None if t is None else t.contiguous() for t in (gamma, beta))
+    gamma = None if gamma is None else gamma.contiguous()
+    beta = None if beta is None else beta.contiguous()
     xr, outer, inner, so, si = _rows(x)
     dt = _DTYPES[x.dtype]
-    with _on(x.device):
-        _lib.call("unblend_layer_norm_forward", xr.data_ptr(), so, si, y.data_ptr(), stats.data_ptr(),
-                  _lib.ptr(gamma), _lib.ptr(beta), eps, outer, inner, x.shape[-1], dt,
-                  _lib.DTYPE_F32 if w is None else _DTYPES[w.dtype])
+    _launch(x, "unblend_layer_norm_forward", xr.data_ptr(), so, si, y.data_ptr(), stats.data_ptr(),
+            _lib.ptr(gamma), _lib.ptr(beta), eps, outer, inner, x.shape[-1], dt,
+            _lib.DTYPE_F32 if w is None else _DTYPES[w.dtype])
     return y, stats
 
 
@@ -166,24 +188,21 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, 
     if stats.shape != (n, 2) or stats.dtype != torch.float32 or stats.device != x.device:
         raise ValueError("stats must be the second result of layer_norm_forward for this x")
     _check_cuda("x", x)
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    dx = _empty(x)
     wt = torch.float32 if gamma is None else gamma.dtype
     dgamma = dbeta = None
     if weight_grads:
-        dgamma, dbeta = (torch.empty(cols, device=x.device, dtype=wt) for _ in range(2))
+        dgamma, dbeta = x.new_empty(cols, dtype=wt), x.new_empty(cols, dtype=wt)
     if n == 0:
         return (dx, dgamma.zero_(), dbeta.zero_()) if weight_grads else (dx, None, None)
     if gamma is not None:
         gamma = gamma.contiguous()
     stats = stats.contiguous()
     (xr, outer, inner, x_so, x_si), (dyr, _, _, d_so, d_si) = _same_split(_rows(x), _rows(dy))
-    work = None
-    with _on(x.device):
-        if weight_grads:
-            work, _ = _workspace("unblend_layer_norm_grad_workspace", n, cols, device=x.device)
-        _lib.call("unblend_layer_norm_backward", dyr.data_ptr(), d_so, d_si, xr.data_ptr(), x_so, x_si,
-                  stats.data_ptr(), _lib.ptr(gamma), dx.data_ptr(), _lib.ptr(dgamma), _lib.ptr(dbeta),
-                  _lib.ptr(work), outer, inner, cols, _DTYPES[x.dtype], _DTYPES[wt])
+    work = _scratch(x, _workspace_bytes("unblend_layer_norm_grad_workspace", n, cols)) if weight_grads else None
+    _launch(x, "unblend_layer_norm_backward", dyr.data_ptr(), d_so, d_si, xr.data_ptr(), x_so, x_si,
+            stats.data_ptr(), _lib.ptr(gamma), dx.data_ptr(), _lib.ptr(dgamma), _lib.ptr(dbeta),
+            _lib.ptr(work), outer, inner, cols, _DTYPES[x.dtype], _DTYPES[wt])
     return dx, dgamma, dbeta
 
 
@@ -256,7 +275,7 @@ def _check_attention(q, k, v, scale, causal, q_lens, k_lens) -> float:
         raise ValueError(f"{q.shape[-2]} query heads must be a multiple of {k.shape[-2]} key/value heads")
     if not 1 <= q.shape[-1] <= MAX_HEAD_DIM:
         raise ValueError(f"head_dim must be 1 to {MAX_HEAD_DIM}, got {q.shape[-1]}")
-    seqs = math.prod(q.shape[:-3])
+    seqs = _seqs(q)
     _check_lens("q_lens", q_lens, seqs, q)
     _check_lens("k_lens", k_lens, seqs, q)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
@@ -271,17 +290,18 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
 
 def _strides(t: torch.Tensor) -> _lib.HeadStrides:
     s = t.stride()
-    return _lib.HeadStrides(s[0], s[1] if t.dim() == 5 else 0, s[-3], s[-2])
+    return _lib.HeadStrides(s[0], s[1] if len(s) == 5 else 0, s[-3], s[-2])
 
 
-def _attn_params(q, k, scale: float, causal: bool, q_lens, k_lens) -> _lib.AttnTrainParams:
-    p = _lib.AttnTrainParams()
-    p.dtype = _DTYPES[q.dtype]
-    p.outer, p.inner = q.shape[0], q.shape[1] if q.dim() == 5 else 1
-    p.heads, p.kv_heads, p.lq, p.lk, p.hd = q.shape[-2], k.shape[-2], q.shape[-3], k.shape[-3], q.shape[-1]
-    p.causal, p.scale = bool(causal), scale
-    p.q_lens, p.k_lens = _lib.ptr(q_lens), _lib.ptr(k_lens)
-    return p
+def _sizes(q, k, scale: float, causal: bool) -> tuple:
+    """The leading fields of ``AttnTrainParams``."""
+    s, lk, kv_heads = q.shape, k.shape[-3], k.shape[-2]
+    return (_DTYPES[q.dtype], s[0], s[1] if len(s) == 5 else 1, s[-2], kv_heads, s[-3], lk, s[-1], bool(causal),
+            scale)
+
+
+def _seqs(q) -> int:
+    return q.shape[0] if q.dim() == 4 else q.shape[0] * q.shape[1]
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None,
@@ -301,21 +321,22 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     """
     scale = _check_attention(q, k, v, scale, causal, q_lens, k_lens)
     _check_cuda("q", q)
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    seqs = math.prod(q.shape[:-3])
-    lse = torch.empty(seqs, q.shape[-2], q.shape[-3], device=q.device, dtype=torch.float32)
+    out = _empty(q)
+    lse = q.new_empty((_seqs(q), q.shape[-2], q.shape[-3]), dtype=torch.float32)
     if lse.numel() == 0:
         return out, lse
     if k.shape[-3] == 0:
         return out.zero_(), lse.fill_(-math.inf)
     q, k, v = _unit(q), _unit(k), _unit(v)
-    q_lens, k_lens = (None if t is None else t.contiguous() for t in (q_lens, k_lens))
-    p = _attn_params(q, k, scale, causal, q_lens, k_lens)
-    p.q, p.k, p.v, p.out = _strides(q), _strides(k), _strides(v), _strides(out)
-    with _on(q.device):
-        work, n = _workspace("unblend_attention_workspace", ctypes.byref(p), 0, device=q.device)
-        _lib.call("unblend_attention_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                  lse.data_ptr(), _lib.ptr(work), n, ctypes.byref(p))
+    q_lens = None if q_lens is None else q_lens.contiguous()
+    k_lens = None if k_lens is None else k_lens.contiguous()
+    sizes = _sizes(q, k, scale, causal)
+    p = _lib.AttnTrainParams(*sizes, _lib.ptr(q_lens), _lib.ptr(k_lens), _strides(q), _strides(k), _strides(v),
+                             _strides(out))
+    n = _attention_workspace_bytes(0, *sizes)
+    work = _scratch(q, n)
+    _launch(q, "unblend_attention_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            _lib.ptr(work), n, ctypes.byref(p))
     return out, lse
 
 
@@ -333,25 +354,25 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         _check_heads(name, t, q)
         if t.shape != q.shape:
             raise ValueError(f"{name} must have q's shape {tuple(q.shape)}, got {tuple(t.shape)}")
-    seqs = math.prod(q.shape[:-3])
+    seqs = _seqs(q)
     if lse.shape != (seqs, q.shape[-2], q.shape[-3]) or lse.dtype != torch.float32 or lse.device != q.device:
         raise ValueError("lse must be the second result of attention_forward for this q")
     _check_cuda("q", q)
-    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
+    dq, dk, dv = _empty(q), _empty(k), _empty(v)
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    q, k, v, out, dout = (_unit(t) for t in (q, k, v, out, dout))
-    q_lens, k_lens = (None if t is None else t.contiguous() for t in (q_lens, k_lens))
-    p = _attn_params(q, k, scale, causal, q_lens, k_lens)
-    p.q, p.k, p.v, p.out, p.dout = (_strides(t) for t in (q, k, v, out, dout))
-    p.dq, p.dk, p.dv = _strides(dq), _strides(dk), _strides(dv)
+    q, k, v, out, dout = _unit(q), _unit(k), _unit(v), _unit(out), _unit(dout)
+    q_lens = None if q_lens is None else q_lens.contiguous()
+    k_lens = None if k_lens is None else k_lens.contiguous()
+    sizes = _sizes(q, k, scale, causal)
+    p = _lib.AttnTrainParams(*sizes, _lib.ptr(q_lens), _lib.ptr(k_lens),
+                             *(_strides(t) for t in (q, k, v, out, dout, dq, dk, dv)))
     lse = lse.contiguous()
-    with _on(q.device):
-        work, n = _workspace("unblend_attention_workspace", ctypes.byref(p), 1, device=q.device)
-        _lib.call("unblend_attention_backward", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(work), n,
-                  ctypes.byref(p))
+    n = _attention_workspace_bytes(1, *sizes)
+    work = _scratch(q, n)
+    _launch(q, "unblend_attention_backward", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(work), n,
+            ctypes.byref(p))
     return dq, dk, dv
 
 
@@ -417,7 +438,7 @@ def dropout_add_forward(x: torch.Tensor, p: float, rng: torch.Tensor, residual: 
     _check_dropout(x, p, rng, residual, scale)
     _check_cuda("x", x)
     t = x.dtype if residual is None else residual.dtype
-    y = torch.empty(x.shape, device=x.device, dtype=t)
+    y = _empty(x, t)
     if x.numel() == 0:
         return y
     rng = rng.contiguous()
@@ -426,10 +447,9 @@ def dropout_add_forward(x: torch.Tensor, p: float, rng: torch.Tensor, residual: 
     rr = (None, 1, 1, 0, 0)
     if residual is not None:
         xr, rr = _same_split(xr, _rows(residual))
-    with _on(x.device):
-        _lib.call("unblend_dropout_add_forward", xr[0].data_ptr(), xr[3], xr[4], _lib.ptr(rr[0]), rr[3], rr[4],
-                  _lib.ptr(scale), y.data_ptr(), float(p), rng.data_ptr(), xr[1], xr[2], x.shape[-1],
-                  _DTYPES[x.dtype], _DTYPES[t], _lib.DTYPE_F32 if scale is None else _DTYPES[scale.dtype])
+    _launch(x, "unblend_dropout_add_forward", xr[0].data_ptr(), xr[3], xr[4], _lib.ptr(rr[0]), rr[3], rr[4],
+            _lib.ptr(scale), y.data_ptr(), float(p), rng.data_ptr(), xr[1], xr[2], x.shape[-1], _DTYPES[x.dtype],
+            _DTYPES[t], _lib.DTYPE_F32 if scale is None else _DTYPES[scale.dtype])
     return y
 
 
@@ -447,10 +467,8 @@ def dropout_add_backward(dy: torch.Tensor, x: torch.Tensor, p: float, rng: torch
         raise ValueError(f"dy must be float32 or {x.dtype} of shape {tuple(x.shape)}, got {dy.dtype} "
                          f"{tuple(dy.shape)}")
     _check_cuda("x", x)
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    dscale = None
-    if scale is not None and scale_grad:
-        dscale = torch.empty(scale.shape, device=x.device, dtype=scale.dtype)
+    dx = _empty(x)
+    dscale = _empty(scale) if scale is not None and scale_grad else None
     if x.numel() == 0:
         return dx, None if dscale is None else dscale.zero_()
     rng = rng.contiguous()
@@ -460,13 +478,12 @@ def dropout_add_backward(dy: torch.Tensor, x: torch.Tensor, p: float, rng: torch
     if dscale is not None:
         dr, xr = _same_split(dr, _rows(x))
     work = None
-    with _on(x.device):
-        if dscale is not None:
-            work, _ = _workspace("unblend_dropout_add_grad_workspace", dr[1] * dr[2], x.shape[-1], device=x.device)
-        _lib.call("unblend_dropout_add_backward", dr[0].data_ptr(), dr[3], dr[4], _lib.ptr(xr[0]), xr[3], xr[4],
-                  _lib.ptr(scale), dx.data_ptr(), _lib.ptr(dscale), _lib.ptr(work), float(p), rng.data_ptr(), dr[1],
-                  dr[2], x.shape[-1], _DTYPES[x.dtype], _DTYPES[dy.dtype],
-                  _lib.DTYPE_F32 if scale is None else _DTYPES[scale.dtype])
+    if dscale is not None:
+        work = _scratch(x, _workspace_bytes("unblend_dropout_add_grad_workspace", dr[1] * dr[2], x.shape[-1]))
+    _launch(x, "unblend_dropout_add_backward", dr[0].data_ptr(), dr[3], dr[4], _lib.ptr(xr[0]), xr[3], xr[4],
+            _lib.ptr(scale), dx.data_ptr(), _lib.ptr(dscale), _lib.ptr(work), float(p), rng.data_ptr(), dr[1], dr[2],
+            x.shape[-1], _DTYPES[x.dtype], _DTYPES[dy.dtype],
+            _lib.DTYPE_F32 if scale is None else _DTYPES[scale.dtype])
     return dx, dscale
 
 
