@@ -56,7 +56,7 @@ __device__ __forceinline__ Words philox(unsigned long long seed, unsigned long l
 
 // Columns in runs of VEC (a multiple of 4, so a run is whole word blocks): thread (tx, ty) keeps its columns and walks
 // the rows blockIdx.y * TY + ty + k * gridDim.y * TY.
-template <typename T, typename TR, typename TW, int VEC, bool BWD>
+template <typename T, typename TR, typename TW, int VEC, bool BWD, bool SUMS>
 __global__ void __launch_bounds__(256) dropout_add_vec_kernel(const __grid_constant__ DropArgs a) {
   extern __shared__ float red[];  // [TY][TX * VEC] of the backward sums
   const int tx = threadIdx.x, ty = threadIdx.y;
@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(256) dropout_add_vec_kernel(const __grid_const
          row += (long long)gridDim.y * blockDim.y) {
       const long long e = row * a.cols + c;
       float x[VEC], r[VEC], o[VEC];
-      if (!BWD || a.part) load_vec<T, VEC>(static_cast<const T*>(a.x) + row_offset(a.xm, (unsigned)row) + c, x);
-      if (a.r) load_vec<TR, VEC>(static_cast<const TR*>(a.r) + row_offset(a.rm, (unsigned)row) + c, r);
+      if (!BWD || SUMS) load_vec<T, VEC>(static_cast<const T*>(a.x) + row_offset(a.xm, (unsigned)row) + c, x);
+      if (BWD || a.r) load_vec<TR, VEC>(static_cast<const TR*>(a.r) + row_offset(a.rm, (unsigned)row) + c, r);
 #pragma unroll
       for (int b = 0; b < VEC / 4; ++b) {
         const Words w = philox(seed, offset, (unsigned long long)(e >> 2) + b);
@@ -85,10 +85,10 @@ __global__ void __launch_bounds__(256) dropout_add_vec_kernel(const __grid_const
           if constexpr (BWD) {
             const float d = keep ? r[i] * a.inv_keep : 0.f;
             o[i] = s[i] * d;
-            if (a.part) ds[i] += keep ? d * x[i] : 0.f;
+            if (SUMS) ds[i] += keep ? d * x[i] : 0.f;
           } else {
             const float v = keep ? s[i] * (x[i] * a.inv_keep) : 0.f;
-            o[i] = a.r ? r[i] + v : v;
+            o[i] = BWD || a.r ? r[i] + v : v;
           }
         }
       }
@@ -98,8 +98,7 @@ __global__ void __launch_bounds__(256) dropout_add_vec_kernel(const __grid_const
         store_vec<TR, VEC>(static_cast<TR*>(a.out) + e, o);
     }
   }
-  if constexpr (BWD) {
-    if (a.part == nullptr) return;
+  if constexpr (SUMS) {
     const int width = blockDim.x * VEC;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) red[ty * width + tx * VEC + i] = ds[i];
@@ -210,8 +209,11 @@ int launch_types(const DropArgs& a, bool vec, int* parts, cudaStream_t st) {
   constexpr int VEC = sizeof(T) == 2 && !BWD ? 8 : 4;
   if (vec) {
     const Shape s = vec_shape(a.rows, a.cols, VEC);
-    const size_t smem = BWD ? sizeof(float) * s.block.x * s.block.y * VEC : 0;
-    dropout_add_vec_kernel<T, TR, TW, VEC, BWD><<<s.grid, s.block, smem, st>>>(a);
+    if (BWD && a.part)
+      dropout_add_vec_kernel<T, TR, TW, VEC, BWD, BWD>
+          <<<s.grid, s.block, sizeof(float) * s.block.x * s.block.y * VEC, st>>>(a);
+    else
+      dropout_add_vec_kernel<T, TR, TW, VEC, BWD, false><<<s.grid, s.block, 0, st>>>(a);
     *parts = s.grid.y;
   } else {
     const Shape s = any_shape(a.rows, a.cols);

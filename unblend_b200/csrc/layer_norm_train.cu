@@ -6,23 +6,28 @@
 //   dgamma = sum_rows dy * xhat,  dbeta = sum_rows dy
 //
 // Statistics, sums and all arithmetic are fp32; x, y, dy and dx are fp32, bf16 or fp16.
-// Both directions are bound by HBM: one read of each input and one write of each output, a row held in registers
-// between its reductions.
+// Both directions are bound by HBM: one read of each input and one write of each output.
 //
-// Rows of up to 1024 columns are handled by one warp each (no barrier), wider ones up to 8192 by one CTA; wider rows
-// are read again for every reduction. Rows come through shared memory, several in flight per warp (cp.async). The weights' gradients are summed in registers over the rows that a warp (or
-// CTA) walks, joined across the CTA in shared memory, and the CTAs' partial rows added in a fixed order by a second
-// kernel: the result is the same on every run.
+// A row of up to 1024 columns belongs to one warp (no barrier), a wider one up to 8192 to a CTA, 16 values per thread;
+// wider rows are read again for every reduction. Rows come through shared memory by cp.async, several in flight per
+// warp, and the arithmetic goes two values at a time: at HBM's rate an SM has some 180 cycles for a row of 1024 bf16
+// columns, and both latency (one row per warp in flight) and issue slots (scalar arithmetic) had been the bound.
+//
+// Rows that do not start on 16-byte boundaries (odd widths, slices) move by aligned 16-byte chunks as well: a thread
+// takes its values out of its own chunk and its neighbour's. Only the values at the ends of a row, whose chunk reaches
+// outside it, move one by one.
+//
+// The weights' gradients are summed in registers over the rows that a group walks, joined across the CTA in shared
+// memory, and the CTAs' partial rows added in a fixed order by a second kernel: the result is the same on every run.
 #include "train_common.cuh"
 
 namespace {
 
 using namespace ub::train;
 
-constexpr int WARP_COLS = 1024;   // widest row of the warp-per-row kernels
+constexpr int WARP_COLS = 1024;   // widest row of a warp
 constexpr int CTA_COLS = 8192;    // widest row held in a CTA's registers
-constexpr int MAX_PARTS = 2 * ub::kNumSMs;
-constexpr int ONE_CTA_ROWS = 64;  // backward calls of up to so many rows run in one CTA, without partial sums
+constexpr int ONE_CTA_ROWS = 64;  // backward calls of up to so many narrow rows run in one CTA, without partial sums
 
 struct NormArgs {
   const void* x;
@@ -36,29 +41,56 @@ struct NormArgs {
   RowMap xm, dym;
   unsigned rows;
   int cols;
-  int stages;      // rows in flight per warp (or CTA)
-  int slot_bytes;  // one row in shared memory, padded
+  int w_vec;  // the weights' base is aligned for 16-byte loads
   float eps;
 };
 
-// Sum of N values over the threads of one row. CTA rows alternate between two shared arrays: an array is written
-// again only after the barrier of the reduction in between, which every reader of it has passed.
+// Sum of N values over the threads of a row: a warp or the CTA. CTA rows alternate between two shared arrays: an array
+// is written again only after the barrier of the reduction in between, which every reader of it has passed.
 template <bool WARP, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[32 * 2], int& phase) {
+__device__ __forceinline__ void row_sum(float (&v)[N], float* red, int& phase) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = ub::warp_sum(v[i]);
   if constexpr (!WARP) {
-    float* r = red[phase];
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;  // at most 16
+    float* r = red + phase * 16 * N;
     phase ^= 1;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     if (lane == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[warp * N + i] = v[i];
+      for (int i = 0; i < N; ++i) r[(threadIdx.x >> 5) * N + i] = v[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = ub::warp_sum(lane < warps ? r[lane * N + i] : 0.f);
+    for (int i = 0; i < N; ++i) {
+      float s = lane < warps ? r[lane * N + i] : 0.f;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      v[i] = __shfl_sync(0xffffffffu, s, 0);
+    }
   }
+}
+
+// The eight words (a, then b) from byte `shift` on (a multiple of the element size), 16 bytes of them.
+__device__ __forceinline__ uint4 take16(const uint4& a, const uint4& b, int shift) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (shift & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (shift & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  if (shift & 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ uint4 shfl_down1(const uint4& v) {
+  return make_uint4(__shfl_down_sync(0xffffffffu, v.x, 1), __shfl_down_sync(0xffffffffu, v.y, 1),
+                    __shfl_down_sync(0xffffffffu, v.z, 1), __shfl_down_sync(0xffffffffu, v.w, 1));
 }
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
@@ -66,165 +98,341 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
                : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_wait(int pending) {  // all but the newest `pending` (1 to 3) groups are there
-  if (pending >= 3)
-    asm volatile("cp.async.wait_group 3;" ::: "memory");
-  else if (pending == 2)
-    asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+template <int N>
+__device__ __forceinline__ void cp_wait() {  // all but the newest N groups are there
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// The rows of one warp or CTA on their way from global to shared memory, `stages` deep. VEC > 1: every row starts on a
-// 16-byte boundary, and a thread copies exactly the 16-byte chunks that it reads back, so no barrier is needed. VEC
-// == 1: rows start anywhere. The whole 16-byte chunks inside a row are copied as such, the elements before and behind
-// them one by one, and the row keeps its offset to the boundary in shared memory; a barrier lets the others read it.
-template <typename T, int VEC, int NV, bool WARP>
-struct RowRing {
-  uint8_t* base;
-  int t, tpr;
+// A run of VEC consecutive values of a row on its way through shared memory: the aligned chunk that holds the first of
+// them and, for the last lane of a warp, the chunk behind it (other lanes get that from their neighbour). A thread
+// reads what it copied itself, so no barrier is needed. `g` is the number of the run.
+template <typename T, bool ALIGNED>
+struct Run {
+  static constexpr int VEC = 16 / (int)sizeof(T);
 
-  __device__ __forceinline__ uint8_t* slot(const NormArgs& a, int i) const { return base + i * a.slot_bytes; }
+  __device__ __forceinline__ static int shift(const T* row) { return (int)(reinterpret_cast<uintptr_t>(row) & 15); }
 
-  __device__ __forceinline__ void fetch(const NormArgs& a, int i, const T* row) const {
-    uint8_t* s = slot(a, i);
-    if constexpr (VEC > 1) {
+  __device__ __forceinline__ static void chunk(uint4* dst, const T* row, int first, int cols) {
+    if (first >= 0 && first + VEC <= cols) {
+      cp_async16(dst, row + first);
+    } else if (first < cols) {  // reaches outside the row: its values one by one
+      uint4 v = make_uint4(0, 0, 0, 0);
+      T* e = reinterpret_cast<T*>(&v);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (k * tpr + t) * VEC;
-        if (c < a.cols) cp_async16(s + c * sizeof(T), row + c);
-      }
-    } else {
-      constexpr int E = 16 / (int)sizeof(T);
-      const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));  // elements past the boundary
-      const int head = min(a.cols, mis ? E - mis : 0);
-      const int chunks = (a.cols - head) / E;
-      const int tail = head + chunks * E;
-      T* d = reinterpret_cast<T*>(s) + mis;
-      for (int k = t; k < chunks; k += tpr) cp_async16(d + head + k * E, row + head + k * E);
-      if (t < head) d[t] = row[t];
-      if (t < a.cols - tail) d[tail + t] = row[tail + t];
+      for (int i = 0; i < VEC; ++i)
+        if (first + i >= 0 && first + i < cols) e[i] = row[first + i];
+      *dst = v;
     }
   }
 
-  // Column values k of this thread: columns (k * tpr + t) * VEC ...
-  __device__ __forceinline__ void read(const NormArgs& a, int i, int mis, int k, float (&v)[VEC]) const {
-    load_vec<T, VEC>(reinterpret_cast<const T*>(slot(a, i)) + (VEC > 1 ? 0 : mis) + (k * tpr + t) * VEC, v);
+  __device__ __forceinline__ static void fetch(uint4* a, uint4* b, const T* row, int g, int cols) {
+    if constexpr (ALIGNED) {
+      if (g * VEC < cols) cp_async16(a, row + g * VEC);
+    } else {
+      const int first = g * VEC - shift(row) / (int)sizeof(T);
+      chunk(a, row, first, cols);
+      if ((threadIdx.x & 31) == 31 && shift(row)) chunk(b, row, first + VEC, cols);
+    }
+  }
+
+  // All lanes of a warp together. Values past the row are 0.
+  __device__ __forceinline__ static void read(const uint4* a, const uint4* b, int row_shift, int g, int cols,
+                                              float2 (&v)[VEC / 2]) {
+    uint4 w = *a;
+    if constexpr (!ALIGNED) {
+      if (row_shift) {
+        uint4 n = shfl_down1(w);
+        if ((threadIdx.x & 31) == 31) n = *b;
+        w = take16(w, n, row_shift);
+      }
+    }
+    unpack16(w, v, T());
+    const int left = cols - g * VEC;
+    if (left < VEC) {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        if (2 * i >= left) v[i].x = 0.f;
+        if (2 * i + 1 >= left) v[i].y = 0.f;
+      }
+    }
   }
 };
 
-template <bool WARP>
-__device__ __forceinline__ void row_sync() {
-  if constexpr (WARP)
-    __syncwarp();
-  else
-    __syncthreads();
-}
-
-template <typename T>
-__device__ __forceinline__ int misalign(const T* p) {
-  return (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
-}
-
-// A row from shared memory (at its own offset to the 16-byte boundary) to global memory, by whole chunks.
-template <typename T>
-__device__ __forceinline__ void store_row(T* row, const T* s, int cols, int t, int tpr) {
-  constexpr int E = 16 / (int)sizeof(T);
-  const int mis = misalign(row);
-  const int head = min(cols, mis ? E - mis : 0);
-  const int chunks = (cols - head) / E, tail = head + chunks * E;
-  for (int k = t; k < chunks; k += tpr)
-    *reinterpret_cast<uint4*>(row + head + k * E) = *reinterpret_cast<const uint4*>(s + mis + head + k * E);
-  if (t < head) row[t] = s[mis + t];
-  if (t < cols - tail) row[tail + t] = s[mis + tail + t];
-}
-
-template <typename T, typename TW, int VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512)
-    layer_norm_fwd_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float red[2][64];
-  extern __shared__ __align__(16) uint8_t rows_smem[];
-  int phase = 0;
-  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int tpr = WARP ? 32 : blockDim.x;
-  const int groups = WARP ? blockDim.x >> 5 : 1, group = WARP ? threadIdx.x >> 5 : 0;
-  const float inv_c = 1.f / (float)a.cols;
-  const long long step = (long long)gridDim.x * groups, row0 = (long long)blockIdx.x * groups + group;
-  const int slots = a.stages + (VEC > 1 ? 0 : 1);  // one more to gather an unaligned output row
-  const RowRing<T, VEC, NV, WARP> ring{rows_smem + (size_t)group * slots * a.slot_bytes, t, tpr};
-  const T* xb = static_cast<const T*>(a.x);
-  for (int s = 0; s < a.stages - 1; ++s) {
-    const long long row = row0 + s * step;
-    if (row < a.rows) ring.fetch(a, s, xb + row_offset(a.xm, (unsigned)row));
-    cp_commit();
+// The rows in flight of a thread: STAGES x RUNS chunks of its own and of its warp's last lane.
+template <int STAGES, int RUNS, bool ALIGNED>
+struct Ring {
+  static constexpr int bytes(int threads) { return STAGES * RUNS * 16 * (threads + (ALIGNED ? 0 : threads / 32)); }
+  uint4* base;
+  __device__ __forceinline__ uint4* a(int stage, int k) const {
+    return base + (stage * RUNS + k) * blockDim.x + threadIdx.x;
   }
-  int cur = 0, next = a.stages - 1;
-  for (long long row = row0; row < a.rows; row += step) {
-    const long long ahead = row + (a.stages - 1) * step;
-    if (ahead < a.rows) ring.fetch(a, next, xb + row_offset(a.xm, (unsigned)ahead));
+  __device__ __forceinline__ uint4* b(int stage, int k) const {
+    return base + STAGES * RUNS * blockDim.x + (stage * RUNS + k) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  }
+};
+
+// Rows in flight: 4, 2 where four of them would leave room for one CTA only.
+template <typename T, int NV, int TENSORS, bool WARP>
+constexpr int stages_of() {
+  return (WARP ? 256 : 512) * NV * TENSORS * 16 * 4 > 112 * 1024 ? 2 : 4;
+}
+
+// Stores VEC values of every lane (runs g of consecutive lanes follow one another) to a row that starts anywhere. The
+// aligned chunk that starts in a lane's values ends in the next lane's.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void store_run(T* row, int g, int cols, const float2 (&o)[8 / sizeof(T)]) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const uint4 w = pack16(o, T());
+  const int c = g * VEC;
+  if constexpr (ALIGNED) {
+    if (c < cols) *reinterpret_cast<uint4*>(row + c) = w;
+  } else {
+    const int lane = threadIdx.x & 31;
+    const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const int h = mis ? VEC - mis : 0;  // values of a run in front of the chunk that starts in it
+    const uint4 n = shfl_down1(w);
+    const bool whole = c + h + VEC <= cols && (lane < 31 || h == 0);
+    if (whole) *reinterpret_cast<uint4*>(row + c + h) = take16(w, n, h * (int)sizeof(T));
+    // Values that no whole chunk takes: in front of a warp's first chunk, behind its last, around the row's end.
+    const bool front = lane == 0 || c + h > cols;
+    if (front || !whole) {
+      const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (c + i < cols && (i < h ? front : !whole)) row[c + i] = e[i];
+    }
+  }
+}
+
+// Weights of run g as fp32 pairs, `none` without weights and past the row.
+template <typename TW, int VEC>
+__device__ __forceinline__ void load_weights(const NormArgs& a, const void* w, float none, int g,
+                                             float2 (&v)[VEC / 2]) {
+  const int c = g * VEC;
+  const TW* p = static_cast<const TW*>(w) + c;
+  if (w && a.w_vec && c + VEC <= a.cols) {
+    load_vec<TW, VEC>(p, reinterpret_cast<float(&)[VEC]>(v));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      v[i].x = w && c + 2 * i < a.cols ? to_f(p[2 * i]) : none;
+      v[i].y = w && c + 2 * i + 1 < a.cols ? to_f(p[2 * i + 1]) : none;
+    }
+  }
+}
+
+template <typename T, typename TW, int NV, bool ALIGNED, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
+    layer_norm_fwd_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr int ST = stages_of<T, NV, 1, WARP>();
+  using R = Run<T, ALIGNED>;
+  __shared__ float red[32];
+  extern __shared__ uint4 dyn[];
+  const Ring<ST, NV, ALIGNED> ring{dyn};
+  int phase = 0;
+  const int tpr = WARP ? 32 : blockDim.x;
+  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int group = WARP ? threadIdx.x >> 5 : 0, groups = WARP ? blockDim.x >> 5 : 1;
+  const float inv_c = 1.f / (float)a.cols;
+  const long long step = (long long)gridDim.x * groups;
+  const T* xb = static_cast<const T*>(a.x);
+  auto fetch = [&](int stage, long long r) {
+    if (r < a.rows) {
+      const T* x = xb + row_offset(a.xm, (unsigned)r);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) R::fetch(ring.a(stage, k), ring.b(stage, k), x, k * tpr + t, a.cols);
+    }
     cp_commit();
-    cp_wait(a.stages - 1);
-    const int mis = misalign(xb + row_offset(a.xm, (unsigned)row));
-    if constexpr (VEC == 1) row_sync<WARP>();
-    float v[NV][VEC];
-    float s[1] = {0.f};
+  };
+  long long row = (long long)blockIdx.x * groups + group;
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) fetch(i, row + i * step);
+  for (int stage = 0; row < a.rows; row += step, stage = (stage + 1) % ST) {
+    fetch((stage + ST - 1) % ST, row + (ST - 1) * step);
+    cp_wait<ST - 1>();
+    const int shift = ALIGNED ? 0 : R::shift(xb + row_offset(a.xm, (unsigned)row));
+    float2 v[NV][VEC / 2], acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (k * tpr + t) * VEC;
-      if (c < a.cols) {
-        ring.read(a, cur, mis, k, v[k]);
-      } else {
+      if (ALIGNED && (k * tpr + t) * VEC >= a.cols) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[k][i] = 0.f;
+        for (int i = 0; i < VEC / 2; ++i) v[k][i] = make_float2(0.f, 0.f);
+      } else {
+        R::read(ring.a(stage, k), ring.b(stage, k), shift, k * tpr + t, ALIGNED ? 1 << 30 : a.cols, v[k]);
       }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s[0] += v[k][i];
+      for (int i = 0; i < VEC / 2; ++i) acc = add2(acc, v[k][i]);
     }
+    float s[1] = {acc.x + acc.y};
     row_sum<WARP, 1>(s, red, phase);
     const float mean = s[0] * inv_c;
-    float q[1] = {0.f};
+    const float2 minus = make_float2(-mean, -mean);
+    acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (k * tpr + t) * VEC;
+      const int left = a.cols - (k * tpr + t) * VEC;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = c < a.cols ? v[k][i] - mean : 0.f;
-        q[0] = fmaf(d, d, q[0]);
-      }
-    }
-    row_sum<WARP, 1>(q, red, phase);
-    const float rstd = 1.f / sqrtf(q[0] * inv_c + a.eps);
-    T* y = static_cast<T*>(a.y) + row * a.cols;
-    T* out = VEC > 1 ? y : reinterpret_cast<T*>(ring.slot(a, a.stages)) + misalign(y);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (k * tpr + t) * VEC;
-      if (c < a.cols) {
-        float g[VEC], b[VEC], o[VEC];
-        if (a.gamma) load_vec<TW, VEC>(static_cast<const TW*>(a.gamma) + c, g);
-        if (a.beta) load_vec<TW, VEC>(static_cast<const TW*>(a.beta) + c, b);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float xhat = (v[k][i] - mean) * rstd;
-          o[i] = fmaf(xhat, a.gamma ? g[i] : 1.f, a.beta ? b[i] : 0.f);
+      for (int i = 0; i < VEC / 2; ++i) {
+        v[k][i] = add2(v[k][i], minus);
+        if (left < VEC) {
+          if (2 * i >= left) v[k][i].x = 0.f;
+          if (2 * i + 1 >= left) v[k][i].y = 0.f;
         }
-        store_vec<T, VEC>(out + c, o);
+        acc = ub::fma2(v[k][i], v[k][i], acc);
       }
     }
-    if constexpr (VEC == 1) {
-      row_sync<WARP>();
-      store_row(y, reinterpret_cast<const T*>(ring.slot(a, a.stages)), a.cols, t, tpr);
+    s[0] = acc.x + acc.y;
+    row_sum<WARP, 1>(s, red, phase);
+    const float rstd = 1.f / sqrtf(s[0] * inv_c + a.eps);
+    const float2 r2 = make_float2(rstd, rstd);
+    T* y = static_cast<T*>(a.y) + row * a.cols;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float2 g[VEC / 2], b[VEC / 2];
+      load_weights<TW, VEC>(a, a.gamma, 1.f, k * tpr + t, g);
+      load_weights<TW, VEC>(a, a.beta, 0.f, k * tpr + t, b);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) b[i] = ub::fma2(mul2(v[k][i], r2), g[i], b[i]);
+      store_run<T, ALIGNED>(y, k * tpr + t, a.cols, b);
     }
     if (t == 0) reinterpret_cast<float2*>(a.stats)[row] = make_float2(mean, rstd);
-    cur = cur + 1 == a.stages ? 0 : cur + 1;
-    next = next + 1 == a.stages ? 0 : next + 1;
+  }
+}
+
+// The sums of the weights' gradients take the registers; a row's x and dy are read again for its second pass.
+template <typename T, typename TW, int NV, bool ALIGNED, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
+    layer_norm_bwd_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr int ST = stages_of<T, NV, 2, WARP>();
+  using R = Run<T, ALIGNED>;
+  __shared__ float red[64];
+  extern __shared__ uint4 dyn[];
+  const Ring<ST, 2 * NV, ALIGNED> ring{dyn};
+  float* sums = reinterpret_cast<float*>(dyn);  // after the rows: [warps][cols]
+  int phase = 0;
+  const int tpr = WARP ? 32 : blockDim.x;
+  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int group = WARP ? threadIdx.x >> 5 : 0, groups = WARP ? blockDim.x >> 5 : 1;
+  const float inv_c = 1.f / (float)a.cols;
+  const long long step = (long long)gridDim.x * groups;
+  const T *xb = static_cast<const T*>(a.x), *dyb = static_cast<const T*>(a.dy);
+  const float2* stats = reinterpret_cast<const float2*>(a.stats);
+  float2 dg[NV][VEC / 2], db[NV][VEC / 2];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) dg[k][i] = db[k][i] = make_float2(0.f, 0.f);
+  auto fetch = [&](int stage, long long r) {
+    if (r < a.rows) {
+      const T* x = xb + row_offset(a.xm, (unsigned)r);
+      const T* dy = dyb + row_offset(a.dym, (unsigned)r);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        R::fetch(ring.a(stage, k), ring.b(stage, k), x, k * tpr + t, a.cols);
+        R::fetch(ring.a(stage, NV + k), ring.b(stage, NV + k), dy, k * tpr + t, a.cols);
+      }
+    }
+    cp_commit();
+  };
+  long long row = (long long)blockIdx.x * groups + group;
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) fetch(i, row + i * step);
+  float2 st_ahead = row < a.rows ? stats[row] : make_float2(0.f, 0.f);
+  for (int stage = 0; row < a.rows; row += step, stage = (stage + 1) % ST) {
+    fetch((stage + ST - 1) % ST, row + (ST - 1) * step);
+    const float2 st = st_ahead;
+    if (row + step < a.rows) st_ahead = stats[row + step];
+    cp_wait<ST - 1>();
+    int sx = 0, sd = 0;
+    if constexpr (!ALIGNED) {
+      sx = R::shift(xb + row_offset(a.xm, (unsigned)row));
+      sd = R::shift(dyb + row_offset(a.dym, (unsigned)row));
+    }
+    const float2 r2 = make_float2(st.y, st.y), shift2 = make_float2(-st.x, -st.x);
+    float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+    // xhat and gy = dy * gamma of run k; dy is 0 past the row.
+    auto values = [&](int k, float2 (&xh)[VEC / 2], float2 (&d)[VEC / 2], float2 (&gy)[VEC / 2]) {
+      const int g = k * tpr + t, cols = ALIGNED ? 1 << 30 : a.cols;
+      R::read(ring.a(stage, k), ring.b(stage, k), sx, g, cols, xh);
+      R::read(ring.a(stage, NV + k), ring.b(stage, NV + k), sd, g, cols, d);
+      float2 gm[VEC / 2];
+      load_weights<TW, VEC>(a, a.gamma, 1.f, g, gm);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        xh[i] = mul2(add2(xh[i], shift2), r2);
+        gy[i] = mul2(d[i], gm[i]);
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (ALIGNED && (k * tpr + t) * VEC >= a.cols) break;
+      float2 xh[VEC / 2], d[VEC / 2], gy[VEC / 2];
+      values(k, xh, d, gy);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        dg[k][i] = ub::fma2(d[i], xh[i], dg[k][i]);
+        db[k][i] = add2(db[k][i], d[i]);
+        s0 = add2(s0, gy[i]);
+        s1 = ub::fma2(gy[i], xh[i], s1);
+      }
+    }
+    float s[2] = {s0.x + s0.y, s1.x + s1.y};
+    row_sum<WARP, 2>(s, red, phase);
+    // dx = rstd gy - rstd m0 - xhat rstd m1
+    const float m0 = -st.y * (s[0] * inv_c), m1 = -st.y * (s[1] * inv_c);
+    const float2 c0 = make_float2(m0, m0), c1 = make_float2(m1, m1);
+    T* dx = static_cast<T*>(a.y) + row * a.cols;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (ALIGNED && (k * tpr + t) * VEC >= a.cols) break;
+      float2 xh[VEC / 2], d[VEC / 2], gy[VEC / 2];
+      values(k, xh, d, gy);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) gy[i] = ub::fma2(xh[i], c1, ub::fma2(gy[i], r2, c0));
+      store_run<T, ALIGNED>(dx, k * tpr + t, a.cols, gy);
+    }
+  }
+  if (a.dgamma == nullptr) return;
+  // Warps leave their sums behind one another in shared memory; the threads add them by column, in warp order.
+  cp_wait<0>();
+  for (int which = 0; which < 2; ++which) {
+    auto put = [&](int c, float v) {
+      if (a.part)
+        a.part[((long long)blockIdx.x * 2 + which) * a.cols + c] = v;
+      else
+        static_cast<TW*>(which ? a.dbeta : a.dgamma)[c] = from_f<TW>(v);
+    };
+    if (WARP) __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int c = (k * tpr + t) * VEC + i;
+        const float2 p = which ? db[k][i / 2] : dg[k][i / 2];
+        const float v = i & 1 ? p.y : p.x;
+        if (c < a.cols) {
+          if (WARP)
+            sums[group * a.cols + c] = v;
+          else
+            put(c, v);
+        }
+      }
+    if (!WARP) continue;
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+      float v = 0.f;
+      for (int w = 0; w < groups; ++w) v += sums[w * a.cols + c];
+      put(c, v);
+    }
   }
 }
 
 // Rows wider than the registers of a CTA: three passes over the row (the second and third hit L2).
 template <typename T, typename TW>
-__global__ void __launch_bounds__(1024) layer_norm_fwd_wide_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float red[2][64];
+__global__ void __launch_bounds__(512) layer_norm_fwd_wide_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float red[64];
   int phase = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row_offset(a.xm, (unsigned)row);
@@ -248,151 +456,10 @@ __global__ void __launch_bounds__(1024) layer_norm_fwd_wide_kernel(const __grid_
   }
 }
 
-// A row's x and dy stay in shared memory between its two passes (sums, then dx), so that registers hold the sums of
-// the weights' gradients and two CTAs fit an SM.
-template <typename T, typename TW, int VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
-    layer_norm_bwd_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float red[2][64];
-  extern __shared__ __align__(16) uint8_t rows_smem[];
-  int phase = 0;
-  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int tpr = WARP ? 32 : blockDim.x;
-  const int groups = WARP ? blockDim.x >> 5 : 1, group = WARP ? threadIdx.x >> 5 : 0;
-  const float inv_c = 1.f / (float)a.cols;
-  const long long step = (long long)gridDim.x * groups, row0 = (long long)blockIdx.x * groups + group;
-  const int slots = 2 * a.stages + (VEC > 1 ? 0 : 1);
-  const RowRing<T, VEC, NV, WARP> ring{rows_smem + (size_t)group * slots * a.slot_bytes, t, tpr};
-  const T *xb = static_cast<const T*>(a.x), *db_ = static_cast<const T*>(a.dy);
-  float dg[NV][VEC], db[NV][VEC];
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) dg[k][i] = db[k][i] = 0.f;
-  for (int s = 0; s < a.stages - 1; ++s) {
-    const long long row = row0 + s * step;
-    if (row < a.rows) {
-      ring.fetch(a, 2 * s, xb + row_offset(a.xm, (unsigned)row));
-      ring.fetch(a, 2 * s + 1, db_ + row_offset(a.dym, (unsigned)row));
-    }
-    cp_commit();
-  }
-  int cur = 0, next = a.stages - 1;
-  float2 st_next = row0 < a.rows ? reinterpret_cast<const float2*>(a.stats)[row0] : make_float2(0.f, 0.f);
-  for (long long row = row0; row < a.rows; row += step) {
-    const long long ahead = row + (a.stages - 1) * step;
-    const float2 st = st_next;
-    if (row + step < a.rows) st_next = reinterpret_cast<const float2*>(a.stats)[row + step];
-    if (ahead < a.rows) {
-      ring.fetch(a, 2 * next, xb + row_offset(a.xm, (unsigned)ahead));
-      ring.fetch(a, 2 * next + 1, db_ + row_offset(a.dym, (unsigned)ahead));
-    }
-    cp_commit();
-    cp_wait(a.stages - 1);
-    int mx = 0, md = 0;
-    if constexpr (VEC == 1) {
-      mx = misalign(xb + row_offset(a.xm, (unsigned)row));
-      md = misalign(db_ + row_offset(a.dym, (unsigned)row));
-      row_sync<WARP>();
-    }
-    float s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (k * tpr + t) * VEC;
-      if (c < a.cols) {
-        float g[VEC], x[VEC], d[VEC];
-        ring.read(a, 2 * cur, mx, k, x);
-        ring.read(a, 2 * cur + 1, md, k, d);
-        if (a.gamma) load_vec<TW, VEC>(static_cast<const TW*>(a.gamma) + c, g);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float xh = (x[i] - st.x) * st.y;
-          dg[k][i] = fmaf(d[i], xh, dg[k][i]);
-          db[k][i] += d[i];
-          const float gy = a.gamma ? d[i] * g[i] : d[i];
-          s[0] += gy;
-          s[1] = fmaf(gy, xh, s[1]);
-        }
-      }
-    }
-    row_sum<WARP, 2>(s, red, phase);
-    const float m0 = s[0] * inv_c, m1 = s[1] * inv_c;
-    T* dx = static_cast<T*>(a.y) + row * a.cols;
-    T* out = VEC > 1 ? dx : reinterpret_cast<T*>(ring.slot(a, 2 * a.stages)) + misalign(dx);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (k * tpr + t) * VEC;
-      if (c < a.cols) {
-        float g[VEC], x[VEC], d[VEC], o[VEC];
-        ring.read(a, 2 * cur, mx, k, x);
-        ring.read(a, 2 * cur + 1, md, k, d);
-        if (a.gamma) load_vec<TW, VEC>(static_cast<const TW*>(a.gamma) + c, g);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float gy = a.gamma ? d[i] * g[i] : d[i];
-          o[i] = st.y * (gy - m0 - (x[i] - st.x) * st.y * m1);
-        }
-        store_vec<T, VEC>(out + c, o);
-      }
-    }
-    if constexpr (VEC == 1) {
-      row_sync<WARP>();
-      store_row(dx, reinterpret_cast<const T*>(ring.slot(a, 2 * a.stages)), a.cols, t, tpr);
-    }
-    cur = cur + 1 == a.stages ? 0 : cur + 1;
-    next = next + 1 == a.stages ? 0 : next + 1;
-  }
-  if (a.dgamma == nullptr) return;
-  auto put = [&](int c, float g, float b) {
-    if (a.part) {
-      float* part = a.part + (long long)blockIdx.x * 2 * a.cols;
-      part[c] = g;
-      part[a.cols + c] = b;
-    } else {
-      static_cast<TW*>(a.dgamma)[c] = from_f<TW>(g);
-      static_cast<TW*>(a.dbeta)[c] = from_f<TW>(b);
-    }
-  };
-  if constexpr (WARP) {
-    // Warps leave their sums behind one another in shared memory; the threads add them by column, in warp order.
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    float* sums = reinterpret_cast<float*>(rows_smem);  // [groups][cols]
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (k * 32 + t) * VEC;
-        if (c < a.cols) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) sums[group * a.cols + c + i] = which ? db[k][i] : dg[k][i];
-        }
-      }
-      __syncthreads();
-      for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
-        float v = 0.f;
-        for (int w = 0; w < groups; ++w) v += sums[w * a.cols + c];
-        if (a.part)
-          a.part[((long long)blockIdx.x * 2 + which) * a.cols + c] = v;
-        else
-          static_cast<TW*>(which ? a.dbeta : a.dgamma)[c] = from_f<TW>(v);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (k * tpr + t) * VEC;
-      if (c < a.cols) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) put(c + i, dg[k][i], db[k][i]);
-      }
-    }
-  }
-}
-
 // Input gradient of rows wider than the registers of a CTA: two passes over the row.
 template <typename T, typename TW>
-__global__ void __launch_bounds__(1024) layer_norm_dx_wide_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float red[2][64];
+__global__ void __launch_bounds__(512) layer_norm_dx_wide_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float red[64];
   int phase = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row_offset(a.xm, (unsigned)row);
@@ -433,44 +500,46 @@ __global__ void __launch_bounds__(256) layer_norm_dw_wide_kernel(const __grid_co
 }
 
 // CTAs of the backward kernel, each of which leaves one partial row of the weights' gradients; 1: none are needed.
-int bwd_parts(long long rows, int cols) {
+int bwd_ctas(long long rows, int cols) {
   if (cols <= WARP_COLS && rows <= ONE_CTA_ROWS) return 1;
   const long long units = cols <= WARP_COLS ? (rows + 7) / 8 : rows;
-  return (int)(units < MAX_PARTS ? units : MAX_PARTS);
+  const long long most = 2LL * ub::kNumSMs;
+  return (int)(units < most ? units : most);
 }
 
-template <typename T, typename TW, int VEC, int NV, bool WARP>
-int launch_one(NormArgs a, bool backward, cudaStream_t st) {
-  const int threads = WARP ? 256 : ((a.cols + VEC * NV - 1) / (VEC * NV) + 31) / 32 * 32;
-  const int groups = WARP ? 8 : 1;
-  // Rows in flight: 4, fewer where two CTAs (three of the smaller wide-row ones) would not fit the shared memory.
-  a.slot_bytes = (a.cols * (int)sizeof(T) + 15) / 16 * 16 + (VEC > 1 ? 0 : 16);
-  const int per_stage = (backward ? 2 : 1) * groups * a.slot_bytes;
-  const int extra = VEC > 1 ? 0 : groups * a.slot_bytes;
-  a.stages = 4;
-  while (a.stages > 2 && a.stages * per_stage + extra > 100 * 1024) --a.stages;
-  int smem = a.stages * per_stage + extra;
+// A wide row's sums always take the second kernel.
+bool joins(long long rows, int cols) { return cols > CTA_COLS || bwd_ctas(rows, cols) > 1; }
+
+template <typename T, typename TW, int NV, bool ALIGNED, bool WARP>
+int launch_one(const NormArgs& a, bool backward, cudaStream_t st) {
+  constexpr int PER = NV * 16 / (int)sizeof(T);  // values per thread
+  const int threads = WARP ? 256 : ((a.cols + PER - 1) / PER + 31) / 32 * 32;
   if (backward) {
-    if (WARP && smem < (int)sizeof(float) * groups * a.cols) smem = sizeof(float) * groups * a.cols;
-    auto kern = layer_norm_bwd_kernel<T, TW, VEC, NV, WARP>;
+    auto kern = layer_norm_bwd_kernel<T, TW, NV, ALIGNED, WARP>;
+    int smem = Ring<stages_of<T, NV, 2, WARP>(), 2 * NV, ALIGNED>::bytes(threads);
+    if (WARP && smem < 8 * 4 * a.cols) smem = 8 * 4 * a.cols;
     if (smem > 40 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    kern<<<bwd_parts(a.rows, a.cols), threads, smem, st>>>(a);
+    kern<<<bwd_ctas(a.rows, a.cols), threads, smem, st>>>(a);
   } else {
-    auto kern = layer_norm_fwd_kernel<T, TW, VEC, NV, WARP>;
+    auto kern = layer_norm_fwd_kernel<T, TW, NV, ALIGNED, WARP>;
+    const int smem = Ring<stages_of<T, NV, 1, WARP>(), NV, ALIGNED>::bytes(threads);
     if (smem > 40 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    const long long cap = ub::kNumSMs * (smem > 56 * 1024 ? 2LL : 4LL);
-    kern<<<WARP ? ub::grid_1d(a.rows, 8, cap) : ub::grid_1d(a.rows, 1, cap), threads, smem, st>>>(a);
+    // As many CTAs as run at once: each walks the same number of rows, a partial second wave would cost a whole one.
+    int per_sm = 1;
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
+    kern<<<ub::grid_1d(a.rows, WARP ? 8 : 1, (long long)per_sm * ub::kNumSMs), threads, smem, st>>>(a);
   }
   UB_CHECK_LAUNCH();
   return 0;
 }
 
-template <typename T, typename TW, int VEC>
-int launch_vec(const NormArgs& a, bool backward, cudaStream_t st) {
-  if (a.cols <= 256) return launch_one<T, TW, VEC, 8 / VEC, true>(a, backward, st);
-  if (a.cols <= 512) return launch_one<T, TW, VEC, 16 / VEC, true>(a, backward, st);
-  if (a.cols <= WARP_COLS) return launch_one<T, TW, VEC, 32 / VEC, true>(a, backward, st);
-  return launch_one<T, TW, VEC, 16 / VEC, false>(a, backward, st);
+template <typename T, typename TW, bool ALIGNED>
+int launch_cols(const NormArgs& a, bool backward, cudaStream_t st) {
+  constexpr int N8 = sizeof(T) / 2;  // 16-byte runs of 8 values
+  if (a.cols <= 256) return launch_one<T, TW, N8, ALIGNED, true>(a, backward, st);
+  if (a.cols <= 512) return launch_one<T, TW, 2 * N8, ALIGNED, true>(a, backward, st);
+  if (a.cols <= WARP_COLS) return launch_one<T, TW, 4 * N8, ALIGNED, true>(a, backward, st);
+  return launch_one<T, TW, 2 * N8, ALIGNED, false>(a, backward, st);
 }
 
 template <typename T, typename TW>
@@ -478,21 +547,20 @@ int launch_types(const NormArgs& a, bool vec, bool backward, cudaStream_t st) {
   if (a.cols > CTA_COLS) {
     const unsigned grid = ub::grid_1d(a.rows, 1, 4LL * ub::kNumSMs);
     if (!backward) {
-      layer_norm_fwd_wide_kernel<T, TW><<<grid, 1024, 0, st>>>(a);
+      layer_norm_fwd_wide_kernel<T, TW><<<grid, 512, 0, st>>>(a);
       UB_CHECK_LAUNCH();
       return 0;
     }
-    layer_norm_dx_wide_kernel<T, TW><<<grid, 1024, 0, st>>>(a);
+    layer_norm_dx_wide_kernel<T, TW><<<grid, 512, 0, st>>>(a);
     UB_CHECK_LAUNCH();
     if (a.dgamma) {
-      const dim3 g((a.cols + 255) / 256, bwd_parts(a.rows, a.cols));
+      const dim3 g((a.cols + 255) / 256, bwd_ctas(a.rows, a.cols));
       layer_norm_dw_wide_kernel<T><<<g, 256, 0, st>>>(a);
       UB_CHECK_LAUNCH();
     }
     return 0;
   }
-  if (vec) return launch_vec<T, TW, 16 / (int)sizeof(T)>(a, backward, st);
-  return launch_vec<T, TW, 1>(a, backward, st);
+  return vec ? launch_cols<T, TW, true>(a, backward, st) : launch_cols<T, TW, false>(a, backward, st);
 }
 
 int launch(const NormArgs& a, int dtype, int w_dtype, bool vec, bool backward, cudaStream_t st) {
@@ -504,9 +572,6 @@ int launch(const NormArgs& a, int dtype, int w_dtype, bool vec, bool backward, c
                                 : launch_types<__half, __half>(a, vec, backward, st);
 }
 
-// A wide row's sums always take the second kernel.
-bool joins(long long rows, int cols) { return cols > CTA_COLS || bwd_parts(rows, cols) > 1; }
-
 bool types_ok(int dtype, int w_dtype) {
   return known_type(dtype) && (w_dtype == UNBLEND_F32 || w_dtype == dtype);
 }
@@ -515,7 +580,7 @@ bool types_ok(int dtype, int w_dtype) {
 
 extern "C" int unblend_layer_norm_grad_workspace(long long rows, int cols, long long* bytes) {
   UB_REQUIRE(bytes && rows_ok(1, rows, cols));
-  *bytes = joins(rows, cols) ? (long long)bwd_parts(rows, cols) * 2 * cols * (long long)sizeof(float) : 0;
+  *bytes = joins(rows, cols) ? (long long)bwd_ctas(rows, cols) * 2 * cols * (long long)sizeof(float) : 0;
   return 0;
 }
 
@@ -534,9 +599,8 @@ extern "C" int unblend_layer_norm_forward(const void* x, long long x_so, long lo
   a.rows = (unsigned)(outer * inner);
   a.cols = cols;
   const int es = elem_size(dtype);
-  const bool vec = cols % (16 / es) == 0 && rows_aligned(x, a.xm, outer, es, 16) &&
-                   aligned16(y) && aligned16(gamma) &&
-                   aligned16(beta);
+  const bool vec = cols % (16 / es) == 0 && rows_aligned(x, a.xm, outer, es, 16) && aligned16(y);
+  a.w_vec = aligned16(gamma) && aligned16(beta);
   return launch(a, dtype, w_dtype, vec, false, ub::as_stream(stream));
 }
 
@@ -561,12 +625,12 @@ extern "C" int unblend_layer_norm_backward(const void* dy, long long dy_so, long
   a.cols = cols;
   const int es = elem_size(dtype);
   const bool vec = cols % (16 / es) == 0 && rows_aligned(x, a.xm, outer, es, 16) &&
-                   rows_aligned(dy, a.dym, outer, es, 16) && aligned16(dx) &&
-                   aligned16(gamma);
+                   rows_aligned(dy, a.dym, outer, es, 16) && aligned16(dx);
+  a.w_vec = aligned16(gamma);
   cudaStream_t st = ub::as_stream(stream);
   const int rc = launch(a, dtype, w_dtype, vec, true, st);
   if (rc || !a.part) return rc;
-  const int parts = bwd_parts(a.rows, cols);
+  const int parts = bwd_ctas(a.rows, cols);
   if (w_dtype == UNBLEND_F32) return launch_column_sums<float>(work, parts, cols, 2, dgamma, dbeta, st);
   if (w_dtype == UNBLEND_BF16) return launch_column_sums<__nv_bfloat16>(work, parts, cols, 2, dgamma, dbeta, st);
   return launch_column_sums<__half>(work, parts, cols, 2, dgamma, dbeta, st);

@@ -29,6 +29,61 @@ __device__ __forceinline__ __half from_f<__half>(float v) {
   return __float2half_rn(v);
 }
 
+// Two fp32 sums or products in one instruction, each rounded once.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+// The elements of a 16-byte chunk as fp32 pairs, and back.
+__device__ __forceinline__ void unpack16(const uint4& w, float2 (&v)[2], float) {
+  v[0] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+  v[1] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
+}
+__device__ __forceinline__ void unpack16(const uint4& w, float2 (&v)[4], __nv_bfloat16) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
+}
+__device__ __forceinline__ void unpack16(const uint4& w, float2 (&v)[4], __half) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+}
+__device__ __forceinline__ uint4 pack16(const float2 (&v)[2], float) {
+  return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x),
+                    __float_as_uint(v[1].y));
+}
+__device__ __forceinline__ uint4 pack16(const float2 (&v)[4], __nv_bfloat16) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[i].x, v[i].y);
+    u[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+__device__ __forceinline__ uint4 pack16(const float2 (&v)[4], __half) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 b = __floats2half2_rn(v[i].x, v[i].y);
+    u[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
 // VEC consecutive elements as fp32. VEC * sizeof(T) is the access width (2, 4, 8, 16 or 32 bytes; p is aligned to
 // it, 32 bytes as two 16-byte halves).
 template <typename T, int VEC>
