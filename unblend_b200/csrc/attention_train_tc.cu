@@ -64,6 +64,15 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t addr, uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// One lane of a converged warp. The MMA warps run their loops and waits with all lanes and issue under this predicate:
+// operands that the compiler knows to be uniform go straight to the tensor core's uniform registers, where issuing
+// from a divergent `lane == 0` branch took 200 cycles per MMA, three times its execution.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // Moves a warpgroup's registers per thread; the warpgroups' shares of a CTA add up to what it was launched with.
 template <int N>
 __device__ __forceinline__ void regs_up() {
@@ -79,8 +88,8 @@ __device__ __forceinline__ uint32_t idesc_of(uint32_t fmt, uint32_t n, uint32_t 
   return instr_desc(fmt, n) | (b_mn << 16);
 }
 
-// MN-major operand: rows (K) of 64 elements (MN), 8-row swizzle atoms back to back; the next 64 elements of MN lie
-// `block_bytes` on.
+// Descriptor of an MN-major operand at `addr`: rows (K) of 64 elements (MN), 8-row swizzle atoms back to back; the next
+// 64 elements of MN lie `block_bytes` on. 16 rows further: + 2048 bytes.
 __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, int block_bytes) {
   uint64_t d = 0;
   d |= (uint64_t)((addr >> 4) & 0x3FFF);
@@ -91,12 +100,25 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, int block_bytes)
   return d;
 }
 
-// D = A B^T over the head dim: A [128 x hd] and B [n x hd] as K-major tiles of a_rows / b_rows rows.
+// D = A B^T over the head dim: A [128 x hd] and B [n x hd] as K-major tiles of a_rows / b_rows rows per column block.
+template <int HD>
 __device__ __forceinline__ void mma_heads(uint32_t d, uint32_t a, uint32_t b, int a_rows, int b_rows, int ksteps,
                                           uint32_t idesc) {
-  for (int ks = 0; ks < ksteps; ++ks)
-    umma_bf16(d, smem_desc(a + (ks >> 2) * a_rows * 128 + (ks & 3) * 32, 128),
-              smem_desc(b + (ks >> 2) * b_rows * 128 + (ks & 3) * 32, 128), idesc, ks > 0 ? 1u : 0u);
+  const uint64_t da = smem_desc(a, 128), db = smem_desc(b, 128);
+#pragma unroll
+  for (int ks = 0; ks < HD / 16; ++ks)
+    if (ks < ksteps)
+      umma_bf16(d, da + (ks >> 2) * a_rows * 8 + (ks & 3) * 2, db + (ks >> 2) * b_rows * 8 + (ks & 3) * 2, idesc,
+                ks > 0 ? 1u : 0u);
+}
+
+// D (+)= A B over the rows of B's tile: A in TMEM, 16 rows (8 columns) per step; step ks of A is at col(ks).
+template <int STEPS, typename Col>
+__device__ __forceinline__ void mma_rows(uint32_t d, Col col, uint32_t b, int block_bytes, uint32_t idesc,
+                                         uint32_t accum) {
+  const uint64_t db = smem_desc_mn(b, block_bytes);
+#pragma unroll
+  for (int ks = 0; ks < STEPS; ++ks) umma_bf16_ts(d, col(ks), db + ks * 128, idesc, ks > 0 ? 1u : accum);
 }
 
 // Rows r with r0 + r outside [lo, hi) of a tile become 0 (thread = row; the tile's products over the head dim are
@@ -286,7 +308,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
         if (!ok) atomicExch(&g_error_flag, 11);
       }
     } else if (warp == NQ * 4 + 1) {
-      if (lane == 0) {
+      {
         const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
         const uint32_t q0 = smem_u32(sQ), r0 = smem_u32(ring);
         bool ok = true;
@@ -310,13 +332,16 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
           }
           ++nq;
           tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int h = 0; h < NQ; ++h) {
-            mma_heads(tmem + h * 256 + C::S_COL, q0 + h * C::TILE_BYTES, stage(it), 128, 128, ta.ksteps, id_s);
-            umma_commit(&s_full[h]);
+            for (int h = 0; h < NQ; ++h) {
+              mma_heads<HD>(tmem + h * 256 + C::S_COL, q0 + h * C::TILE_BYTES, stage(it), 128, 128, ta.ksteps, id_s);
+              umma_commit(&s_full[h]);
+            }
+            umma_commit(&empty[it % C::STAGES]);
+            if (n == 1) umma_commit(q_free);
           }
-          umma_commit(&empty[it % C::STAGES]);
-          if (n == 1) umma_commit(q_free);
+          __syncwarp();
           for (int t = 0; t < n && ok; ++t) {
             const int vi = it + 2 * t + 1, ki = vi + 1;
             const bool more = t + 1 < n;
@@ -332,27 +357,29 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
               if (!ok) break;
               tc_fence_after();
               const uint32_t d = tmem + h * 256;
-              for (int ks = 0; ks < C::BN / 16; ++ks)
-                umma_bf16_ts(d + C::O_COL, d + C::S_COL + 8 * ks, smem_desc_mn(stage(vi) + ks * 2048, 128 * 128), id_o,
-                             (t > 0 || ks > 0) ? 1u : 0u);
-              umma_commit(&pv_done[h]);
-              if (more) {
-                mma_heads(d + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps, id_s);
-                umma_commit(&s_full[h]);
+              if (elect_one()) {
+                mma_rows<C::BN / 16>(d + C::O_COL, [&](int ks) { return d + C::S_COL + 8 * ks; }, stage(vi), 128 * 128,
+                                     id_o, t > 0 ? 1u : 0u);
+                umma_commit(&pv_done[h]);
+                if (more) {
+                  mma_heads<HD>(d + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps, id_s);
+                  umma_commit(&s_full[h]);
+                }
+                if (h == NQ - 1) {
+                  umma_commit(&empty[vi % C::STAGES]);
+                  if (more) umma_commit(&empty[ki % C::STAGES]);
+                  if (t + 2 == n) umma_commit(q_free);
+                }
               }
+              __syncwarp();
             }
             if (!ok) break;
-            umma_commit(&empty[vi % C::STAGES]);
-            if (more) {
-              umma_commit(&empty[ki % C::STAGES]);
-              if (t + 2 == n) umma_commit(q_free);
-            }
             ++g;
           }
           it += 2 * n;
           ++units;
         }
-        if (!ok) atomicExch(&g_error_flag, 12);
+        if (!ok && lane == 0) atomicExch(&g_error_flag, 12);
       }
     }
   } else {
@@ -610,7 +637,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
         if (!ok) atomicExch(&g_error_flag, 21);
       }
     } else if (warp == 9) {
-      if (lane == 0) {
+      {
         const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
         const uint32_t q0 = smem_u32(sQ), o0 = smem_u32(sO), r0 = smem_u32(ring);
         bool ok = true;
@@ -631,8 +658,11 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
           auto issue_s = [&](int t) {
             if (!wait_full(it + 2 * t)) return false;
             tc_fence_after();
-            mma_heads(tmem + C::S_COL + ((g + t) & 1) * 128, q0, stage(it + 2 * t), 128, 128, ta.ksteps, id_s);
-            umma_commit(&s_full[(g + t) & 1]);
+            if (elect_one()) {
+              mma_heads<HD>(tmem + C::S_COL + ((g + t) & 1) * 128, q0, stage(it + 2 * t), 128, 128, ta.ksteps, id_s);
+              umma_commit(&s_full[(g + t) & 1]);
+            }
+            __syncwarp();
             return true;
           };
           auto issue_dp = [&](int t) {
@@ -640,9 +670,13 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
             // dP of the tile before has been read (every tile signals once).
             if (g + t > 0 && !mbar_wait(dp_free, (g + t - 1) & 1)) return false;
             tc_fence_after();
-            mma_heads(tmem + C::DP_COL, o0, stage(it + 2 * t + 1), 128, 128, ta.ksteps, id_s);
-            umma_commit(dp_full);
-            umma_commit(&empty[(it + 2 * t + 1) % C::STAGES]);
+            if (elect_one()) {
+              mma_heads<HD>(tmem + C::DP_COL, o0, stage(it + 2 * t + 1), 128, 128, ta.ksteps, id_s);
+              umma_commit(dp_full);
+              umma_commit(&empty[(it + 2 * t + 1) % C::STAGES]);
+              if (t + 1 == n) umma_commit(q_free);
+            }
+            __syncwarp();
             return true;
           };
           if (!mbar_wait(q_full, nq & 1) || !issue_s(0) || !issue_dp(0)) {
@@ -656,7 +690,6 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
               ok = false;
               break;
             }
-            if (t + 1 >= n) umma_commit(q_free);
             if (t == 0 && units > 0 && !mbar_wait(dq_free, (units - 1) & 1)) {
               ok = false;
               break;
@@ -667,18 +700,20 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
             }
             tc_fence_after();
             const uint32_t ds = tmem + C::S_COL + ((g + t) & 1) * 128;
-            for (int ks = 0; ks < C::BN / 16; ++ks)
-              umma_bf16_ts(tmem + C::DQ_COL, ds + (ks >> 2) * 64 + (ks & 3) * 8,
-                           smem_desc_mn(stage(it + 2 * t) + ks * 2048, 128 * 128), id_o, (t > 0 || ks > 0) ? 1u : 0u);
-            umma_commit(&empty[(it + 2 * t) % C::STAGES]);
+            if (elect_one()) {
+              mma_rows<C::BN / 16>(tmem + C::DQ_COL, [&](int ks) { return ds + (ks >> 2) * 64 + (ks & 3) * 8; },
+                                   stage(it + 2 * t), 128 * 128, id_o, t > 0 ? 1u : 0u);
+              umma_commit(&empty[(it + 2 * t) % C::STAGES]);
+              if (t + 1 == n) umma_commit(dq_done);
+            }
+            __syncwarp();
           }
           if (!ok) break;
-          umma_commit(dq_done);
           g += n;
           it += 2 * n;
           ++units;
         }
-        if (!ok) atomicExch(&g_error_flag, 22);
+        if (!ok && lane == 0) atomicExch(&g_error_flag, 22);
       }
     }
   } else {
@@ -964,7 +999,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         if (!ok) atomicExch(&g_error_flag, 31);
       }
     } else if (warp == 9) {
-      if (lane == 0) {
+      {
         const uint32_t id_s = idesc_of(ta.fmt, C::BN, 0), id_o = idesc_of(ta.fmt, ta.n_hd, 1);
         const uint32_t k0 = smem_u32(sK), v0 = smem_u32(sV), r0 = smem_u32(ring);
         bool ok = true;
@@ -973,15 +1008,22 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         auto issue_s = [&](int i) {
           if (!mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1)) return false;
           tc_fence_after();
-          mma_heads(tmem + C::S_COL + (i & 1) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
-          umma_commit(&s_full[i & 1]);
+          if (elect_one()) {
+            mma_heads<HD>(tmem + C::S_COL + (i & 1) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
+            umma_commit(&s_full[i & 1]);
+          }
+          __syncwarp();
           return true;
         };
-        auto issue_dp = [&](int i) {
+        auto issue_dp = [&](int i, bool last) {
           if (i > 0 && !mbar_wait(dp_free, (i - 1) & 1)) return false;
           tc_fence_after();
-          mma_heads(tmem + C::DP_COL, v0, q_tile(i) + C::TILE_BYTES, 128, C::BN, ta.ksteps, id_s);
-          umma_commit(dp_full);
+          if (elect_one()) {
+            mma_heads<HD>(tmem + C::DP_COL, v0, q_tile(i) + C::TILE_BYTES, 128, C::BN, ta.ksteps, id_s);
+            umma_commit(dp_full);
+            if (last) umma_commit(kv_free);
+          }
+          __syncwarp();
           return true;
         };
         for (int k = 0; ok; ++k) {
@@ -994,16 +1036,15 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
           range(u, b, begin, per, t0, t1);
           if (t0 >= t1) continue;
           const int n = t1 - t0;
-          if (!mbar_wait(kv_full, units & 1) || !issue_s(g) || !issue_dp(g)) {
+          if (!mbar_wait(kv_full, units & 1) || !issue_s(g) || !issue_dp(g, n == 1)) {
             ok = false;
             break;
           }
           for (int t = 0; t < n; ++t) {
-            if (t + 1 < n && (!issue_s(g + t + 1) || !issue_dp(g + t + 1))) {
+            if (t + 1 < n && (!issue_s(g + t + 1) || !issue_dp(g + t + 1, t + 2 == n))) {
               ok = false;
               break;
             }
-            if (t + 1 == n) umma_commit(kv_free);
             if ((t == 0 && units > 0 && !mbar_wait(acc_free, (units - 1) & 1)) || !mbar_wait(ps_ready, (g + t) & 1)) {
               ok = false;
               break;
@@ -1011,21 +1052,22 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
             tc_fence_after();
             const uint32_t p = tmem + C::S_COL + ((g + t) & 1) * C::BN, q = q_tile(g + t);
             constexpr int KH = C::HALF / 16;  // K steps per half of the tile's queries
-            for (int ks = 0; ks < 2 * KH; ++ks)
-              umma_bf16_ts(tmem + C::DV_COL, p + (ks / KH) * C::HALF + (ks % KH) * 8,
-                           smem_desc_mn(q + C::TILE_BYTES + ks * 2048, C::BN * 128), id_o,
-                           (t > 0 || ks > 0) ? 1u : 0u);
-            for (int ks = 0; ks < 2 * KH; ++ks)
-              umma_bf16_ts(tmem + C::DK_COL, p + (ks / KH) * C::HALF + C::HALF / 2 + (ks % KH) * 8,
-                           smem_desc_mn(q + ks * 2048, C::BN * 128), id_o, (t > 0 || ks > 0) ? 1u : 0u);
-            umma_commit(&empty[(g + t) % C::STAGES]);
+            if (elect_one()) {
+              mma_rows<2 * KH>(tmem + C::DV_COL, [&](int ks) { return p + (ks / KH) * C::HALF + (ks % KH) * 8; },
+                               q + C::TILE_BYTES, C::BN * 128, id_o, t > 0 ? 1u : 0u);
+              mma_rows<2 * KH>(tmem + C::DK_COL,
+                               [&](int ks) { return p + (ks / KH) * C::HALF + C::HALF / 2 + (ks % KH) * 8; }, q,
+                               C::BN * 128, id_o, t > 0 ? 1u : 0u);
+              umma_commit(&empty[(g + t) % C::STAGES]);
+              if (t + 1 == n) umma_commit(acc_done);
+            }
+            __syncwarp();
           }
           if (!ok) break;
-          umma_commit(acc_done);
           g += n;
           ++units;
         }
-        if (!ok) atomicExch(&g_error_flag, 32);
+        if (!ok && lane == 0) atomicExch(&g_error_flag, 32);
       }
     } else if (warp == 10) {
       // (lse in log2 units, -D) of each streamed tile; +inf and 0 for rows outside the queries.
