@@ -286,7 +286,7 @@ def check(name: str, rc: int) -> None:
 # The joins of split attention calls depend on the sizes and are not counted.
 KERNELS_PER_CALL = {"unblend_mean_std": 3, "unblend_istft_output": 2, "unblend_istft_masked": 2,
                     "unblend_layer_norm_backward": 2, "unblend_dropout_add_backward": 2,
-                    "unblend_attention_backward": 2}
+                    "unblend_attention_backward": 3}
 
 # Launch accounting: total kernels launched through this binding.
 counters = {"launches": 0}

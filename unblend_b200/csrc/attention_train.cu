@@ -440,7 +440,7 @@ Plan plan_of(const UnblendAttnTrainParams& p, bool tc) {
   return n;
 }
 
-// Workspace: forward [parts][q_rows][hd] and [parts][q_rows] lse; backward D [q_rows], then the larger of the two
+// Workspace: forward [parts][q_rows][hd] and [parts][q_rows] lse; backward D or row statistics [q_rows][2], then the larger of the two
 // kernels' parts (they run one after the other). Room for either kind of kernels: which of them runs depends on the
 // pointers too.
 long long workspace_floats(const UnblendAttnTrainParams& p, bool backward) {
@@ -453,7 +453,7 @@ long long workspace_floats(const UnblendAttnTrainParams& p, bool backward) {
     } else {
       const long long dq = n.dq_splits > 1 ? n.dq_splits * n.q_rows * p.hd : 0;
       const long long dkv = n.dkv_splits > 1 ? 2 * n.dkv_splits * n.k_rows * p.hd : 0;
-      need = round4(n.q_rows) + (dq > dkv ? dq : dkv);
+      need = round4(2 * n.q_rows) + (dq > dkv ? dq : dkv);
     }
     most = need > most ? need : most;
   }
@@ -469,7 +469,8 @@ bool params_ok(const UnblendAttnTrainParams* p) {
   if (seqs >= (1LL << 31)) return false;
   // CTAs of each kernel, splits included (at most 32).
   const long long qt = div_up(p->lq, TILE), kt = div_up(p->lk, TILE);
-  return seqs <= (1LL << 31) / p->heads / qt / 32 && seqs <= (1LL << 31) / p->kv_heads / kt / 32;
+  return seqs <= (1LL << 31) / p->heads / qt / 32 && seqs <= (1LL << 31) / p->kv_heads / kt / 32 &&
+         qt * (p->heads / p->kv_heads) < (1LL << 26) && seqs * p->lq <= (1LL << 38) / p->heads;
 }
 
 bool vec4_ok(const void* p, const UnblendHeadStrides& s, const UnblendAttnTrainParams& a) {
@@ -553,7 +554,8 @@ int forward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Plan
 template <typename T>
 int backward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Plan& n, float* parts, bool tc, bool vec,
                    cudaStream_t st) {
-  int rc;
+  int rc = tc ? attention_stats_tc(a, p, st) : 0;
+  if (rc) return rc;
   if (tc)
     rc = attention_dq_tc(a, p, n.dq_splits, parts, st);
   else
@@ -639,7 +641,7 @@ extern "C" int unblend_attention_backward(const void* dout, const void* q, const
   a.dk = dk;
   a.dv = dv;
   a.dsum = static_cast<float*>(work);
-  float* parts = a.dsum + round4(n.q_rows);
+  float* parts = a.dsum + round4(2 * n.q_rows);
   cudaStream_t st = ub::as_stream(stream);
   const bool vec = p->hd % 4 == 0 && vec4_ok(q, p->q, *p) && vec4_ok(k, p->k, *p) && vec4_ok(v, p->v, *p) &&
                    vec4_ok(dout, p->dout, *p);

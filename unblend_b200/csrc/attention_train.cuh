@@ -12,7 +12,7 @@ struct AttnArgs {
   const void* out_in;  // forward output, read by the backward pass
   void *out, *dq, *dk, *dv;
   float* lse;
-  float* dsum;  // [rows] rowsum(dout * out), written by the dq kernel, read by the dk / dv kernel
+  float* dsum;  // [rows] rowsum(dout * out) (CUDA cores), or [rows][2] row statistics (tensor cores)
   UnblendHeadStrides q_s, k_s, v_s, out_s, dout_s, dq_s, dk_s, dv_s;
   const int *q_lens, *k_lens;
   int seqs, inner, heads, kv_heads, group, lq, lk, hd, causal;
@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(256)
 bool attention_tc_fits(const UnblendAttnTrainParams& p, const void* const* ptrs, const UnblendHeadStrides* strides,
                        const int* heads, const int* rows, int n);
 int attention_fwd_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int rows_per_cta, cudaStream_t st);
+int attention_stats_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, cudaStream_t st);
 int attention_dq_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st);
 int attention_dkv_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st);
 

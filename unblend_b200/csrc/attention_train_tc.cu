@@ -131,37 +131,74 @@ __device__ __forceinline__ void clear_row(uint8_t* tile, int rows, int blocks, i
   }
 }
 
+// n / d for n < 2^31 by a multiplication: with 2^s >= d and m = floor(2^(31 + s) / d) + 1, floor(n m / 2^(31 + s)) is
+// exact because n (m d - 2^(31 + s)) < 2^(31 + s). Unit numbers are taken apart between tiles, where a hardware
+// division's hundred cycles are not hidden.
+struct FastDiv {
+  uint32_t d, m, shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> shift); }
+};
+
+FastDiv fast_div(long long d) {
+  FastDiv f;
+  uint32_t s = 0;
+  while ((1LL << s) < d) ++s;
+  f.d = (uint32_t)d;
+  f.shift = 31 + s;
+  f.m = (uint32_t)((1ULL << f.shift) / (uint64_t)d + 1);
+  return f;
+}
+
 struct TcArgs {
   AttnArgs a;
+  const float2* stats;   // backward: (-lse log2 e, -D) of each query row, (-inf, 0) for rows that see nothing
+  FastDiv by_splits, by_tiles, by_heads, by_inner, by_seq_heads;
   int row_tiles, units;  // units of the kernel's rows
   int ksteps, n_hd;      // head dim / 16 rounded up, and * 16
   uint32_t fmt;
 };
 
 struct TcUnit {
-  int seq, h, tile, split;
+  int seq, so, si;  // sequence, and its outer and inner index
+  int h, tile, split;
 };
 
-// Unit number -> work. Causal units are ordered by row tile across all heads, the longest first (`heavy_last`: the
+// Unit number -> work. Causal units are ordered by row tile across all heads, the longest first (`last_is_long`: the
 // last row tile is the longest); others by head, so that CTAs at work together share the streamed operand in L2.
 __device__ __forceinline__ TcUnit tc_unit(const TcArgs& t, int heads, int u, bool last_is_long) {
   TcUnit r;
-  r.split = u % t.a.splits;
-  u /= t.a.splits;
+  int q = t.by_splits(u);
+  r.split = u - q * t.a.splits;
+  u = q;
+  int sh;
   if (t.a.causal) {
-    const int sh = t.a.seqs * heads;
-    const int rank = u / sh;
-    const int rest = u - rank * sh;
+    const int rank = t.by_seq_heads(u);
+    sh = u - rank * (int)t.by_seq_heads.d;
     r.tile = last_is_long ? t.row_tiles - 1 - rank : rank;
-    r.h = rest % heads;
-    r.seq = rest / heads;
   } else {
-    r.tile = u % t.row_tiles;
-    u /= t.row_tiles;
-    r.h = u % heads;
-    r.seq = u / heads;
+    sh = t.by_tiles(u);
+    r.tile = u - sh * t.row_tiles;
   }
+  r.seq = t.by_heads(sh);
+  r.h = sh - r.seq * heads;
+  r.so = t.by_inner(r.seq);
+  r.si = r.seq - r.so * t.a.inner;
   return r;
+}
+
+__device__ __forceinline__ long long unit_offset(const UnblendHeadStrides& s, const TcUnit& u, int h) {
+  return (long long)u.so * s.outer + (long long)u.si * s.inner + (long long)h * s.head;
+}
+
+// The part `split` of n tiles: [t0, t1).
+__device__ __forceinline__ void split_range(const TcArgs& t, int n, int split, int& t0, int& t1) {
+  if (t.a.splits == 1) {
+    t0 = 0;
+    t1 = n;
+  } else {
+    t0 = t.by_splits(n * split);
+    t1 = t.by_splits(n * (split + 1));
+  }
 }
 
 // The k-th unit of this CTA: alternate rounds walk the CTAs in opposite directions, which evens out causal work.
@@ -171,9 +208,8 @@ __device__ __forceinline__ int unit_index(int k) {
 }
 
 __device__ __forceinline__ void tma_head(void* dst, const CUtensorMap* map, uint64_t* bar, int col, int row, int head,
-                                         int seq, int inner) {
-  const int o = seq / inner;
-  tma_load_5d(dst, map, bar, col, row, head, seq - o * inner, o);
+                                         const TcUnit& u) {
+  tma_load_5d(dst, map, bar, col, row, head, u.si, u.so);
 }
 
 // n consecutive values of a row (n a multiple of 8), times mul, to T or fp32.
@@ -215,7 +251,10 @@ struct FwdCfg {
   // Registers: 3 x 168 = 2 x 208 + 88 (NQ = 2, one CTA per SM), 2 x 128 = 200 + 56 (NQ = 1, two).
   static constexpr int REGS_MORE = NQ == 2 ? 208 : 200, REGS_LESS = NQ == 2 ? 88 : 56;
   static constexpr int TMEM = NQ * 256;
-  static constexpr int S_COL = 0, O_COL = 128;         // per query tile, 256 columns apart
+  // Per query tile, 256 columns apart. P has columns of its own where O leaves room: the scores of the next tile are
+  // made as soon as this tile's have been read. At head dims over 64 P overwrites its scores.
+  static constexpr bool APART = HD == 64;
+  static constexpr int S_COL = 0, O_COL = 128, P_COL = APART ? 192 : 0;
 };
 
 template <typename T, int HD, int NQ>
@@ -236,7 +275,8 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
   uint64_t* p_ready = s_full + NQ;         // [NQ]
   uint64_t* pv_done = p_ready + NQ;        // [NQ]
   uint64_t* o_free = pv_done + NQ;         // [NQ]
-  uint32_t* slot = reinterpret_cast<uint32_t*>(o_free + NQ);
+  uint64_t* s_free = o_free + NQ;          // [NQ] APART: the scores have been read
+  uint32_t* slot = reinterpret_cast<uint32_t*>(s_free + NQ);
 
   const AttnArgs& a = ta.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -249,6 +289,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
       mbar_init(&p_ready[h], 4);
       mbar_init(&pv_done[h], 1);
       mbar_init(&o_free[h], 4);
+      mbar_init(&s_free[h], 4);
     }
     fence_mbar_init();
   }
@@ -261,8 +302,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
   // Key tiles of unit u: [t0, t1).
   auto range = [&](const TcUnit& u, const Bounds& b, int& t0, int& t1) {
     const int n = (key_end(a, b, u.tile * NQ * ROWS, NQ * ROWS) + C::BN - 1) / C::BN;
-    t0 = (int)((long long)n * u.split / a.splits);
-    t1 = (int)((long long)n * (u.split + 1) / a.splits);
+    split_range(ta, n, u.split, t0, t1);
   };
 
   if (warp >= NQ * 4) {
@@ -271,13 +311,13 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
       if (lane == 0) {
         bool ok = true;
         int it = 0, nq = 0;  // ring tiles and Q loads so far
-        auto load = [&](const CUtensorMap* m, int row, int head, int seq) {
+        auto load = [&](const CUtensorMap* m, int row, int head, const TcUnit& u) {
           const int s = it % C::STAGES, r = it / C::STAGES;
           if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) return false;
           mbar_expect_tx(&full[s], C::TILE_BYTES);
 #pragma unroll
           for (int b = 0; b < C::NB; ++b)
-            tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, seq, a.inner);
+            tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, u);
           ++it;
           return true;
         };
@@ -300,10 +340,10 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
           for (int h = 0; h < NQ; ++h)
 #pragma unroll
             for (int c = 0; c < C::NB; ++c)
-              tma_head(sQ + h * C::TILE_BYTES + c * 128 * 128, &mq, q_full, 64 * c, (u.tile * NQ + h) * ROWS, u.h, u.seq,
-                       a.inner);
+              tma_head(sQ + h * C::TILE_BYTES + c * 128 * 128, &mq, q_full, 64 * c, (u.tile * NQ + h) * ROWS, u.h,
+                       u);
           const int hk = u.h / a.group;
-          for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u.seq) && load(&mv, t * C::BN, hk, u.seq);
+          for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u) && load(&mv, t * C::BN, hk, u);
         }
         if (!ok) atomicExch(&g_error_flag, 11);
       }
@@ -331,6 +371,12 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
             break;
           }
           ++nq;
+          if (C::APART && g > 0) {
+#pragma unroll
+            for (int h = 0; h < NQ; ++h)
+              if (!mbar_wait(&s_free[h], (g - 1) & 1)) ok = false;
+            if (!ok) break;
+          }
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -350,25 +396,45 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
               ok = false;
               break;
             }
+            if (C::APART && more) {
+#pragma unroll
+              for (int h = 0; h < NQ; ++h) {
+                if (!mbar_wait(&s_free[h], g & 1)) ok = false;
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                  mma_heads<HD>(tmem + h * 256 + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps,
+                                id_s);
+                  umma_commit(&s_full[h]);
+                  if (h == NQ - 1) {
+                    umma_commit(&empty[ki % C::STAGES]);
+                    if (t + 2 == n) umma_commit(q_free);
+                  }
+                }
+                __syncwarp();
+              }
+            }
 #pragma unroll
             for (int h = 0; h < NQ; ++h) {
-              if (t == 0 && units > 0 && !mbar_wait(&o_free[h], (units - 1) & 1)) ok = false;
+              if (ok && t == 0 && units > 0 && !mbar_wait(&o_free[h], (units - 1) & 1)) ok = false;
               if (ok && !mbar_wait(&p_ready[h], g & 1)) ok = false;
               if (!ok) break;
               tc_fence_after();
               const uint32_t d = tmem + h * 256;
               if (elect_one()) {
-                mma_rows<C::BN / 16>(d + C::O_COL, [&](int ks) { return d + C::S_COL + 8 * ks; }, stage(vi), 128 * 128,
+                mma_rows<C::BN / 16>(d + C::O_COL, [&](int ks) { return d + C::P_COL + 8 * ks; }, stage(vi), 128 * 128,
                                      id_o, t > 0 ? 1u : 0u);
                 umma_commit(&pv_done[h]);
-                if (more) {
+                if (!C::APART && more) {
                   mma_heads<HD>(d + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps, id_s);
                   umma_commit(&s_full[h]);
                 }
                 if (h == NQ - 1) {
                   umma_commit(&empty[vi % C::STAGES]);
-                  if (more) umma_commit(&empty[ki % C::STAGES]);
-                  if (t + 2 == n) umma_commit(q_free);
+                  if (!C::APART && more) {
+                    umma_commit(&empty[ki % C::STAGES]);
+                    if (t + 2 == n) umma_commit(q_free);
+                  }
                 }
               }
               __syncwarp();
@@ -413,6 +479,11 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32_async(lanes + C::S_COL + 32 * q, s + 32 * q);
         tmem_wait_ld();
+        if (C::APART) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[h]);
+        }
         if (j0 + C::BN > b.kl || (a.causal && j0 + C::BN - 1 > i0 + b.off)) {
 #pragma unroll
           for (int e = 0; e < 128; ++e)
@@ -449,13 +520,17 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
           sum2 = add2(sum2, p);
           s[e] = pack2<T>(p.x, p.y);
         }
-        if (__any_sync(0xffffffffu, rescale)) {
-          // O holds the sums up to tile t - 1: they are complete once their product has signalled.
+        const bool any = __any_sync(0xffffffffu, rescale);
+        // O holds the sums up to tile t - 1, and that product has read its P, once it has signalled. Where P lies over
+        // the scores, these would not be there before.
+        if ((C::APART && g > 0) || any) {
           if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[h], (g - 1) & 1))) {
             ok = false;
             break;
           }
           tc_fence_after();
+        }
+        if (any) {
 #pragma unroll 1
           for (int q = 0; q < HD / 32; ++q) {
             uint32_t o[32];
@@ -465,8 +540,8 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
             tmem_st32(lanes + C::O_COL + 32 * q, o);
           }
         }
-        tmem_st32(lanes + C::S_COL, *reinterpret_cast<uint32_t(*)[32]>(s));
-        tmem_st32(lanes + C::S_COL + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+        tmem_st32(lanes + C::P_COL, *reinterpret_cast<uint32_t(*)[32]>(s));
+        tmem_st32(lanes + C::P_COL + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -485,7 +560,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
         }
         tc_fence_after();
       }
-      T* out = static_cast<T*>(a.out) + head_offset(a.out_s, a, u.seq, u.h) + (long long)i * a.out_s.row;
+      T* out = static_cast<T*>(a.out) + unit_offset(a.out_s, u, u.h) + (long long)i * a.out_s.row;
       float* part = a.splits > 1 ? a.part + (u.split * rows + orow) * a.hd : nullptr;
 #pragma unroll 1
       for (int q = 0; q < HD / 32; ++q) {
@@ -526,6 +601,39 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
   }
 }
 
+// ---------------------------------------------------------------------------------------- row statistics
+//
+// (-lse log2 e, -D) of each query row, D = rowsum(dO * O); (-inf, 0) for rows that see nothing. LANES lanes per row, 8
+// values each; rows in memory order (heads fastest) for whole lines. A kernel of its own: inside the dq kernel the
+// loads stood in front of every unit's first tile (5000 of 24000 cycles for 11 tiles).
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_constant__ AttnArgs a, float2* stats) {
+  const int lane = threadIdx.x & (LANES - 1);
+  const long long n = (long long)a.seqs * a.lq * a.heads;
+  const long long id = (blockIdx.x * 256LL + threadIdx.x) / LANES;
+  const bool in = id < n;
+  const long long token = in ? id / a.heads : 0;
+  const int h = in ? (int)(id - token * a.heads) : 0;
+  const int seq = (int)(token / a.lq), i = (int)(token - (long long)seq * a.lq);
+  const Bounds b = bounds_of(a, seq);
+  const long long row = ((long long)seq * a.heads + h) * a.lq + i;
+  const float lse = in && i < b.ql ? a.lse[row] : -INFINITY;
+  float D = 0.f;
+  if (lse != -INFINITY && 8 * lane < a.hd) {
+    const uint4 dv = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout) + head_offset(a.dout_s, a, seq, h) +
+                                                     (long long)i * a.dout_s.row + 8 * lane);
+    const uint4 ov = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.out_in) + head_offset(a.out_s, a, seq, h) +
+                                                     (long long)i * a.out_s.row + 8 * lane);
+    const T* x = reinterpret_cast<const T*>(&dv);
+    const T* y = reinterpret_cast<const T*>(&ov);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) D = fmaf(to_f(x[e]), to_f(y[e]), D);
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) D += __shfl_xor_sync(0xffffffffu, D, o);
+  if (in && lane == 0) stats[row] = make_float2(lse == -INFINITY ? lse : -lse * LOG2E, -D);
+}
+
 // --------------------------------------------------------------------------------------------------- dq
 //
 // 128 queries of one head per unit, keys streamed 128 at a time; two threads per row, 64 keys each. S is double
@@ -560,8 +668,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
   uint64_t* empty = full + C::STAGES;
   uint64_t* q_full = empty + C::STAGES;
   uint64_t* q_free = q_full + 1;
-  uint64_t* s_full = q_free + 1;  // [2]
-  uint64_t* dp_full = s_full + 2;
+  uint64_t* dp_full = q_free + 1;  // S of the tile too: its product is issued before
   uint64_t* dp_free = dp_full + 1;
   uint64_t* ds_ready = dp_free + 1;
   uint64_t* dq_done = ds_ready + 1;
@@ -573,9 +680,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     mbar_init(q_full, 1);
-    mbar_init(q_free, 1 + 8);  // the MMA warp's commit and the row warps, which read dO for D
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
+    mbar_init(q_free, 1);
     mbar_init(dp_full, 1);
     mbar_init(dp_free, 8);
     mbar_init(ds_ready, 8);
@@ -591,8 +696,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
 
   auto range = [&](const TcUnit& u, const Bounds& b, int& t0, int& t1) {
     const int n = (key_end(a, b, u.tile * ROWS, ROWS) + C::BN - 1) / C::BN;
-    t0 = (int)((long long)n * u.split / a.splits);
-    t1 = (int)((long long)n * (u.split + 1) / a.splits);
+    split_range(ta, n, u.split, t0, t1);
   };
 
   if (warp >= 8) {
@@ -601,13 +705,13 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
       if (lane == 0) {
         bool ok = true;
         int it = 0, nq = 0;
-        auto load = [&](const CUtensorMap* m, int row, int head, int seq) {
+        auto load = [&](const CUtensorMap* m, int row, int head, const TcUnit& u) {
           const int s = it % C::STAGES, r = it / C::STAGES;
           if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) return false;
           mbar_expect_tx(&full[s], C::TILE_BYTES);
 #pragma unroll
           for (int b = 0; b < C::NB; ++b)
-            tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, seq, a.inner);
+            tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, u);
           ++it;
           return true;
         };
@@ -628,11 +732,11 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
           mbar_expect_tx(q_full, 2 * C::TILE_BYTES);
 #pragma unroll
           for (int c = 0; c < C::NB; ++c) {
-            tma_head(sQ + c * 128 * 128, &mq, q_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
-            tma_head(sO + c * 128 * 128, &mdo, q_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+            tma_head(sQ + c * 128 * 128, &mq, q_full, 64 * c, u.tile * ROWS, u.h, u);
+            tma_head(sO + c * 128 * 128, &mdo, q_full, 64 * c, u.tile * ROWS, u.h, u);
           }
           const int hk = u.h / a.group;
-          for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u.seq) && load(&mv, t * C::BN, hk, u.seq);
+          for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u) && load(&mv, t * C::BN, hk, u);
         }
         if (!ok) atomicExch(&g_error_flag, 21);
       }
@@ -658,10 +762,8 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
           auto issue_s = [&](int t) {
             if (!wait_full(it + 2 * t)) return false;
             tc_fence_after();
-            if (elect_one()) {
+            if (elect_one())
               mma_heads<HD>(tmem + C::S_COL + ((g + t) & 1) * 128, q0, stage(it + 2 * t), 128, 128, ta.ksteps, id_s);
-              umma_commit(&s_full[(g + t) & 1]);
-            }
             __syncwarp();
             return true;
           };
@@ -723,10 +825,22 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
     const float c = a.scale * LOG2E;
     const long long rows = (long long)a.seqs * a.heads * a.lq;
     bool ok = true;
-    int g = 0, it = 0, nq = 0, units = 0;
+    int g = 0, it = 0, units = 0;
+    // Statistics of this thread's row in the k-th unit.
+    auto load_stats = [&](int k) {
+      const int ui = unit_index(k);
+      if (ui >= ta.units) return make_float2(-INFINITY, 0.f);
+      const TcUnit u = tc_unit(ta, a.heads, ui, true);
+      const int i = u.tile * ROWS + row;
+      if (i >= a.lq) return make_float2(-INFINITY, 0.f);
+      return ta.stats[((long long)u.seq * a.heads + u.h) * a.lq + i];
+    };
+    float2 st_next = load_stats(0);
     for (int k = 0; ok; ++k) {
       const int ui = unit_index(k);
       if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
+      const float2 st = st_next;
+      st_next = load_stats(k + 1);
       if (ui >= ta.units) continue;
       const TcUnit u = tc_unit(ta, a.heads, ui, true);
       const Bounds b = bounds_of(a, u.seq);
@@ -735,69 +849,32 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
       const int i0 = u.tile * ROWS, i = i0 + row;
       const int limit = a.causal ? min(b.kl, i + b.off + 1) : b.kl;
       const long long orow = ((long long)u.seq * a.heads + u.h) * a.lq + i;
-      const bool valid = i < b.ql;
-      float lse = valid ? a.lse[orow] : -INFINITY;
-      const bool live = valid && lse != -INFINITY;
-      float D = 0.f;
-      if (t0 < t1) {
-        // D = rowsum(dO * O), by both threads of the row: dO from shared memory (16-byte chunk j of row r lies at
-        // j ^ (r & 7)), O from global memory, fetched while Q and dO arrive.
-        const T* o = static_cast<const T*>(a.out_in) + head_offset(a.out_s, a, u.seq, u.h) + (long long)i * a.out_s.row;
-        uint4 ov[HD / 8];
-#pragma unroll
-        for (int e = 0; e < HD / 8; ++e)
-          ov[e] = live && 8 * e < a.hd ? *reinterpret_cast<const uint4*>(o + 8 * e) : make_uint4(0, 0, 0, 0);
-        if (!__all_sync(0xffffffffu, mbar_wait(q_full, nq & 1))) {
-          ok = false;
-          break;
-        }
-        ++nq;
-        if (live) {
-#pragma unroll
-          for (int e = 0; e < HD / 8; ++e) {
-            if (8 * e < a.hd) {
-              const uint4 dv = *reinterpret_cast<const uint4*>(sO + (e >> 3) * 128 * 128 + row * 128 +
-                                                               (((e & 7) ^ (row & 7)) << 4));
-              const T* x = reinterpret_cast<const T*>(&dv);
-              const T* y = reinterpret_cast<const T*>(&ov[e]);
-#pragma unroll
-              for (int q = 0; q < 8; ++q) D = fmaf(to_f(x[q]), to_f(y[q]), D);
-            }
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_free);
-      }
-      // One part leaves D: the one with the first key tile, or the first of a unit without any.
-      const bool writer = t0 < t1 ? t0 == 0 : u.split == 0 && key_end(a, b, i0, ROWS) == 0;
-      if (writer && half == 0 && i < a.lq) a.dsum[orow] = D;
-      const float lse2 = live ? lse * LOG2E : INFINITY;
-      const float2 c2 = make_float2(c, c), l2 = make_float2(-lse2, -lse2), d2 = make_float2(-D, -D);
+      const bool live = st.x != -INFINITY;  // dead rows: P = 0
+      const float2 c2 = make_float2(c, c), l2 = make_float2(st.x, st.x), d2 = make_float2(st.y, st.y);
       for (int t = t0; t < t1; ++t, ++g) {
         const int j0 = t * C::BN + half * 64;
         uint32_t dp[64];
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g & 1], (g >> 1) & 1) && mbar_wait(dp_full, g & 1))) {
+        const uint32_t scol = lanes + C::S_COL + (g & 1) * 128 + half * 64;
+        uint32_t s[64];
+        if (!__all_sync(0xffffffffu, mbar_wait(dp_full, g & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
         tmem_ld32_async(lanes + C::DP_COL + half * 64, dp);
         tmem_ld32_async(lanes + C::DP_COL + half * 64 + 32, dp + 32);
+        tmem_ld32_async(scol, s);
+        tmem_ld32_async(scol + 32, s + 32);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(dp_free);
-        const uint32_t scol = lanes + C::S_COL + (g & 1) * 128 + half * 64;
-        uint32_t s[64];
-        tmem_ld32_async(scol, s);
-        tmem_ld32_async(scol + 32, s + 32);
-        tmem_wait_ld();
         const bool edge = t * C::BN + C::BN > b.kl || (a.causal && t * C::BN + C::BN - 1 > i0 + b.off);
         if (edge) {
           // Masked keys: P = exp(-inf) = 0 and dP = D, so dS = 0 whatever the keys hold.
 #pragma unroll
           for (int e = 0; e < 64; ++e)
-            if (j0 + e >= limit) s[e] = __float_as_uint(-INFINITY), dp[e] = __float_as_uint(D);
+            if (j0 + e >= limit) s[e] = __float_as_uint(-INFINITY), dp[e] = __float_as_uint(-st.y);
           if (a.k_lens && t * C::BN + C::BN > b.kl && half == 0) {
             if (t * C::BN + row >= b.kl)
               clear_row(ring + ((it + 2 * (t - t0)) % C::STAGES) * C::TILE_BYTES, 128, C::NB, row);
@@ -828,7 +905,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
         ++units;
         tc_fence_after();
       }
-      T* dq = static_cast<T*>(a.dq) + head_offset(a.dq_s, a, u.seq, u.h) + (long long)i * a.dq_s.row;
+      T* dq = static_cast<T*>(a.dq) + unit_offset(a.dq_s, u, u.h) + (long long)i * a.dq_s.row;
       float* part = a.splits > 1 ? a.part + (u.split * rows + orow) * a.hd : nullptr;
 #pragma unroll 1
       for (int q = half * (HD / 64); q < (half + 1) * (HD / 64); ++q) {
@@ -867,7 +944,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
 // 128 keys of one key/value head per unit; the queries of all heads of its group are streamed (128 at a time, 64 for
 // head dims over 64, where the two accumulators take half of TMEM). Two threads per key, half of the tile's queries
 // each. lse and D go by column here: a warp brings them to shared memory, and rows that must not count come with
-// lse = +inf, P = 0. P^T and dS^T of a thread share the columns of its scores.
+// -lse = -inf, P = 0. P^T and dS^T of a thread share the columns of its scores.
 
 template <int HD>
 struct DkvCfg {
@@ -906,14 +983,13 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
   uint8_t* sK = smem;
   uint8_t* sV = smem + C::KV_BYTES;
   uint8_t* ring = smem + 2 * C::KV_BYTES;  // [STAGES][Q, dO]
-  float* stats = reinterpret_cast<float*>(ring + 2 * C::STAGES * C::TILE_BYTES);  // [STATS][lse2 BN, -D BN]
+  float* stats = reinterpret_cast<float*>(ring + 2 * C::STAGES * C::TILE_BYTES);  // [STATS][-lse2 BN, -D BN]
   uint64_t* bars = reinterpret_cast<uint64_t*>(stats + C::STATS * 2 * C::BN);
   uint64_t* full = bars;                  // [STAGES] Q and dO
   uint64_t* empty = full + C::STAGES;
   uint64_t* kv_full = empty + C::STAGES;
   uint64_t* kv_free = kv_full + 1;
-  uint64_t* s_full = kv_free + 1;         // [2]
-  uint64_t* dp_full = s_full + 2;
+  uint64_t* dp_full = kv_free + 1;        // S of the tile too: its product is issued before
   uint64_t* dp_free = dp_full + 1;
   uint64_t* ps_ready = dp_free + 1;
   uint64_t* st_full = ps_ready + 1;       // [STATS]
@@ -929,8 +1005,6 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
     for (int i = 0; i < C::STATS; ++i) mbar_init(&st_full[i], 32), mbar_init(&st_free[i], 8);
     mbar_init(kv_full, 1);
     mbar_init(kv_free, 1);
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
     mbar_init(dp_full, 1);
     mbar_init(dp_free, 8);
     mbar_init(ps_ready, 8);
@@ -945,13 +1019,18 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
   const uint32_t tmem = *slot;
 
   // Tiles of a unit: for each head of the group, query tiles [begin, begin + per); t in [t0, t1) of all of them.
+  struct Walk {
+    int head, tile, per;  // within the group, within the head
+    __device__ __forceinline__ Walk(int t0, int per_) : head(t0 ? t0 / per_ : 0), tile(t0 - head * per_), per(per_) {}
+    __device__ __forceinline__ void next() {
+      if (++tile == per) tile = 0, ++head;
+    }
+  };
   auto range = [&](const TcUnit& u, const Bounds& b, int& begin, int& per, int& t0, int& t1) {
     const int j0 = u.tile * ROWS;
     begin = query_begin(a, b, j0) / C::BN;
     per = j0 < b.kl ? max(0, (b.ql + C::BN - 1) / C::BN - begin) : 0;
-    const int total = per * a.group;
-    t0 = (int)((long long)total * u.split / a.splits);
-    t1 = (int)((long long)total * (u.split + 1) / a.splits);
+    split_range(ta, per * a.group, u.split, t0, t1);
   };
 
   if (warp >= 8) {
@@ -977,11 +1056,12 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
           mbar_expect_tx(kv_full, 2 * C::KV_BYTES);
 #pragma unroll
           for (int c = 0; c < C::NB; ++c) {
-            tma_head(sK + c * 128 * 128, &mk, kv_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
-            tma_head(sV + c * 128 * 128, &mv, kv_full, 64 * c, u.tile * ROWS, u.h, u.seq, a.inner);
+            tma_head(sK + c * 128 * 128, &mk, kv_full, 64 * c, u.tile * ROWS, u.h, u);
+            tma_head(sV + c * 128 * 128, &mv, kv_full, 64 * c, u.tile * ROWS, u.h, u);
           }
-          for (int t = t0; t < t1; ++t, ++it) {
-            const int h = u.h * a.group + t / per, i0 = (begin + t % per) * C::BN;
+          Walk w(t0, per);
+          for (int t = t0; t < t1; ++t, ++it, w.next()) {
+            const int h = u.h * a.group + w.head, i0 = (begin + w.tile) * C::BN;
             const int s = it % C::STAGES, r = it / C::STAGES;
             if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1)) {
               ok = false;
@@ -991,8 +1071,8 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
             uint8_t* d = ring + 2 * s * C::TILE_BYTES;
 #pragma unroll
             for (int c = 0; c < C::NB; ++c) {
-              tma_head(d + c * C::BN * 128, &mq, &full[s], 64 * c, i0, h, u.seq, a.inner);
-              tma_head(d + C::TILE_BYTES + c * C::BN * 128, &mdo, &full[s], 64 * c, i0, h, u.seq, a.inner);
+              tma_head(d + c * C::BN * 128, &mq, &full[s], 64 * c, i0, h, u);
+              tma_head(d + C::TILE_BYTES + c * C::BN * 128, &mdo, &full[s], 64 * c, i0, h, u);
             }
           }
         }
@@ -1008,10 +1088,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         auto issue_s = [&](int i) {
           if (!mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1)) return false;
           tc_fence_after();
-          if (elect_one()) {
-            mma_heads<HD>(tmem + C::S_COL + (i & 1) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
-            umma_commit(&s_full[i & 1]);
-          }
+          if (elect_one()) mma_heads<HD>(tmem + C::S_COL + (i & 1) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
           __syncwarp();
           return true;
         };
@@ -1070,7 +1147,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         if (!ok && lane == 0) atomicExch(&g_error_flag, 32);
       }
     } else if (warp == 10) {
-      // (lse in log2 units, -D) of each streamed tile; +inf and 0 for rows outside the queries.
+      // (-lse in log2 units, -D) of each streamed tile; -inf and 0 for rows outside the queries.
       bool ok = true;
       int g = 0;
       for (int k = 0; ok; ++k) {
@@ -1081,18 +1158,19 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         const Bounds b = bounds_of(a, u.seq);
         int begin, per, t0, t1;
         range(u, b, begin, per, t0, t1);
-        for (int t = t0; t < t1; ++t, ++g) {
-          const int h = u.h * a.group + t / per, i0 = (begin + t % per) * C::BN;
+        if (t0 >= t1) continue;
+        Walk wk(t0, per);
+        for (int t = t0; t < t1; ++t, ++g, wk.next()) {
+          const int h = u.h * a.group + wk.head, i0 = (begin + wk.tile) * C::BN;
           const long long row0 = ((long long)u.seq * a.heads + h) * a.lq + i0;
           const int sb = g % C::STATS, r = g / C::STATS;
           float l[C::BN / 32], d[C::BN / 32];
 #pragma unroll
           for (int e = 0; e < C::BN / 32; ++e) {
             const int i = 32 * e + lane;
-            const bool in = i0 + i < b.ql;
-            const float x = in ? a.lse[row0 + i] : -INFINITY;
-            l[e] = x == -INFINITY ? INFINITY : x * LOG2E - p_shift<T>();
-            d[e] = in ? -a.dsum[row0 + i] : 0.f;
+            const float2 x = i0 + i < b.ql ? ta.stats[row0 + i] : make_float2(-INFINITY, 0.f);
+            l[e] = x.x + p_shift<T>();
+            d[e] = x.y;
           }
           if (r > 0 && !__all_sync(0xffffffffu, mbar_wait(&st_free[sb], (r - 1) & 1))) {
             ok = false;
@@ -1130,26 +1208,26 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
       const int j0 = u.tile * ROWS, j = j0 + row;
       const int first = a.causal ? max(0, -b.off) : 0;       // queries before it see no key
       const int from = a.causal ? max(first, j - b.off) : 0; // this key is seen by queries [from, b.ql)
-      for (int t = t0; t < t1; ++t, ++g) {
-        const int i0 = (begin + t % per) * C::BN;
+      Walk w(t0 < t1 ? t0 : 0, per);
+      for (int t = t0; t < t1; ++t, ++g, w.next()) {
+        const int i0 = (begin + w.tile) * C::BN;
         uint32_t dp[C::HALF], s[C::HALF];
         const int sb = g % C::STATS;
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g & 1], (g >> 1) & 1) && mbar_wait(dp_full, g & 1) &&
-                                         mbar_wait(&st_full[sb], (g / C::STATS) & 1))) {
+        const uint32_t scol = lanes + C::S_COL + (g & 1) * C::BN + half * C::HALF;
+        if (!__all_sync(0xffffffffu, mbar_wait(&st_full[sb], (g / C::STATS) & 1) && mbar_wait(dp_full, g & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
 #pragma unroll
-        for (int q = 0; q < C::HALF; q += 32) tmem_ld32_async(lanes + C::DP_COL + half * C::HALF + q, dp + q);
+        for (int q = 0; q < C::HALF; q += 32) {
+          tmem_ld32_async(lanes + C::DP_COL + half * C::HALF + q, dp + q);
+          tmem_ld32_async(scol + q, s + q);
+        }
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(dp_free);
-        const uint32_t scol = lanes + C::S_COL + (g & 1) * C::BN + half * C::HALF;
-#pragma unroll
-        for (int q = 0; q < C::HALF; q += 32) tmem_ld32_async(scol + q, s + q);
-        tmem_wait_ld();
         const float4* l4 = reinterpret_cast<const float4*>(stats + sb * 2 * C::BN + half * C::HALF);
         const float4* d4 = reinterpret_cast<const float4*>(stats + sb * 2 * C::BN + C::BN + half * C::HALF);
         if (i0 + C::BN > b.ql || i0 < first || (a.causal && j0 + ROWS - 1 > i0 + b.off)) {
@@ -1169,9 +1247,9 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         for (int e = 0; e < C::HALF / 4; ++e) {
           const float4 l = l4[e], d = d4[e];
           const float2 xa = ub::fma2(make_float2(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1])), c2,
-                                     make_float2(-l.x, -l.y));
+                                     make_float2(l.x, l.y));
           const float2 xb = ub::fma2(make_float2(__uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3])), c2,
-                                     make_float2(-l.z, -l.w));
+                                     make_float2(l.z, l.w));
           const float2 pa = make_float2(ex2(xa.x), ex2(xa.y)), pb = make_float2(ex2(xb.x), ex2(xb.y));
           float2 ga = add2(make_float2(__uint_as_float(dp[4 * e]), __uint_as_float(dp[4 * e + 1])),
                            make_float2(d.x, d.y));
@@ -1212,7 +1290,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
       const bool live = j < b.kl && t0 < t1;
       const long long orow = ((long long)u.seq * a.kv_heads + u.h) * a.lk + j;
       // Threads of half 0 write dV, of half 1 dK.
-      T* out = static_cast<T*>(half ? a.dk : a.dv) + head_offset(half ? a.dk_s : a.dv_s, a, u.seq, u.h) +
+      T* out = static_cast<T*>(half ? a.dk : a.dv) + unit_offset(half ? a.dk_s : a.dv_s, u, u.h) +
                (long long)j * (half ? a.dk_s.row : a.dv_s.row);
       float* part = a.splits > 1 ? a.part + ((half ? 0 : a.splits) + u.split) * rows * a.hd + orow * a.hd : nullptr;
       const float mul = half ? a.scale : unshift;
@@ -1291,6 +1369,12 @@ TcArgs tc_args(const AttnArgs& a, const UnblendAttnTrainParams& p, int heads, in
   t.ksteps = (p.hd + 15) / 16;
   t.n_hd = 16 * t.ksteps;
   t.fmt = p.dtype == UNBLEND_BF16 ? 1u : 0u;
+  t.by_splits = fast_div(splits);
+  t.by_tiles = fast_div(t.row_tiles);
+  t.by_heads = fast_div(heads);
+  t.by_inner = fast_div(a.inner);
+  t.by_seq_heads = fast_div((long long)a.seqs * heads);
+  t.stats = reinterpret_cast<const float2*>(a.dsum);
   return t;
 }
 
@@ -1307,6 +1391,21 @@ int launch_fwd(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, c
   auto kern = attention_fwd_tc_kernel<T, HD, NQ>;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   kern<<<grid_of(t.units, NQ == 2 ? 1 : 2), C::THREADS, C::SMEM, st>>>(mq, mk, mv, t);
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+int launch_stats(const AttnArgs& a, cudaStream_t st) {
+  float2* stats = reinterpret_cast<float2*>(a.dsum);
+  const long long rows = (long long)a.seqs * a.lq * a.heads;
+  auto grid = [&](int lanes) { return (unsigned)((rows * lanes + 255) / 256); };
+  if (a.hd <= 32)
+    attention_stats_kernel<T, 4><<<grid(4), 256, 0, st>>>(a, stats);
+  else if (a.hd <= 64)
+    attention_stats_kernel<T, 8><<<grid(8), 256, 0, st>>>(a, stats);
+  else
+    attention_stats_kernel<T, 16><<<grid(16), 256, 0, st>>>(a, stats);
   UB_CHECK_LAUNCH();
   return 0;
 }
@@ -1354,6 +1453,10 @@ int attention_fwd_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int row
     return p.hd <= 64 ? launch_fwd<T, 64, 1>(a, p, a.splits, st) : launch_fwd<T, 128, 1>(a, p, a.splits, st);
   };
   return p.dtype == UNBLEND_BF16 ? go(__nv_bfloat16()) : go(__half());
+}
+
+int attention_stats_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, cudaStream_t st) {
+  return p.dtype == UNBLEND_BF16 ? launch_stats<__nv_bfloat16>(a, st) : launch_stats<__half>(a, st);
 }
 
 int attention_dq_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st) {
