@@ -401,6 +401,193 @@ __global__ void __launch_bounds__(NT) attention_dkv_kernel(const __grid_constant
   }
 }
 
+// ------------------------------------------------------------------------------------------- few queries
+//
+// Forward for at most 8 rows per key/value head (query heads of the group times queries): single new tokens over a long
+// context. Bound by reading K and V once, 4 hd flops per byte-pair of a key and row: far too little for a tile of 128
+// rows. LANES lanes share a key, 8 dims each, so that O of all rows fits few registers and many warps an SM; a group of
+// lanes holds FEW_KEYS keys of K and V in flight, sums their scores over its lanes and keeps its own running maximum,
+// sum and O, joined at the end over the groups and warps. The key range is split over many CTAs;
+// attention_join_kernel joins those.
+constexpr int FEW_ROWS = 8, FEW_NT = 128, FEW_KEYS = 4, FEW_STAGES = 3;
+
+// K and V of a thread's keys in flight: FEW_STAGES x FEW_KEYS x (K, V) x 32 bytes (fp32) or 16.
+constexpr int few_smem(int elem) { return FEW_STAGES * FEW_KEYS * 2 * 8 * elem * FEW_NT; }
+
+template <typename T, int HD, int R>
+__global__ void __launch_bounds__(FEW_NT) attention_few_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int LANES = HD / 8, GROUPS = 32 / LANES;
+  constexpr int V = 16 / (int)sizeof(T), CH = 8 / V;  // elements per chunk, chunks per lane
+  constexpr int WARPS = FEW_NT / 32;
+  __shared__ float sq[R][HD];
+  __shared__ float so[WARPS][R][HD + 2];  // O, maximum, sum of each warp
+  extern __shared__ uint4 ring[];  // [stage][key][chunk][K, V][thread]: a thread reads what it copied itself
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LANES, grp = lane / LANES;
+  const int split = blockIdx.x % a.splits, sh = blockIdx.x / a.splits;
+  const int seq = sh / a.kv_heads, hk = sh - seq * a.kv_heads;
+  const Bounds b = bounds_of(a, seq);
+  const int n_rows = a.group * a.lq;  // row r: head hk * group + r / lq, query r % lq
+  const float c = a.scale * LOG2E;
+  for (int x = threadIdx.x; x < R * HD; x += FEW_NT) {
+    const int r = x / HD, d = x - r * HD;
+    float v = 0.f;
+    if (r < n_rows && r % a.lq < b.ql && d < a.hd)
+      v = to_f((static_cast<const T*>(a.q) + head_offset(a.q_s, a, seq, hk * a.group + r / a.lq) +
+                (long long)(r % a.lq) * a.q_s.row)[d]) * c;
+    sq[r][d] = v;
+  }
+  __syncthreads();
+  const int keys = key_end(a, b, 0, a.lq);
+  const int begin = (int)((long long)keys * split / a.splits), end = (int)((long long)keys * (split + 1) / a.splits);
+  const T* k = static_cast<const T*>(a.k) + head_offset(a.k_s, a, seq, hk);
+  const T* v = static_cast<const T*>(a.v) + head_offset(a.v_s, a, seq, hk);
+  float o[R][CH * V], m[R], l[R];
+  int limit[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    const int i = r % a.lq;
+    limit[r] = r < n_rows && i < b.ql ? (a.causal ? min(b.kl, i + b.off + 1) : b.kl) : 0;
+#pragma unroll
+    for (int e = 0; e < CH * V; ++e) o[r][e] = 0.f;
+  }
+  constexpr int STEP = WARPS * GROUPS * FEW_KEYS;
+  auto at = [&](int stage, int u, int x, int kv) {
+    return ring + (((stage * FEW_KEYS + u) * CH + x) * 2 + kv) * FEW_NT + threadIdx.x;
+  };
+  auto fetch = [&](int stage, int j0) {
+#pragma unroll
+    for (int u = 0; u < FEW_KEYS; ++u) {
+      const int j = j0 + (u * WARPS + warp) * GROUPS + grp;
+#pragma unroll
+      for (int x = 0; x < CH; ++x) {
+        const int d = (x * LANES + sub) * V;
+        if (j < end && d < a.hd) {
+          cp_async16(at(stage, u, x, 0), k + (long long)j * a.k_s.row + d);
+          cp_async16(at(stage, u, x, 1), v + (long long)j * a.v_s.row + d);
+        } else if (j0 < end) {
+          *at(stage, u, x, 0) = *at(stage, u, x, 1) = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < FEW_STAGES - 1; ++i) fetch(i, begin + i * STEP);
+  for (int j0 = begin, stage = 0; j0 < end; j0 += STEP, stage = (stage + 1) % FEW_STAGES) {
+    fetch((stage + FEW_STAGES - 1) % FEW_STAGES, j0 + (FEW_STAGES - 1) * STEP);
+    cp_wait<FEW_STAGES - 1>();
+    float s[FEW_KEYS][R];
+#pragma unroll
+    for (int u = 0; u < FEW_KEYS; ++u)
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[u][r] = 0.f;
+#pragma unroll
+    for (int x = 0; x < CH; ++x)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float q[V];
+#pragma unroll
+        for (int e = 0; e < V; e += 4)
+          *reinterpret_cast<float4*>(q + e) = *reinterpret_cast<const float4*>(&sq[r][(x * LANES + sub) * V + e]);
+#pragma unroll
+        for (int u = 0; u < FEW_KEYS; ++u) {
+          const uint4 w = *at(stage, u, x, 0);
+          const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+          for (int i = 0; i < V; ++i) s[u][r] = fmaf(q[i], to_f(e[i]), s[u][r]);
+        }
+      }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = m[r];
+#pragma unroll
+      for (int u = 0; u < FEW_KEYS; ++u) {
+#pragma unroll
+        for (int w = LANES / 2; w > 0; w >>= 1) s[u][r] += __shfl_xor_sync(0xffffffffu, s[u][r], w);
+        const int j = j0 + (u * WARPS + warp) * GROUPS + grp;
+        if (j >= end || j >= limit[r]) s[u][r] = -INFINITY;
+        top = fmaxf(top, s[u][r]);
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      const float corr = exp2f(m[r] - base);
+      m[r] = top;
+      l[r] *= corr;
+#pragma unroll
+      for (int e = 0; e < CH * V; ++e) o[r][e] *= corr;
+#pragma unroll
+      for (int u = 0; u < FEW_KEYS; ++u) {
+        s[u][r] = exp2f(s[u][r] - base);
+        l[r] += s[u][r];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < FEW_KEYS; ++u)
+#pragma unroll
+      for (int x = 0; x < CH; ++x) {
+        const uint4 w = *at(stage, u, x, 1);
+        const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float f = to_f(e[i]);
+#pragma unroll
+          for (int r = 0; r < R; ++r) o[r][x * V + i] = fmaf(s[u][r], f, o[r][x * V + i]);
+        }
+      }
+  }
+  // The groups of a warp, then the warps.
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float top = m[r];
+#pragma unroll
+    for (int w = LANES; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    const float f = m[r] == -INFINITY && l[r] == l[r] ? 0.f : exp2f(m[r] - (top == -INFINITY ? 0.f : top));
+    l[r] *= f;
+#pragma unroll
+    for (int w = LANES; w < 32; w <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
+#pragma unroll
+    for (int e = 0; e < CH * V; ++e) {
+      float x = o[r][e] * f;
+#pragma unroll
+      for (int w = LANES; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+      if (grp == 0) so[warp][r][((e / V) * LANES + sub) * V + e % V] = x;
+    }
+    if (lane == 0) {
+      so[warp][r][HD] = top;
+      so[warp][r][HD + 1] = l[r];
+    }
+  }
+  __syncthreads();
+  const long long rows = (long long)a.seqs * a.heads * a.lq;
+  for (int x = threadIdx.x; x < n_rows * HD; x += FEW_NT) {
+    const int r = x / HD, d = x - r * HD;
+    float top = -INFINITY, total = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, so[w][r][HD]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float lw = so[w][r][HD + 1];
+      const float f = so[w][r][HD] == -INFINITY && lw == lw ? 0.f : exp2f(so[w][r][HD] - base);
+      total += lw * f;
+      acc = fmaf(so[w][r][d], f, acc);
+    }
+    const int h = hk * a.group + r / a.lq, i = r % a.lq;
+    const long long row = ((long long)seq * a.heads + h) * a.lq + i;
+    const float out = total == 0.f ? 0.f : acc / total;
+    const float lse = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
+    if (a.splits > 1) {
+      if (d < a.hd) a.part[(split * rows + row) * a.hd + d] = out;
+      if (d == 0) a.part_lse[split * rows + row] = lse;
+    } else {
+      if (d < a.hd)
+        (static_cast<T*>(a.out) + head_offset(a.out_s, a, seq, h) + (long long)i * a.out_s.row)[d] = from_f<T>(out);
+      if (d == 0 && a.lse) a.lse[row] = lse;
+    }
+  }
+}
+
 constexpr int fwd_smem(int hdp) { return 4 * (2 * hdp * LD + TILE * (hdp + 4) + TILE * LD); }
 constexpr int dq_smem(int hdp) { return 4 * (4 * hdp * LD + TILE * (hdp + 4) + TILE * LD); }
 constexpr int dkv_smem(int hdp) { return 4 * (4 * hdp * LD + 2 * TILE * (hdp + 4) + TILE * LD); }
@@ -411,20 +598,24 @@ int split_count(long long units, long long tiles, long long want) {
   if (units >= want || tiles <= 1) return 1;
   long long n = (want + units - 1) / units;
   if (n > tiles) n = tiles;
-  return (int)(n < 32 ? n : 32);
+  return (int)(n < MAX_PARTS ? n : MAX_PARTS);
 }
 
 long long div_up(long long a, long long b) { return (a + b - 1) / b; }
 long long round4(long long n) { return (n + 3) / 4 * 4; }
 
-// Work division of a call on the CUDA cores (tc false) or the tensor cores.
+// What a call runs on. A few rows per key/value head (forward): see attention_few_kernel.
+enum Path { CUDA_CORES = 0, TENSOR_CORES = 1, FEW = 2 };
+
+// Work division of a call.
 struct Plan {
   int fwd_rows;  // queries per CTA of the forward kernel
   int fwd_splits, dq_splits, dkv_splits;
   long long q_rows, k_rows;
 };
 
-Plan plan_of(const UnblendAttnTrainParams& p, bool tc) {
+Plan plan_of(const UnblendAttnTrainParams& p, Path path) {
+  const bool tc = path == TENSOR_CORES;
   Plan n;
   const long long seqs = (long long)p.outer * p.inner, qh = seqs * p.heads, kh = seqs * p.kv_heads;
   const long long tile = tc ? 128 : TILE;
@@ -435,25 +626,30 @@ Plan plan_of(const UnblendAttnTrainParams& p, bool tc) {
   n.fwd_rows = (int)tile;
   if (tc && qh * div_up(p.lq, 256) >= sms && p.lq > 128) n.fwd_rows = 256;
   n.fwd_splits = n.fwd_rows == 256 ? 1 : split_count(qh * qt, kt, 2 * sms);
+  // Few rows: two CTAs per SM, of 128 keys at least.
+  if (path == FEW) n.fwd_splits = split_count(kh, div_up(p.lk, 128), 2 * sms);
   n.dq_splits = split_count(qh * qt, kt, tc ? sms : 2 * sms);
   n.dkv_splits = split_count(kh * kt, qt * group, tc ? sms : 2 * sms);
   return n;
 }
 
-// Workspace: forward [parts][q_rows][hd] and [parts][q_rows] lse; backward D or row statistics [q_rows][2], then the larger of the two
-// kernels' parts (they run one after the other). Room for either kind of kernels: which of them runs depends on the
+// Workspace: forward [parts][q_rows][hd] and [parts][q_rows] lse; backward D or row statistics [q_rows][2], then the parts
+// of dq and of dk and dv, which one kernel joins. Room for either kind of kernels: which of them runs depends on the
 // pointers too.
+long long dq_part_floats(const UnblendAttnTrainParams& p, const Plan& n) {
+  return n.dq_splits > 1 ? round4(n.dq_splits * n.q_rows * p.hd) : 0;
+}
+
 long long workspace_floats(const UnblendAttnTrainParams& p, bool backward) {
   long long most = 0;
-  for (int tc = 0; tc < 2; ++tc) {
-    const Plan n = plan_of(p, tc != 0);
+  for (int path = CUDA_CORES; path <= FEW; ++path) {
+    const Plan n = plan_of(p, (Path)path);
     long long need;
     if (!backward) {
       need = n.fwd_splits > 1 ? n.fwd_splits * n.q_rows * (p.hd + 1LL) : 0;
     } else {
-      const long long dq = n.dq_splits > 1 ? n.dq_splits * n.q_rows * p.hd : 0;
-      const long long dkv = n.dkv_splits > 1 ? 2 * n.dkv_splits * n.k_rows * p.hd : 0;
-      need = round4(2 * n.q_rows) + (dq > dkv ? dq : dkv);
+      need = round4(2 * n.q_rows) + dq_part_floats(p, n);
+      if (n.dkv_splits > 1) need += 2 * n.dkv_splits * n.k_rows * p.hd;
     }
     most = need > most ? need : most;
   }
@@ -478,6 +674,17 @@ bool vec4_ok(const void* p, const UnblendHeadStrides& s, const UnblendAttnTrainP
   auto fits = [&](long long st, int n) { return n <= 1 || st % 4 == 0; };
   return reinterpret_cast<uintptr_t>(p) % w == 0 && fits(s.outer, a.outer) && fits(s.inner, a.inner) && s.row % 4 == 0 &&
          s.head % 4 == 0;
+}
+
+// Few rows per key/value head, K and V in 16-byte chunks.
+bool few_fits(const UnblendAttnTrainParams& p, const void* k, const void* v) {
+  const int e = 16 / elem_size(p.dtype);
+  if ((long long)p.heads / p.kv_heads * p.lq > FEW_ROWS || p.hd % e != 0) return false;
+  for (const UnblendHeadStrides* s : {&p.k, &p.v})
+    if ((p.lk > 1 && s->row % e != 0) || (p.kv_heads > 1 && s->head % e != 0) || (p.inner > 1 && s->inner % e != 0) ||
+        (p.outer > 1 && s->outer % e != 0))
+      return false;
+  return aligned16(k) && aligned16(v);
 }
 
 AttnArgs args_of(const UnblendAttnTrainParams& p) {
@@ -509,7 +716,7 @@ AttnArgs args_of(const UnblendAttnTrainParams& p) {
 template <typename T, int HDP>
 int simt_forward(const AttnArgs& a, bool vec, cudaStream_t st) {
   const long long units = (long long)a.seqs * a.heads * div_up(a.lq, TILE) * a.splits;
-  cudaFuncSetAttribute(attention_fwd_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem(HDP));
+  if (allow_smem<attention_fwd_kernel<T, HDP>>(fwd_smem(HDP)) != cudaSuccess) return (int)cudaGetLastError();
   attention_fwd_kernel<T, HDP><<<(unsigned)units, NT, fwd_smem(HDP), st>>>(a, vec);
   UB_CHECK_LAUNCH();
   return 0;
@@ -520,7 +727,7 @@ int simt_dq(AttnArgs a, int splits, float* parts, bool vec, cudaStream_t st) {
   a.splits = splits;
   a.part = parts;
   const long long units = (long long)a.seqs * a.heads * div_up(a.lq, TILE) * splits;
-  cudaFuncSetAttribute(attention_dq_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, dq_smem(HDP));
+  if (allow_smem<attention_dq_kernel<T, HDP>>(dq_smem(HDP)) != cudaSuccess) return (int)cudaGetLastError();
   attention_dq_kernel<T, HDP><<<(unsigned)units, NT, dq_smem(HDP), st>>>(a, vec);
   UB_CHECK_LAUNCH();
   return 0;
@@ -531,22 +738,45 @@ int simt_dkv(AttnArgs a, int splits, float* parts, bool vec, cudaStream_t st) {
   a.splits = splits;
   a.part = parts;
   const long long units = (long long)a.seqs * a.kv_heads * div_up(a.lk, TILE) * splits;
-  cudaFuncSetAttribute(attention_dkv_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, dkv_smem(HDP));
+  if (allow_smem<attention_dkv_kernel<T, HDP>>(dkv_smem(HDP)) != cudaSuccess) return (int)cudaGetLastError();
   attention_dkv_kernel<T, HDP><<<(unsigned)units, NT, dkv_smem(HDP), st>>>(a, vec);
   UB_CHECK_LAUNCH();
   return 0;
 }
 
+template <typename T, int HD, int R>
+int few_forward(const AttnArgs& a, cudaStream_t st) {
+  const long long grid = (long long)a.seqs * a.kv_heads * a.splits;
+  if (allow_smem<attention_few_kernel<T, HD, R>>(few_smem(sizeof(T))) != cudaSuccess) return (int)cudaGetLastError();
+  attention_few_kernel<T, HD, R><<<(unsigned)grid, FEW_NT, few_smem(sizeof(T)), st>>>(a);
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, int HD>
+int few_rows(const AttnArgs& a, cudaStream_t st) {
+  const int rows = a.group * a.lq;
+  if (rows == 1) return few_forward<T, HD, 1>(a, st);
+  if (rows == 2) return few_forward<T, HD, 2>(a, st);
+  if (rows <= 4) return few_forward<T, HD, 4>(a, st);
+  return few_forward<T, HD, 8>(a, st);
+}
+
 template <typename T>
-int forward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Plan& n, bool tc, bool vec,
+int forward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Plan& n, Path path, bool vec,
                   cudaStream_t st) {
   int rc;
-  if (tc)
+  if (path == FEW)
+    rc = a.hd <= 64 ? few_rows<T, 64>(a, st) : few_rows<T, 128>(a, st);
+  else if (path == TENSOR_CORES)
     rc = attention_fwd_tc(a, p, n.fwd_rows, st);
   else
     rc = a.hd <= 64 ? simt_forward<T, 64>(a, vec, st) : simt_forward<T, 128>(a, vec, st);
   if (rc || a.splits == 1) return rc;
-  attention_join_kernel<T><<<(unsigned)div_up(n.q_rows, 8), 256, 0, st>>>(a);
+  if (a.splits <= 4)
+    attention_join_kernel<T, 1><<<(unsigned)div_up(n.q_rows, JOIN_WARPS), 32 * JOIN_WARPS, 0, st>>>(a);
+  else
+    attention_join_kernel<T, JOIN_WARPS><<<(unsigned)n.q_rows, 32 * JOIN_WARPS, 0, st>>>(a);
   UB_CHECK_LAUNCH();
   return 0;
 }
@@ -561,22 +791,25 @@ int backward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Pla
   else
     rc = a.hd <= 64 ? simt_dq<T, 64>(a, n.dq_splits, parts, vec, st) : simt_dq<T, 128>(a, n.dq_splits, parts, vec, st);
   if (rc) return rc;
-  if (n.dq_splits > 1) {
-    attention_sum_kernel<T><<<(unsigned)div_up(n.q_rows, 8), 256, 0, st>>>(a, parts, n.dq_splits, a.heads, a.lq, a.dq,
-                                                                         a.dq_s);
-    UB_CHECK_LAUNCH();
-  }
+  float* kv_parts = parts + dq_part_floats(p, n);
   if (tc)
-    rc = attention_dkv_tc(a, p, n.dkv_splits, parts, st);
+    rc = attention_dkv_tc(a, p, n.dkv_splits, kv_parts, st);
   else
-    rc = a.hd <= 64 ? simt_dkv<T, 64>(a, n.dkv_splits, parts, vec, st)
-                    : simt_dkv<T, 128>(a, n.dkv_splits, parts, vec, st);
-  if (rc || n.dkv_splits == 1) return rc;
-  const unsigned grid = (unsigned)div_up(n.k_rows, 8);
-  attention_sum_kernel<T><<<grid, 256, 0, st>>>(a, parts, n.dkv_splits, a.kv_heads, a.lk, a.dk, a.dk_s);
-  UB_CHECK_LAUNCH();
-  attention_sum_kernel<T><<<grid, 256, 0, st>>>(a, parts + n.dkv_splits * n.k_rows * a.hd, n.dkv_splits, a.kv_heads,
-                                                a.lk, a.dv, a.dv_s);
+    rc = a.hd <= 64 ? simt_dkv<T, 64>(a, n.dkv_splits, kv_parts, vec, st)
+                    : simt_dkv<T, 128>(a, n.dkv_splits, kv_parts, vec, st);
+  if (rc || (n.dq_splits == 1 && n.dkv_splits == 1)) return rc;
+  SumArgs sums{};
+  auto add = [&](const float* part, int splits, int heads, int len, void* out, const UnblendHeadStrides& to) {
+    SumArgs::One& x = sums.of[sums.count++];
+    x = SumArgs::One{part, out, to, splits, heads, len, (long long)a.seqs * heads * len};
+    sums.rows += x.rows;
+  };
+  if (n.dq_splits > 1) add(parts, n.dq_splits, a.heads, a.lq, a.dq, a.dq_s);
+  if (n.dkv_splits > 1) {
+    add(kv_parts, n.dkv_splits, a.kv_heads, a.lk, a.dk, a.dk_s);
+    add(kv_parts + n.dkv_splits * n.k_rows * a.hd, n.dkv_splits, a.kv_heads, a.lk, a.dv, a.dv_s);
+  }
+  attention_sum_kernel<T><<<(unsigned)div_up(sums.rows, 8), 256, 0, st>>>(a, sums);
   UB_CHECK_LAUNCH();
   return 0;
 }
@@ -598,8 +831,9 @@ extern "C" int unblend_attention_forward(const void* q, const void* k, const voi
   const void* ptrs[] = {q, k, v, out};
   const UnblendHeadStrides strides[] = {p->q, p->k, p->v, p->out};
   const int heads[] = {p->heads, p->kv_heads, p->kv_heads, p->heads}, rows[] = {p->lq, p->lk, p->lk, p->lq};
-  const bool tc = attention_tc_fits(*p, ptrs, strides, heads, rows, 4);
-  const Plan n = plan_of(*p, tc);
+  const Path path = few_fits(*p, k, v) ? FEW
+                    : attention_tc_fits(*p, ptrs, strides, heads, rows, 4) ? TENSOR_CORES : CUDA_CORES;
+  const Plan n = plan_of(*p, path);
   AttnArgs a = args_of(*p);
   a.q = q;
   a.k = k;
@@ -613,9 +847,9 @@ extern "C" int unblend_attention_forward(const void* q, const void* k, const voi
   }
   cudaStream_t st = ub::as_stream(stream);
   const bool vec = p->hd % 4 == 0 && vec4_ok(q, p->q, *p) && vec4_ok(k, p->k, *p) && vec4_ok(v, p->v, *p);
-  if (p->dtype == UNBLEND_F32) return forward_types<float>(a, *p, n, tc, vec, st);
-  if (p->dtype == UNBLEND_BF16) return forward_types<__nv_bfloat16>(a, *p, n, tc, vec, st);
-  return forward_types<__half>(a, *p, n, tc, vec, st);
+  if (p->dtype == UNBLEND_F32) return forward_types<float>(a, *p, n, path, vec, st);
+  if (p->dtype == UNBLEND_BF16) return forward_types<__nv_bfloat16>(a, *p, n, path, vec, st);
+  return forward_types<__half>(a, *p, n, path, vec, st);
 }
 
 extern "C" int unblend_attention_backward(const void* dout, const void* q, const void* k, const void* v,
@@ -629,7 +863,7 @@ extern "C" int unblend_attention_backward(const void* dout, const void* q, const
   const int heads[] = {hq, hk, hk, hq, hq, hq, hk, hk};
   const int rows[] = {p->lq, p->lk, p->lk, p->lq, p->lq, p->lq, p->lk, p->lk};
   const bool tc = attention_tc_fits(*p, ptrs, strides, heads, rows, 8);
-  const Plan n = plan_of(*p, tc);
+  const Plan n = plan_of(*p, tc ? TENSOR_CORES : CUDA_CORES);
   AttnArgs a = args_of(*p);
   a.q = q;
   a.k = k;

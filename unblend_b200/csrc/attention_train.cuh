@@ -56,65 +56,99 @@ __device__ __forceinline__ long long head_offset(const UnblendHeadStrides& s, co
   return (long long)o * s.outer + (long long)(seq - o * a.inner) * s.inner + (long long)h * s.head;
 }
 
-// Joins the forward parts of each row: out = sum_s exp(lse_s - lse) out_s. One warp per row, parts in order.
-template <typename T>
-__global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ AttnArgs a) {
-  const int lane = threadIdx.x & 31;
+// Joins the forward parts of each row (at most 32): out = sum_s exp(lse_s - lse) out_s. W warps per row; lane s weighs
+// part s, warp w adds parts w, w + W, ... (at most 4) and the warps' sums are added in order: the loads of all parts are
+// in flight at once.
+constexpr int MAX_PARTS = 32, JOIN_WARPS = 8;
+
+template <typename T, int W>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const __grid_constant__ AttnArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long rows = (long long)a.seqs * a.heads * a.lq;
-  const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) {
-    const float l = a.part_lse[s * rows + row];
-    if (l > top || l != l) top = l;  // a NaN stays
-  }
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;
-  if (top != -INFINITY) {
-    for (int s = 0; s < a.splits; ++s) {
-      const float l = a.part_lse[s * rows + row];
-      if (l == -INFINITY) continue;
-      const float w = expf(l - top);
-      total += w;
+  const long long row = blockIdx.x * (long long)(JOIN_WARPS / W) + warp / W;
+  if (row >= rows) return;  // W = 1: whole warps, no barrier below
+  const float l = lane < a.splits ? a.part_lse[lane * rows + row] : -INFINITY;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, v[4][4];
+  const float* part = a.part + row * a.hd + lane;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int d = 32 * k + lane;
-        if (d < a.hd) acc[k] = fmaf(w, a.part[(s * rows + row) * a.hd + d], acc[k]);
-      }
-    }
+  for (int x = 0; x < 4; ++x) {
+    const int s = x * W + warp % W;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[x][k] = s < a.splits && 32 * k + lane < a.hd ? part[s * rows * a.hd + 32 * k] : 0.f;
   }
-  const float inv = total > 0.f ? 1.f / total : (top != -INFINITY ? total : 0.f);
+  const bool nan = __any_sync(0xffffffffu, l != l);
+  float top = l;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (nan) top = NAN;
+  const float w = top == -INFINITY || l == -INFINITY ? 0.f : expf(l - top);
+  const float total = ub::warp_sum(w);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const float ws = __shfl_sync(0xffffffffu, w, x * W + warp % W);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = fmaf(ws, v[x][k], acc[k]);
+  }
+  const float inv = top == -INFINITY ? 0.f : 1.f / total;
   const int i = (int)(row % a.lq);
   const long long sh = row / a.lq;
   const int h = (int)(sh % a.heads), seq = (int)(sh / a.heads);
   T* out = static_cast<T*>(a.out) + head_offset(a.out_s, a, seq, h) + i * a.out_s.row;
+  if constexpr (W == 1) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int d = 32 * k + lane;
-    if (d < a.hd) out[d] = from_f<T>(acc[k] * inv);
+    for (int k = 0; k < 4; ++k)
+      if (32 * k + lane < a.hd) out[32 * k + lane] = from_f<T>(acc[k] * inv);
+    if (a.lse && lane == 0) a.lse[row] = top == -INFINITY ? top : top + logf(total);
+  } else {
+    static_assert(W == JOIN_WARPS, "one row per CTA");
+    __shared__ float sums[W][128];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sums[warp][32 * k + lane] = acc[k];
+    __syncthreads();
+    if (threadIdx.x < a.hd) {
+      float t = 0.f;
+#pragma unroll
+      for (int x = 0; x < W; ++x) t += sums[x][threadIdx.x];
+      out[threadIdx.x] = from_f<T>(t * inv);
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[row] = top == -INFINITY ? top : top + logf(total);
   }
-  if (a.lse && lane == 0) a.lse[row] = top == -INFINITY ? top : top + logf(total);
 }
 
-// Adds the parts of a gradient row by row: part [splits][seqs * heads * len][hd] -> out.
+// Adds the parts of the gradients row by row: part [splits][seqs * heads * len][hd] -> out, up to three tensors.
+struct SumArgs {
+  struct One {
+    const float* part;
+    void* out;
+    UnblendHeadStrides to;
+    int splits, heads, len;
+    long long rows;
+  } of[3];
+  int count;
+  long long rows;  // of all
+};
+
 template <typename T>
 __global__ void __launch_bounds__(256)
-    attention_sum_kernel(const __grid_constant__ AttnArgs a, const float* part, int splits, int heads, int len,
-                         void* out, const __grid_constant__ UnblendHeadStrides st) {
+    attention_sum_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ SumArgs s) {
   const int lane = threadIdx.x & 31;
-  const long long rows = (long long)a.seqs * heads * len;
-  const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const long long sh = row / len;
-  const int i = (int)(row - sh * len);
-  const int h = (int)(sh % heads), seq = (int)(sh / heads);
-  T* o = static_cast<T*>(out) + head_offset(st, a, seq, h) + i * st.row;
+  long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
+  if (row >= s.rows) return;
+  int w = 0;
+  while (row >= s.of[w].rows) row -= s.of[w++].rows;
+  const SumArgs::One& x = s.of[w];
+  const long long sh = row / x.len;
+  const int i = (int)(row - sh * x.len);
+  const int h = (int)(sh % x.heads), seq = (int)(sh / x.heads);
+  T* o = static_cast<T*>(x.out) + head_offset(x.to, a, seq, h) + i * x.to.row;
   for (int d = lane; d < a.hd; d += 32) {
     float t = 0.f;
-    for (int s = 0; s < splits; ++s) t += part[(s * rows + row) * a.hd + d];
+#pragma unroll 4
+    for (int p = 0; p < x.splits; ++p) t += x.part[(p * x.rows + row) * a.hd + d];
     o[d] = from_f<T>(t);
   }
 }
-
 
 // The tensor-core kernels (attention_train_tc.cu). `fits`: whether they can address the n tensors of a call.
 bool attention_tc_fits(const UnblendAttnTrainParams& p, const void* const* ptrs, const UnblendHeadStrides* strides,

@@ -38,6 +38,27 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 2^x of a pair on the FMA pipe, for a share of the exponentials (the special function unit takes 16 per cycle and SM,
+// the tightest limit at head dim 64). x = n + f with n the nearest integer, read off the low bits of x + 1.5 2^23; 2^f by
+// a polynomial of degree 5 on [-1/2, 1/2] fitted for the least relative error (2.1e-7 in fp32, half the hardware
+// approximation's two ulp); n goes into the exponent. x below -126 gives 2^-126; f * 0 carries NaN into the result.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  constexpr float MAGIC = 12582912.f;
+  auto both = [](float v) { return make_float2(v, v); };
+  const float2 t = add2(x, both(MAGIC));
+  const float2 f = add2(x, ub::fma2(t, both(-1.f), both(MAGIC)));
+  float2 p = ub::fma2(both(0.0013276470126584172f), f, both(0.009675540961325169f));
+  p = ub::fma2(p, f, both(0.05550713092088699f));
+  p = ub::fma2(p, f, both(0.24022120237350464f));
+  p = ub::fma2(p, f, both(0.6931469440460205f));
+  p = ub::fma2(p, f, both(1.0000001192092896f));
+  p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+  p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+  return ub::fma2(f, both(0.f), p);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -62,7 +83,33 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t addr, uint32_t* r) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ld16_async(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_async(uint32_t addr, uint32_t (&r)[N]) {
+  if constexpr (N == 32)
+    tmem_ld32_async(addr, r);
+  else
+    tmem_ld16_async(addr, r);
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// The same, with the registers as operands: nothing that reads them can move in front of it.
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 16)
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                   "+r"(r[i + 6]), "+r"(r[i + 7]), "+r"(r[i + 8]), "+r"(r[i + 9]), "+r"(r[i + 10]), "+r"(r[i + 11]),
+                   "+r"(r[i + 12]), "+r"(r[i + 13]), "+r"(r[i + 14]), "+r"(r[i + 15])::"memory");
+}
 
 // One lane of a converged warp. The MMA warps run their loops and waits with all lanes and issue under this predicate:
 // operands that the compiler knows to be uniform go straight to the tensor core's uniform registers, where issuing
@@ -212,7 +259,8 @@ __device__ __forceinline__ void tma_head(void* dst, const CUtensorMap* map, uint
   tma_load_5d(dst, map, bar, col, row, head, u.si, u.so);
 }
 
-// n consecutive values of a row (n a multiple of 8), times mul, to T or fp32.
+// Up to 32 consecutive values of a row (n left, a multiple of 8), times mul, to T or fp32. Handing 16-byte chunks round
+// a quad of lanes, to write 64 bytes of a row at a time, was no faster.
 template <typename T>
 __device__ __forceinline__ void store_cols(T* out, const uint32_t* v, float mul, int n) {
 #pragma unroll
@@ -251,10 +299,10 @@ struct FwdCfg {
   // Registers: 3 x 168 = 2 x 208 + 88 (NQ = 2, one CTA per SM), 2 x 128 = 200 + 56 (NQ = 1, two).
   static constexpr int REGS_MORE = NQ == 2 ? 208 : 200, REGS_LESS = NQ == 2 ? 88 : 56;
   static constexpr int TMEM = NQ * 256;
-  // Per query tile, 256 columns apart. P has columns of its own where O leaves room: the scores of the next tile are
-  // made as soon as this tile's have been read. At head dims over 64 P overwrites its scores.
-  static constexpr bool APART = HD == 64;
-  static constexpr int S_COL = 0, O_COL = 128, P_COL = APART ? 192 : 0;
+  static constexpr int S_COL = 0, O_COL = 128;  // per query tile, 256 columns apart; P over its scores
+  // One pair in eight of the exponentials goes to the FMA pipe: 3 % (head dim 128) to 8 % (short sequences) faster than
+  // none; one in four was 3 to 7 % slower.
+  static constexpr int FMA_EVERY = 8;
 };
 
 template <typename T, int HD, int NQ>
@@ -275,8 +323,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
   uint64_t* p_ready = s_full + NQ;         // [NQ]
   uint64_t* pv_done = p_ready + NQ;        // [NQ]
   uint64_t* o_free = pv_done + NQ;         // [NQ]
-  uint64_t* s_free = o_free + NQ;          // [NQ] APART: the scores have been read
-  uint32_t* slot = reinterpret_cast<uint32_t*>(s_free + NQ);
+  uint32_t* slot = reinterpret_cast<uint32_t*>(o_free + NQ);
 
   const AttnArgs& a = ta.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -289,7 +336,6 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
       mbar_init(&p_ready[h], 4);
       mbar_init(&pv_done[h], 1);
       mbar_init(&o_free[h], 4);
-      mbar_init(&s_free[h], 4);
     }
     fence_mbar_init();
   }
@@ -371,12 +417,6 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
             break;
           }
           ++nq;
-          if (C::APART && g > 0) {
-#pragma unroll
-            for (int h = 0; h < NQ; ++h)
-              if (!mbar_wait(&s_free[h], (g - 1) & 1)) ok = false;
-            if (!ok) break;
-          }
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -396,24 +436,6 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
               ok = false;
               break;
             }
-            if (C::APART && more) {
-#pragma unroll
-              for (int h = 0; h < NQ; ++h) {
-                if (!mbar_wait(&s_free[h], g & 1)) ok = false;
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-                  mma_heads<HD>(tmem + h * 256 + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps,
-                                id_s);
-                  umma_commit(&s_full[h]);
-                  if (h == NQ - 1) {
-                    umma_commit(&empty[ki % C::STAGES]);
-                    if (t + 2 == n) umma_commit(q_free);
-                  }
-                }
-                __syncwarp();
-              }
-            }
 #pragma unroll
             for (int h = 0; h < NQ; ++h) {
               if (ok && t == 0 && units > 0 && !mbar_wait(&o_free[h], (units - 1) & 1)) ok = false;
@@ -422,16 +444,16 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
               tc_fence_after();
               const uint32_t d = tmem + h * 256;
               if (elect_one()) {
-                mma_rows<C::BN / 16>(d + C::O_COL, [&](int ks) { return d + C::P_COL + 8 * ks; }, stage(vi), 128 * 128,
+                mma_rows<C::BN / 16>(d + C::O_COL, [&](int ks) { return d + C::S_COL + 8 * ks; }, stage(vi), 128 * 128,
                                      id_o, t > 0 ? 1u : 0u);
                 umma_commit(&pv_done[h]);
-                if (!C::APART && more) {
+                if (more) {
                   mma_heads<HD>(d + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps, id_s);
                   umma_commit(&s_full[h]);
                 }
                 if (h == NQ - 1) {
                   umma_commit(&empty[vi % C::STAGES]);
-                  if (!C::APART && more) {
+                  if (more) {
                     umma_commit(&empty[ki % C::STAGES]);
                     if (t + 2 == n) umma_commit(q_free);
                   }
@@ -456,12 +478,15 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
     const long long rows = (long long)a.seqs * a.heads * a.lq;
     bool ok = true;
     int g = 0, it = 0;
+    // The next unit is worked out before the wait for this one's last product, not after its stores.
+    TcUnit u_next = tc_unit(ta, a.heads, blockIdx.x, true);
+    Bounds b_next = bounds_of(a, u_next.seq);
     for (int k = 0; ok; ++k) {
       const int ui = unit_index(k);
       if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
       if (ui >= ta.units) continue;
-      const TcUnit u = tc_unit(ta, a.heads, ui, true);
-      const Bounds b = bounds_of(a, u.seq);
+      const TcUnit u = u_next;
+      const Bounds b = b_next;
       int t0, t1;
       range(u, b, t0, t1);
       const int i0 = (u.tile * NQ + h) * ROWS, i = i0 + row;
@@ -479,11 +504,6 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32_async(lanes + C::S_COL + 32 * q, s + 32 * q);
         tmem_wait_ld();
-        if (C::APART) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[h]);
-        }
         if (j0 + C::BN > b.kl || (a.causal && j0 + C::BN - 1 > i0 + b.off)) {
 #pragma unroll
           for (int e = 0; e < 128; ++e)
@@ -516,21 +536,17 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
 #pragma unroll
         for (int e = 0; e < 64; ++e) {
           const float2 x = ub::fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, mb);
-          const float2 p = make_float2(ex2(x.x), ex2(x.y));
+          const float2 p = e % C::FMA_EVERY == 1 ? ex2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
           sum2 = add2(sum2, p);
           s[e] = pack2<T>(p.x, p.y);
         }
-        const bool any = __any_sync(0xffffffffu, rescale);
-        // O holds the sums up to tile t - 1, and that product has read its P, once it has signalled. Where P lies over
-        // the scores, these would not be there before.
-        if ((C::APART && g > 0) || any) {
+        if (__any_sync(0xffffffffu, rescale)) {
+          // O holds the sums up to tile t - 1: they are complete once their product has signalled.
           if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[h], (g - 1) & 1))) {
             ok = false;
             break;
           }
           tc_fence_after();
-        }
-        if (any) {
 #pragma unroll 1
           for (int q = 0; q < HD / 32; ++q) {
             uint32_t o[32];
@@ -540,8 +556,8 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
             tmem_st32(lanes + C::O_COL + 32 * q, o);
           }
         }
-        tmem_st32(lanes + C::P_COL, *reinterpret_cast<uint32_t(*)[32]>(s));
-        tmem_st32(lanes + C::P_COL + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+        tmem_st32(lanes + C::S_COL, *reinterpret_cast<uint32_t(*)[32]>(s));
+        tmem_st32(lanes + C::S_COL + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -549,6 +565,10 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
       }
       if (!ok) break;
       it += 2 * (t1 - t0);
+      if (const int un = unit_index(k + 1); un < ta.units) {
+        u_next = tc_unit(ta, a.heads, un, true);
+        b_next = bounds_of(a, u_next.seq);
+      }
       const float sum = sum2.x + sum2.y;
       const bool live = i < b.ql && (m > -INFINITY || sum != sum);  // all scores NaN: no maximum, but a NaN sum
       const float inv = live ? 1.f / sum : 0.f;
@@ -638,7 +658,7 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_const
 //
 // 128 queries of one head per unit, keys streamed 128 at a time; two threads per row, 64 keys each. S is double
 // buffered and dP is read into registers first, so the tensor cores make S and dP of the next tile while this one's
-// exponentials are taken. dS of a thread's 64 keys takes 32 of the 64 columns that its scores came from.
+// exponentials are taken. dS of 32 keys takes 16 of the 32 columns that their scores came from.
 
 template <int HD>
 struct DqCfg {
@@ -650,6 +670,8 @@ struct DqCfg {
   static constexpr int THREADS = 384;  // two warpgroups of rows, one for TMA and MMA issue
   static constexpr int REGS_MORE = 208, REGS_LESS = 88;  // 2 x 208 + 88 = 3 x 168
   static constexpr int S_COL = 0, DP_COL = 256, DQ_COL = 384, TMEM = 512;
+  // Head dims over 64 are bound by the products: dP is read at once, so that the next one starts at once.
+  static constexpr bool EARLY = HD > 64;
 };
 
 template <typename T, int HD>
@@ -803,7 +825,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
             tc_fence_after();
             const uint32_t ds = tmem + C::S_COL + ((g + t) & 1) * 128;
             if (elect_one()) {
-              mma_rows<C::BN / 16>(tmem + C::DQ_COL, [&](int ks) { return ds + (ks >> 2) * 64 + (ks & 3) * 8; },
+              mma_rows<C::BN / 16>(tmem + C::DQ_COL, [&](int ks) { return ds + (ks >> 1) * 32 + (ks & 1) * 8; },
                                    stage(it + 2 * t), 128 * 128, id_o, t > 0 ? 1u : 0u);
               umma_commit(&empty[(it + 2 * t) % C::STAGES]);
               if (t + 1 == n) umma_commit(dq_done);
@@ -851,45 +873,81 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
       const long long orow = ((long long)u.seq * a.heads + u.h) * a.lq + i;
       const bool live = st.x != -INFINITY;  // dead rows: P = 0
       const float2 c2 = make_float2(c, c), l2 = make_float2(st.x, st.x), d2 = make_float2(st.y, st.y);
-      for (int t = t0; t < t1; ++t, ++g) {
-        const int j0 = t * C::BN + half * 64;
-        uint32_t dp[64];
-        const uint32_t scol = lanes + C::S_COL + (g & 1) * 128 + half * 64;
-        uint32_t s[64];
+      // A thread's 64 keys go in two chunks; the loads of the next one are in flight during this one's exponentials.
+      uint32_t s0[32], d0[32], s1[32], d1[32];
+      auto load = [&](int tile, int chunk, uint32_t (&s)[32], uint32_t (&d)[32]) {
+        tmem_ld_async(lanes + C::DP_COL + half * 64 + 32 * chunk, d);
+        tmem_ld_async(lanes + C::S_COL + (tile & 1) * 128 + half * 64 + 32 * chunk, s);
+      };
+      // dS of one chunk from its scores and dP, stored over the scores.
+      auto chunk_ds = [&](int t, int chunk, bool edge, uint32_t (&s)[32], uint32_t (&d)[32]) {
+        if (edge) {
+          // Masked keys: P = exp(-inf) = 0 and dP = D, so dS = 0 whatever the keys hold.
+          const int j0 = t * C::BN + half * 64 + 32 * chunk;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (j0 + e >= limit) s[e] = __float_as_uint(-INFINITY), d[e] = __float_as_uint(-st.y);
+        }
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 x = ub::fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, l2);
+          const float2 p = make_float2(ex2(x.x), ex2(x.y));
+          const float2 ds = mul2(p, add2(make_float2(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1])), d2));
+          w[e] = pack2<T>(ds.x, ds.y);
+        }
+        tmem_st16(lanes + C::S_COL + (g & 1) * 128 + half * 64 + 32 * chunk, w);
+      };
+      if (!C::EARLY && t0 < t1) {
         if (!__all_sync(0xffffffffu, mbar_wait(dp_full, g & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        tmem_ld32_async(lanes + C::DP_COL + half * 64, dp);
-        tmem_ld32_async(lanes + C::DP_COL + half * 64 + 32, dp + 32);
-        tmem_ld32_async(scol, s);
-        tmem_ld32_async(scol + 32, s + 32);
-        tmem_wait_ld();
+        load(g, 0, s0, d0);
+      }
+      for (int t = t0; t < t1; ++t, ++g) {
+        const bool edge = t * C::BN + C::BN > b.kl || (a.causal && t * C::BN + C::BN - 1 > i0 + b.off);
+        if (C::EARLY) {
+          if (!__all_sync(0xffffffffu, mbar_wait(dp_full, g & 1))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          load(g, 0, s0, d0);
+        }
+        if (!C::EARLY) {
+          tmem_wait_ld(s0);
+          tmem_wait_ld(d0);
+        }
+        load(g, 1, s1, d1);
+        if (C::EARLY) {
+          tmem_wait_ld(s0);
+          tmem_wait_ld(d0);
+        } else {
+          chunk_ds(t, 0, edge, s0, d0);
+        }
+        tmem_wait_ld(s1);
+        tmem_wait_ld(d1);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(dp_free);
-        const bool edge = t * C::BN + C::BN > b.kl || (a.causal && t * C::BN + C::BN - 1 > i0 + b.off);
-        if (edge) {
-          // Masked keys: P = exp(-inf) = 0 and dP = D, so dS = 0 whatever the keys hold.
-#pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (j0 + e >= limit) s[e] = __float_as_uint(-INFINITY), dp[e] = __float_as_uint(-st.y);
-          if (a.k_lens && t * C::BN + C::BN > b.kl && half == 0) {
-            if (t * C::BN + row >= b.kl)
-              clear_row(ring + ((it + 2 * (t - t0)) % C::STAGES) * C::TILE_BYTES, 128, C::NB, row);
-            fence_proxy_async_smem();
+        if (C::EARLY) chunk_ds(t, 0, edge, s0, d0);
+        // Keys behind the length (NaN included) must be 0 before dS K; S, which also reads them, is complete.
+        if (edge && a.k_lens && t * C::BN + C::BN > b.kl && half == 0) {
+          if (t * C::BN + row >= b.kl)
+            clear_row(ring + ((it + 2 * (t - t0)) % C::STAGES) * C::TILE_BYTES, 128, C::NB, row);
+          fence_proxy_async_smem();
+        }
+        chunk_ds(t, 1, edge, s1, d1);
+        if (!C::EARLY && t + 1 < t1) {
+          if (!__all_sync(0xffffffffu, mbar_wait(dp_full, (g + 1) & 1))) {
+            ok = false;
+            break;
           }
+          tc_fence_after();
+          load(g + 1, 0, s0, d0);
         }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float2 x = ub::fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, l2);
-          const float2 p = make_float2(ex2(x.x), ex2(x.y));
-          const float2 d = add2(make_float2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1])), d2);
-          const float2 ds = mul2(p, d);
-          s[e] = pack2<T>(ds.x, ds.y);
-        }
-        tmem_st32(scol, *reinterpret_cast<uint32_t(*)[32]>(s));
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -957,9 +1015,11 @@ struct DkvCfg {
   static constexpr int SMEM = 2 * KV_BYTES + 2 * STAGES * TILE_BYTES + STATS * BN * 8 + 1024 + 512;
   static constexpr int THREADS = 384;  // two warpgroups of keys, one for TMA, MMA issue and lse / D
   static constexpr int REGS_MORE = 208, REGS_LESS = 88;  // 2 x 208 + 88 = 3 x 168
-  static constexpr int HALF = BN / 2;
+  static constexpr int HALF = BN / 2;  // queries of a tile per thread
+  static constexpr int CH = HALF / 2;  // taken at once
   static constexpr int S_COL = 0, DP_COL = 2 * BN, DV_COL = 3 * BN, DK_COL = 3 * BN + HD, TMEM = 512;
   static_assert(3 * BN + 2 * HD <= 512, "TMEM columns");
+  static constexpr bool EARLY = HD > 64;  // as in the dq kernel
 };
 
 // P of fp16 calls is kept times 2^12: probabilities of long rows would sink into fp16's subnormals.
@@ -1128,13 +1188,13 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
             }
             tc_fence_after();
             const uint32_t p = tmem + C::S_COL + ((g + t) & 1) * C::BN, q = q_tile(g + t);
-            constexpr int KH = C::HALF / 16;  // K steps per half of the tile's queries
+            // The chunk of K step ks (16 queries, 8 columns): P in its first half, dS in its second.
+            constexpr int KC = C::CH / 16;
+            auto p_col = [&](int ks) { return p + (ks / KC) * C::CH + (ks % KC) * 8; };
+            auto ds_col = [&](int ks) { return p_col(ks) + C::CH / 2; };
             if (elect_one()) {
-              mma_rows<2 * KH>(tmem + C::DV_COL, [&](int ks) { return p + (ks / KH) * C::HALF + (ks % KH) * 8; },
-                               q + C::TILE_BYTES, C::BN * 128, id_o, t > 0 ? 1u : 0u);
-              mma_rows<2 * KH>(tmem + C::DK_COL,
-                               [&](int ks) { return p + (ks / KH) * C::HALF + C::HALF / 2 + (ks % KH) * 8; }, q,
-                               C::BN * 128, id_o, t > 0 ? 1u : 0u);
+              mma_rows<C::BN / 16>(tmem + C::DV_COL, p_col, q + C::TILE_BYTES, C::BN * 128, id_o, t > 0 ? 1u : 0u);
+              mma_rows<C::BN / 16>(tmem + C::DK_COL, ds_col, q, C::BN * 128, id_o, t > 0 ? 1u : 0u);
               umma_commit(&empty[(g + t) % C::STAGES]);
               if (t + 1 == n) umma_commit(acc_done);
             }
@@ -1208,74 +1268,113 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
       const int j0 = u.tile * ROWS, j = j0 + row;
       const int first = a.causal ? max(0, -b.off) : 0;       // queries before it see no key
       const int from = a.causal ? max(first, j - b.off) : 0; // this key is seen by queries [from, b.ql)
-      Walk w(t0 < t1 ? t0 : 0, per);
-      for (int t = t0; t < t1; ++t, ++g, w.next()) {
-        const int i0 = (begin + w.tile) * C::BN;
-        uint32_t dp[C::HALF], s[C::HALF];
-        const int sb = g % C::STATS;
-        const uint32_t scol = lanes + C::S_COL + (g & 1) * C::BN + half * C::HALF;
-        if (!__all_sync(0xffffffffu, mbar_wait(&st_full[sb], (g / C::STATS) & 1) && mbar_wait(dp_full, g & 1))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+      // A thread's queries of a tile go in two chunks; the loads of the next one are in flight during this one's
+      // exponentials.
+      uint32_t s0[C::CH], d0[C::CH], s1[C::CH], d1[C::CH];
+      auto load = [&](int tile, int chunk, uint32_t (&s)[C::CH], uint32_t (&d)[C::CH]) {
+        tmem_ld_async(lanes + C::DP_COL + half * C::HALF + C::CH * chunk, d);
+        tmem_ld_async(lanes + C::S_COL + (tile & 1) * C::BN + half * C::HALF + C::CH * chunk, s);
+      };
+      auto arrived = [&](int tile) {  // S, dP and the row statistics of a tile
+        return __all_sync(0xffffffffu, mbar_wait(&st_full[tile % C::STATS], (tile / C::STATS) & 1) &&
+                                           mbar_wait(dp_full, tile & 1));
+      };
+      // P^T and dS^T of one chunk, stored over its scores.
+      auto chunk_pds = [&](int i0, int chunk, bool edge, uint32_t (&s)[C::CH], uint32_t (&d)[C::CH]) {
+        const int col = half * C::HALF + C::CH * chunk;
+        const float* row_stats = stats + (g % C::STATS) * 2 * C::BN + col;
+        const float4* l4 = reinterpret_cast<const float4*>(row_stats);
+        const float4* d4 = reinterpret_cast<const float4*>(row_stats + C::BN);
+        if (edge) {
 #pragma unroll
-        for (int q = 0; q < C::HALF; q += 32) {
-          tmem_ld32_async(lanes + C::DP_COL + half * C::HALF + q, dp + q);
-          tmem_ld32_async(scol + q, s + q);
+          for (int e = 0; e < C::CH; ++e)
+            if (i0 + col + e < from || i0 + col + e >= b.ql) s[e] = __float_as_uint(-INFINITY), d[e] = 0;
         }
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dp_free);
-        const float4* l4 = reinterpret_cast<const float4*>(stats + sb * 2 * C::BN + half * C::HALF);
-        const float4* d4 = reinterpret_cast<const float4*>(stats + sb * 2 * C::BN + C::BN + half * C::HALF);
-        if (i0 + C::BN > b.ql || i0 < first || (a.causal && j0 + ROWS - 1 > i0 + b.off)) {
-          const int ib = i0 + half * C::HALF;
+        uint32_t w[C::CH];  // P, then dS
 #pragma unroll
-          for (int e = 0; e < C::HALF; ++e)
-            if (ib + e < from || ib + e >= b.ql) s[e] = __float_as_uint(-INFINITY), dp[e] = 0;
-          // Rows of Q and dO that must not count (NaN included) become 0 before they are summed over.
-          if ((a.q_lens && i0 + C::BN > b.ql) || i0 < first) {
-            if (row < C::BN && (i0 + row >= b.ql || i0 + row < first))
-              clear_row(ring + (2 * (g % C::STAGES) + half) * C::TILE_BYTES, C::BN, C::NB, row);
-            fence_proxy_async_smem();
-          }
-        }
-        uint32_t pk[C::HALF / 2];
-#pragma unroll
-        for (int e = 0; e < C::HALF / 4; ++e) {
-          const float4 l = l4[e], d = d4[e];
+        for (int e = 0; e < C::CH / 4; ++e) {
+          const float4 l = l4[e], dd = d4[e];
           const float2 xa = ub::fma2(make_float2(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1])), c2,
                                      make_float2(l.x, l.y));
           const float2 xb = ub::fma2(make_float2(__uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3])), c2,
                                      make_float2(l.z, l.w));
           const float2 pa = make_float2(ex2(xa.x), ex2(xa.y)), pb = make_float2(ex2(xb.x), ex2(xb.y));
-          float2 ga = add2(make_float2(__uint_as_float(dp[4 * e]), __uint_as_float(dp[4 * e + 1])),
-                           make_float2(d.x, d.y));
-          float2 gb = add2(make_float2(__uint_as_float(dp[4 * e + 2]), __uint_as_float(dp[4 * e + 3])),
-                           make_float2(d.z, d.w));
+          float2 ga = add2(make_float2(__uint_as_float(d[4 * e]), __uint_as_float(d[4 * e + 1])),
+                           make_float2(dd.x, dd.y));
+          float2 gb = add2(make_float2(__uint_as_float(d[4 * e + 2]), __uint_as_float(d[4 * e + 3])),
+                           make_float2(dd.z, dd.w));
           if (p_shift<T>() != 0.f) ga = mul2(ga, un2), gb = mul2(gb, un2);
           ga = mul2(pa, ga);
           gb = mul2(pb, gb);
-          pk[2 * e] = pack2<T>(pa.x, pa.y);
-          pk[2 * e + 1] = pack2<T>(pb.x, pb.y);
-          s[2 * e] = pack2<T>(ga.x, ga.y);
-          s[2 * e + 1] = pack2<T>(gb.x, gb.y);
+          w[2 * e] = pack2<T>(pa.x, pa.y);
+          w[2 * e + 1] = pack2<T>(pb.x, pb.y);
+          w[C::CH / 2 + 2 * e] = pack2<T>(ga.x, ga.y);
+          w[C::CH / 2 + 2 * e + 1] = pack2<T>(gb.x, gb.y);
         }
-        if constexpr (C::HALF == 64) {
-          tmem_st32(scol, *reinterpret_cast<uint32_t(*)[32]>(pk));
-          tmem_st32(scol + 32, *reinterpret_cast<uint32_t(*)[32]>(s));
+        const uint32_t to = lanes + C::S_COL + (g & 1) * C::BN + col;
+        if constexpr (C::CH == 32)
+          tmem_st32(to, w);
+        else
+          tmem_st16(to, w);
+      };
+      Walk w(t0 < t1 ? t0 : 0, per);
+      if (!C::EARLY && t0 < t1) {
+        if (!arrived(g)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        load(g, 0, s0, d0);
+      }
+      for (int t = t0; t < t1; ++t, ++g, w.next()) {
+        const int i0 = (begin + w.tile) * C::BN;
+        const bool edge = i0 + C::BN > b.ql || i0 < first || (a.causal && j0 + ROWS - 1 > i0 + b.off);
+        if (C::EARLY) {
+          if (!arrived(g)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          load(g, 0, s0, d0);
+        }
+        if (!C::EARLY) {
+          tmem_wait_ld(s0);
+          tmem_wait_ld(d0);
+        }
+        load(g, 1, s1, d1);
+        if (C::EARLY) {
+          tmem_wait_ld(s0);
+          tmem_wait_ld(d0);
         } else {
-          tmem_st16(scol, *reinterpret_cast<uint32_t(*)[16]>(pk));
-          tmem_st16(scol + 16, *reinterpret_cast<uint32_t(*)[16]>(s));
+          chunk_pds(i0, 0, edge, s0, d0);
+        }
+        tmem_wait_ld(s1);
+        tmem_wait_ld(d1);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dp_free);
+        if (C::EARLY) chunk_pds(i0, 0, edge, s0, d0);
+        // Rows of Q and dO that must not count (NaN included) become 0 before they are summed over.
+        if (edge && ((a.q_lens && i0 + C::BN > b.ql) || i0 < first)) {
+          if (row < C::BN && (i0 + row >= b.ql || i0 + row < first))
+            clear_row(ring + (2 * (g % C::STAGES) + half) * C::TILE_BYTES, C::BN, C::NB, row);
+          fence_proxy_async_smem();
+        }
+        chunk_pds(i0, 1, edge, s1, d1);
+        if (!C::EARLY && t + 1 < t1) {
+          if (!arrived(g + 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          load(g + 1, 0, s0, d0);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(ps_ready);
-          mbar_arrive(&st_free[sb]);
+          mbar_arrive(&st_free[g % C::STATS]);
         }
       }
       if (!ok) break;
@@ -1388,8 +1487,8 @@ int launch_fwd(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, c
       !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, 128))
     return UNBLEND_ERR_INVALID;
   const TcArgs t = tc_args(a, p, p.heads, p.lq, NQ * ROWS, splits, a.part);
-  auto kern = attention_fwd_tc_kernel<T, HD, NQ>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  constexpr auto kern = attention_fwd_tc_kernel<T, HD, NQ>;
+  if (allow_smem<kern>(C::SMEM) != cudaSuccess) return (int)cudaGetLastError();
   kern<<<grid_of(t.units, NQ == 2 ? 1 : 2), C::THREADS, C::SMEM, st>>>(mq, mk, mv, t);
   UB_CHECK_LAUNCH();
   return 0;
@@ -1418,8 +1517,8 @@ int launch_dq(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, fl
       !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, 128) || !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, 128))
     return UNBLEND_ERR_INVALID;
   const TcArgs t = tc_args(a, p, p.heads, p.lq, ROWS, splits, part);
-  auto kern = attention_dq_tc_kernel<T, HD>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  constexpr auto kern = attention_dq_tc_kernel<T, HD>;
+  if (allow_smem<kern>(C::SMEM) != cudaSuccess) return (int)cudaGetLastError();
   kern<<<grid_of(t.units, 1), C::THREADS, C::SMEM, st>>>(mq, mdo, mk, mv, t);
   UB_CHECK_LAUNCH();
   return 0;
@@ -1433,8 +1532,8 @@ int launch_dkv(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, f
       !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, 128) || !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, 128))
     return UNBLEND_ERR_INVALID;
   const TcArgs t = tc_args(a, p, p.kv_heads, p.lk, ROWS, splits, part);
-  auto kern = attention_dkv_tc_kernel<T, HD>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  constexpr auto kern = attention_dkv_tc_kernel<T, HD>;
+  if (allow_smem<kern>(C::SMEM) != cudaSuccess) return (int)cudaGetLastError();
   kern<<<grid_of(t.units, 1), C::THREADS, C::SMEM, st>>>(mk, mv, mq, mdo, t);
   UB_CHECK_LAUNCH();
   return 0;

@@ -93,16 +93,6 @@ __device__ __forceinline__ uint4 shfl_down1(const uint4& v) {
                     __shfl_down_sync(0xffffffffu, v.z, 1), __shfl_down_sync(0xffffffffu, v.w, 1));
 }
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {  // all but the newest N groups are there
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // A run of VEC consecutive values of a row on its way through shared memory: the aligned chunk that holds the first of
 // them and, for the last lane of a warp, the chunk behind it (other lanes get that from their neighbour). A thread
 // reads what it copied itself, so no barrier is needed. `g` is the number of the run.
@@ -514,19 +504,25 @@ template <typename T, typename TW, int NV, bool ALIGNED, bool WARP>
 int launch_one(const NormArgs& a, bool backward, cudaStream_t st) {
   constexpr int PER = NV * 16 / (int)sizeof(T);  // values per thread
   const int threads = WARP ? 256 : ((a.cols + PER - 1) / PER + 31) / 32 * 32;
+  // Most shared memory of any row width: the kernel is allowed that once.
+  constexpr int MOST_THREADS = WARP ? 256 : 512;
   if (backward) {
-    auto kern = layer_norm_bwd_kernel<T, TW, NV, ALIGNED, WARP>;
-    int smem = Ring<stages_of<T, NV, 2, WARP>(), 2 * NV, ALIGNED>::bytes(threads);
-    if (WARP && smem < 8 * 4 * a.cols) smem = 8 * 4 * a.cols;
-    if (smem > 40 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    kern<<<bwd_ctas(a.rows, a.cols), threads, smem, st>>>(a);
+    constexpr auto kern = layer_norm_bwd_kernel<T, TW, NV, ALIGNED, WARP>;
+    using Rows = Ring<stages_of<T, NV, 2, WARP>(), 2 * NV, ALIGNED>;
+    constexpr int JOIN = WARP ? 8 * 4 * 32 * PER : 0;  // the warps' sums
+    constexpr int MOST = Rows::bytes(MOST_THREADS) > JOIN ? Rows::bytes(MOST_THREADS) : JOIN;
+    if (MOST > 40 * 1024 && allow_smem<kern>(MOST) != cudaSuccess) return (int)cudaGetLastError();
+    const int rows = Rows::bytes(threads), join = WARP ? 8 * 4 * a.cols : 0;
+    kern<<<bwd_ctas(a.rows, a.cols), threads, rows > join ? rows : join, st>>>(a);
   } else {
-    auto kern = layer_norm_fwd_kernel<T, TW, NV, ALIGNED, WARP>;
-    const int smem = Ring<stages_of<T, NV, 1, WARP>(), NV, ALIGNED>::bytes(threads);
-    if (smem > 40 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    constexpr auto kern = layer_norm_fwd_kernel<T, TW, NV, ALIGNED, WARP>;
+    using Rows = Ring<stages_of<T, NV, 1, WARP>(), NV, ALIGNED>;
+    constexpr int MOST = Rows::bytes(MOST_THREADS);
+    if (MOST > 40 * 1024 && allow_smem<kern>(MOST) != cudaSuccess) return (int)cudaGetLastError();
+    const int smem = Rows::bytes(threads);
     // As many CTAs as run at once: each walks the same number of rows, a partial second wave would cost a whole one.
     int per_sm = 1;
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
+    if ((a.rows + 7) / 8 > ub::kNumSMs) cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
     kern<<<ub::grid_1d(a.rows, WARP ? 8 : 1, (long long)per_sm * ub::kNumSMs), threads, smem, st>>>(a);
   }
   UB_CHECK_LAUNCH();

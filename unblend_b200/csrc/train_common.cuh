@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ub {
@@ -122,6 +124,30 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
         reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(raw)[i];
     }
   }
+}
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {  // all but the newest N groups are there
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory: a driver call, made once per kernel and device.
+template <auto KERNEL>
+inline cudaError_t allow_smem(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // Rows of a tensor whose leading axes are (outer, inner): row r starts at (r / inner) * so + (r % inner) * si.
