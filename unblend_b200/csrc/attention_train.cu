@@ -403,8 +403,8 @@ __global__ void __launch_bounds__(NT) attention_dkv_kernel(const __grid_constant
 
 // ------------------------------------------------------------------------------------------- few queries
 //
-// Forward for at most 8 rows per key/value head (query heads of the group times queries): single new tokens over a long
-// context. Bound by reading K and V once, 4 hd flops per byte-pair of a key and row: far too little for a tile of 128
+// Forward for at most 8 rows per key/value head (query heads of the group times queries), fp32: single new tokens over a
+// long context. Bound by reading K and V once, 4 hd flops per byte-pair of a key and row: far too little for a tile of 128
 // rows. LANES lanes share a key, 8 dims each, so that O of all rows fits few registers and many warps an SM; a group of
 // lanes holds FEW_KEYS keys of K and V in flight, sums their scores over its lanes and keeps its own running maximum,
 // sum and O, joined at the end over the groups and warps. The key range is split over many CTAs;
@@ -588,6 +588,229 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_kernel(const __grid_cons
   }
 }
 
+// The same for 16-bit types on mma.sync, up to 16 rows per key/value head: on the CUDA cores the products and the sums
+// over lanes took 170 instructions per key, which bound the kernel (22 us where the reads take 5); here 16 keys take
+// about 90. Rows are the M = 16 of m16n8k16: Q stays in registers as A, K rows are B of the scores, P goes from the score
+// fragments into A of P V as it is, V^T comes by transposing loads. tcgen05's 128 rows would leave most lanes idle and
+// wants P in TMEM for tiles too small to hide that. Each warp has its own ring of 16-key tiles and its own maxima, sums
+// and O: no barrier until the end. 16-byte chunk c of a row lies at c ^ (row & 7).
+constexpr int MMA_ROWS = 16, MMA_STAGES = 3;
+constexpr int few_mma_smem(int hd) { return (FEW_NT / 32) * MMA_STAGES * 2 * 16 * hd * 2; }
+
+__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"((uint32_t)__cvta_generic_to_shared(p))
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"((uint32_t)__cvta_generic_to_shared(p))
+               : "memory");
+}
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  const T v[2] = {from_f<T>(lo), from_f<T>(hi)};
+  return *reinterpret_cast<const uint32_t*>(v);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(FEW_NT) attention_few_mma_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int WARPS = FEW_NT / 32, CHUNKS = HD / 8, TILE_E = 16 * HD;  // a K or V tile: 16 keys
+  extern __shared__ __align__(128) uint8_t few_smem_raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, ql = lane & 3;
+  T* tiles = reinterpret_cast<T*>(few_smem_raw) + warp * MMA_STAGES * 2 * TILE_E;
+  const int split = blockIdx.x % a.splits, sh = blockIdx.x / a.splits;
+  const int seq = sh / a.kv_heads, hk = sh - seq * a.kv_heads;
+  const Bounds b = bounds_of(a, seq);
+  const int n_rows = a.group * a.lq;  // row r: head hk * group + r / lq, query r % lq
+  const int keys = key_end(a, b, 0, a.lq);
+  const int begin = (int)((long long)keys * split / a.splits), end = (int)((long long)keys * (split + 1) / a.splits);
+  const T* k = static_cast<const T*>(a.k) + head_offset(a.k_s, a, seq, hk);
+  const T* v = static_cast<const T*>(a.v) + head_offset(a.v_s, a, seq, hk);
+  auto fetch = [&](int stage, int j0) {  // keys j0 .. j0 + 15
+    if (j0 < end) {
+      T* d = tiles + stage * 2 * TILE_E;
+#pragma unroll
+      for (int x = 0; x < 16 * CHUNKS / 32; ++x) {
+        const int id = x * 32 + lane, row = id / CHUNKS, c = id % CHUNKS, j = j0 + row;
+        const bool in = j < end && 8 * c < a.hd;
+        const int to = row * HD + ((c ^ (row & 7)) * 8);
+        cp_async16_or_zero(d + to, in ? k + (long long)j * a.k_s.row + 8 * c : k, in);
+        cp_async16_or_zero(d + TILE_E + to, in ? v + (long long)j * a.v_s.row + 8 * c : v, in);
+      }
+    }
+    cp_commit();
+  };
+  constexpr int STEP = WARPS * 16;
+  const int first = begin + warp * 16;
+#pragma unroll
+  for (int i = 0; i < MMA_STAGES - 1; ++i) fetch(i, first + i * STEP);
+  // Q as A fragments: rows quad and quad + 8, dims 16 ks + 2 ql + {0, 1} and + 8.
+  uint32_t qf[HD / 16][4];
+  int limit[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int r = quad + 8 * x, i = r % a.lq;
+    const bool in = r < n_rows && i < b.ql;
+    limit[x] = in ? (a.causal ? min(b.kl, i + b.off + 1) : b.kl) : 0;
+    const T* q = static_cast<const T*>(a.q) +
+                 (in ? head_offset(a.q_s, a, seq, hk * a.group + r / a.lq) + (long long)i * a.q_s.row : 0);
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int d = 16 * ks + 8 * y + 2 * ql;
+        T e[2] = {from_f<T>(0.f), from_f<T>(0.f)};
+        if (in && d < a.hd) e[0] = q[d];
+        if (in && d + 1 < a.hd) e[1] = q[d + 1];
+        qf[ks][2 * y + x] = *reinterpret_cast<const uint32_t*>(e);
+      }
+  }
+  const float c = a.scale * LOG2E;
+  float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+  const int mi = lane >> 3, mr = lane & 7;  // matrix and row that this lane addresses
+  for (int j0 = first, stage = 0; j0 < end; j0 += STEP, stage = (stage + 1) % MMA_STAGES) {
+    fetch((stage + MMA_STAGES - 1) % MMA_STAGES, j0 + (MMA_STAGES - 1) * STEP);
+    cp_wait<MMA_STAGES - 1>();
+    __syncwarp();
+    const T* tk = tiles + stage * 2 * TILE_E;
+    const T* tv = tk + TILE_E;
+    float s[2][4];  // keys 8 n + 2 ql + {0, 1} of rows quad, quad + 8
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      const int row = (mi >> 1) * 8 + mr;
+      uint32_t f[4];
+      ldmatrix4(f, tk + row * HD + (((2 * ks + (mi & 1)) ^ mr) * 8));
+      mma16(s[0], qf[ks], f[0], f[1], T());
+      mma16(s[1], qf[ks], f[2], f[3], T());
+    }
+    float p[2][4];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float top = m[x];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = j0 + 8 * n + 2 * ql + e;
+          float& z = s[n][2 * x + e];
+          z = j < end && j < limit[x] ? z * c : -INFINITY;
+          top = fmaxf(top, z);
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float base = top == -INFINITY ? 0.f : top;
+      const float corr = exp2f(m[x] - base);
+      m[x] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[n][2 * x + e] = exp2f(s[n][2 * x + e] - base);
+          sum += p[n][2 * x + e];
+        }
+      l[x] = l[x] * corr + sum;  // this lane's keys
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n) o[n][2 * x] *= corr, o[n][2 * x + 1] *= corr;
+    }
+    const uint32_t pf[4] = {pack_pair<T>(p[0][0], p[0][1]), pack_pair<T>(p[0][2], p[0][3]),
+                            pack_pair<T>(p[1][0], p[1][1]), pack_pair<T>(p[1][2], p[1][3])};
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) {
+      const int row = (mi & 1) * 8 + mr;
+      uint32_t f[4];
+      ldmatrix4_trans(f, tv + row * HD + (((2 * d + (mi >> 1)) ^ mr) * 8));
+      mma16(o[2 * d], pf, f[0], f[1], T());
+      mma16(o[2 * d + 1], pf, f[2], f[3], T());
+    }
+    __syncwarp();  // the tile is overwritten by the next but one fetch
+  }
+  // Warps join through shared memory, over the tiles: [warp][row][HD + 2].
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(few_smem_raw);
+  auto at = [&](int w, int r) { return so + (w * MMA_ROWS + r) * (HD + 2); };
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    float* to = at(warp, quad + 8 * x);
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n) {
+      to[8 * n + 2 * ql] = o[n][2 * x];
+      to[8 * n + 2 * ql + 1] = o[n][2 * x + 1];
+    }
+    if (ql == 0) {
+      to[HD] = m[x];
+      to[HD + 1] = l[x];
+    }
+  }
+  __syncthreads();
+  const long long rows = (long long)a.seqs * a.heads * a.lq;
+  for (int r = warp; r < n_rows; r += WARPS) {
+    float top = -INFINITY, total = 0.f, f[WARPS];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, at(w, r)[HD]);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float mw = at(w, r)[HD], lw = at(w, r)[HD + 1];
+      f[w] = mw == -INFINITY && lw == lw ? 0.f : exp2f(mw - (top == -INFINITY ? 0.f : top));
+      total += lw * f[w];
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const float lse = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
+    const int h = hk * a.group + r / a.lq, i = r % a.lq;
+    const long long row = ((long long)seq * a.heads + h) * a.lq + i;
+    T* out = static_cast<T*>(a.out) + head_offset(a.out_s, a, seq, h) + (long long)i * a.out_s.row;
+    for (int d = lane; d < a.hd; d += 32) {
+      float acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) acc = fmaf(at(w, r)[d], f[w], acc);
+      if (a.splits > 1)
+        a.part[(split * rows + row) * a.hd + d] = acc * inv;
+      else
+        out[d] = from_f<T>(acc * inv);
+    }
+    if (lane == 0) {
+      if (a.splits > 1)
+        a.part_lse[split * rows + row] = lse;
+      else if (a.lse)
+        a.lse[row] = lse;
+    }
+  }
+}
+static_assert(few_mma_smem(64) >= (FEW_NT / 32) * MMA_ROWS * (64 + 2) * 4, "the join uses the tiles' memory");
+
 constexpr int fwd_smem(int hdp) { return 4 * (2 * hdp * LD + TILE * (hdp + 4) + TILE * LD); }
 constexpr int dq_smem(int hdp) { return 4 * (4 * hdp * LD + TILE * (hdp + 4) + TILE * LD); }
 constexpr int dkv_smem(int hdp) { return 4 * (4 * hdp * LD + 2 * TILE * (hdp + 4) + TILE * LD); }
@@ -626,8 +849,8 @@ Plan plan_of(const UnblendAttnTrainParams& p, Path path) {
   n.fwd_rows = (int)tile;
   if (tc && qh * div_up(p.lq, 256) >= sms && p.lq > 128) n.fwd_rows = 256;
   n.fwd_splits = n.fwd_rows == 256 ? 1 : split_count(qh * qt, kt, 2 * sms);
-  // Few rows: two CTAs per SM, of 128 keys at least.
-  if (path == FEW) n.fwd_splits = split_count(kh, div_up(p.lk, 128), 2 * sms);
+  // Few rows: CTAs of 128 keys at least, twice as many as run at once, for sequences of unequal lengths.
+  if (path == FEW) n.fwd_splits = split_count(kh, div_up(p.lk, 128), 4 * sms);
   n.dq_splits = split_count(qh * qt, kt, tc ? sms : 2 * sms);
   n.dkv_splits = split_count(kh * kt, qt * group, tc ? sms : 2 * sms);
   return n;
@@ -679,7 +902,8 @@ bool vec4_ok(const void* p, const UnblendHeadStrides& s, const UnblendAttnTrainP
 // Few rows per key/value head, K and V in 16-byte chunks.
 bool few_fits(const UnblendAttnTrainParams& p, const void* k, const void* v) {
   const int e = 16 / elem_size(p.dtype);
-  if ((long long)p.heads / p.kv_heads * p.lq > FEW_ROWS || p.hd % e != 0) return false;
+  const int most = p.dtype == UNBLEND_F32 ? FEW_ROWS : MMA_ROWS;
+  if ((long long)p.heads / p.kv_heads * p.lq > most || p.hd % e != 0) return false;
   for (const UnblendHeadStrides* s : {&p.k, &p.v})
     if ((p.lk > 1 && s->row % e != 0) || (p.kv_heads > 1 && s->head % e != 0) || (p.inner > 1 && s->inner % e != 0) ||
         (p.outer > 1 && s->outer % e != 0))
@@ -762,12 +986,29 @@ int few_rows(const AttnArgs& a, cudaStream_t st) {
   return few_forward<T, HD, 8>(a, st);
 }
 
+template <typename T, int HD>
+int few_mma(const AttnArgs& a, cudaStream_t st) {
+  const long long grid = (long long)a.seqs * a.kv_heads * a.splits;
+  if (allow_smem<attention_few_mma_kernel<T, HD>>(few_mma_smem(HD)) != cudaSuccess) return (int)cudaGetLastError();
+  attention_few_mma_kernel<T, HD><<<(unsigned)grid, FEW_NT, few_mma_smem(HD), st>>>(a);
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+int few_types(const AttnArgs& a, cudaStream_t st) {
+  if constexpr (sizeof(T) == 4)
+    return a.hd <= 64 ? few_rows<T, 64>(a, st) : few_rows<T, 128>(a, st);
+  else
+    return a.hd <= 64 ? few_mma<T, 64>(a, st) : few_mma<T, 128>(a, st);
+}
+
 template <typename T>
 int forward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Plan& n, Path path, bool vec,
                   cudaStream_t st) {
   int rc;
   if (path == FEW)
-    rc = a.hd <= 64 ? few_rows<T, 64>(a, st) : few_rows<T, 128>(a, st);
+    rc = few_types<T>(a, st);
   else if (path == TENSOR_CORES)
     rc = attention_fwd_tc(a, p, n.fwd_rows, st);
   else
