@@ -14,8 +14,9 @@
 // columns, and both latency (one row per warp in flight) and issue slots (scalar arithmetic) had been the bound.
 //
 // Rows that do not start on 16-byte boundaries (odd widths, slices) move by aligned 16-byte chunks as well: a thread
-// takes its values out of its own chunk and its neighbour's. Only the values at the ends of a row, whose chunk reaches
-// outside it, move one by one.
+// takes its values out of its own chunk and its neighbour's. A chunk at the end of a row holds values of the next one,
+// or of the gap between them; only chunks that reach in front of the tensor's first row or behind its last are put
+// together value by value (a load that the thread waits for: done at every row's ends it cost half the bandwidth).
 //
 // The weights' gradients are summed in registers over the rows that a group walks, joined across the CTA in shared
 // memory, and the CTAs' partial rows added in a fixed order by a second kernel: the result is the same on every run.
@@ -42,6 +43,7 @@ struct NormArgs {
   unsigned rows;
   int cols;
   int w_vec;  // the weights' base is aligned for 16-byte loads
+  const void *x_lo, *x_hi, *dy_lo, *dy_hi;  // the memory from the first row's first value to the last one's end
   float eps;
 };
 
@@ -102,26 +104,30 @@ struct Run {
 
   __device__ __forceinline__ static int shift(const T* row) { return (int)(reinterpret_cast<uintptr_t>(row) & 15); }
 
-  __device__ __forceinline__ static void chunk(uint4* dst, const T* row, int first, int cols) {
-    if (first >= 0 && first + VEC <= cols) {
-      cp_async16(dst, row + first);
-    } else if (first < cols) {  // reaches outside the row: its values one by one
+  __device__ __forceinline__ static void chunk(uint4* dst, const T* row, int first, int cols, const void* lo,
+                                               const void* hi) {
+    const T* p = row + first;
+    if (first >= cols) return;
+    if (p >= static_cast<const T*>(lo) && p + VEC <= static_cast<const T*>(hi)) {
+      cp_async16(dst, p);
+    } else {
       uint4 v = make_uint4(0, 0, 0, 0);
       T* e = reinterpret_cast<T*>(&v);
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (first + i >= 0 && first + i < cols) e[i] = row[first + i];
+        if (first + i >= 0 && first + i < cols) e[i] = p[i];
       *dst = v;
     }
   }
 
-  __device__ __forceinline__ static void fetch(uint4* a, uint4* b, const T* row, int g, int cols) {
+  __device__ __forceinline__ static void fetch(uint4* a, uint4* b, const T* row, int g, int cols, const void* lo,
+                                               const void* hi) {
     if constexpr (ALIGNED) {
       if (g * VEC < cols) cp_async16(a, row + g * VEC);
     } else {
       const int first = g * VEC - shift(row) / (int)sizeof(T);
-      chunk(a, row, first, cols);
-      if ((threadIdx.x & 31) == 31 && shift(row)) chunk(b, row, first + VEC, cols);
+      chunk(a, row, first, cols, lo, hi);
+      if ((threadIdx.x & 31) == 31 && shift(row)) chunk(b, row, first + VEC, cols, lo, hi);
     }
   }
 
@@ -161,10 +167,12 @@ struct Ring {
   }
 };
 
-// Rows in flight: 4, 2 where four of them would leave room for one CTA only.
+// Rows in flight: 4, less where they would leave room for one CTA only (a warp per row) or for none (a CTA per row).
 template <typename T, int NV, int TENSORS, bool WARP>
 constexpr int stages_of() {
-  return (WARP ? 256 : 512) * NV * TENSORS * 16 * 4 > 112 * 1024 ? 2 : 4;
+  const int one = (WARP ? 256 : 528) * NV * TENSORS * 16;
+  if (WARP) return 4 * one > 112 * 1024 ? 2 : 4;
+  return 4 * one > 208 * 1024 ? 3 : 4;
 }
 
 // Stores VEC values of every lane (runs g of consecutive lanes follow one another) to a row that starts anywhere. The
@@ -231,7 +239,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
     if (r < a.rows) {
       const T* x = xb + row_offset(a.xm, (unsigned)r);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) R::fetch(ring.a(stage, k), ring.b(stage, k), x, k * tpr + t, a.cols);
+      for (int k = 0; k < NV; ++k) R::fetch(ring.a(stage, k), ring.b(stage, k), x, k * tpr + t, a.cols, a.x_lo, a.x_hi);
     }
     cp_commit();
   };
@@ -290,12 +298,14 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
   }
 }
 
-// The sums of the weights' gradients take the registers; a row's x and dy are read again for its second pass.
+// The sums of the weights' gradients take the registers: a warp reads its row's x and dy again for the second pass, a
+// CTA's thread, with 16 values, keeps them.
 template <typename T, typename TW, int NV, bool ALIGNED, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
     layer_norm_bwd_kernel(const __grid_constant__ NormArgs a) {
   constexpr int VEC = 16 / (int)sizeof(T);
   constexpr int ST = stages_of<T, NV, 2, WARP>();
+  constexpr bool KEEP = !WARP;
   using R = Run<T, ALIGNED>;
   __shared__ float red[64];
   extern __shared__ uint4 dyn[];
@@ -320,8 +330,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
       const T* dy = dyb + row_offset(a.dym, (unsigned)r);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        R::fetch(ring.a(stage, k), ring.b(stage, k), x, k * tpr + t, a.cols);
-        R::fetch(ring.a(stage, NV + k), ring.b(stage, NV + k), dy, k * tpr + t, a.cols);
+        R::fetch(ring.a(stage, k), ring.b(stage, k), x, k * tpr + t, a.cols, a.x_lo, a.x_hi);
+        R::fetch(ring.a(stage, NV + k), ring.b(stage, NV + k), dy, k * tpr + t, a.cols, a.dy_lo, a.dy_hi);
       }
     }
     cp_commit();
@@ -355,17 +365,19 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
         gy[i] = mul2(d[i], gm[i]);
       }
     };
+    float2 xh[KEEP ? NV : 1][VEC / 2], gy[KEEP ? NV : 1][VEC / 2];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if (ALIGNED && (k * tpr + t) * VEC >= a.cols) break;
-      float2 xh[VEC / 2], d[VEC / 2], gy[VEC / 2];
-      values(k, xh, d, gy);
+      float2 d[VEC / 2];
+      const int at = KEEP ? k : 0;
+      values(k, xh[at], d, gy[at]);
 #pragma unroll
       for (int i = 0; i < VEC / 2; ++i) {
-        dg[k][i] = ub::fma2(d[i], xh[i], dg[k][i]);
+        dg[k][i] = ub::fma2(d[i], xh[at][i], dg[k][i]);
         db[k][i] = add2(db[k][i], d[i]);
-        s0 = add2(s0, gy[i]);
-        s1 = ub::fma2(gy[i], xh[i], s1);
+        s0 = add2(s0, gy[at][i]);
+        s1 = ub::fma2(gy[at][i], xh[at][i], s1);
       }
     }
     float s[2] = {s0.x + s0.y, s1.x + s1.y};
@@ -377,11 +389,15 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if (ALIGNED && (k * tpr + t) * VEC >= a.cols) break;
-      float2 xh[VEC / 2], d[VEC / 2], gy[VEC / 2];
-      values(k, xh, d, gy);
+      const int at = KEEP ? k : 0;
+      if (!KEEP) {
+        float2 d[VEC / 2];
+        values(k, xh[at], d, gy[at]);
+      }
+      float2 o[VEC / 2];
 #pragma unroll
-      for (int i = 0; i < VEC / 2; ++i) gy[i] = ub::fma2(xh[i], c1, ub::fma2(gy[i], r2, c0));
-      store_run<T, ALIGNED>(dx, k * tpr + t, a.cols, gy);
+      for (int i = 0; i < VEC / 2; ++i) o[i] = ub::fma2(xh[at][i], c1, ub::fma2(gy[at][i], r2, c0));
+      store_run<T, ALIGNED>(dx, k * tpr + t, a.cols, o);
     }
   }
   if (a.dgamma == nullptr) return;
@@ -534,6 +550,7 @@ int launch_cols(const NormArgs& a, bool backward, cudaStream_t st) {
   constexpr int N8 = sizeof(T) / 2;  // 16-byte runs of 8 values
   if (a.cols <= 256) return launch_one<T, TW, N8, ALIGNED, true>(a, backward, st);
   if (a.cols <= 512) return launch_one<T, TW, 2 * N8, ALIGNED, true>(a, backward, st);
+  if (a.cols <= 768) return launch_one<T, TW, 3 * N8, ALIGNED, true>(a, backward, st);
   if (a.cols <= WARP_COLS) return launch_one<T, TW, 4 * N8, ALIGNED, true>(a, backward, st);
   return launch_one<T, TW, 2 * N8, ALIGNED, false>(a, backward, st);
 }
@@ -568,6 +585,14 @@ int launch(const NormArgs& a, int dtype, int w_dtype, bool vec, bool backward, c
                                 : launch_types<__half, __half>(a, vec, backward, st);
 }
 
+// The bytes from the first to behind the last value of a tensor's rows.
+void span(const void* base, const RowMap& m, long long outer, int cols, int elem, const void** lo, const void** hi) {
+  long long first = 0, last = 0;
+  for (const long long d : {(outer - 1) * m.so, ((long long)m.inner - 1) * m.si}) (d < 0 ? first : last) += d;
+  *lo = static_cast<const char*>(base) + first * elem;
+  *hi = static_cast<const char*>(base) + (last + cols) * elem;
+}
+
 bool types_ok(int dtype, int w_dtype) {
   return known_type(dtype) && (w_dtype == UNBLEND_F32 || w_dtype == dtype);
 }
@@ -597,6 +622,7 @@ extern "C" int unblend_layer_norm_forward(const void* x, long long x_so, long lo
   const int es = elem_size(dtype);
   const bool vec = cols % (16 / es) == 0 && rows_aligned(x, a.xm, outer, es, 16) && aligned16(y);
   a.w_vec = aligned16(gamma) && aligned16(beta);
+  span(x, a.xm, outer, cols, es, &a.x_lo, &a.x_hi);
   return launch(a, dtype, w_dtype, vec, false, ub::as_stream(stream));
 }
 
@@ -623,6 +649,8 @@ extern "C" int unblend_layer_norm_backward(const void* dy, long long dy_so, long
   const bool vec = cols % (16 / es) == 0 && rows_aligned(x, a.xm, outer, es, 16) &&
                    rows_aligned(dy, a.dym, outer, es, 16) && aligned16(dx);
   a.w_vec = aligned16(gamma);
+  span(x, a.xm, outer, cols, es, &a.x_lo, &a.x_hi);
+  span(dy, a.dym, outer, cols, es, &a.dy_lo, &a.dy_hi);
   cudaStream_t st = ub::as_stream(stream);
   const int rc = launch(a, dtype, w_dtype, vec, true, st);
   if (rc || !a.part) return rc;
