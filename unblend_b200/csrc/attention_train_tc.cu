@@ -692,8 +692,10 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
   uint64_t* q_free = q_full + 1;
   uint64_t* dp_full = q_free + 1;  // S of the tile too: its product is issued before
   uint64_t* dp_free = dp_full + 1;
+  // [2], by tile: a warp can be done with tile g + 1 while another still works on g, but not with g + 2, whose dP is
+  // issued after all of g has been waited for.
   uint64_t* ds_ready = dp_free + 1;
-  uint64_t* dq_done = ds_ready + 1;
+  uint64_t* dq_done = ds_ready + 2;
   uint64_t* dq_free = dq_done + 1;
   uint32_t* slot = reinterpret_cast<uint32_t*>(dq_free + 1);
 
@@ -705,7 +707,8 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
     mbar_init(q_free, 1);
     mbar_init(dp_full, 1);
     mbar_init(dp_free, 8);
-    mbar_init(ds_ready, 8);
+    mbar_init(&ds_ready[0], 8);
+    mbar_init(&ds_ready[1], 8);
     mbar_init(dq_done, 1);
     mbar_init(dq_free, 8);
     fence_mbar_init();
@@ -818,7 +821,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
               ok = false;
               break;
             }
-            if (!mbar_wait(ds_ready, (g + t) & 1)) {
+            if (!mbar_wait(&ds_ready[(g + t) & 1], ((g + t) >> 1) & 1)) {
               ok = false;
               break;
             }
@@ -951,7 +954,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(ds_ready);
+        if (lane == 0) mbar_arrive(&ds_ready[g & 1]);
       }
       if (!ok) break;
       it += 2 * (t1 - t0);
@@ -1051,8 +1054,8 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
   uint64_t* kv_free = kv_full + 1;
   uint64_t* dp_full = kv_free + 1;        // S of the tile too: its product is issued before
   uint64_t* dp_free = dp_full + 1;
-  uint64_t* ps_ready = dp_free + 1;
-  uint64_t* st_full = ps_ready + 1;       // [STATS]
+  uint64_t* ps_ready = dp_free + 1;       // [2], by tile, as ds_ready of the dq kernel
+  uint64_t* st_full = ps_ready + 2;       // [STATS]
   uint64_t* st_free = st_full + C::STATS; // [STATS]
   uint64_t* acc_done = st_free + C::STATS;
   uint64_t* acc_free = acc_done + 1;
@@ -1067,7 +1070,8 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
     mbar_init(kv_free, 1);
     mbar_init(dp_full, 1);
     mbar_init(dp_free, 8);
-    mbar_init(ps_ready, 8);
+    mbar_init(&ps_ready[0], 8);
+    mbar_init(&ps_ready[1], 8);
     mbar_init(acc_done, 1);
     mbar_init(acc_free, 8);
     fence_mbar_init();
@@ -1182,7 +1186,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
               ok = false;
               break;
             }
-            if ((t == 0 && units > 0 && !mbar_wait(acc_free, (units - 1) & 1)) || !mbar_wait(ps_ready, (g + t) & 1)) {
+            if ((t == 0 && units > 0 && !mbar_wait(acc_free, (units - 1) & 1)) || !mbar_wait(&ps_ready[(g + t) & 1], ((g + t) >> 1) & 1)) {
               ok = false;
               break;
             }
@@ -1373,7 +1377,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(ps_ready);
+          mbar_arrive(&ps_ready[g & 1]);
           mbar_arrive(&st_free[g % C::STATS]);
         }
       }

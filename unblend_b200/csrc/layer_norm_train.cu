@@ -28,7 +28,8 @@ using namespace ub::train;
 
 constexpr int WARP_COLS = 1024;   // widest row of a warp
 constexpr int CTA_COLS = 8192;    // widest row held in a CTA's registers
-constexpr int ONE_CTA_ROWS = 64;  // backward calls of up to so many narrow rows run in one CTA, without partial sums
+// Backward calls of up to so many narrow rows run in one CTA of 16 warps, without partial sums and their kernel.
+constexpr int ONE_CTA_ROWS = 64;
 
 struct NormArgs {
   const void* x;
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
 // The sums of the weights' gradients take the registers: a warp reads its row's x and dy again for the second pass, a
 // CTA's thread, with 16 values, keeps them.
 template <typename T, typename TW, int NV, bool ALIGNED, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? 2 : 1)
+__global__ void __launch_bounds__(512)
     layer_norm_bwd_kernel(const __grid_constant__ NormArgs a) {
   constexpr int VEC = 16 / (int)sizeof(T);
   constexpr int ST = stages_of<T, NV, 2, WARP>();
@@ -519,21 +520,23 @@ bool joins(long long rows, int cols) { return cols > CTA_COLS || bwd_ctas(rows, 
 template <typename T, typename TW, int NV, bool ALIGNED, bool WARP>
 int launch_one(const NormArgs& a, bool backward, cudaStream_t st) {
   constexpr int PER = NV * 16 / (int)sizeof(T);  // values per thread
-  const int threads = WARP ? 256 : ((a.cols + PER - 1) / PER + 31) / 32 * 32;
-  // Most shared memory of any row width: the kernel is allowed that once.
-  constexpr int MOST_THREADS = WARP ? 256 : 512;
+  int threads = WARP ? 256 : ((a.cols + PER - 1) / PER + 31) / 32 * 32;
   if (backward) {
     constexpr auto kern = layer_norm_bwd_kernel<T, TW, NV, ALIGNED, WARP>;
     using Rows = Ring<stages_of<T, NV, 2, WARP>(), 2 * NV, ALIGNED>;
-    constexpr int JOIN = WARP ? 8 * 4 * 32 * PER : 0;  // the warps' sums
+    // A call of one CTA takes 16 warps where their rows fit shared memory.
+    constexpr int MOST_THREADS = !WARP || Rows::bytes(512) <= 200 * 1024 ? 512 : 256;
+    if (WARP && bwd_ctas(a.rows, a.cols) == 1) threads = MOST_THREADS;
+    // The most of any width, allowed once: the rows in flight, or the warps' sums.
+    constexpr int JOIN = WARP ? MOST_THREADS / 32 * 4 * 32 * PER : 0;
     constexpr int MOST = Rows::bytes(MOST_THREADS) > JOIN ? Rows::bytes(MOST_THREADS) : JOIN;
     if (MOST > 40 * 1024 && allow_smem<kern>(MOST) != cudaSuccess) return (int)cudaGetLastError();
-    const int rows = Rows::bytes(threads), join = WARP ? 8 * 4 * a.cols : 0;
+    const int rows = Rows::bytes(threads), join = WARP ? threads / 32 * 4 * a.cols : 0;
     kern<<<bwd_ctas(a.rows, a.cols), threads, rows > join ? rows : join, st>>>(a);
   } else {
     constexpr auto kern = layer_norm_fwd_kernel<T, TW, NV, ALIGNED, WARP>;
     using Rows = Ring<stages_of<T, NV, 1, WARP>(), NV, ALIGNED>;
-    constexpr int MOST = Rows::bytes(MOST_THREADS);
+    constexpr int MOST = Rows::bytes(WARP ? 256 : 512);
     if (MOST > 40 * 1024 && allow_smem<kern>(MOST) != cudaSuccess) return (int)cudaGetLastError();
     const int smem = Rows::bytes(threads);
     // As many CTAs as run at once: each walks the same number of rows, a partial second wave would cost a whole one.

@@ -157,6 +157,7 @@ struct RowMap {
 };
 
 __device__ __forceinline__ long long row_offset(const RowMap& m, unsigned r) {
+  if (r < m.inner) return (long long)r * m.si;  // one level, or its first run: no division
   const unsigned o = r / m.inner;
   return (long long)o * m.so + (long long)(r - o * m.inner) * m.si;
 }
