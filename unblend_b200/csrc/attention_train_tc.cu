@@ -91,6 +91,11 @@ __device__ __forceinline__ void tmem_ld16_async(uint32_t addr, uint32_t* r) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 template <int N>
 __device__ __forceinline__ void tmem_ld_async(uint32_t addr, uint32_t (&r)[N]) {
   if constexpr (N == 32)
@@ -283,37 +288,45 @@ __device__ __forceinline__ void store_cols_f32(float* out, const uint32_t* v, fl
                       __uint_as_float(v[d + 3]) * mul);
 }
 
+// SHORT kernels (head dims to 64, at most 64 streamed rows): sequences of one tile give nothing to overlap within a
+// unit, so a tile is 64 rows and nothing is double buffered; the forward kernel's CTAs then fit an SM three times. 801
+// sequences of 62 x 62, 8 heads: forward 78 -> 55 us, backward 297 -> 236 us (two CTAs per SM of the backward kernels,
+// with half the registers and spills, took 268).
+constexpr int SHORT_ROWS = 64;
+
 // ---------------------------------------------------------------------------------------------- forward
 //
 // A CTA holds NQ tiles of 128 queries of one head (NQ = 2 shares each K / V tile between 256 queries), each with its
 // own softmax warpgroup; while one warpgroup takes exponentials, the tensor cores work for the other.
 
-template <int HD, int NQ>
+template <int HD, int NQ, bool SHORT>
 struct FwdCfg {
-  static constexpr int BN = 128;                       // keys per tile
+  static constexpr int BN = SHORT ? SHORT_ROWS : 128;  // keys per tile
   static constexpr int NB = HD / 64;                   // 64-column blocks
-  static constexpr int TILE_BYTES = 128 * 128 * NB;    // a Q, K or V tile
+  static constexpr int Q_BYTES = 128 * 128 * NB;       // a Q tile
+  static constexpr int TILE_BYTES = BN * 128 * NB;     // a K or V tile
   static constexpr int STAGES = NQ == 2 ? (HD == 64 ? 8 : 4) : (HD == 64 ? 4 : 2);  // ring of K and V tiles
-  static constexpr int SMEM = (NQ + STAGES) * TILE_BYTES + 1024 + 512;
+  static constexpr int SMEM = NQ * Q_BYTES + STAGES * TILE_BYTES + 1024 + 512;
   static constexpr int THREADS = NQ * 128 + 128;       // softmax warpgroups, then one for TMA and MMA issue
-  // Registers: 3 x 168 = 2 x 208 + 88 (NQ = 2, one CTA per SM), 2 x 128 = 200 + 56 (NQ = 1, two).
-  static constexpr int REGS_MORE = NQ == 2 ? 208 : 200, REGS_LESS = NQ == 2 ? 88 : 56;
-  static constexpr int TMEM = NQ * 256;
-  static constexpr int S_COL = 0, O_COL = 128;  // per query tile, 256 columns apart; P over its scores
+  static constexpr int PER_SM = SHORT ? 3 : NQ == 2 ? 1 : 2;
+  // Registers: 3 x 168 = 2 x 208 + 88 (NQ = 2), 2 x 128 = 200 + 56 (NQ = 1), 2 x 80 = 112 + 48 (SHORT).
+  static constexpr int REGS_MORE = SHORT ? 112 : NQ == 2 ? 208 : 200, REGS_LESS = SHORT ? 48 : NQ == 2 ? 88 : 56;
+  static constexpr int TMEM = SHORT ? 128 : NQ * 256;
+  static constexpr int S_COL = 0, O_COL = BN;  // per query tile, 256 columns apart; P over its scores
   // One pair in eight of the exponentials goes to the FMA pipe: 3 % (head dim 128) to 8 % (short sequences) faster than
   // none; one in four was 3 to 7 % slower.
   static constexpr int FMA_EVERY = 8;
 };
 
-template <typename T, int HD, int NQ>
-__global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
+template <typename T, int HD, int NQ, bool SHORT>
+__global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ, SHORT>::PER_SM)
     attention_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                             const __grid_constant__ CUtensorMap mv, const __grid_constant__ TcArgs ta) {
-  using C = FwdCfg<HD, NQ>;
+  using C = FwdCfg<HD, NQ, SHORT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* ring = smem + NQ * C::TILE_BYTES;
+  uint8_t* ring = smem + NQ * C::Q_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::TILE_BYTES);
   uint64_t* full = bars;                   // [STAGES]
   uint64_t* empty = full + C::STAGES;      // [STAGES]
@@ -363,7 +376,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
           mbar_expect_tx(&full[s], C::TILE_BYTES);
 #pragma unroll
           for (int b = 0; b < C::NB; ++b)
-            tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, u);
+            tma_head(ring + s * C::TILE_BYTES + b * C::BN * 128, m, &full[s], 64 * b, row, head, u);
           ++it;
           return true;
         };
@@ -381,12 +394,12 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
             break;
           }
           ++nq;
-          mbar_expect_tx(q_full, NQ * C::TILE_BYTES);
+          mbar_expect_tx(q_full, NQ * C::Q_BYTES);
 #pragma unroll
           for (int h = 0; h < NQ; ++h)
 #pragma unroll
             for (int c = 0; c < C::NB; ++c)
-              tma_head(sQ + h * C::TILE_BYTES + c * 128 * 128, &mq, q_full, 64 * c, (u.tile * NQ + h) * ROWS, u.h,
+              tma_head(sQ + h * C::Q_BYTES + c * 128 * 128, &mq, q_full, 64 * c, (u.tile * NQ + h) * ROWS, u.h,
                        u);
           const int hk = u.h / a.group;
           for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u) && load(&mv, t * C::BN, hk, u);
@@ -421,7 +434,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
           if (elect_one()) {
 #pragma unroll
             for (int h = 0; h < NQ; ++h) {
-              mma_heads<HD>(tmem + h * 256 + C::S_COL, q0 + h * C::TILE_BYTES, stage(it), 128, 128, ta.ksteps, id_s);
+              mma_heads<HD>(tmem + h * 256 + C::S_COL, q0 + h * C::Q_BYTES, stage(it), 128, C::BN, ta.ksteps, id_s);
               umma_commit(&s_full[h]);
             }
             umma_commit(&empty[it % C::STAGES]);
@@ -444,11 +457,11 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
               tc_fence_after();
               const uint32_t d = tmem + h * 256;
               if (elect_one()) {
-                mma_rows<C::BN / 16>(d + C::O_COL, [&](int ks) { return d + C::S_COL + 8 * ks; }, stage(vi), 128 * 128,
+                mma_rows<C::BN / 16>(d + C::O_COL, [&](int ks) { return d + C::S_COL + 8 * ks; }, stage(vi), C::BN * 128,
                                      id_o, t > 0 ? 1u : 0u);
                 umma_commit(&pv_done[h]);
                 if (more) {
-                  mma_heads<HD>(d + C::S_COL, q0 + h * C::TILE_BYTES, stage(ki), 128, 128, ta.ksteps, id_s);
+                  mma_heads<HD>(d + C::S_COL, q0 + h * C::Q_BYTES, stage(ki), 128, C::BN, ta.ksteps, id_s);
                   umma_commit(&s_full[h]);
                 }
                 if (h == NQ - 1) {
@@ -500,14 +513,14 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
           break;
         }
         tc_fence_after();
-        uint32_t s[128];
+        uint32_t s[C::BN];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32_async(lanes + C::S_COL + 32 * q, s + 32 * q);
+        for (int q = 0; q < C::BN / 32; ++q) tmem_ld32_async(lanes + C::S_COL + 32 * q, s + 32 * q);
         tmem_wait_ld();
         if (j0 + C::BN > b.kl || (a.causal && j0 + C::BN - 1 > i0 + b.off)) {
 #pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (j0 + e >= limit) s[e] = __float_as_uint(-INFINITY);
+          for (int e = 0; e < C::BN; ++e)
+            if (e >= limit - j0) s[e] = __float_as_uint(-INFINITY);
           // V rows behind the length (NaN included) must be 0 before P V. Query tile 0 goes first.
           if (h == 0 && a.k_lens && j0 + C::BN > b.kl) {
             const int vi = it + 2 * (t - t0) + 1;
@@ -515,13 +528,14 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
               ok = false;
               break;
             }
-            if (j0 + row >= b.kl) clear_row(ring + (vi % C::STAGES) * C::TILE_BYTES, 128, C::NB, row);
+            if (row < C::BN && j0 + row >= b.kl)
+              clear_row(ring + (vi % C::STAGES) * C::TILE_BYTES, C::BN, C::NB, row);
             fence_proxy_async_smem();
           }
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
+        for (int e = 0; e < C::BN; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
         bool rescale = false;
         float corr = 1.f;
@@ -534,7 +548,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
         const float base = m == -INFINITY ? 0.f : m;
         const float2 c2 = make_float2(c, c), mb = make_float2(-base, -base);
 #pragma unroll
-        for (int e = 0; e < 64; ++e) {
+        for (int e = 0; e < C::BN / 2; ++e) {
           const float2 x = ub::fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, mb);
           const float2 p = e % C::FMA_EVERY == 1 ? ex2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
           sum2 = add2(sum2, p);
@@ -557,7 +571,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ>::THREADS, NQ == 2 ? 1 : 2)
           }
         }
         tmem_st32(lanes + C::S_COL, *reinterpret_cast<uint32_t(*)[32]>(s));
-        tmem_st32(lanes + C::S_COL + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+        if constexpr (C::BN > 64) tmem_st32(lanes + C::S_COL + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -632,9 +646,18 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_const
   const long long n = (long long)a.seqs * a.lq * a.heads;
   const long long id = (blockIdx.x * 256LL + threadIdx.x) / LANES;
   const bool in = id < n;
-  const long long token = in ? id / a.heads : 0;
-  const int h = in ? (int)(id - token * a.heads) : 0;
-  const int seq = (int)(token / a.lq), i = (int)(token - (long long)seq * a.lq);
+  int h = 0, seq = 0, i = 0;
+  if (n <= 0xFFFFFFFFll) {  // 32-bit divisions where they do
+    const unsigned x = in ? (unsigned)id : 0u, token = x / (unsigned)a.heads;
+    h = (int)(x - token * (unsigned)a.heads);
+    seq = (int)(token / (unsigned)a.lq);
+    i = (int)(token - (unsigned)seq * (unsigned)a.lq);
+  } else if (in) {
+    const long long token = id / a.heads;
+    h = (int)(id - token * a.heads);
+    seq = (int)(token / a.lq);
+    i = (int)(token - (long long)seq * a.lq);
+  }
   const Bounds b = bounds_of(a, seq);
   const long long row = ((long long)seq * a.heads + h) * a.lq + i;
   const float lse = in && i < b.ql ? a.lse[row] : -INFINITY;
@@ -660,31 +683,34 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_const
 // buffered and dP is read into registers first, so the tensor cores make S and dP of the next tile while this one's
 // exponentials are taken. dS of 32 keys takes 16 of the 32 columns that their scores came from.
 
-template <int HD>
+template <int HD, bool SHORT>
 struct DqCfg {
-  static constexpr int BN = 128;
+  static constexpr int BN = SHORT ? SHORT_ROWS : 128;
   static constexpr int NB = HD / 64;
-  static constexpr int TILE_BYTES = 128 * 128 * NB;
-  static constexpr int STAGES = HD == 64 ? 8 : 4;
-  static constexpr int SMEM = (2 + STAGES) * TILE_BYTES + 1024 + 512;
+  static constexpr int Q_BYTES = 128 * 128 * NB;
+  static constexpr int TILE_BYTES = BN * 128 * NB;
+  static constexpr int STAGES = HD == 64 && !SHORT ? 8 : 4;
+  static constexpr int SMEM = 2 * Q_BYTES + STAGES * TILE_BYTES + 1024 + 512;
   static constexpr int THREADS = 384;  // two warpgroups of rows, one for TMA and MMA issue
   static constexpr int REGS_MORE = 208, REGS_LESS = 88;  // 2 x 208 + 88 = 3 x 168
-  static constexpr int S_COL = 0, DP_COL = 256, DQ_COL = 384, TMEM = 512;
+  static constexpr int HALF = BN / 2, CH = HALF / 2;  // keys of a tile per thread, and taken at once
+  static constexpr int SB = SHORT ? 1 : 2;  // S buffers
+  static constexpr int S_COL = 0, DP_COL = SB * BN, DQ_COL = (SB + 1) * BN, TMEM = SHORT ? 256 : 512;
   // Head dims over 64 are bound by the products: dP is read at once, so that the next one starts at once.
-  static constexpr bool EARLY = HD > 64;
+  static constexpr bool EARLY = HD > 64 || SHORT;
 };
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
+template <typename T, int HD, bool SHORT>
+__global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
     attention_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mdo,
                            const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                            const __grid_constant__ TcArgs ta) {
-  using C = DqCfg<HD>;
+  using C = DqCfg<HD, SHORT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                      // Q, then dO
-  uint8_t* sO = smem + C::TILE_BYTES;
-  uint8_t* ring = smem + 2 * C::TILE_BYTES;
+  uint8_t* sO = smem + C::Q_BYTES;
+  uint8_t* ring = smem + 2 * C::Q_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::TILE_BYTES);
   uint64_t* full = bars;
   uint64_t* empty = full + C::STAGES;
@@ -736,7 +762,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
           mbar_expect_tx(&full[s], C::TILE_BYTES);
 #pragma unroll
           for (int b = 0; b < C::NB; ++b)
-            tma_head(ring + s * C::TILE_BYTES + b * 128 * 128, m, &full[s], 64 * b, row, head, u);
+            tma_head(ring + s * C::TILE_BYTES + b * C::BN * 128, m, &full[s], 64 * b, row, head, u);
           ++it;
           return true;
         };
@@ -754,7 +780,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
             break;
           }
           ++nq;
-          mbar_expect_tx(q_full, 2 * C::TILE_BYTES);
+          mbar_expect_tx(q_full, 2 * C::Q_BYTES);
 #pragma unroll
           for (int c = 0; c < C::NB; ++c) {
             tma_head(sQ + c * 128 * 128, &mq, q_full, 64 * c, u.tile * ROWS, u.h, u);
@@ -788,7 +814,8 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
             if (!wait_full(it + 2 * t)) return false;
             tc_fence_after();
             if (elect_one())
-              mma_heads<HD>(tmem + C::S_COL + ((g + t) & 1) * 128, q0, stage(it + 2 * t), 128, 128, ta.ksteps, id_s);
+              mma_heads<HD>(tmem + C::S_COL + ((g + t) % C::SB) * C::BN, q0, stage(it + 2 * t), 128, C::BN, ta.ksteps,
+                            id_s);
             __syncwarp();
             return true;
           };
@@ -798,7 +825,7 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
             if (g + t > 0 && !mbar_wait(dp_free, (g + t - 1) & 1)) return false;
             tc_fence_after();
             if (elect_one()) {
-              mma_heads<HD>(tmem + C::DP_COL, o0, stage(it + 2 * t + 1), 128, 128, ta.ksteps, id_s);
+              mma_heads<HD>(tmem + C::DP_COL, o0, stage(it + 2 * t + 1), 128, C::BN, ta.ksteps, id_s);
               umma_commit(dp_full);
               umma_commit(&empty[(it + 2 * t + 1) % C::STAGES]);
               if (t + 1 == n) umma_commit(q_free);
@@ -812,8 +839,8 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
           }
           ++nq;
           for (int t = 0; t < n; ++t) {
-            // S of the next tile overwrites dS of tile t - 1, whose product was issued before it.
-            if (t + 1 < n && (!issue_s(t + 1) || !issue_dp(t + 1))) {
+            // S of the next tile overwrites dS of tile t - 1 (of tile t with one buffer), whose product is issued first.
+            if (C::SB == 2 && t + 1 < n && (!issue_s(t + 1) || !issue_dp(t + 1))) {
               ok = false;
               break;
             }
@@ -826,14 +853,18 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
               break;
             }
             tc_fence_after();
-            const uint32_t ds = tmem + C::S_COL + ((g + t) & 1) * 128;
+            const uint32_t ds = tmem + C::S_COL + ((g + t) % C::SB) * C::BN;
             if (elect_one()) {
-              mma_rows<C::BN / 16>(tmem + C::DQ_COL, [&](int ks) { return ds + (ks >> 1) * 32 + (ks & 1) * 8; },
-                                   stage(it + 2 * t), 128 * 128, id_o, t > 0 ? 1u : 0u);
+              mma_rows<C::BN / 16>(tmem + C::DQ_COL, [&](int ks) { return ds + ks / (C::CH / 16) * C::CH + ks % (C::CH / 16) * 8; },
+                                   stage(it + 2 * t), C::BN * 128, id_o, t > 0 ? 1u : 0u);
               umma_commit(&empty[(it + 2 * t) % C::STAGES]);
               if (t + 1 == n) umma_commit(dq_done);
             }
             __syncwarp();
+            if (C::SB == 1 && t + 1 < n && (!issue_s(t + 1) || !issue_dp(t + 1))) {
+              ok = false;
+              break;
+            }
           }
           if (!ok) break;
           g += n;
@@ -877,29 +908,38 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
       const bool live = st.x != -INFINITY;  // dead rows: P = 0
       const float2 c2 = make_float2(c, c), l2 = make_float2(st.x, st.x), d2 = make_float2(st.y, st.y);
       // A thread's 64 keys go in two chunks; the loads of the next one are in flight during this one's exponentials.
-      uint32_t s0[32], d0[32], s1[32], d1[32];
-      auto load = [&](int tile, int chunk, uint32_t (&s)[32], uint32_t (&d)[32]) {
-        tmem_ld_async(lanes + C::DP_COL + half * 64 + 32 * chunk, d);
-        tmem_ld_async(lanes + C::S_COL + (tile & 1) * 128 + half * 64 + 32 * chunk, s);
+      uint32_t s0[C::CH], d0[C::CH], s1[C::CH], d1[C::CH];
+      auto load = [&](int tile, int chunk, uint32_t (&s)[C::CH], uint32_t (&d)[C::CH]) {
+        tmem_ld_async(lanes + C::DP_COL + half * C::HALF + C::CH * chunk, d);
+        tmem_ld_async(lanes + C::S_COL + (tile % C::SB) * C::BN + half * C::HALF + C::CH * chunk, s);
       };
       // dS of one chunk from its scores and dP, stored over the scores.
-      auto chunk_ds = [&](int t, int chunk, bool edge, uint32_t (&s)[32], uint32_t (&d)[32]) {
+      auto chunk_ds = [&](int t, int chunk, bool edge, uint32_t (&s)[C::CH], uint32_t (&d)[C::CH]) {
         if (edge) {
-          // Masked keys: P = exp(-inf) = 0 and dP = D, so dS = 0 whatever the keys hold.
-          const int j0 = t * C::BN + half * 64 + 32 * chunk;
+          // Masked keys: P = exp(-inf) = 0, so dS = 0; behind a length, where V may hold NaN, dP is set aside too.
+          const int left = limit - (t * C::BN + half * C::HALF + C::CH * chunk);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (j0 + e >= limit) s[e] = __float_as_uint(-INFINITY), d[e] = __float_as_uint(-st.y);
+          for (int e = 0; e < C::CH; ++e)
+            if (e >= left) s[e] = __float_as_uint(-INFINITY);
+          if (a.k_lens) {
+#pragma unroll
+            for (int e = 0; e < C::CH; ++e)
+              if (e >= left) d[e] = 0;
+          }
         }
-        uint32_t w[16];
+        uint32_t w[C::CH / 2];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < C::CH / 2; ++e) {
           const float2 x = ub::fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, l2);
           const float2 p = make_float2(ex2(x.x), ex2(x.y));
           const float2 ds = mul2(p, add2(make_float2(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1])), d2));
           w[e] = pack2<T>(ds.x, ds.y);
         }
-        tmem_st16(lanes + C::S_COL + (g & 1) * 128 + half * 64 + 32 * chunk, w);
+        const uint32_t to = lanes + C::S_COL + (g % C::SB) * C::BN + half * C::HALF + C::CH * chunk;
+        if constexpr (C::CH == 32)
+          tmem_st16(to, w);
+        else
+          tmem_st8(to, w);
       };
       if (!C::EARLY && t0 < t1) {
         if (!__all_sync(0xffffffffu, mbar_wait(dp_full, g & 1))) {
@@ -938,8 +978,8 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
         if (C::EARLY) chunk_ds(t, 0, edge, s0, d0);
         // Keys behind the length (NaN included) must be 0 before dS K; S, which also reads them, is complete.
         if (edge && a.k_lens && t * C::BN + C::BN > b.kl && half == 0) {
-          if (t * C::BN + row >= b.kl)
-            clear_row(ring + ((it + 2 * (t - t0)) % C::STAGES) * C::TILE_BYTES, 128, C::NB, row);
+          if (row < C::BN && t * C::BN + row >= b.kl)
+            clear_row(ring + ((it + 2 * (t - t0)) % C::STAGES) * C::TILE_BYTES, C::BN, C::NB, row);
           fence_proxy_async_smem();
         }
         chunk_ds(t, 1, edge, s1, d1);
@@ -1007,22 +1047,24 @@ __global__ void __launch_bounds__(DqCfg<HD>::THREADS, 1)
 // each. lse and D go by column here: a warp brings them to shared memory, and rows that must not count come with
 // -lse = -inf, P = 0. P^T and dS^T of a thread share the columns of its scores.
 
-template <int HD>
+template <int HD, bool SHORT>
 struct DkvCfg {
-  static constexpr int BN = HD == 64 ? 128 : 64;
+  static constexpr int BN = HD == 64 && !SHORT ? 128 : 64;
   static constexpr int NB = HD / 64;
   static constexpr int KV_BYTES = 128 * 128 * NB;
   static constexpr int TILE_BYTES = BN * 128 * NB;  // Q or dO: 16 KB
-  static constexpr int STAGES = 4;                  // (Q, dO) pairs
+  static constexpr int STAGES = SHORT ? 2 : 4;                  // (Q, dO) pairs
   static constexpr int STATS = 4;                   // (lse, D) rows
   static constexpr int SMEM = 2 * KV_BYTES + 2 * STAGES * TILE_BYTES + STATS * BN * 8 + 1024 + 512;
   static constexpr int THREADS = 384;  // two warpgroups of keys, one for TMA, MMA issue and lse / D
   static constexpr int REGS_MORE = 208, REGS_LESS = 88;  // 2 x 208 + 88 = 3 x 168
   static constexpr int HALF = BN / 2;  // queries of a tile per thread
   static constexpr int CH = HALF / 2;  // taken at once
-  static constexpr int S_COL = 0, DP_COL = 2 * BN, DV_COL = 3 * BN, DK_COL = 3 * BN + HD, TMEM = 512;
-  static_assert(3 * BN + 2 * HD <= 512, "TMEM columns");
-  static constexpr bool EARLY = HD > 64;  // as in the dq kernel
+  static constexpr int SB = SHORT ? 1 : 2;  // S buffers
+  static constexpr int S_COL = 0, DP_COL = SB * BN, DV_COL = (SB + 1) * BN, DK_COL = DV_COL + HD;
+  static constexpr int TMEM = SHORT ? 256 : 512;
+  static_assert(DK_COL + HD <= TMEM, "TMEM columns");
+  static constexpr bool EARLY = HD > 64 || SHORT;  // as in the dq kernel
 };
 
 // P of fp16 calls is kept times 2^12: probabilities of long rows would sink into fp16's subnormals.
@@ -1035,12 +1077,12 @@ __device__ __forceinline__ constexpr float p_shift<__half>() {
   return 12.f;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
+template <typename T, int HD, bool SHORT>
+__global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
     attention_dkv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                             const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mdo,
                             const __grid_constant__ TcArgs ta) {
-  using C = DkvCfg<HD>;
+  using C = DkvCfg<HD, SHORT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sK = smem;
@@ -1152,7 +1194,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         auto issue_s = [&](int i) {
           if (!mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1)) return false;
           tc_fence_after();
-          if (elect_one()) mma_heads<HD>(tmem + C::S_COL + (i & 1) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
+          if (elect_one()) mma_heads<HD>(tmem + C::S_COL + (i % C::SB) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
           __syncwarp();
           return true;
         };
@@ -1182,7 +1224,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
             break;
           }
           for (int t = 0; t < n; ++t) {
-            if (t + 1 < n && (!issue_s(g + t + 1) || !issue_dp(g + t + 1, t + 2 == n))) {
+            if (C::SB == 2 && t + 1 < n && (!issue_s(g + t + 1) || !issue_dp(g + t + 1, t + 2 == n))) {
               ok = false;
               break;
             }
@@ -1191,7 +1233,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
               break;
             }
             tc_fence_after();
-            const uint32_t p = tmem + C::S_COL + ((g + t) & 1) * C::BN, q = q_tile(g + t);
+            const uint32_t p = tmem + C::S_COL + ((g + t) % C::SB) * C::BN, q = q_tile(g + t);
             // The chunk of K step ks (16 queries, 8 columns): P in its first half, dS in its second.
             constexpr int KC = C::CH / 16;
             auto p_col = [&](int ks) { return p + (ks / KC) * C::CH + (ks % KC) * 8; };
@@ -1203,6 +1245,10 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
               if (t + 1 == n) umma_commit(acc_done);
             }
             __syncwarp();
+            if (C::SB == 1 && t + 1 < n && (!issue_s(g + t + 1) || !issue_dp(g + t + 1, t + 2 == n))) {
+              ok = false;
+              break;
+            }
           }
           if (!ok) break;
           g += n;
@@ -1277,7 +1323,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
       uint32_t s0[C::CH], d0[C::CH], s1[C::CH], d1[C::CH];
       auto load = [&](int tile, int chunk, uint32_t (&s)[C::CH], uint32_t (&d)[C::CH]) {
         tmem_ld_async(lanes + C::DP_COL + half * C::HALF + C::CH * chunk, d);
-        tmem_ld_async(lanes + C::S_COL + (tile & 1) * C::BN + half * C::HALF + C::CH * chunk, s);
+        tmem_ld_async(lanes + C::S_COL + (tile % C::SB) * C::BN + half * C::HALF + C::CH * chunk, s);
       };
       auto arrived = [&](int tile) {  // S, dP and the row statistics of a tile
         return __all_sync(0xffffffffu, mbar_wait(&st_full[tile % C::STATS], (tile / C::STATS) & 1) &&
@@ -1290,9 +1336,10 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
         const float4* l4 = reinterpret_cast<const float4*>(row_stats);
         const float4* d4 = reinterpret_cast<const float4*>(row_stats + C::BN);
         if (edge) {
+          const int lo = from - i0 - col, hi = b.ql - i0 - col;
 #pragma unroll
           for (int e = 0; e < C::CH; ++e)
-            if (i0 + col + e < from || i0 + col + e >= b.ql) s[e] = __float_as_uint(-INFINITY), d[e] = 0;
+            if (e < lo || e >= hi) s[e] = __float_as_uint(-INFINITY), d[e] = 0;
         }
         uint32_t w[C::CH];  // P, then dS
 #pragma unroll
@@ -1315,7 +1362,7 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
           w[C::CH / 2 + 2 * e] = pack2<T>(ga.x, ga.y);
           w[C::CH / 2 + 2 * e + 1] = pack2<T>(gb.x, gb.y);
         }
-        const uint32_t to = lanes + C::S_COL + (g & 1) * C::BN + col;
+        const uint32_t to = lanes + C::S_COL + (g % C::SB) * C::BN + col;
         if constexpr (C::CH == 32)
           tmem_st32(to, w);
         else
@@ -1332,7 +1379,8 @@ __global__ void __launch_bounds__(DkvCfg<HD>::THREADS, 1)
       }
       for (int t = t0; t < t1; ++t, ++g, w.next()) {
         const int i0 = (begin + w.tile) * C::BN;
-        const bool edge = i0 + C::BN > b.ql || i0 < first || (a.causal && j0 + ROWS - 1 > i0 + b.off);
+        // Queries past the tensor need no mask: their rows were read as 0 and come with -lse = -inf.
+        const bool edge = (a.q_lens && i0 + C::BN > b.ql) || i0 < first || (a.causal && j0 + ROWS - 1 > i0 + b.off);
         if (C::EARLY) {
           if (!arrived(g)) {
             ok = false;
@@ -1483,17 +1531,17 @@ TcArgs tc_args(const AttnArgs& a, const UnblendAttnTrainParams& p, int heads, in
 
 int grid_of(int units, int per_sm) { return units < per_sm * ub::kNumSMs ? units : per_sm * ub::kNumSMs; }
 
-template <typename T, int HD, int NQ>
+template <typename T, int HD, int NQ, bool SHORT>
 int launch_fwd(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, cudaStream_t st) {
-  using C = FwdCfg<HD, NQ>;
+  using C = FwdCfg<HD, NQ, SHORT>;
   CUtensorMap mq, mk, mv;
-  if (!head_map(&mq, a.q, p.q, p, p.heads, p.lq, 128) || !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, 128) ||
-      !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, 128))
+  if (!head_map(&mq, a.q, p.q, p, p.heads, p.lq, 128) || !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, C::BN) ||
+      !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, C::BN))
     return UNBLEND_ERR_INVALID;
   const TcArgs t = tc_args(a, p, p.heads, p.lq, NQ * ROWS, splits, a.part);
-  constexpr auto kern = attention_fwd_tc_kernel<T, HD, NQ>;
+  constexpr auto kern = attention_fwd_tc_kernel<T, HD, NQ, SHORT>;
   if (allow_smem<kern>(C::SMEM) != cudaSuccess) return (int)cudaGetLastError();
-  kern<<<grid_of(t.units, NQ == 2 ? 1 : 2), C::THREADS, C::SMEM, st>>>(mq, mk, mv, t);
+  kern<<<grid_of(t.units, C::PER_SM), C::THREADS, C::SMEM, st>>>(mq, mk, mv, t);
   UB_CHECK_LAUNCH();
   return 0;
 }
@@ -1513,30 +1561,30 @@ int launch_stats(const AttnArgs& a, cudaStream_t st) {
   return 0;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool SHORT>
 int launch_dq(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st) {
-  using C = DqCfg<HD>;
+  using C = DqCfg<HD, SHORT>;
   CUtensorMap mq, mdo, mk, mv;
   if (!head_map(&mq, a.q, p.q, p, p.heads, p.lq, 128) || !head_map(&mdo, a.dout, p.dout, p, p.heads, p.lq, 128) ||
-      !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, 128) || !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, 128))
+      !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, C::BN) || !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, C::BN))
     return UNBLEND_ERR_INVALID;
   const TcArgs t = tc_args(a, p, p.heads, p.lq, ROWS, splits, part);
-  constexpr auto kern = attention_dq_tc_kernel<T, HD>;
+  constexpr auto kern = attention_dq_tc_kernel<T, HD, SHORT>;
   if (allow_smem<kern>(C::SMEM) != cudaSuccess) return (int)cudaGetLastError();
   kern<<<grid_of(t.units, 1), C::THREADS, C::SMEM, st>>>(mq, mdo, mk, mv, t);
   UB_CHECK_LAUNCH();
   return 0;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool SHORT>
 int launch_dkv(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st) {
-  using C = DkvCfg<HD>;
+  using C = DkvCfg<HD, SHORT>;
   CUtensorMap mq, mdo, mk, mv;
   if (!head_map(&mq, a.q, p.q, p, p.heads, p.lq, C::BN) || !head_map(&mdo, a.dout, p.dout, p, p.heads, p.lq, C::BN) ||
       !head_map(&mk, a.k, p.k, p, p.kv_heads, p.lk, 128) || !head_map(&mv, a.v, p.v, p, p.kv_heads, p.lk, 128))
     return UNBLEND_ERR_INVALID;
   const TcArgs t = tc_args(a, p, p.kv_heads, p.lk, ROWS, splits, part);
-  constexpr auto kern = attention_dkv_tc_kernel<T, HD>;
+  constexpr auto kern = attention_dkv_tc_kernel<T, HD, SHORT>;
   if (allow_smem<kern>(C::SMEM) != cudaSuccess) return (int)cudaGetLastError();
   kern<<<grid_of(t.units, 1), C::THREADS, C::SMEM, st>>>(mk, mv, mq, mdo, t);
   UB_CHECK_LAUNCH();
@@ -1548,32 +1596,43 @@ int launch_dkv(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, f
 namespace ub {
 namespace train {
 
-int attention_fwd_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int rows_per_cta, cudaStream_t st) {
-  auto go = [&](auto zero) {
-    using T = decltype(zero);
-    if (rows_per_cta == 256)
-      return p.hd <= 64 ? launch_fwd<T, 64, 2>(a, p, a.splits, st) : launch_fwd<T, 128, 2>(a, p, a.splits, st);
-    return p.hd <= 64 ? launch_fwd<T, 64, 1>(a, p, a.splits, st) : launch_fwd<T, 128, 1>(a, p, a.splits, st);
-  };
+template <typename F>
+int by_type(const UnblendAttnTrainParams& p, F go) {
   return p.dtype == UNBLEND_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
 
 int attention_stats_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, cudaStream_t st) {
-  return p.dtype == UNBLEND_BF16 ? launch_stats<__nv_bfloat16>(a, st) : launch_stats<__half>(a, st);
+  return by_type(p, [&](auto x) { return launch_stats<decltype(x)>(a, st); });
+}
+
+int attention_fwd_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int rows_per_cta, cudaStream_t st) {
+  return by_type(p, [&](auto x) {
+    using T = decltype(x);
+    if (p.hd <= 64 && p.lk <= SHORT_ROWS) return launch_fwd<T, 64, 1, true>(a, p, a.splits, st);
+    if (rows_per_cta == 256)
+      return p.hd <= 64 ? launch_fwd<T, 64, 2, false>(a, p, a.splits, st)
+                        : launch_fwd<T, 128, 2, false>(a, p, a.splits, st);
+    return p.hd <= 64 ? launch_fwd<T, 64, 1, false>(a, p, a.splits, st)
+                      : launch_fwd<T, 128, 1, false>(a, p, a.splits, st);
+  });
 }
 
 int attention_dq_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st) {
-  if (p.dtype == UNBLEND_BF16)
-    return p.hd <= 64 ? launch_dq<__nv_bfloat16, 64>(a, p, splits, part, st)
-                      : launch_dq<__nv_bfloat16, 128>(a, p, splits, part, st);
-  return p.hd <= 64 ? launch_dq<__half, 64>(a, p, splits, part, st) : launch_dq<__half, 128>(a, p, splits, part, st);
+  return by_type(p, [&](auto x) {
+    using T = decltype(x);
+    if (p.hd > 64) return launch_dq<T, 128, false>(a, p, splits, part, st);
+    return p.lk <= SHORT_ROWS ? launch_dq<T, 64, true>(a, p, splits, part, st)
+                              : launch_dq<T, 64, false>(a, p, splits, part, st);
+  });
 }
 
 int attention_dkv_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st) {
-  if (p.dtype == UNBLEND_BF16)
-    return p.hd <= 64 ? launch_dkv<__nv_bfloat16, 64>(a, p, splits, part, st)
-                      : launch_dkv<__nv_bfloat16, 128>(a, p, splits, part, st);
-  return p.hd <= 64 ? launch_dkv<__half, 64>(a, p, splits, part, st) : launch_dkv<__half, 128>(a, p, splits, part, st);
+  return by_type(p, [&](auto x) {
+    using T = decltype(x);
+    if (p.hd > 64) return launch_dkv<T, 128, false>(a, p, splits, part, st);
+    return p.lq <= SHORT_ROWS ? launch_dkv<T, 64, true>(a, p, splits, part, st)
+                              : launch_dkv<T, 64, false>(a, p, splits, part, st);
+  });
 }
 
 // What the tensor-core kernels can address: 16-byte rows and strides (TMA, vector stores), a positive scale (the row
