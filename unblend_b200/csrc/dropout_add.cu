@@ -9,9 +9,17 @@
 // captured graph can be replayed with new ones. A dropped element is selected away, not multiplied by 0: infinities
 // and NaN in it leave no trace.
 //
-// Bound: HBM while a block of four words (10 rounds of two 32 x 32 -> 64 bit products) is spread over the bytes of
-// four elements; the products are the second limit, close behind for all-16-bit tensors.
+// Bound: HBM for fp32; for 16-bit tensors the instructions are the second limit, close behind (a block of four words is
+// 10 rounds of two 32 x 32 -> 64 bit products, and only 4 to 10 bytes per element hide it). Measured, 86016 x 512 with
+// all gradients: fp32 72 us forward (7.3 TB/s), 94 us backward (5.6); bf16 on an fp32 stream 84 us (5.2 TB/s) and 78 us
+// (4.5); all bf16 74 us (3.6) and 79 us (3.3).
+//
+// Three kernels. Contiguous tensors on 16-byte boundaries, whatever their width, are one run of 16-byte chunks (flat).
+// Strided rows that are whole 16-byte chunks keep those (vector), and all others are read element by element with the
+// words shared by ballots (any). Both sides at 50000 x 1001, bf16 on an fp32 stream: flat 98 us forward and 89 us
+// backward, any 183 and 286 us; at 86016 x 512 backward: flat 78 us, vector 122 us.
 #include <cmath>
+#include <type_traits>
 
 #include "train_common.cuh"
 
@@ -54,8 +62,8 @@ __device__ __forceinline__ Words philox(unsigned long long seed, unsigned long l
   return Words{{c0, c1, c2, c3}};
 }
 
-// Columns in runs of VEC (a multiple of 4, so a run is whole word blocks): thread (tx, ty) keeps its columns and walks
-// the rows blockIdx.y * TY + ty + k * gridDim.y * TY.
+// Strided rows, columns in runs of VEC (a multiple of 4, so a run is whole word blocks): thread (tx, ty) keeps its
+// columns and walks the rows blockIdx.y * TY + ty + k * gridDim.y * TY.
 template <typename T, typename TR, typename TW, int VEC, bool BWD, bool SUMS>
 __global__ void __launch_bounds__(256) dropout_add_vec_kernel(const __grid_constant__ DropArgs a) {
   extern __shared__ float red[];  // [TY][TX * VEC] of the backward sums
@@ -88,7 +96,7 @@ __global__ void __launch_bounds__(256) dropout_add_vec_kernel(const __grid_const
             if (SUMS) ds[i] += keep ? d * x[i] : 0.f;
           } else {
             const float v = keep ? s[i] * (x[i] * a.inv_keep) : 0.f;
-            o[i] = BWD || a.r ? r[i] + v : v;
+            o[i] = a.r ? r[i] + v : v;
           }
         }
       }
@@ -174,9 +182,102 @@ __global__ void __launch_bounds__(256) dropout_add_any_kernel(const __grid_const
   }
 }
 
+// Contiguous tensors of any width, as one run of 16-byte chunks: T = cols * m threads take chunk t, t + T, ..., and as
+// T chunks are whole rows, a thread's columns stay the same. Its sums are then entries t * VEC ... of a [VEC * m][cols]
+// array of partial sums as they are; where a CTA's entries cover each column twice or more it adds those and leaves one
+// row.
+constexpr bool flat_joins(int cols, int vec) { return 2 * cols <= 256 * vec; }
+
+template <typename T, typename TR, typename TW, bool BWD, bool SUMS>
+__global__ void __launch_bounds__(256) dropout_add_flat_kernel(const __grid_constant__ DropArgs a, int threads) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (!SUMS && t >= threads) return;
+  const unsigned long long seed = a.rng[0], offset = a.rng[1];
+  const bool any = !a.drop_all;
+  const long long n = (long long)a.rows * a.cols, step = (long long)threads * VEC;
+  float s[VEC], ds[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    s[i] = a.scale ? to_f(static_cast<const TW*>(a.scale)[((long long)t * VEC + i) % a.cols]) : 1.f;
+    ds[i] = 0.f;
+  }
+  for (long long e = t < threads ? (long long)t * VEC : n; e < n; e += step) {
+    float x[VEC], r[VEC], o[VEC];
+    const bool whole = e + VEC <= n;
+    if (whole) {
+      if (!BWD || SUMS) load_vec<T, VEC>(static_cast<const T*>(a.x) + e, x);
+      if (BWD || a.r) load_vec<TR, VEC>(static_cast<const TR*>(a.r) + e, r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        x[i] = (!BWD || SUMS) && e + i < n ? to_f(static_cast<const T*>(a.x)[e + i]) : 0.f;
+        r[i] = (BWD || a.r) && e + i < n ? to_f(static_cast<const TR*>(a.r)[e + i]) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < VEC / 4; ++b) {
+      const Words w = philox(seed, offset, (unsigned long long)(e >> 2) + b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = b * 4 + j;
+        const bool keep = any && w.w[j] >= a.threshold;
+        if constexpr (BWD) {
+          const float d = keep ? r[i] * a.inv_keep : 0.f;
+          o[i] = s[i] * d;
+          if (SUMS) ds[i] += keep ? d * x[i] : 0.f;
+        } else {
+          const float v = keep ? s[i] * (x[i] * a.inv_keep) : 0.f;
+          o[i] = a.r ? r[i] + v : v;
+        }
+      }
+    }
+    using TO = typename std::conditional<BWD, T, TR>::type;
+    TO* out = static_cast<TO*>(a.out) + e;
+    if (whole) {
+      store_vec<TO, VEC>(out, o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (e + i < n) out[i] = from_f<TO>(o[i]);
+    }
+  }
+  if constexpr (SUMS) {
+    if (!flat_joins(a.cols, VEC)) {
+      if (t < threads) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) a.part[(long long)t * VEC + i] = ds[i];
+      }
+      return;
+    }
+    __shared__ float sums[256 * VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sums[threadIdx.x * VEC + i] = ds[i];
+    __syncthreads();
+    const int first = (int)((long long)blockIdx.x * 256 * VEC % a.cols);  // column of entry 0
+    for (int c = threadIdx.x; c < a.cols; c += 256) {
+      float v = 0.f;
+      for (int e = c >= first ? c - first : c - first + a.cols; e < 256 * VEC; e += a.cols) v += sums[e];
+      a.part[(long long)blockIdx.x * a.cols + c] = v;
+    }
+  }
+}
+
+enum Path { ANY, VECTOR, FLAT };
+
 struct Shape {
   dim3 grid, block;
 };
+
+// m of the flat kernel, no more than the rows need. Without sums about eight CTAs per SM (fp32 86016 x 512 backward:
+// 67 us, with four 81 us; bf16 74 and 76 us); with sums four, as each CTA leaves partial sums.
+constexpr int FLAT_CTAS = 8, FLAT_SUM_CTAS = 4;
+
+long long flat_runs(long long rows, int cols, int vec, int ctas_per_sm) {
+  const long long fill = ctas_per_sm * 256LL * ub::kNumSMs / cols, need = (rows + vec - 1) / vec;
+  const long long m = fill < need ? fill : need;
+  return m < 1 ? 1 : m;
+}
 
 // Row CTAs: enough to fill the GPU, at most one per `rows_per_cta` rows; the backward partial sums have one row each.
 unsigned row_ctas(long long rows, int rows_per_cta, unsigned col_ctas, int per_sm) {
@@ -204,10 +305,18 @@ Shape any_shape(long long rows, int cols) {
 }
 
 template <typename T, typename TR, typename TW, bool BWD>
-int launch_types(const DropArgs& a, bool vec, int* parts, cudaStream_t st) {
-  // 16-bit: 8 elements per thread forward; 4 backward, where the sums' registers cost more than the wider access wins.
-  constexpr int VEC = sizeof(T) == 2 && !BWD ? 8 : 4;
-  if (vec) {
+int launch_types(const DropArgs& a, Path path, int* parts, cudaStream_t st) {
+  constexpr int VEC = sizeof(T) == 2 ? 8 : 4;
+  if (path == FLAT) {
+    const long long m = flat_runs(a.rows, a.cols, VEC, BWD && a.part ? FLAT_SUM_CTAS : FLAT_CTAS);
+    const int threads = (int)(m * a.cols);
+    const unsigned grid = (threads + 255) / 256;
+    if (BWD && a.part)
+      dropout_add_flat_kernel<T, TR, TW, BWD, BWD><<<grid, 256, 0, st>>>(a, threads);
+    else
+      dropout_add_flat_kernel<T, TR, TW, BWD, false><<<grid, 256, 0, st>>>(a, threads);
+    *parts = flat_joins(a.cols, VEC) ? (int)grid : (int)(m * VEC);
+  } else if (path == VECTOR) {
     const Shape s = vec_shape(a.rows, a.cols, VEC);
     if (BWD && a.part)
       dropout_add_vec_kernel<T, TR, TW, VEC, BWD, BWD>
@@ -225,20 +334,25 @@ int launch_types(const DropArgs& a, bool vec, int* parts, cudaStream_t st) {
 }
 
 template <typename T, bool BWD>
-int launch_streams(const DropArgs& a, int dtype, int r_dtype, int w_dtype, bool vec, int* parts, cudaStream_t st) {
+int launch_streams(const DropArgs& a, int r_dtype, int w_dtype, Path path, int* parts, cudaStream_t st) {
   if (r_dtype == UNBLEND_F32) {
-    if (w_dtype == UNBLEND_F32) return launch_types<T, float, float, BWD>(a, vec, parts, st);
-    return launch_types<T, float, T, BWD>(a, vec, parts, st);
+    if (w_dtype == UNBLEND_F32) return launch_types<T, float, float, BWD>(a, path, parts, st);
+    return launch_types<T, float, T, BWD>(a, path, parts, st);
   }
-  if (w_dtype == UNBLEND_F32) return launch_types<T, T, float, BWD>(a, vec, parts, st);
-  return launch_types<T, T, T, BWD>(a, vec, parts, st);
+  if (w_dtype == UNBLEND_F32) return launch_types<T, T, float, BWD>(a, path, parts, st);
+  return launch_types<T, T, T, BWD>(a, path, parts, st);
 }
 
 template <bool BWD>
-int launch(const DropArgs& a, int dtype, int r_dtype, int w_dtype, bool vec, int* parts, cudaStream_t st) {
-  if (dtype == UNBLEND_F32) return launch_types<float, float, float, BWD>(a, vec, parts, st);
-  if (dtype == UNBLEND_BF16) return launch_streams<__nv_bfloat16, BWD>(a, dtype, r_dtype, w_dtype, vec, parts, st);
-  return launch_streams<__half, BWD>(a, dtype, r_dtype, w_dtype, vec, parts, st);
+int launch(const DropArgs& a, int dtype, int r_dtype, int w_dtype, Path path, int* parts, cudaStream_t st) {
+  if (dtype == UNBLEND_F32) return launch_types<float, float, float, BWD>(a, path, parts, st);
+  if (dtype == UNBLEND_BF16) return launch_streams<__nv_bfloat16, BWD>(a, r_dtype, w_dtype, path, parts, st);
+  return launch_streams<__half, BWD>(a, r_dtype, w_dtype, path, parts, st);
+}
+
+// One run of values; small enough for the flat kernel's 32-bit thread numbers.
+bool contiguous(const RowMap& m, long long outer, int cols) {
+  return (m.inner <= 1 || m.si == cols) && (outer <= 1 || m.so == (long long)m.inner * cols) && cols <= (1 << 26);
 }
 
 void set_p(DropArgs* a, double p) {
@@ -252,11 +366,17 @@ void set_p(DropArgs* a, double p) {
 
 extern "C" int unblend_dropout_add_grad_workspace(long long rows, int cols, long long* bytes) {
   UB_REQUIRE(bytes && rows_ok(1, rows, cols));
-  // The larger of the two layouts (which of them runs depends on the pointers' alignment).
+  // The largest of the layouts (which of them runs depends on the pointers' alignment).
   unsigned parts = any_shape(rows, cols).grid.y;
-  if (cols % 4 == 0) {
-    const unsigned v = vec_shape(rows, cols, 4).grid.y;
-    parts = v > parts ? v : parts;
+  for (int vec = 4; vec <= 8; vec += 4)
+    if (cols % vec == 0) {
+      const unsigned v = vec_shape(rows, cols, vec).grid.y;
+      parts = v > parts ? v : parts;
+    }
+  for (int vec = 4; vec <= 8; vec += 4) {
+    const long long m = flat_runs(rows, cols, vec, FLAT_SUM_CTAS);
+    const long long v = flat_joins(cols, vec) ? (m * cols + 255) / 256 : m * vec;
+    parts = v > parts ? (unsigned)v : parts;
   }
   *bytes = (long long)parts * cols * (long long)sizeof(float);
   return 0;
@@ -284,8 +404,11 @@ extern "C" int unblend_dropout_add_forward(const void* x, long long x_so, long l
   const int vec_n = dtype == UNBLEND_F32 ? 4 : 8;
   const bool vec = cols % vec_n == 0 && rows_aligned(x, a.xm, outer, elem_size(dtype), 16) && aligned16(y) &&
                    aligned16(scale) && (!residual || rows_aligned(residual, a.rm, outer, elem_size(r_dtype), 16));
+  const bool flat = aligned16(x) && aligned16(y) && contiguous(a.xm, outer, cols) &&
+                    (!residual || (aligned16(residual) && contiguous(a.rm, outer, cols)));
+  const Path path = flat ? FLAT : vec ? VECTOR : ANY;
   int parts = 0;
-  return launch<false>(a, dtype, r_dtype, w_dtype, vec, &parts, ub::as_stream(stream));
+  return launch<false>(a, dtype, r_dtype, w_dtype, path, &parts, ub::as_stream(stream));
 }
 
 extern "C" int unblend_dropout_add_backward(const void* dy, long long dy_so, long long dy_si, const void* x,
@@ -309,11 +432,15 @@ extern "C" int unblend_dropout_add_backward(const void* dy, long long dy_so, lon
   a.rows = (unsigned)(outer * inner);
   a.cols = cols;
   set_p(&a, p);
-  const bool vec = cols % 4 == 0 && (!dscale || rows_aligned(x, a.xm, outer, elem_size(dtype), 16)) &&
+  const int vec_n = dtype == UNBLEND_F32 ? 4 : 8;
+  const bool vec = cols % vec_n == 0 && (!dscale || rows_aligned(x, a.xm, outer, elem_size(dtype), 16)) &&
                    aligned16(dx) && aligned16(scale) && rows_aligned(dy, a.rm, outer, elem_size(dy_dtype), 16);
+  const bool flat = aligned16(dy) && aligned16(dx) && contiguous(a.rm, outer, cols) &&
+                    (!dscale || (aligned16(x) && contiguous(a.xm, outer, cols)));
+  const Path path = flat ? FLAT : vec ? VECTOR : ANY;
   cudaStream_t st = ub::as_stream(stream);
   int parts = 0;
-  const int rc = launch<true>(a, dtype, dy_dtype, w_dtype, vec, &parts, st);
+  const int rc = launch<true>(a, dtype, dy_dtype, w_dtype, path, &parts, st);
   if (rc || !dscale) return rc;
   if (w_dtype == UNBLEND_F32) return launch_column_sums<float>(work, parts, cols, 1, dscale, nullptr, st);
   if (w_dtype == UNBLEND_BF16) return launch_column_sums<__nv_bfloat16>(work, parts, cols, 1, dscale, nullptr, st);
