@@ -283,10 +283,10 @@ def check(name: str, rc: int) -> None:
 
 
 # Kernels launched by one call of each entry point (1 unless listed).
-# The joins of split attention calls depend on the sizes and are not counted.
+# Attention calls can launch more (joins of split axes, one kernel per gradient): that depends on the sizes and is not
+# counted.
 KERNELS_PER_CALL = {"unblend_mean_std": 3, "unblend_istft_output": 2, "unblend_istft_masked": 2,
-                    "unblend_layer_norm_backward": 2, "unblend_dropout_add_backward": 2,
-                    "unblend_attention_backward": 3}
+                    "unblend_layer_norm_backward": 2, "unblend_dropout_add_backward": 2}
 
 # Launch accounting: total kernels launched through this binding.
 counters = {"launches": 0}

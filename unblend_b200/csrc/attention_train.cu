@@ -13,6 +13,7 @@
 // The kernels here take every type, stride and alignment, and are the path of fp32: 64 x 64 score tiles on 256
 // threads, 4 x 4 scores per thread, operands in shared memory as fp32 (transposed where the head axis is summed).
 #include "attention_train.cuh"
+#include "warp_mma.cuh"
 
 namespace {
 
@@ -597,43 +598,6 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_kernel(const __grid_cons
 constexpr int MMA_ROWS = 16, MMA_STAGES = 3;
 constexpr int few_mma_smem(int hd) { return (FEW_NT / 32) * MMA_STAGES * 2 * 16 * hd * 2; }
 
-__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
-               "r"(in ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const void* p) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"((uint32_t)__cvta_generic_to_shared(p))
-               : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], const void* p) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"((uint32_t)__cvta_generic_to_shared(p))
-               : "memory");
-}
-__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
-      "%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
-      "%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
-  const T v[2] = {from_f<T>(lo), from_f<T>(hi)};
-  return *reinterpret_cast<const uint32_t*>(v);
-}
-
 template <typename T, int HD>
 __global__ void __launch_bounds__(FEW_NT) attention_few_mma_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int WARPS = FEW_NT / 32, CHUNKS = HD / 8, TILE_E = 16 * HD;  // a K or V tile: 16 keys
@@ -827,8 +791,8 @@ int split_count(long long units, long long tiles, long long want) {
 long long div_up(long long a, long long b) { return (a + b - 1) / b; }
 long long round4(long long n) { return (n + 3) / 4 * 4; }
 
-// What a call runs on. A few rows per key/value head (forward): see attention_few_kernel.
-enum Path { CUDA_CORES = 0, TENSOR_CORES = 1, FEW = 2 };
+// What a call runs on. A few rows per key/value head (forward): see attention_few_kernel. SMALL: sequences of one tile.
+enum Path { CUDA_CORES = 0, TENSOR_CORES = 1, FEW = 2, SMALL = 3 };
 
 // Work division of a call.
 struct Plan {
@@ -846,6 +810,8 @@ Plan plan_of(const UnblendAttnTrainParams& p, Path path) {
   const long long sms = ub::kNumSMs, group = p.heads / p.kv_heads;
   n.q_rows = qh * p.lq;
   n.k_rows = kh * p.lk;
+  n.fwd_splits = n.dq_splits = n.dkv_splits = 1;
+  if (path == SMALL) return n;
   n.fwd_rows = (int)tile;
   if (tc && qh * div_up(p.lq, 256) >= sms && p.lq > 128) n.fwd_rows = 256;
   n.fwd_splits = n.fwd_rows == 256 ? 1 : split_count(qh * qt, kt, 2 * sms);
@@ -1009,6 +975,8 @@ int forward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Plan
   int rc;
   if (path == FEW)
     rc = few_types<T>(a, st);
+  else if (path == SMALL)
+    rc = attention_small_forward(a, p, st);
   else if (path == TENSOR_CORES)
     rc = attention_fwd_tc(a, p, n.fwd_rows, st);
   else
@@ -1072,8 +1040,9 @@ extern "C" int unblend_attention_forward(const void* q, const void* k, const voi
   const void* ptrs[] = {q, k, v, out};
   const UnblendHeadStrides strides[] = {p->q, p->k, p->v, p->out};
   const int heads[] = {p->heads, p->kv_heads, p->kv_heads, p->heads}, rows[] = {p->lq, p->lk, p->lk, p->lq};
-  const Path path = few_fits(*p, k, v) ? FEW
-                    : attention_tc_fits(*p, ptrs, strides, heads, rows, 4) ? TENSOR_CORES : CUDA_CORES;
+  Path path = few_fits(*p, k, v) ? FEW
+              : attention_tc_fits(*p, ptrs, strides, heads, rows, 4) ? TENSOR_CORES : CUDA_CORES;
+  if (path == TENSOR_CORES && attention_is_small(*p, false)) path = SMALL;
   const Plan n = plan_of(*p, path);
   AttnArgs a = args_of(*p);
   a.q = q;
@@ -1118,6 +1087,7 @@ extern "C" int unblend_attention_backward(const void* dout, const void* q, const
   a.dsum = static_cast<float*>(work);
   float* parts = a.dsum + round4(2 * n.q_rows);
   cudaStream_t st = ub::as_stream(stream);
+  if (tc && attention_is_small(*p, true)) return attention_small_backward(a, *p, st);
   const bool vec = p->hd % 4 == 0 && vec4_ok(q, p->q, *p) && vec4_ok(k, p->k, *p) && vec4_ok(v, p->v, *p) &&
                    vec4_ok(dout, p->dout, *p);
   if (p->dtype == UNBLEND_F32) return backward_types<float>(a, *p, n, parts, tc, vec, st);

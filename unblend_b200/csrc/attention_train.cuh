@@ -158,5 +158,10 @@ int attention_stats_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, cudaS
 int attention_dq_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st);
 int attention_dkv_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, float* part, cudaStream_t st);
 
+// Sequences of one tile (attention_train_small.cu), of calls that `attention_tc_fits`.
+bool attention_is_small(const UnblendAttnTrainParams& p, bool backward);
+int attention_small_forward(const AttnArgs& a, const UnblendAttnTrainParams& p, cudaStream_t st);
+int attention_small_backward(const AttnArgs& a, const UnblendAttnTrainParams& p, cudaStream_t st);
+
 }  // namespace train
 }  // namespace ub
