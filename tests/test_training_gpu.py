@@ -308,6 +308,45 @@ def test_attention_ragged(causal, hd, t):
 
 
 @pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("h,hk,hd", [(2, 2, 64), (4, 1, 64), (3, 3, 128), (4, 2, 128), (2, 1, 40), (3, 3, 72)])
+def test_attention_one_tile(h, hk, hd, t):
+    """Sequences of up to 64 queries and keys, which 16-bit types do in one kernel: lengths, layouts, empty rows."""
+    for lq, lk in ((17, 33), (64, 64), (62, 62), (63, 9), (33, 64), (16, 48)):
+        for causal in (False, True):
+            _attn_case(*_attn(lq, lk, h, hk, hd, t, seed=lq + hd), causal=causal)
+    # [outer, inner = bands, tokens]: rows, heads and sequences apart, and gaps between rows.
+    g = _gen(hd)
+    x = _rand(3, 50, 5, h + 2 * hk, hd + 8, g=g, t=t)[..., :hd].transpose(1, 2)
+    q, k, v = x.split((h, hk, hk), -2)
+    _attn_case(q, k, v, _rand(3, 50, 5, h, hd, g=g, t=t).transpose(1, 2), scale=0.2)
+    ql = torch.tensor([0, 1, 15, 16, 17, 64, 99, 40, 60, -3], device="cuda", dtype=torch.int32)
+    kl = torch.tensor([20, 0, 16, 64, 1, 63, 50, 9, 0, 60], device="cuda", dtype=torch.int32)
+    for causal in (False, True):
+        q, k, v, dout = _attn(60, 64, h, hk, hd, t, n=10)
+        for b in range(10):
+            a, c = min(max(int(ql[b]), 0), 60), min(max(int(kl[b]), 0), 64)
+            q[b, a:], dout[b, a:], k[b, c:], v[b, c:] = math.nan, math.inf, math.nan, math.inf
+            if c == 0 or (causal and a > c):  # queries that see no key
+                q[b, : a - c] = math.nan
+                dout[b, : a - c] = math.nan
+        got = _attn_case(q, k, v, dout, causal=causal, q_lens=ql, k_lens=kl)
+        for b in range(10):
+            a, c = min(max(int(ql[b]), 0), 60), min(max(int(kl[b]), 0), 64)
+            assert not got["out"][b, a:].any() and not got["dq"][b, a:].any()
+            assert not got["dk"][b, c:].any() and not got["dv"][b, c:].any()
+
+
+@pytest.mark.parametrize("t", [BF16, F16])
+def test_attention_one_tile_far_rows(t):
+    """Rows of a short sequence 2^24 and more elements apart."""
+    buf = torch.empty(40 * ((1 << 24) + 8), device="cuda", dtype=t)
+    for stride in ((1 << 24) - 8, 1 << 24):
+        q = buf.as_strided((1, 40, 2, 64), (0, stride, 64, 1))
+        q.copy_(_rand(1, 40, 2, 64, g=_gen(4), t=t))
+        _attn_case(q, q, q, q)
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
 def test_attention_layouts(t):
     """One packed projection, the two token axes of an axial model, rows that TMA cannot address, expanded heads."""
     g = _gen(8)

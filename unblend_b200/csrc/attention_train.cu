@@ -620,8 +620,8 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_mma_kernel(const __grid_
         const int id = x * 32 + lane, row = id / CHUNKS, c = id % CHUNKS, j = j0 + row;
         const bool in = j < end && 8 * c < a.hd;
         const int to = row * HD + ((c ^ (row & 7)) * 8);
-        cp_async16_or_zero(d + to, in ? k + (long long)j * a.k_s.row + 8 * c : k, in);
-        cp_async16_or_zero(d + TILE_E + to, in ? v + (long long)j * a.v_s.row + 8 * c : v, in);
+        cp_async16_or_zero(smem_at(d + to), in ? k + (long long)j * a.k_s.row + 8 * c : k, in);
+        cp_async16_or_zero(smem_at(d + TILE_E + to), in ? v + (long long)j * a.v_s.row + 8 * c : v, in);
       }
     }
     cp_commit();
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_mma_kernel(const __grid_
     for (int ks = 0; ks < HD / 16; ++ks) {
       const int row = (mi >> 1) * 8 + mr;
       uint32_t f[4];
-      ldmatrix4(f, tk + row * HD + (((2 * ks + (mi & 1)) ^ mr) * 8));
+      ldmatrix4(f, smem_at(tk + row * HD + (((2 * ks + (mi & 1)) ^ mr) * 8)));
       mma16(s[0], qf[ks], f[0], f[1], T());
       mma16(s[1], qf[ks], f[2], f[3], T());
     }
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_mma_kernel(const __grid_
     for (int d = 0; d < HD / 16; ++d) {
       const int row = (mi & 1) * 8 + mr;
       uint32_t f[4];
-      ldmatrix4_trans(f, tv + row * HD + (((2 * d + (mi >> 1)) ^ mr) * 8));
+      ldmatrix4_trans(f, smem_at(tv + row * HD + (((2 * d + (mi >> 1)) ^ mr) * 8)));
       mma16(o[2 * d], pf, f[0], f[1], T());
       mma16(o[2 * d + 1], pf, f[2], f[3], T());
     }

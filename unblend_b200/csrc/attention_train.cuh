@@ -56,6 +56,24 @@ __device__ __forceinline__ long long head_offset(const UnblendHeadStrides& s, co
   return (long long)o * s.outer + (long long)(seq - o * a.inner) * s.inner + (long long)h * s.head;
 }
 
+// n / d for n < 2^31 by a multiplication: with 2^s >= d and m = floor(2^(31 + s) / d) + 1, floor(n m / 2^(31 + s)) is
+// exact because n (m d - 2^(31 + s)) < 2^(31 + s). A hardware division takes a hundred cycles, which short
+// units of work do not hide.
+struct FastDiv {
+  uint32_t d, m, shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> shift); }
+};
+
+inline FastDiv fast_div(long long d) {
+  FastDiv f;
+  uint32_t s = 0;
+  while ((1LL << s) < d) ++s;
+  f.d = (uint32_t)d;
+  f.shift = 31 + s;
+  f.m = (uint32_t)((1ULL << f.shift) / (uint64_t)d + 1);
+  return f;
+}
+
 // Joins the forward parts of each row (at most 32): out = sum_s exp(lse_s - lse) out_s. W warps per row; lane s weighs
 // part s, warp w adds parts w, w + W, ... (at most 4) and the warps' sums are added in order: the loads of all parts are
 // in flight at once.

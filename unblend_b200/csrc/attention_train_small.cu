@@ -32,6 +32,19 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int ROWS = 64;  // of a tile
 constexpr int NT = 128;
 
+// CTAs per SM, which is what hides latency. Forward, head dim 64: 7 CTAs of 72 registers 38 us for 801 x 62 x 62 and 8
+// heads, 5 of 96 43 us, 8 of 64 (spills) 43 us. Backward: 4 CTAs of 128 registers 76 us; 5, with dS in V's place and 96
+// registers, 79 us. Two warps with 32 rows each, which load half the fragments, were slower in both directions (51 and
+// 101 us against 48 and 85 us of that version), and so was leaving out the products of 16-key blocks behind the
+// sequence (56 and 95 against 50 and 87 us: the branches kept loads and products from overlapping).
+constexpr int fwd_ctas(int hd) { return hd == 64 ? 7 : 4; }
+constexpr int bwd_ctas(int hd, bool grouped) { return hd == 64 ? (grouped ? 3 : 4) : 2; }
+
+struct SmallArgs {
+  AttnArgs a;
+  FastDiv by_heads, by_group, by_inner;  // by_heads: of the CTAs
+};
+
 constexpr int fwd_smem(int hd) { return 3 * ROWS * hd * 2; }
 constexpr int bwd_smem(int hd, bool grouped) { return ((grouped ? 5 : 4) * ROWS * hd + 2 * ROWS * ROWS) * 2; }
 
@@ -39,59 +52,6 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// Rows [0, valid) of one head by cp.async; the rest of the tile is 0.
-template <typename T, int HD>
-__device__ __forceinline__ void fetch(T* tile, const T* src, long long stride, int valid, int hd) {
-  constexpr int CH = HD / 8;
-#pragma unroll
-  for (int x = 0; x < ROWS * CH / NT; ++x) {
-    const int id = x * NT + threadIdx.x, row = id / CH, c = id % CH;
-    const bool in = row < valid && 8 * c < hd;
-    cp_async16_or_zero(tile + row * HD + ((c ^ (row & 7)) * 8), in ? src + row * stride + 8 * c : src, in);
-  }
-}
-
-// Address of a lane's row in ldmatrix: rows r0 .. r0 + 15 and chunks c, c + 1 of a tile, `down` of the four 8 x 8 blocks
-// first.
-template <typename T, int COLS>
-__device__ __forceinline__ const T* block(const T* tile, int r0, int c, bool down) {
-  const int lane = threadIdx.x & 31, m = lane >> 3, r = lane & 7;
-  const int row = r0 + (down ? m & 1 : m >> 1) * 8 + r;
-  return tile + row * COLS + (((c + (down ? m >> 1 : m & 1)) ^ r) * 8);
-}
-
-// d[16 x 64] = A[rows r0 ..][HD] B[64][HD]^T, both tiles as they lie.
-template <typename T, int HD>
-__device__ __forceinline__ void rows_dot(float (&d)[ROWS / 8][4], const T* ta, int r0, const T* tb) {
-#pragma unroll
-  for (int n = 0; n < ROWS / 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) d[n][e] = 0.f;
-#pragma unroll
-  for (int ks = 0; ks < HD / 16; ++ks) {
-    uint32_t af[4], f[4];
-    ldmatrix4(af, block<T, HD>(ta, r0, 2 * ks, true));
-#pragma unroll
-    for (int n = 0; n < ROWS / 16; ++n) {
-      ldmatrix4(f, block<T, HD>(tb, 16 * n, 2 * ks, false));
-      mma16(d[2 * n], af, f[0], f[1], T());
-      mma16(d[2 * n + 1], af, f[2], f[3], T());
-    }
-  }
-}
-
-// d[16 x HD] += A[16][16] B[rows r0 .. r0 + 15][HD].
-template <typename T, int HD>
-__device__ __forceinline__ void rows_sum(float (&d)[HD / 8][4], const uint32_t (&af)[4], const T* tb, int r0) {
-#pragma unroll
-  for (int n = 0; n < HD / 16; ++n) {
-    uint32_t f[4];
-    ldmatrix4_trans(f, block<T, HD>(tb, r0, 2 * n, true));
-    mma16(d[2 * n], af, f[0], f[1], T());
-    mma16(d[2 * n + 1], af, f[2], f[3], T());
-  }
 }
 
 template <int N>
@@ -102,7 +62,80 @@ __device__ __forceinline__ void clear(float (&d)[N][4]) {
     for (int e = 0; e < 4; ++e) d[n][e] = 0.f;
 }
 
-// A warp's 16 rows of results: rounded, through `stage` (the warp's own rows of a tile), to global memory.
+// First byte of a head. Within a head offsets are 32 bits (attention_is_small).
+__device__ __forceinline__ char* head_at(const SmallArgs& s, const void* p, const UnblendHeadStrides& t, int seq, int h) {
+  const int o = s.by_inner(seq), i = seq - o * s.a.inner;
+  return const_cast<char*>(static_cast<const char*>(p)) +
+         2 * ((long long)o * t.outer + (long long)i * t.inner + (long long)h * t.head);
+}
+
+// Rows [first, end) of a head by cp.async; the rest of the tile is 0.
+template <int HD>
+__device__ __forceinline__ void fetch(uint32_t tile, const char* src, const UnblendHeadStrides& t, int first, int end,
+                                      int hd) {
+  constexpr int CH = HD / 8, STEP = NT / CH;  // STEP is a multiple of 8: a thread's chunk keeps its place
+  const int r = threadIdx.x / CH, c = threadIdx.x % CH;
+  const uint32_t stride = 2 * (uint32_t)t.row;
+  const int mine = 8 * c < hd ? end : 0, last = max(mine - 1, 0);
+  tile += r * (2 * HD) + ((c ^ (r & 7)) * 16);
+  src += 8 * c < hd ? 16 * c : 0;
+#pragma unroll
+  for (int x = 0; x < ROWS / STEP; ++x) {
+    const int row = r + x * STEP;
+    cp_async16_or_zero(tile + x * STEP * 2 * HD, src + min(row, last) * stride, row >= first && row < mine);
+  }
+}
+
+// Address of a lane's row in ldmatrix: rows r0 .. r0 + 15 (r0 a multiple of 16) and chunks c, c + 1 (c even) of a tile,
+// `DOWN` of the four 8 x 8 blocks first.
+template <int COLS, bool DOWN>
+__device__ __forceinline__ uint32_t block(uint32_t tile, int r0, int c) {
+  const uint32_t lane = threadIdx.x & 31, r = lane & 7, m0 = (lane >> 3) & 1, m1 = lane >> 4;
+  const uint32_t at = ((DOWN ? m0 : m1) * 8 + r) * (2 * COLS) + (((DOWN ? m1 : m0) ^ r) * 16);
+  return tile + r0 * (2 * COLS) + (at ^ (c * 16));
+}
+
+// d[16 x 64] = A[rows r0 ..][HD] B[64][HD]^T, both tiles as they lie.
+template <typename T, int HD>
+__device__ __forceinline__ void rows_dot(float (&d)[ROWS / 8][4], uint32_t ta, int r0, uint32_t tb) {
+  clear(d);
+#pragma unroll
+  for (int ks = 0; ks < HD / 16; ++ks) {
+    uint32_t af[4], f[4];
+    ldmatrix4(af, block<HD, true>(ta, r0, 2 * ks));
+#pragma unroll
+    for (int n = 0; n < ROWS / 16; ++n) {
+      ldmatrix4(f, block<HD, false>(tb, 16 * n, 2 * ks));
+      mma16(d[2 * n], af, f[0], f[1], T());
+      mma16(d[2 * n + 1], af, f[2], f[3], T());
+    }
+  }
+}
+
+// d[16 x HD] += A[16][16] B[rows r0 .. r0 + 15][HD].
+template <typename T, int HD>
+__device__ __forceinline__ void rows_sum(float (&d)[HD / 8][4], const uint32_t (&af)[4], uint32_t tb, int r0) {
+#pragma unroll
+  for (int n = 0; n < HD / 16; ++n) {
+    uint32_t f[4];
+    ldmatrix4_trans(f, block<HD, true>(tb, r0, 2 * n));
+    mma16(d[2 * n], af, f[0], f[1], T());
+    mma16(d[2 * n + 1], af, f[2], f[3], T());
+  }
+}
+
+// d[16 x HD] += A^T B with A[64][64] (its columns r0 ..) and B[64][HD].
+template <typename T, int HD>
+__device__ __forceinline__ void columns_sum(float (&d)[HD / 8][4], uint32_t ta, int r0, uint32_t tb) {
+#pragma unroll
+  for (int ks = 0; ks < ROWS / 16; ++ks) {
+    uint32_t f[4];
+    ldmatrix4_trans(f, block<ROWS, false>(ta, 16 * ks, r0 / 8));
+    rows_sum<T, HD>(d, f, tb, 16 * ks);
+  }
+}
+
+// A warp's 16 rows of results, rounded.
 template <typename T, int N>
 __device__ __forceinline__ void pack_rows(uint32_t (&o)[N][2], const float (&d)[N][4], float f0, float f1) {
 #pragma unroll
@@ -111,24 +144,36 @@ __device__ __forceinline__ void pack_rows(uint32_t (&o)[N][2], const float (&d)[
     o[n][1] = pack_pair<T>(d[n][2] * f1, d[n][3] * f1);
   }
 }
-template <typename T, int HD>
-__device__ __forceinline__ void put_rows(T* stage, const uint32_t (&o)[HD / 8][2], T* dst, long long stride, int r0,
-                                         int rows, int hd) {
-  constexpr int CH = HD / 8;
+
+// Rows r0 .. r0 + 15 through `stage`, where these rows are the warp's own, to the first `rows` of dst; 0 where no key or
+// query counts (the products there may hold NaN).
+template <int HD, typename F>
+__device__ __forceinline__ void put_rows(uint32_t stage, const uint32_t (&o)[HD / 8][2], char* dst,
+                                         const UnblendHeadStrides& t, int r0, int rows, int hd, F&& counts) {
+  constexpr int CH = HD / 8, STEP = 32 / CH;
   const int lane = threadIdx.x & 31, quad = lane >> 2, ql = lane & 3;
+  stage += r0 * (2 * HD);
+  const uint32_t at = quad * (2 * HD) + quad * 16 + ql * 4;
   __syncwarp();
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int n = 0; n < CH; ++n)
 #pragma unroll
-    for (int n = 0; n < CH; ++n)
-      *reinterpret_cast<uint32_t*>(stage + (r0 + quad + 8 * x) * HD + ((n ^ quad) * 8) + 2 * ql) = o[n][x];
+    for (int x = 0; x < 2; ++x)
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(stage + (at ^ (n * 16)) + x * 8 * (2 * HD)), "r"(o[n][x]) : "memory");
   __syncwarp();
+  const int r = lane / CH, c = lane % CH;
+  const uint32_t from = r * (2 * HD) + ((c ^ r) * 16), stride = 2 * (uint32_t)t.row;
 #pragma unroll
-  for (int x = 0; x < 16 * CH / 32; ++x) {
-    const int id = x * 32 + lane, row = r0 + id / CH, c = id % CH;
-    if (row < rows && 8 * c < hd)
-      *reinterpret_cast<uint4*>(dst + row * stride + 8 * c) =
-          *reinterpret_cast<const uint4*>(stage + row * HD + ((c ^ (row & 7)) * 8));
+  for (int x = 0; x < 16 / STEP; ++x) {
+    const int row = r0 + r + x * STEP;
+    if (row < rows && 8 * c < hd) {
+      uint4 v;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "r"(stage + (from ^ (((x * STEP) & 7) * 16)) + x * STEP * (2 * HD))
+                   : "memory");
+      *reinterpret_cast<uint4*>(dst + row * stride + 16 * c) = counts(row) ? v : make_uint4(0, 0, 0, 0);
+    }
   }
 }
 
@@ -136,53 +181,71 @@ __device__ __forceinline__ void put_rows(T* stage, const uint32_t (&o)[HD / 8][2
 __device__ __forceinline__ int key_limit(const AttnArgs& a, const Bounds& b, int i) {
   return i < b.ql ? (a.causal ? min(b.kl, i + b.off + 1) : b.kl) : 0;
 }
+// Queries [first, end) see some key; the others, whatever they hold, count nowhere.
+struct Used {
+  int first, end;
+};
+__device__ __forceinline__ Used used_queries(const AttnArgs& a, const Bounds& b) {
+  return Used{a.causal ? max(0, -b.off) : 0, b.kl > 0 ? b.ql : 0};
+}
+// Keys that each of the rows r0 .. r0 + 15 sees: no mask below.
+__device__ __forceinline__ int keys_of_all(const AttnArgs& a, const Bounds& b, int r0) {
+  return r0 + 16 <= b.ql ? key_limit(a, b, r0) : 0;
+}
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(NT, HD == 64 ? 5 : 3) attention_small_fwd_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(NT, fwd_ctas(HD))
+    attention_small_fwd_kernel(const __grid_constant__ SmallArgs args) {
+  const AttnArgs& a = args.a;
+  constexpr uint32_t TILE = ROWS * HD * 2;
   extern __shared__ __align__(128) uint8_t small_smem[];
-  T* tq = reinterpret_cast<T*>(small_smem);
-  T *tk = tq + ROWS * HD, *tv = tk + ROWS * HD;
+  const uint32_t tq = smem_at(small_smem), tk = tq + TILE, tv = tk + TILE;
   const int lane = threadIdx.x & 31, r0 = (threadIdx.x >> 5) * 16, quad = lane >> 2, ql = lane & 3;
-  const int seq = blockIdx.x / a.heads, h = blockIdx.x - seq * a.heads, hk = h / a.group;
+  const int seq = args.by_heads(blockIdx.x), h = blockIdx.x - seq * a.heads, hk = args.by_group(h);
   const Bounds b = bounds_of(a, seq);
-  fetch<T, HD>(tq, static_cast<const T*>(a.q) + head_offset(a.q_s, a, seq, h), a.q_s.row, b.ql, a.hd);
-  fetch<T, HD>(tk, static_cast<const T*>(a.k) + head_offset(a.k_s, a, seq, hk), a.k_s.row, b.kl, a.hd);
+  const Used rows = used_queries(a, b);
+  fetch<HD>(tq, head_at(args, a.q, a.q_s, seq, h), a.q_s, rows.first, rows.end, a.hd);
+  fetch<HD>(tk, head_at(args, a.k, a.k_s, seq, hk), a.k_s, 0, b.kl, a.hd);
   cp_commit();
-  fetch<T, HD>(tv, static_cast<const T*>(a.v) + head_offset(a.v_s, a, seq, hk), a.v_s.row, b.kl, a.hd);
+  fetch<HD>(tv, head_at(args, a.v, a.v_s, seq, hk), a.v_s, 0, b.kl, a.hd);
   cp_commit();
   cp_wait<1>();
   __syncthreads();
   float s[ROWS / 8][4], inv[2];
   rows_dot<T, HD>(s, tq, r0, tk);
   const float c = a.scale * LOG2E;
+  const int all = keys_of_all(a, b, r0);
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const int i = r0 + quad + 8 * x, limit = key_limit(a, b, i);
-    float top = -INFINITY, sum = 0.f;
+    float top = -INFINITY;
 #pragma unroll
-    for (int n = 0; n < ROWS / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float& z = s[n][2 * x + e];
-        z = 8 * n + 2 * ql + e < limit ? z * c : -INFINITY;
-        top = fmaxf(top, z);
+    for (int n = 0; n < ROWS / 8; ++n) {
+      float &z0 = s[n][2 * x], &z1 = s[n][2 * x + 1];
+      if (8 * n + 8 > all) {
+        z0 = 8 * n + 2 * ql < limit ? z0 : -INFINITY;
+        z1 = 8 * n + 2 * ql + 1 < limit ? z1 : -INFINITY;
       }
+      top = fmaxf(top, fmaxf(z0, z1));
+    }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float base = top == -INFINITY ? 0.f : top;
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * c;
+    const float base = top == -INFINITY ? 0.f : -top;
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int n = 0; n < ROWS / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float& z = s[n][2 * x + e];
-        z = ex2(z - base);
-        sum += z;
-      }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    inv[x] = sum == 0.f ? 0.f : 1.f / sum;
+    for (int n = 0; n < ROWS / 8; ++n) {
+      float &z0 = s[n][2 * x], &z1 = s[n][2 * x + 1];
+      const float2 z = ub::fma2(make_float2(z0, z1), make_float2(c, c), make_float2(base, base));
+      z0 = ex2(z.x);
+      z1 = ex2(z.y);
+      sum = add2(sum, make_float2(z0, z1));
+    }
+    float total = sum.x + sum.y;
+    total += __shfl_xor_sync(0xffffffffu, total, 1);
+    total += __shfl_xor_sync(0xffffffffu, total, 2);
+    inv[x] = total == 0.f ? 0.f : __frcp_rn(total);
     if (a.lse && ql == 0 && i < a.lq)
-      a.lse[((long long)seq * a.heads + h) * a.lq + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+      a.lse[(long long)blockIdx.x * a.lq + i] = total == 0.f ? -INFINITY : (top + __log2f(total)) * LN2;
   }
   cp_wait<0>();
   __syncthreads();
@@ -190,95 +253,97 @@ __global__ void __launch_bounds__(NT, HD == 64 ? 5 : 3) attention_small_fwd_kern
   clear(o);
 #pragma unroll
   for (int ks = 0; ks < ROWS / 16; ++ks) {
-    const uint32_t pf[4] = {pack_pair<T>(s[2 * ks][0], s[2 * ks][1]), pack_pair<T>(s[2 * ks][2], s[2 * ks][3]),
-                            pack_pair<T>(s[2 * ks + 1][0], s[2 * ks + 1][1]),
-                            pack_pair<T>(s[2 * ks + 1][2], s[2 * ks + 1][3])};
+    uint32_t pf[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pf[e] = pack_pair<T>(s[2 * ks + e / 2][2 * (e & 1)], s[2 * ks + e / 2][2 * (e & 1) + 1]);
     rows_sum<T, HD>(o, pf, tv, 16 * ks);
   }
   uint32_t packed[HD / 8][2];
   pack_rows<T>(packed, o, inv[0], inv[1]);
-  put_rows<T, HD>(tq, packed, static_cast<T*>(a.out) + head_offset(a.out_s, a, seq, h), a.out_s.row, r0, a.lq, a.hd);
+  put_rows<HD>(tq, packed, head_at(args, a.out, a.out_s, seq, h), a.out_s, r0, a.lq, a.hd,
+               [&](int i) { return key_limit(a, b, i) > 0; });
 }
 
 // GROUPED: a CTA walks the query heads of its key/value head and keeps dK and dV in registers.
 template <typename T, int HD, bool GROUPED>
-__global__ void __launch_bounds__(NT, HD == 64 ? (GROUPED ? 3 : 4) : 2)
-    attention_small_bwd_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
+    attention_small_bwd_kernel(const __grid_constant__ SmallArgs args) {
+  const AttnArgs& a = args.a;
+  constexpr uint32_t TILE = ROWS * HD * 2, P_TILE = ROWS * ROWS * 2;
   constexpr float P_SCALE = std::is_same<T, __half>::value ? 4096.f : 1.f;
   extern __shared__ __align__(128) uint8_t small_smem[];
-  T* tk = reinterpret_cast<T*>(small_smem);
-  T *tv = tk + ROWS * HD, *tq = tv + ROWS * HD, *td = tq + ROWS * HD;
-  T *tp = td + ROWS * HD, *ts = tp + ROWS * ROWS;
-  T* stage = GROUPED ? ts + ROWS * ROWS : tv;  // of dQ: V is needed again by the next head
+  const uint32_t tk = smem_at(small_smem), tv = tk + TILE, tq = tv + TILE, td = tq + TILE;
+  const uint32_t tp = td + TILE, ts = tp + P_TILE;
+  const uint32_t stage = GROUPED ? ts + P_TILE : tv;  // of dQ: V is needed again by the next head
   const int lane = threadIdx.x & 31, r0 = (threadIdx.x >> 5) * 16, quad = lane >> 2, ql = lane & 3;
-  const int seq = blockIdx.x / a.kv_heads, hk = blockIdx.x - seq * a.kv_heads;
+  const int seq = args.by_heads(blockIdx.x), hk = blockIdx.x - seq * a.kv_heads;
   const Bounds b = bounds_of(a, seq);
+  const Used rows = used_queries(a, b);
   const float c = a.scale * LOG2E;
+  const int all = keys_of_all(a, b, r0);
   float dk[HD / 8][4], dv[HD / 8][4];
   clear(dk);
   clear(dv);
   for (int g = 0; g < (GROUPED ? a.group : 1); ++g) {
-    const int h = hk * a.group + g;
+    const int h = GROUPED ? hk * a.group + g : hk;
     if (g > 0) __syncthreads();  // the last head's tiles have been read
-    fetch<T, HD>(tq, static_cast<const T*>(a.q) + head_offset(a.q_s, a, seq, h), a.q_s.row, b.ql, a.hd);
-    if (g == 0)
-      fetch<T, HD>(tk, static_cast<const T*>(a.k) + head_offset(a.k_s, a, seq, hk), a.k_s.row, b.kl, a.hd);
+    fetch<HD>(tq, head_at(args, a.q, a.q_s, seq, h), a.q_s, rows.first, rows.end, a.hd);
+    if (g == 0) fetch<HD>(tk, head_at(args, a.k, a.k_s, seq, hk), a.k_s, 0, b.kl, a.hd);
     cp_commit();
-    fetch<T, HD>(td, static_cast<const T*>(a.dout) + head_offset(a.dout_s, a, seq, h), a.dout_s.row, b.ql, a.hd);
-    if (g == 0)
-      fetch<T, HD>(tv, static_cast<const T*>(a.v) + head_offset(a.v_s, a, seq, hk), a.v_s.row, b.kl, a.hd);
+    fetch<HD>(td, head_at(args, a.dout, a.dout_s, seq, h), a.dout_s, rows.first, rows.end, a.hd);
+    if (g == 0) fetch<HD>(tv, head_at(args, a.v, a.v_s, seq, hk), a.v_s, 0, b.kl, a.hd);
     cp_commit();
-    int limit[2];
     float base[2];
+    const float* lse = a.lse + ((long long)seq * a.heads + h) * a.lq;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int i = r0 + quad + 8 * x;
-      limit[x] = key_limit(a, b, i);
-      const float lse = i < b.ql ? a.lse[((long long)seq * a.heads + h) * a.lq + i] : -INFINITY;
-      base[x] = lse == -INFINITY ? INFINITY : lse * LOG2E;  // a row that sees nothing: P = 0
+      const float l = i < b.ql ? lse[i] : -INFINITY;
+      base[x] = l == -INFINITY ? -INFINITY : -l * LOG2E;  // a row that sees nothing: P = 0
     }
     cp_wait<1>();
     __syncthreads();
     float s[ROWS / 8][4], dp[ROWS / 8][4];
     rows_dot<T, HD>(s, tq, r0, tk);
 #pragma unroll
-    for (int n = 0; n < ROWS / 8; ++n)
+    for (int x = 0; x < 2; ++x) {
+      const int limit = key_limit(a, b, r0 + quad + 8 * x);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        s[n][e] = 8 * n + 2 * ql + (e & 1) < limit[e >> 1] ? ex2(fmaf(s[n][e], c, -base[e >> 1])) : 0.f;
+      for (int n = 0; n < ROWS / 8; ++n) {
+        float &z0 = s[n][2 * x], &z1 = s[n][2 * x + 1];
+        const float2 z = ub::fma2(make_float2(z0, z1), make_float2(c, c), make_float2(base[x], base[x]));
+        z0 = ex2(z.x);
+        z1 = ex2(z.y);
+        if (8 * n + 8 > all) {
+          z0 = 8 * n + 2 * ql < limit ? z0 : 0.f;
+          z1 = 8 * n + 2 * ql + 1 < limit ? z1 : 0.f;
+        }
+      }
+    }
     cp_wait<0>();
     __syncthreads();
     rows_dot<T, HD>(dp, td, r0, tv);
+    uint32_t sf[ROWS / 16][4];  // dS as A fragments
+    const uint32_t at = (r0 + quad) * (2 * ROWS) + quad * 16 + ql * 4;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      float d = 0.f;
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int n = 0; n < ROWS / 8; ++n)
-#pragma unroll
-        for (int e = 2 * x; e < 2 * x + 2; ++e) {
-          // Keys that the row does not see may hold anything.
-          dp[n][e] = 8 * n + 2 * ql + (e & 1) < limit[x] ? dp[n][e] : 0.f;
-          d = fmaf(s[n][e], dp[n][e], d);
-        }
+        sum = ub::fma2(make_float2(s[n][2 * x], s[n][2 * x + 1]), make_float2(dp[n][2 * x], dp[n][2 * x + 1]), sum);
+      float d = sum.x + sum.y;
       d += __shfl_xor_sync(0xffffffffu, d, 1);
       d += __shfl_xor_sync(0xffffffffu, d, 2);
 #pragma unroll
-      for (int n = 0; n < ROWS / 8; ++n)
-#pragma unroll
-        for (int e = 2 * x; e < 2 * x + 2; ++e)
-          dp[n][e] = 8 * n + 2 * ql + (e & 1) < limit[x] ? s[n][e] * (dp[n][e] - d) : 0.f;
-    }
-    uint32_t sf[ROWS / 16][4];  // dS as A fragments
-#pragma unroll
-    for (int n = 0; n < ROWS / 8; ++n)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int at = (r0 + quad + 8 * x) * ROWS + ((n ^ quad) * 8) + 2 * ql;
-        *reinterpret_cast<uint32_t*>(tp + at) = pack_pair<T>(s[n][2 * x] * P_SCALE, s[n][2 * x + 1] * P_SCALE);
-        const uint32_t w = pack_pair<T>(dp[n][2 * x], dp[n][2 * x + 1]);
-        *reinterpret_cast<uint32_t*>(ts + at) = w;
+      for (int n = 0; n < ROWS / 8; ++n) {
+        const float2 p = make_float2(s[n][2 * x], s[n][2 * x + 1]);
+        const float2 e = mul2(p, add2(make_float2(dp[n][2 * x], dp[n][2 * x + 1]), make_float2(-d, -d)));
+        const uint32_t w = pack_pair<T>(e.x, e.y), to = (at ^ (n * 16)) + x * 8 * (2 * ROWS);
         sf[n / 2][2 * (n & 1) + x] = w;
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(tp + to), "r"(pack_pair<T>(p.x * P_SCALE, p.y * P_SCALE)) : "memory");
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(ts + to), "r"(w) : "memory");
       }
+    }
     uint32_t packed[HD / 8][2];
     {
       float dq[HD / 8][4];
@@ -287,33 +352,29 @@ __global__ void __launch_bounds__(NT, HD == 64 ? (GROUPED ? 3 : 4) : 2)
       for (int ks = 0; ks < ROWS / 16; ++ks) rows_sum<T, HD>(dq, sf[ks], tk, 16 * ks);
       pack_rows<T>(packed, dq, a.scale, a.scale);
     }
-    __syncthreads();  // P and dS are written, V (and K, after the last head) read
-    put_rows<T, HD>(stage, packed, static_cast<T*>(a.dq) + head_offset(a.dq_s, a, seq, h), a.dq_s.row, r0, a.lq, a.hd);
-#pragma unroll
-    for (int ks = 0; ks < ROWS / 16; ++ks) {
-      uint32_t f[4];
-      ldmatrix4_trans(f, block<T, ROWS>(tp, 16 * ks, r0 / 8, false));
-      rows_sum<T, HD>(dv, f, td, 16 * ks);
-    }
-#pragma unroll
-    for (int ks = 0; ks < ROWS / 16; ++ks) {
-      uint32_t f[4];
-      ldmatrix4_trans(f, block<T, ROWS>(ts, 16 * ks, r0 / 8, false));
-      rows_sum<T, HD>(dk, f, tq, 16 * ks);
-    }
+    __syncthreads();  // P and dS are written, K and V are read
+    put_rows<HD>(stage, packed, head_at(args, a.dq, a.dq_s, seq, h), a.dq_s, r0, a.lq, a.hd,
+                 [&](int i) { return key_limit(a, b, i) > 0; });
+    columns_sum<T, HD>(dv, tp, r0, td);
+    columns_sum<T, HD>(dk, ts, r0, tq);
   }
+  auto counts = [&](int j) { return j < b.kl; };
   uint32_t packed[HD / 8][2];
   pack_rows<T>(packed, dv, 1.f / P_SCALE, 1.f / P_SCALE);
-  put_rows<T, HD>(tv, packed, static_cast<T*>(a.dv) + head_offset(a.dv_s, a, seq, hk), a.dv_s.row, r0, a.lk, a.hd);
+  put_rows<HD>(tv, packed, head_at(args, a.dv, a.dv_s, seq, hk), a.dv_s, r0, a.lk, a.hd, counts);
   pack_rows<T>(packed, dk, a.scale, a.scale);
-  put_rows<T, HD>(tk, packed, static_cast<T*>(a.dk) + head_offset(a.dk_s, a, seq, hk), a.dk_s.row, r0, a.lk, a.hd);
+  put_rows<HD>(tk, packed, head_at(args, a.dk, a.dk_s, seq, hk), a.dk_s, r0, a.lk, a.hd, counts);
+}
+
+SmallArgs small_args(const AttnArgs& a, int heads) {
+  return SmallArgs{a, fast_div(heads), fast_div(a.group), fast_div(a.inner)};
 }
 
 template <typename T, int HD>
 int launch_fwd(const AttnArgs& a, cudaStream_t st) {
   constexpr int bytes = fwd_smem(HD);
   if (allow_smem<attention_small_fwd_kernel<T, HD>>(bytes) != cudaSuccess) return (int)cudaGetLastError();
-  attention_small_fwd_kernel<T, HD><<<(unsigned)(a.seqs * a.heads), NT, bytes, st>>>(a);
+  attention_small_fwd_kernel<T, HD><<<(unsigned)(a.seqs * a.heads), NT, bytes, st>>>(small_args(a, a.heads));
   UB_CHECK_LAUNCH();
   return 0;
 }
@@ -322,7 +383,7 @@ template <typename T, int HD, bool GROUPED>
 int launch_bwd(const AttnArgs& a, cudaStream_t st) {
   constexpr int bytes = bwd_smem(HD, GROUPED);
   if (allow_smem<attention_small_bwd_kernel<T, HD, GROUPED>>(bytes) != cudaSuccess) return (int)cudaGetLastError();
-  attention_small_bwd_kernel<T, HD, GROUPED><<<(unsigned)(a.seqs * a.kv_heads), NT, bytes, st>>>(a);
+  attention_small_bwd_kernel<T, HD, GROUPED><<<(unsigned)(a.seqs * a.kv_heads), NT, bytes, st>>>(small_args(a, a.kv_heads));
   UB_CHECK_LAUNCH();
   return 0;
 }
@@ -339,7 +400,14 @@ namespace ub {
 namespace train {
 
 bool attention_is_small(const UnblendAttnTrainParams& p, bool backward) {
-  return p.lq <= ROWS && p.lk <= ROWS && (!backward || p.hd <= 64 || p.heads == p.kv_heads);
+  if (p.lq > ROWS || p.lk > ROWS || (backward && p.hd > 64 && p.heads > p.kv_heads)) return false;
+  // 32-bit byte offsets within a head (the row stride of a tensor of one row is not used).
+  constexpr long long MOST = 1LL << 24;
+  for (const UnblendHeadStrides* t : {&p.q, &p.out, &p.dout, &p.dq})
+    if (p.lq > 1 && t->row >= MOST && (backward || t == &p.q || t == &p.out)) return false;
+  for (const UnblendHeadStrides* t : {&p.k, &p.v, &p.dk, &p.dv})
+    if (p.lk > 1 && t->row >= MOST && (backward || t == &p.k || t == &p.v)) return false;
+  return true;
 }
 
 int attention_small_forward(const AttnArgs& a, const UnblendAttnTrainParams& p, cudaStream_t st) {

@@ -183,24 +183,6 @@ __device__ __forceinline__ void clear_row(uint8_t* tile, int rows, int blocks, i
   }
 }
 
-// n / d for n < 2^31 by a multiplication: with 2^s >= d and m = floor(2^(31 + s) / d) + 1, floor(n m / 2^(31 + s)) is
-// exact because n (m d - 2^(31 + s)) < 2^(31 + s). Unit numbers are taken apart between tiles, where a hardware
-// division's hundred cycles are not hidden.
-struct FastDiv {
-  uint32_t d, m, shift;
-  __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> shift); }
-};
-
-FastDiv fast_div(long long d) {
-  FastDiv f;
-  uint32_t s = 0;
-  while ((1LL << s) < d) ++s;
-  f.d = (uint32_t)d;
-  f.shift = 31 + s;
-  f.m = (uint32_t)((1ULL << f.shift) / (uint64_t)d + 1);
-  return f;
-}
-
 struct TcArgs {
   AttnArgs a;
   const float2* stats;   // backward: (-lse log2 e, -D) of each query row, (-inf, 0) for rows that see nothing

@@ -7,21 +7,22 @@
 namespace ub {
 namespace train {
 
-__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
-               "r"(in ? 16 : 0)
-               : "memory");
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 bytes to shared memory, of src or zeros.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const void* p) {
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"((uint32_t)__cvta_generic_to_shared(p))
+               : "r"(p)
                : "memory");
 }
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], const void* p) {
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"((uint32_t)__cvta_generic_to_shared(p))
+               : "r"(p)
                : "memory");
 }
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
