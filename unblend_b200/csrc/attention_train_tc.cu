@@ -620,43 +620,65 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
 // ---------------------------------------------------------------------------------------- row statistics
 //
 // (-lse log2 e, -D) of each query row, D = rowsum(dO * O); (-inf, 0) for rows that see nothing. LANES lanes per row, 8
-// values each; rows in memory order (heads fastest) for whole lines. A kernel of its own: inside the dq kernel the
-// loads stood in front of every unit's first tile (5000 of 24000 cycles for 11 tiles).
+// values each; rows in memory order (heads fastest) for whole lines; all loads of a thread's STATS_ROWS rows are issued
+// before the first is used. A kernel of its own: inside the dq kernel the loads stood in front of every unit's first
+// tile (5000 of 24000 cycles for 11 tiles). Bound: HBM, one read of dO and O.
+constexpr int STATS_ROWS = 4;
+
 template <typename T, int LANES>
-__global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_constant__ AttnArgs a, float2* stats) {
+__global__ void __launch_bounds__(256)
+    attention_stats_kernel(const __grid_constant__ AttnArgs a, float2* stats, FastDiv by_heads, FastDiv by_lq,
+                           FastDiv by_inner) {
+  constexpr int STEP = 256 / LANES;
   const int lane = threadIdx.x & (LANES - 1);
   const long long n = (long long)a.seqs * a.lq * a.heads;
-  const long long id = (blockIdx.x * 256LL + threadIdx.x) / LANES;
-  const bool in = id < n;
-  int h = 0, seq = 0, i = 0;
-  if (n <= 0xFFFFFFFFll) {  // 32-bit divisions where they do
-    const unsigned x = in ? (unsigned)id : 0u, token = x / (unsigned)a.heads;
-    h = (int)(x - token * (unsigned)a.heads);
-    seq = (int)(token / (unsigned)a.lq);
-    i = (int)(token - (unsigned)seq * (unsigned)a.lq);
-  } else if (in) {
-    const long long token = id / a.heads;
-    h = (int)(id - token * a.heads);
-    seq = (int)(token / a.lq);
-    i = (int)(token - (long long)seq * a.lq);
+  const long long first = (long long)blockIdx.x * (STEP * STATS_ROWS) + threadIdx.x / LANES;
+  const bool small = n < (1LL << 31);
+  long long row[STATS_ROWS];
+  float lse[STATS_ROWS];
+  uint4 dv[STATS_ROWS], ov[STATS_ROWS];
+#pragma unroll
+  for (int u = 0; u < STATS_ROWS; ++u) {
+    const long long id = min(first + u * STEP, n - 1);  // the last row again: the same values
+    int h, seq, i, o;
+    if (small) {
+      const int token = by_heads((int)id);
+      h = (int)id - token * a.heads;
+      seq = by_lq(token);
+      i = token - seq * a.lq;
+      o = by_inner(seq);
+    } else {
+      const long long token = id / a.heads;
+      h = (int)(id - token * a.heads);
+      seq = (int)(token / a.lq);
+      i = (int)(token - (long long)seq * a.lq);
+      o = seq / a.inner;
+    }
+    const Bounds b = bounds_of(a, seq);
+    row[u] = ((long long)seq * a.heads + h) * a.lq + i;
+    const bool in = i < b.ql;
+    auto at = [&](const void* p, const UnblendHeadStrides& t) {
+      return static_cast<const T*>(p) + (long long)o * t.outer + (long long)(seq - o * a.inner) * t.inner +
+             (long long)h * t.head + (long long)i * t.row + 8 * lane;
+    };
+    lse[u] = in ? a.lse[row[u]] : -INFINITY;
+    dv[u] = ov[u] = make_uint4(0, 0, 0, 0);
+    if (in && 8 * lane < a.hd) {
+      dv[u] = *reinterpret_cast<const uint4*>(at(a.dout, a.dout_s));
+      ov[u] = *reinterpret_cast<const uint4*>(at(a.out_in, a.out_s));
+    }
   }
-  const Bounds b = bounds_of(a, seq);
-  const long long row = ((long long)seq * a.heads + h) * a.lq + i;
-  const float lse = in && i < b.ql ? a.lse[row] : -INFINITY;
-  float D = 0.f;
-  if (lse != -INFINITY && 8 * lane < a.hd) {
-    const uint4 dv = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout) + head_offset(a.dout_s, a, seq, h) +
-                                                     (long long)i * a.dout_s.row + 8 * lane);
-    const uint4 ov = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.out_in) + head_offset(a.out_s, a, seq, h) +
-                                                     (long long)i * a.out_s.row + 8 * lane);
-    const T* x = reinterpret_cast<const T*>(&dv);
-    const T* y = reinterpret_cast<const T*>(&ov);
+#pragma unroll
+  for (int u = 0; u < STATS_ROWS; ++u) {
+    const T* x = reinterpret_cast<const T*>(&dv[u]);
+    const T* y = reinterpret_cast<const T*>(&ov[u]);
+    float D = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) D = fmaf(to_f(x[e]), to_f(y[e]), D);
-  }
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) D += __shfl_xor_sync(0xffffffffu, D, o);
-  if (in && lane == 0) stats[row] = make_float2(lse == -INFINITY ? lse : -lse * LOG2E, -D);
+    for (int o = LANES / 2; o > 0; o >>= 1) D += __shfl_xor_sync(0xffffffffu, D, o);
+    if (lane == 0) stats[row[u]] = lse[u] == -INFINITY ? make_float2(-INFINITY, 0.f) : make_float2(-lse[u] * LOG2E, -D);
+  }
 }
 
 // --------------------------------------------------------------------------------------------------- dq
@@ -1532,13 +1554,14 @@ template <typename T>
 int launch_stats(const AttnArgs& a, cudaStream_t st) {
   float2* stats = reinterpret_cast<float2*>(a.dsum);
   const long long rows = (long long)a.seqs * a.lq * a.heads;
-  auto grid = [&](int lanes) { return (unsigned)((rows * lanes + 255) / 256); };
+  const FastDiv by_heads = fast_div(a.heads), by_lq = fast_div(a.lq), by_inner = fast_div(a.inner);
+  auto grid = [&](int lanes) { return (unsigned)((rows + STATS_ROWS * 256 / lanes - 1) / (STATS_ROWS * 256 / lanes)); };
   if (a.hd <= 32)
-    attention_stats_kernel<T, 4><<<grid(4), 256, 0, st>>>(a, stats);
+    attention_stats_kernel<T, 4><<<grid(4), 256, 0, st>>>(a, stats, by_heads, by_lq, by_inner);
   else if (a.hd <= 64)
-    attention_stats_kernel<T, 8><<<grid(8), 256, 0, st>>>(a, stats);
+    attention_stats_kernel<T, 8><<<grid(8), 256, 0, st>>>(a, stats, by_heads, by_lq, by_inner);
   else
-    attention_stats_kernel<T, 16><<<grid(16), 256, 0, st>>>(a, stats);
+    attention_stats_kernel<T, 16><<<grid(16), 256, 0, st>>>(a, stats, by_heads, by_lq, by_inner);
   UB_CHECK_LAUNCH();
   return 0;
 }
