@@ -813,7 +813,10 @@ Plan plan_of(const UnblendAttnTrainParams& p, Path path) {
   n.fwd_splits = n.dq_splits = n.dkv_splits = 1;
   if (path == SMALL) return n;
   n.fwd_rows = (int)tile;
-  if (tc && qh * div_up(p.lq, 256) >= sms && p.lq > 128) n.fwd_rows = 256;
+  // 256 queries per CTA halve the reads of K and V tiles, which only pays for wide heads and long rows: at head dim 128
+  // 2048 x 2048 253 us against 267 us, 1536 169 against 170, 1024 88 against 86 (801: 134 against 118); at head dim 64
+  // 8192 x 8192 448 against 414 us, 62 x 801 x 801 211 against 172 us (two CTAs per SM fill each other's waits).
+  if (tc && p.hd > 64 && p.lk > 1024 && p.lq > 128 && qh * div_up(p.lq, 256) >= sms) n.fwd_rows = 256;
   n.fwd_splits = n.fwd_rows == 256 ? 1 : split_count(qh * qt, kt, 2 * sms);
   // Few rows: CTAs of 128 keys at least, twice as many as run at once, for sequences of unequal lengths.
   if (path == FEW) n.fwd_splits = split_count(kh, div_up(p.lk, 128), 4 * sms);

@@ -287,7 +287,7 @@ struct FwdCfg {
   static constexpr int NB = HD / 64;                   // 64-column blocks
   static constexpr int Q_BYTES = 128 * 128 * NB;       // a Q tile
   static constexpr int TILE_BYTES = BN * 128 * NB;     // a K or V tile
-  static constexpr int STAGES = NQ == 2 ? (HD == 64 ? 8 : 4) : (HD == 64 ? 4 : 2);  // ring of K and V tiles
+  static constexpr int STAGES = NQ == 1 && HD == 128 ? 2 : 4;  // ring of K and V tiles
   static constexpr int SMEM = NQ * Q_BYTES + STAGES * TILE_BYTES + 1024 + 512;
   static constexpr int THREADS = NQ * 128 + 128;       // softmax warpgroups, then one for TMA and MMA issue
   static constexpr int PER_SM = SHORT ? 3 : NQ == 2 ? 1 : 2;
@@ -1614,9 +1614,7 @@ int attention_fwd_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int row
   return by_type(p, [&](auto x) {
     using T = decltype(x);
     if (p.hd <= 64 && p.lk <= SHORT_ROWS) return launch_fwd<T, 64, 1, true>(a, p, a.splits, st);
-    if (rows_per_cta == 256)
-      return p.hd <= 64 ? launch_fwd<T, 64, 2, false>(a, p, a.splits, st)
-                        : launch_fwd<T, 128, 2, false>(a, p, a.splits, st);
+    if (rows_per_cta == 256) return launch_fwd<T, 128, 2, false>(a, p, a.splits, st);  // head dims over 64 only
     return p.hd <= 64 ? launch_fwd<T, 64, 1, false>(a, p, a.splits, st)
                       : launch_fwd<T, 128, 1, false>(a, p, a.splits, st);
   });
