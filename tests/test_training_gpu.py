@@ -392,6 +392,24 @@ def test_attention_large_scores(t):
     _attn_case(q, k, v, dout, scale=0.0)
 
 
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("lq,lk,cut,h,hk,hd", [(60, 64, 31, 2, 2, 64), (50, 60, 20, 4, 2, 48), (64, 64, 63, 3, 3, 128),
+                                               (150, 300, 130, 2, 1, 64), (33, 200, 100, 2, 1, 128)])
+def test_attention_blocks_of_keys(lq, lk, cut, h, hk, hd, t):
+    """Two blocks of keys, each with a backward call of its own from the joined output and lse: the gradients of the
+    whole. The output in t is the joined one rounded, as the whole's is, so the whole's bounds hold; dq is a sum of two
+    rounded results."""
+    q, k, v, dout = _attn(lq, lk, h, hk, hd, t)
+    ref = attention_reference(q, k, v, dout)
+    out, lse = training.attention_forward(q, k, v)
+    parts = [training.attention_backward(dout, q, k[:, s], v[:, s], out, lse) for s in (slice(0, cut), slice(cut, lk))]
+    got = {"dk": torch.cat([x[1] for x in parts], 1), "dv": torch.cat([x[2] for x in parts], 1)}
+    _check({n: ref[n] for n in got}, got)
+    want, tol = ref["dq"]
+    each = half(t) * sum(x[0].double().abs() for x in parts)
+    assert_within("dq", parts[0][0].double() + parts[1][0].double(), want, tol + each + floor(t))
+
+
 def test_attention_nan_stays_in_its_sequence():
     q, k, v, dout = _attn(100, 100, 2, 2, 64, BF16, n=3)
     clean = _attn_case(q, k, v, dout)

@@ -2,14 +2,14 @@
 // sequence and head, so each tensor is read once and written once.
 //
 //   S = scale Q K^T, P = softmax(S), O = P V
-//   dP = dO V^T, D = rowsum(P * dP) (= rowsum(dO * O)), dS = P * (dP - D)
+//   dP = dO V^T, D = rowsum(dO * O), dS = P * (dP - D)
 //   dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO
 //
-// With all keys of a row at hand D comes from P and dP in fp32: the output is not read. One kernel makes the three
-// gradients, where the kernels for long rows need one for the statistics, one for dq and one for dk and dv, and read
-// the inputs in each.
+// One kernel makes the three gradients, where the kernels for long rows need one for the statistics, one for dq and one
+// for dk and dv, and read the inputs in each. (D = rowsum(P * dP) would save the read of O, but holds only when lse and
+// O are of these keys alone, which a caller that joins several blocks of keys does not give.)
 //
-// Bound: HBM. A sequence and head gives 5 products of 64 x 64 x head dim for 7 tensors of 64 rows, far below what the
+// Bound: HBM. A sequence and head gives 5 products of 64 x 64 x head dim for 8 tensors of 64 rows, far below what the
 // tensor cores need per byte, so mma.sync is enough (m16n8k16, fp32 accumulators); tcgen05's 128 rows would be half
 // empty, with one round trip through TMEM after the other and nothing to overlap it within a sequence. What hides
 // latency here is several independent CTAs per SM.
@@ -52,6 +52,15 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(p)
+               : "memory");
+  return v;
 }
 
 template <int N>
@@ -135,6 +144,27 @@ __device__ __forceinline__ void columns_sum(float (&d)[HD / 8][4], uint32_t ta, 
   }
 }
 
+// Dot product of row `row` of two tiles, on all four lanes of a quad; every quad takes other banks first.
+template <typename T, int HD>
+__device__ __forceinline__ float row_product(uint32_t ta, uint32_t tb, int row) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t at = row * (2 * HD) + (((lane & 3) + 4 * ((lane >> 2) & 1)) ^ (row & 7)) * 16;
+  float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < HD / 32; ++k) {
+    const uint4 x = lds16(ta + (at ^ (k * 64))), y = lds16(tb + (at ^ (k * 64)));
+    float2 u[4], v[4];
+    unpack16(x, u, T());
+    unpack16(y, v, T());
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = ub::fma2(u[e], v[e], sum);
+  }
+  float d = sum.x + sum.y;
+  d += __shfl_xor_sync(0xffffffffu, d, 1);
+  d += __shfl_xor_sync(0xffffffffu, d, 2);
+  return d;
+}
+
 // A warp's 16 rows of results, rounded.
 template <typename T, int N>
 __device__ __forceinline__ void pack_rows(uint32_t (&o)[N][2], const float (&d)[N][4], float f0, float f1) {
@@ -167,11 +197,7 @@ __device__ __forceinline__ void put_rows(uint32_t stage, const uint32_t (&o)[HD 
   for (int x = 0; x < 16 / STEP; ++x) {
     const int row = r0 + r + x * STEP;
     if (row < rows && 8 * c < hd) {
-      uint4 v;
-      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                   : "r"(stage + (from ^ (((x * STEP) & 7) * 16)) + x * STEP * (2 * HD))
-                   : "memory");
+      const uint4 v = lds16(stage + (from ^ (((x * STEP) & 7) * 16)) + x * STEP * (2 * HD));
       *reinterpret_cast<uint4*>(dst + row * stride + 16 * c) = counts(row) ? v : make_uint4(0, 0, 0, 0);
     }
   }
@@ -274,6 +300,8 @@ __global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
   extern __shared__ __align__(128) uint8_t small_smem[];
   const uint32_t tk = smem_at(small_smem), tv = tk + TILE, tq = tv + TILE, td = tq + TILE;
   const uint32_t tp = td + TILE, ts = tp + P_TILE;
+  const uint32_t to = tp;  // O, before P (head dims over 64: and dS) takes its place
+  static_assert(HD == 64 || HD == 128, "O fits P's tile, or P's and dS's");
   const uint32_t stage = GROUPED ? ts + P_TILE : tv;  // of dQ: V is needed again by the next head
   const int lane = threadIdx.x & 31, r0 = (threadIdx.x >> 5) * 16, quad = lane >> 2, ql = lane & 3;
   const int seq = args.by_heads(blockIdx.x), hk = blockIdx.x - seq * a.kv_heads;
@@ -291,6 +319,7 @@ __global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
     if (g == 0) fetch<HD>(tk, head_at(args, a.k, a.k_s, seq, hk), a.k_s, 0, b.kl, a.hd);
     cp_commit();
     fetch<HD>(td, head_at(args, a.dout, a.dout_s, seq, h), a.dout_s, rows.first, rows.end, a.hd);
+    fetch<HD>(to, head_at(args, a.out_in, a.out_s, seq, h), a.out_s, rows.first, rows.end, a.hd);
     if (g == 0) fetch<HD>(tv, head_at(args, a.v, a.v_s, seq, hk), a.v_s, 0, b.kl, a.hd);
     cp_commit();
     float base[2];
@@ -323,25 +352,25 @@ __global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
     cp_wait<0>();
     __syncthreads();
     rows_dot<T, HD>(dp, td, r0, tv);
+    float D[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) D[x] = row_product<T, HD>(td, to, r0 + quad + 8 * x);
+    if (HD > 64)
+      __syncthreads();  // O's rows lie under other warps' rows of P and dS
+    else
+      __syncwarp();
     uint32_t sf[ROWS / 16][4];  // dS as A fragments
     const uint32_t at = (r0 + quad) * (2 * ROWS) + quad * 16 + ql * 4;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int n = 0; n < ROWS / 8; ++n)
-        sum = ub::fma2(make_float2(s[n][2 * x], s[n][2 * x + 1]), make_float2(dp[n][2 * x], dp[n][2 * x + 1]), sum);
-      float d = sum.x + sum.y;
-      d += __shfl_xor_sync(0xffffffffu, d, 1);
-      d += __shfl_xor_sync(0xffffffffu, d, 2);
 #pragma unroll
       for (int n = 0; n < ROWS / 8; ++n) {
         const float2 p = make_float2(s[n][2 * x], s[n][2 * x + 1]);
-        const float2 e = mul2(p, add2(make_float2(dp[n][2 * x], dp[n][2 * x + 1]), make_float2(-d, -d)));
-        const uint32_t w = pack_pair<T>(e.x, e.y), to = (at ^ (n * 16)) + x * 8 * (2 * ROWS);
+        const float2 e = mul2(p, add2(make_float2(dp[n][2 * x], dp[n][2 * x + 1]), make_float2(-D[x], -D[x])));
+        const uint32_t w = pack_pair<T>(e.x, e.y), put = (at ^ (n * 16)) + x * 8 * (2 * ROWS);
         sf[n / 2][2 * (n & 1) + x] = w;
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(tp + to), "r"(pack_pair<T>(p.x * P_SCALE, p.y * P_SCALE)) : "memory");
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(ts + to), "r"(w) : "memory");
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(tp + put), "r"(pack_pair<T>(p.x * P_SCALE, p.y * P_SCALE)) : "memory");
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(ts + put), "r"(w) : "memory");
       }
     }
     uint32_t packed[HD / 8][2];
