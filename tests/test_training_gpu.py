@@ -202,6 +202,26 @@ def test_dropout_strides(cols):
         _drop_case(x, 0.25, rng, res, s, d)
 
 
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("cols", [8, 64, 520, 4096])
+def test_dropout_aligned_slices(cols, t):
+    """Rows of 16-byte chunks with gaps between them, in one tensor or in all."""
+    g = _gen(cols)
+    rng = torch.tensor([8, 1 << 40], device="cuda")
+    x, r, dy = (_rand(70, 3, cols + 16, g=g, t=a)[..., 8:-8] for a in (t, F32, F32))
+    s = _rand(cols, g=g)
+    _drop_case(x, 0.25, rng, r, s, dy)
+    _drop_case(x, 0.25, rng, r.contiguous(), s, dy.contiguous())
+    _drop_case(x.contiguous(), 0.25, rng, r, None, dy)
+
+
+@pytest.mark.parametrize("cols", [1 << 22, (1 << 22) + 8, (1 << 22) + 5])
+def test_dropout_very_wide_rows(cols):
+    g = _gen(12)
+    x, r, dy = (_rand(2, cols, g=g, t=a) for a in (BF16, F32, F32))
+    _drop_case(x, 0.1, torch.tensor([3, 4], device="cuda"), r, _rand(cols, g=g), dy)
+
+
 def test_dropout_keep_rate_and_streams():
     x = torch.ones(4000, 1000, device="cuda")
     seen = []

@@ -350,9 +350,9 @@ int launch(const DropArgs& a, int dtype, int r_dtype, int w_dtype, Path path, in
   return launch_streams<__half, BWD>(a, r_dtype, w_dtype, path, parts, st);
 }
 
-// One run of values; small enough for the flat kernel's 32-bit thread numbers.
+// One run of values. Very wide rows are left to the other kernels: each of the VEC rows of partial sums is as wide.
 bool contiguous(const RowMap& m, long long outer, int cols) {
-  return (m.inner <= 1 || m.si == cols) && (outer <= 1 || m.so == (long long)m.inner * cols) && cols <= (1 << 26);
+  return (m.inner <= 1 || m.si == cols) && (outer <= 1 || m.so == (long long)m.inner * cols) && cols <= (1 << 22);
 }
 
 void set_p(DropArgs* a, double p) {
