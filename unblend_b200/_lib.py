@@ -311,7 +311,7 @@ def call(name: str, *args, work: float | None = None) -> None:
         probe.append((name, start, end, work))
     else:
         # The handle alone: building a torch.cuda.Stream object costs more than most launches.
-        rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
     counters["launches"] += KERNELS_PER_CALL.get(name, 1)
     check(name, rc)
 
