@@ -12,8 +12,10 @@
 //
 // The kernels here take every type, stride and alignment, and are the path of fp32: 64 x 64 score tiles on 256
 // threads, 4 x 4 scores per thread, operands in shared memory as fp32 (transposed where the head axis is summed). Bound
-// by the FP32 pipes and the shared-memory reads that feed them: 8 x 1344 x 1344, 8 heads of 64, fp32 1.14 ms forward
-// and 3.92 ms backward, 26 TFLOP/s in both.
+// by the shared-memory reads that feed the FP32 pipes (78 % of their rate in the forward kernel): 8 x 1344 x 1344, 8
+// heads of 64, fp32 1.09 ms forward (27 TFLOP/s) and 3.32 ms backward (31 TFLOP/s). 4 x 8 scores on 128 threads halve
+// the reads, but with as few warps were only faster forward at head dim 64 (0.97 ms; backward 3.58 ms, at head dim 128
+// 2.62 and 9.17 ms against 2.17 and 7.50 ms).
 #include "attention_train.cuh"
 #include "warp_mma.cuh"
 
@@ -100,6 +102,13 @@ __device__ __forceinline__ void zero(float2 (&acc)[4][HDP / 64][2]) {
     for (int g = 0; g < HDP / 64; ++g) acc[r][g][0] = acc[r][g][1] = make_float2(0.f, 0.f);
 }
 
+// A thread's 4 x 4 values transposed: S[4 tx + e][4 ty ..].
+__device__ __forceinline__ void put_scores(float* S, const float (&v)[4][4], int ty, int tx) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    *reinterpret_cast<float4*>(S + (4 * tx + e) * LD + 4 * ty) = make_float4(v[0][e], v[1][e], v[2][e], v[3][e]);
+}
+
 // One accumulator row (64 g + 4 tx + e over all tx, g) times mul to out[d] (T) or to a fp32 part row.
 template <typename T, int HDP>
 __device__ __forceinline__ void store_row(const float2 (&acc)[HDP / 64][2], float mul, T* out, int hd, int tx) {
@@ -174,13 +183,15 @@ __global__ void __launch_bounds__(NT) attention_fwd_kernel(const __grid_constant
     __syncthreads();
     float2 s[4][2];
     mm_nt(s, sQ, sK, hd, ty, tx);
+    float p[4][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
+      const int limit = key_limit(a, b, i0 + 4 * ty + r) - j0;
       float x[4] = {s[r][0].x * c, s[r][0].y * c, s[r][1].x * c, s[r][1].y * c};
       float top = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (!sees(a, b, i0 + 4 * ty + r, j0 + 4 * tx + e)) x[e] = -INFINITY;
+        if (4 * tx + e >= limit) x[e] = -INFINITY;
         top = fmaxf(top, x[e]);
       }
       top = fmaxf(row_max16(top), m[r]);
@@ -189,9 +200,8 @@ __global__ void __launch_bounds__(NT) attention_fwd_kernel(const __grid_constant
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p = exp2f(x[e] - base);
-        sum += p;
-        sP[(4 * tx + e) * LD + 4 * ty + r] = p;
+        p[r][e] = exp2f(x[e] - base);
+        sum += p[r][e];
       }
       l[r] = l[r] * corr + row_sum16(sum);
       m[r] = top;
@@ -200,6 +210,7 @@ __global__ void __launch_bounds__(NT) attention_fwd_kernel(const __grid_constant
 #pragma unroll
         for (int e = 0; e < 2; ++e) o[r][g][e].x *= corr, o[r][g][e].y *= corr;
     }
+    put_scores(sP, p, ty, tx);
     __syncthreads();
     mm_wn<HDP>(o, sP, sV, ty, tx);
   }
@@ -277,17 +288,17 @@ __global__ void __launch_bounds__(NT) attention_dq_kernel(const __grid_constant_
     float2 s[4][2], dp[4][2];
     mm_nt(s, sQ, sK, hd, ty, tx);
     mm_nt(dp, sO, sV, hd, ty, tx);
+    float ds[4][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
+      const int limit = key_limit(a, b, i0 + 4 * ty + r) - j0;
       const float x[4] = {s[r][0].x, s[r][0].y, s[r][1].x, s[r][1].y};
       const float g[4] = {dp[r][0].x, dp[r][0].y, dp[r][1].x, dp[r][1].y};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float ds = 0.f;
-        if (sees(a, b, i0 + 4 * ty + r, j0 + 4 * tx + e)) ds = exp2f(x[e] * c - lse[r] * LOG2E) * (g[e] - D[r]);
-        sS[(4 * tx + e) * LD + 4 * ty + r] = ds;
-      }
+      for (int e = 0; e < 4; ++e)
+        ds[r][e] = 4 * tx + e < limit ? exp2f(x[e] * c - lse[r] * LOG2E) * (g[e] - D[r]) : 0.f;
     }
+    put_scores(sS, ds, ty, tx);
     __syncthreads();
     mm_wn<HDP>(acc, sS, sKr, ty, tx);
   }
@@ -315,7 +326,7 @@ __global__ void __launch_bounds__(NT) attention_dkv_kernel(const __grid_constant
   float* sO = sQ + HDP * LD;              // [HDP][LD] dO
   float* sQr = sO + HDP * LD;             // [64][HDP + 4]
   float* sOr = sQr + TILE * (HDP + 4);    // [64][HDP + 4]
-  float* sS = sOr + TILE * (HDP + 4);     // [64 queries][LD]: P^T, then dS^T
+  float *sP = sQ, *sS = sO;               // [64 queries][LD] P^T and dS^T, once S^T and dP^T are there
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const Unit u = unit_of((a.lk + TILE - 1) / TILE, a.kv_heads, a.splits);
   const Bounds b = bounds_of(a, u.seq);
@@ -354,34 +365,24 @@ __global__ void __launch_bounds__(NT) attention_dkv_kernel(const __grid_constant
     float2 s[4][2], dp[4][2];
     mm_nt(s, sK, sQ, hd, ty, tx);
     mm_nt(dp, sV, sO, hd, ty, tx);
-    float ds[4][4];
-    float lse[4], D[4];
+    float p[4][4], ds[4][4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int i = i0 + 4 * tx + e;
-      lse[e] = i < b.ql ? a.lse[row0 + i] * LOG2E : 0.f;
-      D[e] = i < b.ql ? a.dsum[row0 + i] : 0.f;
-    }
+      const int i = i0 + 4 * tx + e, limit = key_limit(a, b, i) - j0;
+      const float lse = i < b.ql ? a.lse[row0 + i] * LOG2E : 0.f, D = i < b.ql ? a.dsum[row0 + i] : 0.f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float x[4] = {s[r][0].x, s[r][0].y, s[r][1].x, s[r][1].y};
-      const float g[4] = {dp[r][0].x, dp[r][0].y, dp[r][1].x, dp[r][1].y};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool on = sees(a, b, i0 + 4 * tx + e, j0 + 4 * ty + r);
-        const float p = on ? exp2f(x[e] * c - lse[e]) : 0.f;
-        ds[r][e] = on ? p * (g[e] - D[e]) : 0.f;
-        sS[(4 * tx + e) * LD + 4 * ty + r] = p;
+      for (int r = 0; r < 4; ++r) {
+        const float x = e & 1 ? s[r][e / 2].y : s[r][e / 2].x, g = e & 1 ? dp[r][e / 2].y : dp[r][e / 2].x;
+        const bool on = 4 * ty + r < limit;
+        p[r][e] = on ? exp2f(x * c - lse) : 0.f;
+        ds[r][e] = on ? p[r][e] * (g - D) : 0.f;
       }
     }
     __syncthreads();
-    mm_wn<HDP>(dv, sS, sOr, ty, tx);
+    put_scores(sP, p, ty, tx);
+    put_scores(sS, ds, ty, tx);
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sS[(4 * tx + e) * LD + 4 * ty + r] = ds[r][e];
-    __syncthreads();
+    mm_wn<HDP>(dv, sP, sOr, ty, tx);
     mm_wn<HDP>(dk, sS, sQr, ty, tx);
   }
   const long long rows = (long long)a.seqs * a.kv_heads * a.lk;
@@ -780,7 +781,7 @@ static_assert(few_mma_smem(64) >= (FEW_NT / 32) * MMA_ROWS * (64 + 2) * 4, "the 
 
 constexpr int fwd_smem(int hdp) { return 4 * (2 * hdp * LD + TILE * (hdp + 4) + TILE * LD); }
 constexpr int dq_smem(int hdp) { return 4 * (4 * hdp * LD + TILE * (hdp + 4) + TILE * LD); }
-constexpr int dkv_smem(int hdp) { return 4 * (4 * hdp * LD + 2 * TILE * (hdp + 4) + TILE * LD); }
+constexpr int dkv_smem(int hdp) { return 4 * (4 * hdp * LD + 2 * TILE * (hdp + 4)); }
 static_assert(dkv_smem(128) <= 227 * 1024 && dq_smem(128) <= 227 * 1024, "shared memory of one CTA");
 
 // Parts of the walked axis (`tiles` long) for at least `want` CTAs, at most one part per tile.

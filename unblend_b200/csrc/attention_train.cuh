@@ -47,8 +47,9 @@ __device__ __forceinline__ int query_begin(const AttnArgs& a, const Bounds& b, i
   return a.causal ? max(0, j0 - b.off) : 0;
 }
 
-__device__ __forceinline__ bool sees(const AttnArgs& a, const Bounds& b, int i, int j) {
-  return i < b.ql && j < b.kl && (!a.causal || j <= i + b.off);
+// Query i sees keys [0, limit).
+__device__ __forceinline__ int key_limit(const AttnArgs& a, const Bounds& b, int i) {
+  return i < b.ql ? (a.causal ? min(b.kl, i + b.off + 1) : b.kl) : 0;
 }
 
 __device__ __forceinline__ long long head_offset(const UnblendHeadStrides& s, const AttnArgs& a, int seq, int h) {

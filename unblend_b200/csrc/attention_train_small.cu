@@ -208,10 +208,6 @@ __device__ __forceinline__ void put_rows(uint32_t stage, const uint32_t (&o)[HD 
   }
 }
 
-// Keys [0, limit) are seen by query i.
-__device__ __forceinline__ int key_limit(const AttnArgs& a, const Bounds& b, int i) {
-  return i < b.ql ? (a.causal ? min(b.kl, i + b.off + 1) : b.kl) : 0;
-}
 // Queries [first, end) see some key; the others, whatever they hold, count nowhere.
 struct Used {
   int first, end;
