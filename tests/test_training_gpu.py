@@ -331,7 +331,7 @@ def test_attention_ragged(causal, hd, t):
 @pytest.mark.parametrize("h,hk,hd", [(2, 2, 64), (4, 1, 64), (3, 3, 128), (4, 2, 128), (2, 1, 40), (3, 3, 72)])
 def test_attention_one_tile(h, hk, hd, t):
     """Sequences of up to 64 queries and keys, which 16-bit types do in one kernel: lengths, layouts, empty rows."""
-    for lq, lk in ((17, 33), (64, 64), (62, 62), (63, 9), (33, 64), (16, 48)):
+    for lq, lk in ((17, 33), (64, 64), (62, 62), (63, 9), (33, 64), (16, 48), (32, 32), (17, 31), (1, 30), (31, 1), (16, 16)):
         for causal in (False, True):
             _attn_case(*_attn(lq, lk, h, hk, hd, t, seed=lq + hd), causal=causal)
     # [outer, inner = bands, tokens]: rows, heads and sequences apart, and gaps between rows.
@@ -354,6 +354,23 @@ def test_attention_one_tile(h, hk, hd, t):
             a, c = min(max(int(ql[b]), 0), 60), min(max(int(kl[b]), 0), 64)
             assert not got["out"][b, a:].any() and not got["dq"][b, a:].any()
             assert not got["dk"][b, c:].any() and not got["dv"][b, c:].any()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("h,hk,hd", [(2, 2, 64), (6, 2, 48), (2, 1, 128)])
+def test_attention_half_tile_ragged(h, hk, hd, t, causal):
+    """Sequences of up to 32 queries and keys with lengths of their own; padding holds NaN."""
+    ql = torch.tensor([0, 1, 15, 16, 17, 31, 40, 30, 5, -1], device="cuda", dtype=torch.int32)
+    kl = torch.tensor([20, 0, 16, 32, 1, 29, 50, 9, 0, 17], device="cuda", dtype=torch.int32)
+    q, k, v, dout = _attn(31, 32, h, hk, hd, t, n=10)
+    for b in range(10):
+        a, c = min(max(int(ql[b]), 0), 31), min(max(int(kl[b]), 0), 32)
+        q[b, a:], dout[b, a:], k[b, c:], v[b, c:] = math.nan, math.inf, math.nan, math.inf
+        if c == 0 or (causal and a > c):  # queries that see no key
+            q[b, : a - c] = math.nan
+            dout[b, : a - c] = math.nan
+    _attn_case(q, k, v, dout, causal=causal, q_lens=ql, k_lens=kl)
 
 
 @pytest.mark.parametrize("t", [BF16, F16])

@@ -784,15 +784,21 @@ constexpr int dq_smem(int hdp) { return 4 * (4 * hdp * LD + TILE * (hdp + 4) + T
 constexpr int dkv_smem(int hdp) { return 4 * (4 * hdp * LD + 2 * TILE * (hdp + 4)); }
 static_assert(dkv_smem(128) <= 227 * 1024 && dq_smem(128) <= 227 * 1024, "shared memory of one CTA");
 
-// Parts of the walked axis (`tiles` long) for at least `want` CTAs, at most one part per tile.
-int split_count(long long units, long long tiles, long long want) {
-  if (units >= want || tiles <= 1) return 1;
-  long long n = (want + units - 1) / units;
-  if (n > tiles) n = tiles;
-  return (int)(n < MAX_PARTS ? n : MAX_PARTS);
+long long div_up(long long a, long long b) { return (a + b - 1) / b; }
+
+// Parts of the walked axis (`tiles` long) for units that do not fill the `slots` CTAs that run at once: as many as make
+// the last CTA end first, fewer where that is equal.
+int split_count(long long units, long long tiles, long long slots) {
+  if (units >= slots || tiles <= 1) return 1;
+  int best = 1;
+  long long least = tiles;
+  for (int n = 2; n <= tiles && n <= MAX_PARTS; ++n) {
+    const long long steps = div_up(units * n, slots) * div_up(tiles, n);
+    if (steps < least) least = steps, best = n;
+  }
+  return best;
 }
 
-long long div_up(long long a, long long b) { return (a + b - 1) / b; }
 long long round4(long long n) { return (n + 3) / 4 * 4; }
 
 // What a call runs on. A few rows per key/value head (forward): see attention_few_kernel. SMALL: sequences of one tile.
@@ -823,7 +829,10 @@ Plan plan_of(const UnblendAttnTrainParams& p, Path path) {
   if (tc && p.hd > 64 && p.lk > 1024 && p.lq > 128 && qh * div_up(p.lq, 256) >= sms) n.fwd_rows = 256;
   n.fwd_splits = n.fwd_rows == 256 ? 1 : split_count(qh * qt, kt, 2 * sms);
   // Few rows: CTAs of 128 keys at least, twice as many as run at once, for sequences of unequal lengths.
-  if (path == FEW) n.fwd_splits = split_count(kh, div_up(p.lk, 128), 4 * sms);
+  if (path == FEW) {
+    const long long most = div_up(p.lk, 128), fill = div_up(4 * sms, kh);
+    n.fwd_splits = (int)(fill < most ? (fill < MAX_PARTS ? fill : MAX_PARTS) : (most < MAX_PARTS ? most : MAX_PARTS));
+  }
   n.dq_splits = split_count(qh * qt, kt, tc ? sms : 2 * sms);
   n.dkv_splits = split_count(kh * kt, qt * group, tc ? sms : 2 * sms);
   return n;
@@ -1047,9 +1056,11 @@ extern "C" int unblend_attention_forward(const void* q, const void* k, const voi
   const void* ptrs[] = {q, k, v, out};
   const UnblendHeadStrides strides[] = {p->q, p->k, p->v, p->out};
   const int heads[] = {p->heads, p->kv_heads, p->kv_heads, p->heads}, rows[] = {p->lq, p->lk, p->lk, p->lq};
-  Path path = few_fits(*p, k, v) ? FEW
-              : attention_tc_fits(*p, ptrs, strides, heads, rows, 4) ? TENSOR_CORES : CUDA_CORES;
+  Path path = attention_tc_fits(*p, ptrs, strides, heads, rows, 4) ? TENSOR_CORES : CUDA_CORES;
   if (path == TENSOR_CORES && attention_is_small(*p, false)) path = SMALL;
+  // Few rows: shared heads read K and V once for the group (801 x 4 x 62, 8 over 2 heads of 64: 26 us, SMALL 33 us);
+  // without them a short sequence is better off as one tile (801 x 16 x 62, 8 heads: 88 us, SMALL 36 us).
+  if (few_fits(*p, k, v) && (path != SMALL || p->heads > p->kv_heads)) path = FEW;
   const Plan n = plan_of(*p, path);
   AttnArgs a = args_of(*p);
   a.q = q;

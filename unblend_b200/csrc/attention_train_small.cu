@@ -14,7 +14,7 @@
 // empty, with one round trip through TMEM after the other and nothing to overlap it within a sequence. What hides
 // latency here is several independent CTAs per SM.
 //
-// Four warps, 16 query rows each for S, dP and dQ; P and dS go through shared memory, and each warp takes 16 keys for
+// A warp has 16 query rows for S, dP and dQ; P and dS go through shared memory, and each warp takes 16 keys for
 // dK and dV. P and dS are rounded to the inputs' type, as the tensor cores take both operands in one 16-bit type; P of
 // fp16 calls is kept times 2^12 there (small probabilities would be subnormal). Softmax, D and all sums are fp32.
 // Results leave through shared memory in 16-byte chunks. 16-byte chunk c of a tile's row lies at c ^ (row & 7).
@@ -29,24 +29,24 @@ using namespace ub::train;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr int ROWS = 64;  // of a tile
-constexpr int NT = 128;
+constexpr int P_COLS = 64;  // pitch of P and dS
+
+// R: rows of a tile, 64, or 32 for shorter sequences; a warp per 16.
+constexpr int fwd_smem(int hd, int r) { return 3 * r * hd * 2; }
+constexpr int bwd_smem(int hd, int r, bool grouped) { return ((grouped ? 5 : 4) * r * hd + 2 * r * P_COLS) * 2; }
 
 // CTAs per SM, which is what hides latency. 801 x 62 x 62, 8 heads of 64, bf16: forward 39 us (5.2 TB/s) with 7 CTAs of
 // 72 registers, 43 us with 5 of 96 and with 8 of 64 (spills); backward 82 us (5.0 TB/s) with 4 of 128 (5 of 96, with dS
 // in V's place, were 1 us slower). Head dim 128: 70 and 184 us. Earlier versions of 48 and 85 us were slower with two
 // warps of 32 rows each, which load half the fragments (51 and 101 us), and with the products of 16-key blocks behind
 // the sequence left out (56 and 95 us: the branches kept loads and products from overlapping).
-constexpr int fwd_ctas(int hd) { return hd == 64 ? 7 : 4; }
-constexpr int bwd_ctas(int hd, bool grouped) { return hd == 64 ? (grouped ? 3 : 4) : 2; }
+constexpr int fwd_ctas(int hd, int r) { return hd == 64 ? 7 * 64 / r : 4; }
+constexpr int bwd_ctas(int hd, int r, bool grouped) { return hd == 64 ? (grouped ? 3 : 4) * 64 / r : 2; }
 
 struct SmallArgs {
   AttnArgs a;
   FastDiv by_heads, by_group, by_inner;  // by_heads: of the CTAs
 };
-
-constexpr int fwd_smem(int hd) { return 3 * ROWS * hd * 2; }
-constexpr int bwd_smem(int hd, bool grouped) { return ((grouped ? 5 : 4) * ROWS * hd + 2 * ROWS * ROWS) * 2; }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -84,17 +84,18 @@ __device__ __forceinline__ char* head_at(const SmallArgs& s, const void* p, cons
 }
 
 // Rows [first, end) of a head by cp.async; the rest of the tile is 0.
-template <int HD>
+template <int HD, int R>
 __device__ __forceinline__ void fetch(uint32_t tile, const char* src, const UnblendHeadStrides& t, int first, int end,
                                       int hd) {
-  constexpr int CH = HD / 8, STEP = NT / CH;  // STEP is a multiple of 8: a thread's chunk keeps its place
+  constexpr int CH = HD / 8, STEP = 2 * R / CH;
+  static_assert(STEP % 8 == 0, "a thread's chunk keeps its place");
   const int r = threadIdx.x / CH, c = threadIdx.x % CH;
   const uint32_t stride = 2 * (uint32_t)t.row;
   const int mine = 8 * c < hd ? end : 0, last = max(mine - 1, 0);
   tile += r * (2 * HD) + ((c ^ (r & 7)) * 16);
   src += 8 * c < hd ? 16 * c : 0;
 #pragma unroll
-  for (int x = 0; x < ROWS / STEP; ++x) {
+  for (int x = 0; x < R / STEP; ++x) {
     const int row = r + x * STEP;
     cp_async16_or_zero(tile + x * STEP * 2 * HD, src + min(row, last) * stride, row >= first && row < mine);
   }
@@ -109,16 +110,16 @@ __device__ __forceinline__ uint32_t block(uint32_t tile, int r0, int c) {
   return tile + r0 * (2 * COLS) + (at ^ (c * 16));
 }
 
-// d[16 x 64] = A[rows r0 ..][HD] B[64][HD]^T, both tiles as they lie.
-template <typename T, int HD>
-__device__ __forceinline__ void rows_dot(float (&d)[ROWS / 8][4], uint32_t ta, int r0, uint32_t tb) {
+// d[16 x R] = A[rows r0 ..][HD] B[R][HD]^T, both tiles as they lie.
+template <typename T, int HD, int R>
+__device__ __forceinline__ void rows_dot(float (&d)[R / 8][4], uint32_t ta, int r0, uint32_t tb) {
   clear(d);
 #pragma unroll
   for (int ks = 0; ks < HD / 16; ++ks) {
     uint32_t af[4], f[4];
     ldmatrix4(af, block<HD, true>(ta, r0, 2 * ks));
 #pragma unroll
-    for (int n = 0; n < ROWS / 16; ++n) {
+    for (int n = 0; n < R / 16; ++n) {
       ldmatrix4(f, block<HD, false>(tb, 16 * n, 2 * ks));
       mma16(d[2 * n], af, f[0], f[1], T());
       mma16(d[2 * n + 1], af, f[2], f[3], T());
@@ -138,13 +139,13 @@ __device__ __forceinline__ void rows_sum(float (&d)[HD / 8][4], const uint32_t (
   }
 }
 
-// d[16 x HD] += A^T B with A[64][64] (its columns r0 ..) and B[64][HD].
-template <typename T, int HD>
+// d[16 x HD] += A^T B with A[R][R] (its columns r0 ..) and B[R][HD].
+template <typename T, int HD, int R>
 __device__ __forceinline__ void columns_sum(float (&d)[HD / 8][4], uint32_t ta, int r0, uint32_t tb) {
 #pragma unroll
-  for (int ks = 0; ks < ROWS / 16; ++ks) {
+  for (int ks = 0; ks < R / 16; ++ks) {
     uint32_t f[4];
-    ldmatrix4_trans(f, block<ROWS, false>(ta, 16 * ks, r0 / 8));
+    ldmatrix4_trans(f, block<P_COLS, false>(ta, 16 * ks, r0 / 8));
     rows_sum<T, HD>(d, f, tb, 16 * ks);
   }
 }
@@ -220,26 +221,26 @@ __device__ __forceinline__ int keys_of_all(const AttnArgs& a, const Bounds& b, i
   return r0 + 16 <= b.ql ? key_limit(a, b, r0) : 0;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(NT, fwd_ctas(HD))
+template <typename T, int HD, int R>
+__global__ void __launch_bounds__(2 * R, fwd_ctas(HD, R))
     attention_small_fwd_kernel(const __grid_constant__ SmallArgs args) {
   const AttnArgs& a = args.a;
-  constexpr uint32_t TILE = ROWS * HD * 2;
+  constexpr uint32_t TILE = R * HD * 2;
   extern __shared__ __align__(128) uint8_t small_smem[];
   const uint32_t tq = smem_at(small_smem), tk = tq + TILE, tv = tk + TILE;
   const int lane = threadIdx.x & 31, r0 = (threadIdx.x >> 5) * 16, quad = lane >> 2, ql = lane & 3;
   const int seq = args.by_heads(blockIdx.x), h = blockIdx.x - seq * a.heads, hk = args.by_group(h);
   const Bounds b = bounds_of(a, seq);
   const Used rows = used_queries(a, b);
-  fetch<HD>(tq, head_at(args, a.q, a.q_s, seq, h), a.q_s, rows.first, rows.end, a.hd);
-  fetch<HD>(tk, head_at(args, a.k, a.k_s, seq, hk), a.k_s, 0, b.kl, a.hd);
+  fetch<HD, R>(tq, head_at(args, a.q, a.q_s, seq, h), a.q_s, rows.first, rows.end, a.hd);
+  fetch<HD, R>(tk, head_at(args, a.k, a.k_s, seq, hk), a.k_s, 0, b.kl, a.hd);
   cp_commit();
-  fetch<HD>(tv, head_at(args, a.v, a.v_s, seq, hk), a.v_s, 0, b.kl, a.hd);
+  fetch<HD, R>(tv, head_at(args, a.v, a.v_s, seq, hk), a.v_s, 0, b.kl, a.hd);
   cp_commit();
   cp_wait<1>();
   __syncthreads();
-  float s[ROWS / 8][4], inv[2];
-  rows_dot<T, HD>(s, tq, r0, tk);
+  float s[R / 8][4], inv[2];
+  rows_dot<T, HD, R>(s, tq, r0, tk);
   const float c = a.scale * LOG2E;
   const int all = keys_of_all(a, b, r0);
 #pragma unroll
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(NT, fwd_ctas(HD))
     const int i = r0 + quad + 8 * x, limit = key_limit(a, b, i);
     float top = -INFINITY;
 #pragma unroll
-    for (int n = 0; n < ROWS / 8; ++n) {
+    for (int n = 0; n < R / 8; ++n) {
       float &z0 = s[n][2 * x], &z1 = s[n][2 * x + 1];
       if (8 * n + 8 > all) {
         z0 = 8 * n + 2 * ql < limit ? z0 : -INFINITY;
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(NT, fwd_ctas(HD))
     const float base = top == -INFINITY ? 0.f : -top;
     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int n = 0; n < ROWS / 8; ++n) {
+    for (int n = 0; n < R / 8; ++n) {
       float &z0 = s[n][2 * x], &z1 = s[n][2 * x + 1];
       const float2 z = ub::fma2(make_float2(z0, z1), make_float2(c, c), make_float2(base, base));
       z0 = ex2(z.x);
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(NT, fwd_ctas(HD))
   float o[HD / 8][4];
   clear(o);
 #pragma unroll
-  for (int ks = 0; ks < ROWS / 16; ++ks) {
+  for (int ks = 0; ks < R / 16; ++ks) {
     uint32_t pf[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -295,11 +296,11 @@ __global__ void __launch_bounds__(NT, fwd_ctas(HD))
 }
 
 // GROUPED: a CTA walks the query heads of its key/value head and keeps dK and dV in registers.
-template <typename T, int HD, bool GROUPED>
-__global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
+template <typename T, int HD, int R, bool GROUPED>
+__global__ void __launch_bounds__(2 * R, bwd_ctas(HD, R, GROUPED))
     attention_small_bwd_kernel(const __grid_constant__ SmallArgs args) {
   const AttnArgs& a = args.a;
-  constexpr uint32_t TILE = ROWS * HD * 2, P_TILE = ROWS * ROWS * 2;
+  constexpr uint32_t TILE = R * HD * 2, P_TILE = R * P_COLS * 2;
   constexpr float P_SCALE = std::is_same<T, __half>::value ? 4096.f : 1.f;
   extern __shared__ __align__(128) uint8_t small_smem[];
   const uint32_t tk = smem_at(small_smem), tv = tk + TILE, tq = tv + TILE, td = tq + TILE;
@@ -319,12 +320,12 @@ __global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
   for (int g = 0; g < (GROUPED ? a.group : 1); ++g) {
     const int h = GROUPED ? hk * a.group + g : hk;
     if (g > 0) __syncthreads();  // the last head's tiles have been read
-    fetch<HD>(tq, head_at(args, a.q, a.q_s, seq, h), a.q_s, rows.first, rows.end, a.hd);
-    if (g == 0) fetch<HD>(tk, head_at(args, a.k, a.k_s, seq, hk), a.k_s, 0, b.kl, a.hd);
+    fetch<HD, R>(tq, head_at(args, a.q, a.q_s, seq, h), a.q_s, rows.first, rows.end, a.hd);
+    if (g == 0) fetch<HD, R>(tk, head_at(args, a.k, a.k_s, seq, hk), a.k_s, 0, b.kl, a.hd);
     cp_commit();
-    fetch<HD>(td, head_at(args, a.dout, a.dout_s, seq, h), a.dout_s, rows.first, rows.end, a.hd);
-    fetch<HD>(to, head_at(args, a.out_in, a.out_s, seq, h), a.out_s, rows.first, rows.end, a.hd);
-    if (g == 0) fetch<HD>(tv, head_at(args, a.v, a.v_s, seq, hk), a.v_s, 0, b.kl, a.hd);
+    fetch<HD, R>(td, head_at(args, a.dout, a.dout_s, seq, h), a.dout_s, rows.first, rows.end, a.hd);
+    fetch<HD, R>(to, head_at(args, a.out_in, a.out_s, seq, h), a.out_s, rows.first, rows.end, a.hd);
+    if (g == 0) fetch<HD, R>(tv, head_at(args, a.v, a.v_s, seq, hk), a.v_s, 0, b.kl, a.hd);
     cp_commit();
     float base[2];
     const float* lse = a.lse + ((long long)seq * a.heads + h) * a.lq;
@@ -336,13 +337,13 @@ __global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
     }
     cp_wait<1>();
     __syncthreads();
-    float s[ROWS / 8][4], dp[ROWS / 8][4];
-    rows_dot<T, HD>(s, tq, r0, tk);
+    float s[R / 8][4], dp[R / 8][4];
+    rows_dot<T, HD, R>(s, tq, r0, tk);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int limit = key_limit(a, b, r0 + quad + 8 * x);
 #pragma unroll
-      for (int n = 0; n < ROWS / 8; ++n) {
+      for (int n = 0; n < R / 8; ++n) {
         float &z0 = s[n][2 * x], &z1 = s[n][2 * x + 1];
         const float2 z = ub::fma2(make_float2(z0, z1), make_float2(c, c), make_float2(base[x], base[x]));
         z0 = ex2(z.x);
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
     }
     cp_wait<0>();
     __syncthreads();
-    rows_dot<T, HD>(dp, td, r0, tv);
+    rows_dot<T, HD, R>(dp, td, r0, tv);
     float D[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) D[x] = row_product<T, HD>(td, to, r0 + quad + 8 * x);
@@ -363,15 +364,15 @@ __global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
       __syncthreads();  // O's rows lie under other warps' rows of P and dS
     else
       __syncwarp();
-    uint32_t sf[ROWS / 16][4];  // dS as A fragments
-    const uint32_t at = (r0 + quad) * (2 * ROWS) + quad * 16 + ql * 4;
+    uint32_t sf[R / 16][4];  // dS as A fragments
+    const uint32_t at = (r0 + quad) * (2 * P_COLS) + quad * 16 + ql * 4;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
 #pragma unroll
-      for (int n = 0; n < ROWS / 8; ++n) {
+      for (int n = 0; n < R / 8; ++n) {
         const float2 p = make_float2(s[n][2 * x], s[n][2 * x + 1]);
         const float2 e = mul2(p, add2(make_float2(dp[n][2 * x], dp[n][2 * x + 1]), make_float2(-D[x], -D[x])));
-        const uint32_t w = pack_pair<T>(e.x, e.y), put = (at ^ (n * 16)) + x * 8 * (2 * ROWS);
+        const uint32_t w = pack_pair<T>(e.x, e.y), put = (at ^ (n * 16)) + x * 8 * (2 * P_COLS);
         sf[n / 2][2 * (n & 1) + x] = w;
         sts4(tp + put, pack_pair<T>(p.x * P_SCALE, p.y * P_SCALE));
         sts4(ts + put, w);
@@ -382,14 +383,14 @@ __global__ void __launch_bounds__(NT, bwd_ctas(HD, GROUPED))
       float dq[HD / 8][4];
       clear(dq);
 #pragma unroll
-      for (int ks = 0; ks < ROWS / 16; ++ks) rows_sum<T, HD>(dq, sf[ks], tk, 16 * ks);
+      for (int ks = 0; ks < R / 16; ++ks) rows_sum<T, HD>(dq, sf[ks], tk, 16 * ks);
       pack_rows<T>(packed, dq, a.scale, a.scale);
     }
     __syncthreads();  // P and dS are written, K and V are read
     put_rows<HD>(stage, packed, head_at(args, a.dq, a.dq_s, seq, h), a.dq_s, r0, a.lq, a.hd,
                  [&](int i) { return key_limit(a, b, i) > 0; });
-    columns_sum<T, HD>(dv, tp, r0, td);
-    columns_sum<T, HD>(dk, ts, r0, tq);
+    columns_sum<T, HD, R>(dv, tp, r0, td);
+    columns_sum<T, HD, R>(dk, ts, r0, tq);
   }
   auto counts = [&](int j) { return j < b.kl; };
   uint32_t packed[HD / 8][2];
@@ -403,29 +404,41 @@ SmallArgs small_args(const AttnArgs& a, int heads) {
   return SmallArgs{a, fast_div(heads), fast_div(a.group), fast_div(a.inner)};
 }
 
-template <typename T, int HD>
+template <typename T, int HD, int R>
 int launch_fwd(const AttnArgs& a, cudaStream_t st) {
-  constexpr int bytes = fwd_smem(HD);
-  if (allow_smem<attention_small_fwd_kernel<T, HD>>(bytes) != cudaSuccess) return (int)cudaGetLastError();
-  attention_small_fwd_kernel<T, HD><<<(unsigned)(a.seqs * a.heads), NT, bytes, st>>>(small_args(a, a.heads));
+  constexpr int bytes = fwd_smem(HD, R);
+  if (allow_smem<attention_small_fwd_kernel<T, HD, R>>(bytes) != cudaSuccess) return (int)cudaGetLastError();
+  const unsigned grid = (unsigned)(a.seqs * a.heads);
+  attention_small_fwd_kernel<T, HD, R><<<grid, 2 * R, bytes, st>>>(small_args(a, a.heads));
   UB_CHECK_LAUNCH();
   return 0;
 }
 
-template <typename T, int HD, bool GROUPED>
+template <typename T, int HD, int R, bool GROUPED>
 int launch_bwd(const AttnArgs& a, cudaStream_t st) {
-  constexpr int bytes = bwd_smem(HD, GROUPED);
-  if (allow_smem<attention_small_bwd_kernel<T, HD, GROUPED>>(bytes) != cudaSuccess) return (int)cudaGetLastError();
+  constexpr int bytes = bwd_smem(HD, R, GROUPED);
+  if (allow_smem<attention_small_bwd_kernel<T, HD, R, GROUPED>>(bytes) != cudaSuccess) return (int)cudaGetLastError();
   const unsigned grid = (unsigned)(a.seqs * a.kv_heads);
-  attention_small_bwd_kernel<T, HD, GROUPED><<<grid, NT, bytes, st>>>(small_args(a, a.kv_heads));
+  attention_small_bwd_kernel<T, HD, R, GROUPED><<<grid, 2 * R, bytes, st>>>(small_args(a, a.kv_heads));
   UB_CHECK_LAUNCH();
   return 0;
+}
+
+// Tiles of 32 rows take a quarter of the products: 801 x 32 x 32, 8 heads of 64, bf16 19 us forward (5.6 TB/s) and 38 us
+// backward (4.9 TB/s); 801 x 17 x 17 17 and 33 us, with tiles of 64 rows 33 and 74 us.
+bool half_tiles(const AttnArgs& a) { return a.lq <= 32 && a.lk <= 32; }
+
+template <typename T>
+int forward_types(const AttnArgs& a, cudaStream_t st) {
+  if (a.hd > 64) return launch_fwd<T, 128, 64>(a, st);
+  return half_tiles(a) ? launch_fwd<T, 64, 32>(a, st) : launch_fwd<T, 64, 64>(a, st);
 }
 
 template <typename T>
 int backward_types(const AttnArgs& a, cudaStream_t st) {
-  if (a.hd > 64) return launch_bwd<T, 128, false>(a, st);
-  return a.group > 1 ? launch_bwd<T, 64, true>(a, st) : launch_bwd<T, 64, false>(a, st);
+  if (a.hd > 64) return launch_bwd<T, 128, 64, false>(a, st);
+  if (a.group > 1) return half_tiles(a) ? launch_bwd<T, 64, 32, true>(a, st) : launch_bwd<T, 64, 64, true>(a, st);
+  return half_tiles(a) ? launch_bwd<T, 64, 32, false>(a, st) : launch_bwd<T, 64, 64, false>(a, st);
 }
 
 }  // namespace
@@ -434,7 +447,7 @@ namespace ub {
 namespace train {
 
 bool attention_is_small(const UnblendAttnTrainParams& p, bool backward) {
-  if (p.lq > ROWS || p.lk > ROWS || (backward && p.hd > 64 && p.heads > p.kv_heads)) return false;
+  if (p.lq > 64 || p.lk > 64 || (backward && p.hd > 64 && p.heads > p.kv_heads)) return false;
   // 32-bit byte offsets within a head (the row stride of a tensor of one row is not used).
   constexpr long long MOST = 1LL << 24;
   for (const UnblendHeadStrides* t : {&p.q, &p.out, &p.dout, &p.dq})
@@ -445,9 +458,7 @@ bool attention_is_small(const UnblendAttnTrainParams& p, bool backward) {
 }
 
 int attention_small_forward(const AttnArgs& a, const UnblendAttnTrainParams& p, cudaStream_t st) {
-  if (p.dtype == UNBLEND_BF16)
-    return a.hd <= 64 ? launch_fwd<__nv_bfloat16, 64>(a, st) : launch_fwd<__nv_bfloat16, 128>(a, st);
-  return a.hd <= 64 ? launch_fwd<__half, 64>(a, st) : launch_fwd<__half, 128>(a, st);
+  return p.dtype == UNBLEND_BF16 ? forward_types<__nv_bfloat16>(a, st) : forward_types<__half>(a, st);
 }
 
 int attention_small_backward(const AttnArgs& a, const UnblendAttnTrainParams& p, cudaStream_t st) {
