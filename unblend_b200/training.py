@@ -352,7 +352,8 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     """``(dq, dk, dv)`` from the gradient of ``out``, the inputs and the results of ``attention_forward``.
 
     The probabilities are computed again from q, k and ``lse``; dk and dv are summed over the query heads that share a
-    head. The gradients are contiguous; rows behind the lengths are 0.
+    head. The gradients are contiguous; rows behind the lengths are 0. Keys that are processed in blocks may give each
+    block ``out`` and ``lse`` of all of them: dk and dv are then the block's rows, and the blocks' dq add up.
     """
     scale = _check_attention(q, k, v, scale, causal, q_lens, k_lens)
     for name, t in (("dout", dout), ("out", out)):
