@@ -790,13 +790,14 @@ long long div_up(long long a, long long b) { return (a + b - 1) / b; }
 // the last CTA end first, fewer where that is equal.
 int split_count(long long units, long long tiles, long long slots) {
   if (units >= slots || tiles <= 1) return 1;
-  int best = 1;
-  long long least = tiles;
-  for (int n = 2; n <= tiles && n <= MAX_PARTS; ++n) {
-    const long long steps = div_up(units * n, slots) * div_up(tiles, n);
-    if (steps < least) least = steps, best = n;
+  long long best = 1, least = tiles;
+  const long long most = tiles < MAX_PARTS ? tiles : MAX_PARTS;
+  for (int waves = 1; waves <= 4; ++waves) {
+    const long long n = slots * waves / units, part = div_up(tiles, n < most ? n : most);  // n >= 1: units < slots
+    if (waves * part < least) least = waves * part, best = div_up(tiles, part);
+    if (n >= most) break;
   }
-  return best;
+  return (int)best;
 }
 
 long long round4(long long n) { return (n + 3) / 4 * 4; }

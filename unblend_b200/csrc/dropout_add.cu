@@ -350,9 +350,11 @@ int launch(const DropArgs& a, int dtype, int r_dtype, int w_dtype, Path path, in
   return launch_streams<__half, BWD>(a, r_dtype, w_dtype, path, parts, st);
 }
 
+constexpr int FLAT_COLS = 1 << 22;
+
 // One run of values. Very wide rows are left to the other kernels: each of the VEC rows of partial sums is as wide.
 bool contiguous(const RowMap& m, long long outer, int cols) {
-  return (m.inner <= 1 || m.si == cols) && (outer <= 1 || m.so == (long long)m.inner * cols) && cols <= (1 << 22);
+  return (m.inner <= 1 || m.si == cols) && (outer <= 1 || m.so == (long long)m.inner * cols) && cols <= FLAT_COLS;
 }
 
 void set_p(DropArgs* a, double p) {
@@ -373,7 +375,7 @@ extern "C" int unblend_dropout_add_grad_workspace(long long rows, int cols, long
       const unsigned v = vec_shape(rows, cols, vec).grid.y;
       parts = v > parts ? v : parts;
     }
-  for (int vec = 4; vec <= 8; vec += 4) {
+  for (int vec = 4; vec <= 8 && cols <= FLAT_COLS; vec += 4) {
     const long long m = flat_runs(rows, cols, vec, FLAT_SUM_CTAS);
     const long long v = flat_joins(cols, vec) ? (m * cols + 255) / 256 : m * vec;
     parts = v > parts ? (unsigned)v : parts;
