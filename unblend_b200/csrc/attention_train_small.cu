@@ -38,8 +38,8 @@ constexpr int fwd_smem(int hd, int r) { return 3 * r * hd * 2; }
 constexpr int bwd_smem(int hd, int r, bool grouped) { return ((grouped ? 5 : 4) * r * hd + 2 * r * P_COLS) * 2; }
 
 // CTAs per SM, which is what hides latency. 801 x 62 x 62, 8 heads of 64, bf16: forward 39 us (5.2 TB/s) with 7 CTAs of
-// 72 registers, 43 us with 5 of 96 and with 8 of 64 (spills); backward 82 us (5.0 TB/s) with 4 of 128 (5 of 96, with dS
-// in V's place, were 1 us slower). Head dim 128: 70 and 184 us. Earlier versions of 48 and 85 us were slower with two
+// 72 registers, 43 us with 5 of 96 and with 8 of 64 (spills); backward 80 us (5.1 TB/s) with 4 of 128 (5 of 96, with dS
+// in V's place, were 1 us slower). Head dim 128: 70 and 171 us. Earlier versions of 48 and 85 us were slower with two
 // warps of 32 rows each, which load half the fragments (51 and 101 us), and with the products of 16-key blocks behind
 // the sequence left out (56 and 95 us: the branches kept loads and products from overlapping).
 constexpr int fwd_ctas(int hd, int r) { return hd == 64 ? 7 * 64 / r : 4; }
