@@ -616,6 +616,7 @@ extern "C" int unblend_layer_norm_forward(const void* x, long long x_so, long lo
                                           const void* gamma, const void* beta, float eps, long long outer,
                                           long long inner, int cols, int dtype, int w_dtype, void* stream) {
   UB_REQUIRE(x && y && stats && rows_ok(outer, inner, cols) && types_ok(dtype, w_dtype) && eps >= 0.f);
+  UB_REQUIRE(reinterpret_cast<uintptr_t>(stats) % sizeof(float2) == 0);
   NormArgs a{};
   a.x = x;
   a.y = y;
@@ -638,6 +639,7 @@ extern "C" int unblend_layer_norm_backward(const void* dy, long long dy_so, long
                                            void* dx, void* dgamma, void* dbeta, float* work, long long outer,
                                            long long inner, int cols, int dtype, int w_dtype, void* stream) {
   UB_REQUIRE(dy && x && stats && dx && rows_ok(outer, inner, cols) && types_ok(dtype, w_dtype));
+  UB_REQUIRE(reinterpret_cast<uintptr_t>(stats) % sizeof(float2) == 0);
   UB_REQUIRE((dgamma != nullptr) == (dbeta != nullptr) && (!dgamma || work || !joins(outer * inner, cols)));
   NormArgs a{};
   a.x = x;

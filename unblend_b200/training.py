@@ -203,6 +203,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, 
     if gamma is not None:
         gamma = gamma.contiguous()
     stats = stats.contiguous()
+    if stats.data_ptr() % 8:  # a row's two values are one access; a slice of a larger buffer may lie between
+        stats = stats.clone()
     (xr, outer, inner, x_so, x_si), (dyr, _, _, d_so, d_si) = _same_split(_rows(x), _rows(dy))
     work = _scratch(x, _workspace_bytes("unblend_layer_norm_grad_workspace", n, cols)) if weight_grads else None
     _launch(x, "unblend_layer_norm_backward", dyr.data_ptr(), d_so, d_si, xr.data_ptr(), x_so, x_si,
