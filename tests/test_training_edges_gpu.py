@@ -1,0 +1,63 @@
+"""Calls of the training operators at the edge of what they allow, on the GPU against their 64-bit definitions."""
+
+from __future__ import annotations
+
+
+import pytest
+import torch
+
+from training_reference import assert_within, attention_reference, norm_reference
+from unblend_b200 import _lib, training
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _rand(*shape, seed, t=F32, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).to(t)
+
+
+def _attn(n, lq, lk, h, hk, hd, t, seed=0):
+    return (_rand(n, lq, h, hd, seed=seed, t=t), _rand(n, lk, hk, hd, seed=seed + 1, t=t),
+            _rand(n, lk, hk, hd, seed=seed + 2, t=t), _rand(n, lq, h, hd, seed=seed + 3, t=t))
+
+
+def test_norm_statistics_inside_a_larger_buffer():
+    """``stats`` on either 4-byte boundary gives the gradients that the forward's own tensor gives."""
+    x, dy, gamma = _rand(37, 200, seed=1), _rand(37, 200, seed=2), _rand(200, seed=3)
+    y, stats = training.layer_norm_forward(x, gamma)
+    want = training.layer_norm_backward(dy, x, stats, gamma)
+    for at in (0, 1, 2, 3):
+        buf = torch.zeros(37 * 2 + 4, device="cuda")
+        view = buf[at:at + 74].view(37, 2)
+        view.copy_(stats)
+        for a, b in zip(training.layer_norm_backward(dy, x, view, gamma), want):
+            assert torch.equal(a, b)
+    for name, got in (("dx", want[0]), ("dgamma", want[1])):
+        assert_within(name, got.reshape(norm_reference(x, gamma, None, 1e-5, dy)[name][0].shape),
+                      *norm_reference(x, gamma, None, 1e-5, dy)[name])
+
+
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_calls_end_with_everything_used(hd, t):
+    """CTAs whose last unit leaves any number of tiles in their rings (none, one, fewer and more than the ring holds):
+    many calls behind one another, none of which may find what the one before left."""
+    lk = 1200
+    kl = torch.tensor([0, 1, 128, 129, 256, 400, 512, 640, 900, lk], device="cuda", dtype=torch.int32)
+    q, k, v, dout = _attn(10, 130, lk, 2, 1, hd, t)
+    first = None
+    for _ in range(20):
+        out, lse = training.attention_forward(q, k, v, k_lens=kl)
+        got = (out, *training.attention_backward(dout, q, k, v, out, lse, k_lens=kl))
+        first = first or [x.clone() for x in got]
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+    none = torch.zeros_like(kl)
+    out, lse = training.attention_forward(q, k, v, k_lens=none)
+    assert not out.any() and not any(x.any() for x in training.attention_backward(dout, q, k, v, out, lse, k_lens=none))
+    assert _lib.error_flag() == 0
+    ref = attention_reference(q, k, v, dout, k_lens=kl)
+    for name, x in zip(("out", "dq", "dk", "dv"), first):
+        assert_within(name, x, *ref[name])

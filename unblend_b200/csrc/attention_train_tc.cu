@@ -14,7 +14,10 @@
 // statistics and all sums are fp32. 2^x is the hardware approximation (2 ulp).
 //
 // A thread owns a row (or half a row), so row maxima and sums need no shuffles. One warp issues TMA, one the MMAs;
-// every barrier wait gives up after two seconds and sets the error flag.
+// every barrier wait gives up after two seconds and sets the error flag. A warp gives up as a whole (its lanes vote), as
+// the instructions behind a wait need all of them, and a CTA leaves only when what it started is done: the TMA warp
+// waits until its last copies have been used, or, after a wait that ran out, until they have landed; a MMA warp that
+// gives up waits for the products that it issued.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
@@ -123,6 +126,32 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
+}
+
+// A wait of a whole warp: true for all lanes or for none.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// The end of a TMA warp's work (one lane): `n` tiles went through a ring of STAGES, `nr` through the resident tiles.
+// All of them have been used, `ok`, or at least nothing is in flight any more.
+template <int STAGES>
+__device__ __forceinline__ bool drain_tma(bool ok, uint64_t* full, uint64_t* empty, int n, uint64_t* res_full,
+                                          uint64_t* res_free, int nr) {
+  const int first = n > STAGES ? n - STAGES : 0;
+  for (int i = first; ok && i < n; ++i) ok = mbar_wait(&empty[i % STAGES], (i / STAGES) & 1);
+  if (ok && nr > 0) ok = mbar_wait(res_free, (nr - 1) & 1);
+  if (ok) return true;
+  for (int i = first; i < n; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+  if (nr > 0) mbar_wait(res_full, (nr - 1) & 1);
+  return false;
+}
+
+// A MMA warp that gives up (all lanes): the products that it issued are complete.
+__device__ __forceinline__ void drain_mma(uint64_t* idle) {
+  if (elect_one()) umma_commit(idle);
+  __syncwarp();
+  warp_wait(idle, 0);
 }
 
 // Moves a warpgroup's registers per thread; the warpgroups' shares of a CTA add up to what it was launched with.
@@ -322,7 +351,8 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
   uint64_t* p_ready = s_full + NQ;         // [NQ]
   uint64_t* pv_done = p_ready + NQ;        // [NQ]
   uint64_t* o_free = pv_done + NQ;         // [NQ]
-  uint32_t* slot = reinterpret_cast<uint32_t*>(o_free + NQ);
+  uint64_t* idle = o_free + NQ;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(idle + 1);
 
   const AttnArgs& a = ta.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -336,6 +366,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
       mbar_init(&pv_done[h], 1);
       mbar_init(&o_free[h], 4);
     }
+    mbar_init(idle, 1);
     fence_mbar_init();
   }
   if (warp == NQ * 4 + 1) tmem_alloc(slot, C::TMEM);
@@ -390,6 +421,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
           const int hk = u.h / a.group;
           for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u) && load(&mv, t * C::BN, hk, u);
         }
+        ok = drain_tma<C::STAGES>(ok, full, empty, it, q_full, q_free, nq);
         if (!ok) atomicExch(&g_error_flag, 11);
       }
     } else if (warp == NQ * 4 + 1) {
@@ -411,7 +443,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
           if (t0 >= t1) continue;
           const int n = t1 - t0;
           // K of tile t is ring tile it + 2 t, V is it + 2 t + 1.
-          if (!mbar_wait(q_full, nq & 1) || !mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1)) {
+          if (!warp_wait(q_full, nq & 1) || !warp_wait(&full[it % C::STAGES], (it / C::STAGES) & 1)) {
             ok = false;
             break;
           }
@@ -430,15 +462,15 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
           for (int t = 0; t < n && ok; ++t) {
             const int vi = it + 2 * t + 1, ki = vi + 1;
             const bool more = t + 1 < n;
-            if (!mbar_wait(&full[vi % C::STAGES], (vi / C::STAGES) & 1) ||
-                (more && !mbar_wait(&full[ki % C::STAGES], (ki / C::STAGES) & 1))) {
+            if (!warp_wait(&full[vi % C::STAGES], (vi / C::STAGES) & 1) ||
+                (more && !warp_wait(&full[ki % C::STAGES], (ki / C::STAGES) & 1))) {
               ok = false;
               break;
             }
 #pragma unroll
             for (int h = 0; h < NQ; ++h) {
-              if (ok && t == 0 && units > 0 && !mbar_wait(&o_free[h], (units - 1) & 1)) ok = false;
-              if (ok && !mbar_wait(&p_ready[h], g & 1)) ok = false;
+              if (ok && t == 0 && units > 0 && !warp_wait(&o_free[h], (units - 1) & 1)) ok = false;
+              if (ok && !warp_wait(&p_ready[h], g & 1)) ok = false;
               if (!ok) break;
               tc_fence_after();
               const uint32_t d = tmem + h * 256;
@@ -466,7 +498,10 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
           it += 2 * n;
           ++units;
         }
-        if (!ok && lane == 0) atomicExch(&g_error_flag, 12);
+        if (!ok) {
+          drain_mma(idle);
+          if (lane == 0) atomicExch(&g_error_flag, 12);
+        }
       }
     }
   } else {
@@ -494,7 +529,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
       float2 sum2 = make_float2(0.f, 0.f);
       for (int t = t0; t < t1; ++t, ++g) {
         const int j0 = t * C::BN;
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[h], g & 1))) {
+        if (!warp_wait(&s_full[h], g & 1)) {
           ok = false;
           break;
         }
@@ -510,7 +545,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
           // V rows behind the length (NaN included) must be 0 before P V. Query tile 0 goes first.
           if (h == 0 && a.k_lens && j0 + C::BN > b.kl) {
             const int vi = it + 2 * (t - t0) + 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(&full[vi % C::STAGES], (vi / C::STAGES) & 1))) {
+            if (!warp_wait(&full[vi % C::STAGES], (vi / C::STAGES) & 1)) {
               ok = false;
               break;
             }
@@ -542,7 +577,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
         }
         if (__any_sync(0xffffffffu, rescale)) {
           // O holds the sums up to tile t - 1: they are complete once their product has signalled.
-          if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[h], (g - 1) & 1))) {
+          if (!warp_wait(&pv_done[h], (g - 1) & 1)) {
             ok = false;
             break;
           }
@@ -574,7 +609,7 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
       const float inv = live ? 1.f / sum : 0.f;
       const long long orow = ((long long)u.seq * a.heads + u.h) * a.lq + i;
       if (t0 < t1) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[h], (g - 1) & 1))) {
+        if (!warp_wait(&pv_done[h], (g - 1) & 1)) {
           ok = false;
           break;
         }
@@ -611,7 +646,11 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
           a.lse[orow] = lse;
       }
     }
-    if (!ok) atomicExch(&g_error_flag, 13);
+    if (!ok) {
+      tmem_wait_ld();
+      tmem_st_wait();
+      atomicExch(&g_error_flag, 13);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -734,7 +773,8 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
   uint64_t* ds_ready = dp_free + 1;
   uint64_t* dq_done = ds_ready + 2;
   uint64_t* dq_free = dq_done + 1;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(dq_free + 1);
+  uint64_t* idle = dq_free + 1;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(idle + 1);
 
   const AttnArgs& a = ta.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -748,6 +788,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
     mbar_init(&ds_ready[1], 8);
     mbar_init(dq_done, 1);
     mbar_init(dq_free, 8);
+    mbar_init(idle, 1);
     fence_mbar_init();
   }
   if (warp == 9) tmem_alloc(slot, C::TMEM);
@@ -800,6 +841,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
           const int hk = u.h / a.group;
           for (int t = t0; t < t1 && ok; ++t) ok = load(&mk, t * C::BN, hk, u) && load(&mv, t * C::BN, hk, u);
         }
+        ok = drain_tma<C::STAGES>(ok, full, empty, it, q_full, q_free, nq);
         if (!ok) atomicExch(&g_error_flag, 21);
       }
     } else if (warp == 9) {
@@ -809,7 +851,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
         bool ok = true;
         int it = 0, nq = 0, g = 0, units = 0;
         auto stage = [&](int i) { return r0 + (i % C::STAGES) * C::TILE_BYTES; };
-        auto wait_full = [&](int i) { return mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1); };
+        auto wait_full = [&](int i) { return warp_wait(&full[i % C::STAGES], (i / C::STAGES) & 1); };
         for (int k = 0; ok; ++k) {
           const int ui = unit_index(k);
           if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
@@ -833,7 +875,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
           auto issue_dp = [&](int t) {
             if (!wait_full(it + 2 * t + 1)) return false;
             // dP of the tile before has been read (every tile signals once).
-            if (g + t > 0 && !mbar_wait(dp_free, (g + t - 1) & 1)) return false;
+            if (g + t > 0 && !warp_wait(dp_free, (g + t - 1) & 1)) return false;
             tc_fence_after();
             if (elect_one()) {
               mma_heads<HD>(tmem + C::DP_COL, o0, stage(it + 2 * t + 1), 128, C::BN, ta.ksteps, id_s);
@@ -844,7 +886,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
             __syncwarp();
             return true;
           };
-          if (!mbar_wait(q_full, nq & 1) || !issue_s(0) || !issue_dp(0)) {
+          if (!warp_wait(q_full, nq & 1) || !issue_s(0) || !issue_dp(0)) {
             ok = false;
             break;
           }
@@ -856,11 +898,11 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
               ok = false;
               break;
             }
-            if (t == 0 && units > 0 && !mbar_wait(dq_free, (units - 1) & 1)) {
+            if (t == 0 && units > 0 && !warp_wait(dq_free, (units - 1) & 1)) {
               ok = false;
               break;
             }
-            if (!mbar_wait(&ds_ready[(g + t) & 1], ((g + t) >> 1) & 1)) {
+            if (!warp_wait(&ds_ready[(g + t) & 1], ((g + t) >> 1) & 1)) {
               ok = false;
               break;
             }
@@ -883,7 +925,10 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
           it += 2 * n;
           ++units;
         }
-        if (!ok && lane == 0) atomicExch(&g_error_flag, 22);
+        if (!ok) {
+          drain_mma(idle);
+          if (lane == 0) atomicExch(&g_error_flag, 22);
+        }
       }
     }
   } else {
@@ -954,7 +999,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
           tmem_st8(to, w);
       };
       if (!C::EARLY && t0 < t1) {
-        if (!__all_sync(0xffffffffu, mbar_wait(dp_full, g & 1))) {
+        if (!warp_wait(dp_full, g & 1)) {
           ok = false;
           break;
         }
@@ -964,7 +1009,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
       for (int t = t0; t < t1; ++t, ++g) {
         const bool edge = t * C::BN + C::BN > b.kl || (a.causal && t * C::BN + C::BN - 1 > i0 + b.off);
         if (C::EARLY) {
-          if (!__all_sync(0xffffffffu, mbar_wait(dp_full, g & 1))) {
+          if (!warp_wait(dp_full, g & 1)) {
             ok = false;
             break;
           }
@@ -996,7 +1041,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
         }
         chunk_ds(t, 1, edge, s1, d1);
         if (!C::EARLY && t + 1 < t1) {
-          if (!__all_sync(0xffffffffu, mbar_wait(dp_full, (g + 1) & 1))) {
+          if (!warp_wait(dp_full, (g + 1) & 1)) {
             ok = false;
             break;
           }
@@ -1011,7 +1056,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
       if (!ok) break;
       it += 2 * (t1 - t0);
       if (t0 < t1) {
-        if (!__all_sync(0xffffffffu, mbar_wait(dq_done, units & 1))) {
+        if (!warp_wait(dq_done, units & 1)) {
           ok = false;
           break;
         }
@@ -1042,7 +1087,11 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
         if (lane == 0) mbar_arrive(dq_free);
       }
     }
-    if (!ok) atomicExch(&g_error_flag, 23);
+    if (!ok) {
+      tmem_wait_ld();
+      tmem_st_wait();
+      atomicExch(&g_error_flag, 23);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -1114,7 +1163,8 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
   uint64_t* st_free = st_full + C::STATS; // [STATS]
   uint64_t* acc_done = st_free + C::STATS;
   uint64_t* acc_free = acc_done + 1;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(acc_free + 1);
+  uint64_t* idle = acc_free + 1;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(idle + 1);
 
   const AttnArgs& a = ta.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1129,6 +1179,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
     mbar_init(&ps_ready[1], 8);
     mbar_init(acc_done, 1);
     mbar_init(acc_free, 8);
+    mbar_init(idle, 1);
     fence_mbar_init();
   }
   if (warp == 9) tmem_alloc(slot, C::TMEM);
@@ -1195,6 +1246,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
             }
           }
         }
+        ok = drain_tma<C::STAGES>(ok, full, empty, it, kv_full, kv_free, nkv);
         if (!ok) atomicExch(&g_error_flag, 31);
       }
     } else if (warp == 9) {
@@ -1205,7 +1257,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
         int g = 0, units = 0;  // tiles of all units: ring, S buffers and barriers go by g
         auto q_tile = [&](int i) { return r0 + 2 * (i % C::STAGES) * C::TILE_BYTES; };
         auto issue_s = [&](int i) {
-          if (!mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1)) return false;
+          if (!warp_wait(&full[i % C::STAGES], (i / C::STAGES) & 1)) return false;
           tc_fence_after();
           if (elect_one())
             mma_heads<HD>(tmem + C::S_COL + (i % C::SB) * C::BN, k0, q_tile(i), 128, C::BN, ta.ksteps, id_s);
@@ -1213,7 +1265,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
           return true;
         };
         auto issue_dp = [&](int i, bool last) {
-          if (i > 0 && !mbar_wait(dp_free, (i - 1) & 1)) return false;
+          if (i > 0 && !warp_wait(dp_free, (i - 1) & 1)) return false;
           tc_fence_after();
           if (elect_one()) {
             mma_heads<HD>(tmem + C::DP_COL, v0, q_tile(i) + C::TILE_BYTES, 128, C::BN, ta.ksteps, id_s);
@@ -1233,7 +1285,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
           range(u, b, begin, per, t0, t1);
           if (t0 >= t1) continue;
           const int n = t1 - t0;
-          if (!mbar_wait(kv_full, units & 1) || !issue_s(g) || !issue_dp(g, n == 1)) {
+          if (!warp_wait(kv_full, units & 1) || !issue_s(g) || !issue_dp(g, n == 1)) {
             ok = false;
             break;
           }
@@ -1242,8 +1294,8 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
               ok = false;
               break;
             }
-            if ((t == 0 && units > 0 && !mbar_wait(acc_free, (units - 1) & 1)) ||
-                !mbar_wait(&ps_ready[(g + t) & 1], ((g + t) >> 1) & 1)) {
+            if ((t == 0 && units > 0 && !warp_wait(acc_free, (units - 1) & 1)) ||
+                !warp_wait(&ps_ready[(g + t) & 1], ((g + t) >> 1) & 1)) {
               ok = false;
               break;
             }
@@ -1269,7 +1321,10 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
           g += n;
           ++units;
         }
-        if (!ok && lane == 0) atomicExch(&g_error_flag, 32);
+        if (!ok) {
+          drain_mma(idle);
+          if (lane == 0) atomicExch(&g_error_flag, 32);
+        }
       }
     } else if (warp == 10) {
       // (-lse in log2 units, -D) of each streamed tile; -inf and 0 for rows outside the queries.
@@ -1297,7 +1352,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
             l[e] = x.x + p_shift<T>();
             d[e] = x.y;
           }
-          if (r > 0 && !__all_sync(0xffffffffu, mbar_wait(&st_free[sb], (r - 1) & 1))) {
+          if (r > 0 && !warp_wait(&st_free[sb], (r - 1) & 1)) {
             ok = false;
             break;
           }
@@ -1341,8 +1396,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
         tmem_ld_async(lanes + C::S_COL + (tile % C::SB) * C::BN + half * C::HALF + C::CH * chunk, s);
       };
       auto arrived = [&](int tile) {  // S, dP and the row statistics of a tile
-        return __all_sync(0xffffffffu, mbar_wait(&st_full[tile % C::STATS], (tile / C::STATS) & 1) &&
-                                           mbar_wait(dp_full, tile & 1));
+        return warp_wait(&st_full[tile % C::STATS], (tile / C::STATS) & 1) && warp_wait(dp_full, tile & 1);
       };
       // P^T and dS^T of one chunk, stored over its scores.
       auto chunk_pds = [&](int i0, int chunk, bool edge, uint32_t (&s)[C::CH], uint32_t (&d)[C::CH]) {
@@ -1446,7 +1500,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
       }
       if (!ok) break;
       if (t0 < t1) {
-        if (!__all_sync(0xffffffffu, mbar_wait(acc_done, units & 1))) {
+        if (!warp_wait(acc_done, units & 1)) {
           ok = false;
           break;
         }
@@ -1482,7 +1536,11 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
         if (lane == 0) mbar_arrive(acc_free);
       }
     }
-    if (!ok) atomicExch(&g_error_flag, 33);
+    if (!ok) {
+      tmem_wait_ld();
+      tmem_st_wait();
+      atomicExch(&g_error_flag, 33);
+    }
   }
   tc_fence_before();
   __syncthreads();
