@@ -61,3 +61,19 @@ def test_attention_calls_end_with_everything_used(hd, t):
     ref = attention_reference(q, k, v, dout, k_lens=kl)
     for name, x in zip(("out", "dq", "dk", "dv"), first):
         assert_within(name, x, *ref[name])
+
+
+# ------------------------------------------------------------------------------- weights of masked keys
+
+
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_masked_keys_have_no_weight(hd, t):
+    """Values of the type's largest size at keys that a causal query does not see leave its row as it is, bit for bit:
+    a weight of 2^-126 in their place would add up to 4 in bf16."""
+    q, k, v, _ = _attn(1, 400, 400, 1, 1, hd, t)
+    clean, lse = training.attention_forward(q, k, v, causal=True)
+    big = v.clone()
+    big[:, 350:] = torch.finfo(t).max
+    out, lse2 = training.attention_forward(q, k, big, causal=True)
+    assert torch.equal(out[:, :350], clean[:, :350]) and torch.equal(lse, lse2)

@@ -44,10 +44,13 @@ __device__ __forceinline__ float ex2(float x) {
 // 2^x of a pair on the FMA pipe, for a share of the exponentials (the special function unit takes 16 per cycle and SM,
 // the tightest limit at head dim 64). x = n + f with n the nearest integer, read off the low bits of x + 1.5 2^23; 2^f
 // by a polynomial of degree 5 on [-1/2, 1/2] fitted for the least relative error (2.1e-7 in fp32, half the hardware
-// approximation's two ulp); n goes into the exponent. x below -126 gives 2^-126; f * 0 carries NaN into the result.
+// approximation's two ulp); n goes into the exponent. x below -127 counts as -127, where the exponent field comes out as
+// 0 and 2^f as 1 + 2^-23: 2^-149, which the 16-bit types round to 0 (a masked key must not keep even 2^-126, which a
+// value near bf16's largest would carry into the sum). Between -127 and -126 the result is off by up to 2^-126. f * 0
+// carries NaN into the result.
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
   constexpr float MAGIC = 12582912.f;
   auto both = [](float v) { return make_float2(v, v); };
   const float2 t = add2(x, both(MAGIC));
