@@ -77,3 +77,22 @@ def test_attention_masked_keys_have_no_weight(hd, t):
     big[:, 350:] = torch.finfo(t).max
     out, lse2 = training.attention_forward(q, k, big, causal=True)
     assert torch.equal(out[:, :350], clean[:, :350]) and torch.equal(lse, lse2)
+
+
+# ------------------------------------------------------------------------------------------- rows of NaN
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("n,lq,lk", [(1, 100, 900), (40, 100, 900), (1, 2, 3000), (3, 40, 50)])
+def test_attention_rows_of_nan_say_so(n, lq, lk, t):
+    """A query of NaN has an output and a log-sum of NaN, however its keys are divided, and no other row has."""
+    q, k, v, dout = _attn(n, lq, lk, 2, 2, 64, t)
+    clean, clean_lse = training.attention_forward(q, k, v)
+    q[0, 1, 1, 5] = float("nan")
+    out, lse = training.attention_forward(q, k, v)
+    assert out[0, 1, 1].isnan().all() and lse[0, 1, 1].isnan()
+    clean[0, 1, 1], clean_lse[0, 1, 1] = out[0, 1, 1], lse[0, 1, 1]
+    assert torch.equal(out.nan_to_num(7.0), clean.nan_to_num(7.0))
+    assert torch.equal(lse.nan_to_num(7.0), clean_lse.nan_to_num(7.0))
+    dq, _, _ = training.attention_backward(dout, q, k, v, out, lse)
+    assert dq[0, 1, 1].isnan().all() and not dq[0, 0].isnan().any() and not dq[0, 1, 0].isnan().any()

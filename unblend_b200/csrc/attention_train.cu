@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(NT) attention_fwd_kernel(const __grid_constant
     if (i >= a.lq) continue;
     const long long row = ((long long)u.seq * a.heads + u.h) * a.lq + i;
     const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-    const float lse = m[r] == -INFINITY ? -INFINITY : (m[r] + log2f(l[r])) * LN2;
+    // Scores that are all NaN leave no maximum, but a sum of NaN.
+    const float lse = l[r] == 0.f ? -INFINITY : (m[r] + log2f(l[r])) * LN2;
     if (a.splits > 1) {
       store_row<float, HDP>(o[r], inv, a.part + (u.split * rows + row) * hd, hd, tx);
       if (tx == 0) a.part_lse[u.split * rows + row] = lse;
