@@ -632,6 +632,7 @@ typedef struct {
   const int* k_lens;
   UnblendHeadStrides q, k, v, out;
   UnblendHeadStrides dout, dq, dk, dv; /* backward only */
+  int all_keys; /* backward only: not 0 when out and lse are of these keys alone, see unblend_attention_backward */
 } UnblendAttnTrainParams;
 
 /* Workspace bytes of a call (0: none needed, work may be NULL). */
@@ -641,7 +642,9 @@ int unblend_attention_forward(const void* q, const void* k, const void* v, void*
                               long long work_bytes, const UnblendAttnTrainParams* p, void* stream);
 
 /* dv = P^T dout, dS = P * (dout V^T - rowsum(dout * out)), dq = scale dS K, dk = scale dS^T Q; dk and dv are summed
- * over the query heads that share a key/value head. P is computed again from q, k and lse. */
+ * over the query heads that share a key/value head. P is computed again from q, k and lse. Keys that are processed in
+ * blocks may give each block out and lse of all of them. With all_keys the rowsum of short sequences, rowsum(P * (dout
+ * V^T)) then, is taken in fp32 without the rounding of out: only for calls that are not such a block. */
 int unblend_attention_backward(const void* dout, const void* q, const void* k, const void* v, const void* out,
                                const float* lse, void* dq, void* dk, void* dv, void* work, long long work_bytes,
                                const UnblendAttnTrainParams* p, void* stream);

@@ -96,3 +96,43 @@ def test_attention_rows_of_nan_say_so(n, lq, lk, t):
     assert torch.equal(lse.nan_to_num(7.0), clean_lse.nan_to_num(7.0))
     dq, _, _ = training.attention_backward(dout, q, k, v, out, lse)
     assert dq[0, 1, 1].isnan().all() and not dq[0, 0].isnan().any() and not dq[0, 1, 0].isnan().any()
+
+
+# ------------------------------------------------------------------------------------------ blocks of keys
+
+
+@pytest.mark.parametrize("lq,lk,cut,h,hk,hd", [(60, 64, 60, 2, 2, 64), (40, 64, 60, 4, 2, 64), (30, 36, 32, 2, 2, 64),
+                                               (50, 64, 60, 2, 2, 128)])
+def test_a_block_of_little_weight_and_large_values(lq, lk, cut, h, hk, hd):
+    """The last keys hold about 2^-17.5 of a row's weight, and values a million times larger than the others: D of the
+    joined output is mostly theirs, in the gradients of the first block too."""
+    q, k, v, dout = _attn(2, lq, lk, h, hk, hd, BF16)
+    q, k = q * 0.3, k * 0.3
+    q[..., 0], k[..., 0] = hd**0.5, 0.0
+    k[:, cut:, :, 0] = -(17.5 * 0.6931 + torch.tensor((lk - cut) / cut).log().item())
+    v[:, cut:] *= 1e6
+    out, lse = training.attention_forward(q, k, v)
+    ref = attention_reference(q, k, v, dout)
+    parts = [training.attention_backward(dout, q, k[:, s], v[:, s], out, lse) for s in (slice(0, cut), slice(cut, lk))]
+    for i, name in ((1, "dk"), (2, "dv")):
+        assert_within(name, torch.cat([x[i] for x in parts], 1), *ref[name])
+    want, tol = ref["dq"]
+    each = 2.0**-8 * sum(x[0].double().abs() for x in parts)
+    assert_within("dq", parts[0][0].double() + parts[1][0].double(), want, tol + each)
+
+
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("lq,lk,h,hk,hd,causal", [(62, 62, 2, 2, 64, False), (50, 64, 4, 2, 64, True),
+                                                  (64, 40, 2, 2, 128, True), (20, 30, 2, 2, 48, False),
+                                                  (150, 200, 2, 1, 64, True)])
+def test_all_keys_gives_the_same_gradients(lq, lk, h, hk, hd, causal, t):
+    """``all_keys`` (D of short sequences from the probabilities), and the differentiable function, which says so."""
+    q, k, v, dout = _attn(3, lq, lk, h, hk, hd, t)
+    ref = attention_reference(q, k, v, dout, causal=causal)
+    out, lse = training.attention_forward(q, k, v, causal=causal)
+    got = training.attention_backward(dout, q, k, v, out, lse, causal=causal, all_keys=True)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        assert_within(name, x, *ref[name])
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    training.attention(*leaves, causal=causal).backward(dout)
+    assert all(torch.equal(x.grad, y) for x, y in zip(leaves, got))

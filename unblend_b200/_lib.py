@@ -97,6 +97,7 @@ class AttnTrainParams(ctypes.Structure):
         ("q_lens", c_void_p), ("k_lens", c_void_p),
         ("q", HeadStrides), ("k", HeadStrides), ("v", HeadStrides), ("out", HeadStrides),
         ("dout", HeadStrides), ("dq", HeadStrides), ("dk", HeadStrides), ("dv", HeadStrides),
+        ("all_keys", c_int),
     ]
 
 

@@ -916,6 +916,7 @@ AttnArgs args_of(const UnblendAttnTrainParams& p) {
   a.lk = p.lk;
   a.hd = p.hd;
   a.causal = p.causal ? 1 : 0;
+  a.all_keys = p.all_keys ? 1 : 0;
   a.scale = p.scale;
   a.splits = 1;
   return a;

@@ -16,6 +16,7 @@ struct AttnArgs {
   UnblendHeadStrides q_s, k_s, v_s, out_s, dout_s, dq_s, dk_s, dv_s;
   const int *q_lens, *k_lens;
   int seqs, inner, heads, kv_heads, group, lq, lk, hd, causal;
+  int all_keys;  // backward: lse and out are of these keys alone
   float scale;
   int splits;       // parts of the streamed axis
   float* part;      // [splits][rows][hd] (dk / dv: two of them), null when splits == 1

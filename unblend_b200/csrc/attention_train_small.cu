@@ -7,8 +7,8 @@
 //
 // One kernel makes the three gradients, where the kernels for long rows need one for the statistics, one for dq and one
 // for dk and dv, and read the inputs in each. D = rowsum(P * dP) in fp32 is better than from the rounded O (bf16, 6
-// queries over 16 keys: gradients off by 0.0024 instead of 0.0029 relative), but holds only when lse and O are of these
-// keys alone: a caller that joins several blocks of keys gives those of all. So it is taken where P adds up to 1.
+// queries over 16 keys: gradients off by 0.0024 instead of 0.0029 relative) and needs no O, but holds only when lse and O
+// are of these keys alone, which the caller says with all_keys: whoever joins several blocks of keys gives those of all.
 //
 // Bound: HBM. A sequence and head gives 5 products of 64 x 64 x head dim for 8 tensors of 64 rows, far below what the
 // tensor cores need per byte, so mma.sync is enough (m16n8k16, fp32 accumulators); tcgen05's 128 rows would be half
@@ -31,7 +31,6 @@ using namespace ub::train;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int P_COLS = 64;  // pitch of P and dS
-constexpr float WHOLE = 1.f / 65536;  // sums of P this near to 1 leave out less than the roundings of P and dS
 
 // R: rows of a tile, 64, or 32 for shorter sequences; a warp per 16.
 constexpr int fwd_smem(int hd, int r) { return 3 * r * hd * 2; }
@@ -326,7 +325,7 @@ __global__ void __launch_bounds__(2 * R, bwd_ctas(HD, R, GROUPED))
     if (g == 0) fetch<HD, R>(tk, head_at(args, a.k, a.k_s, seq, hk), a.k_s, 0, b.kl, a.hd);
     cp_commit();
     fetch<HD, R>(td, head_at(args, a.dout, a.dout_s, seq, h), a.dout_s, rows.first, rows.end, a.hd);
-    fetch<HD, R>(to, head_at(args, a.out_in, a.out_s, seq, h), a.out_s, rows.first, rows.end, a.hd);
+    if (!a.all_keys) fetch<HD, R>(to, head_at(args, a.out_in, a.out_s, seq, h), a.out_s, rows.first, rows.end, a.hd);
     if (g == 0) fetch<HD, R>(tv, head_at(args, a.v, a.v_s, seq, hk), a.v_s, 0, b.kl, a.hd);
     cp_commit();
     float base[2];
@@ -359,31 +358,19 @@ __global__ void __launch_bounds__(2 * R, bwd_ctas(HD, R, GROUPED))
     cp_wait<0>();
     __syncthreads();
     rows_dot<T, HD, R>(dp, td, r0, tv);
-    // D of a row whose keys are all here (its P adds up to 1) from P and dP in fp32; of others from O.
     float D[2];
-    bool whole = true;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      float2 sum = make_float2(0.f, 0.f), prod = make_float2(0.f, 0.f);
+      if (a.all_keys) {
+        float2 prod = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int n = 0; n < R / 8; ++n) {
-        const float2 p = make_float2(s[n][2 * x], s[n][2 * x + 1]);
-        sum = add2(sum, p);
-        prod = ub::fma2(p, make_float2(dp[n][2 * x], dp[n][2 * x + 1]), prod);
-      }
-      float total = sum.x + sum.y, d = prod.x + prod.y;
-      total += __shfl_xor_sync(0xffffffffu, total, 1);
-      d += __shfl_xor_sync(0xffffffffu, d, 1);
-      total += __shfl_xor_sync(0xffffffffu, total, 2);
-      d += __shfl_xor_sync(0xffffffffu, d, 2);
-      D[x] = d;
-      whole &= fabsf(total - 1.f) < WHOLE || r0 + quad + 8 * x >= b.ql;
-    }
-    if (!__all_sync(0xffffffffu, whole)) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float d = row_product<T, HD>(td, to, r0 + quad + 8 * x);
-        D[x] = whole ? D[x] : d;
+        for (int n = 0; n < R / 8; ++n)
+          prod = ub::fma2(make_float2(s[n][2 * x], s[n][2 * x + 1]), make_float2(dp[n][2 * x], dp[n][2 * x + 1]), prod);
+        D[x] = prod.x + prod.y;
+        D[x] += __shfl_xor_sync(0xffffffffu, D[x], 1);
+        D[x] += __shfl_xor_sync(0xffffffffu, D[x], 2);
+      } else {
+        D[x] = row_product<T, HD>(td, to, r0 + quad + 8 * x);
       }
     }
     if (HD > 64)

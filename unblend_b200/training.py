@@ -349,13 +349,15 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
 
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
                        lse: torch.Tensor, scale: float | None = None, causal: bool = False,
-                       q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None
-                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                       q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None,
+                       all_keys: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(dq, dk, dv)`` from the gradient of ``out``, the inputs and the results of ``attention_forward``.
 
     The probabilities are computed again from q, k and ``lse``; dk and dv are summed over the query heads that share a
     head. The gradients are contiguous; rows behind the lengths are 0. Keys that are processed in blocks may give each
     block ``out`` and ``lse`` of all of them: dk and dv are then the block's rows, and the blocks' dq add up.
+    ``all_keys=True`` says that this call is not such a block: 16-bit sequences of up to 64 queries and keys then take
+    ``rowsum(dout * out)`` from the fp32 probabilities, without the rounding of ``out``, and do not read ``out``.
     """
     scale = _check_attention(q, k, v, scale, causal, q_lens, k_lens)
     for name, t in (("dout", dout), ("out", out)):
@@ -374,7 +376,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     k_lens = None if k_lens is None else k_lens.contiguous()
     sizes = _sizes(q, k, scale, causal)
     p = _lib.AttnTrainParams(*sizes, _lib.ptr(q_lens), _lib.ptr(k_lens),
-                             *(_strides(t) for t in (q, k, v, out, dout, dq, dk, dv)))
+                             *(_strides(t) for t in (q, k, v, out, dout, dq, dk, dv)), bool(all_keys))
     lse = lse.contiguous()
     n = _attention_workspace_bytes(1, *sizes)
     work = _scratch(q, n)
@@ -397,7 +399,8 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, dout):
         _refuse_capture("attention")
         q, k, v, out, lse, q_lens, k_lens = ctx.saved_tensors
-        dq, dk, dv = attention_backward(dout, q, k, v, out, lse, ctx.scale, ctx.causal, q_lens, k_lens)
+        dq, dk, dv = attention_backward(dout, q, k, v, out, lse, ctx.scale, ctx.causal, q_lens, k_lens,
+                                        all_keys=True)
         need = ctx.needs_input_grad
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
