@@ -136,3 +136,70 @@ def test_all_keys_gives_the_same_gradients(lq, lk, h, hk, hd, causal, t):
     leaves = [x.clone().requires_grad_() for x in (q, k, v)]
     training.attention(*leaves, causal=causal).backward(dout)
     assert all(torch.equal(x.grad, y) for x, y in zip(leaves, got))
+
+
+# --------------------------------------------------------------------------------- sizes of fp16 gradients
+
+
+def _relative(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+def _fp16_gradients(q, k, v, dout, **kw):
+    """Relative error of each gradient next to what rounding its exact value to fp16 costs (subnormals included).
+
+    dS and P are rounded once more on the way, by half a step of 2^-11 each, and so is the output that D is made from;
+    errors that do not all point one way add up to less than the sum of both, doubled here.
+    """
+    out, lse = training.attention_forward(q, k, v, **kw)
+    got = training.attention_backward(dout, q, k, v, out, lse, **kw)
+    assert _lib.error_flag() == 0
+    ref = attention_reference(q, k, v, dout, **kw)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        want = ref[name][0]
+        least = _relative(want.half(), want)
+        assert _relative(x, want) <= 2 * (least + 2.0**-11), (name, _relative(x, want), least)
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("lq,lk,h,hk,hd,causal", [
+    (512, 1344, 1, 1, 64, False), (512, 8192, 1, 1, 64, False), (700, 2000, 2, 1, 128, True), (300, 60, 2, 1, 64, False),
+    (50, 700, 2, 2, 64, False), (62, 62, 2, 2, 64, False), (64, 50, 4, 2, 48, True), (30, 31, 2, 2, 64, False),
+    (60, 60, 2, 2, 128, False), (20, 30, 4, 1, 40, True)])
+def test_fp16_gradients_of_small_losses(lq, lk, h, hk, hd, causal, size):
+    """Gradients as small as a loss averaged over tokens gives: dS = P (dP - D) must not sink into the subnormals."""
+    q, k, v, dout = _attn(2, lq, lk, h, hk, hd, F16, seed=lk)
+    _fp16_gradients(q, k, v, (dout.float() * size).half(), causal=causal)
+
+
+@pytest.mark.parametrize("lq,lk,hd", [(70, 90, 64), (40, 60, 64), (30, 20, 64), (150, 200, 128)])
+def test_fp16_gradients_of_scaled_losses(lq, lk, hd):
+    """A loss scaled up: dS beyond fp16's largest value, the gradients within it."""
+    q, k, v, dout = _attn(2, lq, lk, 1, 1, hd, F16)
+    _fp16_gradients(q * 8, k * 8, v * 30, torch.sign(dout) * 500, scale=1 / hd)
+
+
+def test_fp16_gradients_of_uneven_sequences():
+    """Sequences whose gradients differ by 10^6, rows that differ by 10^3, lengths, and NaN behind them."""
+    q, k, v, dout = _attn(3, 300, 500, 2, 1, 64, F16)
+    dout = dout.float() * torch.tensor([1e-4, 100.0, 1e-2], device="cuda")[:, None, None, None]
+    dout[:, ::2] *= 1e-3
+    dout = dout.half()
+    ql = torch.tensor([300, 200, 77], device="cuda", dtype=torch.int32)
+    kl = torch.tensor([500, 333, 450], device="cuda", dtype=torch.int32)
+    for b in range(3):
+        q[b, int(ql[b]):], dout[b, int(ql[b]):] = float("nan"), float("inf")
+        k[b, int(kl[b]):], v[b, int(kl[b]):] = float("nan"), float("inf")
+    for b in range(3):
+        s = slice(b, b + 1)
+        _fp16_gradients(q[s], k[s], v[s], dout[s], q_lens=ql[s], k_lens=kl[s])
+    out, lse = training.attention_forward(q, k, v, q_lens=ql, k_lens=kl)
+    got = training.attention_backward(dout, q, k, v, out, lse, q_lens=ql, k_lens=kl)
+    ref = attention_reference(q, k, v, dout, q_lens=ql, k_lens=kl)
+    for b in range(3):
+        for name, x in zip(("dq", "dk", "dv"), got):
+            want = ref[name][0][b]
+            assert _relative(x[b], want) <= 2 * (_relative(want.half(), want) + 2.0**-11), (b, name)
+        # The small rows of dq on their own.
+        want = ref["dq"][0][b, :int(ql[b]):2]
+        assert _relative(got[0][b, :int(ql[b]):2], want) <= 2 * (_relative(want.half(), want) + 2.0**-11), b

@@ -840,9 +840,18 @@ Plan plan_of(const UnblendAttnTrainParams& p, Path path) {
   return n;
 }
 
-// Workspace: forward [parts][q_rows][hd] and [parts][q_rows] lse; backward D or row statistics [q_rows][2], then the
-// parts of dq and of dk and dv, which one kernel joins. Room for either kind of kernels: which of them runs depends on
-// the pointers too.
+// Workspace: forward [parts][q_rows][hd] and [parts][q_rows] lse; backward D or row statistics [q_rows][2], for fp16
+// norms [q_rows] and ranges [seqs * kv_heads][4], then the parts of dq and of dk and dv, which one kernel joins. Room
+// for either kind of kernels: which of them runs depends on the pointers too.
+long long norm_floats(const UnblendAttnTrainParams& p, const Plan& n) {
+  return p.dtype == UNBLEND_F16 ? round4(n.q_rows) : 0;
+}
+
+long long stats_floats(const UnblendAttnTrainParams& p, const Plan& n) {
+  const long long ranges = p.dtype == UNBLEND_F16 ? 4LL * p.outer * p.inner * p.kv_heads : 0;
+  return round4(2 * n.q_rows) + norm_floats(p, n) + ranges;
+}
+
 long long dq_part_floats(const UnblendAttnTrainParams& p, const Plan& n) {
   return n.dq_splits > 1 ? round4(n.dq_splits * n.q_rows * p.hd) : 0;
 }
@@ -855,7 +864,7 @@ long long workspace_floats(const UnblendAttnTrainParams& p, bool backward) {
     if (!backward) {
       need = n.fwd_splits > 1 ? n.fwd_splits * n.q_rows * (p.hd + 1LL) : 0;
     } else {
-      need = round4(2 * n.q_rows) + dq_part_floats(p, n);
+      need = stats_floats(p, n) + dq_part_floats(p, n);
       if (n.dkv_splits > 1) need += 2 * n.dkv_splits * n.k_rows * p.hd;
     }
     most = need > most ? need : most;
@@ -1106,7 +1115,9 @@ extern "C" int unblend_attention_backward(const void* dout, const void* q, const
   a.dk = dk;
   a.dv = dv;
   a.dsum = static_cast<float*>(work);
-  float* parts = a.dsum + round4(2 * n.q_rows);
+  a.dnorm = a.dsum + round4(2 * n.q_rows);
+  a.range = reinterpret_cast<unsigned*>(a.dnorm + norm_floats(*p, n));
+  float* parts = a.dsum + stats_floats(*p, n);
   cudaStream_t st = ub::as_stream(stream);
   if (tc && attention_is_small(*p, true)) return attention_small_backward(a, *p, st);
   const bool vec = p->hd % 4 == 0 && vec4_ok(q, p->q, *p) && vec4_ok(k, p->k, *p) && vec4_ok(v, p->v, *p) &&

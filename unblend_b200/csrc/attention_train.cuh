@@ -13,6 +13,8 @@ struct AttnArgs {
   void *out, *dq, *dk, *dv;
   float* lse;
   float* dsum;  // [rows] rowsum(dout * out) (CUDA cores), or [rows][2] row statistics (tensor cores)
+  float* dnorm;     // [rows] norms of the rows of dout (tensor cores, fp16)
+  unsigned* range;  // [seqs * kv_heads][4] bits of the largest norm of a row of v and of dout, and |D| (the same)
   UnblendHeadStrides q_s, k_s, v_s, out_s, dout_s, dq_s, dk_s, dv_s;
   const int *q_lens, *k_lens;
   int seqs, inner, heads, kv_heads, group, lq, lk, hd, causal;
@@ -57,6 +59,16 @@ __device__ __forceinline__ long long head_offset(const UnblendHeadStrides& s, co
   const int o = seq / a.inner;
   return (long long)o * s.outer + (long long)(seq - o * a.inner) * s.inner + (long long)h * s.head;
 }
+
+// dS = P (dP - D) of fp16 calls is stored times a power of two: unscaled, the gradients of a loss averaged over tokens
+// would sink into fp16's subnormals (dout of size 1e-4 over 8192 keys: dq off by 10 %), those of a loss scaled up pass
+// its largest value. For values of size `bound` (0 up to infinity; as bits) this is the k for which bound 2^k lies in
+// [2^14, 2^15); 40 at most, so that fp32 sums times 2^k stay finite, and 0 where the bound is infinite or NaN.
+__device__ __forceinline__ int fp16_shift(unsigned bound_bits) {
+  const int e = (int)(bound_bits >> 23) - 127;
+  return e > 127 ? 0 : min(14 - e, 40);
+}
+__device__ __forceinline__ float pow2(int k) { return __uint_as_float((unsigned)(127 + k) << 23); }
 
 // n / d for n < 2^31 by a multiplication: with 2^s >= d and m = floor(2^(31 + s) / d) + 1, floor(n m / 2^(31 + s)) is
 // exact because n (m d - 2^(31 + s)) < 2^(31 + s). A hardware division takes a hundred cycles, which short

@@ -16,8 +16,10 @@
 // latency here is several independent CTAs per SM.
 //
 // A warp has 16 query rows for S, dP and dQ; P and dS go through shared memory, and each warp takes 16 keys for
-// dK and dV. P and dS are rounded to the inputs' type, as the tensor cores take both operands in one 16-bit type; P of
-// fp16 calls is kept times 2^12 there (small probabilities would be subnormal). Softmax, D and all sums are fp32.
+// dK and dV. P and dS are rounded to the inputs' type, as the tensor cores take both operands in one 16-bit type; fp16
+// calls keep P times 2^12 there (small probabilities would be subnormal) and dS times the power of two that brings the
+// head's largest one below 2^15 (small gradients would be subnormal, large ones infinite). Softmax, D and all sums are
+// fp32.
 // Results leave through shared memory in 16-byte chunks. 16-byte chunk c of a tile's row lies at c ^ (row & 7).
 #include <type_traits>
 
@@ -302,7 +304,9 @@ __global__ void __launch_bounds__(2 * R, bwd_ctas(HD, R, GROUPED))
     attention_small_bwd_kernel(const __grid_constant__ SmallArgs args) {
   const AttnArgs& a = args.a;
   constexpr uint32_t TILE = R * HD * 2, P_TILE = R * P_COLS * 2;
-  constexpr float P_SCALE = std::is_same<T, __half>::value ? 4096.f : 1.f;
+  constexpr bool FP16 = std::is_same<T, __half>::value;
+  constexpr float P_SCALE = FP16 ? 4096.f : 1.f;
+  __shared__ unsigned largest[R / 16];  // fp16: bits of the warps' largest |dS|
   extern __shared__ __align__(128) uint8_t small_smem[];
   const uint32_t tk = smem_at(small_smem), tv = tk + TILE, tq = tv + TILE, td = tq + TILE;
   const uint32_t tp = td + TILE, ts = tp + P_TILE;
@@ -315,6 +319,7 @@ __global__ void __launch_bounds__(2 * R, bwd_ctas(HD, R, GROUPED))
   const Used rows = used_queries(a, b);
   const float c = a.scale * LOG2E;
   const int all = keys_of_all(a, b, r0);
+  int shift = 0;  // dS and dK are times 2^shift (fp16)
   float dk[HD / 8][4], dv[HD / 8][4];
   clear(dk);
   clear(dv);
@@ -373,21 +378,49 @@ __global__ void __launch_bounds__(2 * R, bwd_ctas(HD, R, GROUPED))
         D[x] = row_product<T, HD>(td, to, r0 + quad + 8 * x);
       }
     }
-    if (HD > 64)
+    unsigned most = 0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int n = 0; n < R / 8; ++n) {
+        float2 e = add2(make_float2(dp[n][2 * x], dp[n][2 * x + 1]), make_float2(-D[x], -D[x]));
+        e = mul2(make_float2(s[n][2 * x], s[n][2 * x + 1]), e);
+        dp[n][2 * x] = e.x;
+        dp[n][2 * x + 1] = e.y;
+        if constexpr (FP16) most = max(most, max(__float_as_uint(fabsf(e.x)), __float_as_uint(fabsf(e.y))));
+      }
+    float up = 1.f;
+    if constexpr (FP16) {
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0) largest[threadIdx.x >> 5] = most;
+      __syncthreads();  // O's rows, too, lie under other warps' rows of P and dS
+#pragma unroll
+      for (int w = 0; w < R / 16; ++w) most = max(most, largest[w]);
+      const int k = fp16_shift(most);
+      up = pow2(k);
+      if (GROUPED && g > 0) {  // dK of the heads before, to this head's scale
+        const float f = pow2(k - shift);
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dk[n][e] *= f;
+      }
+      shift = k;
+    } else if (HD > 64) {
       __syncthreads();  // O's rows lie under other warps' rows of P and dS
-    else
+    } else {
       __syncwarp();
+    }
     uint32_t sf[R / 16][4];  // dS as A fragments
     const uint32_t at = (r0 + quad) * (2 * P_COLS) + quad * 16 + ql * 4;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
 #pragma unroll
       for (int n = 0; n < R / 8; ++n) {
-        const float2 p = make_float2(s[n][2 * x], s[n][2 * x + 1]);
-        const float2 e = mul2(p, add2(make_float2(dp[n][2 * x], dp[n][2 * x + 1]), make_float2(-D[x], -D[x])));
-        const uint32_t w = pack_pair<T>(e.x, e.y), put = (at ^ (n * 16)) + x * 8 * (2 * P_COLS);
+        const uint32_t w = pack_pair<T>(dp[n][2 * x] * up, dp[n][2 * x + 1] * up);
+        const uint32_t put = (at ^ (n * 16)) + x * 8 * (2 * P_COLS);
         sf[n / 2][2 * (n & 1) + x] = w;
-        sts4(tp + put, pack_pair<T>(p.x * P_SCALE, p.y * P_SCALE));
+        sts4(tp + put, pack_pair<T>(s[n][2 * x] * P_SCALE, s[n][2 * x + 1] * P_SCALE));
         sts4(ts + put, w);
       }
     }
@@ -397,7 +430,7 @@ __global__ void __launch_bounds__(2 * R, bwd_ctas(HD, R, GROUPED))
       clear(dq);
 #pragma unroll
       for (int ks = 0; ks < R / 16; ++ks) rows_sum<T, HD>(dq, sf[ks], tk, 16 * ks);
-      pack_rows<T>(packed, dq, a.scale, a.scale);
+      pack_rows<T>(packed, dq, a.scale * pow2(-shift), a.scale * pow2(-shift));
     }
     __syncthreads();  // P and dS are written, K and V are read
     put_rows<HD>(stage, packed, head_at(args, a.dq, a.dq_s, seq, h), a.dq_s, r0, a.lq, a.hd,
@@ -409,7 +442,7 @@ __global__ void __launch_bounds__(2 * R, bwd_ctas(HD, R, GROUPED))
   uint32_t packed[HD / 8][2];
   pack_rows<T>(packed, dv, 1.f / P_SCALE, 1.f / P_SCALE);
   put_rows<HD>(tv, packed, head_at(args, a.dv, a.dv_s, seq, hk), a.dv_s, r0, a.lk, a.hd, counts);
-  pack_rows<T>(packed, dk, a.scale, a.scale);
+  pack_rows<T>(packed, dk, a.scale * pow2(-shift), a.scale * pow2(-shift));
   put_rows<HD>(tk, packed, head_at(args, a.dk, a.dk_s, seq, hk), a.dk_s, r0, a.lk, a.hd, counts);
 }
 

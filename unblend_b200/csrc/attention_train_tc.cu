@@ -11,7 +11,10 @@
 //   dk / dv   rows = keys:    S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
 //
 // P and dS are rounded to the inputs' type, as the tensor cores take both operands in one 16-bit type; softmax, its
-// statistics and all sums are fp32. 2^x is the hardware approximation (2 ulp).
+// statistics and all sums are fp32. 2^x is the hardware approximation (2 ulp). Backward, fp16 keeps P times 2^12 and dS
+// times a power of two that its bound |dS| <= |dO_i| |V_j| + |D_i| (norms of the rows) gives: for dQ one per query, for
+// dK, which is summed over queries, one per sequence and key/value head. Both cost nothing in the loops: dQ's is added to
+// the exponent of P, dK's to the factor that takes P's 2^12 back.
 //
 // A thread owns a row (or half a row), so row maxima and sums need no shuffles. One warp issues TMA, one the MMAs;
 // every barrier wait gives up after two seconds and sets the error flag. A warp gives up as a whole (its lanes vote), as
@@ -21,6 +24,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
+
+#include <type_traits>
 
 #include "attention_train.cuh"
 #include "tc_common.cuh"
@@ -218,7 +223,7 @@ __device__ __forceinline__ void clear_row(uint8_t* tile, int rows, int blocks, i
 struct TcArgs {
   AttnArgs a;
   const float2* stats;   // backward: (-lse log2 e, -D) of each query row, (-inf, 0) for rows that see nothing
-  FastDiv by_splits, by_tiles, by_heads, by_inner, by_seq_heads;
+  FastDiv by_splits, by_tiles, by_heads, by_inner, by_seq_heads, by_group;
   int row_tiles, units;  // units of the kernel's rows
   int ksteps, n_hd;      // head dim / 16 rounded up, and * 16
   uint32_t fmt;
@@ -728,6 +733,102 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// The same for fp16, with the norms of dO's rows and, per sequence and key/value head, the largest norm of a row of dO
+// and V and the largest |D|: by integer maxima of the bits, whose order does not matter. Queries that see nothing and
+// keys behind the length stay out. A warp walks rows of one head, so many that the GPU is full once (its maxima go to
+// memory once); units below q_units are rows of dO, the rest rows of V. 62 x 801, 8 heads of 64: 44 us (3.5 TB/s; 96
+// warps per SM 40 us, but 2 x 2000, 16 over 4 heads of 128 17 instead of 13 us, for the maxima of few heads).
+struct RangeArgs {
+  unsigned q_units, units;
+  int q_chunks, v_chunks;  // units of a head
+  int q_steps, v_steps;    // of a unit, STATS_ROWS * 32 / LANES rows each
+  FastDiv by_heads, by_kv_heads, by_q_chunks, by_v_chunks, by_group, by_inner;
+};
+
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) attention_stats_range_kernel(const __grid_constant__ AttnArgs a, float2* stats,
+                                                                    const __grid_constant__ RangeArgs ra) {
+  constexpr int APART = 32 / LANES, STEP = APART * STATS_ROWS;
+  const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= ra.units) return;
+  const bool is_v = unit >= ra.q_units;
+  const int id = (int)(is_v ? unit - ra.q_units : unit);
+  int h, hk, seq, chunk;  // heads fastest, then the rows
+  if (is_v) {
+    const int rest = ra.by_kv_heads(id);
+    h = hk = id - rest * a.kv_heads;
+    seq = ra.by_v_chunks(rest);
+    chunk = rest - seq * ra.v_chunks;
+  } else {
+    const int rest = ra.by_heads(id);
+    h = id - rest * a.heads;
+    hk = ra.by_group(h);
+    seq = ra.by_q_chunks(rest);
+    chunk = rest - seq * ra.q_chunks;
+  }
+  const int o = ra.by_inner(seq), lane = threadIdx.x & (LANES - 1);
+  const Bounds b = bounds_of(a, seq);
+  const int valid = is_v ? b.kl : b.ql, rows = is_v ? b.kl : a.lq;
+  const long long row0 = ((long long)seq * a.heads + h) * a.lq;
+  auto head = [&](const void* p, const UnblendHeadStrides& t) {
+    return static_cast<const T*>(p) + (long long)o * t.outer + (long long)(seq - o * a.inner) * t.inner +
+           (long long)h * t.head + 8 * lane;
+  };
+  const T* x_at = is_v ? head(a.v, a.v_s) : head(a.dout, a.dout_s);
+  const T* o_at = is_v ? nullptr : head(a.out_in, a.out_s);
+  const long long x_row = is_v ? a.v_s.row : a.dout_s.row, o_row = a.out_s.row;
+  unsigned top_norm = 0, top_D = 0;
+  const int span = (is_v ? ra.v_steps : ra.q_steps) * STEP, begin = chunk * span, end = min(rows, begin + span);
+  for (int i0 = begin; i0 < end; i0 += STEP) {
+    const int first = i0 + (threadIdx.x & 31) / LANES;
+    uint4 xv[STATS_ROWS], ov[STATS_ROWS];
+    float lse[STATS_ROWS];
+#pragma unroll
+    for (int u = 0; u < STATS_ROWS; ++u) {
+      const int i = first + u * APART;
+      xv[u] = ov[u] = make_uint4(0, 0, 0, 0);
+      lse[u] = i < valid ? (is_v ? 0.f : a.lse[row0 + i]) : -INFINITY;
+      if (i < valid && 8 * lane < a.hd) {
+        xv[u] = *reinterpret_cast<const uint4*>(x_at + i * x_row);
+        if (!is_v) ov[u] = *reinterpret_cast<const uint4*>(o_at + i * o_row);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < STATS_ROWS; ++u) {
+      const int i = first + u * APART;
+      const T* x = reinterpret_cast<const T*>(&xv[u]);
+      const T* y = reinterpret_cast<const T*>(&ov[u]);
+      float D = 0.f, square = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) square = fmaf(to_f(x[e]), to_f(x[e]), square);
+#pragma unroll
+      for (int s = LANES / 2; s > 0; s >>= 1) square += __shfl_xor_sync(0xffffffffu, square, s);
+      if (!is_v) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) D = fmaf(to_f(x[e]), to_f(y[e]), D);
+#pragma unroll
+        for (int s = LANES / 2; s > 0; s >>= 1) D += __shfl_xor_sync(0xffffffffu, D, s);
+      }
+      const bool counts = lse[u] != -INFINITY;
+      const float norm = counts ? sqrtf(square) : 0.f;
+      if (!counts) D = 0.f;
+      top_norm = max(top_norm, __float_as_uint(norm));
+      top_D = max(top_D, __float_as_uint(fabsf(D)));
+      if (!is_v && lane == 0 && i < end) {
+        stats[row0 + i] = counts ? make_float2(-lse[u] * LOG2E, -D) : make_float2(-INFINITY, 0.f);
+        a.dnorm[row0 + i] = norm;
+      }
+    }
+  }
+  top_norm = __reduce_max_sync(0xffffffffu, top_norm);
+  top_D = __reduce_max_sync(0xffffffffu, top_D);
+  if ((threadIdx.x & 31) == 0) {
+    unsigned* to = a.range + 4 * ((long long)seq * a.kv_heads + hk);
+    atomicMax(to + (is_v ? 0 : 1), top_norm);
+    if (!is_v) atomicMax(to + 2, top_D);
+  }
+}
+
 // --------------------------------------------------------------------------------------------------- dq
 //
 // 128 queries of one head per unit, keys streamed 128 at a time; two threads per row, 64 keys each. S is double
@@ -942,22 +1043,32 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
     const long long rows = (long long)a.seqs * a.heads * a.lq;
     bool ok = true;
     int g = 0, it = 0, units = 0;
-    // Statistics of this thread's row in the k-th unit.
+    // Statistics of this thread's row in the k-th unit; fp16: the norm of its dO too.
+    struct Row {
+      float2 st;
+      float dnorm;
+    };
     auto load_stats = [&](int k) {
+      Row r{make_float2(-INFINITY, 0.f), 0.f};
       const int ui = unit_index(k);
-      if (ui >= ta.units) return make_float2(-INFINITY, 0.f);
+      if (ui >= ta.units) return r;
       const TcUnit u = tc_unit(ta, a.heads, ui, true);
       const int i = u.tile * ROWS + row;
-      if (i >= a.lq) return make_float2(-INFINITY, 0.f);
-      return ta.stats[((long long)u.seq * a.heads + u.h) * a.lq + i];
+      if (i >= a.lq) return r;
+      const long long at = ((long long)u.seq * a.heads + u.h) * a.lq + i;
+      r.st = ta.stats[at];
+      if constexpr (std::is_same<T, __half>::value) r.dnorm = a.dnorm[at];
+      return r;
     };
-    float2 st_next = load_stats(0);
+    Row next = load_stats(0);
     for (int k = 0; ok; ++k) {
       const int ui = unit_index(k);
       if (ui >= ta.units && k * (int)gridDim.x >= ta.units) break;
-      const float2 st = st_next;
-      st_next = load_stats(k + 1);
+      const Row own = next;
+      next = load_stats(k + 1);
       if (ui >= ta.units) continue;
+      float2 st = own.st;
+      float unscale = a.scale;
       const TcUnit u = tc_unit(ta, a.heads, ui, true);
       const Bounds b = bounds_of(a, u.seq);
       int t0, t1;
@@ -966,6 +1077,12 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
       const int limit = a.causal ? min(b.kl, i + b.off + 1) : b.kl;
       const long long orow = ((long long)u.seq * a.heads + u.h) * a.lq + i;
       const bool live = st.x != -INFINITY;  // dead rows: P = 0
+      if constexpr (std::is_same<T, __half>::value) {
+        const float vnorm = __uint_as_float(a.range[4 * ((long long)u.seq * a.kv_heads + ta.by_group(u.h))]);
+        const int shift = fp16_shift(__float_as_uint(fmaf(own.dnorm, vnorm, fabsf(st.y))));
+        st.x += (float)shift;
+        unscale *= pow2(-shift);
+      }
       const float2 c2 = make_float2(c, c), l2 = make_float2(st.x, st.x), d2 = make_float2(st.y, st.y);
       // A thread's 64 keys go in two chunks; the loads of the next one are in flight during this one's exponentials.
       uint32_t s0[C::CH], d0[C::CH], s1[C::CH], d1[C::CH];
@@ -1079,9 +1196,9 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
         const int n = a.hd - 32 * q;
         if (i < a.lq && n > 0) {
           if (part)
-            store_cols_f32(part + 32 * q, v, a.scale, n);
+            store_cols_f32(part + 32 * q, v, unscale, n);
           else
-            store_cols<T>(dq + 32 * q, v, a.scale, n);
+            store_cols<T>(dq + 32 * q, v, unscale, n);
         }
       }
       if (t0 < t1) {
@@ -1376,7 +1493,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c = a.scale * LOG2E;
     const float unshift = exp2f(-p_shift<T>());
-    const float2 c2 = make_float2(c, c), un2 = make_float2(unshift, unshift);
+    const float2 c2 = make_float2(c, c);
     const long long rows = (long long)a.seqs * a.kv_heads * a.lk;
     bool ok = true;
     int g = 0, units = 0;
@@ -1389,6 +1506,15 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
       int begin, per, t0, t1;
       range(u, b, begin, per, t0, t1);
       const int j0 = u.tile * ROWS, j = j0 + row;
+      float ds_scale = unshift, dk_scale = a.scale;  // of dS next to P, and back
+      if constexpr (std::is_same<T, __half>::value) {
+        const uint4 r = *reinterpret_cast<const uint4*>(a.range + 4 * ((long long)u.seq * a.kv_heads + u.h));
+        const int shift = fp16_shift(
+            __float_as_uint(fmaf(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z))));
+        ds_scale *= pow2(shift);
+        dk_scale *= pow2(-shift);
+      }
+      const float2 un2 = make_float2(ds_scale, ds_scale);
       const int first = a.causal ? max(0, -b.off) : 0;       // queries before it see no key
       const int from = a.causal ? max(first, j - b.off) : 0; // this key is seen by queries [from, b.ql)
       // A thread's queries of a tile go in two chunks; the loads of the next one are in flight during this one's
@@ -1516,7 +1642,7 @@ __global__ void __launch_bounds__(DkvCfg<HD, SHORT>::THREADS, 1)
       T* out = static_cast<T*>(half ? a.dk : a.dv) + unit_offset(half ? a.dk_s : a.dv_s, u, u.h) +
                (long long)j * (half ? a.dk_s.row : a.dv_s.row);
       float* part = a.splits > 1 ? a.part + ((half ? 0 : a.splits) + u.split) * rows * a.hd + orow * a.hd : nullptr;
-      const float mul = half ? a.scale : unshift;
+      const float mul = half ? dk_scale : unshift;
 #pragma unroll 1
       for (int q = 0; q < HD / 32; ++q) {
         uint32_t v[32];
@@ -1600,6 +1726,7 @@ TcArgs tc_args(const AttnArgs& a, const UnblendAttnTrainParams& p, int heads, in
   t.by_tiles = fast_div(t.row_tiles);
   t.by_heads = fast_div(heads);
   t.by_inner = fast_div(a.inner);
+  t.by_group = fast_div(a.group);
   t.by_seq_heads = fast_div((long long)a.seqs * heads);
   t.stats = reinterpret_cast<const float2*>(a.dsum);
   return t;
@@ -1622,20 +1749,48 @@ int launch_fwd(const AttnArgs& a, const UnblendAttnTrainParams& p, int splits, c
   return 0;
 }
 
-template <typename T>
-int launch_stats(const AttnArgs& a, cudaStream_t st) {
+template <typename T, int LANES>
+int launch_stats_lanes(const AttnArgs& a, cudaStream_t st) {
   float2* stats = reinterpret_cast<float2*>(a.dsum);
-  const long long rows = (long long)a.seqs * a.lq * a.heads;
-  const FastDiv by_heads = fast_div(a.heads), by_lq = fast_div(a.lq), by_inner = fast_div(a.inner);
-  auto grid = [&](int lanes) { return (unsigned)((rows + STATS_ROWS * 256 / lanes - 1) / (STATS_ROWS * 256 / lanes)); };
-  if (a.hd <= 32)
-    attention_stats_kernel<T, 4><<<grid(4), 256, 0, st>>>(a, stats, by_heads, by_lq, by_inner);
-  else if (a.hd <= 64)
-    attention_stats_kernel<T, 8><<<grid(8), 256, 0, st>>>(a, stats, by_heads, by_lq, by_inner);
-  else
-    attention_stats_kernel<T, 16><<<grid(16), 256, 0, st>>>(a, stats, by_heads, by_lq, by_inner);
+  if constexpr (std::is_same<T, __half>::value) {
+    constexpr int STEP = STATS_ROWS * 32 / LANES;
+    RangeArgs ra{};
+    // About 32 warps per SM, what runs at once; a unit's rows are of one head, whose units are alike.
+    const long long rows = (long long)a.seqs * ((long long)a.heads * a.lq + (long long)a.kv_heads * a.lk);
+    const long long most = rows / (32LL * ub::kNumSMs * STEP);  // steps of a unit
+    auto share = [&](int len, int* chunks, int* each) {
+      const int steps = (len + STEP - 1) / STEP;
+      *each = (int)(most < 1 ? 1 : most < steps ? most : steps);
+      *chunks = (steps + *each - 1) / *each;
+      *each = (steps + *chunks - 1) / *chunks;
+    };
+    share(a.lq, &ra.q_chunks, &ra.q_steps);
+    share(a.lk, &ra.v_chunks, &ra.v_steps);
+    ra.q_units = (unsigned)((long long)a.seqs * a.heads * ra.q_chunks);
+    ra.units = ra.q_units + (unsigned)((long long)a.seqs * a.kv_heads * ra.v_chunks);
+    ra.by_heads = fast_div(a.heads);
+    ra.by_kv_heads = fast_div(a.kv_heads);
+    ra.by_q_chunks = fast_div(ra.q_chunks);
+    ra.by_v_chunks = fast_div(ra.v_chunks);
+    ra.by_group = fast_div(a.group);
+    ra.by_inner = fast_div(a.inner);
+    const cudaError_t e = cudaMemsetAsync(a.range, 0, sizeof(unsigned) * 4 * a.seqs * a.kv_heads, st);
+    if (e != cudaSuccess) return (int)e;
+    attention_stats_range_kernel<T, LANES><<<ra.units / 8 + (ra.units % 8 != 0), 256, 0, st>>>(a, stats, ra);
+  } else {
+    constexpr int PER_CTA = STATS_ROWS * 256 / LANES;
+    const long long rows = (long long)a.seqs * a.lq * a.heads;
+    attention_stats_kernel<T, LANES><<<(unsigned)((rows + PER_CTA - 1) / PER_CTA), 256, 0, st>>>(
+        a, stats, fast_div(a.heads), fast_div(a.lq), fast_div(a.inner));
+  }
   UB_CHECK_LAUNCH();
   return 0;
+}
+
+template <typename T>
+int launch_stats(const AttnArgs& a, cudaStream_t st) {
+  if (a.hd <= 32) return launch_stats_lanes<T, 4>(a, st);
+  return a.hd <= 64 ? launch_stats_lanes<T, 8>(a, st) : launch_stats_lanes<T, 16>(a, st);
 }
 
 template <typename T, int HD, bool SHORT>
