@@ -37,3 +37,48 @@ def test_statistics_off_their_alignment_are_copied(monkeypatch):
     x = torch.zeros(16, 8)
     training.layer_norm_backward(x, x, stats)
     assert seen["unblend_layer_norm_backward"][6] % 8 == 0
+
+
+def _attention_workspace(backward=False, **kw):
+    p = _lib.AttnTrainParams()
+    base = dict(dtype=_lib.DTYPE_BF16, outer=1, inner=1, heads=8, kv_heads=8, lq=100, lk=100, hd=64, causal=0,
+                scale=0.125)
+    for name, v in {**base, **kw}.items():
+        setattr(p, name, v)
+    n = ctypes.c_longlong(-1)
+    assert _lib.load().unblend_attention_workspace(ctypes.byref(p), int(backward), ctypes.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("dtype", [_lib.DTYPE_F32, _lib.DTYPE_BF16, _lib.DTYPE_F16])
+@pytest.mark.parametrize("kw", [
+    dict(lq=8192, lk=8192, heads=16, kv_heads=4, hd=128, causal=1), dict(outer=8, lq=2688, lk=1344),
+    dict(inner=62, lq=801, lk=801), dict(lq=65536, lk=65536, heads=32, kv_heads=8, hd=128),
+    dict(inner=801, lq=62, lk=62), dict(outer=64, lq=300, lk=8000, heads=16, kv_heads=1)])
+def test_calls_that_fill_the_gpu_need_no_forward_workspace(kw, dtype):
+    """Parts of split keys are for calls with too few rows of queries: no room for them where there are enough."""
+    assert _attention_workspace(dtype=dtype, **kw) == 0
+
+
+def test_workspace_is_what_the_parts_take():
+    """A few rows per key/value head are split into at most 32 parts, other calls into what four waves of CTAs take."""
+    # 4 sequences of 4 key/value heads: 592 CTAs wanted, 32 parts each of 64 rows with their sums.
+    assert _attention_workspace(outer=4, lq=1, lk=8191, heads=16, kv_heads=4, hd=128) == 32 * 64 * 129 * 4
+    for dtype in (_lib.DTYPE_F32, _lib.DTYPE_BF16, _lib.DTYPE_F16):
+        size = 4 if dtype == _lib.DTYPE_F32 else 2
+        for outer, heads, kv, lq, lk, hd in ((1, 8, 8, 300, 5000, 64), (2, 16, 4, 40, 4097, 128), (1, 1, 1, 17, 9000, 40),
+                                             (3, 4, 2, 129, 700, 96), (1, 2, 2, 8, 100000, 64), (7, 8, 1, 2, 3000, 72),
+                                             (1, 4, 4, 5000, 130, 64), (1, 1, 1, 1, 1, 1)):
+            few = heads // kv * lq <= (8 if size == 4 else 16) and hd * size % 16 == 0
+            tiles = outer * heads * -(-lq // 64)
+            parts = max(1, 4 * 296 // tiles, 32 if few else 1)
+            if tiles >= 296 and not few:
+                parts = 0
+            rows = outer * heads * lq
+            kw = dict(dtype=dtype, outer=outer, heads=heads, kv_heads=kv, lq=lq, lk=lk, hd=hd)
+            assert _attention_workspace(**kw) <= 4 * min(32, parts) * rows * (hd + 1)
+            key_rows, key_tiles = outer * kv * lk, outer * kv * -(-lk // 64)
+            most = 4 * (3 * rows + 8 + 4 * outer * kv)  # statistics, norms, ranges
+            most += 4 * min(32, max(0 if tiles >= 296 else 1, 4 * 296 // tiles)) * rows * hd
+            most += 8 * min(32, max(0 if key_tiles >= 296 else 1, 4 * 296 // key_tiles)) * key_rows * hd
+            assert _attention_workspace(True, **kw) <= most + 64

@@ -840,9 +840,15 @@ Plan plan_of(const UnblendAttnTrainParams& p, Path path) {
   return n;
 }
 
+// Few rows per key/value head, of whole 16-byte chunks: what the sizes alone say.
+bool few_rows_fit(const UnblendAttnTrainParams& p) {
+  const int most = p.dtype == UNBLEND_F32 ? FEW_ROWS : MMA_ROWS;
+  return (long long)p.heads / p.kv_heads * p.lq <= most && p.hd % (16 / elem_size(p.dtype)) == 0;
+}
+
 // Workspace: forward [parts][q_rows][hd] and [parts][q_rows] lse; backward D or row statistics [q_rows][2], for fp16
 // norms [q_rows] and ranges [seqs * kv_heads][4], then the parts of dq and of dk and dv, which one kernel joins. Room
-// for either kind of kernels: which of them runs depends on the pointers too.
+// for each kind of kernels that the sizes allow: which of them runs depends on the pointers too.
 long long norm_floats(const UnblendAttnTrainParams& p, const Plan& n) {
   return p.dtype == UNBLEND_F16 ? round4(n.q_rows) : 0;
 }
@@ -858,8 +864,10 @@ long long dq_part_floats(const UnblendAttnTrainParams& p, const Plan& n) {
 
 long long workspace_floats(const UnblendAttnTrainParams& p, bool backward) {
   long long most = 0;
-  for (int path = CUDA_CORES; path <= FEW; ++path) {
-    const Plan n = plan_of(p, (Path)path);
+  for (const Path path : {CUDA_CORES, TENSOR_CORES, FEW}) {
+    if (path == TENSOR_CORES && !attention_tc_sizes(p)) continue;
+    if (path == FEW && (backward || !few_rows_fit(p))) continue;
+    const Plan n = plan_of(p, path);
     long long need;
     if (!backward) {
       need = n.fwd_splits > 1 ? n.fwd_splits * n.q_rows * (p.hd + 1LL) : 0;
@@ -895,8 +903,7 @@ bool vec4_ok(const void* p, const UnblendHeadStrides& s, const UnblendAttnTrainP
 // Few rows per key/value head, K and V in 16-byte chunks.
 bool few_fits(const UnblendAttnTrainParams& p, const void* k, const void* v) {
   const int e = 16 / elem_size(p.dtype);
-  const int most = p.dtype == UNBLEND_F32 ? FEW_ROWS : MMA_ROWS;
-  if ((long long)p.heads / p.kv_heads * p.lq > most || p.hd % e != 0) return false;
+  if (!few_rows_fit(p)) return false;
   for (const UnblendHeadStrides* s : {&p.k, &p.v})
     if ((p.lk > 1 && s->row % e != 0) || (p.kv_heads > 1 && s->head % e != 0) || (p.inner > 1 && s->inner % e != 0) ||
         (p.outer > 1 && s->outer % e != 0))

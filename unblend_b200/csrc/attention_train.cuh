@@ -182,7 +182,9 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// The tensor-core kernels (attention_train_tc.cu). `fits`: whether they can address the n tensors of a call.
+// The tensor-core kernels (attention_train_tc.cu). `sizes`: whether they take a call of this type, head dim and scale;
+// `fits`: and can address its n tensors.
+bool attention_tc_sizes(const UnblendAttnTrainParams& p);
 bool attention_tc_fits(const UnblendAttnTrainParams& p, const void* const* ptrs, const UnblendHeadStrides* strides,
                        const int* heads, const int* rows, int n);
 int attention_fwd_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int rows_per_cta, cudaStream_t st);

@@ -1865,11 +1865,15 @@ int attention_dkv_tc(const AttnArgs& a, const UnblendAttnTrainParams& p, int spl
   });
 }
 
-// What the tensor-core kernels can address: 16-byte rows and strides (TMA, vector stores), a positive scale (the row
-// maximum is taken before the scale).
+// Rows of whole 16-byte chunks, and a positive scale (the row maximum is taken before the scale).
+bool attention_tc_sizes(const UnblendAttnTrainParams& p) {
+  return p.dtype != UNBLEND_F32 && p.hd % 8 == 0 && p.scale > 0.f;
+}
+
+// What the tensor-core kernels can address: bases and strides of whole 16-byte chunks (TMA, vector stores).
 bool attention_tc_fits(const UnblendAttnTrainParams& p, const void* const* ptrs, const UnblendHeadStrides* strides,
                        const int* heads, const int* rows, int n) {
-  if (p.dtype == UNBLEND_F32 || p.hd % 8 != 0 || !(p.scale > 0.f)) return false;
+  if (!attention_tc_sizes(p)) return false;
   for (int i = 0; i < n; ++i) {
     if (reinterpret_cast<uintptr_t>(ptrs[i]) % 16 != 0) return false;
     const UnblendHeadStrides& s = strides[i];
