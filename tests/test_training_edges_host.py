@@ -82,3 +82,25 @@ def test_workspace_is_what_the_parts_take():
             most += 4 * min(32, max(0 if tiles >= 296 else 1, 4 * 296 // tiles)) * rows * hd
             most += 8 * min(32, max(0 if key_tiles >= 296 else 1, 4 * 296 // key_tiles)) * key_rows * hd
             assert _attention_workspace(True, **kw) <= most + 64
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A dual tensor has ``requires_grad`` false: it must not pass as a plain one, its tangent lost without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    monkeypatch.setattr(training, "_check_cuda", lambda *a: None)
+    monkeypatch.setattr(training, "_launch", lambda *a, **kw: None)
+    x, w, q = torch.randn(3, 8), torch.ones(8), torch.randn(1, 3, 2, 8)
+    rng = torch.zeros(2, dtype=torch.int64)
+    with fwd.dual_level():
+        dx, dw, dq = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, w, q))
+        for call in (lambda: training.layer_norm(dx), lambda: training.layer_norm(x, dw),
+                     lambda: training.layer_norm(x, w, dw), lambda: training.attention(dq, q, q),
+                     lambda: training.attention(q, dq, q), lambda: training.attention(q, q, dq),
+                     lambda: training.dropout_add(dx, 0.1, rng), lambda: training.dropout_add(x, 0.1, rng, dx),
+                     lambda: training.dropout_add(x, 0.1, rng, x, dw)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        training.layer_norm(x, w)  # no tangents: a plain call, inside a dual level too

@@ -13,7 +13,7 @@ Memory is allocated by torch for each call, so calls on several streams and capt
 
 CUDA graphs: capture the plain calls. The differentiable functions refuse to record or run a backward pass while a
 stream is being captured: autograd's gradient accumulation of leaves that an earlier eager pass still holds runs on
-that pass's stream, which breaks the capture.
+that pass's stream, which breaks the capture. Second derivatives and forward-mode derivatives are refused too.
 """
 
 from __future__ import annotations
@@ -23,6 +23,7 @@ import math
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -234,7 +235,11 @@ class _LayerNorm(torch.autograd.Function):
         return dx, dgamma, dbeta, None
 
 
-def _wants_grad(*tensors) -> bool:
+def _wants_grad(what: str, *tensors) -> bool:
+    """Whether a call has to be recorded; tangents of forward mode, which no operator here carries on, are refused."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
@@ -242,7 +247,7 @@ def layer_norm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.T
                eps: float = 1e-5) -> torch.Tensor:
     """Differentiable layer norm over the last axis (``layer_norm_forward`` / ``layer_norm_backward``)."""
     _check_norm(x, gamma, beta, eps)
-    if _wants_grad(x, gamma, beta):
+    if _wants_grad("layer_norm", x, gamma, beta):
         _check_cuda("x", x)
         _refuse_capture("layer_norm")
         return _LayerNorm.apply(x, gamma, beta, eps)
@@ -409,7 +414,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
               q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None) -> torch.Tensor:
     """Differentiable multi-head attention (arguments as ``attention_forward``)."""
     scale = _check_attention(q, k, v, scale, causal, q_lens, k_lens)
-    if _wants_grad(q, k, v):
+    if _wants_grad("attention", q, k, v):
         _check_cuda("q", q)
         _refuse_capture("attention")
         return _Attention.apply(q, k, v, scale, causal, q_lens, k_lens)
@@ -523,7 +528,7 @@ def dropout_add(x: torch.Tensor, p: float, rng: torch.Tensor, residual: torch.Te
                 scale: torch.Tensor | None = None) -> torch.Tensor:
     """Differentiable ``residual + scale * dropout(x, p)`` (arguments as ``dropout_add_forward``)."""
     _check_dropout(x, p, rng, residual, scale)
-    if _wants_grad(x, residual, scale):
+    if _wants_grad("dropout_add", x, residual, scale):
         _check_cuda("x", x)
         _refuse_capture("dropout_add")
         return _DropoutAdd.apply(x, p, rng, residual, scale)
