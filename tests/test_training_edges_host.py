@@ -104,3 +104,36 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                 call()
         training.layer_norm(x, w)  # no tangents: a plain call, inside a dual level too
+
+
+def test_sizes_beyond_the_kernels_are_value_errors(monkeypatch):
+    """As every wrong argument, and before anything is allocated or launched. Expanded tensors need no memory here."""
+    monkeypatch.setattr(training, "_launch", lambda *a, **kw: pytest.fail("launched"))
+    rng = torch.zeros(2, dtype=torch.int64)
+    for shape in ((1 << 31, 1), (1 << 16, 1 << 16, 1), (1, 1 << 31)):
+        x = torch.zeros((1,) * len(shape)).expand(shape)
+        rows = x.numel() // shape[-1]
+        for call in (lambda: training.layer_norm_forward(x),
+                     lambda: training.layer_norm_backward(x, x, torch.zeros(1, 1).expand(rows, 2)),
+                     lambda: training.dropout_add_forward(x, 0.5, rng),
+                     lambda: training.dropout_add_backward(x, x, 0.5, rng)):
+            with pytest.raises(ValueError, match="rows"):
+                call()
+    for shape in ((1, 1 << 30, 1, 1), (1 << 31, 1, 1, 1), (1 << 16, 1 << 16, 1, 1, 1), (1, (1 << 32) + 5, 1, 1),
+                  (1 << 20, 1, 1 << 10, 1), (1, 1, 1 << 32, 1)):
+        q = torch.zeros((1,) * len(shape)).expand(shape)
+        lse = torch.zeros(1, 1, 1).expand(q.numel() // shape[-3] // shape[-2], shape[-2], shape[-3])
+        with pytest.raises(ValueError, match="beyond"):
+            training.attention_forward(q, q, q)
+        with pytest.raises(ValueError, match="beyond"):
+            training.attention_backward(q, q, q, q, q, lse)
+
+
+def test_arguments_that_fp32_cannot_hold_and_missing_results():
+    q, x = torch.zeros(1, 2, 1, 8), torch.zeros(2, 8)
+    for call in (lambda: training.attention(q, q, q, scale=1e39), lambda: training.attention(q, q, q, scale=-1e300),
+                 lambda: training.layer_norm_backward(x, x, None), lambda: training.layer_norm_backward(x, x, 1.0),
+                 lambda: training.attention_backward(q, q, q, q, q, None)):
+        with pytest.raises(ValueError) as e:
+            call()
+        assert "CUDA devices only" not in str(e.value)

@@ -29,6 +29,8 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 MAX_HEAD_DIM = 128
+_F32_MAX = torch.finfo(torch.float32).max
+_MOST = 1 << 31  # rows, and columns, of layer norm and dropout-add
 
 
 def _launch(t: torch.Tensor, name: str, *args) -> None:
@@ -53,6 +55,11 @@ def _check_tensor(name: str, t, like: torch.Tensor | None = None) -> None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     if like is not None and t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+
+
+def _check_rows(x: torch.Tensor) -> None:
+    if x.shape[-1] >= _MOST or x.numel() >= _MOST * x.shape[-1]:
+        raise ValueError(f"x must have fewer than 2^31 rows and columns, got shape {tuple(x.shape)}")
 
 
 def _check_cuda(name: str, t: torch.Tensor) -> None:
@@ -122,10 +129,16 @@ def _workspace_bytes(name: str, rows: int, cols: int) -> int:
 
 @lru_cache(maxsize=4096)
 def _attention_workspace_bytes(backward: int, *sizes) -> int:
+    """Refuses sizes that the kernels do not take, on the way."""
     p = _lib.AttnTrainParams(*sizes)
     n = ctypes.c_longlong(0)
-    _lib.check("unblend_attention_workspace",
-               _lib.load().unblend_attention_workspace(ctypes.byref(p), backward, ctypes.byref(n)))
+    rc = _lib.ERR_INVALID
+    if max(sizes[:-1]) < _MOST:  # the fields are 32 bits
+        rc = _lib.load().unblend_attention_workspace(ctypes.byref(p), backward, ctypes.byref(n))
+    if rc == _lib.ERR_INVALID:
+        raise ValueError("sizes beyond what attention takes: outer {1}, inner {2}, {3} heads over {4}, {5} queries, "
+                         "{6} keys, head_dim {7}".format(*sizes))
+    _lib.check("unblend_attention_workspace", rc)
     return n.value
 
 
@@ -146,6 +159,7 @@ def _check_norm(x, gamma, beta, eps: float) -> None:
     _check_tensor("x", x)
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must have a last axis to normalise over, got shape {tuple(x.shape)}")
+    _check_rows(x)
     if not (isinstance(eps, (int, float)) and eps >= 0):
         raise ValueError(f"eps must be >= 0, got {eps!r}")
     for name, w in (("gamma", gamma), ("beta", beta)):
@@ -191,7 +205,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, 
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"dy must be {x.dtype} of shape {tuple(x.shape)}, got {dy.dtype} {tuple(dy.shape)}")
     n, cols = x.numel() // x.shape[-1], x.shape[-1]
-    if stats.shape != (n, 2) or stats.dtype != torch.float32 or stats.device != x.device:
+    if not isinstance(stats, torch.Tensor) or stats.shape != (n, 2) or stats.dtype != torch.float32 or stats.device != x.device:
         raise ValueError("stats must be the second result of layer_norm_forward for this x")
     _check_cuda("x", x)
     dx = _empty(x)
@@ -291,8 +305,8 @@ def _check_attention(q, k, v, scale, causal, q_lens, k_lens) -> float:
     _check_lens("q_lens", q_lens, seqs, q)
     _check_lens("k_lens", k_lens, seqs, q)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= _F32_MAX:
+        raise ValueError(f"scale must be finite in float32, got {scale}")
     return scale
 
 
@@ -332,20 +346,19 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     ``lse`` (fp32, ``[sequences, heads, lq]``) is what ``attention_backward`` recomputes the probabilities from.
     """
     scale = _check_attention(q, k, v, scale, causal, q_lens, k_lens)
+    empty = q.numel() == 0 or k.shape[-3] == 0
+    sizes = _sizes(q, k, scale, causal)
+    n = 0 if empty else _attention_workspace_bytes(0, *sizes)
     _check_cuda("q", q)
     out = _empty(q)
     lse = q.new_empty((_seqs(q), q.shape[-2], q.shape[-3]), dtype=torch.float32)
-    if lse.numel() == 0:
-        return out, lse
-    if k.shape[-3] == 0:
+    if empty:
         return out.zero_(), lse.fill_(-math.inf)
     q, k, v = _unit(q), _unit(k), _unit(v)
     q_lens = None if q_lens is None else q_lens.contiguous()
     k_lens = None if k_lens is None else k_lens.contiguous()
-    sizes = _sizes(q, k, scale, causal)
     p = _lib.AttnTrainParams(*sizes, _lib.ptr(q_lens), _lib.ptr(k_lens), _strides(q), _strides(k), _strides(v),
                              _strides(out))
-    n = _attention_workspace_bytes(0, *sizes)
     work = _scratch(q, n)
     _launch(q, "unblend_attention_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
             _lib.ptr(work), n, ctypes.byref(p))
@@ -370,20 +383,22 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         if t.shape != q.shape:
             raise ValueError(f"{name} must have q's shape {tuple(q.shape)}, got {tuple(t.shape)}")
     seqs = _seqs(q)
-    if lse.shape != (seqs, q.shape[-2], q.shape[-3]) or lse.dtype != torch.float32 or lse.device != q.device:
+    if not isinstance(lse, torch.Tensor) or lse.shape != (seqs, q.shape[-2], q.shape[-3]) or \
+            lse.dtype != torch.float32 or lse.device != q.device:
         raise ValueError("lse must be the second result of attention_forward for this q")
+    empty = q.numel() == 0 or k.numel() == 0
+    sizes = _sizes(q, k, scale, causal)
+    n = 0 if empty else _attention_workspace_bytes(1, *sizes)
     _check_cuda("q", q)
     dq, dk, dv = _empty(q), _empty(k), _empty(v)
-    if q.numel() == 0 or k.numel() == 0:
+    if empty:
         return dq.zero_(), dk.zero_(), dv.zero_()
     q, k, v, out, dout = _unit(q), _unit(k), _unit(v), _unit(out), _unit(dout)
     q_lens = None if q_lens is None else q_lens.contiguous()
     k_lens = None if k_lens is None else k_lens.contiguous()
-    sizes = _sizes(q, k, scale, causal)
     p = _lib.AttnTrainParams(*sizes, _lib.ptr(q_lens), _lib.ptr(k_lens),
                              *(_strides(t) for t in (q, k, v, out, dout, dq, dk, dv)), bool(all_keys))
     lse = lse.contiguous()
-    n = _attention_workspace_bytes(1, *sizes)
     work = _scratch(q, n)
     _launch(q, "unblend_attention_backward", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
             out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(work), n,
@@ -428,6 +443,7 @@ def _check_dropout(x, p: float, rng, residual, scale) -> None:
     _check_tensor("x", x)
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must have a last axis, got shape {tuple(x.shape)}")
+    _check_rows(x)
     if not (isinstance(p, (int, float)) and 0 <= p <= 1):
         raise ValueError(f"p must be a probability, got {p!r}")
     if not isinstance(rng, torch.Tensor) or rng.dtype != torch.int64 or rng.numel() != 2 or rng.device != x.device:
