@@ -137,3 +137,26 @@ def test_arguments_that_fp32_cannot_hold_and_missing_results():
         with pytest.raises(ValueError) as e:
             call()
         assert "CUDA devices only" not in str(e.value)
+
+
+def test_dropout_keeps_its_input_only_for_the_scale(monkeypatch):
+    """The branch's activations are read for the LayerScale's gradient alone; without it they may be freed."""
+    launched = []
+    monkeypatch.setattr(training, "_check_cuda", lambda *a: None)
+    monkeypatch.setattr(training, "_refuse_capture", lambda *a: None)
+    monkeypatch.setattr(training, "_launch", lambda t, name, *args, **kw: launched.append((name, args)))
+    rng, w = torch.zeros(2, dtype=torch.int64), torch.ones(8)
+    for x_dtype in (torch.float32, torch.bfloat16):
+        for scale in (None, w, w.clone().requires_grad_()):
+            x = torch.randn(5, 3, 8, dtype=x_dtype).requires_grad_()
+            res = torch.randn(5, 3, 8)
+            y = training.dropout_add(x, 0.1, rng, res, scale)
+            kept = [t.data_ptr() for t in y.grad_fn.saved_tensors if t is not None]
+            learns = scale is not None and scale.requires_grad
+            assert (x.data_ptr() in kept) == learns
+            y.backward(torch.ones(5, 3, 8))
+            assert x.grad.shape == x.shape and x.grad.dtype == x_dtype
+            name, args = launched[-1]
+            assert name == "unblend_dropout_add_backward" and (args[3] == x.data_ptr()) == learns
+            assert not learns or scale.grad.shape == w.shape
+            assert args[12:15] == (1, 15, 8) and args[15:17] == (training._DTYPES[x_dtype], _lib.DTYPE_F32)

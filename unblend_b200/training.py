@@ -499,22 +499,26 @@ def dropout_add_backward(dy: torch.Tensor, x: torch.Tensor, p: float, rng: torch
         raise ValueError(f"dy must be float32 or {x.dtype} of shape {tuple(x.shape)}, got {dy.dtype} "
                          f"{tuple(dy.shape)}")
     _check_cuda("x", x)
-    dx = _empty(x)
-    dscale = _empty(scale) if scale is not None and scale_grad else None
-    if x.numel() == 0:
+    return _dropout_backward(dy, x, x.dtype, p, rng, scale, scale is not None and scale_grad)
+
+
+def _dropout_backward(dy, x, dtype, p: float, rng, scale, scale_grad: bool):
+    """The backward pass of checked arguments; x, of type ``dtype``, is read only with ``scale_grad``."""
+    dx = _empty(dy) if dy.dtype == dtype else _empty(dy, dtype)
+    dscale = _empty(scale) if scale_grad else None
+    if dy.numel() == 0:
         return dx, None if dscale is None else dscale.zero_()
     rng = rng.contiguous()
     scale = None if scale is None else scale.contiguous()
     dr = _rows(dy)
     xr = (None, dr[1], dr[2], 0, 0)
-    if dscale is not None:
-        dr, xr = _same_split(dr, _rows(x))
     work = None
-    if dscale is not None:
-        work = _scratch(x, _workspace_bytes("unblend_dropout_add_grad_workspace", dr[1] * dr[2], x.shape[-1]))
-    _launch(x, "unblend_dropout_add_backward", dr[0].data_ptr(), dr[3], dr[4], _lib.ptr(xr[0]), xr[3], xr[4],
+    if scale_grad:
+        dr, xr = _same_split(dr, _rows(x))
+        work = _scratch(dy, _workspace_bytes("unblend_dropout_add_grad_workspace", dr[1] * dr[2], dy.shape[-1]))
+    _launch(dy, "unblend_dropout_add_backward", dr[0].data_ptr(), dr[3], dr[4], _lib.ptr(xr[0]), xr[3], xr[4],
             _lib.ptr(scale), dx.data_ptr(), _lib.ptr(dscale), _lib.ptr(work), float(p), rng.data_ptr(), dr[1], dr[2],
-            x.shape[-1], _DTYPES[x.dtype], _DTYPES[dy.dtype],
+            dy.shape[-1], _DTYPES[dtype], _DTYPES[dy.dtype],
             _lib.DTYPE_F32 if scale is None else _DTYPES[scale.dtype])
     return dx, dscale
 
@@ -524,8 +528,8 @@ class _DropoutAdd(torch.autograd.Function):
     def forward(ctx, x, p, rng, residual, scale):
         # The backward pass draws the mask again: it keeps a copy, so that the caller may advance rng in place.
         rng = rng.clone()
-        ctx.save_for_backward(x, rng, scale)
-        ctx.p, ctx.residual = p, residual is not None
+        ctx.save_for_backward(x if scale is not None and ctx.needs_input_grad[4] else None, rng, scale)
+        ctx.p, ctx.residual, ctx.dtype = p, residual is not None, x.dtype
         return dropout_add_forward(x, p, rng, residual, scale)
 
     @staticmethod
@@ -536,7 +540,7 @@ class _DropoutAdd(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dscale = None
         if need[0] or need[4]:
-            dx, dscale = dropout_add_backward(dy, x, ctx.p, rng, scale, need[4])
+            dx, dscale = _dropout_backward(dy, x, ctx.dtype, ctx.p, rng, scale, need[4])
         return dx if need[0] else None, None, None, dy if ctx.residual and need[3] else None, dscale
 
 
