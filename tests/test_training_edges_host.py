@@ -160,3 +160,24 @@ def test_dropout_keeps_its_input_only_for_the_scale(monkeypatch):
             assert name == "unblend_dropout_add_backward" and (args[3] == x.data_ptr()) == learns
             assert not learns or scale.grad.shape == w.shape
             assert args[12:15] == (1, 15, 8) and args[15:17] == (training._DTYPES[x_dtype], _lib.DTYPE_F32)
+
+
+def test_launch_counts_are_what_a_call_launches(monkeypatch):
+    """Layer norm's backward pass is one kernel, two where partial sums are joined, three for rows over 8192 columns;
+    dropout's two with a scale's gradient."""
+    counts = []
+    monkeypatch.setattr(training, "_check_cuda", lambda *a: None)
+    monkeypatch.setattr(training, "_launch", lambda t, name, *args, kernels=1: counts.append(kernels))
+    for rows, cols, weights, want in ((64, 512, True, 1), (65, 512, True, 2), (1000, 512, False, 1), (1, 1024, True, 1),
+                                      (1, 1025, True, 1), (2, 1025, True, 2), (2, 8192, False, 1), (1, 8193, True, 3),
+                                      (300, 9000, True, 3), (300, 9000, False, 1)):
+        x = torch.zeros(rows, cols)
+        training.layer_norm_backward(x, x, torch.zeros(rows, 2), weight_grads=weights)
+        assert counts.pop() == want, (rows, cols, weights)
+    x, rng, w = torch.zeros(4, 8), torch.zeros(2, dtype=torch.int64), torch.ones(8)
+    for scale, grad, want in ((None, True, 1), (w, False, 1), (w, True, 2)):
+        training.dropout_add_backward(x, x, 0.5, rng, scale, grad)
+        assert counts.pop() == want
+    training.dropout_add_forward(x, 0.5, rng)
+    training.layer_norm_forward(x)
+    assert counts == [1, 1]

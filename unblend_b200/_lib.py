@@ -283,11 +283,10 @@ def check(name: str, rc: int) -> None:
     raise RuntimeError(f"{name} failed: {text} ({rc})")
 
 
-# Kernels launched by one call of each entry point (1 unless listed).
-# Attention calls can launch more (joins of split axes, one kernel per gradient): that depends on the sizes and is not
-# counted.
-KERNELS_PER_CALL = {"unblend_mean_std": 3, "unblend_istft_output": 2, "unblend_istft_masked": 2,
-                    "unblend_layer_norm_backward": 2, "unblend_dropout_add_backward": 2}
+# Kernels launched by one call of each entry point (1 unless listed, or given by the caller). The attention with
+# gradients can launch more (joins of split axes, a kernel per gradient), which depends on sizes and pointers and is not
+# counted: its counts are lower bounds.
+KERNELS_PER_CALL = {"unblend_mean_std": 3, "unblend_istft_output": 2, "unblend_istft_masked": 2}
 
 # Launch accounting: total kernels launched through this binding.
 counters = {"launches": 0}
@@ -299,8 +298,8 @@ counters = {"launches": 0}
 probe: list | None = None
 
 
-def call(name: str, *args, work: float | None = None) -> None:
-    """Invoke ``name`` with ``args`` (the trailing stream is appended) and check it."""
+def call(name: str, *args, work: float | None = None, kernels: int | None = None) -> None:
+    """Invoke ``name`` with ``args`` (the trailing stream is appended) and check it; ``kernels``: what it launches."""
     lib = load()
     if probe is not None:
         cur = torch.cuda.current_stream()
@@ -313,7 +312,7 @@ def call(name: str, *args, work: float | None = None) -> None:
     else:
         # The handle alone: building a torch.cuda.Stream object costs more than most launches.
         rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
-    counters["launches"] += KERNELS_PER_CALL.get(name, 1)
+    counters["launches"] += KERNELS_PER_CALL.get(name, 1) if kernels is None else kernels
     check(name, rc)
 
 

@@ -30,16 +30,17 @@ from . import _lib
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 MAX_HEAD_DIM = 128
 _F32_MAX = torch.finfo(torch.float32).max
+_REGISTER_COLS = 8192  # widest rows whose layer norm sums the weights' gradients beside the input's
 _MOST = 1 << 31  # rows, and columns, of layer norm and dropout-add
 
 
-def _launch(t: torch.Tensor, name: str, *args) -> None:
-    """Calls an entry point on the current stream of ``t``'s device."""
+def _launch(t: torch.Tensor, name: str, *args, kernels: int = 1) -> None:
+    """Calls an entry point, which launches ``kernels`` kernels, on the current stream of ``t``'s device."""
     if torch._C._cuda_getDevice() == t.get_device():
-        _lib.call(name, *args)
+        _lib.call(name, *args, kernels=kernels)
     else:
         with torch.cuda.device(t.get_device()):
-            _lib.call(name, *args)
+            _lib.call(name, *args, kernels=kernels)
 
 
 def _empty(like: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -224,7 +225,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, 
     work = _scratch(x, _workspace_bytes("unblend_layer_norm_grad_workspace", n, cols)) if weight_grads else None
     _launch(x, "unblend_layer_norm_backward", dyr.data_ptr(), d_so, d_si, xr.data_ptr(), x_so, x_si,
             stats.data_ptr(), _lib.ptr(gamma), dx.data_ptr(), _lib.ptr(dgamma), _lib.ptr(dbeta),
-            _lib.ptr(work), outer, inner, cols, _DTYPES[x.dtype], _DTYPES[wt])
+            _lib.ptr(work), outer, inner, cols, _DTYPES[x.dtype], _DTYPES[wt],
+            kernels=1 + (work is not None) + (weight_grads and cols > _REGISTER_COLS))
     return dx, dgamma, dbeta
 
 
@@ -519,7 +521,7 @@ def _dropout_backward(dy, x, dtype, p: float, rng, scale, scale_grad: bool):
     _launch(dy, "unblend_dropout_add_backward", dr[0].data_ptr(), dr[3], dr[4], _lib.ptr(xr[0]), xr[3], xr[4],
             _lib.ptr(scale), dx.data_ptr(), _lib.ptr(dscale), _lib.ptr(work), float(p), rng.data_ptr(), dr[1], dr[2],
             dy.shape[-1], _DTYPES[dtype], _DTYPES[dy.dtype],
-            _lib.DTYPE_F32 if scale is None else _DTYPES[scale.dtype])
+            _lib.DTYPE_F32 if scale is None else _DTYPES[scale.dtype], kernels=1 + scale_grad)
     return dx, dscale
 
 
