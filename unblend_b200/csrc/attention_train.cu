@@ -26,8 +26,6 @@ using namespace ub::train;
 constexpr int TILE = 64;
 constexpr int NT = 256;
 constexpr int LD = TILE + 4;  // row pitch of [dim][row] tiles: 16-byte rows, 4-bank shift per dim
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 
 // Rows [r0, r0 + 64) of a head into shared memory: transposed [dim][LD] and / or as rows [row][HDP + 4]. Rows from
 // `valid` on and dims from hd up to a multiple of 4 become 0. Lane = row, so the transposed stores do not conflict.
@@ -416,13 +414,13 @@ __global__ void __launch_bounds__(NT) attention_dkv_kernel(const __grid_constant
 // attention_join_kernel joins those. 4 x 8191 keys, 16 over 4 heads of 128, fp32: 40 us with the join (3.4 TB/s).
 constexpr int FEW_ROWS = 8, FEW_NT = 128, FEW_KEYS = 4, FEW_STAGES = 3;
 
-// K and V of a thread's keys in flight: FEW_STAGES x FEW_KEYS x (K, V) x 32 bytes (fp32) or 16.
-constexpr int few_smem(int elem) { return FEW_STAGES * FEW_KEYS * 2 * 8 * elem * FEW_NT; }
+// K and V of a thread's keys in flight: FEW_STAGES x FEW_KEYS x (K, V) x 32 bytes.
+constexpr int FEW_SMEM = FEW_STAGES * FEW_KEYS * 2 * 8 * (int)sizeof(float) * FEW_NT;
 
-template <typename T, int HD, int R>
+template <int HD, int R>
 __global__ void __launch_bounds__(FEW_NT) attention_few_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int LANES = HD / 8, GROUPS = 32 / LANES;
-  constexpr int V = 16 / (int)sizeof(T), CH = 8 / V;  // elements per chunk, chunks per lane
+  constexpr int V = 4, CH = 2;  // elements per chunk, chunks per lane
   constexpr int WARPS = FEW_NT / 32;
   __shared__ float sq[R][HD];
   __shared__ float so[WARPS][R][HD + 2];  // O, maximum, sum of each warp
@@ -437,15 +435,15 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_kernel(const __grid_cons
     const int r = x / HD, d = x - r * HD;
     float v = 0.f;
     if (r < n_rows && r % a.lq < b.ql && d < a.hd)
-      v = to_f((static_cast<const T*>(a.q) + head_offset(a.q_s, a, seq, hk * a.group + r / a.lq) +
-                (long long)(r % a.lq) * a.q_s.row)[d]) * c;
+      v = (static_cast<const float*>(a.q) + head_offset(a.q_s, a, seq, hk * a.group + r / a.lq) +
+           (long long)(r % a.lq) * a.q_s.row)[d] * c;
     sq[r][d] = v;
   }
   __syncthreads();
   const int keys = key_end(a, b, 0, a.lq);
   const int begin = (int)((long long)keys * split / a.splits), end = (int)((long long)keys * (split + 1) / a.splits);
-  const T* k = static_cast<const T*>(a.k) + head_offset(a.k_s, a, seq, hk);
-  const T* v = static_cast<const T*>(a.v) + head_offset(a.v_s, a, seq, hk);
+  const float* k = static_cast<const float*>(a.k) + head_offset(a.k_s, a, seq, hk);
+  const float* v = static_cast<const float*>(a.v) + head_offset(a.v_s, a, seq, hk);
   float o[R][CH * V], m[R], l[R];
   int limit[R];
 #pragma unroll
@@ -492,16 +490,14 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_kernel(const __grid_cons
     for (int x = 0; x < CH; ++x)
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        float q[V];
-#pragma unroll
-        for (int e = 0; e < V; e += 4)
-          *reinterpret_cast<float4*>(q + e) = *reinterpret_cast<const float4*>(&sq[r][(x * LANES + sub) * V + e]);
+        const float4 qw = *reinterpret_cast<const float4*>(&sq[r][(x * LANES + sub) * V]);
+        const float q[V] = {qw.x, qw.y, qw.z, qw.w};
 #pragma unroll
         for (int u = 0; u < FEW_KEYS; ++u) {
-          const uint4 w = *at(stage, u, x, 0);
-          const T* e = reinterpret_cast<const T*>(&w);
+          const float4 w = *reinterpret_cast<const float4*>(at(stage, u, x, 0));
+          const float e[V] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int i = 0; i < V; ++i) s[u][r] = fmaf(q[i], to_f(e[i]), s[u][r]);
+          for (int i = 0; i < V; ++i) s[u][r] = fmaf(q[i], e[i], s[u][r]);
         }
       }
 #pragma unroll
@@ -531,14 +527,12 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_kernel(const __grid_cons
     for (int u = 0; u < FEW_KEYS; ++u)
 #pragma unroll
       for (int x = 0; x < CH; ++x) {
-        const uint4 w = *at(stage, u, x, 1);
-        const T* e = reinterpret_cast<const T*>(&w);
+        const float4 w = *reinterpret_cast<const float4*>(at(stage, u, x, 1));
+        const float e[V] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float f = to_f(e[i]);
+        for (int i = 0; i < V; ++i)
 #pragma unroll
-          for (int r = 0; r < R; ++r) o[r][x * V + i] = fmaf(s[u][r], f, o[r][x * V + i]);
-        }
+          for (int r = 0; r < R; ++r) o[r][x * V + i] = fmaf(s[u][r], e[i], o[r][x * V + i]);
       }
   }
   // The groups of a warp, then the warps.
@@ -587,7 +581,7 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_kernel(const __grid_cons
       if (d == 0) a.part_lse[split * rows + row] = lse;
     } else {
       if (d < a.hd)
-        (static_cast<T*>(a.out) + head_offset(a.out_s, a, seq, h) + (long long)i * a.out_s.row)[d] = from_f<T>(out);
+        (static_cast<float*>(a.out) + head_offset(a.out_s, a, seq, h) + (long long)i * a.out_s.row)[d] = out;
       if (d == 0 && a.lse) a.lse[row] = lse;
     }
   }
@@ -650,7 +644,7 @@ __global__ void __launch_bounds__(FEW_NT) attention_few_mma_kernel(const __grid_
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const int d = 16 * ks + 8 * y + 2 * ql;
-        T e[2] = {from_f<T>(0.f), from_f<T>(0.f)};
+        alignas(4) T e[2] = {from_f<T>(0.f), from_f<T>(0.f)};
         if (in && d < a.hd) e[0] = q[d];
         if (in && d + 1 < a.hd) e[1] = q[d + 1];
         qf[ks][2 * y + x] = *reinterpret_cast<const uint32_t*>(e);
@@ -969,22 +963,22 @@ int simt_dkv(AttnArgs a, int splits, float* parts, bool vec, cudaStream_t st) {
   return 0;
 }
 
-template <typename T, int HD, int R>
+template <int HD, int R>
 int few_forward(const AttnArgs& a, cudaStream_t st) {
   const long long grid = (long long)a.seqs * a.kv_heads * a.splits;
-  if (allow_smem<attention_few_kernel<T, HD, R>>(few_smem(sizeof(T))) != cudaSuccess) return (int)cudaGetLastError();
-  attention_few_kernel<T, HD, R><<<(unsigned)grid, FEW_NT, few_smem(sizeof(T)), st>>>(a);
+  if (allow_smem<attention_few_kernel<HD, R>>(FEW_SMEM) != cudaSuccess) return (int)cudaGetLastError();
+  attention_few_kernel<HD, R><<<(unsigned)grid, FEW_NT, FEW_SMEM, st>>>(a);
   UB_CHECK_LAUNCH();
   return 0;
 }
 
-template <typename T, int HD>
+template <int HD>
 int few_rows(const AttnArgs& a, cudaStream_t st) {
   const int rows = a.group * a.lq;
-  if (rows == 1) return few_forward<T, HD, 1>(a, st);
-  if (rows == 2) return few_forward<T, HD, 2>(a, st);
-  if (rows <= 4) return few_forward<T, HD, 4>(a, st);
-  return few_forward<T, HD, 8>(a, st);
+  if (rows == 1) return few_forward<HD, 1>(a, st);
+  if (rows == 2) return few_forward<HD, 2>(a, st);
+  if (rows <= 4) return few_forward<HD, 4>(a, st);
+  return few_forward<HD, 8>(a, st);
 }
 
 template <typename T, int HD>
@@ -999,7 +993,7 @@ int few_mma(const AttnArgs& a, cudaStream_t st) {
 template <typename T>
 int few_types(const AttnArgs& a, cudaStream_t st) {
   if constexpr (sizeof(T) == 4)
-    return a.hd <= 64 ? few_rows<T, 64>(a, st) : few_rows<T, 128>(a, st);
+    return a.hd <= 64 ? few_rows<64>(a, st) : few_rows<128>(a, st);
   else
     return a.hd <= 64 ? few_mma<T, 64>(a, st) : few_mma<T, 128>(a, st);
 }
@@ -1043,8 +1037,9 @@ int backward_types(const AttnArgs& a, const UnblendAttnTrainParams& p, const Pla
                     : simt_dkv<T, 128>(a, n.dkv_splits, kv_parts, vec, st);
   if (rc || (n.dq_splits == 1 && n.dkv_splits == 1)) return rc;
   SumArgs sums{};
+  int tensors = 0;
   auto add = [&](const float* part, int splits, int heads, int len, void* out, const UnblendHeadStrides& to) {
-    SumArgs::One& x = sums.of[sums.count++];
+    SumArgs::One& x = sums.of[tensors++];
     x = SumArgs::One{part, out, to, splits, heads, len, (long long)a.seqs * heads * len};
     sums.rows += x.rows;
   };

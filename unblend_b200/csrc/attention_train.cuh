@@ -7,6 +7,9 @@
 namespace ub {
 namespace train {
 
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
 struct AttnArgs {
   const void *q, *k, *v, *dout;
   const void* out_in;  // forward output, read by the backward pass
@@ -58,6 +61,13 @@ __device__ __forceinline__ int key_limit(const AttnArgs& a, const Bounds& b, int
 __device__ __forceinline__ long long head_offset(const UnblendHeadStrides& s, const AttnArgs& a, int seq, int h) {
   const int o = seq / a.inner;
   return (long long)o * s.outer + (long long)(seq - o * a.inner) * s.inner + (long long)h * s.head;
+}
+
+// 2^x, the hardware approximation (2 ulp).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // dS = P (dP - D) of fp16 calls is stored times a power of two: unscaled, the gradients of a loss averaged over tokens
@@ -157,7 +167,6 @@ struct SumArgs {
     int splits, heads, len;
     long long rows;
   } of[3];
-  int count;
   long long rows;  // of all
 };
 

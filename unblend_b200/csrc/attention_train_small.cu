@@ -30,8 +30,6 @@ namespace {
 
 using namespace ub::train;
 
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 constexpr int P_COLS = 64;  // pitch of P and dS
 
 // R: rows of a tile, 64, or 32 for shorter sequences; a warp per 16.
@@ -50,12 +48,6 @@ struct SmallArgs {
   AttnArgs a;
   FastDiv by_heads, by_group, by_inner;  // by_heads: of the CTAs
 };
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ uint4 lds16(uint32_t p) {
   uint4 v;

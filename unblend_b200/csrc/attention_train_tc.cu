@@ -35,16 +35,8 @@ namespace {
 using namespace ub::tc;
 using namespace ub::train;
 
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 constexpr int ROWS = 128;                  // rows of a tile: TMEM lanes
 constexpr float RESCALE_THRESHOLD = 8.f;   // log2 units by which the maximum may grow before O is rescaled
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // 2^x of a pair on the FMA pipe, for a share of the exponentials (the special function unit takes 16 per cycle and SM,
 // the tightest limit at head dim 64). x = n + f with n the nearest integer, read off the low bits of x + 1.5 2^23; 2^f

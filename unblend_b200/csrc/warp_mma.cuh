@@ -41,7 +41,7 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
-  const T v[2] = {from_f<T>(lo), from_f<T>(hi)};
+  alignas(4) const T v[2] = {from_f<T>(lo), from_f<T>(hi)};
   return *reinterpret_cast<const uint32_t*>(v);
 }
 
