@@ -203,3 +203,55 @@ def test_fp16_gradients_of_uneven_sequences():
         # The small rows of dq on their own.
         want = ref["dq"][0][b, :int(ql[b]):2]
         assert _relative(got[0][b, :int(ql[b]):2], want) <= 2 * (_relative(want.half(), want) + 2.0**-11), b
+
+
+@pytest.mark.parametrize("lq,lk,h,hk", [(200, 300, 4, 2), (50, 60, 4, 4), (25, 30, 4, 2)])
+def test_infinite_gradients_stay_in_their_head(lq, lk, h, hk):
+    """An overflow in one head's dout leaves the scale, and every bit, of the others as they are."""
+    q, k, v, dout = _attn(3, lq, lk, h, hk, 64, F16)
+    out, lse = training.attention_forward(q, k, v)
+    clean = training.attention_backward(dout, q, k, v, out, lse)
+    bad = dout.clone()
+    bad[1, 7, h - 1, 3] = float("inf")
+    got = training.attention_backward(bad, q, k, v, out, lse)
+    for x, y in zip(got, clean):
+        assert torch.equal(x[[0, 2]], y[[0, 2]]) and torch.equal(x[1, :, 0], y[1, :, 0])
+    assert not got[0][1, 7, h - 1].isfinite().any() and not got[1][1, :, hk - 1].isfinite().all()
+
+
+def test_fp16_passes_captured_and_replayed():
+    """Graphs of fp16 passes (long rows, one tile, a few tokens of shared heads) replay on two streams at once, with new
+    inputs of another size."""
+    shapes = [(2, 200, 300, 4, 2, 64), (20, 50, 60, 4, 4, 64), (20, 20, 30, 4, 2, 48), (1, 500, 700, 4, 1, 128)]
+
+    def step(s):
+        out, lse = training.attention_forward(*s[:3])
+        return (out, *training.attention_backward(s[3], *s[:3], out, lse))
+
+    sets = [[list(_attn(*c, F16, seed=10 * n + i)) for i, c in enumerate(shapes)] for n in range(2)]
+    for s in sets[1]:
+        s[3] *= 1e-3
+    want = [[[x.clone() for x in step(s)] for s in group] for group in sets]
+    held = [[x.clone() for x in s] for s in sets[0]]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append([step(s) for s in held])
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for n in (0, 1, 0):
+        for mine, new in zip(held, sets[n]):
+            for x, y in zip(mine, new):
+                x.copy_(y)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for graph, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for got in outs:
+            for a, b in zip(got, want[n]):
+                assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert _lib.error_flag() == 0
