@@ -7,6 +7,7 @@ import ctypes
 import pytest
 import torch
 
+from training_reference import philox_words
 from unblend_b200 import _lib, training
 
 
@@ -181,3 +182,25 @@ def test_launch_counts_are_what_a_call_launches(monkeypatch):
     training.dropout_add_forward(x, 0.5, rng)
     training.layer_norm_forward(x)
     assert counts == [1, 1]
+
+
+def test_philox_against_all_published_vectors():
+    """Philox-4x32-10 by the paper's definition in Python integers, against its three known answers, and the words that
+    the other tests use against that."""
+    def philox(counter, key):
+        c, k = list(counter), list(key)
+        for _ in range(10):
+            a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+            c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+            k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+        return c
+
+    ones = 0xFFFFFFFF
+    assert philox([0] * 4, [0] * 2) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    assert philox([ones] * 4, [ones] * 2) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert philox([0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344], [0xA4093822, 0x299F31D0]) == \
+        [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+    for seed, offset, block in ((-1, -1, 0), (1 << 62, 3, 5), (-(1 << 63), 1 << 40, (1 << 60) + 7), (77, -2, 1 << 33)):
+        want = philox([block & ones, block >> 32, offset & ones, (offset >> 32) & ones],
+                      [seed & ones, (seed >> 32) & ones])
+        assert [int(w) for w in philox_words(seed, offset, 4 * block, 4)] == want
