@@ -255,3 +255,22 @@ def test_fp16_passes_captured_and_replayed():
             for a, b in zip(got, want[n]):
                 assert all(torch.equal(x, y) for x, y in zip(a, b))
     assert _lib.error_flag() == 0
+
+
+def test_calls_run_on_the_current_stream_without_torchs_private_handle(monkeypatch):
+    """The stream's handle comes from a function that torch does not document; without it the public one serves."""
+    x = _rand(500, 64, seed=5)
+    want = training.layer_norm_forward(x)[0].clone()
+    side = torch.cuda.Stream()
+    for gone in (False, True):
+        if gone:
+            monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+            monkeypatch.setattr(_lib, "_raw_stream", None)
+            monkeypatch.setattr(_lib, "current_device", torch.cuda.current_device)
+        for stream in (torch.cuda.current_stream(), side):
+            with torch.cuda.stream(stream):
+                assert _lib.current_stream() == stream.cuda_stream
+                y = x * 1
+                got = training.layer_norm_forward(y)[0]
+            stream.synchronize()
+            assert torch.equal(got, want)

@@ -298,6 +298,19 @@ counters = {"launches": 0}
 probe: list | None = None
 
 
+# The current device, and its stream's handle alone: building a torch.cuda.Stream object costs more than most launches.
+# Neither is part of torch's documented interface; where one is missing the public way serves.
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def current_stream() -> int:
+    """Handle of the current stream of the current device."""
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(current_device())
+
+
 def call(name: str, *args, work: float | None = None, kernels: int | None = None) -> None:
     """Invoke ``name`` with ``args`` (the trailing stream is appended) and check it; ``kernels``: what it launches."""
     lib = load()
@@ -310,8 +323,7 @@ def call(name: str, *args, work: float | None = None, kernels: int | None = None
         end.record(cur)
         probe.append((name, start, end, work))
     else:
-        # The handle alone: building a torch.cuda.Stream object costs more than most launches.
-        rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+        rc = getattr(lib, name)(*args, current_stream())
     counters["launches"] += KERNELS_PER_CALL.get(name, 1) if kernels is None else kernels
     check(name, rc)
 

@@ -36,7 +36,7 @@ _MOST = 1 << 31  # rows, and columns, of layer norm and dropout-add
 
 def _launch(t: torch.Tensor, name: str, *args, kernels: int = 1) -> None:
     """Calls an entry point, which launches ``kernels`` kernels, on the current stream of ``t``'s device."""
-    if torch._C._cuda_getDevice() == t.get_device():
+    if _lib.current_device() == t.get_device():
         _lib.call(name, *args, kernels=kernels)
     else:
         with torch.cuda.device(t.get_device()):
