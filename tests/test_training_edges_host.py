@@ -204,3 +204,19 @@ def test_philox_against_all_published_vectors():
         want = philox([block & ones, block >> 32, offset & ones, (offset >> 32) & ones],
                       [seed & ones, (seed >> 32) & ones])
         assert [int(w) for w in philox_words(seed, offset, 4 * block, 4)] == want
+
+
+def test_lazily_negated_views_are_refused(monkeypatch):
+    """``z.conj().imag`` shares z's memory with a sign that only torch's own operators apply."""
+    monkeypatch.setattr(training, "_check_cuda", lambda *a: None)
+    monkeypatch.setattr(training, "_launch", lambda *a, **kw: pytest.fail("launched"))
+    x = torch.randn(4, 8, dtype=torch.complex64).conj().imag
+    assert x.is_neg()
+    q, plain, rng = x.view(1, 4, 1, 8), torch.zeros(4, 8), torch.zeros(2, dtype=torch.int64)
+    for call in (lambda: training.layer_norm(x), lambda: training.layer_norm_backward(x, plain, torch.zeros(4, 2)),
+                 lambda: training.attention(q, q, q), lambda: training.dropout_add(plain, 0.1, rng, x),
+                 lambda: training.dropout_add(plain, 0.1, rng, None, x[0]),
+                 lambda: training.dropout_add_backward(x, plain, 0.1, rng)):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+    torch.testing.assert_close(x.resolve_neg(), x)

@@ -54,6 +54,8 @@ def _check_tensor(name: str, t, like: torch.Tensor | None = None) -> None:
         raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.is_neg():  # the memory holds the other sign
+        raise ValueError(f"{name} is a lazily negated view: give {name}.resolve_neg()")
     if like is not None and t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, expected {like.device}")
 
