@@ -569,8 +569,9 @@ enum UnblendDtype { UNBLEND_F32 = 0, UNBLEND_BF16 = 1, UNBLEND_F16 = 2 };
 
 /*
  * y = (x - mean) * rstd * gamma + beta over rows of `cols` elements, stats[row] = (mean, rstd) (float2, on an
- * 8-byte boundary) for the backward pass. Row (o, i) of x starts at x + o * x_so + i * x_si, i < inner, o < outer (fewer than 2^31 rows); y is
- * contiguous. gamma / beta may be NULL; their type w_dtype is fp32 or x's (the gradients' too).
+ * 8-byte boundary) for the backward pass. Row (o, i) of x starts at x + o * x_so + i * x_si, i < inner, o < outer
+ * (fewer than 2^31 rows); y is contiguous. gamma / beta may be NULL; their type w_dtype is fp32 or x's (the gradients'
+ * too).
  */
 int unblend_layer_norm_forward(const void* x, long long x_so, long long x_si, void* y, float* stats,
                                const void* gamma, const void* beta, float eps, long long outer, long long inner,

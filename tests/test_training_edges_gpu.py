@@ -163,7 +163,8 @@ def _fp16_gradients(q, k, v, dout, **kw):
 
 @pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4])
 @pytest.mark.parametrize("lq,lk,h,hk,hd,causal", [
-    (512, 1344, 1, 1, 64, False), (512, 8192, 1, 1, 64, False), (700, 2000, 2, 1, 128, True), (300, 60, 2, 1, 64, False),
+    (512, 1344, 1, 1, 64, False), (512, 8192, 1, 1, 64, False), (700, 2000, 2, 1, 128, True),
+    (300, 60, 2, 1, 64, False),
     (50, 700, 2, 2, 64, False), (62, 62, 2, 2, 64, False), (64, 50, 4, 2, 48, True), (30, 31, 2, 2, 64, False),
     (60, 60, 2, 2, 128, False), (20, 30, 4, 1, 40, True)])
 def test_fp16_gradients_of_small_losses(lq, lk, h, hk, hd, causal, size):

@@ -67,8 +67,9 @@ def test_workspace_is_what_the_parts_take():
     assert _attention_workspace(outer=4, lq=1, lk=8191, heads=16, kv_heads=4, hd=128) == 32 * 64 * 129 * 4
     for dtype in (_lib.DTYPE_F32, _lib.DTYPE_BF16, _lib.DTYPE_F16):
         size = 4 if dtype == _lib.DTYPE_F32 else 2
-        for outer, heads, kv, lq, lk, hd in ((1, 8, 8, 300, 5000, 64), (2, 16, 4, 40, 4097, 128), (1, 1, 1, 17, 9000, 40),
-                                             (3, 4, 2, 129, 700, 96), (1, 2, 2, 8, 100000, 64), (7, 8, 1, 2, 3000, 72),
+        for outer, heads, kv, lq, lk, hd in ((1, 8, 8, 300, 5000, 64), (2, 16, 4, 40, 4097, 128),
+                                             (1, 1, 1, 17, 9000, 40), (3, 4, 2, 129, 700, 96), (1, 2, 2, 8, 100000, 64),
+                                             (7, 8, 1, 2, 3000, 72),
                                              (1, 4, 4, 5000, 130, 64), (1, 1, 1, 1, 1, 1)):
             few = heads // kv * lq <= (8 if size == 4 else 16) and hd * size % 16 == 0
             tiles = outer * heads * -(-lq // 64)

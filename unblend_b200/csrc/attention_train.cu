@@ -12,10 +12,10 @@
 //
 // The kernels here take every type, stride and alignment, and are the path of fp32: 64 x 64 score tiles on 256
 // threads, 4 x 4 scores per thread, operands in shared memory as fp32 (transposed where the head axis is summed). Bound
-// by the shared-memory reads that feed the FP32 pipes (78 % of their rate in the forward kernel): 8 x 1344 x 1344, 8
-// heads of 64, fp32 1.09 ms forward (27 TFLOP/s) and 3.32 ms backward (31 TFLOP/s). 4 x 8 scores on 128 threads halve
-// the reads, but with as few warps were only faster forward at head dim 64 (0.97 ms; backward 3.58 ms, at head dim 128
-// 2.62 and 9.17 ms against 2.17 and 7.50 ms).
+// by the shared-memory reads that feed the FP32 pipes (89 % of their rate in the forward kernel, FMA 45 %): 8 x 1344 x
+// 1344, 8 heads of 64, fp32 1.09 ms forward (27 TFLOP/s) and 3.32 ms backward (31 TFLOP/s). 4 x 8 scores on 128
+// threads halve the reads, but with as few warps were only faster forward at head dim 64 (0.97 ms; backward 3.58 ms,
+// at head dim 128 2.62 and 9.17 ms against 2.17 and 7.50 ms).
 #include "attention_train.cuh"
 #include "warp_mma.cuh"
 

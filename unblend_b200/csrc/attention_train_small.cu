@@ -7,8 +7,9 @@
 //
 // One kernel makes the three gradients, where the kernels for long rows need one for the statistics, one for dq and one
 // for dk and dv, and read the inputs in each. D = rowsum(P * dP) in fp32 is better than from the rounded O (bf16, 6
-// queries over 16 keys: gradients off by 0.0024 instead of 0.0029 relative) and needs no O, but holds only when lse and O
-// are of these keys alone, which the caller says with all_keys: whoever joins several blocks of keys gives those of all.
+// queries over 16 keys: gradients off by 0.0024 instead of 0.0029 relative) and needs no O, but holds only when lse
+// and O are of these keys alone, which the caller says with all_keys: whoever joins several blocks of keys gives those
+// of all.
 //
 // Bound: HBM. A sequence and head gives 5 products of 64 x 64 x head dim for 8 tensors of 64 rows, far below what the
 // tensor cores need per byte, so mma.sync is enough (m16n8k16, fp32 accumulators); tcgen05's 128 rows would be half
@@ -37,10 +38,10 @@ constexpr int fwd_smem(int hd, int r) { return 3 * r * hd * 2; }
 constexpr int bwd_smem(int hd, int r, bool grouped) { return ((grouped ? 5 : 4) * r * hd + 2 * r * P_COLS) * 2; }
 
 // CTAs per SM, which is what hides latency. 801 x 62 x 62, 8 heads of 64, bf16: forward 39 us (5.2 TB/s) with 7 CTAs of
-// 72 registers, 43 us with 5 of 96 and with 8 of 64 (spills); backward 80 us (5.1 TB/s) with 4 of 128 (5 of 96, with dS
-// in V's place, were 1 us slower). Head dim 128: 70 and 171 us. Earlier versions of 48 and 85 us were slower with two
-// warps of 32 rows each, which load half the fragments (51 and 101 us), and with the products of 16-key blocks behind
-// the sequence left out (56 and 95 us: the branches kept loads and products from overlapping).
+// 72 registers, 43 us with 5 of 96 and with 8 of 64 (spills); backward 83 us (4.9 TB/s; fp16 87 us) with 4 of 128 (5
+// of 96, with dS in V's place, were 1 us slower). Head dim 128: 70 and 171 us. Earlier versions of 48 and 85 us were
+// slower with two warps of 32 rows each, which load half the fragments (51 and 101 us), and with the products of
+// 16-key blocks behind the sequence left out (56 and 95 us: the branches kept loads and products from overlapping).
 constexpr int fwd_ctas(int hd, int r) { return hd == 64 ? 7 * 64 / r : 4; }
 constexpr int bwd_ctas(int hd, int r, bool grouped) { return hd == 64 ? (grouped ? 3 : 4) * 64 / r : 2; }
 
@@ -462,8 +463,8 @@ int launch_bwd(const AttnArgs& a, cudaStream_t st) {
   return 0;
 }
 
-// Tiles of 32 rows take a quarter of the products: 801 x 32 x 32, 8 heads of 64, bf16 19 us forward (5.6 TB/s) and 38 us
-// backward (4.9 TB/s); 801 x 17 x 17 17 and 33 us, with tiles of 64 rows 33 and 74 us.
+// Tiles of 32 rows take a quarter of the products: 801 x 32 x 32, 8 heads of 64, bf16 19 us forward (5.6 TB/s) and 38
+// us backward (4.9 TB/s); 801 x 17 x 17 17 and 33 us, with tiles of 64 rows 33 and 74 us.
 bool half_tiles(const AttnArgs& a) { return a.lq <= 32 && a.lk <= 32; }
 
 template <typename T>

@@ -13,12 +13,12 @@
 // P and dS are rounded to the inputs' type, as the tensor cores take both operands in one 16-bit type; softmax, its
 // statistics and all sums are fp32. 2^x is the hardware approximation (2 ulp). Backward, fp16 keeps P times 2^12 and dS
 // times a power of two that its bound |dS| <= |dO_i| |V_j| + |D_i| (norms of the rows) gives: for dQ one per query, for
-// dK, which is summed over queries, one per sequence and key/value head. Both cost nothing in the loops: dQ's is added to
-// the exponent of P, dK's to the factor that takes P's 2^12 back.
+// dK, which is summed over queries, one per sequence and key/value head. Both cost nothing in the loops: dQ's is added
+// to the exponent of P, dK's to the factor that takes P's 2^12 back.
 //
 // A thread owns a row (or half a row), so row maxima and sums need no shuffles. One warp issues TMA, one the MMAs;
-// every barrier wait gives up after two seconds and sets the error flag. A warp gives up as a whole (its lanes vote), as
-// the instructions behind a wait need all of them, and a CTA leaves only when what it started is done: the TMA warp
+// every barrier wait gives up after two seconds and sets the error flag. A warp gives up as a whole (its lanes vote),
+// as the instructions behind a wait need all of them, and a CTA leaves only when what it started is done: the TMA warp
 // waits until its last copies have been used, or, after a wait that ran out, until they have landed; a MMA warp that
 // gives up waits for the products that it issued.
 #include <cuda_bf16.h>
@@ -41,10 +41,10 @@ constexpr float RESCALE_THRESHOLD = 8.f;   // log2 units by which the maximum ma
 // 2^x of a pair on the FMA pipe, for a share of the exponentials (the special function unit takes 16 per cycle and SM,
 // the tightest limit at head dim 64). x = n + f with n the nearest integer, read off the low bits of x + 1.5 2^23; 2^f
 // by a polynomial of degree 5 on [-1/2, 1/2] fitted for the least relative error (2.1e-7 in fp32, half the hardware
-// approximation's two ulp); n goes into the exponent. x below -127 counts as -127, where the exponent field comes out as
-// 0 and 2^f as 1 + 2^-23: 2^-149, which the 16-bit types round to 0 (a masked key must not keep even 2^-126, which a
-// value near bf16's largest would carry into the sum). Between -127 and -126 the result is off by up to 2^-126. f * 0
-// carries NaN into the result.
+// approximation's two ulp); n goes into the exponent. x below -127 counts as -127, where the exponent field comes out
+// as 0 and 2^f as 1 + 2^-23: 2^-149, which the 16-bit types round to 0 (a masked key must not keep even 2^-126, which
+// a value near bf16's largest would carry into the sum). Between -127 and -126 the result is off by up to 2^-126. f *
+// 0 carries NaN into the result.
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
@@ -310,9 +310,10 @@ constexpr int SHORT_ROWS = 64;
 //
 // A CTA holds NQ tiles of 128 queries of one head (NQ = 2 shares each K / V tile between 256 queries), each with its
 // own softmax warpgroup; while one warpgroup takes exponentials, the tensor cores work for the other. With NQ = 1 that
-// is another CTA's. Bound by the warpgroups' exponentials and conversions between the two products: 62 x 801 x 801, 8
-// heads of 64 173 us (471 TFLOP/s of visible pairs), causal 8192, 16 over 4 heads of 128 246 us (1118 TFLOP/s). Making
-// the next scores ahead, with P beside S in TMEM, gained 1 to 2 % at head dim 64 and is left out.
+// is another CTA's. Bound by the chain from one product to the next, through TMEM, the exponentials (49 % of the
+// special function rate) and TMEM again; tensor cores 28 % busy, issue slots 43 %: 62 x 801 x 801, 8 heads of 64 173
+// us (471 TFLOP/s of visible pairs), causal 8192, 16 over 4 heads of 128 249 us (1104 TFLOP/s). Making the next scores
+// ahead, with P beside S in TMEM, gained 1 to 2 % at head dim 64 and is left out.
 
 template <int HD, int NQ, bool SHORT>
 struct FwdCfg {
@@ -662,11 +663,12 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
 
 // ---------------------------------------------------------------------------------------- row statistics
 //
-// (-lse log2 e, -D) of each query row, D = rowsum(dO * O); (-inf, 0) for rows that see nothing. LANES lanes per row, 8
-// values each; rows in memory order (heads fastest) for whole lines; all loads of a thread's STATS_ROWS rows are issued
-// before the first is used. A kernel of its own: inside the dq kernel the loads stood in front of every unit's first
-// tile (5000 of 24000 cycles for 11 tiles). Bound: HBM, one read of dO and O; 62 x 801, 8 heads of 64 22 us (4.6 TB/s;
-// one row per thread and hardware divisions 31 us).
+// (-lse log2 e, -D) of each query row, D = rowsum(dO * O) (from O as the caller keeps it, in the inputs' type: half a
+// step of its values, next to the like rounding of dS); (-inf, 0) for rows that see nothing. LANES lanes per
+// row, 8 values each; rows in memory order (heads fastest) for whole lines; all loads of a thread's STATS_ROWS rows
+// are issued before the first is used. A kernel of its own: inside the dq kernel the loads stood in front of every
+// unit's first tile (5000 of 24000 cycles for 11 tiles). Bound: HBM, one read of dO and O; 62 x 801, 8 heads of 64 22
+// us (4.6 TB/s; one row per thread and hardware divisions 31 us).
 constexpr int STATS_ROWS = 4;
 
 template <typename T, int LANES>
@@ -826,8 +828,8 @@ __global__ void __launch_bounds__(256) attention_stats_range_kernel(const __grid
 // 128 queries of one head per unit, keys streamed 128 at a time; two threads per row, 64 keys each. S is double
 // buffered and dP is read into registers first, so the tensor cores make S and dP of the next tile while this one's
 // exponentials are taken. dS of 32 keys takes 16 of the 32 columns that their scores came from. Bound as the forward
-// pass, with one more product to read and one CTA per SM: 62 x 801 x 801, 8 heads of 64 216 us (566 TFLOP/s of visible
-// pairs), causal 8192, 16 over 4 heads of 128 390 us (1057 TFLOP/s).
+// pass, with one more product to read and one CTA per SM: 62 x 801 x 801, 8 heads of 64 222 us (550 TFLOP/s of visible
+// pairs), causal 8192, 16 over 4 heads of 128 410 us (1005 TFLOP/s).
 
 template <int HD, bool SHORT>
 struct DqCfg {
@@ -1219,7 +1221,7 @@ __global__ void __launch_bounds__(DqCfg<HD, SHORT>::THREADS, 1)
 // head dims over 64, where the two accumulators take half of TMEM). Two threads per key, half of the tile's queries
 // each. lse and D go by column here: a warp brings them to shared memory, and rows that must not count come with
 // -lse = -inf, P = 0. P^T and dS^T of a thread share the columns of its scores. 62 x 801 x 801, 8 heads of 64:
-// 274 us (595 TFLOP/s of visible pairs), causal 8192, 16 over 4 heads of 128 520 us (1057 TFLOP/s).
+// 273 us (597 TFLOP/s of visible pairs), causal 8192, 16 over 4 heads of 128 551 us (998 TFLOP/s).
 
 template <int HD, bool SHORT>
 struct DkvCfg {

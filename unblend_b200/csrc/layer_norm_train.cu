@@ -6,7 +6,8 @@
 //   dgamma = sum_rows dy * xhat,  dbeta = sum_rows dy
 //
 // Statistics, sums and all arithmetic are fp32; x, y, dy and dx are fp32, bf16 or fp16.
-// Both directions are bound by HBM: one read of each input and one write of each output.
+// Floor of both directions: one read of each input and one write of each output. The forward pass of wide 16-bit rows
+// stops at the L1 path before HBM (78 and 39 % of their rates at 65536 x 1024 bf16): each row reads the weights again.
 //
 // A row of up to 1024 columns belongs to one warp (no barrier), a wider one up to 8192 to a CTA, 16 values per thread;
 // wider rows are read again for every reduction. Rows come through shared memory by cp.async, several in flight per

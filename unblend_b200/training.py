@@ -11,6 +11,10 @@ wrong arguments raise ``ValueError`` before anything is launched, and there is n
 sums are fp32 whatever the type. No result depends on scheduling: two calls on the same inputs agree bit for bit.
 Memory is allocated by torch for each call, so calls on several streams and captured graphs share nothing.
 
+The attention kernels on the tensor cores wait for one another's steps with a limit of two seconds. A wait that runs out
+leaves the outputs unfinished and sets a flag on the device, which no call reads (that would wait for the GPU): read
+``_lib.error_flag()`` where a step is checked anyway; it is 0 unless something is wrong.
+
 CUDA graphs: capture the plain calls. The differentiable functions refuse to record or run a backward pass while a
 stream is being captured: autograd's gradient accumulation of leaves that an earlier eager pass still holds runs on
 that pass's stream, which breaks the capture. Second derivatives and forward-mode derivatives are refused too.
@@ -208,7 +212,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, 
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"dy must be {x.dtype} of shape {tuple(x.shape)}, got {dy.dtype} {tuple(dy.shape)}")
     n, cols = x.numel() // x.shape[-1], x.shape[-1]
-    if not isinstance(stats, torch.Tensor) or stats.shape != (n, 2) or stats.dtype != torch.float32 or stats.device != x.device:
+    if not isinstance(stats, torch.Tensor) or stats.shape != (n, 2) or stats.dtype != torch.float32 or \
+            stats.device != x.device:
         raise ValueError("stats must be the second result of layer_norm_forward for this x")
     _check_cuda("x", x)
     dx = _empty(x)
@@ -342,7 +347,10 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     q is ``[batch, lq, heads, head_dim]`` or, for axial sequences, ``[outer, inner, lq, heads, head_dim]``; k and v
     likewise with lk and their own number of heads, which divides q's (head h of q reads head ``h // (heads //
     kv_heads)``). Any strides with a unit last one are taken as they are: slices of one packed projection, transposed
-    token axes. ``scale`` defaults to ``head_dim ** -0.5``; head_dim is at most 128.
+    token axes. ``scale`` defaults to ``head_dim ** -0.5``; head_dim is at most 128. 16-bit calls run on the tensor cores
+    when head_dim is a multiple of 8, ``scale`` positive, and every tensor starts, and strides along each axis of more
+    than one, by a positive multiple of 16 bytes; others (keys expanded over heads: give the shared head itself) run on
+    the CUDA cores, many times slower.
 
     ``q_lens`` / ``k_lens`` (int32, one per sequence) are the sequences' lengths in a padded batch; rows behind them
     are not used, whatever they hold. With ``causal``, query i sees keys ``j <= i + k_len - q_len``. Queries that see
