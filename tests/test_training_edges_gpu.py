@@ -275,3 +275,25 @@ def test_calls_run_on_the_current_stream_without_torchs_private_handle(monkeypat
                 got = training.layer_norm_forward(y)[0]
             stream.synchronize()
             assert torch.equal(got, want)
+
+
+def test_gradients_that_arrive_as_lazily_negated_views():
+    """The gradient of the imaginary part of a conjugated number is a view with its sign beside it: it counts."""
+    rng = torch.tensor([5, 6], device="cuda")
+    x, w, q = _rand(6, 40, 64, seed=1), _rand(64, seed=2), _rand(2, 30, 4, 64, seed=3)
+    weight = torch.complex(_rand(6, 40, 64, seed=4), _rand(6, 40, 64, seed=5))
+    qw = torch.complex(_rand(2, 30, 4, 64, seed=6), _rand(2, 30, 4, 64, seed=7))
+    calls = ((lambda a: training.layer_norm(a, w), x, weight), (lambda a: training.attention(a, a, a), q, qw),
+             (lambda a: training.dropout_add(a, 0.2, rng, a, w), x, weight),
+             (lambda a: training.dropout_add(a, 0.2, rng), x, weight))
+    for call, inp, wt in calls:
+        grads = []
+        for lazy in (True, False):
+            leaf = inp.clone().requires_grad_()
+            y = call(leaf)
+            if lazy:  # |(0 + i y)* - wt|^2 / 2 without the square of y: Re(wt * conj(i y)) = Im(wt) y
+                (torch.complex(torch.zeros_like(y), y).conj() * wt).real.sum().backward()
+            else:
+                (y * wt.imag).sum().backward()
+            grads.append(leaf.grad)
+        assert torch.equal(grads[0], grads[1])

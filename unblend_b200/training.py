@@ -251,7 +251,7 @@ class _LayerNorm(torch.autograd.Function):
         _refuse_capture("layer_norm")
         x, gamma, stats = ctx.saved_tensors
         need_w = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dx, dgamma, dbeta = layer_norm_backward(dy, x, stats, gamma, need_w)
+        dx, dgamma, dbeta = layer_norm_backward(dy.resolve_neg(), x, stats, gamma, need_w)
         if not ctx.needs_input_grad[1]:
             dgamma = None
         dbeta = dbeta.to(ctx.beta_dtype) if ctx.needs_input_grad[2] else None
@@ -431,7 +431,7 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, dout):
         _refuse_capture("attention")
         q, k, v, out, lse, q_lens, k_lens = ctx.saved_tensors
-        dq, dk, dv = attention_backward(dout, q, k, v, out, lse, ctx.scale, ctx.causal, q_lens, k_lens,
+        dq, dk, dv = attention_backward(dout.resolve_neg(), q, k, v, out, lse, ctx.scale, ctx.causal, q_lens, k_lens,
                                         all_keys=True)
         need = ctx.needs_input_grad
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
@@ -552,7 +552,7 @@ class _DropoutAdd(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dscale = None
         if need[0] or need[4]:
-            dx, dscale = _dropout_backward(dy, x, ctx.dtype, ctx.p, rng, scale, need[4])
+            dx, dscale = _dropout_backward(dy.resolve_neg(), x, ctx.dtype, ctx.p, rng, scale, need[4])
         return dx if need[0] else None, None, None, dy if ctx.residual and need[3] else None, dscale
 
 
