@@ -664,11 +664,11 @@ __global__ void __launch_bounds__(FwdCfg<HD, NQ, SHORT>::THREADS, FwdCfg<HD, NQ,
 // ---------------------------------------------------------------------------------------- row statistics
 //
 // (-lse log2 e, -D) of each query row, D = rowsum(dO * O) (from O as the caller keeps it, in the inputs' type: half a
-// step of its values, next to the like rounding of dS); (-inf, 0) for rows that see nothing. LANES lanes per
-// row, 8 values each; rows in memory order (heads fastest) for whole lines; all loads of a thread's STATS_ROWS rows
-// are issued before the first is used. A kernel of its own: inside the dq kernel the loads stood in front of every
-// unit's first tile (5000 of 24000 cycles for 11 tiles). Bound: HBM, one read of dO and O; 62 x 801, 8 heads of 64 22
-// us (4.6 TB/s; one row per thread and hardware divisions 31 us).
+// step of its values, next to the like rounding of dS); (-inf, 0) for rows that see nothing. LANES lanes per row, 8
+// values each; rows in memory order (heads fastest) for whole lines; all loads of a thread's STATS_ROWS rows are issued
+// before the first is used. A kernel of its own: inside the dq kernel the loads stood in front of every unit's first
+// tile (5000 of 24000 cycles for 11 tiles). Bound: HBM, one read of dO and O; 62 x 801, 8 heads of 64 22 us (4.6 TB/s;
+// one row per thread and hardware divisions 31 us).
 constexpr int STATS_ROWS = 4;
 
 template <typename T, int LANES>
@@ -1768,8 +1768,8 @@ int launch_stats_lanes(const AttnArgs& a, cudaStream_t st) {
     ra.by_v_chunks = fast_div(ra.v_chunks);
     ra.by_group = fast_div(a.group);
     ra.by_inner = fast_div(a.inner);
-    const cudaError_t e = cudaMemsetAsync(a.range, 0, sizeof(unsigned) * 4 * a.seqs * a.kv_heads, st);
-    if (e != cudaSuccess) return (int)e;
+    if (cudaMemsetAsync(a.range, 0, sizeof(unsigned) * 4 * a.seqs * a.kv_heads, st) != cudaSuccess)
+      return (int)cudaGetLastError();
     attention_stats_range_kernel<T, LANES><<<ra.units / 8 + (ra.units % 8 != 0), 256, 0, st>>>(a, stats, ra);
   } else {
     constexpr int PER_CTA = STATS_ROWS * 256 / LANES;
