@@ -607,6 +607,54 @@ int unblend_dropout_add_backward(const void* dy, long long dy_so, long long dy_s
 int unblend_dropout_add_grad_workspace(long long rows, int cols, long long* bytes);
 
 /*
+ * Rotary positions of queries and keys, alone or behind an RMS norm of each head, with gradients. Tensors are addressed
+ * as in attention below; outputs are contiguous [outer, inner, length, heads, hd]. Pair i < pairs of a head's dims is
+ * (2i, 2i + 1), or (i, i + pairs) with half; at position p it turns by p * freqs[i] and is multiplied by scale:
+ *
+ *   (a, b) -> scale * (a cos - b sin, a sin + b cos)
+ *
+ * Dims from 2 pairs on stay. Angles are reduced in double precision: integer positions below 2^53 lose nothing.
+ */
+typedef struct {
+  long long outer, inner, row, head;
+} UnblendHeadStrides;
+
+typedef struct {
+  int dtype; /* UnblendDtype of q, k and their gradients */
+  int outer, inner, length, heads, k_heads; /* k_heads 0: no k */
+  int hd, pairs, half; /* hd <= 256, 2 pairs <= hd */
+  float scale;
+  const void* freqs; /* [pairs], double with freqs_f64, else float; may be NULL without pairs */
+  int freqs_f64;
+  int positions_i64;
+  const void* positions; /* [length] per sequence, 64-bit integers with positions_i64, else 32; NULL: 0, 1, ... */
+  long long positions_stride; /* from sequence to sequence; 0: the same for all */
+  UnblendHeadStrides q, k; /* inputs, or the gradients that come in */
+  /* the norm only: */
+  UnblendHeadStrides q0, k0; /* backward: the forward's inputs */
+  const void* gamma_q; /* [hd], may be NULL */
+  const void* gamma_k;
+  int w_dtype; /* of the weights and their gradients: fp32 or dtype */
+  float eps;
+  const int* lens; /* [outer * inner] lengths in a padded batch, may be NULL: rows behind them are not read, and 0 */
+} UnblendRotaryParams;
+
+/* The rotation, or with inverse its transpose (the gradients' way back, which needs no other input). */
+int unblend_rotary(const void* q, const void* k, void* q_out, void* k_out, const UnblendRotaryParams* p, int inverse,
+                   void* stream);
+
+/* y = rot(x * (mean(x^2) + eps)^-1/2 * gamma), the mean over a head's dims. */
+int unblend_qk_norm_rotary_forward(const void* q, const void* k, void* q_out, void* k_out,
+                                   const UnblendRotaryParams* p, void* stream);
+
+/* Gradients of the forward's inputs q, k from dq, dk of its outputs, and dgamma_q, dgamma_k [hd] (both or neither). work:
+ * unblend_qk_norm_rotary_grad_workspace bytes, not needed without them. */
+int unblend_qk_norm_rotary_backward(const void* dq, const void* dk, const void* q, const void* k, void* dq_out,
+                                    void* dk_out, void* dgamma_q, void* dgamma_k, float* work,
+                                    const UnblendRotaryParams* p, void* stream);
+int unblend_qk_norm_rotary_grad_workspace(const UnblendRotaryParams* p, long long* bytes);
+
+/*
  * Multi-head attention with gradients. Sequence (o, i), row r, head h, dim d of a tensor is at
  * base + o * outer + i * inner + r * row + h * head + d (strides in elements). Query head h reads key/value head
  * h / (heads / kv_heads).
@@ -620,10 +668,6 @@ int unblend_dropout_add_grad_workspace(long long rows, int cols, long long* byte
  * gradient; rows of dk and dv behind k_len are 0. What lies in rows behind the lengths, NaN included, is not used;
  * NaN or infinities within them may reach any output of their sequence.
  */
-typedef struct {
-  long long outer, inner, row, head;
-} UnblendHeadStrides;
-
 typedef struct {
   int dtype; /* UnblendDtype of q, k, v, out, dout, dq, dk, dv */
   int outer, inner, heads, kv_heads, lq, lk, hd; /* hd <= 128 */

@@ -101,6 +101,19 @@ class AttnTrainParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    """Mirror of ``UnblendRotaryParams``."""
+
+    _fields_ = [
+        ("dtype", c_int), ("outer", c_int), ("inner", c_int), ("length", c_int), ("heads", c_int), ("k_heads", c_int),
+        ("hd", c_int), ("pairs", c_int), ("half", c_int), ("scale", c_float),
+        ("freqs", c_void_p), ("freqs_f64", c_int), ("positions_i64", c_int),
+        ("positions", c_void_p), ("positions_stride", c_ll),
+        ("q", HeadStrides), ("k", HeadStrides), ("q0", HeadStrides), ("k0", HeadStrides),
+        ("gamma_q", c_void_p), ("gamma_k", c_void_p), ("w_dtype", c_int), ("eps", c_float), ("lens", c_void_p),
+    ]
+
+
 # name -> argtypes (all return int)
 _SIGNATURES = {
     "unblend_conv2d_f32": [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(ConvParams), c_void_p],
@@ -184,6 +197,10 @@ _SIGNATURES = {
                                   ctypes.POINTER(AttnTrainParams), c_void_p],
     "unblend_attention_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_ll, ctypes.POINTER(AttnTrainParams), c_void_p],
+    "unblend_rotary": [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(RotaryParams), c_int, c_void_p],
+    "unblend_qk_norm_rotary_forward": [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(RotaryParams), c_void_p],
+    "unblend_qk_norm_rotary_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, ctypes.POINTER(RotaryParams), c_void_p],
 }
 
 # Entry points without a stream argument.
@@ -196,6 +213,7 @@ _HOST_SIGNATURES = {
     "unblend_attention_train_error_flag": [ctypes.POINTER(c_int), c_int],
     "unblend_layer_norm_grad_workspace": [c_ll, c_int, ctypes.POINTER(c_ll)],
     "unblend_dropout_add_grad_workspace": [c_ll, c_int, ctypes.POINTER(c_ll)],
+    "unblend_qk_norm_rotary_grad_workspace": [ctypes.POINTER(RotaryParams), ctypes.POINTER(c_ll)],
     "unblend_attention_workspace": [ctypes.POINTER(AttnTrainParams), c_int, ctypes.POINTER(c_ll)],
 }
 

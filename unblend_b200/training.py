@@ -1,9 +1,10 @@
 """Transformer operators with gradients, for fine-tuning the separation models.
 
-Three operators of the models' pre-norm block ``x + LayerScale * dropout(attention(layer_norm(x)))``
-(unblend/transformer.py:290-301, 328-359; unblend/roformer.py:478-511), each as
+Operators of the models' pre-norm block ``x + LayerScale * dropout(attention(layer_norm(x)))``
+(unblend/transformer.py:290-301, 328-359; unblend/roformer.py:478-511), with rotary positions and a norm of queries and
+keys in front of the attention, each as
 
-* a differentiable function (``layer_norm``, ``attention``, ``dropout_add``), and
+* a differentiable function (``layer_norm``, ``rotary``, ``qk_norm_rotary``, ``attention``, ``dropout_add``), and
 * its two passes as plain calls (``*_forward``, ``*_backward``) for callers that keep the saved tensors themselves.
 
 All take CUDA tensors in fp32, bf16 or fp16 and run hand-written kernels on the current stream of the tensors' device;
@@ -33,6 +34,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 MAX_HEAD_DIM = 128
+MAX_ROTARY_DIM = 256
 _F32_MAX = torch.finfo(torch.float32).max
 _REGISTER_COLS = 8192  # widest rows whose layer norm sums the weights' gradients beside the input's
 _MOST = 1 << 31  # rows, and columns, of layer norm and dropout-add
@@ -446,6 +448,335 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
         _refuse_capture("attention")
         return _Attention.apply(q, k, v, scale, causal, q_lens, k_lens)
     return attention_forward(q, k, v, scale, causal, q_lens, k_lens)[0]
+
+
+# --------------------------------------------------------------------------------------------- rotary
+
+
+def rotary_freqs(dims: int, base: float = 10000.0, factor: float = 1.0, method: str = "linear",
+                 trained_length: int | None = None, slow: float = 1.0, fast: float = 32.0,
+                 device: torch.device | str | None = None) -> torch.Tensor:
+    """Frequencies of ``dims // 2`` pairs, ``base ** (-2 i / dims)`` radians per position, as float64 ``[dims // 2]``.
+
+    ``factor`` > 1 stretches them for contexts that many times longer than the trained ones:
+
+    * ``"linear"``: all frequencies divided by the factor (position interpolation, Chen et al. 2023);
+    * ``"base"``: the base times ``factor ** (dims / (dims - 2))``, which divides the slowest frequency by the factor and
+      keeps the fastest (dims above 2);
+    * ``"parts"``: pairs that turn ``fast`` times or more within ``trained_length`` are kept, those of ``slow`` turns or
+      fewer are divided by the factor, and the ones between are mixed linearly in their turns (Peng et al. 2023, who also
+      multiply the rotated values by ``0.1 ln(factor) + 1``: the ``scale`` of ``rotary``).
+    """
+    if not isinstance(dims, int) or dims < 2 or dims % 2:
+        raise ValueError(f"dims must be even and positive, got {dims!r}")
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError(f"base must be positive, got {base!r}")
+    if not (factor >= 1 and math.isfinite(factor)):
+        raise ValueError(f"factor must be 1 or more, got {factor!r}")
+    exponent = torch.arange(0, dims, 2, dtype=torch.float64) / dims
+    if method == "linear":
+        f = base ** -exponent / factor
+    elif method == "base":
+        if dims == 2 and factor != 1:
+            raise ValueError("a single pair has no slower frequency to keep the fastest beside: use another method")
+        f = (base * factor ** (dims / max(dims - 2, 1))) ** -exponent
+    elif method == "parts":
+        if not (isinstance(trained_length, int) and trained_length > 0):
+            raise ValueError(f"trained_length must be a positive integer for this method, got {trained_length!r}")
+        if not 0 <= slow < fast:
+            raise ValueError(f"slow and fast must be turns with 0 <= slow < fast, got {slow!r} and {fast!r}")
+        f = base ** -exponent
+        keep = ((trained_length * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+    else:
+        raise ValueError(f"method must be 'linear', 'base' or 'parts', got {method!r}")
+    return f.to(device) if device is not None else f
+
+
+def _check_rotary(q, k, freqs, positions, scale, eps: float = 0.0) -> float:
+    _check_heads("q", q)
+    if k is not None:
+        _check_heads("k", k, q)
+        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree but for their heads")
+    hd = q.shape[-1]
+    if not 1 <= hd <= MAX_ROTARY_DIM:
+        raise ValueError(f"head_dim must be 1 to {MAX_ROTARY_DIM}, got {hd}")
+    if freqs is not None:
+        if not isinstance(freqs, torch.Tensor) or freqs.dtype not in (torch.float32, torch.float64) or \
+                freqs.dim() != 1 or freqs.device != q.device:
+            raise ValueError(f"freqs must be a float32 or float64 tensor [pairs] on {q.device}")
+        if 2 * freqs.shape[0] > hd:
+            raise ValueError(f"{freqs.shape[0]} pairs do not fit into head_dim {hd}")
+        if freqs.is_neg():
+            raise ValueError("freqs is a lazily negated view: give freqs.resolve_neg()")
+        if freqs.requires_grad and torch.is_grad_enabled():
+            raise ValueError("freqs has no gradient here: give freqs.detach()")
+    if positions is not None:
+        if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64) or \
+                positions.device != q.device:
+            raise ValueError(f"positions must be an int32 or int64 tensor on {q.device}")
+        if positions.shape not in (q.shape[:-2], q.shape[-3:-2]):
+            raise ValueError(f"positions must have shape {tuple(q.shape[-3:-2])} or {tuple(q.shape[:-2])}, got "
+                             f"{tuple(positions.shape)}")
+    if not (isinstance(eps, (int, float)) and 0 <= eps <= _F32_MAX):
+        raise ValueError(f"eps must be >= 0, got {eps!r}")
+    scale = float(scale)
+    if not abs(scale) <= _F32_MAX:
+        raise ValueError(f"scale must be finite in float32, got {scale}")
+    if q.numel() // hd >= _MOST or (k is not None and k.numel() // hd >= _MOST):
+        raise ValueError(f"q and k must have fewer than 2^31 rows each, got shapes {tuple(q.shape)}"
+                         + (f" and {tuple(k.shape)}" if k is not None else ""))
+    return scale
+
+
+def _rotary_params(q, k, freqs, positions, interleaved: bool, scale: float):
+    """The call's parameters, and the tensors that they point to."""
+    s = q.shape
+    seqs = _seqs(q)
+    freqs = None if freqs is None else freqs.contiguous()
+    per_seq = positions is not None and positions.dim() > 1
+    positions = None if positions is None else positions.contiguous()
+    p = _lib.RotaryParams(_DTYPES[q.dtype], s[0], s[1] if len(s) == 5 else 1, s[-3], s[-2],
+                          0 if k is None else k.shape[-2], s[-1], 0 if freqs is None else freqs.shape[0],
+                          not interleaved, scale, _lib.ptr(freqs),
+                          freqs is not None and freqs.dtype == torch.float64,
+                          positions is not None and positions.dtype == torch.int64, _lib.ptr(positions),
+                          s[-3] if per_seq and seqs > 1 else 0, _strides(q))
+    if k is not None:
+        p.k = _strides(k)
+    return p, (freqs, positions)
+
+
+def _rotate(q, k, freqs, positions, interleaved: bool, scale: float, inverse: bool):
+    """The rotation of checked arguments. A side without heads, or None, is left out."""
+    q_out = _empty(q)
+    k_out = None if k is None else _empty(k)
+    if q.numel() == 0:  # q without heads: k alone
+        if k is not None and k.numel():
+            k_out = _rotate(k, None, freqs, positions, interleaved, scale, inverse)[0]
+        return q_out, k_out
+    q = _unit(q)
+    k = None if k is None or k.numel() == 0 else _unit(k)
+    p, held = _rotary_params(q, k, freqs, positions, interleaved, scale)
+    _launch(q, "unblend_rotary", q.data_ptr(), _lib.ptr(k), q_out.data_ptr(), _lib.ptr(k_out), ctypes.byref(p),
+            inverse)
+    return q_out, k_out
+
+
+def rotary_forward(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor,
+                   positions: torch.Tensor | None = None, interleaved: bool = True, scale: float = 1.0
+                   ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions of queries and keys: ``(q', k')``, contiguous, in q's type.
+
+    q is ``[batch, length, heads, head_dim]`` or ``[outer, inner, length, heads, head_dim]`` as in ``attention``, with any
+    strides of a unit last one; k likewise with its own number of heads, or None. head_dim is at most 256. Pair i of
+    the first ``2 len(freqs)`` dims, ``(2i, 2i + 1)`` or with ``interleaved=False`` ``(i, i + len(freqs))``, turns by
+    ``position * freqs[i]`` and is multiplied by ``scale``; the dims behind stay as they are.
+
+    ``freqs`` (float32 or float64, ``rotary_freqs`` or a checkpoint's) is in radians per position. ``positions`` (int32 or
+    int64) are ``[length]`` for all sequences or one row for each, ``q.shape[:-2]``; None counts rows from 0. Angles are
+    formed and reduced in 64 bits, so that positions below 2^53 lose nothing.
+    """
+    scale = _check_rotary(q, k, freqs, positions, scale)
+    _check_freqs(freqs)
+    _check_cuda("q", q)
+    return _rotate(q, k, freqs, positions, interleaved, scale, False)
+
+
+def _check_freqs(freqs) -> None:
+    if freqs is None:
+        raise ValueError("freqs must be a float32 or float64 tensor [pairs]")
+
+
+def rotary_backward(dq: torch.Tensor, dk: torch.Tensor | None, freqs: torch.Tensor,
+                    positions: torch.Tensor | None = None, interleaved: bool = True, scale: float = 1.0
+                    ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Gradients of the inputs of ``rotary_forward`` from those of its outputs: the transposed rotation."""
+    scale = _check_rotary(dq, dk, freqs, positions, scale)
+    _check_freqs(freqs)
+    _check_cuda("dq", dq)
+    return _rotate(dq, dk, freqs, positions, interleaved, scale, True)
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, freqs, positions, interleaved, scale):
+        ctx.save_for_backward(freqs, positions)
+        ctx.args = interleaved, scale
+        ctx.set_materialize_grads(False)
+        return _rotate(q, k, freqs, positions, interleaved, scale, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        _refuse_capture("rotary")
+        freqs, positions = ctx.saved_tensors
+        interleaved, scale = ctx.args
+        need = ctx.needs_input_grad
+        dq = dq.resolve_neg() if need[0] and dq is not None else None
+        dk = dk.resolve_neg() if need[1] and dk is not None else None
+        if dq is None and dk is not None:  # one output unused
+            return None, _rotate(dk, None, freqs, positions, interleaved, scale, True)[0], None, None, None, None
+        if dq is not None:
+            dq, dk = _rotate(dq, dk, freqs, positions, interleaved, scale, True)
+        return dq, dk, None, None, None, None
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions: torch.Tensor | None = None,
+           interleaved: bool = True, scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Differentiable rotary positions of queries and keys (arguments as ``rotary_forward``)."""
+    scale = _check_rotary(q, k, freqs, positions, scale)
+    _check_freqs(freqs)
+    if _wants_grad("rotary", q, k):
+        _check_cuda("q", q)
+        _refuse_capture("rotary")
+        return _Rotary.apply(q, k, freqs, positions, interleaved, scale)
+    return rotary_forward(q, k, freqs, positions, interleaved, scale)
+
+
+# ------------------------------------------------------------------------ norm of queries and keys, rotary
+
+
+def _check_qk_norm(q, k, gamma_q, gamma_k, freqs, positions, scale, eps, lens) -> float:
+    scale = _check_rotary(q, k, freqs, positions, scale, eps)
+    for name, w in (("gamma_q", gamma_q), ("gamma_k", gamma_k)):
+        if w is not None:
+            _check_weight(name, w, q)
+    if gamma_k is not None and k is None:
+        raise ValueError("gamma_k needs k")
+    if gamma_q is not None and gamma_k is not None and gamma_q.dtype != gamma_k.dtype:
+        raise ValueError(f"gamma_q and gamma_k must share a type, got {gamma_q.dtype} and {gamma_k.dtype}")
+    _check_lens("lens", lens, _seqs(q), q)
+    return scale
+
+
+def _norm_params(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens):
+    p, held = _rotary_params(q, k, freqs, positions, interleaved, scale)
+    gamma_q, gamma_k, lens = (None if t is None else t.contiguous() for t in (gamma_q, gamma_k, lens))
+    w = gamma_q if gamma_q is not None else gamma_k
+    p.gamma_q, p.gamma_k, p.lens, p.eps = _lib.ptr(gamma_q), _lib.ptr(gamma_k), _lib.ptr(lens), eps
+    p.w_dtype = _lib.DTYPE_F32 if w is None else _DTYPES[w.dtype]
+    return p, (*held, gamma_q, gamma_k, lens)
+
+
+def qk_norm_rotary_forward(q: torch.Tensor, k: torch.Tensor | None, gamma_q: torch.Tensor | None = None,
+                           gamma_k: torch.Tensor | None = None, freqs: torch.Tensor | None = None,
+                           positions: torch.Tensor | None = None, interleaved: bool = True, scale: float = 1.0,
+                           eps: float = 1e-6, lens: torch.Tensor | None = None
+                           ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """RMS norm of queries and keys over each head's dims and their rotary positions in one pass: ``(q', k')``.
+
+    ``x' = rot(x / sqrt(mean(x^2) + eps) * gamma)`` in x's type, contiguous. ``gamma_q`` and ``gamma_k`` (``[head_dim]``,
+    shared by the heads) are fp32 or x's type, or None; without ``freqs`` nothing turns. ``lens`` (int32, one per
+    sequence) are the sequences' lengths in a padded batch: rows behind them are not read, whatever they hold, and come
+    out as 0. Other arguments as in ``rotary_forward``.
+    """
+    scale = _check_qk_norm(q, k, gamma_q, gamma_k, freqs, positions, scale, eps, lens)
+    _check_cuda("q", q)
+    return _qk_norm_forward(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
+
+
+def _qk_norm_forward(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens):
+    q_out = _empty(q)
+    k_out = None if k is None else _empty(k)
+    if q.numel() == 0:
+        if k is not None and k.numel():
+            k_out = _qk_norm_forward(k, None, gamma_k, None, freqs, positions, interleaved, scale, eps, lens)[0]
+        return q_out, k_out
+    q = _unit(q)
+    k = None if k is None or k.numel() == 0 else _unit(k)
+    p, held = _norm_params(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
+    _launch(q, "unblend_qk_norm_rotary_forward", q.data_ptr(), _lib.ptr(k), q_out.data_ptr(), _lib.ptr(k_out),
+            ctypes.byref(p))
+    return q_out, k_out
+
+
+def qk_norm_rotary_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor | None,
+                            gamma_q: torch.Tensor | None = None, gamma_k: torch.Tensor | None = None,
+                            freqs: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                            interleaved: bool = True, scale: float = 1.0, eps: float = 1e-6,
+                            lens: torch.Tensor | None = None, weight_grads: bool = True
+                            ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """``(dq, dk, dgamma_q, dgamma_k)`` from the gradients of the outputs of ``qk_norm_rotary_forward`` and its arguments.
+
+    The weights' gradients have the weights' type; they are None without the weight or with ``weight_grads=False``. Rows
+    behind ``lens`` are 0 and add to no gradient.
+    """
+    scale = _check_qk_norm(q, k, gamma_q, gamma_k, freqs, positions, scale, eps, lens)
+    for name, d, x in (("dq", dq, q), ("dk", dk, k)):
+        if (d is None) != (x is None):
+            raise ValueError(f"{name} must be given with its input, and only then")
+        if d is not None:
+            _check_heads(name, d, q)
+            if d.shape != x.shape:
+                raise ValueError(f"{name} must have shape {tuple(x.shape)}, got {tuple(d.shape)}")
+    _check_cuda("q", q)
+    return _qk_norm_backward(dq, dk, q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens,
+                             weight_grads)
+
+
+def _qk_norm_backward(dq, dk, q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens, weight_grads):
+    weight_grads = weight_grads and (gamma_q is not None or gamma_k is not None)
+    dq_out = _empty(q)
+    dk_out = None if k is None else _empty(k)
+    if q.numel() == 0:
+        dgamma_k = _empty(gamma_k).zero_() if weight_grads and gamma_k is not None else None
+        if k is not None and k.numel():
+            dk_out, _, dgamma_k, _ = _qk_norm_backward(dk, None, k, None, gamma_k, None, freqs, positions, interleaved,
+                                                       scale, eps, lens, weight_grads)
+        return dq_out, dk_out, _empty(gamma_q).zero_() if weight_grads and gamma_q is not None else None, dgamma_k
+    q, dq = _unit(q), _unit(dq)
+    k, dk = (None, None) if k is None or k.numel() == 0 else (_unit(k), _unit(dk))
+    p, held = _norm_params(dq, dk, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
+    p.q0 = _strides(q)
+    if k is not None:
+        p.k0 = _strides(k)
+    dgamma_q = dgamma_k = work = None
+    if weight_grads:
+        w = gamma_q if gamma_q is not None else gamma_k
+        dgamma_q, dgamma_k = (q.new_empty(q.shape[-1], dtype=w.dtype) for _ in range(2))
+        n = ctypes.c_longlong(0)
+        _lib.check("unblend_qk_norm_rotary_grad_workspace",
+                   _lib.load().unblend_qk_norm_rotary_grad_workspace(ctypes.byref(p), ctypes.byref(n)))
+        work = _scratch(q, n.value)
+    _launch(q, "unblend_qk_norm_rotary_backward", dq.data_ptr(), _lib.ptr(dk), q.data_ptr(), _lib.ptr(k),
+            dq_out.data_ptr(), _lib.ptr(dk_out), _lib.ptr(dgamma_q), _lib.ptr(dgamma_k), _lib.ptr(work),
+            ctypes.byref(p), kernels=1 + weight_grads)
+    return dq_out, dk_out, dgamma_q if gamma_q is not None else None, dgamma_k if gamma_k is not None else None
+
+
+class _QKNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens):
+        ctx.save_for_backward(q, k, gamma_q, gamma_k, freqs, positions, lens)
+        ctx.args = interleaved, scale, eps
+        return _qk_norm_forward(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        _refuse_capture("qk_norm_rotary")
+        q, k, gamma_q, gamma_k, freqs, positions, lens = ctx.saved_tensors
+        interleaved, scale, eps = ctx.args
+        need = ctx.needs_input_grad
+        got = _qk_norm_backward(dq.resolve_neg(), None if k is None else dk.resolve_neg(), q, k, gamma_q, gamma_k,
+                                freqs, positions, interleaved, scale, eps, lens, need[2] or need[3])
+        return *(d if n else None for d, n in zip(got, need)), None, None, None, None, None, None
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, gamma_q: torch.Tensor | None = None,
+                   gamma_k: torch.Tensor | None = None, freqs: torch.Tensor | None = None,
+                   positions: torch.Tensor | None = None, interleaved: bool = True, scale: float = 1.0,
+                   eps: float = 1e-6, lens: torch.Tensor | None = None
+                   ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Differentiable RMS norm and rotary positions of queries and keys (arguments as ``qk_norm_rotary_forward``)."""
+    scale = _check_qk_norm(q, k, gamma_q, gamma_k, freqs, positions, scale, eps, lens)
+    if _wants_grad("qk_norm_rotary", q, k, gamma_q, gamma_k):
+        _check_cuda("q", q)
+        _refuse_capture("qk_norm_rotary")
+        return _QKNormRotary.apply(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
+    return qk_norm_rotary_forward(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
 
 
 # ----------------------------------------------------------------------------------------- dropout-add
