@@ -23,6 +23,7 @@ extern "C" {
 
 #define UNBLEND_ERR_INVALID 1000
 #define UNBLEND_ERR_TOO_LARGE 1001 /* request exceeds a fixed built-in capacity */
+#define UNBLEND_ERR_OVERLAP 1002   /* tensors that a call writes share memory with others of it */
 
 /* Activation applied in a convolution epilogue. */
 enum UnblendAct {
@@ -696,6 +697,48 @@ int unblend_attention_backward(const void* dout, const void* q, const void* k, c
 
 /* Device flag set when a bounded wait of the two entry points above gives up (0 = none). Synchronous host call. */
 int unblend_attention_train_error_flag(int* out_host, int clear);
+
+/*
+ * AdamW over many tensors at once, and the 2-norm of many tensors. The table is host memory, read before the call
+ * returns; captured graphs keep what it held.
+ */
+typedef struct {
+  void* param;      /* n contiguous elements of dtype, updated in place (not read by unblend_grad_norm) */
+  const void* grad; /* n contiguous elements of grad_dtype */
+  long long n;      /* >= 1 */
+  long long block;  /* the tensor's moments start at element 256 * block of exp_avg and exp_avg_sq */
+} UnblendAdamWTensor;
+
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  long long step;               /* number of this update, from 1 */
+  const long long* step_device; /* its place in device memory instead, or NULL */
+  const float* lr_device;       /* lr in device memory instead, or NULL */
+  const float* grad_scale;      /* device, factor on the gradients, or NULL; not finite: the call changes nothing */
+} UnblendAdamWParams;
+
+/*
+ * m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
+ * p = (1 - lr weight_decay) p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps).
+ * bits 32: exp_avg and exp_avg_sq are float, whole blocks of 256 per tensor. bits 8: uint8 codes, and scales holds two
+ * floats per block, the largest |m| and the largest u = sqrt(v). With c = code & 127 a code of exp_avg stands for the
+ * float of the bit pattern (c + 889) << 20 (0 for c = 0) times the first scale, negative with bit 7; a code of exp_avg_sq
+ * for the square of the pattern (code + 1777) << 19 (0 for 0) times the second. Parameters must not share memory with
+ * one another or with a gradient (UNBLEND_ERR_OVERLAP).
+ */
+int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, void* exp_avg, void* exp_avg_sq, float* scales,
+                       int bits, int dtype, int grad_dtype, const UnblendAdamWParams* p, void* stream);
+
+/* The values of `blocks` blocks of 8-bit moments: m and v, float. */
+int unblend_adamw_values(const void* exp_avg, const void* exp_avg_sq, const float* scales, float* m, float* v,
+                         long long blocks, void* stream);
+
+/* norm = sqrt(sum of all squares), summed in double; scale (may be NULL) = min(1, max_norm / norm), NaN for a norm that
+ * is not finite. counts[t]: how many tensors of UnblendDtype t the table holds, fp32 first. work:
+ * unblend_grad_norm_workspace bytes for the sum of the counts. */
+int unblend_grad_norm(const UnblendAdamWTensor* tensors, const int* counts, float max_norm, float* norm, float* scale,
+                      double* work, void* stream);
+int unblend_grad_norm_workspace(int count, long long* bytes);
 
 
 #ifdef __cplusplus

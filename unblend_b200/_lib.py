@@ -18,6 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_lib", "libunblend_b200.so")
 ERR_INVALID = 1000
 ERR_TOO_LARGE = 1001
+ERR_OVERLAP = 1002
 NOALLOC_MAX_BATCH = 4096
 
 c_int = ctypes.c_int
@@ -114,6 +115,15 @@ class RotaryParams(ctypes.Structure):
     ]
 
 
+class AdamWParams(ctypes.Structure):
+    """Mirror of ``UnblendAdamWParams``."""
+
+    _fields_ = [
+        ("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
+        ("step", c_ll), ("step_device", c_void_p), ("lr_device", c_void_p), ("grad_scale", c_void_p),
+    ]
+
+
 # name -> argtypes (all return int)
 _SIGNATURES = {
     "unblend_conv2d_f32": [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(ConvParams), c_void_p],
@@ -197,6 +207,10 @@ _SIGNATURES = {
                                   ctypes.POINTER(AttnTrainParams), c_void_p],
     "unblend_attention_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_ll, ctypes.POINTER(AttnTrainParams), c_void_p],
+    "unblend_adamw_step": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                           ctypes.POINTER(AdamWParams), c_void_p],
+    "unblend_adamw_values": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p],
+    "unblend_grad_norm": [c_void_p, ctypes.POINTER(c_int), c_float, c_void_p, c_void_p, c_void_p, c_void_p],
     "unblend_rotary": [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(RotaryParams), c_int, c_void_p],
     "unblend_qk_norm_rotary_forward": [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(RotaryParams), c_void_p],
     "unblend_qk_norm_rotary_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -213,6 +227,7 @@ _HOST_SIGNATURES = {
     "unblend_attention_train_error_flag": [ctypes.POINTER(c_int), c_int],
     "unblend_layer_norm_grad_workspace": [c_ll, c_int, ctypes.POINTER(c_ll)],
     "unblend_dropout_add_grad_workspace": [c_ll, c_int, ctypes.POINTER(c_ll)],
+    "unblend_grad_norm_workspace": [c_int, ctypes.POINTER(c_ll)],
     "unblend_qk_norm_rotary_grad_workspace": [ctypes.POINTER(RotaryParams), ctypes.POINTER(c_ll)],
     "unblend_attention_workspace": [ctypes.POINTER(AttnTrainParams), c_int, ctypes.POINTER(c_ll)],
 }
@@ -295,6 +310,8 @@ def check(name: str, rc: int) -> None:
         raise RuntimeError(f"{name}: request exceeds the entry point's fixed built-in capacity")
     if rc == ERR_INVALID:
         raise RuntimeError(f"{name}: invalid arguments")
+    if rc == ERR_OVERLAP:
+        raise ValueError(f"{name}: tensors that are written share memory with others of the call")
     text = _cuda_error_string(rc)
     if rc == 2:  # cudaErrorMemoryAllocation
         raise RuntimeError(f"CUDA out of memory in {name} ({text})")

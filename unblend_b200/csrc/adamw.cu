@@ -1,0 +1,532 @@
+// An AdamW step over many tensors in one launch, its moments in fp32 or 8 bits, and the 2-norm of many tensors.
+//
+//   g' = c g,  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+//   p  = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// The moments of all tensors lie in one array each; every tensor starts at a block of 256 elements of its own. A warp
+// takes a block at a time and finds its tensor in the table of the launch (kernel parameters: nothing is copied to the
+// device, and a captured graph keeps them) by bisection. Bound: HBM, 28 bytes per element for fp32 and 32 bits, 10 + 1/16
+// for 16-bit tensors and 8 bits.
+//
+// 8 bits: a block has two scales, the largest |m| and the largest u = sqrt(v). u is kept instead of v because its range is
+// half as many octaves. Codes are small floats relative to the scale, whose largest code is 1: m has a sign, 3 bits of
+// mantissa and 15.9 octaves, u 4 bits and 15.9 octaves. Both are the leading bits of the fp32 pattern, rounded to
+// nearest even (a step is 2^-3, 2^-4 of the octave's start). An m below half the smallest magnitude is 0; a u that is not
+// 0 never becomes 0, since the update divides by it. The update itself uses m and v before they are rounded. What decides
+// a code is computed in fp32 one operation at a time (no fused multiply-add), so that the codes are defined bit for bit.
+// A value that is not finite makes its block's scale infinite or NaN, and with it every moment of the block.
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "train_common.cuh"
+
+namespace {
+
+using namespace ub::train;
+
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int BLOCK = 256;            // elements that share scales
+constexpr int SMALL = 64, LARGE = 896;  // tensors of a launch: 2.3 or 32 KB of kernel parameters
+
+template <int N>
+struct Table {
+  UnblendAdamWTensor t[N];
+  unsigned start[N];  // first of the launch's units of each tensor
+  int count;
+  unsigned total;
+};
+
+// The tensor that a unit belongs to.
+template <int N>
+__device__ __forceinline__ int tensor_of(const Table<N>& tab, unsigned unit) {
+  int lo = 0, hi = tab.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (tab.start[mid] <= unit)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+struct StepArgs {
+  void* m;
+  void* v;
+  float2* scales;
+  const float* grad_scale;
+  const long long* step;  // device: the bias corrections and factors below are computed from it
+  const float* lr;        // device
+  double b1d, b2d, lrd, wdd;
+  float b1, c1, b2, c2, eps;
+  float decay, size, root;  // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+};
+
+// The smallest code's patterns: 2^-16 * 1.25 and 2^-16 * 1.125 are code 1.
+constexpr unsigned M_SHIFT = 20, M_LOW = (127u << 3) - 127u, U_SHIFT = 19, U_LOW = (127u << 4) - 255u;
+constexpr float M_LEAST = 0.625f / 65536.f;  // half of code 1
+
+__device__ __forceinline__ float m_value(unsigned code) {
+  const unsigned c = code & 127u;
+  const float v = c ? __uint_as_float((c + M_LOW) << M_SHIFT) : 0.f;
+  return code & 128u ? -v : v;
+}
+__device__ __forceinline__ float u_value(unsigned code) {
+  return code ? __uint_as_float((code + U_LOW) << U_SHIFT) : 0.f;
+}
+
+template <unsigned SHIFT>
+__device__ __forceinline__ int leading(float r) {  // the pattern's leading bits, to nearest even
+  const unsigned w = __float_as_uint(r);
+  return (int)((w + ((1u << (SHIFT - 1)) - 1u) + ((w >> SHIFT) & 1u)) >> SHIFT);
+}
+__device__ __forceinline__ unsigned m_code(float m, float inv) {
+  const float r = __fmul_rn(fabsf(m), inv);
+  const int c = min(max(leading<M_SHIFT>(r) - (int)M_LOW, 1), 127);
+  return (r > M_LEAST ? (unsigned)c : 0u) | (m < 0.f ? 128u : 0u);
+}
+__device__ __forceinline__ unsigned u_code(float u, float inv) {
+  const float r = __fmul_rn(u, inv);
+  return r > 0.f ? (unsigned)min(max(leading<U_SHIFT>(r) - (int)U_LOW, 1), 255) : 0u;
+}
+
+// 1 / top, 0 for a block of zeros (or below the normal range, where 1 / top could overflow).
+__device__ __forceinline__ float inverse(float top) { return top >= 1.17549435e-38f ? __frcp_rn(top) : 0.f; }
+
+// Four consecutive elements; without `full`, those below n.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&v)[4], bool full, int n) {
+  if (full) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 w = *reinterpret_cast<const float4*>(p);
+      v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+    } else {
+      alignas(8) T raw[4];
+      *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = to_f(raw[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? to_f(p[i]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4], bool full, int n) {
+  if (full) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      alignas(8) T raw[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = from_f<T>(v[i]);
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(raw);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = from_f<T>(v[i]);
+  }
+}
+
+// Largest of non-negative values by their patterns: NaN is above infinity.
+__device__ __forceinline__ float warp_top(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
+
+template <typename T, typename TG, bool EIGHT, int N>
+__global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ Table<N> tab,
+                                                        const __grid_constant__ StepArgs a) {
+  float decay = a.decay, size = a.size, root = a.root;
+  const float gs = a.grad_scale ? *a.grad_scale : 1.f;
+  if (!isfinite(gs)) return;  // an overflow somewhere in the gradients: nothing changes
+  if (a.step || a.lr) {
+    __shared__ float f[3];
+    if (threadIdx.x == 0) {
+      const double lr = a.lr ? (double)*a.lr : a.lrd;
+      f[0] = (float)(1.0 - lr * a.wdd);
+      if (a.step) {
+        const double t = (double)max(*a.step, 1LL);
+        f[1] = (float)(lr / (1.0 - pow(a.b1d, t)));
+        f[2] = (float)(1.0 / sqrt(1.0 - pow(a.b2d, t)));
+      } else {  // size is 1 / (1 - b1^t) here
+        f[1] = (float)(lr * (double)size);
+        f[2] = root;
+      }
+    }
+    __syncthreads();
+    decay = f[0], size = f[1], root = f[2];
+  }
+  const int lane = threadIdx.x & 31;
+  for (unsigned unit = blockIdx.x * WARPS + (threadIdx.x >> 5); unit < tab.total; unit += gridDim.x * WARPS) {
+    const int k = tensor_of(tab, unit);
+    const long long local = unit - tab.start[k];
+    const long long left = tab.t[k].n - local * BLOCK;
+    T* p = static_cast<T*>(tab.t[k].param) + local * BLOCK;
+    const TG* g = static_cast<const TG*>(tab.t[k].grad) + local * BLOCK;
+    const long long block = tab.t[k].block + local;
+    const bool full = left >= BLOCK && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 &&
+                      reinterpret_cast<uintptr_t>(g) % (4 * sizeof(TG)) == 0;
+    float pv[2][4], gv[2][4], mv[2][4], uv[2][4];
+    unsigned mc[2], uc[2];
+    float2 sc;
+    const long long at = block * BLOCK + lane * 4;
+    if constexpr (EIGHT) {
+      sc = a.scales[block];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        mc[j] = *reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(a.m) + at + j * 128);
+        uc[j] = *reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(a.v) + at + j * 128);
+      }
+    }
+    int n[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int e = lane * 4 + j * 128;
+      n[j] = left >= BLOCK ? 4 : min(max((int)left - e, 0), 4);
+      load4(p + e, pv[j], full, n[j]);
+      load4(g + e, gv[j], full, n[j]);
+      if constexpr (!EIGHT) {
+        load4(static_cast<const float*>(a.m) + at + j * 128, mv[j], true, 4);
+        load4(static_cast<const float*>(a.v) + at + j * 128, uv[j], true, 4);
+      }
+    }
+    float top_m = 0.f, top_u = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float gr = __fmul_rn(gv[j][i], gs);
+        float m, v;
+        if constexpr (EIGHT) {
+          m = __fmul_rn(m_value((mc[j] >> (8 * i)) & 255u), sc.x);
+          const float u = __fmul_rn(u_value((uc[j] >> (8 * i)) & 255u), sc.y);
+          v = __fmul_rn(u, u);
+        } else {
+          m = mv[j][i], v = uv[j][i];
+        }
+        m = __fadd_rn(__fmul_rn(m, a.b1), __fmul_rn(gr, a.c1));
+        v = __fadd_rn(__fmul_rn(v, a.b2), __fmul_rn(__fmul_rn(gr, gr), a.c2));
+        const float u = __fsqrt_rn(v);
+        pv[j][i] = pv[j][i] * decay - size * (m / (u * root + a.eps));
+        mv[j][i] = m;
+        uv[j][i] = EIGHT ? u : v;
+        if constexpr (EIGHT) {
+          // by patterns, as a NaN has to come through
+          top_m = __uint_as_float(max(__float_as_uint(top_m), __float_as_uint(fabsf(m))));
+          top_u = __uint_as_float(max(__float_as_uint(top_u), __float_as_uint(u) & 0x7fffffffu));
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      store4(p + lane * 4 + j * 128, pv[j], full, n[j]);
+      if constexpr (!EIGHT) {
+        store4(static_cast<float*>(a.m) + at + j * 128, mv[j], true, 4);
+        store4(static_cast<float*>(a.v) + at + j * 128, uv[j], true, 4);
+      }
+    }
+    if constexpr (EIGHT) {
+      top_m = warp_top(top_m), top_u = warp_top(top_u);
+      const float inv_m = inverse(top_m), inv_u = inverse(top_u);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        unsigned cm = 0, cu = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          cm |= m_code(mv[j][i], inv_m) << (8 * i);
+          cu |= u_code(uv[j][i], inv_u) << (8 * i);
+        }
+        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.m) + at + j * 128) = cm;
+        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.v) + at + j * 128) = cu;
+      }
+      if (lane == 0) a.scales[block] = make_float2(top_m, top_u);
+    }
+  }
+}
+
+// The values that 8-bit moments stand for. A warp per block.
+__global__ void __launch_bounds__(THREADS) adamw_values_kernel(const uint8_t* m, const uint8_t* u, const float2* scales,
+                                                               float* m_out, float* v_out, unsigned blocks) {
+  const int lane = threadIdx.x & 31;
+  for (unsigned b = blockIdx.x * WARPS + (threadIdx.x >> 5); b < blocks; b += gridDim.x * WARPS) {
+    const float2 sc = scales[b];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const long long at = (long long)b * BLOCK + lane * 4 + j * 128;
+      const unsigned mc = *reinterpret_cast<const unsigned*>(m + at), uc = *reinterpret_cast<const unsigned*>(u + at);
+      float mv[4], vv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mv[i] = __fmul_rn(m_value((mc >> (8 * i)) & 255u), sc.x);
+        const float w = __fmul_rn(u_value((uc >> (8 * i)) & 255u), sc.y);
+        vv[i] = __fmul_rn(w, w);
+      }
+      store4(m_out + at, mv, true, 4);
+      store4(v_out + at, vv, true, 4);
+    }
+  }
+}
+
+// Sums of squares in double: exact products, and neither overflow nor underflow for any fp32 value. Warps take runs of
+// 1024 elements; CTAs leave a sum each, and one CTA adds those in a fixed order.
+constexpr int RUN = 1024;
+
+template <typename T, int N>
+__global__ void __launch_bounds__(THREADS) square_sums_kernel(const __grid_constant__ Table<N> tab, double* part) {
+  __shared__ double red[WARPS];
+  constexpr int VEC = 16 / (int)sizeof(T), LOADS = RUN / 32 / VEC;
+  const int lane = threadIdx.x & 31;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  for (unsigned unit = blockIdx.x * WARPS + (threadIdx.x >> 5); unit < tab.total; unit += gridDim.x * WARPS) {
+    const int k = tensor_of(tab, unit);
+    const long long local = unit - tab.start[k];
+    const long long left = tab.t[k].n - local * RUN;
+    const T* g = static_cast<const T*>(tab.t[k].grad) + local * RUN;
+    if (left >= RUN && reinterpret_cast<uintptr_t>(g) % 16 == 0) {
+      uint4 w[LOADS];
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) w[j] = reinterpret_cast<const uint4*>(g)[j * 32 + lane];
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        float2 v[VEC / 2];
+        unpack16(w[j], v, T());
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+          s[(2 * i) % 4] = fma((double)v[i].x, (double)v[i].x, s[(2 * i) % 4]);
+          s[(2 * i + 1) % 4] = fma((double)v[i].y, (double)v[i].y, s[(2 * i + 1) % 4]);
+        }
+      }
+    } else {
+      for (int e = lane; e < RUN && e < left; e += 32) {
+        const double x = (double)to_f(g[e]);
+        s[0] = fma(x, x, s[0]);
+      }
+    }
+  }
+  double t = ub::warp_sum_d((s[0] + s[1]) + (s[2] + s[3]));
+  if (lane == 0) red[threadIdx.x >> 5] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    t = red[0];
+    for (int w = 1; w < WARPS; ++w) t += red[w];
+    part[blockIdx.x] = t;
+  }
+}
+
+__global__ void __launch_bounds__(1024) norm_join_kernel(const double* part, int n, float max_norm, float* norm,
+                                                         float* scale) {
+  __shared__ double red[32];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) s += part[i];
+  s = ub::warp_sum_d(s);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = ub::warp_sum_d(red[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      const double r = sqrt(s);
+      *norm = (float)r;
+      if (scale) *scale = !isfinite(r) ? (float)(r - r) : r > max_norm ? (float)(max_norm / r) : 1.f;
+    }
+  }
+}
+
+template <int N>
+Table<N> make_table(const UnblendAdamWTensor* t, int count, int unit) {
+  Table<N> tab;
+  tab.count = count;
+  unsigned at = 0;
+  for (int i = 0; i < count; ++i) {
+    tab.t[i] = t[i];
+    tab.start[i] = at;
+    at += (unsigned)((t[i].n + unit - 1) / unit);
+  }
+  tab.total = at;
+  return tab;
+}
+
+bool tensors_ok(const UnblendAdamWTensor* t, int count, bool params, int elem, int grad_elem) {
+  if (!t || count < 1) return false;
+  long long units = 0;
+  for (int i = 0; i < count; ++i) {
+    if (t[i].n < 1 || t[i].n >= (1LL << 39) || !t[i].grad || reinterpret_cast<uintptr_t>(t[i].grad) % grad_elem)
+      return false;
+    if (params && (!t[i].param || reinterpret_cast<uintptr_t>(t[i].param) % elem || t[i].block < 0)) return false;
+    units += (t[i].n + BLOCK - 1) / BLOCK;
+  }
+  return units < (1LL << 31);
+}
+
+// Whether no two parameters share memory with one another, nor a parameter with a gradient.
+bool apart(const UnblendAdamWTensor* t, int count, int elem, int grad_elem) {
+  struct Span {
+    uintptr_t from, to;
+    bool param;
+  };
+  std::vector<Span> s;
+  s.reserve(2 * (size_t)count);
+  for (int i = 0; i < count; ++i) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t[i].param), g = reinterpret_cast<uintptr_t>(t[i].grad);
+    s.push_back(Span{p, p + (uintptr_t)t[i].n * elem, true});
+    s.push_back(Span{g, g + (uintptr_t)t[i].n * grad_elem, false});
+  }
+  std::sort(s.begin(), s.end(), [](const Span& x, const Span& y) { return x.from < y.from; });
+  uintptr_t params = 0, all = 0;
+  for (const Span& x : s) {
+    if (x.from < (x.param ? all : params)) return false;
+    if (x.param) params = std::max(params, x.to);
+    all = std::max(all, x.to);
+  }
+  return true;
+}
+
+unsigned grid_of(unsigned units, int per_sm) {
+  const unsigned ctas = (units + WARPS - 1) / WARPS, cap = ub::kNumSMs * per_sm;
+  return ctas < cap ? ctas : cap;
+}
+
+template <typename T, typename TG, bool EIGHT>
+int launch_step(const UnblendAdamWTensor* t, int count, const StepArgs& a, cudaStream_t st) {
+  for (int i = 0; i < count; i += LARGE) {
+    const int n = std::min(LARGE, count - i);
+    if (n <= SMALL) {
+      const Table<SMALL> tab = make_table<SMALL>(t + i, n, BLOCK);
+      adamw_kernel<T, TG, EIGHT, SMALL><<<grid_of(tab.total, 8), THREADS, 0, st>>>(tab, a);
+    } else {
+      const Table<LARGE> tab = make_table<LARGE>(t + i, n, BLOCK);
+      adamw_kernel<T, TG, EIGHT, LARGE><<<grid_of(tab.total, 8), THREADS, 0, st>>>(tab, a);
+    }
+    UB_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+template <typename T, typename TG>
+int launch_bits(const UnblendAdamWTensor* t, int count, int bits, const StepArgs& a, cudaStream_t st) {
+  return bits == 8 ? launch_step<T, TG, true>(t, count, a, st) : launch_step<T, TG, false>(t, count, a, st);
+}
+
+template <typename T>
+int launch_grad(const UnblendAdamWTensor* t, int count, int grad_dtype, int bits, const StepArgs& a, cudaStream_t st) {
+  switch (grad_dtype) {
+    case UNBLEND_F32: return launch_bits<T, float>(t, count, bits, a, st);
+    case UNBLEND_BF16: return launch_bits<T, __nv_bfloat16>(t, count, bits, a, st);
+    default: return launch_bits<T, __half>(t, count, bits, a, st);
+  }
+}
+
+constexpr int NORM_GRID = ub::kNumSMs * 8;
+
+template <typename T>
+int launch_squares(const UnblendAdamWTensor* t, int count, double* part, int* used, cudaStream_t st) {
+  for (int i = 0; i < count; i += LARGE) {
+    const int n = std::min(LARGE, count - i);
+    unsigned grid;
+    if (n <= SMALL) {
+      const Table<SMALL> tab = make_table<SMALL>(t + i, n, RUN);
+      square_sums_kernel<T, SMALL><<<grid = grid_of(tab.total, 8), THREADS, 0, st>>>(tab, part + *used);
+    } else {
+      const Table<LARGE> tab = make_table<LARGE>(t + i, n, RUN);
+      square_sums_kernel<T, LARGE><<<grid = grid_of(tab.total, 8), THREADS, 0, st>>>(tab, part + *used);
+    }
+    UB_CHECK_LAUNCH();
+    *used += (int)grid;
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, void* exp_avg, void* exp_avg_sq,
+                                  float* scales, int bits, int dtype, int grad_dtype, const UnblendAdamWParams* p,
+                                  void* stream) {
+  UB_REQUIRE(p && known_type(dtype) && known_type(grad_dtype) && (bits == 32 || bits == 8));
+  UB_REQUIRE(exp_avg && exp_avg_sq && aligned16(exp_avg) && aligned16(exp_avg_sq));
+  UB_REQUIRE(bits == 32 || (scales && reinterpret_cast<uintptr_t>(scales) % 8 == 0));
+  UB_REQUIRE(p->beta1 >= 0 && p->beta1 < 1 && p->beta2 >= 0 && p->beta2 < 1 && p->eps >= 0 && std::isfinite(p->eps));
+  UB_REQUIRE(std::isfinite(p->weight_decay) && (p->lr_device || std::isfinite(p->lr)));
+  UB_REQUIRE(p->step_device || p->step >= 1);
+  UB_REQUIRE(reinterpret_cast<uintptr_t>(p->step_device) % 8 == 0 && reinterpret_cast<uintptr_t>(p->lr_device) % 4 == 0 &&
+             reinterpret_cast<uintptr_t>(p->grad_scale) % 4 == 0);
+  UB_REQUIRE(tensors_ok(tensors, count, true, elem_size(dtype), elem_size(grad_dtype)));
+  try {
+    if (!apart(tensors, count, elem_size(dtype), elem_size(grad_dtype))) return UNBLEND_ERR_OVERLAP;
+  } catch (const std::bad_alloc&) {
+    return (int)cudaErrorMemoryAllocation;
+  }
+  StepArgs a{};
+  a.m = exp_avg;
+  a.v = exp_avg_sq;
+  a.scales = reinterpret_cast<float2*>(scales);
+  a.grad_scale = p->grad_scale;
+  a.step = p->step_device;
+  a.lr = p->lr_device;
+  a.b1d = p->beta1;
+  a.b2d = p->beta2;
+  a.lrd = p->lr;
+  a.wdd = p->weight_decay;
+  a.b1 = (float)p->beta1;
+  a.c1 = (float)(1.0 - p->beta1);
+  a.b2 = (float)p->beta2;
+  a.c2 = (float)(1.0 - p->beta2);
+  a.eps = (float)p->eps;
+  const double t = p->step_device ? 1.0 : (double)p->step;
+  const double correction = 1.0 - std::pow(p->beta1, t);
+  a.decay = (float)(1.0 - p->lr * p->weight_decay);
+  a.size = (float)((p->lr_device ? 1.0 : p->lr) / correction);
+  a.root = (float)(1.0 / std::sqrt(1.0 - std::pow(p->beta2, t)));
+  cudaStream_t st = ub::as_stream(stream);
+  switch (dtype) {
+    case UNBLEND_F32: return launch_grad<float>(tensors, count, grad_dtype, bits, a, st);
+    case UNBLEND_BF16: return launch_grad<__nv_bfloat16>(tensors, count, grad_dtype, bits, a, st);
+    default: return launch_grad<__half>(tensors, count, grad_dtype, bits, a, st);
+  }
+}
+
+extern "C" int unblend_adamw_values(const void* exp_avg, const void* exp_avg_sq, const float* scales, float* m, float* v,
+                                    long long blocks, void* stream) {
+  UB_REQUIRE(exp_avg && exp_avg_sq && scales && m && v && blocks >= 1 && blocks < (1LL << 31));
+  UB_REQUIRE(aligned16(exp_avg) && aligned16(exp_avg_sq) && aligned16(m) && aligned16(v) &&
+             reinterpret_cast<uintptr_t>(scales) % 8 == 0);
+  adamw_values_kernel<<<grid_of((unsigned)blocks, 8), THREADS, 0, ub::as_stream(stream)>>>(
+      static_cast<const uint8_t*>(exp_avg), static_cast<const uint8_t*>(exp_avg_sq),
+      reinterpret_cast<const float2*>(scales), m, v, (unsigned)blocks);
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
+extern "C" int unblend_grad_norm_workspace(int count, long long* bytes) {
+  UB_REQUIRE(count >= 1 && bytes);
+  // A launch for every LARGE tensors of each of the three types.
+  *bytes = ((count + LARGE - 1) / LARGE + 2LL) * NORM_GRID * (long long)sizeof(double);
+  return 0;
+}
+
+extern "C" int unblend_grad_norm(const UnblendAdamWTensor* tensors, const int* counts, float max_norm, float* norm,
+                                 float* scale, double* work, void* stream) {
+  UB_REQUIRE(tensors && counts && norm && work && reinterpret_cast<uintptr_t>(work) % 8 == 0);
+  UB_REQUIRE(!scale || (max_norm > 0.f && std::isfinite(max_norm)));
+  int used = 0, first = 0;
+  for (int t = 0; t < 3; ++t) {
+    UB_REQUIRE(counts[t] >= 0);
+    UB_REQUIRE(counts[t] == 0 || tensors_ok(tensors + first, counts[t], false, 1, elem_size(t)));
+    first += counts[t];
+  }
+  first = 0;
+  cudaStream_t st = ub::as_stream(stream);
+  for (int t = 0; t < 3; ++t) {
+    int rc = 0;
+    if (counts[t] == 0) continue;
+    if (t == UNBLEND_F32)
+      rc = launch_squares<float>(tensors + first, counts[t], work, &used, st);
+    else if (t == UNBLEND_BF16)
+      rc = launch_squares<__nv_bfloat16>(tensors + first, counts[t], work, &used, st);
+    else
+      rc = launch_squares<__half>(tensors + first, counts[t], work, &used, st);
+    if (rc) return rc;
+    first += counts[t];
+  }
+  norm_join_kernel<<<1, 1024, 0, st>>>(work, used, max_norm, norm, scale);
+  UB_CHECK_LAUNCH();
+  return 0;
+}

@@ -25,7 +25,11 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
+from collections.abc import Sequence
 from functools import lru_cache
+from itertools import accumulate
+from typing import NamedTuple
 
 import torch
 from torch.autograd import forward_ad
@@ -35,6 +39,8 @@ from . import _lib
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 MAX_HEAD_DIM = 128
 MAX_ROTARY_DIM = 256
+ADAMW_BLOCK = 256  # elements of a moment that share a scale in 8 bits; each parameter starts a block of its own
+_TABLE = 896  # tensors of one launch
 _F32_MAX = torch.finfo(torch.float32).max
 _REGISTER_COLS = 8192  # widest rows whose layer norm sums the weights' gradients beside the input's
 _MOST = 1 << 31  # rows, and columns, of layer norm and dropout-add
@@ -896,3 +902,256 @@ def dropout_add(x: torch.Tensor, p: float, rng: torch.Tensor, residual: torch.Te
         _refuse_capture("dropout_add")
         return _DropoutAdd.apply(x, p, rng, residual, scale)
     return dropout_add_forward(x, p, rng, residual, scale)
+
+
+# ------------------------------------------------------------------------------- AdamW, norm of gradients
+
+
+class AdamWState(NamedTuple):
+    """Moments of ``adamw_step``, to be kept, saved and loaded as they are.
+
+    The moments of all parameters lie in one array each, every parameter's from a multiple of ``ADAMW_BLOCK`` elements
+    on. In 32 bits both are fp32 and ``scales`` is None. In 8 bits they are uint8 codes of ``exp_avg`` and of the root of
+    ``exp_avg_sq``, and ``scales`` (fp32, ``[blocks, 2]``) holds the largest magnitudes of each block.
+    """
+
+    exp_avg: torch.Tensor
+    exp_avg_sq: torch.Tensor
+    scales: torch.Tensor | None = None
+
+
+def _check_list(name: str, tensors) -> list:
+    if isinstance(tensors, torch.Tensor):
+        raise ValueError(f"{name} must be a list of tensors, got one tensor")
+    try:
+        return list(tensors)
+    except TypeError:
+        raise ValueError(f"{name} must be a list of tensors, got {type(tensors).__name__}") from None
+
+
+def _check_dense(name: str, tensors: list) -> None:
+    """Contiguous tensors of known types on one device (whole-list passes: models have hundreds of parameters)."""
+    if not all(isinstance(t, torch.Tensor) for t in tensors):
+        raise ValueError(f"{name} must hold tensors only")
+    if any(t.layout != torch.strided for t in tensors):
+        raise ValueError(f"{name} must be dense tensors")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        i = [t.is_contiguous() for t in tensors].index(False)
+        raise ValueError(f"{name}[{i}] must be contiguous, got shape {tuple(tensors[i].shape)} with strides "
+                         f"{tensors[i].stride()}")
+    if len(set(map(torch.Tensor.get_device, tensors))) > 1:
+        raise ValueError(f"{name} must be on one device")
+    for t in {t.dtype for t in tensors}:
+        if t not in _DTYPES:
+            raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t}")
+    if any(map(torch.Tensor.is_neg, tensors)):
+        raise ValueError(f"{name} holds a lazily negated view: give its resolve_neg()")
+
+
+def _blocks(tensors: list) -> list[int]:
+    return [-(-n // ADAMW_BLOCK) for n in map(torch.Tensor.numel, tensors)]
+
+
+def adamw_state(params: Sequence[torch.Tensor], bits: int = 32) -> AdamWState:
+    """Moments of zeros for ``params``, in 32 or 8 bits."""
+    params = _check_list("params", params)
+    _check_dense("params", params)
+    if bits not in (32, 8):
+        raise ValueError(f"bits must be 32 or 8, got {bits!r}")
+    if not params:
+        raise ValueError("params must hold at least one tensor")
+    n = sum(_blocks(params))
+    dev = params[0].device
+    t = torch.float32 if bits == 32 else torch.uint8
+    return AdamWState(torch.zeros(n * ADAMW_BLOCK, dtype=t, device=dev), torch.zeros(n * ADAMW_BLOCK, dtype=t, device=dev),
+                      torch.zeros(n, 2, device=dev) if bits == 8 else None)
+
+
+def _check_state(state) -> int:
+    """Blocks of a state's moments."""
+    if not isinstance(state, AdamWState):
+        raise ValueError(f"state must be an AdamWState, got {type(state).__name__}")
+    m, v, scales = state
+    t = torch.float32 if scales is None else torch.uint8
+    for name, x in (("exp_avg", m), ("exp_avg_sq", v)):
+        if not isinstance(x, torch.Tensor) or x.dtype != t or x.dim() != 1 or x.numel() % ADAMW_BLOCK or \
+                not x.is_contiguous() or x.data_ptr() % 16:
+            raise ValueError(f"state.{name} must be contiguous {t} from a 16-byte boundary on, whole blocks of "
+                             f"{ADAMW_BLOCK} ({'without' if scales is None else 'with'} scales)")
+    blocks = m.numel() // ADAMW_BLOCK
+    if m.shape != v.shape or m.device != v.device:
+        raise ValueError("state.exp_avg and state.exp_avg_sq must have one shape and device")
+    if blocks and m.data_ptr() == v.data_ptr():
+        raise ValueError("state.exp_avg and state.exp_avg_sq must be two tensors")
+    if scales is not None and (not isinstance(scales, torch.Tensor) or scales.dtype != torch.float32 or
+                               scales.shape != (blocks, 2) or not scales.is_contiguous() or
+                               scales.device != m.device or scales.data_ptr() % 8):
+        raise ValueError(f"state.scales must be contiguous float32 ({blocks}, 2) on {m.device}")
+    return blocks
+
+
+def _check_scalar(name: str, t, dtype: torch.dtype, device: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.numel() != 1 or t.device != device or t.is_neg():
+        raise ValueError(f"{name} must be a {dtype} tensor of one element on {device}")
+
+
+def _number(name: str, x, low: float, high: float = math.inf) -> float:
+    if isinstance(x, bool) or not isinstance(x, (int, float)) or not low <= x < high:
+        raise ValueError(f"{name} must be a number in [{low:g}, {high:g}), got {x!r}")
+    return float(x)
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | None], state: AdamWState,
+               step: int | torch.Tensor, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
+               eps: float = 1e-8, weight_decay: float = 0.01, grad_scale: torch.Tensor | None = None) -> None:
+    """One AdamW update of all ``params`` and of ``state``, in place.
+
+    With g the gradient times ``grad_scale``, ``m = beta1 m + (1 - beta1) g``, ``v = beta2 v + (1 - beta2) g^2`` and
+    ``p = (1 - lr weight_decay) p - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)``, in fp32, rounded once
+    to the parameter's type. Parameters are contiguous fp32, bf16 or fp16 in any mixture, gradients likewise with a type of
+    their own (fp32 parameters may be given 16-bit gradients). A gradient of None leaves its parameter and moments as
+    they are. Parameters that share memory are refused.
+
+    ``step`` is the number of this update, from 1: an int, or an int64 tensor on the device that the caller advances (for
+    captured graphs, as ``lr`` may be an fp32 tensor). ``grad_scale`` (fp32 tensor, one element, such as the second result
+    of ``grad_norm``) multiplies the gradients; when it is not finite the call changes nothing.
+
+    In 8 bits a moment is held relative to the largest of its block of ``ADAMW_BLOCK`` elements: m with a sign and 3 bits of
+    mantissa, the root of v with 4, both over 15.9 octaves, rounded to nearest. The update uses the moments before they
+    are rounded. A value that is not finite spoils its whole block.
+    """
+    params, grads = _check_list("params", params), _check_list("grads", grads)
+    if len(params) != len(grads) or not params:
+        raise ValueError(f"params and grads must be lists of one length, got {len(params)} and {len(grads)}")
+    _check_dense("params", params)
+    blocks = _blocks(params)
+    have = _check_state(state)
+    if have != sum(blocks):
+        raise ValueError(f"state holds {have} blocks of {ADAMW_BLOCK} moments, params need {sum(blocks)}")
+    device = params[0].device
+    if state.exp_avg.device != device:
+        raise ValueError(f"state is on {state.exp_avg.device}, expected {device}")
+    first = list(accumulate(blocks, initial=0))
+    if any(g is None for g in grads) or 0 in blocks:
+        kept = [i for i, g in enumerate(grads) if g is not None and blocks[i]]
+        params, grads, first = [params[i] for i in kept], [grads[i] for i in kept], [first[i] for i in kept]
+    _check_dense("grads", grads)
+    if grads and grads[0].device != device:
+        raise ValueError(f"grads are on {grads[0].device}, expected {device}")
+    if list(map(torch.Tensor.size, params)) != list(map(torch.Tensor.size, grads)):
+        i = [p.shape == g.shape for p, g in zip(params, grads)].index(False)
+        raise ValueError(f"a gradient must have its parameter's shape {tuple(params[i].shape)}, got "
+                         f"{tuple(grads[i].shape)}")
+    if not (isinstance(betas, (tuple, list)) and len(betas) == 2):
+        raise ValueError(f"betas must be two numbers, got {betas!r}")
+    a = _lib.AdamWParams(0.0, _number("betas[0]", betas[0], 0, 1), _number("betas[1]", betas[1], 0, 1),
+                         _number("eps", eps, 0), _number("weight_decay", weight_decay, 0))
+    if isinstance(step, torch.Tensor):
+        _check_scalar("step", step, torch.int64, device)
+        a.step_device = step.data_ptr()
+    elif isinstance(step, int) and not isinstance(step, bool) and 1 <= step < 1 << 62:
+        a.step = step
+    else:
+        raise ValueError(f"step must be the update's number from 1 on, got {step!r}")
+    if isinstance(lr, torch.Tensor):
+        _check_scalar("lr", lr, torch.float32, device)
+        a.lr_device = lr.data_ptr()
+    else:
+        a.lr = _number("lr", lr, 0)
+    if grad_scale is not None:
+        _check_scalar("grad_scale", grad_scale, torch.float32, device)
+        a.grad_scale = grad_scale.data_ptr()
+    _check_cuda("params", state.exp_avg)
+    if not params:
+        return
+    bits = 32 if state.scales is None else 8
+    types = list(zip([p.dtype for p in params], [g.dtype for g in grads]))
+    kinds = set(types)
+    if len(kinds) > 1:  # within a kind the entry point checks
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes, t is p) for p, g in zip(params, grads) for t in (p, g))
+        written = seen = 0
+        for start, end, is_param in spans:
+            if start < (seen if is_param else written):
+                raise ValueError("params must not share memory with one another or with grads")
+            written, seen = max(written, end if is_param else 0), max(seen, end)
+    for kind in sorted(kinds, key=str):
+        pick = None if len(kinds) == 1 else [i for i, t in enumerate(types) if t == kind]
+        rows = [x if pick is None else [x[i] for i in pick] for x in (params, grads, first)]
+        table = _tensor_table(*rows)
+        n = len(rows[0])
+        _launch(state.exp_avg, "unblend_adamw_step", table.buffer_info()[0], n, state.exp_avg.data_ptr(),
+                state.exp_avg_sq.data_ptr(), _lib.ptr(state.scales), bits, _DTYPES[kind[0]], _DTYPES[kind[1]],
+                ctypes.byref(a), kernels=-(-n // _TABLE))
+    torch.autograd.graph.increment_version([*params, *(t for t in state if t is not None)])
+
+
+def _tensor_table(params: list | None, grads: list, first: list[int] | None = None) -> array:
+    """``UnblendAdamWTensor`` for each tensor."""
+    n = len(grads)
+    table = array("q", bytes(32 * n))
+    if params is not None:
+        table[0::4] = array("q", map(torch.Tensor.data_ptr, params))
+    table[1::4] = array("q", map(torch.Tensor.data_ptr, grads))
+    table[2::4] = array("q", map(torch.Tensor.numel, grads))
+    if first is not None:
+        table[3::4] = array("q", first[:n])
+    return table
+
+
+def adamw_moments(state: AdamWState) -> tuple[torch.Tensor, torch.Tensor]:
+    """The moments' values ``(exp_avg, exp_avg_sq)``, fp32, in the state's layout (32 bits: the state's own tensors)."""
+    blocks = _check_state(state)
+    if state.scales is None:
+        return state.exp_avg, state.exp_avg_sq
+    _check_cuda("state", state.exp_avg)
+    m, v = (_empty(state.exp_avg, torch.float32) for _ in range(2))
+    if blocks:
+        _launch(state.exp_avg, "unblend_adamw_values", state.exp_avg.data_ptr(), state.exp_avg_sq.data_ptr(),
+                state.scales.data_ptr(), m.data_ptr(), v.data_ptr(), blocks)
+    return m, v
+
+
+def adamw_views(params: Sequence[torch.Tensor], flat: torch.Tensor) -> list[torch.Tensor]:
+    """Views of each parameter's part of an array in the state's layout, in the parameter's shape."""
+    params = _check_list("params", params)
+    _check_dense("params", params)
+    blocks = _blocks(params)
+    if not isinstance(flat, torch.Tensor) or flat.dim() != 1 or flat.numel() != sum(blocks) * ADAMW_BLOCK:
+        raise ValueError(f"flat must have {sum(blocks) * ADAMW_BLOCK} elements in one axis")
+    return [x[:p.numel()].view(p.shape) for p, x in zip(params, flat.split([b * ADAMW_BLOCK for b in blocks]))]
+
+
+def grad_norm(grads: Sequence[torch.Tensor | None], max_norm: float | None = None
+              ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``(norm, scale)``: the 2-norm of all gradients together, and the factor that clips it to ``max_norm``.
+
+    Both are fp32 tensors of one element on the device (the host does not wait). Squares are summed in 64 bits. ``scale``
+    is ``min(1, max_norm / norm)``, NaN when the norm is not finite (``adamw_step`` then changes nothing), and None
+    without ``max_norm``. Gradients are contiguous fp32, bf16 or fp16 in any mixture; None counts for nothing.
+    """
+    grads = [g for g in _check_list("grads", grads) if g is not None]
+    _check_dense("grads", grads)
+    if not grads:
+        raise ValueError("grads must hold at least one tensor")
+    if max_norm is not None and not (_number("max_norm", max_norm, 0) > 0 and max_norm <= _F32_MAX):
+        raise ValueError(f"max_norm must be positive, got {max_norm!r}")
+    _check_cuda("grads", grads[0])
+    like = grads[0]
+    norm = like.new_empty((), dtype=torch.float32)
+    scale = None if max_norm is None else like.new_empty((), dtype=torch.float32)
+    if 0 in map(torch.Tensor.numel, grads):
+        grads = [g for g in grads if g.numel()]
+        if not grads:
+            return norm.zero_(), None if scale is None else scale.fill_(1.0)
+    types = [_DTYPES[g.dtype] for g in grads]
+    counts = [types.count(t) for t in range(3)]
+    if max(counts) < len(grads):
+        grads = [g for _, g in sorted(zip(types, grads), key=lambda x: x[0])]
+    table = _tensor_table(None, grads)
+    n = ctypes.c_longlong(0)
+    _lib.check("unblend_grad_norm_workspace", _lib.load().unblend_grad_norm_workspace(len(grads), ctypes.byref(n)))
+    work = _scratch(like, n.value)
+    _launch(like, "unblend_grad_norm", table.buffer_info()[0], (ctypes.c_int * 3)(*counts),
+            0.0 if max_norm is None else float(max_norm), norm.data_ptr(), _lib.ptr(scale), work.data_ptr(),
+            kernels=1 + sum(-(-c // _TABLE) for c in counts))
+    return norm, scale
