@@ -275,6 +275,31 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_tensor_lists = None
+
+
+def tensor_lists():
+    """The Python extension that reads lists of tensors (loaded once)."""
+    global _tensor_lists
+    if _tensor_lists is None:
+        import importlib.util
+
+        from .build import EXTENSION
+
+        path = os.path.join(os.path.dirname(LIB_PATH), EXTENSION + ".so")
+        load()
+        if not os.path.exists(path):
+            raise RuntimeError(f"unblend_b200 extension not built ({path}); run `python -m unblend_b200.build`")
+        spec = importlib.util.spec_from_file_location(EXTENSION, path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        if module.torch_version != torch.__version__.split("+")[0]:
+            raise RuntimeError(f"{path} was built for torch {module.torch_version}, this is {torch.__version__}; run "
+                               "`python -m unblend_b200.build`")
+        _tensor_lists = module
+    return _tensor_lists
+
+
 def exported_symbols() -> list[str]:
     """Entry points this binding declares (all must exist in the library)."""
     return list(_SIGNATURES) + list(_HOST_SIGNATURES)

@@ -2,8 +2,8 @@
 
 Every ``csrc/*.cu`` file is compiled with ``nvcc -gencode
 arch=compute_100a,code=sm_100a`` and linked into one C-ABI shared library that
-the host code loads with ctypes. Objects are rebuilt only when a source or
-header is newer. The FFT twiddle table (``csrc/twiddle4096.inc``) is generated
+the host code loads with ctypes, and ``csrc/tensor_lists.cpp`` into a Python extension
+beside it. Objects are rebuilt only when a source or header is newer. The FFT twiddle table (``csrc/twiddle4096.inc``) is generated
 here in double precision, so the kernels hold it as static module data.
 
 Usage: ``python -m unblend_b200.build [-j N] [--force]``.
@@ -66,7 +66,7 @@ def source_digest() -> str:
     import hashlib
 
     files = []
-    for pat in ("*.cu", "*.cuh", "*.inc"):
+    for pat in ("*.cu", "*.cuh", "*.inc", "*.cpp"):
         files += glob.glob(os.path.join(CSRC, pat))
     files += glob.glob(os.path.join(INCLUDE, "*.h"))
     h = hashlib.sha256()
@@ -75,6 +75,33 @@ def source_digest() -> str:
         with open(f, "rb") as fh:
             h.update(fh.read())
     return h.hexdigest()
+
+
+EXTENSION = "tensor_lists"
+
+
+def _extension(force: bool) -> None:
+    """The Python extension, against the headers of the installed torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    src, out = os.path.join(CSRC, EXTENSION + ".cpp"), os.path.join(LIBDIR, EXTENSION + ".so")
+    stamp = out + ".torch"  # another torch needs another build
+    if not force and os.path.exists(out) and os.path.exists(stamp) and open(stamp).read() == torch.__version__ and \
+            os.path.getmtime(out) >= max(os.path.getmtime(src), _deps()):
+        return
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f for p in include_paths() for f in ("-isystem", p)), "-isystem", sysconfig.get_path("include"),
+           src, "-o", out + ".tmp", *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{res.stderr}")
+    os.replace(out + ".tmp", out)
+    with open(stamp, "w") as f:
+        f.write(torch.__version__)
 
 
 DIGEST_NAME = "libunblend_b200.digest"
@@ -106,7 +133,9 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False) -> str:
     sources = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     log: list = []
     with ThreadPoolExecutor(max_workers=jobs) as ex:
+        extension = ex.submit(_extension, force)
         objs = list(ex.map(lambda s: _compile(s, force, log), sources))
+        extension.result()
     lib = os.path.join(LIBDIR, LIBNAME)
     if force or not os.path.exists(lib) or os.path.getmtime(lib) < max(os.path.getmtime(o) for o in objs):
         cmd = [nvcc(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", *objs, "-o", lib + ".tmp", "-lcuda"]

@@ -25,10 +25,8 @@ from __future__ import annotations
 
 import ctypes
 import math
-from array import array
 from collections.abc import Sequence
 from functools import lru_cache
-from itertools import accumulate
 from typing import NamedTuple
 
 import torch
@@ -40,7 +38,7 @@ _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch
 MAX_HEAD_DIM = 128
 MAX_ROTARY_DIM = 256
 ADAMW_BLOCK = 256  # elements of a moment that share a scale in 8 bits; each parameter starts a block of its own
-_TABLE = 896  # tensors of one launch
+_TABLE, _TABLE_ROW = 896, 32  # tensors of one launch; bytes of UnblendAdamWTensor
 _F32_MAX = torch.finfo(torch.float32).max
 _REGISTER_COLS = 8192  # widest rows whose layer norm sums the weights' gradients beside the input's
 _MOST = 1 << 31  # rows, and columns, of layer norm and dropout-add
@@ -929,38 +927,21 @@ def _check_list(name: str, tensors) -> list:
         raise ValueError(f"{name} must be a list of tensors, got {type(tensors).__name__}") from None
 
 
-def _check_dense(name: str, tensors: list) -> None:
-    """Contiguous tensors of known types on one device (whole-list passes: models have hundreds of parameters)."""
-    if not all(isinstance(t, torch.Tensor) for t in tensors):
-        raise ValueError(f"{name} must hold tensors only")
-    if any(t.layout != torch.strided for t in tensors):
-        raise ValueError(f"{name} must be dense tensors")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
-        i = [t.is_contiguous() for t in tensors].index(False)
-        raise ValueError(f"{name}[{i}] must be contiguous, got shape {tuple(tensors[i].shape)} with strides "
-                         f"{tensors[i].stride()}")
-    if len(set(map(torch.Tensor.get_device, tensors))) > 1:
-        raise ValueError(f"{name} must be on one device")
-    for t in {t.dtype for t in tensors}:
-        if t not in _DTYPES:
-            raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t}")
-    if any(map(torch.Tensor.is_neg, tensors)):
-        raise ValueError(f"{name} holds a lazily negated view: give its resolve_neg()")
-
-
-def _blocks(tensors: list) -> list[int]:
-    return [-(-n // ADAMW_BLOCK) for n in map(torch.Tensor.numel, tensors)]
+def _sizes_of(params) -> tuple[list, list[int], list[int]]:
+    """Checked parameters, their numbers of elements and of blocks."""
+    params = _check_list("params", params)
+    sizes = _lib.tensor_lists().sizes("params", params)
+    return params, sizes, [-(-n // ADAMW_BLOCK) for n in sizes]
 
 
 def adamw_state(params: Sequence[torch.Tensor], bits: int = 32) -> AdamWState:
     """Moments of zeros for ``params``, in 32 or 8 bits."""
-    params = _check_list("params", params)
-    _check_dense("params", params)
+    params, _, blocks = _sizes_of(params)
     if bits not in (32, 8):
         raise ValueError(f"bits must be 32 or 8, got {bits!r}")
     if not params:
         raise ValueError("params must hold at least one tensor")
-    n = sum(_blocks(params))
+    n = sum(blocks)
     dev = params[0].device
     t = torch.float32 if bits == 32 else torch.uint8
     return AdamWState(torch.zeros(n * ADAMW_BLOCK, dtype=t, device=dev), torch.zeros(n * ADAMW_BLOCK, dtype=t, device=dev),
@@ -1021,27 +1002,15 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     are rounded. A value that is not finite spoils its whole block.
     """
     params, grads = _check_list("params", params), _check_list("grads", grads)
-    if len(params) != len(grads) or not params:
-        raise ValueError(f"params and grads must be lists of one length, got {len(params)} and {len(grads)}")
-    _check_dense("params", params)
-    blocks = _blocks(params)
+    table, kinds, blocks = _lib.tensor_lists().table(params, grads)
+    if not params:
+        raise ValueError("params must hold at least one tensor")
     have = _check_state(state)
-    if have != sum(blocks):
-        raise ValueError(f"state holds {have} blocks of {ADAMW_BLOCK} moments, params need {sum(blocks)}")
+    if have != blocks:
+        raise ValueError(f"state holds {have} blocks of {ADAMW_BLOCK} moments, params need {blocks}")
     device = params[0].device
     if state.exp_avg.device != device:
         raise ValueError(f"state is on {state.exp_avg.device}, expected {device}")
-    first = list(accumulate(blocks, initial=0))
-    if any(g is None for g in grads) or 0 in blocks:
-        kept = [i for i, g in enumerate(grads) if g is not None and blocks[i]]
-        params, grads, first = [params[i] for i in kept], [grads[i] for i in kept], [first[i] for i in kept]
-    _check_dense("grads", grads)
-    if grads and grads[0].device != device:
-        raise ValueError(f"grads are on {grads[0].device}, expected {device}")
-    if list(map(torch.Tensor.size, params)) != list(map(torch.Tensor.size, grads)):
-        i = [p.shape == g.shape for p, g in zip(params, grads)].index(False)
-        raise ValueError(f"a gradient must have its parameter's shape {tuple(params[i].shape)}, got "
-                         f"{tuple(grads[i].shape)}")
     if not (isinstance(betas, (tuple, list)) and len(betas) == 2):
         raise ValueError(f"betas must be two numbers, got {betas!r}")
     a = _lib.AdamWParams(0.0, _number("betas[0]", betas[0], 0, 1), _number("betas[1]", betas[1], 0, 1),
@@ -1062,40 +1031,26 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
         _check_scalar("grad_scale", grad_scale, torch.float32, device)
         a.grad_scale = grad_scale.data_ptr()
     _check_cuda("params", state.exp_avg)
-    if not params:
-        return
-    bits = 32 if state.scales is None else 8
-    types = list(zip([p.dtype for p in params], [g.dtype for g in grads]))
-    kinds = set(types)
     if len(kinds) > 1:  # within a kind the entry point checks
-        spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes, t is p) for p, g in zip(params, grads) for t in (p, g))
-        written = seen = 0
-        for start, end, is_param in spans:
-            if start < (seen if is_param else written):
-                raise ValueError("params must not share memory with one another or with grads")
-            written, seen = max(written, end if is_param else 0), max(seen, end)
-    for kind in sorted(kinds, key=str):
-        pick = None if len(kinds) == 1 else [i for i, t in enumerate(types) if t == kind]
-        rows = [x if pick is None else [x[i] for i in pick] for x in (params, grads, first)]
-        table = _tensor_table(*rows)
-        n = len(rows[0])
-        _launch(state.exp_avg, "unblend_adamw_step", table.buffer_info()[0], n, state.exp_avg.data_ptr(),
-                state.exp_avg_sq.data_ptr(), _lib.ptr(state.scales), bits, _DTYPES[kind[0]], _DTYPES[kind[1]],
-                ctypes.byref(a), kernels=-(-n // _TABLE))
-    torch.autograd.graph.increment_version([*params, *(t for t in state if t is not None)])
+        _check_apart(params, grads)
+    bits = 32 if state.scales is None else 8
+    at = ctypes.cast(ctypes.c_char_p(table), ctypes.c_void_p).value
+    for t, tg, n in kinds:
+        _launch(state.exp_avg, "unblend_adamw_step", at, n, state.exp_avg.data_ptr(), state.exp_avg_sq.data_ptr(),
+                _lib.ptr(state.scales), bits, t, tg, ctypes.byref(a), kernels=-(-n // _TABLE))
+        at += n * _TABLE_ROW
+    _lib.tensor_lists().changed(params, grads)  # autograd refuses to use what it saved of them before
+    torch.autograd.graph.increment_version([t for t in state if t is not None])
 
 
-def _tensor_table(params: list | None, grads: list, first: list[int] | None = None) -> array:
-    """``UnblendAdamWTensor`` for each tensor."""
-    n = len(grads)
-    table = array("q", bytes(32 * n))
-    if params is not None:
-        table[0::4] = array("q", map(torch.Tensor.data_ptr, params))
-    table[1::4] = array("q", map(torch.Tensor.data_ptr, grads))
-    table[2::4] = array("q", map(torch.Tensor.numel, grads))
-    if first is not None:
-        table[3::4] = array("q", first[:n])
-    return table
+def _check_apart(params: list, grads: list) -> None:
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes, t is p) for p, g in zip(params, grads) if g is not None
+                   for t in (p, g) if t.numel())
+    written = seen = 0
+    for start, end, is_param in spans:
+        if start < (seen if is_param else written):
+            raise ValueError("params must not share memory with one another or with grads")
+        written, seen = max(written, end if is_param else 0), max(seen, end)
 
 
 def adamw_moments(state: AdamWState) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1113,12 +1068,11 @@ def adamw_moments(state: AdamWState) -> tuple[torch.Tensor, torch.Tensor]:
 
 def adamw_views(params: Sequence[torch.Tensor], flat: torch.Tensor) -> list[torch.Tensor]:
     """Views of each parameter's part of an array in the state's layout, in the parameter's shape."""
-    params = _check_list("params", params)
-    _check_dense("params", params)
-    blocks = _blocks(params)
+    params, sizes, blocks = _sizes_of(params)
     if not isinstance(flat, torch.Tensor) or flat.dim() != 1 or flat.numel() != sum(blocks) * ADAMW_BLOCK:
         raise ValueError(f"flat must have {sum(blocks) * ADAMW_BLOCK} elements in one axis")
-    return [x[:p.numel()].view(p.shape) for p, x in zip(params, flat.split([b * ADAMW_BLOCK for b in blocks]))]
+    parts = flat.split([b * ADAMW_BLOCK for b in blocks])
+    return [x[:n].view(p.shape) for p, n, x in zip(params, sizes, parts)]
 
 
 def grad_norm(grads: Sequence[torch.Tensor | None], max_norm: float | None = None
@@ -1129,29 +1083,25 @@ def grad_norm(grads: Sequence[torch.Tensor | None], max_norm: float | None = Non
     is ``min(1, max_norm / norm)``, NaN when the norm is not finite (``adamw_step`` then changes nothing), and None
     without ``max_norm``. Gradients are contiguous fp32, bf16 or fp16 in any mixture; None counts for nothing.
     """
-    grads = [g for g in _check_list("grads", grads) if g is not None]
-    _check_dense("grads", grads)
-    if not grads:
+    grads = _check_list("grads", grads)
+    table, kinds, _ = _lib.tensor_lists().table(None, grads)
+    like = next((g for g in grads if g is not None), None)
+    if like is None:
         raise ValueError("grads must hold at least one tensor")
     if max_norm is not None and not (_number("max_norm", max_norm, 0) > 0 and max_norm <= _F32_MAX):
         raise ValueError(f"max_norm must be positive, got {max_norm!r}")
-    _check_cuda("grads", grads[0])
-    like = grads[0]
+    _check_cuda("grads", like)
     norm = like.new_empty((), dtype=torch.float32)
     scale = None if max_norm is None else like.new_empty((), dtype=torch.float32)
-    if 0 in map(torch.Tensor.numel, grads):
-        grads = [g for g in grads if g.numel()]
-        if not grads:
-            return norm.zero_(), None if scale is None else scale.fill_(1.0)
-    types = [_DTYPES[g.dtype] for g in grads]
-    counts = [types.count(t) for t in range(3)]
-    if max(counts) < len(grads):
-        grads = [g for _, g in sorted(zip(types, grads), key=lambda x: x[0])]
-    table = _tensor_table(None, grads)
+    if not kinds:
+        return norm.zero_(), None if scale is None else scale.fill_(1.0)
+    counts = (ctypes.c_int * 3)()
+    for _, t, n in kinds:
+        counts[t] = n
+    total = sum(counts)
     n = ctypes.c_longlong(0)
-    _lib.check("unblend_grad_norm_workspace", _lib.load().unblend_grad_norm_workspace(len(grads), ctypes.byref(n)))
+    _lib.check("unblend_grad_norm_workspace", _lib.load().unblend_grad_norm_workspace(total, ctypes.byref(n)))
     work = _scratch(like, n.value)
-    _launch(like, "unblend_grad_norm", table.buffer_info()[0], (ctypes.c_int * 3)(*counts),
-            0.0 if max_norm is None else float(max_norm), norm.data_ptr(), _lib.ptr(scale), work.data_ptr(),
-            kernels=1 + sum(-(-c // _TABLE) for c in counts))
+    _launch(like, "unblend_grad_norm", table, counts, 0.0 if max_norm is None else float(max_norm), norm.data_ptr(),
+            _lib.ptr(scale), work.data_ptr(), kernels=1 + sum(-(-c // _TABLE) for c in counts))
     return norm, scale
