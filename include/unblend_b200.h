@@ -719,7 +719,8 @@ typedef struct {
 
 /*
  * m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
- * p = (1 - lr weight_decay) p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps).
+ * p = (1 - lr weight_decay) p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps); eps is 0
+ * or between 2^-126 and 1e30.
  * bits 32: exp_avg and exp_avg_sq are float, whole blocks of 256 per tensor. bits 8: uint8 codes, and scales holds two
  * floats per block, the largest |m| and the largest u = sqrt(v). With c = code & 127 a code of exp_avg stands for the
  * float of the bit pattern (c + 889) << 20 (0 for c = 0) times the first scale, negative with bit 7; a code of exp_avg_sq

@@ -132,3 +132,22 @@ def test_param_struct_layout(tmp_path):
     from test_capi import test_param_struct_layout_matches_c
 
     test_param_struct_layout_matches_c(tmp_path, _lib.RotaryParams, "UnblendRotaryParams")
+
+
+def test_packed_parameters():
+    """The bytes that the calls pass are the structure's."""
+    assert training._ROTARY_PARAMS.size == ctypes.sizeof(_lib.RotaryParams)
+    q, k = torch.zeros(2, 3, 5, 4, 16)[:, 1:], torch.zeros(2, 2, 5, 2, 18)[..., :16]
+    f, pos, w = torch.ones(8, dtype=torch.float64), torch.zeros(2, 2, 5, dtype=torch.int64), torch.ones(16)
+    lens = torch.zeros(4, dtype=torch.int32)
+    p, held = training._rotary_params(q, k, f, pos, False, 0.5, k, q, w, None, 1e-3, lens)
+    p = _lib.RotaryParams.from_buffer_copy(p)
+    got = {n: getattr(p, n) for n, _ in p._fields_ if n not in ("q", "k", "q0", "k0")}
+    assert got.pop("eps") == pytest.approx(1e-3)
+    assert got == dict(dtype=0, outer=2, inner=2, length=5, heads=4, k_heads=2, hd=16, pairs=8, half=1, scale=0.5,
+                       freqs=f.data_ptr(), freqs_f64=1, positions_i64=1, positions=pos.data_ptr(), positions_stride=5,
+                       gamma_q=w.data_ptr(), gamma_k=None, w_dtype=0, lens=lens.data_ptr())
+    strides = [tuple(getattr(getattr(p, n), m) for m in ("outer", "inner", "row", "head"))
+               for n in ("q", "k", "q0", "k0")]
+    assert strides == [(960, 320, 64, 16), (360, 180, 36, 18), (360, 180, 36, 18), (960, 320, 64, 16)]
+    assert training._rotary_workspace_bytes(bytes(p)[:training._ROTARY_SIZES]) >= 2 * 16 * 4

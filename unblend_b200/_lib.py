@@ -211,10 +211,11 @@ _SIGNATURES = {
                            ctypes.POINTER(AdamWParams), c_void_p],
     "unblend_adamw_values": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p],
     "unblend_grad_norm": [c_void_p, ctypes.POINTER(c_int), c_float, c_void_p, c_void_p, c_void_p, c_void_p],
-    "unblend_rotary": [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(RotaryParams), c_int, c_void_p],
-    "unblend_qk_norm_rotary_forward": [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(RotaryParams), c_void_p],
+    # The parameters may be a RotaryParams by reference or its bytes.
+    "unblend_rotary": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
+    "unblend_qk_norm_rotary_forward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "unblend_qk_norm_rotary_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                        c_void_p, ctypes.POINTER(RotaryParams), c_void_p],
+                                        c_void_p, c_void_p, c_void_p],
 }
 
 # Entry points without a stream argument.

@@ -60,74 +60,102 @@ struct StepArgs {
   const long long* step;  // device: the bias corrections and factors below are computed from it
   const float* lr;        // device
   double b1d, b2d, lrd, wdd;
-  float b1, c1, b2, c2, eps;
+  float b1, c1, b2, c2, eps, one;
   float decay, size, root;  // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
 };
 
-// The smallest code's patterns: 2^-16 * 1.25 and 2^-16 * 1.125 are code 1.
+// A code of m is bits 20 .. 26 of the pattern minus M_LOW (code 1 is 2^-16 * 1.25), one of u bits 19 .. 26 minus U_LOW (code
+// 1 is 2^-16 * 1.125); the patterns' own places are kept until four codes are packed into a word.
 constexpr unsigned M_SHIFT = 20, M_LOW = (127u << 3) - 127u, U_SHIFT = 19, U_LOW = (127u << 4) - 255u;
-constexpr float M_LEAST = 0.625f / 65536.f;  // half of code 1
+constexpr unsigned M_LEAST = 0x37200000u;  // 0.625 * 2^-16, half of code 1
 
-__device__ __forceinline__ float m_value(unsigned code) {
-  const unsigned c = code & 127u;
-  const float v = c ? __uint_as_float((c + M_LOW) << M_SHIFT) : 0.f;
-  return code & 128u ? -v : v;
+// The value of code I of four, relative to its scale.
+template <int I>
+__device__ __forceinline__ float m_value(unsigned w) {
+  const unsigned x = I < 3 ? w << (20 - 8 * I) : w >> 4;  // the code at bits 20 .. 26, its sign at 27
+  const unsigned c = x & (127u << M_SHIFT);
+  const unsigned v = c ? c + (M_LOW << M_SHIFT) : 0u;
+  return __uint_as_float(v | (x << 4 & 0x80000000u));
 }
-__device__ __forceinline__ float u_value(unsigned code) {
-  return code ? __uint_as_float((code + U_LOW) << U_SHIFT) : 0.f;
+template <int I>
+__device__ __forceinline__ float u_value(unsigned w) {
+  const unsigned c = (I < 3 ? w << (19 - 8 * I) : w >> 5) & (255u << U_SHIFT);
+  return __uint_as_float(c ? c + (U_LOW << U_SHIFT) : 0u);
 }
 
-template <unsigned SHIFT>
-__device__ __forceinline__ int leading(float r) {  // the pattern's leading bits, to nearest even
-  const unsigned w = __float_as_uint(r);
-  return (int)((w + ((1u << (SHIFT - 1)) - 1u) + ((w >> SHIFT) & 1u)) >> SHIFT);
+// Codes of magnitudes relative to their block's largest, in the highest byte (the bits below are not cleared). The pattern
+// is rounded to nearest even by adding just less than half a step, and the lowest bit that stays.
+template <unsigned SHIFT, unsigned LOW>
+__device__ __forceinline__ int leading(unsigned mag) {
+  return (int)(mag + (mag >> SHIFT & 1u) + ((1u << (SHIFT - 1)) - 1u - (LOW << SHIFT)));
 }
-__device__ __forceinline__ unsigned m_code(float m, float inv) {
-  const float r = __fmul_rn(fabsf(m), inv);
-  const int c = min(max(leading<M_SHIFT>(r) - (int)M_LOW, 1), 127);
-  return (r > M_LEAST ? (unsigned)c : 0u) | (m < 0.f ? 128u : 0u);
+__device__ __forceinline__ unsigned m_code(float r) {
+  const unsigned w = __float_as_uint(r), mag = w & 0x7fffffffu;
+  const int least = mag > M_LEAST ? 1 << M_SHIFT : 0;
+  const unsigned c = (unsigned)max(leading<M_SHIFT, M_LOW>(mag), least) << 4;
+  return (c & 0x7fffffffu) | (w & 0x80000000u);
 }
-__device__ __forceinline__ unsigned u_code(float u, float inv) {
-  const float r = __fmul_rn(u, inv);
-  return r > 0.f ? (unsigned)min(max(leading<U_SHIFT>(r) - (int)U_LOW, 1), 255) : 0u;
+__device__ __forceinline__ unsigned u_code(float r) {
+  const unsigned mag = __float_as_uint(r);
+  const int least = mag ? 1 << U_SHIFT : 0;
+  return (unsigned)max(leading<U_SHIFT, U_LOW>(mag), least) << 5;
 }
+__device__ __forceinline__ unsigned high_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+
+// Largest magnitude of three, NaN if one is.
+__device__ __forceinline__ float top3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 1 / x to within an ulp for normal x.
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // 1 / top, 0 for a block of zeros (or below the normal range, where 1 / top could overflow).
 __device__ __forceinline__ float inverse(float top) { return top >= 1.17549435e-38f ? __frcp_rn(top) : 0.f; }
 
 // Four consecutive elements; without `full`, those below n.
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&v)[4], bool full, int n) {
+__device__ __forceinline__ void load4(const T* p, float2 (&v)[2], bool full, int n) {
   if (full) {
     if constexpr (sizeof(T) == 4) {
       const float4 w = *reinterpret_cast<const float4*>(p);
-      v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+      v[0] = make_float2(w.x, w.y), v[1] = make_float2(w.z, w.w);
     } else {
-      alignas(8) T raw[4];
-      *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = to_f(raw[i]);
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      float2 u[4];
+      unpack16(make_uint4(w.x, w.y, 0u, 0u), u, T());
+      v[0] = u[0], v[1] = u[1];
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? to_f(p[i]) : 0.f;
+    v[0] = make_float2(n > 0 ? to_f(p[0]) : 0.f, n > 1 ? to_f(p[1]) : 0.f);
+    v[1] = make_float2(n > 2 ? to_f(p[2]) : 0.f, n > 3 ? to_f(p[3]) : 0.f);
   }
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* p, const float (&v)[4], bool full, int n) {
+__device__ __forceinline__ void store4(T* p, const float2 (&v)[2], bool full, int n) {
   if (full) {
     if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
     } else {
-      alignas(8) T raw[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) raw[i] = from_f<T>(v[i]);
-      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(raw);
+      const float2 u[4] = {v[0], v[1], both(0.f), both(0.f)};
+      const uint4 w = pack16(u, T());
+      *reinterpret_cast<uint2*>(p) = make_uint2(w.x, w.y);
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) p[i] = from_f<T>(v[i]);
+    if (n > 0) p[0] = from_f<T>(v[0].x);
+    if (n > 1) p[1] = from_f<T>(v[0].y);
+    if (n > 2) p[2] = from_f<T>(v[1].x);
+    if (n > 3) p[3] = from_f<T>(v[1].y);
   }
 }
 
@@ -167,7 +195,7 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
     const long long block = tab.t[k].block + local;
     const bool full = left >= BLOCK && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 &&
                       reinterpret_cast<uintptr_t>(g) % (4 * sizeof(TG)) == 0;
-    float pv[2][4], gv[2][4], mv[2][4], uv[2][4];
+    float2 pv[2][2], gv[2][2], mv[2][2], uv[2][2];  // uv: v, and in 8 bits u once the codes are read
     unsigned mc[2], uc[2];
     float2 sc;
     const long long at = block * BLOCK + lane * 4;
@@ -191,30 +219,35 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
         load4(static_cast<const float*>(a.v) + at + j * 128, uv[j], true, 4);
       }
     }
+    if constexpr (EIGHT) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        mv[j][0] = mul2(make_float2(m_value<0>(mc[j]), m_value<1>(mc[j])), both(sc.x));
+        mv[j][1] = mul2(make_float2(m_value<2>(mc[j]), m_value<3>(mc[j])), both(sc.x));
+        uv[j][0] = mul2(make_float2(u_value<0>(uc[j]), u_value<1>(uc[j])), both(sc.y));
+        uv[j][1] = mul2(make_float2(u_value<2>(uc[j]), u_value<3>(uc[j])), both(sc.y));
+      }
+    }
     float top_m = 0.f, top_u = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float gr = __fmul_rn(gv[j][i], gs);
-        float m, v;
-        if constexpr (EIGHT) {
-          m = __fmul_rn(m_value((mc[j] >> (8 * i)) & 255u), sc.x);
-          const float u = __fmul_rn(u_value((uc[j] >> (8 * i)) & 255u), sc.y);
-          v = __fmul_rn(u, u);
-        } else {
-          m = mv[j][i], v = uv[j][i];
-        }
-        m = __fadd_rn(__fmul_rn(m, a.b1), __fmul_rn(gr, a.c1));
-        v = __fadd_rn(__fmul_rn(v, a.b2), __fmul_rn(__fmul_rn(gr, gr), a.c2));
-        const float u = __fsqrt_rn(v);
-        pv[j][i] = pv[j][i] * decay - size * (m / (u * root + a.eps));
+      for (int i = 0; i < 2; ++i) {
+        const float2 gr = mul2(gv[j][i], both(gs));
+        float2 m = mv[j][i], v = uv[j][i];
+        if (EIGHT) v = mul2(v, v);
+        // Sums as fma with a factor of 1 that the compiler does not know: it would fuse a packed product into them.
+        m = ub::fma2(mul2(m, both(a.b1)), both(a.one), mul2(gr, both(a.c1)));
+        v = ub::fma2(mul2(v, both(a.b2)), both(a.one), mul2(mul2(gr, gr), both(a.c2)));
+        const float2 u = make_float2(__fsqrt_rn(v.x), __fsqrt_rn(v.y));
+        const float2 denom = ub::fma2(u, both(root), both(a.eps));
+        const float2 step = mul2(m, make_float2(reciprocal(denom.x), reciprocal(denom.y)));
+        pv[j][i] = ub::fma2(step, both(-size), mul2(pv[j][i], both(decay)));
         mv[j][i] = m;
         uv[j][i] = EIGHT ? u : v;
         if constexpr (EIGHT) {
-          // by patterns, as a NaN has to come through
-          top_m = __uint_as_float(max(__float_as_uint(top_m), __float_as_uint(fabsf(m))));
-          top_u = __uint_as_float(max(__float_as_uint(top_u), __float_as_uint(u) & 0x7fffffffu));
+          top_m = top3(top_m, m.x, m.y);
+          top_u = top3(top_u, u.x, u.y);
         }
       }
 #pragma unroll
@@ -230,14 +263,12 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
       const float inv_m = inverse(top_m), inv_u = inverse(top_u);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        unsigned cm = 0, cu = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          cm |= m_code(mv[j][i], inv_m) << (8 * i);
-          cu |= u_code(uv[j][i], inv_u) << (8 * i);
-        }
-        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.m) + at + j * 128) = cm;
-        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.v) + at + j * 128) = cu;
+        const float2 m0 = mul2(mv[j][0], both(inv_m)), m1 = mul2(mv[j][1], both(inv_m));
+        const float2 u0 = mul2(uv[j][0], both(inv_u)), u1 = mul2(uv[j][1], both(inv_u));
+        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.m) + at + j * 128) =
+            high_bytes(m_code(m0.x), m_code(m0.y), m_code(m1.x), m_code(m1.y));
+        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.v) + at + j * 128) =
+            high_bytes(u_code(u0.x), u_code(u0.y), u_code(u1.x), u_code(u1.y));
       }
       if (lane == 0) a.scales[block] = make_float2(top_m, top_u);
     }
@@ -254,13 +285,11 @@ __global__ void __launch_bounds__(THREADS) adamw_values_kernel(const uint8_t* m,
     for (int j = 0; j < 2; ++j) {
       const long long at = (long long)b * BLOCK + lane * 4 + j * 128;
       const unsigned mc = *reinterpret_cast<const unsigned*>(m + at), uc = *reinterpret_cast<const unsigned*>(u + at);
-      float mv[4], vv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mv[i] = __fmul_rn(m_value((mc >> (8 * i)) & 255u), sc.x);
-        const float w = __fmul_rn(u_value((uc >> (8 * i)) & 255u), sc.y);
-        vv[i] = __fmul_rn(w, w);
-      }
+      const float2 mv[2] = {mul2(make_float2(m_value<0>(mc), m_value<1>(mc)), both(sc.x)),
+                            mul2(make_float2(m_value<2>(mc), m_value<3>(mc)), both(sc.x))};
+      const float2 u0 = mul2(make_float2(u_value<0>(uc), u_value<1>(uc)), both(sc.y));
+      const float2 u1 = mul2(make_float2(u_value<2>(uc), u_value<3>(uc)), both(sc.y));
+      const float2 vv[2] = {mul2(u0, u0), mul2(u1, u1)};
       store4(m_out + at, mv, true, 4);
       store4(v_out + at, vv, true, 4);
     }
@@ -437,13 +466,16 @@ int launch_squares(const UnblendAdamWTensor* t, int count, double* part, int* us
 
 }  // namespace
 
+// The update multiplies by an approximate reciprocal, which takes normal numbers only; the root of v is 0 or above 2^-75.
+static bool eps_ok(double eps) { return eps == 0 || (eps >= 1.17549435e-38 && eps <= 1e30); }
+
 extern "C" int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, void* exp_avg, void* exp_avg_sq,
                                   float* scales, int bits, int dtype, int grad_dtype, const UnblendAdamWParams* p,
                                   void* stream) {
   UB_REQUIRE(p && known_type(dtype) && known_type(grad_dtype) && (bits == 32 || bits == 8));
   UB_REQUIRE(exp_avg && exp_avg_sq && aligned16(exp_avg) && aligned16(exp_avg_sq));
   UB_REQUIRE(bits == 32 || (scales && reinterpret_cast<uintptr_t>(scales) % 8 == 0));
-  UB_REQUIRE(p->beta1 >= 0 && p->beta1 < 1 && p->beta2 >= 0 && p->beta2 < 1 && p->eps >= 0 && std::isfinite(p->eps));
+  UB_REQUIRE(p->beta1 >= 0 && p->beta1 < 1 && p->beta2 >= 0 && p->beta2 < 1 && eps_ok(p->eps));
   UB_REQUIRE(std::isfinite(p->weight_decay) && (p->lr_device || std::isfinite(p->lr)));
   UB_REQUIRE(p->step_device || p->step >= 1);
   UB_REQUIRE(reinterpret_cast<uintptr_t>(p->step_device) % 8 == 0 && reinterpret_cast<uintptr_t>(p->lr_device) % 4 == 0 &&
@@ -470,6 +502,7 @@ extern "C" int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, 
   a.b2 = (float)p->beta2;
   a.c2 = (float)(1.0 - p->beta2);
   a.eps = (float)p->eps;
+  a.one = 1.f;
   const double t = p->step_device ? 1.0 : (double)p->step;
   const double correction = 1.0 - std::pow(p->beta1, t);
   a.decay = (float)(1.0 - p->lr * p->weight_decay);

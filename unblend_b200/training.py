@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from collections.abc import Sequence
 from functools import lru_cache
 from typing import NamedTuple
@@ -37,6 +38,11 @@ from . import _lib
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 MAX_HEAD_DIM = 128
 MAX_ROTARY_DIM = 256
+_FREQ_DTYPES = (torch.float32, torch.float64)
+_POSITION_DTYPES = (torch.int32, torch.int64)
+# UnblendRotaryParams: packed here, as building the ctypes structure takes four times as long.
+_ROTARY_PARAMS = struct.Struct("@9if P2i P17q 2Pif P")
+_ROTARY_SIZES = _lib.RotaryParams.scale.offset  # bytes of the fields that say how large a call is
 ADAMW_BLOCK = 256  # elements of a moment that share a scale in 8 bits; each parameter starts a block of its own
 _TABLE, _TABLE_ROW = 896, 32  # tensors of one launch; bytes of UnblendAdamWTensor
 _F32_MAX = torch.finfo(torch.float32).max
@@ -499,57 +505,93 @@ def rotary_freqs(dims: int, base: float = 10000.0, factor: float = 1.0, method: 
 
 def _check_rotary(q, k, freqs, positions, scale, eps: float = 0.0) -> float:
     _check_heads("q", q)
+    shape = q.shape
+    rows, hd = shape[:-2], shape[-1]
     if k is not None:
         _check_heads("k", k, q)
-        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
-            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree but for their heads")
-    hd = q.shape[-1]
+        if k.shape[:-2] != rows or k.shape[-1] != hd:
+            raise ValueError(f"q {tuple(shape)} and k {tuple(k.shape)} must agree but for their heads")
     if not 1 <= hd <= MAX_ROTARY_DIM:
         raise ValueError(f"head_dim must be 1 to {MAX_ROTARY_DIM}, got {hd}")
     if freqs is not None:
-        if not isinstance(freqs, torch.Tensor) or freqs.dtype not in (torch.float32, torch.float64) or \
-                freqs.dim() != 1 or freqs.device != q.device:
+        if not isinstance(freqs, torch.Tensor) or freqs.dtype not in _FREQ_DTYPES or freqs.dim() != 1 or \
+                freqs.device != q.device:
             raise ValueError(f"freqs must be a float32 or float64 tensor [pairs] on {q.device}")
-        if 2 * freqs.shape[0] > hd:
-            raise ValueError(f"{freqs.shape[0]} pairs do not fit into head_dim {hd}")
+        if 2 * freqs.numel() > hd:
+            raise ValueError(f"{freqs.numel()} pairs do not fit into head_dim {hd}")
         if freqs.is_neg():
             raise ValueError("freqs is a lazily negated view: give freqs.resolve_neg()")
         if freqs.requires_grad and torch.is_grad_enabled():
             raise ValueError("freqs has no gradient here: give freqs.detach()")
     if positions is not None:
-        if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64) or \
+        if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_DTYPES or \
                 positions.device != q.device:
             raise ValueError(f"positions must be an int32 or int64 tensor on {q.device}")
-        if positions.shape not in (q.shape[:-2], q.shape[-3:-2]):
-            raise ValueError(f"positions must have shape {tuple(q.shape[-3:-2])} or {tuple(q.shape[:-2])}, got "
+        if positions.shape not in (rows, rows[-1:]):
+            raise ValueError(f"positions must have shape {tuple(rows[-1:])} or {tuple(rows)}, got "
                              f"{tuple(positions.shape)}")
     if not (isinstance(eps, (int, float)) and 0 <= eps <= _F32_MAX):
         raise ValueError(f"eps must be >= 0, got {eps!r}")
     scale = float(scale)
     if not abs(scale) <= _F32_MAX:
         raise ValueError(f"scale must be finite in float32, got {scale}")
-    if q.numel() // hd >= _MOST or (k is not None and k.numel() // hd >= _MOST):
-        raise ValueError(f"q and k must have fewer than 2^31 rows each, got shapes {tuple(q.shape)}"
+    if q.numel() >= _MOST * hd or (k is not None and k.numel() >= _MOST * hd):
+        raise ValueError(f"q and k must have fewer than 2^31 rows each, got shapes {tuple(shape)}"
                          + (f" and {tuple(k.shape)}" if k is not None else ""))
     return scale
 
 
-def _rotary_params(q, k, freqs, positions, interleaved: bool, scale: float):
-    """The call's parameters, and the tensors that they point to."""
+def _four_strides(t) -> tuple[int, int, int, int]:
+    """(outer, inner, row, head), as ``HeadStrides``."""
+    s = t.stride()
+    return s[0], s[1] if len(s) == 5 else 0, s[-3], s[-2]
+
+
+def _rotary_params(q, k, freqs, positions, interleaved: bool, scale: float, q0=None, k0=None, gamma_q=None,
+                   gamma_k=None, eps: float = 0.0, lens=None) -> tuple[bytes, tuple]:
+    """``UnblendRotaryParams`` of a call on checked tensors with unit last strides, and the tensors that it points to."""
     s = q.shape
-    seqs = _seqs(q)
-    freqs = None if freqs is None else freqs.contiguous()
-    per_seq = positions is not None and positions.dim() > 1
-    positions = None if positions is None else positions.contiguous()
-    p = _lib.RotaryParams(_DTYPES[q.dtype], s[0], s[1] if len(s) == 5 else 1, s[-3], s[-2],
-                          0 if k is None else k.shape[-2], s[-1], 0 if freqs is None else freqs.shape[0],
-                          not interleaved, scale, _lib.ptr(freqs),
-                          freqs is not None and freqs.dtype == torch.float64,
-                          positions is not None and positions.dtype == torch.int64, _lib.ptr(positions),
-                          s[-3] if per_seq and seqs > 1 else 0, _strides(q))
-    if k is not None:
-        p.k = _strides(k)
-    return p, (freqs, positions)
+    five = len(s) == 5
+    f_ptr = pairs = f64 = p_ptr = p64 = per_seq = lens_ptr = 0
+    held = []
+    if freqs is not None:
+        freqs = freqs.contiguous()
+        f_ptr, pairs, f64 = freqs.data_ptr(), freqs.numel(), freqs.dtype == torch.float64
+        held.append(freqs)
+    if positions is not None:
+        if positions.dim() > 1:
+            per_seq = s[-3]
+        positions = positions.contiguous()
+        p_ptr, p64 = positions.data_ptr(), positions.dtype == torch.int64
+        held.append(positions)
+    w_dtype, gammas = _lib.DTYPE_F32, [0, 0]
+    for i, g in enumerate((gamma_q, gamma_k)):
+        if g is not None:
+            g = g.contiguous()
+            gammas[i], w_dtype = g.data_ptr(), _DTYPES[g.dtype]
+            held.append(g)
+    if lens is not None:
+        lens = lens.contiguous()
+        lens_ptr = lens.data_ptr()
+        held.append(lens)
+    none = (0, 0, 0, 0)
+    p = _ROTARY_PARAMS.pack(
+        _DTYPES[q.dtype], s[0], s[1] if five else 1, s[-3], s[-2], 0 if k is None else k.shape[-2], s[-1], pairs,
+        not interleaved, scale, f_ptr, f64, p64, p_ptr, per_seq, *_four_strides(q),
+        *(none if k is None else _four_strides(k)), *(none if q0 is None else _four_strides(q0)),
+        *(none if k0 is None else _four_strides(k0)), *gammas, w_dtype, eps, lens_ptr)
+    return p, tuple(held)
+
+
+@lru_cache(maxsize=4096)
+def _rotary_workspace_bytes(sizes: bytes) -> int:
+    """Workspace of the norm's backward pass, by the leading fields of ``UnblendRotaryParams``."""
+    p = _lib.RotaryParams.from_buffer_copy(sizes.ljust(ctypes.sizeof(_lib.RotaryParams), b"\0"))
+    p.pairs = 0  # the workspace does not depend on them, and their frequencies are not here
+    n = ctypes.c_longlong(0)
+    _lib.check("unblend_qk_norm_rotary_grad_workspace",
+               _lib.load().unblend_qk_norm_rotary_grad_workspace(ctypes.byref(p), ctypes.byref(n)))
+    return n.value
 
 
 def _rotate(q, k, freqs, positions, interleaved: bool, scale: float, inverse: bool):
@@ -563,8 +605,7 @@ def _rotate(q, k, freqs, positions, interleaved: bool, scale: float, inverse: bo
     q = _unit(q)
     k = None if k is None or k.numel() == 0 else _unit(k)
     p, held = _rotary_params(q, k, freqs, positions, interleaved, scale)
-    _launch(q, "unblend_rotary", q.data_ptr(), _lib.ptr(k), q_out.data_ptr(), _lib.ptr(k_out), ctypes.byref(p),
-            inverse)
+    _launch(q, "unblend_rotary", q.data_ptr(), _lib.ptr(k), q_out.data_ptr(), _lib.ptr(k_out), p, inverse)
     return q_out, k_out
 
 
@@ -655,15 +696,6 @@ def _check_qk_norm(q, k, gamma_q, gamma_k, freqs, positions, scale, eps, lens) -
     return scale
 
 
-def _norm_params(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens):
-    p, held = _rotary_params(q, k, freqs, positions, interleaved, scale)
-    gamma_q, gamma_k, lens = (None if t is None else t.contiguous() for t in (gamma_q, gamma_k, lens))
-    w = gamma_q if gamma_q is not None else gamma_k
-    p.gamma_q, p.gamma_k, p.lens, p.eps = _lib.ptr(gamma_q), _lib.ptr(gamma_k), _lib.ptr(lens), eps
-    p.w_dtype = _lib.DTYPE_F32 if w is None else _DTYPES[w.dtype]
-    return p, (*held, gamma_q, gamma_k, lens)
-
-
 def qk_norm_rotary_forward(q: torch.Tensor, k: torch.Tensor | None, gamma_q: torch.Tensor | None = None,
                            gamma_k: torch.Tensor | None = None, freqs: torch.Tensor | None = None,
                            positions: torch.Tensor | None = None, interleaved: bool = True, scale: float = 1.0,
@@ -690,9 +722,8 @@ def _qk_norm_forward(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scal
         return q_out, k_out
     q = _unit(q)
     k = None if k is None or k.numel() == 0 else _unit(k)
-    p, held = _norm_params(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
-    _launch(q, "unblend_qk_norm_rotary_forward", q.data_ptr(), _lib.ptr(k), q_out.data_ptr(), _lib.ptr(k_out),
-            ctypes.byref(p))
+    p, held = _rotary_params(q, k, freqs, positions, interleaved, scale, None, None, gamma_q, gamma_k, eps, lens)
+    _launch(q, "unblend_qk_norm_rotary_forward", q.data_ptr(), _lib.ptr(k), q_out.data_ptr(), _lib.ptr(k_out), p)
     return q_out, k_out
 
 
@@ -732,21 +763,15 @@ def _qk_norm_backward(dq, dk, q, k, gamma_q, gamma_k, freqs, positions, interlea
         return dq_out, dk_out, _empty(gamma_q).zero_() if weight_grads and gamma_q is not None else None, dgamma_k
     q, dq = _unit(q), _unit(dq)
     k, dk = (None, None) if k is None or k.numel() == 0 else (_unit(k), _unit(dk))
-    p, held = _norm_params(dq, dk, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
-    p.q0 = _strides(q)
-    if k is not None:
-        p.k0 = _strides(k)
+    p, held = _rotary_params(dq, dk, freqs, positions, interleaved, scale, q, k, gamma_q, gamma_k, eps, lens)
     dgamma_q = dgamma_k = work = None
     if weight_grads:
         w = gamma_q if gamma_q is not None else gamma_k
         dgamma_q, dgamma_k = (q.new_empty(q.shape[-1], dtype=w.dtype) for _ in range(2))
-        n = ctypes.c_longlong(0)
-        _lib.check("unblend_qk_norm_rotary_grad_workspace",
-                   _lib.load().unblend_qk_norm_rotary_grad_workspace(ctypes.byref(p), ctypes.byref(n)))
-        work = _scratch(q, n.value)
+        work = _scratch(q, _rotary_workspace_bytes(p[:_ROTARY_SIZES]))
     _launch(q, "unblend_qk_norm_rotary_backward", dq.data_ptr(), _lib.ptr(dk), q.data_ptr(), _lib.ptr(k),
-            dq_out.data_ptr(), _lib.ptr(dk_out), _lib.ptr(dgamma_q), _lib.ptr(dgamma_k), _lib.ptr(work),
-            ctypes.byref(p), kernels=1 + weight_grads)
+            dq_out.data_ptr(), _lib.ptr(dk_out), _lib.ptr(dgamma_q), _lib.ptr(dgamma_k), _lib.ptr(work), p,
+            kernels=1 + weight_grads)
     return dq_out, dk_out, dgamma_q if gamma_q is not None else None, dgamma_k if gamma_k is not None else None
 
 
@@ -1014,7 +1039,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     if not (isinstance(betas, (tuple, list)) and len(betas) == 2):
         raise ValueError(f"betas must be two numbers, got {betas!r}")
     a = _lib.AdamWParams(0.0, _number("betas[0]", betas[0], 0, 1), _number("betas[1]", betas[1], 0, 1),
-                         _number("eps", eps, 0), _number("weight_decay", weight_decay, 0))
+                         _number("eps", eps, 0, 1e30), _number("weight_decay", weight_decay, 0))
+    if 0 < eps < torch.finfo(torch.float32).smallest_normal:
+        raise ValueError(f"eps must be 0 or a normal float32, got {eps!r}")
     if isinstance(step, torch.Tensor):
         _check_scalar("step", step, torch.int64, device)
         a.step_device = step.data_ptr()
