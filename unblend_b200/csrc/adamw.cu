@@ -28,6 +28,7 @@ using namespace ub::train;
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int BLOCK = 256;            // elements that share scales
+constexpr int EIGHT_CTAS = 3;         // CTAs per SM of the 8-bit step: registers for two blocks per warp
 constexpr int SMALL = 64, LARGE = 896;  // tensors of a launch: 2.3 or 32 KB of kernel parameters
 
 template <int N>
@@ -123,47 +124,123 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // 1 / top, 0 for a block of zeros (or below the normal range, where 1 / top could overflow).
 __device__ __forceinline__ float inverse(float top) { return top >= 1.17549435e-38f ? __frcp_rn(top) : 0.f; }
 
-// Four consecutive elements; without `full`, those below n.
+// What a lane holds of a block, as read: eight elements in two groups of four.
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, float2 (&v)[2], bool full, int n) {
-  if (full) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 w = *reinterpret_cast<const float4*>(p);
-      v[0] = make_float2(w.x, w.y), v[1] = make_float2(w.z, w.w);
+struct Eight {
+  alignas(16) T e[8];
+
+  // `one`: the groups follow one another; full: the block is whole and p on a boundary of four elements (one: of eight)
+  __device__ __forceinline__ void load(const T* p, int gap, bool one, bool full, int left) {
+    if (full) {
+      if (sizeof(T) == 2 && one) {
+        *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint2*>(e + 4 * j) = *reinterpret_cast<const uint2*>(p + j * gap);
+          else
+            *reinterpret_cast<uint4*>(e + 4 * j) = *reinterpret_cast<const uint4*>(p + j * gap);
+        }
+      }
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
-      float2 u[4];
-      unpack16(make_uint4(w.x, w.y, 0u, 0u), u, T());
-      v[0] = u[0], v[1] = u[1];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = (i & 3) + (i >> 2) * gap;
+        e[i] = at < left ? p[at] : from_f<T>(0.f);
+      }
     }
-  } else {
-    v[0] = make_float2(n > 0 ? to_f(p[0]) : 0.f, n > 1 ? to_f(p[1]) : 0.f);
-    v[1] = make_float2(n > 2 ? to_f(p[2]) : 0.f, n > 3 ? to_f(p[3]) : 0.f);
   }
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float2 (&v)[2], bool full, int n) {
-  if (full) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+  __device__ __forceinline__ void store(T* p, int gap, bool one, bool full, int left) const {
+    if (full) {
+      if (sizeof(T) == 2 && one) {
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint2*>(p + j * gap) = *reinterpret_cast<const uint2*>(e + 4 * j);
+          else
+            *reinterpret_cast<uint4*>(p + j * gap) = *reinterpret_cast<const uint4*>(e + 4 * j);
+        }
+      }
     } else {
-      const float2 u[4] = {v[0], v[1], both(0.f), both(0.f)};
-      const uint4 w = pack16(u, T());
-      *reinterpret_cast<uint2*>(p) = make_uint2(w.x, w.y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = (i & 3) + (i >> 2) * gap;
+        if (at < left) p[at] = e[i];
+      }
     }
-  } else {
-    if (n > 0) p[0] = from_f<T>(v[0].x);
-    if (n > 1) p[1] = from_f<T>(v[0].y);
-    if (n > 2) p[2] = from_f<T>(v[1].x);
-    if (n > 3) p[3] = from_f<T>(v[1].y);
   }
-}
+  __device__ __forceinline__ void get(float2 (&v)[4]) const {
+    if constexpr (sizeof(T) == 2) {
+      unpack16(*reinterpret_cast<const uint4*>(e), v, T());
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = make_float2(e[2 * i], e[2 * i + 1]);
+    }
+  }
+  __device__ __forceinline__ void set(const float2 (&v)[4]) {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(e) = pack16(v, T());
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[2 * i] = v[i].x, e[2 * i + 1] = v[i].y;
+    }
+  }
+};
 
 // Largest of non-negative values by their patterns: NaN is above infinity.
 __device__ __forceinline__ float warp_top(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
 
+// A lane's part of a block of one tensor. In 8 bits its elements are consecutive for 16-bit tensors (accesses of 16 and 8
+// bytes); otherwise two groups of four 128 elements apart (whole lines per access).
 template <typename T, typename TG, bool EIGHT, int N>
-__global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ Table<N> tab,
+struct Unit {
+  static constexpr bool ONE = EIGHT && sizeof(T) == 2 && sizeof(TG) == 2;
+  static constexpr int GAP = ONE ? 4 : 128;
+  T* p;
+  long long at;  // of the moments
+  int left;      // elements of the tensor from the lane's first on
+  bool full;
+  Eight<T> param;
+  Eight<TG> grad;
+  unsigned mc[2], uc[2];
+  float2 scale;
+
+  __device__ __forceinline__ void fetch(const Table<N>& tab, const StepArgs& a, unsigned unit, int lane) {
+    const int k = tensor_of(tab, unit);
+    const long long local = unit - tab.start[k], n = tab.t[k].n - local * BLOCK;
+    const int mine = lane * (ONE ? 8 : 4);
+    p = static_cast<T*>(tab.t[k].param) + local * BLOCK;
+    const TG* g = static_cast<const TG*>(tab.t[k].grad) + local * BLOCK;
+    full = n >= BLOCK && reinterpret_cast<uintptr_t>(p) % ((ONE ? 8 : 4) * sizeof(T)) == 0 &&
+           reinterpret_cast<uintptr_t>(g) % ((ONE ? 8 : 4) * sizeof(TG)) == 0;
+    left = (int)min(n, (long long)BLOCK) - mine;
+    p += mine;
+    const long long block = tab.t[k].block + local;
+    at = block * BLOCK + mine;
+    if constexpr (EIGHT) {
+      scale = a.scales[block];
+      if constexpr (ONE) {
+        const uint2 m = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + at);
+        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + at);
+        mc[0] = m.x, mc[1] = m.y, uc[0] = u.x, uc[1] = u.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          mc[j] = *reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(a.m) + at + j * GAP);
+          uc[j] = *reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(a.v) + at + j * GAP);
+        }
+      }
+    }
+    param.load(p, GAP, ONE, full, left);
+    grad.load(g + mine, GAP, ONE, full, left);
+  }
+};
+
+template <typename T, typename TG, bool EIGHT, int N>
+__global__ void __launch_bounds__(THREADS, EIGHT ? EIGHT_CTAS : 4) adamw_kernel(const __grid_constant__ Table<N> tab,
                                                         const __grid_constant__ StepArgs a) {
   float decay = a.decay, size = a.size, root = a.root;
   const float gs = a.grad_scale ? *a.grad_scale : 1.f;
@@ -186,91 +263,90 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
     decay = f[0], size = f[1], root = f[2];
   }
   const int lane = threadIdx.x & 31;
-  for (unsigned unit = blockIdx.x * WARPS + (threadIdx.x >> 5); unit < tab.total; unit += gridDim.x * WARPS) {
-    const int k = tensor_of(tab, unit);
-    const long long local = unit - tab.start[k];
-    const long long left = tab.t[k].n - local * BLOCK;
-    T* p = static_cast<T*>(tab.t[k].param) + local * BLOCK;
-    const TG* g = static_cast<const TG*>(tab.t[k].grad) + local * BLOCK;
-    const long long block = tab.t[k].block + local;
-    const bool full = left >= BLOCK && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 &&
-                      reinterpret_cast<uintptr_t>(g) % (4 * sizeof(TG)) == 0;
-    float2 pv[2][2], gv[2][2], mv[2][2], uv[2][2];  // uv: v, and in 8 bits u once the codes are read
-    unsigned mc[2], uc[2];
-    float2 sc;
-    const long long at = block * BLOCK + lane * 4;
-    if constexpr (EIGHT) {
-      sc = a.scales[block];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        mc[j] = *reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(a.m) + at + j * 128);
-        uc[j] = *reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(a.v) + at + j * 128);
-      }
+  const unsigned stride = gridDim.x * WARPS;
+  unsigned unit = blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (unit >= tab.total) return;
+  using U = Unit<T, TG, EIGHT, N>;
+  U next;
+  if (EIGHT) next.fetch(tab, a, unit, lane);
+  for (; unit < tab.total; unit += stride) {
+    U x;
+    if constexpr (EIGHT) {  // the codes' arithmetic is long: the next block is on its way meanwhile
+      x = next;
+      if (unit + stride < tab.total) next.fetch(tab, a, unit + stride, lane);
+    } else {
+      x.fetch(tab, a, unit, lane);
     }
-    int n[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int e = lane * 4 + j * 128;
-      n[j] = left >= BLOCK ? 4 : min(max((int)left - e, 0), 4);
-      load4(p + e, pv[j], full, n[j]);
-      load4(g + e, gv[j], full, n[j]);
-      if constexpr (!EIGHT) {
-        load4(static_cast<const float*>(a.m) + at + j * 128, mv[j], true, 4);
-        load4(static_cast<const float*>(a.v) + at + j * 128, uv[j], true, 4);
-      }
-    }
+    float2 pv[4], gv[4], mv[4], uv[4];  // uv: v, and in 8 bits u once the codes are read
     if constexpr (EIGHT) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        mv[j][0] = mul2(make_float2(m_value<0>(mc[j]), m_value<1>(mc[j])), both(sc.x));
-        mv[j][1] = mul2(make_float2(m_value<2>(mc[j]), m_value<3>(mc[j])), both(sc.x));
-        uv[j][0] = mul2(make_float2(u_value<0>(uc[j]), u_value<1>(uc[j])), both(sc.y));
-        uv[j][1] = mul2(make_float2(u_value<2>(uc[j]), u_value<3>(uc[j])), both(sc.y));
+        const unsigned mc = x.mc[j], uc = x.uc[j];
+        mv[2 * j] = mul2(make_float2(m_value<0>(mc), m_value<1>(mc)), both(x.scale.x));
+        mv[2 * j + 1] = mul2(make_float2(m_value<2>(mc), m_value<3>(mc)), both(x.scale.x));
+        uv[2 * j] = mul2(make_float2(u_value<0>(uc), u_value<1>(uc)), both(x.scale.y));
+        uv[2 * j + 1] = mul2(make_float2(u_value<2>(uc), u_value<3>(uc)), both(x.scale.y));
       }
+    } else {
+      Eight<float> w;
+      w.load(static_cast<const float*>(a.m) + x.at, U::GAP, false, true, 0);
+      w.get(mv);
+      w.load(static_cast<const float*>(a.v) + x.at, U::GAP, false, true, 0);
+      w.get(uv);
     }
+    x.param.get(pv);
+    x.grad.get(gv);
     float top_m = 0.f, top_u = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float2 gr = mul2(gv[j][i], both(gs));
-        float2 m = mv[j][i], v = uv[j][i];
-        if (EIGHT) v = mul2(v, v);
-        // Sums as fma with a factor of 1 that the compiler does not know: it would fuse a packed product into them.
-        m = ub::fma2(mul2(m, both(a.b1)), both(a.one), mul2(gr, both(a.c1)));
-        v = ub::fma2(mul2(v, both(a.b2)), both(a.one), mul2(mul2(gr, gr), both(a.c2)));
-        const float2 u = make_float2(__fsqrt_rn(v.x), __fsqrt_rn(v.y));
-        const float2 denom = ub::fma2(u, both(root), both(a.eps));
-        const float2 step = mul2(m, make_float2(reciprocal(denom.x), reciprocal(denom.y)));
-        pv[j][i] = ub::fma2(step, both(-size), mul2(pv[j][i], both(decay)));
-        mv[j][i] = m;
-        uv[j][i] = EIGHT ? u : v;
-        if constexpr (EIGHT) {
-          top_m = top3(top_m, m.x, m.y);
-          top_u = top3(top_u, u.x, u.y);
-        }
-      }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      store4(p + lane * 4 + j * 128, pv[j], full, n[j]);
-      if constexpr (!EIGHT) {
-        store4(static_cast<float*>(a.m) + at + j * 128, mv[j], true, 4);
-        store4(static_cast<float*>(a.v) + at + j * 128, uv[j], true, 4);
+    for (int i = 0; i < 4; ++i) {
+      const float2 gr = mul2(gv[i], both(gs));
+      float2 m = mv[i], v = uv[i];
+      if (EIGHT) v = mul2(v, v);
+      // Sums as fma with a factor of 1 that the compiler does not know: it would fuse a packed product into them.
+      m = ub::fma2(mul2(m, both(a.b1)), both(a.one), mul2(gr, both(a.c1)));
+      v = ub::fma2(mul2(v, both(a.b2)), both(a.one), mul2(mul2(gr, gr), both(a.c2)));
+      const float2 u = make_float2(__fsqrt_rn(v.x), __fsqrt_rn(v.y));
+      const float2 denom = ub::fma2(u, both(root), both(a.eps));
+      const float2 step = mul2(m, make_float2(reciprocal(denom.x), reciprocal(denom.y)));
+      pv[i] = ub::fma2(step, both(-size), mul2(pv[i], both(decay)));
+      mv[i] = m;
+      uv[i] = EIGHT ? u : v;
+      if constexpr (EIGHT) {
+        top_m = top3(top_m, m.x, m.y);
+        top_u = top3(top_u, u.x, u.y);
       }
     }
+    x.param.set(pv);
+    x.param.store(x.p, U::GAP, U::ONE, x.full, x.left);
     if constexpr (EIGHT) {
       top_m = warp_top(top_m), top_u = warp_top(top_u);
       const float inv_m = inverse(top_m), inv_u = inverse(top_u);
+      unsigned cm[2], cu[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float2 m0 = mul2(mv[j][0], both(inv_m)), m1 = mul2(mv[j][1], both(inv_m));
-        const float2 u0 = mul2(uv[j][0], both(inv_u)), u1 = mul2(uv[j][1], both(inv_u));
-        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.m) + at + j * 128) =
-            high_bytes(m_code(m0.x), m_code(m0.y), m_code(m1.x), m_code(m1.y));
-        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.v) + at + j * 128) =
-            high_bytes(u_code(u0.x), u_code(u0.y), u_code(u1.x), u_code(u1.y));
+        const float2 m0 = mul2(mv[2 * j], both(inv_m)), m1 = mul2(mv[2 * j + 1], both(inv_m));
+        const float2 u0 = mul2(uv[2 * j], both(inv_u)), u1 = mul2(uv[2 * j + 1], both(inv_u));
+        cm[j] = high_bytes(m_code(m0.x), m_code(m0.y), m_code(m1.x), m_code(m1.y));
+        cu[j] = high_bytes(u_code(u0.x), u_code(u0.y), u_code(u1.x), u_code(u1.y));
       }
-      if (lane == 0) a.scales[block] = make_float2(top_m, top_u);
+      uint8_t *pm = static_cast<uint8_t*>(a.m) + x.at, *pu = static_cast<uint8_t*>(a.v) + x.at;
+      if constexpr (U::ONE) {
+        *reinterpret_cast<uint2*>(pm) = make_uint2(cm[0], cm[1]);
+        *reinterpret_cast<uint2*>(pu) = make_uint2(cu[0], cu[1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          *reinterpret_cast<unsigned*>(pm + j * U::GAP) = cm[j];
+          *reinterpret_cast<unsigned*>(pu + j * U::GAP) = cu[j];
+        }
+      }
+      if (lane == 0) a.scales[x.at / BLOCK] = make_float2(top_m, top_u);
+    } else {
+      Eight<float> w;
+      w.set(mv);
+      w.store(static_cast<float*>(a.m) + x.at, U::GAP, false, true, 0);
+      w.set(uv);
+      w.store(static_cast<float*>(a.v) + x.at, U::GAP, false, true, 0);
     }
   }
 }
@@ -285,13 +361,13 @@ __global__ void __launch_bounds__(THREADS) adamw_values_kernel(const uint8_t* m,
     for (int j = 0; j < 2; ++j) {
       const long long at = (long long)b * BLOCK + lane * 4 + j * 128;
       const unsigned mc = *reinterpret_cast<const unsigned*>(m + at), uc = *reinterpret_cast<const unsigned*>(u + at);
-      const float2 mv[2] = {mul2(make_float2(m_value<0>(mc), m_value<1>(mc)), both(sc.x)),
-                            mul2(make_float2(m_value<2>(mc), m_value<3>(mc)), both(sc.x))};
-      const float2 u0 = mul2(make_float2(u_value<0>(uc), u_value<1>(uc)), both(sc.y));
-      const float2 u1 = mul2(make_float2(u_value<2>(uc), u_value<3>(uc)), both(sc.y));
-      const float2 vv[2] = {mul2(u0, u0), mul2(u1, u1)};
-      store4(m_out + at, mv, true, 4);
-      store4(v_out + at, vv, true, 4);
+      const float2 m0 = mul2(make_float2(m_value<0>(mc), m_value<1>(mc)), both(sc.x));
+      const float2 m1 = mul2(make_float2(m_value<2>(mc), m_value<3>(mc)), both(sc.x));
+      float2 u0 = mul2(make_float2(u_value<0>(uc), u_value<1>(uc)), both(sc.y));
+      float2 u1 = mul2(make_float2(u_value<2>(uc), u_value<3>(uc)), both(sc.y));
+      u0 = mul2(u0, u0), u1 = mul2(u1, u1);
+      __stcs(reinterpret_cast<float4*>(m_out + at), make_float4(m0.x, m0.y, m1.x, m1.y));
+      __stcs(reinterpret_cast<float4*>(v_out + at), make_float4(u0.x, u0.y, u1.x, u1.y));
     }
   }
 }
@@ -420,10 +496,10 @@ int launch_step(const UnblendAdamWTensor* t, int count, const StepArgs& a, cudaS
     const int n = std::min(LARGE, count - i);
     if (n <= SMALL) {
       const Table<SMALL> tab = make_table<SMALL>(t + i, n, BLOCK);
-      adamw_kernel<T, TG, EIGHT, SMALL><<<grid_of(tab.total, 8), THREADS, 0, st>>>(tab, a);
+      adamw_kernel<T, TG, EIGHT, SMALL><<<grid_of(tab.total, EIGHT ? EIGHT_CTAS : 8), THREADS, 0, st>>>(tab, a);
     } else {
       const Table<LARGE> tab = make_table<LARGE>(t + i, n, BLOCK);
-      adamw_kernel<T, TG, EIGHT, LARGE><<<grid_of(tab.total, 8), THREADS, 0, st>>>(tab, a);
+      adamw_kernel<T, TG, EIGHT, LARGE><<<grid_of(tab.total, EIGHT ? EIGHT_CTAS : 8), THREADS, 0, st>>>(tab, a);
     }
     UB_CHECK_LAUNCH();
   }
