@@ -65,44 +65,56 @@ struct StepArgs {
   float decay, size, root;  // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
 };
 
-// A code of m is bits 20 .. 26 of the pattern minus M_LOW (code 1 is 2^-16 * 1.25), one of u bits 19 .. 26 minus U_LOW (code
-// 1 is 2^-16 * 1.125); the patterns' own places are kept until four codes are packed into a word.
-constexpr unsigned M_SHIFT = 20, M_LOW = (127u << 3) - 127u, U_SHIFT = 19, U_LOW = (127u << 4) - 255u;
-constexpr unsigned M_LEAST = 0x37200000u;  // 0.625 * 2^-16, half of code 1
+// Codes travel two at a time as fp16: four times a code's value is the fp16 pattern (c + 9) << 7 for m and (c + 17) << 6
+// for u (code 1 is 2^-16 * 1.25 and 2^-16 * 1.125), which the fp16 pipes decode, zero and convert with half the integer
+// instructions that 32-bit patterns take; those had bound the kernel.
+constexpr unsigned M_BIAS = 0x04800480u, U_BIAS = 0x04400440u;
+constexpr float M_ONE = 1.25f / 65536.f, U_ONE = 1.125f / 65536.f;
 
-// The value of code I of four, relative to its scale.
+__device__ __forceinline__ __half2 as_half2(unsigned w) { return *reinterpret_cast<__half2*>(&w); }
+__device__ __forceinline__ unsigned as_word(__half2 h) { return *reinterpret_cast<unsigned*>(&h); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// The values of codes 2 I and 2 I + 1 of four, relative to their scale.
 template <int I>
-__device__ __forceinline__ float m_value(unsigned w) {
-  const unsigned x = I < 3 ? w << (20 - 8 * I) : w >> 4;  // the code at bits 20 .. 26, its sign at 27
-  const unsigned c = x & (127u << M_SHIFT);
-  const unsigned v = c ? c + (M_LOW << M_SHIFT) : 0u;
-  return __uint_as_float(v | (x << 4 & 0x80000000u));
+__device__ __forceinline__ float2 m_values(unsigned w) {
+  const unsigned x = __byte_perm(w, 0, I ? 0x4342 : 0x4140), c = x & 0x007f007fu;
+  const __half2 there = __hne2(as_half2(c), as_half2(0));  // 1 or 0
+  const unsigned h = as_word(__hmul2(as_half2(c * 128u + M_BIAS), there)) | (x << 8 & 0x80008000u);
+  return mul2(__half22float2(as_half2(h)), both(0.25f));
 }
 template <int I>
-__device__ __forceinline__ float u_value(unsigned w) {
-  const unsigned c = (I < 3 ? w << (19 - 8 * I) : w >> 5) & (255u << U_SHIFT);
-  return __uint_as_float(c ? c + (U_LOW << U_SHIFT) : 0u);
+__device__ __forceinline__ float2 u_values(unsigned w) {
+  const unsigned x = __byte_perm(w, 0, I ? 0x4342 : 0x4140);
+  const __half2 there = __hne2(as_half2(x), as_half2(0));
+  return mul2(__half22float2(__hmul2(as_half2(x * 64u + U_BIAS), there)), both(0.25f));
 }
 
-// Codes of magnitudes relative to their block's largest, in the highest byte (the bits below are not cleared). The pattern
-// is rounded to nearest even by adding just less than half a step, and the lowest bit that stays.
-template <unsigned SHIFT, unsigned LOW>
-__device__ __forceinline__ int leading(unsigned mag) {
-  return (int)(mag + (mag >> SHIFT & 1u) + ((1u << (SHIFT - 1)) - 1u - (LOW << SHIFT)));
+// Rounds to BITS bits of mantissa (the leading one not counted) by Veltkamp's splitting (Dekker, "A floating-point technique
+// for extending the available precision", 1971); in radix 2 and for these lengths that is to nearest even for every
+// mantissa. `one` is a factor of 1 that the compiler does not know: it would fuse the product into the sums.
+template <int BITS>
+__device__ __forceinline__ float2 rounded(float2 r, float one) {
+  const float2 p = mul2(r, both((float)(1 << (23 - BITS)) + 1.f));
+  const float2 q = ub::fma2(p, both(-one), r);
+  return ub::fma2(p, both(one), q);
 }
-__device__ __forceinline__ unsigned m_code(float r) {
-  const unsigned w = __float_as_uint(r), mag = w & 0x7fffffffu;
-  const int least = mag > M_LEAST ? 1 << M_SHIFT : 0;
-  const unsigned c = (unsigned)max(leading<M_SHIFT, M_LOW>(mag), least) << 4;
-  return (c & 0x7fffffffu) | (w & 0x80000000u);
+
+// Codes of two values relative to their block's largest, in the upper bytes of the halves.
+__device__ __forceinline__ unsigned m_codes(float2 r, float one) {
+  float2 a = make_float2(fmaxf(fabsf(r.x), M_ONE), fmaxf(fabsf(r.y), M_ONE));
+  a.x = fabsf(r.x) > 0.5f * M_ONE ? a.x : 0.f;
+  a.y = fabsf(r.y) > 0.5f * M_ONE ? a.y : 0.f;
+  a = mul2(rounded<3>(a, one), both(4.f));
+  const unsigned c = __vmaxu2(as_word(__floats2half2_rn(a.x, a.y)), M_BIAS) - M_BIAS;
+  return c * 2u | (__byte_perm(__float_as_uint(r.x), __float_as_uint(r.y), 0x7632) & 0x80008000u);
 }
-__device__ __forceinline__ unsigned u_code(float r) {
-  const unsigned mag = __float_as_uint(r);
-  const int least = mag ? 1 << U_SHIFT : 0;
-  return (unsigned)max(leading<U_SHIFT, U_LOW>(mag), least) << 5;
-}
-__device__ __forceinline__ unsigned high_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
-  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+__device__ __forceinline__ unsigned u_codes(float2 r, float one) {
+  float2 a = make_float2(fmaxf(r.x, U_ONE), fmaxf(r.y, U_ONE));
+  a.x = r.x > 0.f ? a.x : 0.f;
+  a.y = r.y > 0.f ? a.y : 0.f;
+  a = mul2(rounded<4>(a, one), both(4.f));
+  return (__vmaxu2(as_word(__floats2half2_rn(a.x, a.y)), U_BIAS) - U_BIAS) * 4u;
 }
 
 // Largest magnitude of three, NaN if one is.
@@ -119,7 +131,32 @@ __device__ __forceinline__ float reciprocal(float x) {
   return r;
 }
 
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// Correctly rounded roots of eight values (not below 0). An approximate reciprocal root y is off by 2^-22; s = v y and one
+// Newton step with the residual v - s^2, which an fma computes exactly, round as the true root does for every fp32 number
+// from 2^-80 on (compared with the library's for each of them). Zeros, smaller values, infinities and NaN take the library's
+// function, which tests each value for its own.
+__device__ __forceinline__ void roots(const float2 (&v)[4], float2 (&u)[4], float& top) {
+  float low = v[0].x;
+  top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(v[i].x));
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(v[i].y));
+    const float2 s = mul2(v[i], y), h = mul2(y, both(0.5f));
+    u[i] = ub::fma2(ub::fma2(mul2(s, both(-1.f)), s, v[i]), h, s);
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(low) : "f"(low), "f"(v[i].x), "f"(v[i].y));
+    top = top3(top, u[i].x, u[i].y);
+  }
+  if (!(low >= 0x1p-80f && top <= 3.402823466e38f)) {
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u[i] = make_float2(__fsqrt_rn(v[i].x), __fsqrt_rn(v[i].y));
+      top = top3(top, u[i].x, u[i].y);
+    }
+  }
+}
 
 // 1 / top, 0 for a block of zeros (or below the normal range, where 1 / top could overflow).
 __device__ __forceinline__ float inverse(float top) { return top >= 1.17549435e-38f ? __frcp_rn(top) : 0.f; }
@@ -277,15 +314,14 @@ __global__ void __launch_bounds__(THREADS, EIGHT ? EIGHT_CTAS : 4) adamw_kernel(
     } else {
       x.fetch(tab, a, unit, lane);
     }
-    float2 pv[4], gv[4], mv[4], uv[4];  // uv: v, and in 8 bits u once the codes are read
+    float2 pv[4], gv[4], mv[4], uv[4];  // uv: v, in 8 bits u as the codes are read
     if constexpr (EIGHT) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const unsigned mc = x.mc[j], uc = x.uc[j];
-        mv[2 * j] = mul2(make_float2(m_value<0>(mc), m_value<1>(mc)), both(x.scale.x));
-        mv[2 * j + 1] = mul2(make_float2(m_value<2>(mc), m_value<3>(mc)), both(x.scale.x));
-        uv[2 * j] = mul2(make_float2(u_value<0>(uc), u_value<1>(uc)), both(x.scale.y));
-        uv[2 * j + 1] = mul2(make_float2(u_value<2>(uc), u_value<3>(uc)), both(x.scale.y));
+        mv[2 * j] = mul2(m_values<0>(x.mc[j]), both(x.scale.x));
+        mv[2 * j + 1] = mul2(m_values<1>(x.mc[j]), both(x.scale.x));
+        uv[2 * j] = mul2(u_values<0>(x.uc[j]), both(x.scale.y));
+        uv[2 * j + 1] = mul2(u_values<1>(x.uc[j]), both(x.scale.y));
       }
     } else {
       Eight<float> w;
@@ -296,25 +332,23 @@ __global__ void __launch_bounds__(THREADS, EIGHT ? EIGHT_CTAS : 4) adamw_kernel(
     }
     x.param.get(pv);
     x.grad.get(gv);
-    float top_m = 0.f, top_u = 0.f;
+    float top_m = 0.f, top_u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 gr = mul2(gv[i], both(gs));
-      float2 m = mv[i], v = uv[i];
-      if (EIGHT) v = mul2(v, v);
-      // Sums as fma with a factor of 1 that the compiler does not know: it would fuse a packed product into them.
-      m = ub::fma2(mul2(m, both(a.b1)), both(a.one), mul2(gr, both(a.c1)));
-      v = ub::fma2(mul2(v, both(a.b2)), both(a.one), mul2(mul2(gr, gr), both(a.c2)));
-      const float2 u = make_float2(__fsqrt_rn(v.x), __fsqrt_rn(v.y));
-      const float2 denom = ub::fma2(u, both(root), both(a.eps));
-      const float2 step = mul2(m, make_float2(reciprocal(denom.x), reciprocal(denom.y)));
+      if (EIGHT) uv[i] = mul2(uv[i], uv[i]);
+      // Sums as fma with the factor `one`: a packed product would be fused into them.
+      mv[i] = ub::fma2(mul2(mv[i], both(a.b1)), both(a.one), mul2(gr, both(a.c1)));
+      uv[i] = ub::fma2(mul2(uv[i], both(a.b2)), both(a.one), mul2(mul2(gr, gr), both(a.c2)));
+      if (EIGHT) top_m = top3(top_m, mv[i].x, mv[i].y);
+    }
+    float2 root_v[4];
+    roots(uv, root_v, top_u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 denom = ub::fma2(root_v[i], both(root), both(a.eps));
+      const float2 step = mul2(mv[i], make_float2(reciprocal(denom.x), reciprocal(denom.y)));
       pv[i] = ub::fma2(step, both(-size), mul2(pv[i], both(decay)));
-      mv[i] = m;
-      uv[i] = EIGHT ? u : v;
-      if constexpr (EIGHT) {
-        top_m = top3(top_m, m.x, m.y);
-        top_u = top3(top_u, u.x, u.y);
-      }
     }
     x.param.set(pv);
     x.param.store(x.p, U::GAP, U::ONE, x.full, x.left);
@@ -324,10 +358,10 @@ __global__ void __launch_bounds__(THREADS, EIGHT ? EIGHT_CTAS : 4) adamw_kernel(
       unsigned cm[2], cu[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float2 m0 = mul2(mv[2 * j], both(inv_m)), m1 = mul2(mv[2 * j + 1], both(inv_m));
-        const float2 u0 = mul2(uv[2 * j], both(inv_u)), u1 = mul2(uv[2 * j + 1], both(inv_u));
-        cm[j] = high_bytes(m_code(m0.x), m_code(m0.y), m_code(m1.x), m_code(m1.y));
-        cu[j] = high_bytes(u_code(u0.x), u_code(u0.y), u_code(u1.x), u_code(u1.y));
+        cm[j] = __byte_perm(m_codes(mul2(mv[2 * j], both(inv_m)), a.one),
+                            m_codes(mul2(mv[2 * j + 1], both(inv_m)), a.one), 0x7531);
+        cu[j] = __byte_perm(u_codes(mul2(root_v[2 * j], both(inv_u)), a.one),
+                            u_codes(mul2(root_v[2 * j + 1], both(inv_u)), a.one), 0x7531);
       }
       uint8_t *pm = static_cast<uint8_t*>(a.m) + x.at, *pu = static_cast<uint8_t*>(a.v) + x.at;
       if constexpr (U::ONE) {
@@ -361,10 +395,8 @@ __global__ void __launch_bounds__(THREADS) adamw_values_kernel(const uint8_t* m,
     for (int j = 0; j < 2; ++j) {
       const long long at = (long long)b * BLOCK + lane * 4 + j * 128;
       const unsigned mc = *reinterpret_cast<const unsigned*>(m + at), uc = *reinterpret_cast<const unsigned*>(u + at);
-      const float2 m0 = mul2(make_float2(m_value<0>(mc), m_value<1>(mc)), both(sc.x));
-      const float2 m1 = mul2(make_float2(m_value<2>(mc), m_value<3>(mc)), both(sc.x));
-      float2 u0 = mul2(make_float2(u_value<0>(uc), u_value<1>(uc)), both(sc.y));
-      float2 u1 = mul2(make_float2(u_value<2>(uc), u_value<3>(uc)), both(sc.y));
+      const float2 m0 = mul2(m_values<0>(mc), both(sc.x)), m1 = mul2(m_values<1>(mc), both(sc.x));
+      float2 u0 = mul2(u_values<0>(uc), both(sc.y)), u1 = mul2(u_values<1>(uc), both(sc.y));
       u0 = mul2(u0, u0), u1 = mul2(u1, u1);
       __stcs(reinterpret_cast<float4*>(m_out + at), make_float4(m0.x, m0.y, m1.x, m1.y));
       __stcs(reinterpret_cast<float4*>(v_out + at), make_float4(u0.x, u0.y, u1.x, u1.y));
@@ -543,7 +575,7 @@ int launch_squares(const UnblendAdamWTensor* t, int count, double* part, int* us
 }  // namespace
 
 // The update multiplies by an approximate reciprocal, which takes normal numbers only; the root of v is 0 or above 2^-75.
-static bool eps_ok(double eps) { return eps == 0 || (eps >= 1.17549435e-38 && eps <= 1e30); }
+bool eps_ok(double eps) { return eps == 0 || (eps >= 1.17549435e-38 && eps <= 1e30); }
 
 extern "C" int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, void* exp_avg, void* exp_avg_sq,
                                   float* scales, int bits, int dtype, int grad_dtype, const UnblendAdamWParams* p,
