@@ -28,13 +28,14 @@ using namespace ub::train;
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int BLOCK = 256;            // elements that share scales
+constexpr int FULL_CTAS = 4;
 constexpr int EIGHT_CTAS = 3;         // CTAs per SM of the 8-bit step: registers for two blocks per warp
 constexpr int SMALL = 64, LARGE = 896;  // tensors of a launch: 2.3 or 32 KB of kernel parameters
 
 template <int N>
 struct Table {
   UnblendAdamWTensor t[N];
-  unsigned start[N];  // first of the launch's units of each tensor
+  unsigned start[N + 1];  // first of the launch's units of each tensor, and their number
   int count;
   unsigned total;
 };
@@ -62,32 +63,35 @@ struct StepArgs {
   const float* lr;        // device
   double b1d, b2d, lrd, wdd;
   float b1, c1, b2, c2, eps, one;
+  unsigned run;  // consecutive blocks of a warp
   float decay, size, root;  // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
 };
 
-// Codes travel two at a time as fp16: four times a code's value is the fp16 pattern (c + 9) << 7 for m and (c + 17) << 6
-// for u (code 1 is 2^-16 * 1.25 and 2^-16 * 1.125), which the fp16 pipes decode, zero and convert with half the integer
-// instructions that 32-bit patterns take; those had bound the kernel.
-constexpr unsigned M_BIAS = 0x04800480u, U_BIAS = 0x04400440u;
-constexpr float M_ONE = 1.25f / 65536.f, U_ONE = 1.125f / 65536.f;
+// Codes travel two at a time as bf16: a code's value is the bf16 pattern (c + 889) << 4 for m and (c + 1777) << 3 for u (code
+// 1 is 2^-16 * 1.25 and 2^-16 * 1.125), which the packed 16-bit pipes decode and zero with half the integer instructions that
+// 32-bit patterns take; those had bound the kernel.
+constexpr unsigned M_BIAS = (889u << 4) * 0x10001u, U_BIAS = (1777u << 3) * 0x10001u;
+constexpr float M_ONE = 1.25f / 65536.f;
 
-__device__ __forceinline__ __half2 as_half2(unsigned w) { return *reinterpret_cast<__half2*>(&w); }
-__device__ __forceinline__ unsigned as_word(__half2 h) { return *reinterpret_cast<unsigned*>(&h); }
+__device__ __forceinline__ __nv_bfloat162 as_bf2(unsigned w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+__device__ __forceinline__ unsigned as_word(__nv_bfloat162 h) { return *reinterpret_cast<unsigned*>(&h); }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 wide(unsigned w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 
 // The values of codes 2 I and 2 I + 1 of four, relative to their scale.
 template <int I>
 __device__ __forceinline__ float2 m_values(unsigned w) {
   const unsigned x = __byte_perm(w, 0, I ? 0x4342 : 0x4140), c = x & 0x007f007fu;
-  const __half2 there = __hne2(as_half2(c), as_half2(0));  // 1 or 0
-  const unsigned h = as_word(__hmul2(as_half2(c * 128u + M_BIAS), there)) | (x << 8 & 0x80008000u);
-  return mul2(__half22float2(as_half2(h)), both(0.25f));
+  const __nv_bfloat162 there = __hne2(as_bf2(c), as_bf2(0));  // 1 or 0
+  return wide(as_word(__hmul2(as_bf2(c * 16u + M_BIAS), there)) | (x << 8 & 0x80008000u));
 }
 template <int I>
 __device__ __forceinline__ float2 u_values(unsigned w) {
   const unsigned x = __byte_perm(w, 0, I ? 0x4342 : 0x4140);
-  const __half2 there = __hne2(as_half2(x), as_half2(0));
-  return mul2(__half22float2(__hmul2(as_half2(x * 64u + U_BIAS), there)), both(0.25f));
+  const __nv_bfloat162 there = __hne2(as_bf2(x), as_bf2(0));
+  return wide(as_word(__hmul2(as_bf2(x * 8u + U_BIAS), there)));
 }
 
 // Rounds to BITS bits of mantissa (the leading one not counted) by Veltkamp's splitting (Dekker, "A floating-point technique
@@ -100,21 +104,23 @@ __device__ __forceinline__ float2 rounded(float2 r, float one) {
   return ub::fma2(p, both(one), q);
 }
 
+// Upper halves of two patterns: the floats as bf16, cut off.
+__device__ __forceinline__ unsigned upper(float2 v) {
+  return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
+}
+
 // Codes of two values relative to their block's largest, in the upper bytes of the halves.
 __device__ __forceinline__ unsigned m_codes(float2 r, float one) {
   float2 a = make_float2(fmaxf(fabsf(r.x), M_ONE), fmaxf(fabsf(r.y), M_ONE));
   a.x = fabsf(r.x) > 0.5f * M_ONE ? a.x : 0.f;
   a.y = fabsf(r.y) > 0.5f * M_ONE ? a.y : 0.f;
-  a = mul2(rounded<3>(a, one), both(4.f));
-  const unsigned c = __vmaxu2(as_word(__floats2half2_rn(a.x, a.y)), M_BIAS) - M_BIAS;
-  return c * 2u | (__byte_perm(__float_as_uint(r.x), __float_as_uint(r.y), 0x7632) & 0x80008000u);
+  const unsigned c = __vmaxu2(upper(rounded<3>(a, one)), M_BIAS) - M_BIAS;
+  return c * 16u | (upper(r) & 0x80008000u);
 }
+// What is not 0 has code 1 or more (the mask looks at the bf16 pattern: above 2^-133 of the largest).
 __device__ __forceinline__ unsigned u_codes(float2 r, float one) {
-  float2 a = make_float2(fmaxf(r.x, U_ONE), fmaxf(r.y, U_ONE));
-  a.x = r.x > 0.f ? a.x : 0.f;
-  a.y = r.y > 0.f ? a.y : 0.f;
-  a = mul2(rounded<4>(a, one), both(4.f));
-  return (__vmaxu2(as_word(__floats2half2_rn(a.x, a.y)), U_BIAS) - U_BIAS) * 4u;
+  const unsigned there = __hne2_mask(as_bf2(upper(r)), as_bf2(0));
+  return (__vmaxu2(upper(rounded<4>(r, one)), U_BIAS + 0x00080008u) - U_BIAS & there) * 32u;
 }
 
 // Largest magnitude of three, NaN if one is.
@@ -242,11 +248,11 @@ struct Unit {
   bool full;
   Eight<T> param;
   Eight<TG> grad;
-  unsigned mc[2], uc[2];
+  unsigned mc[2], uc[2];  // 8 bits: codes and scales
   float2 scale;
+  Eight<float> m, v;  // 32 bits
 
-  __device__ __forceinline__ void fetch(const Table<N>& tab, const StepArgs& a, unsigned unit, int lane) {
-    const int k = tensor_of(tab, unit);
+  __device__ __forceinline__ void fetch(const Table<N>& tab, const StepArgs& a, int k, unsigned unit, int lane) {
     const long long local = unit - tab.start[k], n = tab.t[k].n - local * BLOCK;
     const int mine = lane * (ONE ? 8 : 4);
     p = static_cast<T*>(tab.t[k].param) + local * BLOCK;
@@ -271,116 +277,152 @@ struct Unit {
         }
       }
     }
+    if constexpr (!EIGHT) {
+      m.load(static_cast<const float*>(a.m) + at, GAP, false, true, 0);
+      v.load(static_cast<const float*>(a.v) + at, GAP, false, true, 0);
+    }
     param.load(p, GAP, ONE, full, left);
     grad.load(g + mine, GAP, ONE, full, left);
   }
 };
 
+struct Factors {
+  float decay, size, root, grad;
+};
+
+// The update of a lane's part of a block.
 template <typename T, typename TG, bool EIGHT, int N>
-__global__ void __launch_bounds__(THREADS, EIGHT ? EIGHT_CTAS : 4) adamw_kernel(const __grid_constant__ Table<N> tab,
-                                                        const __grid_constant__ StepArgs a) {
-  float decay = a.decay, size = a.size, root = a.root;
-  const float gs = a.grad_scale ? *a.grad_scale : 1.f;
-  if (!isfinite(gs)) return;  // an overflow somewhere in the gradients: nothing changes
+__device__ __forceinline__ void update(Unit<T, TG, EIGHT, N>& x, const StepArgs& a, const Factors& f, int lane) {
+  using U = Unit<T, TG, EIGHT, N>;
+  float2 pv[4], gv[4], mv[4], uv[4];  // uv: v, in 8 bits u as the codes are read
+  if constexpr (EIGHT) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      mv[2 * j] = mul2(m_values<0>(x.mc[j]), both(x.scale.x));
+      mv[2 * j + 1] = mul2(m_values<1>(x.mc[j]), both(x.scale.x));
+      uv[2 * j] = mul2(u_values<0>(x.uc[j]), both(x.scale.y));
+      uv[2 * j + 1] = mul2(u_values<1>(x.uc[j]), both(x.scale.y));
+    }
+  } else {
+    x.m.get(mv);
+    x.v.get(uv);
+  }
+  x.param.get(pv);
+  x.grad.get(gv);
+  [[maybe_unused]] float top_m = 0.f, top_u = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 gr = mul2(gv[i], both(f.grad));
+    if (EIGHT) uv[i] = mul2(uv[i], uv[i]);
+    // Sums as fma with the factor `one`: a packed product would be fused into them.
+    mv[i] = ub::fma2(mul2(mv[i], both(a.b1)), both(a.one), mul2(gr, both(a.c1)));
+    uv[i] = ub::fma2(mul2(uv[i], both(a.b2)), both(a.one), mul2(mul2(gr, gr), both(a.c2)));
+    if (EIGHT) top_m = top3(top_m, mv[i].x, mv[i].y);
+  }
+  float2 root_v[4];
+  if constexpr (EIGHT) {
+    roots(uv, root_v, top_u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) root_v[i] = make_float2(__fsqrt_rn(uv[i].x), __fsqrt_rn(uv[i].y));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 denom = ub::fma2(root_v[i], both(f.root), both(a.eps));
+    const float2 step = mul2(mv[i], make_float2(reciprocal(denom.x), reciprocal(denom.y)));
+    pv[i] = ub::fma2(step, both(-f.size), mul2(pv[i], both(f.decay)));
+  }
+  x.param.set(pv);
+  x.param.store(x.p, U::GAP, U::ONE, x.full, x.left);
+  if constexpr (EIGHT) {
+    top_m = warp_top(top_m), top_u = warp_top(top_u);
+    const float inv_m = inverse(top_m), inv_u = inverse(top_u);
+    unsigned cm[2], cu[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      cm[j] = __byte_perm(m_codes(mul2(mv[2 * j], both(inv_m)), a.one),
+                          m_codes(mul2(mv[2 * j + 1], both(inv_m)), a.one), 0x7531);
+      cu[j] = __byte_perm(u_codes(mul2(root_v[2 * j], both(inv_u)), a.one),
+                          u_codes(mul2(root_v[2 * j + 1], both(inv_u)), a.one), 0x7531);
+    }
+    uint8_t *pm = static_cast<uint8_t*>(a.m) + x.at, *pu = static_cast<uint8_t*>(a.v) + x.at;
+    if constexpr (U::ONE) {
+      *reinterpret_cast<uint2*>(pm) = make_uint2(cm[0], cm[1]);
+      *reinterpret_cast<uint2*>(pu) = make_uint2(cu[0], cu[1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        *reinterpret_cast<unsigned*>(pm + j * U::GAP) = cm[j];
+        *reinterpret_cast<unsigned*>(pu + j * U::GAP) = cu[j];
+      }
+    }
+    if (lane == 0) a.scales[x.at / BLOCK] = make_float2(top_m, top_u);
+  } else {
+    x.m.set(mv);
+    x.m.store(static_cast<float*>(a.m) + x.at, U::GAP, false, true, 0);
+    x.v.set(uv);
+    x.v.store(static_cast<float*>(a.v) + x.at, U::GAP, false, true, 0);
+  }
+}
+
+template <typename T, typename TG, bool EIGHT, int N>
+__global__ void __launch_bounds__(THREADS, EIGHT ? EIGHT_CTAS : FULL_CTAS) adamw_kernel(
+    const __grid_constant__ Table<N> tab, const __grid_constant__ StepArgs a) {
+  Factors f{a.decay, a.size, a.root, a.grad_scale ? *a.grad_scale : 1.f};
+  if (!isfinite(f.grad)) return;  // an overflow somewhere in the gradients: nothing changes
   if (a.step || a.lr) {
-    __shared__ float f[3];
+    __shared__ float computed[3];
     if (threadIdx.x == 0) {
       const double lr = a.lr ? (double)*a.lr : a.lrd;
-      f[0] = (float)(1.0 - lr * a.wdd);
+      computed[0] = (float)(1.0 - lr * a.wdd);
       if (a.step) {
         const double t = (double)max(*a.step, 1LL);
-        f[1] = (float)(lr / (1.0 - pow(a.b1d, t)));
-        f[2] = (float)(1.0 / sqrt(1.0 - pow(a.b2d, t)));
+        computed[1] = (float)(lr / (1.0 - pow(a.b1d, t)));
+        computed[2] = (float)(1.0 / sqrt(1.0 - pow(a.b2d, t)));
       } else {  // size is 1 / (1 - b1^t) here
-        f[1] = (float)(lr * (double)size);
-        f[2] = root;
+        computed[1] = (float)(lr * (double)f.size);
+        computed[2] = f.root;
       }
     }
     __syncthreads();
-    decay = f[0], size = f[1], root = f[2];
+    f.decay = computed[0], f.size = computed[1], f.root = computed[2];
   }
   const int lane = threadIdx.x & 31;
-  const unsigned stride = gridDim.x * WARPS;
-  unsigned unit = blockIdx.x * WARPS + (threadIdx.x >> 5);
+  // Runs of a.run blocks per warp: the tensor is searched for at the first, and followed from there.
+  const unsigned warps = gridDim.x * WARPS;
+  unsigned run = blockIdx.x * WARPS + (threadIdx.x >> 5), unit = run * a.run, end = min(unit + a.run, tab.total);
   if (unit >= tab.total) return;
-  using U = Unit<T, TG, EIGHT, N>;
-  U next;
-  if (EIGHT) next.fetch(tab, a, unit, lane);
-  for (; unit < tab.total; unit += stride) {
-    U x;
-    if constexpr (EIGHT) {  // the codes' arithmetic is long: the next block is on its way meanwhile
-      x = next;
-      if (unit + stride < tab.total) next.fetch(tab, a, unit + stride, lane);
-    } else {
-      x.fetch(tab, a, unit, lane);
+  int k = tensor_of(tab, unit);
+  const auto advance = [&] {  // whether there is another block
+    if (++unit < end) {
+      while (unit >= tab.start[k + 1]) ++k;
+      return true;
     }
-    float2 pv[4], gv[4], mv[4], uv[4];  // uv: v, in 8 bits u as the codes are read
-    if constexpr (EIGHT) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        mv[2 * j] = mul2(m_values<0>(x.mc[j]), both(x.scale.x));
-        mv[2 * j + 1] = mul2(m_values<1>(x.mc[j]), both(x.scale.x));
-        uv[2 * j] = mul2(u_values<0>(x.uc[j]), both(x.scale.y));
-        uv[2 * j + 1] = mul2(u_values<1>(x.uc[j]), both(x.scale.y));
-      }
-    } else {
-      Eight<float> w;
-      w.load(static_cast<const float*>(a.m) + x.at, U::GAP, false, true, 0);
-      w.get(mv);
-      w.load(static_cast<const float*>(a.v) + x.at, U::GAP, false, true, 0);
-      w.get(uv);
+    run += warps;
+    if (run > (tab.total - 1) / a.run) return false;
+    unit = run * a.run;
+    end = min(unit + a.run, tab.total);
+    k = tensor_of(tab, unit);
+    return true;
+  };
+  Unit<T, TG, EIGHT, N> x, y;
+  x.fetch(tab, a, k, unit, lane);
+  if constexpr (EIGHT) {  // long arithmetic: the next block is on its way meanwhile
+    for (;;) {
+      bool more = advance();
+      if (more) y.fetch(tab, a, k, unit, lane);
+      update(x, a, f, lane);
+      if (!more) return;
+      more = advance();
+      if (more) x.fetch(tab, a, k, unit, lane);
+      update(y, a, f, lane);
+      if (!more) return;
     }
-    x.param.get(pv);
-    x.grad.get(gv);
-    float top_m = 0.f, top_u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 gr = mul2(gv[i], both(gs));
-      if (EIGHT) uv[i] = mul2(uv[i], uv[i]);
-      // Sums as fma with the factor `one`: a packed product would be fused into them.
-      mv[i] = ub::fma2(mul2(mv[i], both(a.b1)), both(a.one), mul2(gr, both(a.c1)));
-      uv[i] = ub::fma2(mul2(uv[i], both(a.b2)), both(a.one), mul2(mul2(gr, gr), both(a.c2)));
-      if (EIGHT) top_m = top3(top_m, mv[i].x, mv[i].y);
-    }
-    float2 root_v[4];
-    roots(uv, root_v, top_u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 denom = ub::fma2(root_v[i], both(root), both(a.eps));
-      const float2 step = mul2(mv[i], make_float2(reciprocal(denom.x), reciprocal(denom.y)));
-      pv[i] = ub::fma2(step, both(-size), mul2(pv[i], both(decay)));
-    }
-    x.param.set(pv);
-    x.param.store(x.p, U::GAP, U::ONE, x.full, x.left);
-    if constexpr (EIGHT) {
-      top_m = warp_top(top_m), top_u = warp_top(top_u);
-      const float inv_m = inverse(top_m), inv_u = inverse(top_u);
-      unsigned cm[2], cu[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        cm[j] = __byte_perm(m_codes(mul2(mv[2 * j], both(inv_m)), a.one),
-                            m_codes(mul2(mv[2 * j + 1], both(inv_m)), a.one), 0x7531);
-        cu[j] = __byte_perm(u_codes(mul2(root_v[2 * j], both(inv_u)), a.one),
-                            u_codes(mul2(root_v[2 * j + 1], both(inv_u)), a.one), 0x7531);
-      }
-      uint8_t *pm = static_cast<uint8_t*>(a.m) + x.at, *pu = static_cast<uint8_t*>(a.v) + x.at;
-      if constexpr (U::ONE) {
-        *reinterpret_cast<uint2*>(pm) = make_uint2(cm[0], cm[1]);
-        *reinterpret_cast<uint2*>(pu) = make_uint2(cu[0], cu[1]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          *reinterpret_cast<unsigned*>(pm + j * U::GAP) = cm[j];
-          *reinterpret_cast<unsigned*>(pu + j * U::GAP) = cu[j];
-        }
-      }
-      if (lane == 0) a.scales[x.at / BLOCK] = make_float2(top_m, top_u);
-    } else {
-      Eight<float> w;
-      w.set(mv);
-      w.store(static_cast<float*>(a.m) + x.at, U::GAP, false, true, 0);
-      w.set(uv);
-      w.store(static_cast<float*>(a.v) + x.at, U::GAP, false, true, 0);
+  } else {
+    update(x, a, f, lane);
+    while (advance()) {
+      x.fetch(tab, a, k, unit, lane);
+      update(x, a, f, lane);
     }
   }
 }
@@ -478,7 +520,7 @@ Table<N> make_table(const UnblendAdamWTensor* t, int count, int unit) {
     tab.start[i] = at;
     at += (unsigned)((t[i].n + unit - 1) / unit);
   }
-  tab.total = at;
+  tab.total = tab.start[count] = at;
   return tab;
 }
 
@@ -522,18 +564,23 @@ unsigned grid_of(unsigned units, int per_sm) {
   return ctas < cap ? ctas : cap;
 }
 
+template <typename T, typename TG, bool EIGHT, int N>
+int launch_table(const UnblendAdamWTensor* t, int count, StepArgs a, cudaStream_t st) {
+  const Table<N> tab = make_table<N>(t, count, BLOCK);
+  const unsigned grid = grid_of(tab.total, EIGHT ? EIGHT_CTAS : 2 * FULL_CTAS);
+  if (EIGHT) a.run = std::min(16u, std::max(1u, tab.total / (grid * WARPS * 4)));  // four runs per warp at least
+  adamw_kernel<T, TG, EIGHT, N><<<grid, THREADS, 0, st>>>(tab, a);
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
 template <typename T, typename TG, bool EIGHT>
 int launch_step(const UnblendAdamWTensor* t, int count, const StepArgs& a, cudaStream_t st) {
   for (int i = 0; i < count; i += LARGE) {
     const int n = std::min(LARGE, count - i);
-    if (n <= SMALL) {
-      const Table<SMALL> tab = make_table<SMALL>(t + i, n, BLOCK);
-      adamw_kernel<T, TG, EIGHT, SMALL><<<grid_of(tab.total, EIGHT ? EIGHT_CTAS : 8), THREADS, 0, st>>>(tab, a);
-    } else {
-      const Table<LARGE> tab = make_table<LARGE>(t + i, n, BLOCK);
-      adamw_kernel<T, TG, EIGHT, LARGE><<<grid_of(tab.total, EIGHT ? EIGHT_CTAS : 8), THREADS, 0, st>>>(tab, a);
-    }
-    UB_CHECK_LAUNCH();
+    const int rc = n <= SMALL ? launch_table<T, TG, EIGHT, SMALL>(t + i, n, a, st)
+                              : launch_table<T, TG, EIGHT, LARGE>(t + i, n, a, st);
+    if (rc) return rc;
   }
   return 0;
 }
@@ -595,6 +642,7 @@ extern "C" int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, 
     return (int)cudaErrorMemoryAllocation;
   }
   StepArgs a{};
+  a.run = 1;
   a.m = exp_avg;
   a.v = exp_avg_sq;
   a.scales = reinterpret_cast<float2*>(scales);
