@@ -28,14 +28,16 @@ using namespace ub::train;
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int BLOCK = 256;            // elements that share scales
+// CTAs per SM that the registers allow: in 8 bits a warp has two blocks in flight, for fp32 tensors of twice the size (75 M fp32
+// parameters with values: 616 us with two CTAs, 690 with three and spills).
 constexpr int FULL_CTAS = 4;
-constexpr int EIGHT_CTAS = 3;         // CTAs per SM of the 8-bit step: registers for two blocks per warp
+constexpr int eight_ctas(int elem, int grad_elem) { return elem + grad_elem > 4 ? 2 : 3; }
 constexpr int SMALL = 64, LARGE = 896;  // tensors of a launch: 2.3 or 32 KB of kernel parameters
 
 template <int N>
 struct Table {
   UnblendAdamWTensor t[N];
-  unsigned start[N + 1];  // first of the launch's units of each tensor, and their number
+  unsigned start[N];  // first of the launch's units of each tensor
   int count;
   unsigned total;
 };
@@ -250,7 +252,6 @@ struct Unit {
   Eight<TG> grad;
   unsigned mc[2], uc[2];  // 8 bits: codes and scales
   float2 scale;
-  Eight<float> m, v;  // 32 bits
 
   __device__ __forceinline__ void fetch(const Table<N>& tab, const StepArgs& a, int k, unsigned unit, int lane) {
     const long long local = unit - tab.start[k], n = tab.t[k].n - local * BLOCK;
@@ -277,10 +278,6 @@ struct Unit {
         }
       }
     }
-    if constexpr (!EIGHT) {
-      m.load(static_cast<const float*>(a.m) + at, GAP, false, true, 0);
-      v.load(static_cast<const float*>(a.v) + at, GAP, false, true, 0);
-    }
     param.load(p, GAP, ONE, full, left);
     grad.load(g + mine, GAP, ONE, full, left);
   }
@@ -304,33 +301,43 @@ __device__ __forceinline__ void update(Unit<T, TG, EIGHT, N>& x, const StepArgs&
       uv[2 * j + 1] = mul2(u_values<1>(x.uc[j]), both(x.scale.y));
     }
   } else {
-    x.m.get(mv);
-    x.v.get(uv);
+    Eight<float> w;
+    w.load(static_cast<const float*>(a.m) + x.at, U::GAP, false, true, 0);
+    w.get(mv);
+    w.load(static_cast<const float*>(a.v) + x.at, U::GAP, false, true, 0);
+    w.get(uv);
   }
   x.param.get(pv);
   x.grad.get(gv);
-  [[maybe_unused]] float top_m = 0.f, top_u = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  // Sums as fma with the factor `one`: a packed product would be fused into them.
+  const auto moments = [&](int i) {
     const float2 gr = mul2(gv[i], both(f.grad));
-    if (EIGHT) uv[i] = mul2(uv[i], uv[i]);
-    // Sums as fma with the factor `one`: a packed product would be fused into them.
     mv[i] = ub::fma2(mul2(mv[i], both(a.b1)), both(a.one), mul2(gr, both(a.c1)));
     uv[i] = ub::fma2(mul2(uv[i], both(a.b2)), both(a.one), mul2(mul2(gr, gr), both(a.c2)));
-    if (EIGHT) top_m = top3(top_m, mv[i].x, mv[i].y);
-  }
-  float2 root_v[4];
-  if constexpr (EIGHT) {
-    roots(uv, root_v, top_u);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) root_v[i] = make_float2(__fsqrt_rn(uv[i].x), __fsqrt_rn(uv[i].y));
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 denom = ub::fma2(root_v[i], both(f.root), both(a.eps));
+  };
+  const auto param = [&](int i, float2 u) {
+    const float2 denom = ub::fma2(u, both(f.root), both(a.eps));
     const float2 step = mul2(mv[i], make_float2(reciprocal(denom.x), reciprocal(denom.y)));
     pv[i] = ub::fma2(step, both(-f.size), mul2(pv[i], both(f.decay)));
+  };
+  [[maybe_unused]] float top_m = 0.f, top_u = 0.f;
+  [[maybe_unused]] float2 root_v[4];
+  if constexpr (EIGHT) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uv[i] = mul2(uv[i], uv[i]);
+      moments(i);
+      top_m = top3(top_m, mv[i].x, mv[i].y);
+    }
+    roots(uv, root_v, top_u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) param(i, root_v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      moments(i);
+      param(i, make_float2(__fsqrt_rn(uv[i].x), __fsqrt_rn(uv[i].y)));
+    }
   }
   x.param.set(pv);
   x.param.store(x.p, U::GAP, U::ONE, x.full, x.left);
@@ -358,15 +365,16 @@ __device__ __forceinline__ void update(Unit<T, TG, EIGHT, N>& x, const StepArgs&
     }
     if (lane == 0) a.scales[x.at / BLOCK] = make_float2(top_m, top_u);
   } else {
-    x.m.set(mv);
-    x.m.store(static_cast<float*>(a.m) + x.at, U::GAP, false, true, 0);
-    x.v.set(uv);
-    x.v.store(static_cast<float*>(a.v) + x.at, U::GAP, false, true, 0);
+    Eight<float> w;
+    w.set(mv);
+    w.store(static_cast<float*>(a.m) + x.at, U::GAP, false, true, 0);
+    w.set(uv);
+    w.store(static_cast<float*>(a.v) + x.at, U::GAP, false, true, 0);
   }
 }
 
 template <typename T, typename TG, bool EIGHT, int N>
-__global__ void __launch_bounds__(THREADS, EIGHT ? EIGHT_CTAS : FULL_CTAS) adamw_kernel(
+__global__ void __launch_bounds__(THREADS, EIGHT ? eight_ctas(sizeof(T), sizeof(TG)) : FULL_CTAS) adamw_kernel(
     const __grid_constant__ Table<N> tab, const __grid_constant__ StepArgs a) {
   Factors f{a.decay, a.size, a.root, a.grad_scale ? *a.grad_scale : 1.f};
   if (!isfinite(f.grad)) return;  // an overflow somewhere in the gradients: nothing changes
@@ -388,26 +396,36 @@ __global__ void __launch_bounds__(THREADS, EIGHT ? EIGHT_CTAS : FULL_CTAS) adamw
     f.decay = computed[0], f.size = computed[1], f.root = computed[2];
   }
   const int lane = threadIdx.x & 31;
-  // Runs of a.run blocks per warp: the tensor is searched for at the first, and followed from there.
   const unsigned warps = gridDim.x * WARPS;
-  unsigned run = blockIdx.x * WARPS + (threadIdx.x >> 5), unit = run * a.run, end = min(unit + a.run, tab.total);
-  if (unit >= tab.total) return;
-  int k = tensor_of(tab, unit);
-  const auto advance = [&] {  // whether there is another block
-    if (++unit < end) {
-      while (unit >= tab.start[k + 1]) ++k;
-      return true;
+  unsigned run = blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (run >= tab.total) return;
+  if constexpr (!EIGHT) {
+    for (unsigned unit = run; unit < tab.total; unit += warps) {
+      Unit<T, TG, EIGHT, N> x;
+      x.fetch(tab, a, tensor_of(tab, unit), unit, lane);
+      update(x, a, f, lane);
     }
-    run += warps;
-    if (run > (tab.total - 1) / a.run) return false;
-    unit = run * a.run;
-    end = min(unit + a.run, tab.total);
-    k = tensor_of(tab, unit);
-    return true;
-  };
-  Unit<T, TG, EIGHT, N> x, y;
-  x.fetch(tab, a, k, unit, lane);
-  if constexpr (EIGHT) {  // long arithmetic: the next block is on its way meanwhile
+  } else {
+    // Runs of a.run blocks per warp: the tensor is searched for at the first, and followed from there.
+    unsigned unit = run * a.run, end = min(unit + a.run, tab.total);
+    if (unit >= tab.total) return;
+    const unsigned last = (tab.total - 1) / a.run;
+    int k = tensor_of(tab, unit);
+    const auto advance = [&] {  // whether there is another block
+      if (++unit < end) {
+        while (k + 1 < tab.count && unit >= tab.start[k + 1]) ++k;
+        return true;
+      }
+      run += warps;
+      if (run > last) return false;
+      unit = run * a.run;
+      end = min(unit + a.run, tab.total);
+      k = tensor_of(tab, unit);
+      return true;
+    };
+    // The arithmetic is long: the next block is on its way meanwhile.
+    Unit<T, TG, EIGHT, N> x, y;
+    x.fetch(tab, a, k, unit, lane);
     for (;;) {
       bool more = advance();
       if (more) y.fetch(tab, a, k, unit, lane);
@@ -418,30 +436,35 @@ __global__ void __launch_bounds__(THREADS, EIGHT ? EIGHT_CTAS : FULL_CTAS) adamw
       update(y, a, f, lane);
       if (!more) return;
     }
-  } else {
-    update(x, a, f, lane);
-    while (advance()) {
-      x.fetch(tab, a, k, unit, lane);
-      update(x, a, f, lane);
-    }
   }
 }
 
-// The values that 8-bit moments stand for. A warp per block.
+// The values that 8-bit moments stand for: 4096 of them per CTA, four times four per thread, all loads first.
+constexpr int VALUES = 4;
+
 __global__ void __launch_bounds__(THREADS) adamw_values_kernel(const uint8_t* m, const uint8_t* u, const float2* scales,
-                                                               float* m_out, float* v_out, unsigned blocks) {
-  const int lane = threadIdx.x & 31;
-  for (unsigned b = blockIdx.x * WARPS + (threadIdx.x >> 5); b < blocks; b += gridDim.x * WARPS) {
-    const float2 sc = scales[b];
+                                                               float* m_out, float* v_out, long long n) {
+  const long long first = blockIdx.x * (long long)(VALUES * THREADS * 4) + threadIdx.x * 4;
+  unsigned mc[VALUES], uc[VALUES];
+  float2 sc[VALUES];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const long long at = (long long)b * BLOCK + lane * 4 + j * 128;
-      const unsigned mc = *reinterpret_cast<const unsigned*>(m + at), uc = *reinterpret_cast<const unsigned*>(u + at);
-      const float2 m0 = mul2(m_values<0>(mc), both(sc.x)), m1 = mul2(m_values<1>(mc), both(sc.x));
-      float2 u0 = mul2(u_values<0>(uc), both(sc.y)), u1 = mul2(u_values<1>(uc), both(sc.y));
+  for (int i = 0; i < VALUES; ++i) {
+    const long long at = first + i * (THREADS * 4);
+    if (at < n) {
+      mc[i] = *reinterpret_cast<const unsigned*>(m + at);
+      uc[i] = *reinterpret_cast<const unsigned*>(u + at);
+      sc[i] = scales[at / BLOCK];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VALUES; ++i) {
+    const long long at = first + i * (THREADS * 4);
+    if (at < n) {
+      const float2 m0 = mul2(m_values<0>(mc[i]), both(sc[i].x)), m1 = mul2(m_values<1>(mc[i]), both(sc[i].x));
+      float2 u0 = mul2(u_values<0>(uc[i]), both(sc[i].y)), u1 = mul2(u_values<1>(uc[i]), both(sc[i].y));
       u0 = mul2(u0, u0), u1 = mul2(u1, u1);
-      __stcs(reinterpret_cast<float4*>(m_out + at), make_float4(m0.x, m0.y, m1.x, m1.y));
-      __stcs(reinterpret_cast<float4*>(v_out + at), make_float4(u0.x, u0.y, u1.x, u1.y));
+      *reinterpret_cast<float4*>(m_out + at) = make_float4(m0.x, m0.y, m1.x, m1.y);
+      *reinterpret_cast<float4*>(v_out + at) = make_float4(u0.x, u0.y, u1.x, u1.y);
     }
   }
 }
@@ -520,7 +543,7 @@ Table<N> make_table(const UnblendAdamWTensor* t, int count, int unit) {
     tab.start[i] = at;
     at += (unsigned)((t[i].n + unit - 1) / unit);
   }
-  tab.total = tab.start[count] = at;
+  tab.total = at;
   return tab;
 }
 
@@ -567,7 +590,7 @@ unsigned grid_of(unsigned units, int per_sm) {
 template <typename T, typename TG, bool EIGHT, int N>
 int launch_table(const UnblendAdamWTensor* t, int count, StepArgs a, cudaStream_t st) {
   const Table<N> tab = make_table<N>(t, count, BLOCK);
-  const unsigned grid = grid_of(tab.total, EIGHT ? EIGHT_CTAS : 2 * FULL_CTAS);
+  const unsigned grid = grid_of(tab.total, EIGHT ? eight_ctas(sizeof(T), sizeof(TG)) : 2 * FULL_CTAS);
   if (EIGHT) a.run = std::min(16u, std::max(1u, tab.total / (grid * WARPS * 4)));  // four runs per warp at least
   adamw_kernel<T, TG, EIGHT, N><<<grid, THREADS, 0, st>>>(tab, a);
   UB_CHECK_LAUNCH();
@@ -677,9 +700,10 @@ extern "C" int unblend_adamw_values(const void* exp_avg, const void* exp_avg_sq,
   UB_REQUIRE(exp_avg && exp_avg_sq && scales && m && v && blocks >= 1 && blocks < (1LL << 31));
   UB_REQUIRE(aligned16(exp_avg) && aligned16(exp_avg_sq) && aligned16(m) && aligned16(v) &&
              reinterpret_cast<uintptr_t>(scales) % 8 == 0);
-  adamw_values_kernel<<<grid_of((unsigned)blocks, 8), THREADS, 0, ub::as_stream(stream)>>>(
+  const long long n = blocks * BLOCK, per_cta = VALUES * THREADS * 4;
+  adamw_values_kernel<<<(unsigned)((n + per_cta - 1) / per_cta), THREADS, 0, ub::as_stream(stream)>>>(
       static_cast<const uint8_t*>(exp_avg), static_cast<const uint8_t*>(exp_avg_sq),
-      reinterpret_cast<const float2*>(scales), m, v, (unsigned)blocks);
+      reinterpret_cast<const float2*>(scales), m, v, n);
   UB_CHECK_LAUNCH();
   return 0;
 }
