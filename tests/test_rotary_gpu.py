@@ -389,3 +389,22 @@ def test_in_front_of_attention(t):
         rel = float((y.double() - w).norm() / w.norm())
         assert rel <= 10 * half(t) + 2e-6, rel
     assert _lib.error_flag() == 0
+
+
+def test_packed_parameters():
+    """The parameters that a call passes: sizes, strides and addresses of what it was given."""
+    q, k = torch.zeros(2, 3, 5, 4, 16, device="cuda")[:, 1:], torch.zeros(2, 2, 5, 2, 18, device="cuda")[..., :16]
+    f, pos = torch.ones(8, dtype=F64, device="cuda"), torch.zeros(2, 2, 5, dtype=torch.int64, device="cuda")
+    w, lens = torch.ones(16, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    dq, dk = torch.zeros(q.shape, device="cuda"), torch.zeros(k.shape, device="cuda")
+    q_out, k_out, at, p, _ = _lib.tensor_lists().heads(dq, dk, w, None, f, pos, False, 0.5, 1e-3, lens, q, k)
+    assert at == tuple(x.data_ptr() for x in (dq, dk, q, k, q_out, k_out))
+    p = _lib.RotaryParams.from_buffer_copy(p)
+    got = {n: getattr(p, n) for n, _ in p._fields_ if n not in ("q", "k", "q0", "k0")}
+    assert got.pop("eps") == pytest.approx(1e-3)
+    assert got == dict(dtype=0, outer=2, inner=2, length=5, heads=4, k_heads=2, hd=16, pairs=8, half=1, scale=0.5,
+                       freqs=f.data_ptr(), freqs_f64=1, positions_i64=1, positions=pos.data_ptr(), positions_stride=5,
+                       gamma_q=w.data_ptr(), gamma_k=None, w_dtype=0, lens=lens.data_ptr())
+    strides = [tuple(getattr(getattr(p, n), m) for m in ("outer", "inner", "row", "head"))
+               for n in ("q", "k", "q0", "k0")]
+    assert strides == [(640, 320, 64, 16), (320, 160, 32, 16), (960, 320, 64, 16), (360, 180, 36, 18)]

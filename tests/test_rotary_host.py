@@ -59,7 +59,8 @@ def test_rotary_refuses():
                     lambda: call(q, k, f, [0, 1, 2, 3, 4]), lambda: call(q, k, f, scale=math.inf),
                     lambda: call(q, k, f, scale=math.nan), lambda: call(q, k, f, scale=1e39),
                     lambda: call(torch.zeros(1, 1, 1, 257), None, f), lambda: call(torch.zeros(1, 1, 1, 0), None, f),
-                    lambda: call(q, k, f.clone().requires_grad_()), lambda: call([1.0], None, f),
+                    lambda: call(q, k, f.clone().requires_grad_()),
+                    lambda: call(q.clone().requires_grad_(), k, f.clone().requires_grad_()), lambda: call([1.0], None, f),
                     lambda: call(torch.zeros(1, 1, 1, 1).expand(1 << 16, 1 << 15, 1, 1), None, f[:0])):
             with pytest.raises(ValueError):
                 bad()
@@ -134,20 +135,6 @@ def test_param_struct_layout(tmp_path):
     test_param_struct_layout_matches_c(tmp_path, _lib.RotaryParams, "UnblendRotaryParams")
 
 
-def test_packed_parameters():
-    """The bytes that the calls pass are the structure's."""
-    assert training._ROTARY_PARAMS.size == ctypes.sizeof(_lib.RotaryParams)
-    q, k = torch.zeros(2, 3, 5, 4, 16)[:, 1:], torch.zeros(2, 2, 5, 2, 18)[..., :16]
-    f, pos, w = torch.ones(8, dtype=torch.float64), torch.zeros(2, 2, 5, dtype=torch.int64), torch.ones(16)
-    lens = torch.zeros(4, dtype=torch.int32)
-    p, held = training._rotary_params(q, k, f, pos, False, 0.5, k, q, w, None, 1e-3, lens)
-    p = _lib.RotaryParams.from_buffer_copy(p)
-    got = {n: getattr(p, n) for n, _ in p._fields_ if n not in ("q", "k", "q0", "k0")}
-    assert got.pop("eps") == pytest.approx(1e-3)
-    assert got == dict(dtype=0, outer=2, inner=2, length=5, heads=4, k_heads=2, hd=16, pairs=8, half=1, scale=0.5,
-                       freqs=f.data_ptr(), freqs_f64=1, positions_i64=1, positions=pos.data_ptr(), positions_stride=5,
-                       gamma_q=w.data_ptr(), gamma_k=None, w_dtype=0, lens=lens.data_ptr())
-    strides = [tuple(getattr(getattr(p, n), m) for m in ("outer", "inner", "row", "head"))
-               for n in ("q", "k", "q0", "k0")]
-    assert strides == [(960, 320, 64, 16), (360, 180, 36, 18), (360, 180, 36, 18), (960, 320, 64, 16)]
-    assert training._rotary_workspace_bytes(bytes(p)[:training._ROTARY_SIZES]) >= 2 * 16 * 4
+def test_workspace_by_the_sizes_alone():
+    p = bytes(_params(pairs=8, freqs=16))
+    assert training._rotary_workspace_bytes(p[:training._ROTARY_SIZES]) >= 2 * 64 * 4

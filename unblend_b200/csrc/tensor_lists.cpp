@@ -1,9 +1,13 @@
-// Checks of lists of tensors and their tables for the entry points that take many tensors at once (unblend_adamw_step,
-// unblend_grad_norm), as a Python extension: a model has hundreds of parameters, and a dozen attributes of each cost 1.5
-// us a tensor from Python (675 parameters: 1.0 ms, twice what the update takes on the GPU), 0.1 us from here.
+// The host side of operators whose arguments take longer to check from Python than the GPU takes to work on them, as a Python
+// extension. Lists of tensors (unblend_adamw_step, unblend_grad_norm): a model has hundreds of parameters, and a dozen
+// attributes of each cost 1.5 us a tensor from Python (675 parameters: 1.0 ms, twice the update's time on the GPU), 0.05 us
+// from here. Heads of queries and keys (the rotary operators): the checks, outputs and parameters of a call.
+#define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -172,10 +176,235 @@ PyObject* changed(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   Py_RETURN_NONE;
 }
 
+// ------------------------------------------------------------------------------------------ heads of queries and keys
+
+constexpr int64_t MAX_HD = 256, MOST_ROWS = INT64_C(1) << 31;
+constexpr double F32_MAX = 3.4028234663852886e38;
+
+const at::Tensor* tensor(PyObject* o) { return o == Py_None ? nullptr : &THPVariable_Unpack(o); }
+
+std::string shape(const at::Tensor& t) { return text(t.sizes()); }
+
+// A tensor of one of the three types; `like`: on its device.
+bool element_ok(const char* name, PyObject* o, const at::Tensor* like) {
+  const std::string n(name);
+  if (!THPVariable_Check(o)) return raised(n + " must be a tensor, got " + Py_TYPE(o)->tp_name);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.layout() != at::kStrided) return raised(n + " must be a dense tensor");
+  if (type_of(t) < 0)
+    return raised(n + " must be float32, bfloat16 or float16, got " + std::string(toString(t.scalar_type())));
+  if (t.is_neg()) return raised(n + " is a lazily negated view: give " + n + ".resolve_neg()");
+  if (like && t.device() != like->device())
+    return raised(n + " is on " + t.device().str() + ", expected " + like->device().str());
+  return true;
+}
+
+bool heads_ok(const char* name, PyObject* o, const at::Tensor* q) {
+  if (!element_ok(name, o, q)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.dim() != 4 && t.dim() != 5)
+    return raised(std::string(name) +
+                  " must be [batch, length, heads, head_dim] or [outer, inner, length, heads, head_dim], got shape " +
+                  shape(t));
+  if (q && t.scalar_type() != q->scalar_type())
+    return raised(std::string(name) + " must be of q's type " + std::string(toString(q->scalar_type())) + ", got " +
+                  std::string(toString(t.scalar_type())));
+  return true;
+}
+
+bool weight_ok(const char* name, PyObject* o, const at::Tensor& q) {
+  if (!element_ok(name, o, &q)) return false;
+  const at::Tensor& w = THPVariable_Unpack(o);
+  if (w.scalar_type() != at::kFloat && w.scalar_type() != q.scalar_type())
+    return raised(std::string(name) + " must be float32 or of its input's type, got " +
+                  std::string(toString(w.scalar_type())));
+  if (w.dim() != 1 || w.size(0) != q.size(-1))
+    return raised(std::string(name) + " must have shape (" + std::to_string(q.size(-1)) + ",), got " + shape(w));
+  return true;
+}
+
+bool is_number(PyObject* o) { return PyFloat_Check(o) || PyLong_Check(o); }
+
+// Arguments of a call, in this order.
+enum Arg { Q, K, GAMMA_Q, GAMMA_K, FREQS, POSITIONS, INTERLEAVED, SCALE, EPS, LENS, N_ARGS };
+
+struct Call {
+  const at::Tensor *q, *k, *gamma[2], *freqs, *positions, *lens;
+  bool half;
+  double scale, eps;
+};
+
+bool read(PyObject* const* o, const char* const (&names)[2], Call& c) {
+  if (!heads_ok(names[0], o[Q], nullptr)) return false;
+  c.q = tensor(o[Q]), c.k = nullptr;
+  const at::Tensor& q = *c.q;
+  const int64_t dims = q.dim(), hd = q.size(-1);
+  if (o[K] != Py_None) {
+    if (!heads_ok(names[1], o[K], c.q)) return false;
+    c.k = tensor(o[K]);
+    if (c.k->dim() != dims || c.k->size(-1) != hd || c.k->sizes().slice(0, dims - 2) != q.sizes().slice(0, dims - 2))
+      return raised("q " + shape(q) + " and k " + shape(*c.k) + " must agree but for their heads");
+  }
+  if (hd < 1 || hd > MAX_HD)
+    return raised("head_dim must be 1 to " + std::to_string(MAX_HD) + ", got " + std::to_string(hd));
+  c.freqs = c.positions = c.lens = nullptr;
+  if (o[FREQS] != Py_None) {
+    c.freqs = THPVariable_Check(o[FREQS]) ? tensor(o[FREQS]) : nullptr;
+    if (!c.freqs || (c.freqs->scalar_type() != at::kFloat && c.freqs->scalar_type() != at::kDouble) ||
+        c.freqs->dim() != 1 || c.freqs->device() != q.device())
+      return raised("freqs must be a float32 or float64 tensor [pairs] on " + q.device().str());
+    if (2 * c.freqs->numel() > hd)
+      return raised(std::to_string(c.freqs->numel()) + " pairs do not fit into head_dim " + std::to_string(hd));
+    if (c.freqs->is_neg()) return raised("freqs is a lazily negated view: give freqs.resolve_neg()");
+    if (c.freqs->requires_grad() && at::GradMode::is_enabled())
+      return raised("freqs has no gradient here: give freqs.detach()");
+  }
+  if (o[POSITIONS] != Py_None) {
+    c.positions = THPVariable_Check(o[POSITIONS]) ? tensor(o[POSITIONS]) : nullptr;
+    if (!c.positions || (c.positions->scalar_type() != at::kInt && c.positions->scalar_type() != at::kLong) ||
+        c.positions->device() != q.device())
+      return raised("positions must be an int32 or int64 tensor on " + q.device().str());
+    const auto all = q.sizes().slice(0, dims - 2), row = q.sizes().slice(dims - 3, 1);
+    if (c.positions->sizes() != all && c.positions->sizes() != row)
+      return raised("positions must have shape " + text(row) + " or " + text(all) + ", got " + shape(*c.positions));
+  }
+  if (!is_number(o[EPS]) || !((c.eps = PyFloat_AsDouble(o[EPS])) >= 0 && c.eps <= F32_MAX)) {
+    PyErr_Clear();
+    return raised("eps must be >= 0");
+  }
+  c.scale = PyFloat_AsDouble(o[SCALE]);
+  if (c.scale == -1.0 && PyErr_Occurred()) return false;
+  if (!(c.scale >= -F32_MAX && c.scale <= F32_MAX))
+    return raised("scale must be finite in float32, got " + std::to_string(c.scale));
+  if (q.numel() >= MOST_ROWS * hd || (c.k && c.k->numel() >= MOST_ROWS * hd))
+    return raised("q and k must have fewer than 2^31 rows each, got shapes " + shape(q) +
+                  (c.k ? " and " + shape(*c.k) : ""));
+  static const char* const weights[2] = {"gamma_q", "gamma_k"};
+  for (int i = 0; i < 2; ++i) {
+    c.gamma[i] = nullptr;
+    if (o[GAMMA_Q + i] == Py_None) continue;
+    if (!weight_ok(weights[i], o[GAMMA_Q + i], q)) return false;
+    c.gamma[i] = tensor(o[GAMMA_Q + i]);
+  }
+  if (c.gamma[1] && !c.k) return raised("gamma_k needs k");
+  if (c.gamma[0] && c.gamma[1] && c.gamma[0]->scalar_type() != c.gamma[1]->scalar_type())
+    return raised("gamma_q and gamma_k must share a type");
+  if (o[LENS] != Py_None) {
+    c.lens = THPVariable_Check(o[LENS]) ? tensor(o[LENS]) : nullptr;
+    const int64_t seqs = q.size(0) * (dims == 5 ? q.size(1) : 1);
+    if (!c.lens || c.lens->scalar_type() != at::kInt || c.lens->device() != q.device())
+      return raised("lens must be an int32 tensor on " + q.device().str());
+    if (c.lens->numel() != seqs)
+      return raised("lens must hold one length for each of " + std::to_string(seqs) + " sequences, got " +
+                    std::to_string(c.lens->numel()));
+  }
+  const int truth = PyObject_IsTrue(o[INTERLEAVED]);
+  if (truth < 0) return false;
+  c.half = !truth;
+  return true;
+}
+
+// A tensor as the kernels take it: unit last stride.
+at::Tensor unit(const at::Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+UnblendHeadStrides strides(const at::Tensor& t) {
+  const int64_t d = t.dim();
+  return UnblendHeadStrides{t.stride(0), d == 5 ? t.stride(1) : 0, t.stride(d - 3), t.stride(d - 2)};
+}
+
+long long pointer(const at::Tensor& t) { return (long long)reinterpret_cast<uintptr_t>(t.const_data_ptr()); }
+
+PyObject* wrap(const at::Tensor& t) {
+  if (t.defined()) return THPVariable_Wrap(t);
+  Py_RETURN_NONE;
+}
+
+// heads(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens[, q0, k0])
+//   -> None for a side without elements or tensors off the GPU, after the checks; else
+//      (q_out, k_out, (addresses of q, k, [q0, k0,] q_out, k_out), UnblendRotaryParams, tensors that it points to)
+//
+// With q0 and k0, q and k are the gradients of the norm's outputs for those inputs.
+PyObject* heads(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
+  if (n_args != N_ARGS && n_args != N_ARGS + 2) return refuse("heads: wrong number of arguments");
+  try {
+    Call c;
+    const bool backward = n_args > N_ARGS;
+    const char* const names[2] = {backward ? "dq" : "q", backward ? "dk" : "k"};
+    if (!read(o, names, c)) return nullptr;
+    if (backward) {
+      for (int i = 0; i < 2; ++i) {
+        if ((o[N_ARGS + i] == Py_None) != (o[i] == Py_None))
+          return refuse(std::string(names[i]) + " must be given with its input, and only then");
+        if (o[i] == Py_None) continue;
+        if (!heads_ok(names[i] + 1, o[N_ARGS + i], c.q)) return nullptr;
+        if (THPVariable_Unpack(o[N_ARGS + i]).sizes() != THPVariable_Unpack(o[i]).sizes())
+          return refuse(std::string(names[i]) + " must have shape " + shape(THPVariable_Unpack(o[N_ARGS + i])) + ", got " +
+                        shape(THPVariable_Unpack(o[i])));
+      }
+    }
+    if (!c.q->is_cuda() || c.q->numel() == 0 || (c.k && c.k->numel() == 0)) Py_RETURN_NONE;
+    const at::NoGradGuard no_grad;
+    const int64_t d = c.q->dim();
+    const at::Tensor q = unit(*c.q), k = c.k ? unit(*c.k) : at::Tensor();
+    const at::Tensor q0 = backward ? unit(THPVariable_Unpack(o[N_ARGS])) : at::Tensor();
+    const at::Tensor k0 = backward && c.k ? unit(THPVariable_Unpack(o[N_ARGS + 1])) : at::Tensor();
+    at::Tensor freqs, positions, gammas[2], lens;
+    UnblendRotaryParams p{};
+    p.dtype = type_of(q);
+    p.outer = (int)q.size(0);
+    p.inner = d == 5 ? (int)q.size(1) : 1;
+    p.length = (int)q.size(d - 3);
+    p.heads = (int)q.size(d - 2);
+    p.k_heads = c.k ? (int)k.size(d - 2) : 0;
+    p.hd = (int)q.size(d - 1);
+    p.half = c.half;
+    p.scale = (float)c.scale;
+    p.eps = (float)c.eps;
+    if (c.freqs) {
+      freqs = c.freqs->contiguous();
+      p.pairs = (int)freqs.numel();
+      p.freqs = freqs.const_data_ptr();
+      p.freqs_f64 = freqs.scalar_type() == at::kDouble;
+    }
+    if (c.positions) {
+      positions = c.positions->contiguous();
+      p.positions = positions.const_data_ptr();
+      p.positions_i64 = positions.scalar_type() == at::kLong;
+      p.positions_stride = positions.dim() > 1 ? p.length : 0;
+    }
+    for (int i = 0; i < 2; ++i) {
+      if (!c.gamma[i]) continue;
+      gammas[i] = c.gamma[i]->contiguous();
+      p.w_dtype = type_of(gammas[i]);
+      (i ? p.gamma_k : p.gamma_q) = gammas[i].const_data_ptr();
+    }
+    if (c.lens) {
+      lens = c.lens->contiguous();
+      p.lens = lens.const_data_ptr<int>();
+    }
+    p.q = strides(q);
+    if (c.k) p.k = strides(k);
+    if (backward) p.q0 = strides(q0);
+    if (backward && c.k) p.k0 = strides(k0);
+    const at::Tensor q_out = at::empty(q.sizes(), q.options());
+    const at::Tensor k_out = c.k ? at::empty(k.sizes(), k.options()) : at::Tensor();
+    const auto address = [](const at::Tensor& t) { return t.defined() ? pointer(t) : 0LL; };
+    PyObject* at_ = backward ? Py_BuildValue("(LLLLLL)", address(q), address(k), address(q0), address(k0),
+                                             address(q_out), address(k_out))
+                             : Py_BuildValue("(LLLL)", address(q), address(k), address(q_out), address(k_out));
+    return Py_BuildValue("(NNNy#(NNNNNNNNN))", wrap(q_out), wrap(k_out), at_, reinterpret_cast<const char*>(&p),
+                         (Py_ssize_t)sizeof(p), wrap(q), wrap(k), wrap(q0), wrap(k0), wrap(freqs), wrap(positions),
+                         wrap(gammas[0]), wrap(gammas[1]), wrap(lens));
+  } catch (const std::exception& e) {
+    return refuse(std::string("q and k: ") + e.what());
+  }
+}
+
 PyMethodDef methods[] = {
     {"sizes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sizes)), METH_FASTCALL, nullptr},
     {"table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(table)), METH_FASTCALL, nullptr},
     {"changed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(changed)), METH_FASTCALL, nullptr},
+    {"heads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(heads)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

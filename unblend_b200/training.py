@@ -25,7 +25,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-import struct
 from collections.abc import Sequence
 from functools import lru_cache
 from typing import NamedTuple
@@ -37,11 +36,6 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 MAX_HEAD_DIM = 128
-MAX_ROTARY_DIM = 256
-_FREQ_DTYPES = (torch.float32, torch.float64)
-_POSITION_DTYPES = (torch.int32, torch.int64)
-# UnblendRotaryParams: packed here, as building the ctypes structure takes four times as long.
-_ROTARY_PARAMS = struct.Struct("@9if P2i P17q 2Pif P")
 _ROTARY_SIZES = _lib.RotaryParams.scale.offset  # bytes of the fields that say how large a call is
 ADAMW_BLOCK = 256  # elements of a moment that share a scale in 8 bits; each parameter starts a block of its own
 _TABLE, _TABLE_ROW = 896, 32  # tensors of one launch; bytes of UnblendAdamWTensor
@@ -503,86 +497,6 @@ def rotary_freqs(dims: int, base: float = 10000.0, factor: float = 1.0, method: 
     return f.to(device) if device is not None else f
 
 
-def _check_rotary(q, k, freqs, positions, scale, eps: float = 0.0) -> float:
-    _check_heads("q", q)
-    shape = q.shape
-    rows, hd = shape[:-2], shape[-1]
-    if k is not None:
-        _check_heads("k", k, q)
-        if k.shape[:-2] != rows or k.shape[-1] != hd:
-            raise ValueError(f"q {tuple(shape)} and k {tuple(k.shape)} must agree but for their heads")
-    if not 1 <= hd <= MAX_ROTARY_DIM:
-        raise ValueError(f"head_dim must be 1 to {MAX_ROTARY_DIM}, got {hd}")
-    if freqs is not None:
-        if not isinstance(freqs, torch.Tensor) or freqs.dtype not in _FREQ_DTYPES or freqs.dim() != 1 or \
-                freqs.device != q.device:
-            raise ValueError(f"freqs must be a float32 or float64 tensor [pairs] on {q.device}")
-        if 2 * freqs.numel() > hd:
-            raise ValueError(f"{freqs.numel()} pairs do not fit into head_dim {hd}")
-        if freqs.is_neg():
-            raise ValueError("freqs is a lazily negated view: give freqs.resolve_neg()")
-        if freqs.requires_grad and torch.is_grad_enabled():
-            raise ValueError("freqs has no gradient here: give freqs.detach()")
-    if positions is not None:
-        if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_DTYPES or \
-                positions.device != q.device:
-            raise ValueError(f"positions must be an int32 or int64 tensor on {q.device}")
-        if positions.shape not in (rows, rows[-1:]):
-            raise ValueError(f"positions must have shape {tuple(rows[-1:])} or {tuple(rows)}, got "
-                             f"{tuple(positions.shape)}")
-    if not (isinstance(eps, (int, float)) and 0 <= eps <= _F32_MAX):
-        raise ValueError(f"eps must be >= 0, got {eps!r}")
-    scale = float(scale)
-    if not abs(scale) <= _F32_MAX:
-        raise ValueError(f"scale must be finite in float32, got {scale}")
-    if q.numel() >= _MOST * hd or (k is not None and k.numel() >= _MOST * hd):
-        raise ValueError(f"q and k must have fewer than 2^31 rows each, got shapes {tuple(shape)}"
-                         + (f" and {tuple(k.shape)}" if k is not None else ""))
-    return scale
-
-
-def _four_strides(t) -> tuple[int, int, int, int]:
-    """(outer, inner, row, head), as ``HeadStrides``."""
-    s = t.stride()
-    return s[0], s[1] if len(s) == 5 else 0, s[-3], s[-2]
-
-
-def _rotary_params(q, k, freqs, positions, interleaved: bool, scale: float, q0=None, k0=None, gamma_q=None,
-                   gamma_k=None, eps: float = 0.0, lens=None) -> tuple[bytes, tuple]:
-    """``UnblendRotaryParams`` of a call on checked tensors with unit last strides, and the tensors that it points to."""
-    s = q.shape
-    five = len(s) == 5
-    f_ptr = pairs = f64 = p_ptr = p64 = per_seq = lens_ptr = 0
-    held = []
-    if freqs is not None:
-        freqs = freqs.contiguous()
-        f_ptr, pairs, f64 = freqs.data_ptr(), freqs.numel(), freqs.dtype == torch.float64
-        held.append(freqs)
-    if positions is not None:
-        if positions.dim() > 1:
-            per_seq = s[-3]
-        positions = positions.contiguous()
-        p_ptr, p64 = positions.data_ptr(), positions.dtype == torch.int64
-        held.append(positions)
-    w_dtype, gammas = _lib.DTYPE_F32, [0, 0]
-    for i, g in enumerate((gamma_q, gamma_k)):
-        if g is not None:
-            g = g.contiguous()
-            gammas[i], w_dtype = g.data_ptr(), _DTYPES[g.dtype]
-            held.append(g)
-    if lens is not None:
-        lens = lens.contiguous()
-        lens_ptr = lens.data_ptr()
-        held.append(lens)
-    none = (0, 0, 0, 0)
-    p = _ROTARY_PARAMS.pack(
-        _DTYPES[q.dtype], s[0], s[1] if five else 1, s[-3], s[-2], 0 if k is None else k.shape[-2], s[-1], pairs,
-        not interleaved, scale, f_ptr, f64, p64, p_ptr, per_seq, *_four_strides(q),
-        *(none if k is None else _four_strides(k)), *(none if q0 is None else _four_strides(q0)),
-        *(none if k0 is None else _four_strides(k0)), *gammas, w_dtype, eps, lens_ptr)
-    return p, tuple(held)
-
-
 @lru_cache(maxsize=4096)
 def _rotary_workspace_bytes(sizes: bytes) -> int:
     """Workspace of the norm's backward pass, by the leading fields of ``UnblendRotaryParams``."""
@@ -594,18 +508,25 @@ def _rotary_workspace_bytes(sizes: bytes) -> int:
     return n.value
 
 
+def _heads(*args):
+    """The checks of a call on heads, and its outputs and parameters (None for a side without elements, or on the CPU)."""
+    return _lib.tensor_lists().heads(*args)
+
+
 def _rotate(q, k, freqs, positions, interleaved: bool, scale: float, inverse: bool):
-    """The rotation of checked arguments. A side without heads, or None, is left out."""
-    q_out = _empty(q)
-    k_out = None if k is None else _empty(k)
-    if q.numel() == 0:  # q without heads: k alone
-        if k is not None and k.numel():
+    got = _heads(q, k, None, None, freqs, positions, interleaved, scale, 0.0, None)
+    if freqs is None:
+        raise ValueError("freqs must be a float32 or float64 tensor [pairs]")
+    if got is None:  # a side without heads is left out
+        _check_cuda("q", q)
+        q_out, k_out = _empty(q), None if k is None else _empty(k)
+        if q.numel():
+            q_out = _rotate(q, None, freqs, positions, interleaved, scale, inverse)[0]
+        elif k is not None and k.numel():
             k_out = _rotate(k, None, freqs, positions, interleaved, scale, inverse)[0]
         return q_out, k_out
-    q = _unit(q)
-    k = None if k is None or k.numel() == 0 else _unit(k)
-    p, held = _rotary_params(q, k, freqs, positions, interleaved, scale)
-    _launch(q, "unblend_rotary", q.data_ptr(), _lib.ptr(k), q_out.data_ptr(), _lib.ptr(k_out), p, inverse)
+    q_out, k_out, at, p, _held = got
+    _launch(q_out, "unblend_rotary", *at, p, inverse)
     return q_out, k_out
 
 
@@ -623,25 +544,22 @@ def rotary_forward(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor,
     int64) are ``[length]`` for all sequences or one row for each, ``q.shape[:-2]``; None counts rows from 0. Angles are
     formed and reduced in 64 bits, so that positions below 2^53 lose nothing.
     """
-    scale = _check_rotary(q, k, freqs, positions, scale)
-    _check_freqs(freqs)
-    _check_cuda("q", q)
     return _rotate(q, k, freqs, positions, interleaved, scale, False)
-
-
-def _check_freqs(freqs) -> None:
-    if freqs is None:
-        raise ValueError("freqs must be a float32 or float64 tensor [pairs]")
 
 
 def rotary_backward(dq: torch.Tensor, dk: torch.Tensor | None, freqs: torch.Tensor,
                     positions: torch.Tensor | None = None, interleaved: bool = True, scale: float = 1.0
                     ) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Gradients of the inputs of ``rotary_forward`` from those of its outputs: the transposed rotation."""
-    scale = _check_rotary(dq, dk, freqs, positions, scale)
-    _check_freqs(freqs)
-    _check_cuda("dq", dq)
     return _rotate(dq, dk, freqs, positions, interleaved, scale, True)
+
+
+def _tracked(what: str, freqs, *tensors) -> bool:
+    """As ``_wants_grad``, of arguments that are yet to be checked."""
+    if isinstance(freqs, torch.Tensor) and freqs.requires_grad and torch.is_grad_enabled():
+        raise ValueError("freqs has no gradient here: give freqs.detach()")
+    tensors = [t for t in tensors if isinstance(t, torch.Tensor)]
+    return _wants_grad(what, *tensors) and all(t.is_cuda for t in tensors)
 
 
 class _Rotary(torch.autograd.Function):
@@ -671,29 +589,13 @@ class _Rotary(torch.autograd.Function):
 def rotary(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions: torch.Tensor | None = None,
            interleaved: bool = True, scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Differentiable rotary positions of queries and keys (arguments as ``rotary_forward``)."""
-    scale = _check_rotary(q, k, freqs, positions, scale)
-    _check_freqs(freqs)
-    if _wants_grad("rotary", q, k):
-        _check_cuda("q", q)
+    if _tracked("rotary", freqs, q, k):
         _refuse_capture("rotary")
         return _Rotary.apply(q, k, freqs, positions, interleaved, scale)
     return rotary_forward(q, k, freqs, positions, interleaved, scale)
 
 
 # ------------------------------------------------------------------------ norm of queries and keys, rotary
-
-
-def _check_qk_norm(q, k, gamma_q, gamma_k, freqs, positions, scale, eps, lens) -> float:
-    scale = _check_rotary(q, k, freqs, positions, scale, eps)
-    for name, w in (("gamma_q", gamma_q), ("gamma_k", gamma_k)):
-        if w is not None:
-            _check_weight(name, w, q)
-    if gamma_k is not None and k is None:
-        raise ValueError("gamma_k needs k")
-    if gamma_q is not None and gamma_k is not None and gamma_q.dtype != gamma_k.dtype:
-        raise ValueError(f"gamma_q and gamma_k must share a type, got {gamma_q.dtype} and {gamma_k.dtype}")
-    _check_lens("lens", lens, _seqs(q), q)
-    return scale
 
 
 def qk_norm_rotary_forward(q: torch.Tensor, k: torch.Tensor | None, gamma_q: torch.Tensor | None = None,
@@ -708,22 +610,22 @@ def qk_norm_rotary_forward(q: torch.Tensor, k: torch.Tensor | None, gamma_q: tor
     sequence) are the sequences' lengths in a padded batch: rows behind them are not read, whatever they hold, and come
     out as 0. Other arguments as in ``rotary_forward``.
     """
-    scale = _check_qk_norm(q, k, gamma_q, gamma_k, freqs, positions, scale, eps, lens)
-    _check_cuda("q", q)
     return _qk_norm_forward(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
 
 
-def _qk_norm_forward(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens):
-    q_out = _empty(q)
-    k_out = None if k is None else _empty(k)
-    if q.numel() == 0:
-        if k is not None and k.numel():
-            k_out = _qk_norm_forward(k, None, gamma_k, None, freqs, positions, interleaved, scale, eps, lens)[0]
+def _qk_norm_forward(q, k, gamma_q, gamma_k, *args):
+    """``args``: freqs, positions, interleaved, scale, eps, lens."""
+    got = _heads(q, k, gamma_q, gamma_k, *args)
+    if got is None:
+        _check_cuda("q", q)
+        q_out, k_out = _empty(q), None if k is None else _empty(k)
+        if q.numel():
+            q_out = _qk_norm_forward(q, None, gamma_q, None, *args)[0]
+        elif k is not None and k.numel():
+            k_out = _qk_norm_forward(k, None, gamma_k, None, *args)[0]
         return q_out, k_out
-    q = _unit(q)
-    k = None if k is None or k.numel() == 0 else _unit(k)
-    p, held = _rotary_params(q, k, freqs, positions, interleaved, scale, None, None, gamma_q, gamma_k, eps, lens)
-    _launch(q, "unblend_qk_norm_rotary_forward", q.data_ptr(), _lib.ptr(k), q_out.data_ptr(), _lib.ptr(k_out), p)
+    q_out, k_out, at, p, _held = got
+    _launch(q_out, "unblend_qk_norm_rotary_forward", *at, p)
     return q_out, k_out
 
 
@@ -738,40 +640,30 @@ def qk_norm_rotary_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.
     The weights' gradients have the weights' type; they are None without the weight or with ``weight_grads=False``. Rows
     behind ``lens`` are 0 and add to no gradient.
     """
-    scale = _check_qk_norm(q, k, gamma_q, gamma_k, freqs, positions, scale, eps, lens)
-    for name, d, x in (("dq", dq, q), ("dk", dk, k)):
-        if (d is None) != (x is None):
-            raise ValueError(f"{name} must be given with its input, and only then")
-        if d is not None:
-            _check_heads(name, d, q)
-            if d.shape != x.shape:
-                raise ValueError(f"{name} must have shape {tuple(x.shape)}, got {tuple(d.shape)}")
-    _check_cuda("q", q)
-    return _qk_norm_backward(dq, dk, q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens,
-                             weight_grads)
+    return _qk_norm_backward(dq, dk, q, k, weight_grads, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps,
+                             lens)
 
 
-def _qk_norm_backward(dq, dk, q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens, weight_grads):
-    weight_grads = weight_grads and (gamma_q is not None or gamma_k is not None)
-    dq_out = _empty(q)
-    dk_out = None if k is None else _empty(k)
-    if q.numel() == 0:
-        dgamma_k = _empty(gamma_k).zero_() if weight_grads and gamma_k is not None else None
-        if k is not None and k.numel():
-            dk_out, _, dgamma_k, _ = _qk_norm_backward(dk, None, k, None, gamma_k, None, freqs, positions, interleaved,
-                                                       scale, eps, lens, weight_grads)
-        return dq_out, dk_out, _empty(gamma_q).zero_() if weight_grads and gamma_q is not None else None, dgamma_k
-    q, dq = _unit(q), _unit(dq)
-    k, dk = (None, None) if k is None or k.numel() == 0 else (_unit(k), _unit(dk))
-    p, held = _rotary_params(dq, dk, freqs, positions, interleaved, scale, q, k, gamma_q, gamma_k, eps, lens)
+def _qk_norm_backward(dq, dk, q, k, weight_grads: bool, gamma_q, gamma_k, *args):
+    """``args``: freqs, positions, interleaved, scale, eps, lens."""
+    got = _heads(dq, dk, gamma_q, gamma_k, *args, q, k)
+    weights = [g for g in (gamma_q, gamma_k) if g is not None] if weight_grads else []
+    if got is None:
+        _check_cuda("q", q)
+        dq_out, dk_out = _empty(q), None if k is None else _empty(k)
+        dgamma_q, dgamma_k = (_empty(g).zero_() if weight_grads and g is not None else None for g in (gamma_q, gamma_k))
+        if q.numel():
+            dq_out, _, dgamma_q, _ = _qk_norm_backward(dq, None, q, None, weight_grads, gamma_q, None, *args)
+        elif k is not None and k.numel():
+            dk_out, _, dgamma_k, _ = _qk_norm_backward(dk, None, k, None, weight_grads, gamma_k, None, *args)
+        return dq_out, dk_out, dgamma_q, dgamma_k
+    dq_out, dk_out, at, p, _held = got
     dgamma_q = dgamma_k = work = None
-    if weight_grads:
-        w = gamma_q if gamma_q is not None else gamma_k
-        dgamma_q, dgamma_k = (q.new_empty(q.shape[-1], dtype=w.dtype) for _ in range(2))
-        work = _scratch(q, _rotary_workspace_bytes(p[:_ROTARY_SIZES]))
-    _launch(q, "unblend_qk_norm_rotary_backward", dq.data_ptr(), _lib.ptr(dk), q.data_ptr(), _lib.ptr(k),
-            dq_out.data_ptr(), _lib.ptr(dk_out), _lib.ptr(dgamma_q), _lib.ptr(dgamma_k), _lib.ptr(work), p,
-            kernels=1 + weight_grads)
+    if weights:
+        dgamma_q, dgamma_k = (dq_out.new_empty(dq_out.shape[-1], dtype=weights[0].dtype) for _ in range(2))
+        work = _scratch(dq_out, _rotary_workspace_bytes(p[:_ROTARY_SIZES]))
+    _launch(dq_out, "unblend_qk_norm_rotary_backward", *at, _lib.ptr(dgamma_q), _lib.ptr(dgamma_k), _lib.ptr(work), p,
+            kernels=1 + bool(weights))
     return dq_out, dk_out, dgamma_q if gamma_q is not None else None, dgamma_k if gamma_k is not None else None
 
 
@@ -789,8 +681,8 @@ class _QKNormRotary(torch.autograd.Function):
         q, k, gamma_q, gamma_k, freqs, positions, lens = ctx.saved_tensors
         interleaved, scale, eps = ctx.args
         need = ctx.needs_input_grad
-        got = _qk_norm_backward(dq.resolve_neg(), None if k is None else dk.resolve_neg(), q, k, gamma_q, gamma_k,
-                                freqs, positions, interleaved, scale, eps, lens, need[2] or need[3])
+        got = _qk_norm_backward(dq.resolve_neg(), None if k is None else dk.resolve_neg(), q, k, need[2] or need[3],
+                                gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
         return *(d if n else None for d, n in zip(got, need)), None, None, None, None, None, None
 
 
@@ -800,9 +692,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, gamma_q: torch.Tenso
                    eps: float = 1e-6, lens: torch.Tensor | None = None
                    ) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Differentiable RMS norm and rotary positions of queries and keys (arguments as ``qk_norm_rotary_forward``)."""
-    scale = _check_qk_norm(q, k, gamma_q, gamma_k, freqs, positions, scale, eps, lens)
-    if _wants_grad("qk_norm_rotary", q, k, gamma_q, gamma_k):
-        _check_cuda("q", q)
+    if _tracked("qk_norm_rotary", freqs, q, k, gamma_q, gamma_k):
         _refuse_capture("qk_norm_rotary")
         return _QKNormRotary.apply(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
     return qk_norm_rotary_forward(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens)
