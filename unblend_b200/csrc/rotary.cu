@@ -24,9 +24,19 @@ constexpr int VEC = 8;
 
 enum Mode { ROTATE = 0, NORM = 1, NORM_BACKWARD = 2 };
 
+// How a row comes into registers: ADJACENT and HALF pairs straight from memory, where a lane's pairs are whole 8- or 16-byte
+// pieces of it; any other row by way of shared memory.
+enum Layout { ADJACENT = 0, HALF = 1, STAGED = 2 };
+
 // CTAs per SM that the registers have to allow, and that are launched.
-constexpr int resident(bool vectors, int elem, int mode) {
-  return !vectors ? 2 : (mode == NORM_BACKWARD ? 3 : 4) - (elem == 4);
+constexpr int resident(int layout, int elem, int mode) {
+  return layout == STAGED ? 2 : (mode == NORM_BACKWARD ? 3 : 4) - (elem == 4);
+}
+
+// Heads of a team in flight.
+constexpr int batch(int layout, int elem, int mode) {
+  const int most = layout == STAGED ? 2 : elem == 4 ? 2 : 4;
+  return mode == NORM_BACKWARD ? most / 2 : most;
 }
 
 struct Side {  // q or k
@@ -49,7 +59,7 @@ struct Args {
   int split;  // teams that share a token's heads
   int hd, pairs, half;
   float scale, eps, sign;
-  bool f64, pos64, w_is_t;
+  bool f64, pos64, w_is_t, pieces;
 };
 
 // Cosine and sine of position p times a frequency, times scale. The frequency comes in turns, as the sum of two doubles,
@@ -116,46 +126,53 @@ struct Token {
   }
 };
 
-// ---------------------------------------------------------------------------------- rows of 8-element pieces
-
 // A lane's four pairs (a, b) as packed fp32: A = (a0, a1), (a2, a3), B likewise.
 struct Pairs {
   float2 A[2], B[2];
 };
 
-// Eight elements of a row in two groups of four at off0 and off1. Adjacent pairs: the groups follow one another for 16-bit
-// types (one 16-byte access) and are half a row apart for fp32 (whole lines per access). Half layout: the groups are the
-// pairs' first and second members, so that a pair is in one lane; behind the pairs they are consecutive.
-template <typename T, bool HALF>
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
+__device__ __forceinline__ float& part_of(float2 (&v)[2], int j) { return j & 1 ? v[j >> 1].y : v[j >> 1].x; }
+
+// A lane's place in its row. Its pairs are number 4 c + j of the row's; behind the turned ones they are two neighbours, so that
+// hd / 2 of them (rounded up) make a row for any number of turned pairs. For ADJACENT and HALF they lie in two groups of four
+// elements at off0 and off1: consecutive for 16-bit adjacent pairs (one 16-byte access), half a row apart for fp32 ones (whole
+// lines per access), the pairs' first and second members for HALF.
+template <typename T, int LAYOUT>
+struct Place {
+  int off0, off1, c;
+  bool has;
+  unsigned turned;  // bit j: pair j turns
+
+  __device__ __forceinline__ Place(const Args& a, int lane) {
+    c = lane;
+    has = c * VEC < a.hd;
+    off0 = VEC * c, off1 = off0 + 4;
+    if (LAYOUT == HALF && 4 * c < a.pairs) off0 = 4 * c, off1 = a.pairs + 4 * c;
+    if (LAYOUT == ADJACENT && sizeof(T) == 4) off0 = 4 * c, off1 = a.hd / 2 + 4 * c;
+    turned = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (has && pair(a, j) < a.pairs) turned |= 1u << j;
+  }
+  __device__ __forceinline__ int pair(const Args& a, int j) const {
+    if (LAYOUT == ADJACENT) return ((j < 2 ? off0 : off1 - 4) >> 1) + j;
+    return 4 * c + j;
+  }
+  // element that A (b = 0) or B (b = 1) holds of pair j; STAGED: may be hd, behind a row of odd width
+  __device__ __forceinline__ int element(const Args& a, int j, int b) const {
+    if (LAYOUT == HALF) return (b ? off1 : off0) + j;
+    if (LAYOUT == ADJACENT) return (j < 2 ? off0 : off1 - 4) + 2 * j + b;
+    const int p = 4 * c + j;
+    return a.half && p < a.pairs ? p + b * a.pairs : 2 * p + b;
+  }
+};
+
+// Eight elements of a row as they lie in memory: groups of four at off0 and off1.
+template <typename T, int LAYOUT>
 struct Piece {
   uint32_t w[2 * sizeof(T)];
-
-  __device__ __forceinline__ void load(const T* row, int off0, int off1, bool on) {
-    if constexpr (sizeof(T) == 4) {
-      const uint4 u = on ? *reinterpret_cast<const uint4*>(row + off0) : make_uint4(0, 0, 0, 0);
-      const uint4 v = on ? *reinterpret_cast<const uint4*>(row + off1) : make_uint4(0, 0, 0, 0);
-      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w, w[4] = v.x, w[5] = v.y, w[6] = v.z, w[7] = v.w;
-    } else if constexpr (!HALF) {
-      const uint4 u = on ? *reinterpret_cast<const uint4*>(row + off0) : make_uint4(0, 0, 0, 0);
-      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-    } else {
-      const uint2 u = on ? *reinterpret_cast<const uint2*>(row + off0) : make_uint2(0, 0);
-      const uint2 v = on ? *reinterpret_cast<const uint2*>(row + off1) : make_uint2(0, 0);
-      w[0] = u.x, w[1] = u.y, w[2] = v.x, w[3] = v.y;
-    }
-  }
-
-  __device__ __forceinline__ void store(T* row, int off0, int off1) const {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<uint4*>(row + off0) = make_uint4(w[0], w[1], w[2], w[3]);
-      *reinterpret_cast<uint4*>(row + off1) = make_uint4(w[4], w[5], w[6], w[7]);
-    } else if constexpr (!HALF) {
-      *reinterpret_cast<uint4*>(row + off0) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      *reinterpret_cast<uint2*>(row + off0) = make_uint2(w[0], w[1]);
-      *reinterpret_cast<uint2*>(row + off1) = make_uint2(w[2], w[3]);
-    }
-  }
 
   __device__ __forceinline__ static float2 two(uint32_t u, __nv_bfloat16) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
@@ -178,14 +195,14 @@ struct Piece {
     for (int k = 0; k < 2; ++k) {
       if constexpr (sizeof(T) == 4) {
         const float* f = reinterpret_cast<const float*>(w);
-        if (HALF) {
+        if (LAYOUT == HALF) {
           r.A[k] = make_float2(f[2 * k], f[2 * k + 1]);
           r.B[k] = make_float2(f[4 + 2 * k], f[5 + 2 * k]);
         } else {
           r.A[k] = make_float2(f[4 * k], f[4 * k + 2]);
           r.B[k] = make_float2(f[4 * k + 1], f[4 * k + 3]);
         }
-      } else if (HALF) {
+      } else if (LAYOUT == HALF) {
         r.A[k] = two(w[k], T());
         r.B[k] = two(w[2 + k], T());
       } else {
@@ -202,12 +219,12 @@ struct Piece {
     for (int k = 0; k < 2; ++k) {
       if constexpr (sizeof(T) == 4) {
         float* f = reinterpret_cast<float*>(w);
-        if (HALF) {
+        if (LAYOUT == HALF) {
           f[2 * k] = r.A[k].x, f[2 * k + 1] = r.A[k].y, f[4 + 2 * k] = r.B[k].x, f[5 + 2 * k] = r.B[k].y;
         } else {
           f[4 * k] = r.A[k].x, f[4 * k + 1] = r.B[k].x, f[4 * k + 2] = r.A[k].y, f[4 * k + 3] = r.B[k].y;
         }
-      } else if (HALF) {
+      } else if (LAYOUT == HALF) {
         w[k] = word(r.A[k].x, r.A[k].y, T());
         w[2 + k] = word(r.B[k].x, r.B[k].y, T());
       } else {
@@ -216,193 +233,356 @@ struct Piece {
       }
     }
   }
-};
 
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
-
-// A lane's place in its row: its groups' offsets, and for pair j which one it is (-1: not turned).
-template <typename T, bool HALF>
-struct Place {
-  int off0, off1, c;
-  bool has;
-
-  __device__ __forceinline__ Place(const Args& a, int lane) {
-    c = lane;
-    has = c * VEC < a.hd;
-    if (HALF) {
-      const int turned = a.pairs / 4;  // lanes with pairs
-      off0 = c < turned ? 4 * c : 2 * a.pairs + VEC * (c - turned);
-      off1 = c < turned ? a.pairs + 4 * c : off0 + 4;
-    } else if (sizeof(T) == 4) {
-      off0 = 4 * c, off1 = a.hd / 2 + 4 * c;
+  __device__ __forceinline__ void store(T* row, int off0, int off1) const {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<uint4*>(row + off0) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(row + off1) = make_uint4(w[4], w[5], w[6], w[7]);
+    } else if constexpr (LAYOUT == ADJACENT) {
+      *reinterpret_cast<uint4*>(row + off0) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-      off0 = VEC * c, off1 = off0 + 4;
+      *reinterpret_cast<uint2*>(row + off0) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(row + off1) = make_uint2(w[2], w[3]);
     }
   }
-  // element that A (b = 0) or B (b = 1) holds of pair j
-  __device__ __forceinline__ int element(int j, int b) const {
-    if (HALF) return (b ? off1 : off0) + j;
-    return (j < 2 ? off0 : off1 - 4) + 2 * j + b;
+
+  // On its way to the thread's own place in shared memory, which no other thread reads: no barrier is needed. Not `on`: zeros.
+  __device__ __forceinline__ static void fetch(uint32_t* to, const T* row, int off0, int off1, bool on) {
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+    if constexpr (sizeof(T) == 4) {
+      const int n = on ? 16 : 0;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(row + off0), "r"(n) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + THREADS * 16), "l"(row + off1), "r"(n)
+                   : "memory");
+    } else if constexpr (LAYOUT == ADJACENT) {
+      const int n = on ? 16 : 0;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(row + off0), "r"(n) : "memory");
+    } else {
+      const int n = on ? 8 : 0;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(row + off0), "r"(n) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + 8), "l"(row + off1), "r"(n) : "memory");
+    }
   }
-  __device__ __forceinline__ int pair(const Args& a, int j) const {
-    const int p = HALF ? 4 * c + j : element(j, 0) / 2;
-    return has && p < a.pairs ? p : -1;
+  __device__ __forceinline__ void read(const uint32_t* from) {
+    const uint4 u = *reinterpret_cast<const uint4*>(from);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    if constexpr (sizeof(T) == 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(from + THREADS * 4);
+      w[4] = v.x, w[5] = v.y, w[6] = v.z, w[7] = v.w;
+    }
   }
 };
 
-__device__ __forceinline__ float& part_of(float2 (&v)[2], int j) { return j & 1 ? v[j >> 1].y : v[j >> 1].x; }
-
-template <typename T, bool HALF, int G, int MODE>
-struct Team {
-  static constexpr int U = sizeof(T) == 4 || MODE == NORM_BACKWARD ? 2 : 4;  // heads in flight
-
-  // One token's heads of one side. C, S: cosines and sines; NORM folds gamma into them for each side.
-  static __device__ __forceinline__ void heads(const Args& a, const Side& sd, const Place<T, HALF>& at, const Token& t,
-                                               const float2 (&C)[2], const float2 (&S)[2], unsigned turns,
-                                               const float* gamma, Pairs& dgamma) {
-    const T* x = static_cast<const T*>(sd.x) + (t.o * sd.s.outer + t.i * sd.s.inner + t.l * sd.s.row + t.part * sd.s.head);
-    const long long x_step = sd.s.head * a.split;
-    const T* x0 = nullptr;
-    long long x0_step = 0;
-    if constexpr (MODE == NORM_BACKWARD) {
-      x0 = static_cast<const T*>(sd.x0) + (t.o * sd.s0.outer + t.i * sd.s0.inner + t.l * sd.s0.row + t.part * sd.s0.head);
-      x0_step = sd.s0.head * a.split;
-    }
-    T* out = static_cast<T*>(sd.out) + ((long long)t.token * sd.heads + t.part) * a.hd;
-    const int out_step = a.hd * a.split;
-    Pairs gm;  // weights
-    float2 CA[2], SA[2], CB[2], SB[2];
-    if constexpr (MODE != ROTATE) {
+// A row by way of shared memory, a row of [G * VEC] elements for each team: in 16-byte pieces where it lies on such boundaries,
+// else element by element; zeros behind hd.
+template <typename T, int G>
+__device__ __forceinline__ void stage(T* buf, const T* row, int c, int hd, bool on, bool pieces) {
+  if (pieces) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        part_of(gm.A, j) = at.has ? gamma[at.element(j, 0)] : 0.f;
-        part_of(gm.B, j) = at.has ? gamma[at.element(j, 1)] : 0.f;
-      }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const int e = (i * G + c) * (16 / (int)sizeof(T));
+      *reinterpret_cast<uint4*>(buf + e) =
+          on && e < hd ? *reinterpret_cast<const uint4*>(row + e) : make_uint4(0, 0, 0, 0);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int e = i * G + c;
+      buf[e] = on && e < hd ? row[e] : from_f<T>(0.f);
+    }
+  }
+}
+template <typename T, int G>
+__device__ __forceinline__ void unstage(const T* buf, T* row, int c, int hd, bool pieces) {
+  if (pieces) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const int e = (i * G + c) * (16 / (int)sizeof(T));
+      if (e < hd) *reinterpret_cast<uint4*>(row + e) = *reinterpret_cast<const uint4*>(buf + e);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int e = i * G + c;
+      if (e < hd) row[e] = buf[e];
+    }
+  }
+}
+
+// What a team's arithmetic needs for one token and side: cosines and sines, for the norm's forward pass times gamma.
+template <int MODE>
+struct Factors {
+  float2 CA[2], SA[2], CB[2], SB[2];
+  Pairs gamma;
+};
+
+// The arithmetic on a lane's pairs of one row: v the input (the output's gradient), w the forward's input for its gradient.
+// live: whether the row counts for the weights' gradients.
+template <int G, int MODE>
+__device__ __forceinline__ Pairs compute(const Args& a, const Factors<MODE>& f, unsigned turned, float inv_hd, Pairs v,
+                                         const Pairs& w, bool live, Pairs& dgamma) {
+  Pairs y;
+  if constexpr (MODE == NORM) {
+    float2 ss = mul2(v.A[0], v.A[0]);
+    ss = ub::fma2(v.A[1], v.A[1], ss);
+    ss = ub::fma2(v.B[0], v.B[0], ss);
+    ss = ub::fma2(v.B[1], v.B[1], ss);
+    const float2 rstd = both(rsqrtf(team_sum<G>(ss.x + ss.y) * inv_hd + a.eps));
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      CA[k] = MODE == NORM ? mul2(C[k], gm.A[k]) : C[k];
-      CB[k] = MODE == NORM ? mul2(C[k], gm.B[k]) : C[k];
-      SA[k] = MODE == NORM ? mul2(S[k], gm.A[k]) : S[k];
-      SB[k] = neg(MODE == NORM ? mul2(S[k], gm.B[k]) : S[k]);
+      const float2 A = mul2(v.A[k], rstd), B = mul2(v.B[k], rstd);
+      y.A[k] = ub::fma2(f.SB[k], B, mul2(f.CA[k], A));
+      y.B[k] = ub::fma2(f.SA[k], A, mul2(f.CB[k], B));
     }
-    const float inv_hd = 1.f / (float)a.hd;
-    const bool partial = 2 * a.pairs != a.hd;
-    const bool reads = t.active && t.inside && at.has, writes = t.active && at.has;
-    int left = sd.heads - t.part;
-    for (int rounds = (sd.heads + U * a.split - 1) / (U * a.split); rounds > 0; --rounds) {  // the same for all parts
-      Piece<T, HALF> r[U], r0[U];
+  } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool on = reads && u * a.split < left;
-        r[u].load(x + u * x_step, at.off0, at.off1, on);
-        if constexpr (MODE == NORM_BACKWARD) r0[u].load(x0 + u * x0_step, at.off0, at.off1, on);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Pairs v = r[u].get();
-        Pairs y;
-        if constexpr (MODE == NORM) {
-          float2 ss = mul2(v.A[0], v.A[0]);
-          ss = ub::fma2(v.A[1], v.A[1], ss);
-          ss = ub::fma2(v.B[0], v.B[0], ss);
-          ss = ub::fma2(v.B[1], v.B[1], ss);
-          const float2 rstd = both(rsqrtf(team_sum<G>(ss.x + ss.y) * inv_hd + a.eps));
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2 A = mul2(v.A[k], rstd), B = mul2(v.B[k], rstd);
-            y.A[k] = ub::fma2(SB[k], B, mul2(CA[k], A));
-            y.B[k] = ub::fma2(SA[k], A, mul2(CB[k], B));
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            y.A[k] = ub::fma2(SB[k], v.B[k], mul2(CA[k], v.A[k]));
-            y.B[k] = ub::fma2(SA[k], v.A[k], mul2(CB[k], v.B[k]));
-          }
-          if (partial) {  // not 1 a - 0 b: b may be infinite
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (!(turns >> j & 1)) {
-                Pairs w = v;
-                part_of(y.A, j) = part_of(w.A, j);
-                part_of(y.B, j) = part_of(w.B, j);
-              }
-          }
-        }
-        if constexpr (MODE == NORM_BACKWARD) {
-          const Pairs w = r0[u].get(), g = y;
-          float2 ss = both(0.f), dot = both(0.f);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            y.A[k] = mul2(g.A[k], gm.A[k]);
-            y.B[k] = mul2(g.B[k], gm.B[k]);
-            ss = ub::fma2(w.A[k], w.A[k], ss);
-            dot = ub::fma2(y.A[k], w.A[k], dot);
-            ss = ub::fma2(w.B[k], w.B[k], ss);
-            dot = ub::fma2(y.B[k], w.B[k], dot);
-          }
-          const float rstd = rsqrtf(team_sum<G>(ss.x + ss.y) * inv_hd + a.eps);
-          const float2 m = both(-team_sum<G>(dot.x + dot.y) * rstd * inv_hd);
-          // Rows that do not count: not 0 * x r, as their r may be infinite.
-          const float2 rs = both(rstd), live = both(t.active && t.inside && u * a.split < left ? rstd : 0.f);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            dgamma.A[k] = ub::fma2(g.A[k], mul2(w.A[k], live), dgamma.A[k]);
-            dgamma.B[k] = ub::fma2(g.B[k], mul2(w.B[k], live), dgamma.B[k]);
-            y.A[k] = mul2(rs, ub::fma2(mul2(w.A[k], rs), m, y.A[k]));
-            y.B[k] = mul2(rs, ub::fma2(mul2(w.B[k], rs), m, y.B[k]));
-          }
-        }
-        if (writes && u * a.split < left) {
-          Piece<T, HALF> o;
-          o.set(y);
-          if (MODE != ROTATE && !t.inside) {
-#pragma unroll
-            for (int k = 0; k < (int)(2 * sizeof(T)); ++k) o.w[k] = 0;
-          }
-          o.store(out + u * out_step, at.off0, at.off1);
-        }
-      }
-      x += U * x_step;
-      if constexpr (MODE == NORM_BACKWARD) x0 += U * x0_step;
-      out += U * out_step;
-      left -= U * a.split;
+    for (int k = 0; k < 2; ++k) {
+      y.A[k] = ub::fma2(f.SB[k], v.B[k], mul2(f.CA[k], v.A[k]));
+      y.B[k] = ub::fma2(f.SA[k], v.A[k], mul2(f.CB[k], v.B[k]));
     }
+    if (2 * a.pairs != a.hd) {  // not 1 a - 0 b: b may be infinite
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!(turned >> j & 1)) {
+          part_of(y.A, j) = part_of(v.A, j);
+          part_of(y.B, j) = part_of(v.B, j);
+        }
+    }
+  }
+  if constexpr (MODE == NORM_BACKWARD) {
+    const Pairs g = y;
+    float2 ss = both(0.f), dot = both(0.f);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      y.A[k] = mul2(g.A[k], f.gamma.A[k]);
+      y.B[k] = mul2(g.B[k], f.gamma.B[k]);
+      ss = ub::fma2(w.A[k], w.A[k], ss);
+      dot = ub::fma2(y.A[k], w.A[k], dot);
+      ss = ub::fma2(w.B[k], w.B[k], ss);
+      dot = ub::fma2(y.B[k], w.B[k], dot);
+    }
+    const float rstd = rsqrtf(team_sum<G>(ss.x + ss.y) * inv_hd + a.eps);
+    const float2 m = both(-team_sum<G>(dot.x + dot.y) * rstd * inv_hd);
+    // Rows that do not count: not 0 * x r, as their r may be infinite.
+    const float2 rs = both(rstd), counts = both(live ? rstd : 0.f);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      dgamma.A[k] = ub::fma2(g.A[k], mul2(w.A[k], counts), dgamma.A[k]);
+      dgamma.B[k] = ub::fma2(g.B[k], mul2(w.B[k], counts), dgamma.B[k]);
+      y.A[k] = mul2(rs, ub::fma2(mul2(w.A[k], rs), m, y.A[k]));
+      y.B[k] = mul2(rs, ub::fma2(mul2(w.B[k], rs), m, y.B[k]));
+    }
+  }
+  return y;
+}
+
+// Where a team's rows of one side and token come from.
+template <typename T, int MODE>
+struct Source {
+  const T *x, *x0;
+  long long step, step0;  // to the team's next head
+  int left;               // heads from the current one on
+  bool on;
+
+  __device__ __forceinline__ Source(const Args& a, const Side& sd, const Token& t) {
+    x = static_cast<const T*>(sd.x) + (t.o * sd.s.outer + t.i * sd.s.inner + t.l * sd.s.row + t.part * sd.s.head);
+    step = sd.s.head * a.split;
+    x0 = nullptr, step0 = 0;
+    if constexpr (MODE == NORM_BACKWARD) {
+      x0 = static_cast<const T*>(sd.x0) + (t.o * sd.s0.outer + t.i * sd.s0.inner + t.l * sd.s0.row + t.part * sd.s0.head);
+      step0 = sd.s0.head * a.split;
+    }
+    left = sd.heads - t.part;
+    on = t.active && t.inside;
   }
 };
 
-template <typename T, bool HALF, int G, int MODE>
-__global__ void __launch_bounds__(THREADS, resident(true, sizeof(T), MODE)) rotary_kernel(const __grid_constant__ Args a) {
-  constexpr int TEAMS = THREADS / G;
+template <typename T, int LAYOUT, int G, int MODE>
+__global__ void __launch_bounds__(THREADS, resident(LAYOUT, sizeof(T), MODE)) rotary_kernel(
+    const __grid_constant__ Args a) {
+  constexpr int TEAMS = THREADS / G, U = batch(LAYOUT, sizeof(T), MODE), PIECES = MODE == NORM_BACKWARD ? 2 * U : U;
+  constexpr int PIECE = THREADS * VEC * (int)sizeof(T) / 4;  // words of a piece of all threads
   __shared__ double2 freqs[MAX_HD / 2];
   __shared__ float gamma[2][MODE != ROTATE ? MAX_HD : 1];
-  __shared__ float red[MODE == NORM_BACKWARD ? THREADS * VEC : 1];
+  // Pieces on their way, in two halves; at the end the sums for the weights' gradients.
+  __shared__ __align__(16) uint32_t ring[(LAYOUT == STAGED ? 1 : 2) * PIECES * PIECE];
+  static_assert(MODE != NORM_BACKWARD || sizeof(ring) >= THREADS * VEC * sizeof(float), "the sums use the ring");
   load_tables<T, MODE>(a, freqs, reinterpret_cast<float (*)[MAX_HD]>(gamma));
-  const Place<T, HALF> at(a, threadIdx.x % G);
-  unsigned turns = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) turns |= at.pair(a, j) >= 0 ? 1u << j : 0u;
+  const Place<T, LAYOUT> at(a, threadIdx.x % G);
+  const float inv_hd = 1.f / (float)a.hd;
   Pairs d[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) d[0].A[k] = d[0].B[k] = d[1].A[k] = d[1].B[k] = both(0.f);
 
-  for (long long base = (long long)blockIdx.x * TEAMS; base < a.items; base += (long long)gridDim.x * TEAMS) {
-    const Token t(a, (unsigned)base + threadIdx.x / G);
-    float2 C[2], S[2];
+  float2 C[2], S[2];
+  const auto factors = [&](int side) {
+    Factors<MODE> f;
+    if constexpr (MODE != ROTATE) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int ea = at.element(a, j, 0), eb = at.element(a, j, 1);
+        part_of(f.gamma.A, j) = at.has && ea < a.hd ? gamma[side][ea] : 0.f;
+        part_of(f.gamma.B, j) = at.has && eb < a.hd ? gamma[side][eb] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      f.CA[k] = MODE == NORM ? mul2(C[k], f.gamma.A[k]) : C[k];
+      f.CB[k] = MODE == NORM ? mul2(C[k], f.gamma.B[k]) : C[k];
+      f.SA[k] = MODE == NORM ? mul2(S[k], f.gamma.A[k]) : S[k];
+      f.SB[k] = neg(MODE == NORM ? mul2(S[k], f.gamma.B[k]) : S[k]);
+    }
+    return f;
+  };
+  const auto cosines = [&](const Token& t) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float c = 1.f, s = 0.f;
-      if (turns >> j & 1) turn(t.p, freqs[at.pair(a, j)], a.scale, c, s);
+      if (at.turned >> j & 1) turn(t.p, freqs[at.pair(a, j)], a.scale, c, s);
       part_of(C, j) = c;
       part_of(S, j) = s * a.sign;
     }
-    Team<T, HALF, G, MODE>::heads(a, a.side[0], at, t, C, S, turns, gamma[0], d[0]);
-    Team<T, HALF, G, MODE>::heads(a, a.side[1], at, t, C, S, turns, gamma[1], d[1]);
+  };
+
+  const long long stride = (long long)gridDim.x * TEAMS;
+  const int per_round = U * a.split;
+  if constexpr (LAYOUT != STAGED) {
+    uint32_t* const mine = ring + threadIdx.x * 4;
+    int half = 0;
+    const auto fetch = [&](Source<T, MODE>& s) {  // the next heads into the other half
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool on = s.on && at.has && u * a.split < s.left;
+        uint32_t* const to = mine + (half * PIECES + u) * PIECE;
+        Piece<T, LAYOUT>::fetch(to, on ? s.x + u * s.step : static_cast<const T*>(a.side[0].x), at.off0, at.off1, on);
+        if constexpr (MODE == NORM_BACKWARD)
+          Piece<T, LAYOUT>::fetch(to + U * PIECE, on ? s.x0 + u * s.step0 : static_cast<const T*>(a.side[0].x0), at.off0,
+                                  at.off1, on);
+      }
+      cp_commit();
+      half ^= 1;
+      s.x += U * s.step;
+      if constexpr (MODE == NORM_BACKWARD) s.x0 += U * s.step0;
+      s.left -= per_round;
+    };
+    long long base = (long long)blockIdx.x * TEAMS;
+    Token t(a, (unsigned)base + threadIdx.x / G);
+    Source<T, MODE> src(a, a.side[0], t);
+    fetch(src);
+    for (; base < a.items; base += stride) {
+      cosines(t);
+      const Token next(a, base + stride < a.items ? (unsigned)(base + stride) + threadIdx.x / G : a.items);
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const Side& sd = a.side[side];
+        const Factors<MODE> f = factors(side);
+        T* out = static_cast<T*>(sd.out) + ((long long)t.token * sd.heads + t.part) * a.hd;
+        int left = sd.heads - t.part;
+        // the same number of rounds for all parts
+        for (int rounds = (sd.heads + per_round - 1) / per_round; rounds > 0; --rounds) {
+          if (rounds == 1) {  // the next heads are the other side's, or the next token's
+            if (side == 0 && a.side[1].heads > 0)
+              src = Source<T, MODE>(a, a.side[1], t);
+            else
+              src = Source<T, MODE>(a, a.side[0], next);
+          }
+          fetch(src);
+          cp_wait<1>();
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const uint32_t* const from = mine + (half * PIECES + u) * PIECE;
+            Piece<T, LAYOUT> r, r0;
+            r.read(from);
+            Pairs w;
+            if constexpr (MODE == NORM_BACKWARD) {
+              r0.read(from + U * PIECE);
+              w = r0.get();
+            }
+            const bool row = t.active && u * a.split < left;
+            r.set(compute<G, MODE>(a, f, at.turned, inv_hd, r.get(), w, row && t.inside, d[side]));
+            if (row && at.has) {
+              if (MODE != ROTATE && !t.inside) {
+#pragma unroll
+                for (int k = 0; k < (int)(2 * sizeof(T)); ++k) r.w[k] = 0;
+              }
+              r.store(out + (long long)u * a.split * a.hd, at.off0, at.off1);
+            }
+          }
+          out += (long long)per_round * a.hd;
+          left -= per_round;
+        }
+      }
+      t = next;
+    }
+    cp_wait<0>();
+  } else {
+    T* const buf = reinterpret_cast<T*>(ring) + (threadIdx.x / G) * (G * VEC);
+    constexpr int ROW = THREADS * VEC;  // from piece to piece
+    const auto pairs = [&](const T* from) {
+      Pairs v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // elements behind hd are zeros: hd is below G * VEC where it is odd
+        const int ea = at.element(a, j, 0), eb = at.element(a, j, 1);
+        part_of(v.A, j) = at.has ? to_f(from[ea]) : 0.f;
+        part_of(v.B, j) = at.has ? to_f(from[eb]) : 0.f;
+      }
+      return v;
+    };
+    for (long long base = (long long)blockIdx.x * TEAMS; base < a.items; base += stride) {
+      const Token t(a, (unsigned)base + threadIdx.x / G);
+      cosines(t);
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const Side& sd = a.side[side];
+        const Factors<MODE> f = factors(side);
+        Source<T, MODE> src(a, sd, t);
+        T* out = static_cast<T*>(sd.out) + ((long long)t.token * sd.heads + t.part) * a.hd;
+        for (int rounds = (sd.heads + per_round - 1) / per_round; rounds > 0; --rounds) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const bool on = src.on && u * a.split < src.left;
+            stage<T, G>(buf + u * ROW, src.x + u * src.step, at.c, a.hd, on, a.pieces);
+            if constexpr (MODE == NORM_BACKWARD)
+              stage<T, G>(buf + (U + u) * ROW, src.x0 + u * src.step0, at.c, a.hd, on, a.pieces);
+          }
+          __syncwarp();
+          Pairs v[U], w[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            v[u] = pairs(buf + u * ROW);
+            if constexpr (MODE == NORM_BACKWARD) w[u] = pairs(buf + (U + u) * ROW);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const bool row = t.active && u * a.split < src.left;
+            Pairs y = compute<G, MODE>(a, f, at.turned, inv_hd, v[u], w[u], row && t.inside, d[side]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool zero = MODE != ROTATE && !t.inside;
+              if (at.has) {
+                buf[u * ROW + at.element(a, j, 0)] = from_f<T>(zero ? 0.f : part_of(y.A, j));
+                buf[u * ROW + at.element(a, j, 1)] = from_f<T>(zero ? 0.f : part_of(y.B, j));
+              }
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (t.active && u * a.split < src.left)
+              unstage<T, G>(buf + u * ROW, out + (long long)u * a.split * a.hd, at.c, a.hd, a.pieces);
+          __syncwarp();
+          src.x += U * src.step;
+          if constexpr (MODE == NORM_BACKWARD) src.x0 += U * src.step0;
+          src.left -= per_round;
+          out += (long long)per_round * a.hd;
+        }
+      }
+    }
   }
   if constexpr (MODE == NORM_BACKWARD) {
     if (a.part == nullptr) return;
+    float* const red = reinterpret_cast<float*>(ring);
     const int team = threadIdx.x / G;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -410,8 +590,8 @@ __global__ void __launch_bounds__(THREADS, resident(true, sizeof(T), MODE)) rota
       if (at.has) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          red[team * (G * VEC) + at.element(j, 0)] = part_of(d[k].A, j);
-          red[team * (G * VEC) + at.element(j, 1)] = part_of(d[k].B, j);
+          red[team * (G * VEC) + at.element(a, j, 0)] = part_of(d[k].A, j);
+          red[team * (G * VEC) + at.element(a, j, 1)] = part_of(d[k].B, j);
         }
       }
       __syncthreads();
@@ -425,113 +605,10 @@ __global__ void __launch_bounds__(THREADS, resident(true, sizeof(T), MODE)) rota
   }
 }
 
-// --------------------------------------------------------------------------------------------- any other row
-
-// A warp per item; lane c holds elements c, c + 32, ... of a row and reads what stands across from them in their pairs.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(THREADS) rotary_any_kernel(const __grid_constant__ Args a) {
-  constexpr int WARPS = THREADS / 32;
-  __shared__ double2 freqs[MAX_HD / 2];
-  __shared__ float gamma[2][MODE != ROTATE ? MAX_HD : 1];
-  __shared__ float red[MODE == NORM_BACKWARD ? THREADS * VEC : 1];
-  load_tables<T, MODE>(a, freqs, reinterpret_cast<float (*)[MAX_HD]>(gamma));
-  const int lane = threadIdx.x & 31;
-  float d[2][VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) d[0][j] = d[1][j] = 0.f;
-  const float inv_hd = 1.f / (float)a.hd;
-  for (long long base = (long long)blockIdx.x * WARPS; base < a.items; base += (long long)gridDim.x * WARPS) {
-    const Token t(a, (unsigned)base + threadIdx.x / 32);
-    float c[VEC], s[VEC];
-    int across[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int e = lane + 32 * j;
-      c[j] = 1.f, s[j] = 0.f, across[j] = e;
-      if (e < 2 * a.pairs) {
-        const bool second = a.half ? e >= a.pairs : e & 1;
-        across[j] = a.half ? (second ? e - a.pairs : e + a.pairs) : e ^ 1;
-        turn(t.p, freqs[a.half ? (second ? e - a.pairs : e) : e >> 1], a.scale, c[j], s[j]);
-        s[j] *= second ? a.sign : -a.sign;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const Side& sd = a.side[k];
-      const T* x = static_cast<const T*>(sd.x) + (t.o * sd.s.outer + t.i * sd.s.inner + t.l * sd.s.row);
-      const T* x0 = static_cast<const T*>(sd.x0) + (t.o * sd.s0.outer + t.i * sd.s0.inner + t.l * sd.s0.row);
-      T* out = static_cast<T*>(sd.out) + (long long)t.token * sd.heads * a.hd;
-      for (int h = t.part; t.active && h < sd.heads; h += a.split) {  // the same for the whole warp
-        float own[VEC], y[VEC], w[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const int e = lane + 32 * j;
-          const bool has = t.inside && e < a.hd;
-          own[j] = has ? to_f(x[h * sd.s.head + e]) : 0.f;
-          y[j] = has && across[j] != e ? to_f(x[h * sd.s.head + across[j]]) : 0.f;
-          w[j] = MODE == NORM_BACKWARD && has ? to_f(x0[h * sd.s0.head + e]) : 0.f;
-        }
-        if constexpr (MODE == NORM) {
-          float ss = 0.f;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) ss += own[j] * own[j];
-          const float rstd = rsqrtf(team_sum<32>(ss) * inv_hd + a.eps);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int e = lane + 32 * j;
-            own[j] = e < a.hd ? own[j] * rstd * gamma[k][e] : 0.f;
-            y[j] = across[j] != e ? y[j] * rstd * gamma[k][across[j]] : 0.f;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = across[j] != lane + 32 * j ? c[j] * own[j] + s[j] * y[j] : own[j];
-        if constexpr (MODE == NORM_BACKWARD) {
-          float ss = 0.f, dot = 0.f, g[VEC];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int e = lane + 32 * j;
-            g[j] = y[j];
-            y[j] = e < a.hd ? g[j] * gamma[k][e] : 0.f;
-            ss += w[j] * w[j];
-            dot += y[j] * w[j];
-          }
-          const float rstd = rsqrtf(team_sum<32>(ss) * inv_hd + a.eps);
-          const float m = team_sum<32>(dot) * rstd * inv_hd;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float xhat = w[j] * rstd;
-            d[k][j] += t.inside ? g[j] * xhat : 0.f;
-            y[j] = rstd * (y[j] - xhat * m);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          if (lane + 32 * j < a.hd)
-            out[(long long)h * a.hd + lane + 32 * j] = from_f<T>(MODE == ROTATE || t.inside ? y[j] : 0.f);
-      }
-    }
-  }
-  if constexpr (MODE == NORM_BACKWARD) {
-    if (a.part == nullptr) return;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) red[(threadIdx.x >> 5) * (32 * VEC) + lane + 32 * j] = d[k][j];
-      __syncthreads();
-      for (int e = threadIdx.x; e < a.hd; e += THREADS) {
-        float s = red[e];
-#pragma unroll
-        for (int y = 1; y < WARPS; ++y) s += red[y * (32 * VEC) + e];
-        a.part[((long long)blockIdx.x * 2 + k) * a.hd + e] = s;
-      }
-    }
-  }
-}
-
 // What a call launches: teams of G lanes, `split` of them to a token, `grid` CTAs.
 struct Plan {
-  bool vectors;
+  int layout;
+  bool pieces;  // STAGED: rows are whole 16-byte pieces
   int lanes, split;
   unsigned grid, items;
 };
@@ -543,14 +620,12 @@ bool heads_ok(const UnblendHeadStrides& s, const void* x, const UnblendRotaryPar
 
 // Enough teams for all SMs come first: a token's heads are divided among teams, which compute its cosines each for
 // itself, until there are about 1024 threads per SM. Larger calls keep a token's heads together.
-Plan make_plan(const UnblendRotaryParams* p, bool vectors, int mode) {
+Plan make_plan(const UnblendRotaryParams* p, bool aligned, int mode) {
   Plan r;
-  r.vectors = vectors;
-  r.lanes = 32;
-  if (vectors) {
-    r.lanes = 4;
-    while (r.lanes * VEC < p->hd) r.lanes *= 2;
-  }
+  r.pieces = aligned && p->hd % VEC == 0;
+  r.layout = !r.pieces || (p->half && p->pairs % 4) ? STAGED : p->half ? HALF : ADJACENT;
+  r.lanes = 4;
+  while (r.lanes * VEC < p->hd) r.lanes *= 2;
   const long long tokens = (long long)p->outer * p->inner * p->length;
   const int most = p->heads > p->k_heads ? p->heads : p->k_heads;
   long long split = (ub::kNumSMs * 1024LL + tokens * r.lanes - 1) / (tokens * r.lanes);
@@ -558,7 +633,7 @@ Plan make_plan(const UnblendRotaryParams* p, bool vectors, int mode) {
   r.split = (int)split;
   r.items = (unsigned)(tokens * split);
   const long long teams = THREADS / r.lanes, ctas = (r.items + teams - 1) / teams;
-  const long long cap = ub::kNumSMs * resident(vectors, elem_size(p->dtype), mode);
+  const long long cap = ub::kNumSMs * resident(r.layout, elem_size(p->dtype), mode);
   r.grid = (unsigned)(ctas < cap ? ctas : cap);
   return r;
 }
@@ -575,13 +650,13 @@ bool params_ok(const UnblendRotaryParams* p) {
          (p->positions == nullptr || reinterpret_cast<uintptr_t>(p->positions) % (p->positions_i64 ? 8 : 4) == 0);
 }
 
-template <typename T, bool HALF, int MODE>
+template <typename T, int LAYOUT, int MODE>
 int launch_lanes(const Args& a, const Plan& pl, cudaStream_t st) {
   switch (pl.lanes) {
-    case 4: rotary_kernel<T, HALF, 4, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
-    case 8: rotary_kernel<T, HALF, 8, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
-    case 16: rotary_kernel<T, HALF, 16, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
-    default: rotary_kernel<T, HALF, 32, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
+    case 4: rotary_kernel<T, LAYOUT, 4, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
+    case 8: rotary_kernel<T, LAYOUT, 8, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
+    case 16: rotary_kernel<T, LAYOUT, 16, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
+    default: rotary_kernel<T, LAYOUT, 32, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
   }
   UB_CHECK_LAUNCH();
   return 0;
@@ -589,10 +664,11 @@ int launch_lanes(const Args& a, const Plan& pl, cudaStream_t st) {
 
 template <typename T, int MODE>
 int launch_layout(const Args& a, const Plan& pl, cudaStream_t st) {
-  if (pl.vectors) return a.half ? launch_lanes<T, true, MODE>(a, pl, st) : launch_lanes<T, false, MODE>(a, pl, st);
-  rotary_any_kernel<T, MODE><<<pl.grid, THREADS, 0, st>>>(a);
-  UB_CHECK_LAUNCH();
-  return 0;
+  switch (pl.layout) {
+    case ADJACENT: return launch_lanes<T, ADJACENT, MODE>(a, pl, st);
+    case HALF: return launch_lanes<T, HALF, MODE>(a, pl, st);
+    default: return launch_lanes<T, STAGED, MODE>(a, pl, st);
+  }
 }
 
 template <int MODE>
@@ -611,6 +687,7 @@ int run(Args& a, const UnblendRotaryParams* p, const void* q, const void* k, con
   a.hd = p->hd;
   a.pairs = p->pairs;
   a.half = p->half;
+  a.pieces = pl.pieces;
   a.scale = p->scale;
   a.eps = p->eps;
   a.sign = inverse ? -1.f : 1.f;
@@ -624,11 +701,11 @@ int run(Args& a, const UnblendRotaryParams* p, const void* q, const void* k, con
   }
 }
 
-// Whether every row is whole pieces of eight dims on 16-byte boundaries, half layouts four pairs at a time.
-bool vectors_ok(const UnblendRotaryParams* p, const void* q, const void* k, const void* q0, const void* k0,
+// Whether every row starts on a 16-byte boundary.
+bool rows_aligned16(const UnblendRotaryParams* p, const void* q, const void* k, const void* q0, const void* k0,
                 const void* qo, const void* ko) {
   const int e = elem_size(p->dtype);
-  if (p->hd % VEC || (p->half && p->pairs % 4)) return false;
+  if (p->hd % VEC) return false;  // nor would the outputs' rows
   if (!heads_ok(p->q, q, p, p->heads, e) || !aligned16(qo) || (q0 && !heads_ok(p->q0, q0, p, p->heads, e)))
     return false;
   return p->k_heads == 0 ||
@@ -644,7 +721,7 @@ bool norm_ok(const UnblendRotaryParams* p) {
 extern "C" int unblend_rotary(const void* q, const void* k, void* q_out, void* k_out, const UnblendRotaryParams* p,
                               int inverse, void* stream) {
   UB_REQUIRE(params_ok(p) && q && q_out && (p->k_heads == 0 || (k && k_out)));
-  Plan pl = make_plan(p, vectors_ok(p, q, k, nullptr, nullptr, q_out, k_out), ROTATE);
+  Plan pl = make_plan(p, rows_aligned16(p, q, k, nullptr, nullptr, q_out, k_out), ROTATE);
   Args a{};
   return run<ROTATE>(a, p, q, k, nullptr, nullptr, q_out, k_out, inverse, pl, ub::as_stream(stream));
 }
@@ -652,7 +729,7 @@ extern "C" int unblend_rotary(const void* q, const void* k, void* q_out, void* k
 extern "C" int unblend_qk_norm_rotary_forward(const void* q, const void* k, void* q_out, void* k_out,
                                               const UnblendRotaryParams* p, void* stream) {
   UB_REQUIRE(params_ok(p) && norm_ok(p) && q && q_out && (p->k_heads == 0 || (k && k_out)));
-  Plan pl = make_plan(p, vectors_ok(p, q, k, nullptr, nullptr, q_out, k_out), NORM);
+  Plan pl = make_plan(p, rows_aligned16(p, q, k, nullptr, nullptr, q_out, k_out), NORM);
   Args a{};
   return run<NORM>(a, p, q, k, nullptr, nullptr, q_out, k_out, false, pl, ub::as_stream(stream));
 }
@@ -669,7 +746,7 @@ extern "C" int unblend_qk_norm_rotary_backward(const void* dq, const void* dk, c
                                                const UnblendRotaryParams* p, void* stream) {
   UB_REQUIRE(params_ok(p) && norm_ok(p) && dq && q && dq_out && (p->k_heads == 0 || (dk && k && dk_out)));
   UB_REQUIRE((dgamma_q == nullptr) == (dgamma_k == nullptr) && (dgamma_q == nullptr || work != nullptr));
-  Plan pl = make_plan(p, vectors_ok(p, dq, dk, q, k, dq_out, dk_out), NORM_BACKWARD);
+  Plan pl = make_plan(p, rows_aligned16(p, dq, dk, q, k, dq_out, dk_out), NORM_BACKWARD);
   Args a{};
   a.part = dgamma_q ? work : nullptr;
   cudaStream_t st = ub::as_stream(stream);
