@@ -15,6 +15,8 @@
 // 0 never becomes 0, since the update divides by it. The update itself uses m and v before they are rounded. What decides
 // a code is computed in fp32 one operation at a time (no fused multiply-add), so that the codes are defined bit for bit.
 // A value that is not finite makes its block's scale infinite or NaN, and with it every moment of the block.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -32,7 +34,7 @@ constexpr int BLOCK = 256;            // elements that share scales
 // parameters with values: 616 us with two CTAs, 690 with three and spills).
 constexpr int FULL_CTAS = 4;
 constexpr int eight_ctas(int elem, int grad_elem) { return elem + grad_elem > 4 ? 2 : 3; }
-constexpr int SMALL = 64, LARGE = 896;  // tensors of a launch: 2.3 or 32 KB of kernel parameters
+constexpr int SMALL = 64, MIDDLE = 256, LARGE = 896;  // tensors of a launch: 2.3, 9 or 32 KB of kernel parameters
 
 template <int N>
 struct Table {
@@ -470,49 +472,75 @@ __global__ void __launch_bounds__(THREADS) adamw_values_kernel(const uint8_t* m,
 }
 
 // Sums of squares in double: exact products, and neither overflow nor underflow for any fp32 value. Warps take runs of
-// 1024 elements; CTAs leave a sum each, and one CTA adds those in a fixed order.
-constexpr int RUN = 1024;
+// 1024 elements; CTAs leave a sum each, and one CTA adds those in a fixed order. Up to FEW runs one cluster of eight CTAs does
+// both, which saves a launch (90 fp16 tensors of 0.6 M elements: 23 us with two launches).
+constexpr int RUN = 1024, FEW = 1024, CLUSTER = 8, CLUSTER_THREADS = 512;
 
-template <typename T, int N>
-__global__ void __launch_bounds__(THREADS) square_sums_kernel(const __grid_constant__ Table<N> tab, double* part) {
-  __shared__ double red[WARPS];
+template <typename T>
+__device__ __forceinline__ void add_squares(const T* g, long long left, int lane, double (&s)[4]) {
   constexpr int VEC = 16 / (int)sizeof(T), LOADS = RUN / 32 / VEC;
-  const int lane = threadIdx.x & 31;
-  double s[4] = {0.0, 0.0, 0.0, 0.0};
-  for (unsigned unit = blockIdx.x * WARPS + (threadIdx.x >> 5); unit < tab.total; unit += gridDim.x * WARPS) {
-    const int k = tensor_of(tab, unit);
-    const long long local = unit - tab.start[k];
-    const long long left = tab.t[k].n - local * RUN;
-    const T* g = static_cast<const T*>(tab.t[k].grad) + local * RUN;
-    if (left >= RUN && reinterpret_cast<uintptr_t>(g) % 16 == 0) {
-      uint4 w[LOADS];
+  const int n = (int)min(left, (long long)RUN);
+  const auto add = [&](float x, int i) { s[i] = fma((double)x, (double)x, s[i]); };
+  if (reinterpret_cast<uintptr_t>(g) % 16 == 0) {
+    uint4 w[LOADS];
+    if (n == RUN) {
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) w[j] = reinterpret_cast<const uint4*>(g)[j * 32 + lane];
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        float2 v[VEC / 2];
-        unpack16(w[j], v, T());
-#pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) {
-          s[(2 * i) % 4] = fma((double)v[i].x, (double)v[i].x, s[(2 * i) % 4]);
-          s[(2 * i + 1) % 4] = fma((double)v[i].y, (double)v[i].y, s[(2 * i + 1) % 4]);
-        }
-      }
     } else {
-      for (int e = lane; e < RUN && e < left; e += 32) {
-        const double x = (double)to_f(g[e]);
-        s[0] = fma(x, x, s[0]);
-      }
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j)
+        w[j] = (j * 32 + lane + 1) * VEC <= n ? reinterpret_cast<const uint4*>(g)[j * 32 + lane] : make_uint4(0, 0, 0, 0);
+      const int rest = n / VEC * VEC + lane;
+      if (rest < n) add(to_f(g[rest]), 0);
     }
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      float2 v[VEC / 2];
+      unpack16(w[j], v, T());
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) add(v[i].x, (2 * i) % 4), add(v[i].y, (2 * i + 1) % 4);
+    }
+  } else {
+#pragma unroll 1
+    for (int at = lane; at < n; at += 8 * 32) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = at + 32 * j < n ? to_f(g[at + 32 * j]) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) add(v[j], j % 4);
+    }
+  }
+}
+
+// The sum of the runs that a CTA's warps take, in thread 0.
+template <typename T, int N, int WARPS_>
+__device__ __forceinline__ double cta_squares(const Table<N>& tab) {
+  __shared__ double red[WARPS_];
+  const int lane = threadIdx.x & 31;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  for (unsigned unit = blockIdx.x * WARPS_ + (threadIdx.x >> 5); unit < tab.total; unit += gridDim.x * WARPS_) {
+    const int k = tensor_of(tab, unit);
+    const long long at = (long long)(unit - tab.start[k]) * RUN;
+    add_squares(static_cast<const T*>(tab.t[k].grad) + at, tab.t[k].n - at, lane, s);
   }
   double t = ub::warp_sum_d((s[0] + s[1]) + (s[2] + s[3]));
   if (lane == 0) red[threadIdx.x >> 5] = t;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    t = red[0];
-    for (int w = 1; w < WARPS; ++w) t += red[w];
-    part[blockIdx.x] = t;
-  }
+  if (threadIdx.x == 0)
+    for (int w = 1; w < WARPS_; ++w) t += red[w];
+  return t;
+}
+
+__device__ __forceinline__ void norm_out(double sum, float max_norm, float* norm, float* scale) {
+  const double r = sqrt(sum);
+  *norm = (float)r;
+  if (scale) *scale = !isfinite(r) ? (float)(r - r) : r > max_norm ? (float)(max_norm / r) : 1.f;
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(THREADS) square_sums_kernel(const __grid_constant__ Table<N> tab, double* part) {
+  const double t = cta_squares<T, N, WARPS>(tab);
+  if (threadIdx.x == 0) part[blockIdx.x] = t;
 }
 
 __global__ void __launch_bounds__(1024) norm_join_kernel(const double* part, int n, float max_norm, float* norm,
@@ -525,11 +553,24 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const double* part, int
   __syncthreads();
   if (threadIdx.x < 32) {
     s = ub::warp_sum_d(red[threadIdx.x]);
-    if (threadIdx.x == 0) {
-      const double r = sqrt(s);
-      *norm = (float)r;
-      if (scale) *scale = !isfinite(r) ? (float)(r - r) : r > max_norm ? (float)(max_norm / r) : 1.f;
-    }
+    if (threadIdx.x == 0) norm_out(s, max_norm, norm, scale);
+  }
+}
+
+template <typename T, int N>
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(CLUSTER_THREADS)
+    few_squares_kernel(const __grid_constant__ Table<N> tab, float max_norm, float* norm, float* scale) {
+  __shared__ double sums[CLUSTER];  // in the first CTA
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  cluster.barrier_arrive();
+  const double t = cta_squares<T, N, CLUSTER_THREADS / 32>(tab);
+  cluster.barrier_wait();  // the first CTA is there
+  if (threadIdx.x == 0) *cluster.map_shared_rank(&sums[blockIdx.x], 0) = t;
+  cluster.sync();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    double s = sums[0];
+    for (int i = 1; i < CLUSTER; ++i) s += sums[i];
+    norm_out(s, max_norm, norm, scale);
   }
 }
 
@@ -563,21 +604,24 @@ bool tensors_ok(const UnblendAdamWTensor* t, int count, bool params, int elem, i
 bool apart(const UnblendAdamWTensor* t, int count, int elem, int grad_elem) {
   struct Span {
     uintptr_t from, to;
-    bool param;
   };
-  std::vector<Span> s;
-  s.reserve(2 * (size_t)count);
+  const auto before = [](const Span& x, const Span& y) { return x.from < y.from; };
+  std::vector<Span> spans(2 * (size_t)count);  // parameters, then gradients
   for (int i = 0; i < count; ++i) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(t[i].param), g = reinterpret_cast<uintptr_t>(t[i].grad);
-    s.push_back(Span{p, p + (uintptr_t)t[i].n * elem, true});
-    s.push_back(Span{g, g + (uintptr_t)t[i].n * grad_elem, false});
+    spans[i] = Span{p, p + (uintptr_t)t[i].n * elem};
+    spans[count + i] = Span{g, g + (uintptr_t)t[i].n * grad_elem};
   }
-  std::sort(s.begin(), s.end(), [](const Span& x, const Span& y) { return x.from < y.from; });
-  uintptr_t params = 0, all = 0;
-  for (const Span& x : s) {
-    if (x.from < (x.param ? all : params)) return false;
-    if (x.param) params = std::max(params, x.to);
-    all = std::max(all, x.to);
+  for (Span* s : {spans.data(), spans.data() + count})  // usually they were allocated one after another
+    if (!std::is_sorted(s, s + count, before)) std::sort(s, s + count, before);
+  const Span *p = spans.data(), *p_end = p + count, *g = p_end, *g_end = g + count;
+  uintptr_t written = 0, seen = 0;  // ends of the parameters, and of both, so far
+  while (p < p_end || g < g_end) {
+    const bool param = g == g_end || (p < p_end && p->from <= g->from);
+    const Span& x = param ? *p++ : *g++;
+    if (x.from < (param ? seen : written)) return false;
+    if (param) written = std::max(written, x.to);
+    seen = std::max(seen, x.to);
   }
   return true;
 }
@@ -601,8 +645,9 @@ template <typename T, typename TG, bool EIGHT>
 int launch_step(const UnblendAdamWTensor* t, int count, const StepArgs& a, cudaStream_t st) {
   for (int i = 0; i < count; i += LARGE) {
     const int n = std::min(LARGE, count - i);
-    const int rc = n <= SMALL ? launch_table<T, TG, EIGHT, SMALL>(t + i, n, a, st)
-                              : launch_table<T, TG, EIGHT, LARGE>(t + i, n, a, st);
+    const int rc = n <= SMALL    ? launch_table<T, TG, EIGHT, SMALL>(t + i, n, a, st)
+                   : n <= MIDDLE ? launch_table<T, TG, EIGHT, MIDDLE>(t + i, n, a, st)
+                                 : launch_table<T, TG, EIGHT, LARGE>(t + i, n, a, st);
     if (rc) return rc;
   }
   return 0;
@@ -622,22 +667,39 @@ int launch_grad(const UnblendAdamWTensor* t, int count, int grad_dtype, int bits
   }
 }
 
-constexpr int NORM_GRID = ub::kNumSMs * 8;
+constexpr int NORM_CTAS = 8;  // per SM
 
+template <typename T, int N>
+int launch_few(const UnblendAdamWTensor* t, int count, float max_norm, float* norm, float* scale, cudaStream_t st) {
+  few_squares_kernel<T, N><<<CLUSTER, CLUSTER_THREADS, 0, st>>>(make_table<N>(t, count, RUN), max_norm, norm, scale);
+  UB_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, int N>
+int launch_sums(const UnblendAdamWTensor* t, int count, double* part, int* used, cudaStream_t st) {
+  const Table<N> tab = make_table<N>(t, count, RUN);
+  const unsigned grid = grid_of(tab.total, NORM_CTAS);
+  square_sums_kernel<T, N><<<grid, THREADS, 0, st>>>(tab, part + *used);
+  UB_CHECK_LAUNCH();
+  *used += (int)grid;
+  return 0;
+}
+
+// All tensors of one type. Few: the norm itself; else partial sums.
 template <typename T>
-int launch_squares(const UnblendAdamWTensor* t, int count, double* part, int* used, cudaStream_t st) {
+int launch_squares(const UnblendAdamWTensor* t, int count, bool few, float max_norm, float* norm, float* scale,
+                   double* part, int* used, cudaStream_t st) {
+  if (few)
+    return count <= SMALL    ? launch_few<T, SMALL>(t, count, max_norm, norm, scale, st)
+           : count <= MIDDLE ? launch_few<T, MIDDLE>(t, count, max_norm, norm, scale, st)
+                             : launch_few<T, LARGE>(t, count, max_norm, norm, scale, st);
   for (int i = 0; i < count; i += LARGE) {
     const int n = std::min(LARGE, count - i);
-    unsigned grid;
-    if (n <= SMALL) {
-      const Table<SMALL> tab = make_table<SMALL>(t + i, n, RUN);
-      square_sums_kernel<T, SMALL><<<grid = grid_of(tab.total, 8), THREADS, 0, st>>>(tab, part + *used);
-    } else {
-      const Table<LARGE> tab = make_table<LARGE>(t + i, n, RUN);
-      square_sums_kernel<T, LARGE><<<grid = grid_of(tab.total, 8), THREADS, 0, st>>>(tab, part + *used);
-    }
-    UB_CHECK_LAUNCH();
-    *used += (int)grid;
+    const int rc = n <= SMALL    ? launch_sums<T, SMALL>(t + i, n, part, used, st)
+                   : n <= MIDDLE ? launch_sums<T, MIDDLE>(t + i, n, part, used, st)
+                                 : launch_sums<T, LARGE>(t + i, n, part, used, st);
+    if (rc) return rc;
   }
   return 0;
 }
@@ -711,7 +773,7 @@ extern "C" int unblend_adamw_values(const void* exp_avg, const void* exp_avg_sq,
 extern "C" int unblend_grad_norm_workspace(int count, long long* bytes) {
   UB_REQUIRE(count >= 1 && bytes);
   // A launch for every LARGE tensors of each of the three types.
-  *bytes = ((count + LARGE - 1) / LARGE + 2LL) * NORM_GRID * (long long)sizeof(double);
+  *bytes = ((count + LARGE - 1) / LARGE + 2LL) * (ub::kNumSMs * NORM_CTAS) * (long long)sizeof(double);
   return 0;
 }
 
@@ -719,26 +781,30 @@ extern "C" int unblend_grad_norm(const UnblendAdamWTensor* tensors, const int* c
                                  float* scale, double* work, void* stream) {
   UB_REQUIRE(tensors && counts && norm && work && reinterpret_cast<uintptr_t>(work) % 8 == 0);
   UB_REQUIRE(!scale || (max_norm > 0.f && std::isfinite(max_norm)));
-  int used = 0, first = 0;
+  long long runs = 0;
+  int first = 0, used = 0, kinds = 0;
   for (int t = 0; t < 3; ++t) {
     UB_REQUIRE(counts[t] >= 0);
     UB_REQUIRE(counts[t] == 0 || tensors_ok(tensors + first, counts[t], false, 1, elem_size(t)));
+    for (int i = first; i < first + counts[t]; ++i) runs += (tensors[i].n + RUN - 1) / RUN;
     first += counts[t];
+    kinds += counts[t] > 0;
   }
-  first = 0;
+  const bool few = kinds == 1 && first <= LARGE && runs <= FEW;
   cudaStream_t st = ub::as_stream(stream);
+  first = 0;
   for (int t = 0; t < 3; ++t) {
-    int rc = 0;
     if (counts[t] == 0) continue;
-    if (t == UNBLEND_F32)
-      rc = launch_squares<float>(tensors + first, counts[t], work, &used, st);
-    else if (t == UNBLEND_BF16)
-      rc = launch_squares<__nv_bfloat16>(tensors + first, counts[t], work, &used, st);
-    else
-      rc = launch_squares<__half>(tensors + first, counts[t], work, &used, st);
+    const UnblendAdamWTensor* mine = tensors + first;
+    const int rc =
+        t == UNBLEND_F32 ? launch_squares<float>(mine, counts[t], few, max_norm, norm, scale, work, &used, st)
+        : t == UNBLEND_BF16
+            ? launch_squares<__nv_bfloat16>(mine, counts[t], few, max_norm, norm, scale, work, &used, st)
+            : launch_squares<__half>(mine, counts[t], few, max_norm, norm, scale, work, &used, st);
     if (rc) return rc;
     first += counts[t];
   }
+  if (few) return 0;
   norm_join_kernel<<<1, 1024, 0, st>>>(work, used, max_norm, norm, scale);
   UB_CHECK_LAUNCH();
   return 0;

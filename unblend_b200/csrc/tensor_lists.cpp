@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int64_t BLOCK = 256;  // elements per block of the moments
+constexpr int64_t BLOCK = 256, RUN = 1024;  // elements per block of the moments, and per run of the norm
 
 // Raises ValueError.
 PyObject* refuse(const std::string& what) {
@@ -37,6 +37,11 @@ std::string text(at::IntArrayRef v) {
   std::string s = "(";
   for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
   return s + (v.size() == 1 ? ",)" : ")");
+}
+
+PyObject* wrap(const at::Tensor& t) {
+  if (t.defined()) return THPVariable_Wrap(t);
+  Py_RETURN_NONE;
 }
 
 int type_of(const at::Tensor& t) {
@@ -99,7 +104,7 @@ PyObject* sizes(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   }
 }
 
-// table(params or None, grads) -> (table, [(type of params, type of grads, tensors), ...], blocks, grads' device index)
+// table(params or None, grads) -> (table, [(type of params, type of grads, tensors), ...], blocks, runs)
 //
 // The table holds an UnblendAdamWTensor for every gradient that is not None and has elements, sorted by the types (by the
 // gradients' alone without params) and in the lists' order within them; blocks counts all params, whatever their
@@ -115,7 +120,7 @@ PyObject* table(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     std::vector<UnblendAdamWTensor> rows[9];
     at::Device room(at::kCPU);
     const at::Device* device = nullptr;
-    int64_t blocks = 0;
+    int64_t blocks = 0, runs = 0;
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* go = PyList_GET_ITEM(args[1], i);
       const at::Tensor *p = nullptr, *g = nullptr;
@@ -135,6 +140,7 @@ PyObject* table(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       row.grad = g->const_data_ptr();
       row.n = g->numel();
       row.block = first;
+      runs += (row.n + RUN - 1) / RUN;
       rows[(with ? 3 * type_of(*p) : 0) + type_of(*g)].push_back(row);
     }
     size_t count = 0;
@@ -157,9 +163,26 @@ PyObject* table(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       Py_XDECREF(kinds);
       return nullptr;
     }
-    return Py_BuildValue("(NNL)", bytes, kinds, (long long)blocks);
+    return Py_BuildValue("(NNLL)", bytes, kinds, (long long)blocks, (long long)runs);
   } catch (const std::exception& e) {
     return refuse(std::string("params and grads: ") + e.what());
+  }
+}
+
+// norm_outputs(like, with scale, bytes) -> (norm, scale or None, workspace) on like's device
+PyObject* norm_outputs(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  if (n_args != 3 || !THPVariable_Check(args[0])) return refuse("norm_outputs(like, with scale, bytes)");
+  const long long bytes = PyLong_AsLongLong(args[2]);
+  if (bytes < 0) return PyErr_Occurred() ? nullptr : refuse("norm_outputs: bytes below 0");
+  try {
+    const at::TensorOptions options = at::TensorOptions().device(THPVariable_Unpack(args[0]).device());
+    const at::Tensor norm = at::empty({}, options.dtype(at::kFloat));
+    const at::Tensor scale = args[1] == Py_True ? at::empty({}, options.dtype(at::kFloat)) : at::Tensor();
+    const at::Tensor work = at::empty({bytes}, options.dtype(at::kByte));
+    return Py_BuildValue("(NNN)", wrap(norm), wrap(scale), wrap(work));
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());  // out of memory
+    return nullptr;
   }
 }
 
@@ -314,11 +337,6 @@ UnblendHeadStrides strides(const at::Tensor& t) {
 
 long long pointer(const at::Tensor& t) { return (long long)reinterpret_cast<uintptr_t>(t.const_data_ptr()); }
 
-PyObject* wrap(const at::Tensor& t) {
-  if (t.defined()) return THPVariable_Wrap(t);
-  Py_RETURN_NONE;
-}
-
 // heads(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens[, q0, k0])
 //   -> None for a side without elements or tensors off the GPU, after the checks; else
 //      (q_out, k_out, (addresses of q, k, [q0, k0,] q_out, k_out), UnblendRotaryParams, tensors that it points to)
@@ -396,13 +414,15 @@ PyObject* heads(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
                          (Py_ssize_t)sizeof(p), wrap(q), wrap(k), wrap(q0), wrap(k0), wrap(freqs), wrap(positions),
                          wrap(gammas[0]), wrap(gammas[1]), wrap(lens));
   } catch (const std::exception& e) {
-    return refuse(std::string("q and k: ") + e.what());
+    PyErr_SetString(PyExc_RuntimeError, e.what());  // out of memory
+    return nullptr;
   }
 }
 
 PyMethodDef methods[] = {
     {"sizes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sizes)), METH_FASTCALL, nullptr},
     {"table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(table)), METH_FASTCALL, nullptr},
+    {"norm_outputs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(norm_outputs)), METH_FASTCALL, nullptr},
     {"changed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(changed)), METH_FASTCALL, nullptr},
     {"heads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(heads)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -39,6 +39,7 @@ MAX_HEAD_DIM = 128
 _ROTARY_SIZES = _lib.RotaryParams.scale.offset  # bytes of the fields that say how large a call is
 ADAMW_BLOCK = 256  # elements of a moment that share a scale in 8 bits; each parameter starts a block of its own
 _TABLE, _TABLE_ROW = 896, 32  # tensors of one launch; bytes of UnblendAdamWTensor
+_FEW_RUNS = 1024  # runs of 1024 elements that the norm takes in one kernel
 _F32_MAX = torch.finfo(torch.float32).max
 _REGISTER_COLS = 8192  # widest rows whose layer norm sums the weights' gradients beside the input's
 _MOST = 1 << 31  # rows, and columns, of layer norm and dropout-add
@@ -917,7 +918,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     are rounded. A value that is not finite spoils its whole block.
     """
     params, grads = _check_list("params", params), _check_list("grads", grads)
-    table, kinds, blocks = _lib.tensor_lists().table(params, grads)
+    table, kinds, blocks, _ = _lib.tensor_lists().table(params, grads)
     if not params:
         raise ValueError("params must hold at least one tensor")
     have = _check_state(state)
@@ -1001,24 +1002,29 @@ def grad_norm(grads: Sequence[torch.Tensor | None], max_norm: float | None = Non
     without ``max_norm``. Gradients are contiguous fp32, bf16 or fp16 in any mixture; None counts for nothing.
     """
     grads = _check_list("grads", grads)
-    table, kinds, _ = _lib.tensor_lists().table(None, grads)
+    table, kinds, _, runs = _lib.tensor_lists().table(None, grads)
     like = next((g for g in grads if g is not None), None)
     if like is None:
         raise ValueError("grads must hold at least one tensor")
     if max_norm is not None and not (_number("max_norm", max_norm, 0) > 0 and max_norm <= _F32_MAX):
         raise ValueError(f"max_norm must be positive, got {max_norm!r}")
     _check_cuda("grads", like)
-    norm = like.new_empty((), dtype=torch.float32)
-    scale = None if max_norm is None else like.new_empty((), dtype=torch.float32)
-    if not kinds:
-        return norm.zero_(), None if scale is None else scale.fill_(1.0)
     counts = (ctypes.c_int * 3)()
     for _, t, n in kinds:
         counts[t] = n
     total = sum(counts)
-    n = ctypes.c_longlong(0)
-    _lib.check("unblend_grad_norm_workspace", _lib.load().unblend_grad_norm_workspace(total, ctypes.byref(n)))
-    work = _scratch(like, n.value)
+    norm, scale, work = _lib.tensor_lists().norm_outputs(like, max_norm is not None, _norm_workspace_bytes(total))
+    if not kinds:
+        return norm.zero_(), None if scale is None else scale.fill_(1.0)
+    few = len(kinds) == 1 and total <= _TABLE and runs <= _FEW_RUNS  # one kernel
     _launch(like, "unblend_grad_norm", table, counts, 0.0 if max_norm is None else float(max_norm), norm.data_ptr(),
-            _lib.ptr(scale), work.data_ptr(), kernels=1 + sum(-(-c // _TABLE) for c in counts))
+            _lib.ptr(scale), work.data_ptr(), kernels=1 if few else 1 + sum(-(-c // _TABLE) for c in counts))
     return norm, scale
+
+
+@lru_cache(maxsize=4096)
+def _norm_workspace_bytes(tensors: int) -> int:
+    n = ctypes.c_longlong(0)
+    if tensors:
+        _lib.check("unblend_grad_norm_workspace", _lib.load().unblend_grad_norm_workspace(tensors, ctypes.byref(n)))
+    return n.value
