@@ -30,7 +30,8 @@ enum Layout { ADJACENT = 0, HALF = 1, STAGED = 2 };
 
 // CTAs per SM that the registers have to allow, and that are launched.
 constexpr int resident(int layout, int elem, int mode) {
-  return layout == STAGED ? 2 : (mode == NORM_BACKWARD ? 3 : 4) - (elem == 4);
+  if (layout == STAGED) return mode == NORM_BACKWARD ? 2 : 3;
+  return (mode == NORM_BACKWARD ? 3 : 4) - (elem == 4);
 }
 
 // Heads of a team in flight.
@@ -273,16 +274,18 @@ struct Piece {
   }
 };
 
-// A row by way of shared memory, a row of [G * VEC] elements for each team: in 16-byte pieces where it lies on such boundaries,
-// else element by element; zeros behind hd.
+// A row by way of shared memory, [G * VEC] elements for each team: in 16-byte pieces, asynchronously, where it lies on such
+// boundaries, else element by element; zeros behind hd.
 template <typename T, int G>
 __device__ __forceinline__ void stage(T* buf, const T* row, int c, int hd, bool on, bool pieces) {
   if (pieces) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
       const int e = (i * G + c) * (16 / (int)sizeof(T));
-      *reinterpret_cast<uint4*>(buf + e) =
-          on && e < hd ? *reinterpret_cast<const uint4*>(row + e) : make_uint4(0, 0, 0, 0);
+      const bool has = on && e < hd;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(buf + e)),
+                   "l"(has ? row + e : row), "r"(has ? 16 : 0)
+                   : "memory");
     }
   } else {
 #pragma unroll
@@ -316,9 +319,17 @@ struct Factors {
   Pairs gamma;
 };
 
+// 1 / sqrt(x); the function is off by two ulp, which fp32 results would show: one Newton step more for them.
+template <typename T>
+__device__ __forceinline__ float reciprocal_root(float x) {
+  const float r = rsqrtf(x);
+  if (sizeof(T) == 2 || !(x >= 1e-30f && x <= 1e30f)) return r;
+  return fmaf(0.5f * r, fmaf(-x * r, r, 1.f), r);
+}
+
 // The arithmetic on a lane's pairs of one row: v the input (the output's gradient), w the forward's input for its gradient.
 // live: whether the row counts for the weights' gradients.
-template <int G, int MODE>
+template <typename T, int G, int MODE>
 __device__ __forceinline__ Pairs compute(const Args& a, const Factors<MODE>& f, unsigned turned, float inv_hd, Pairs v,
                                          const Pairs& w, bool live, Pairs& dgamma) {
   Pairs y;
@@ -327,7 +338,7 @@ __device__ __forceinline__ Pairs compute(const Args& a, const Factors<MODE>& f, 
     ss = ub::fma2(v.A[1], v.A[1], ss);
     ss = ub::fma2(v.B[0], v.B[0], ss);
     ss = ub::fma2(v.B[1], v.B[1], ss);
-    const float2 rstd = both(rsqrtf(team_sum<G>(ss.x + ss.y) * inv_hd + a.eps));
+    const float2 rstd = both(reciprocal_root<T>(team_sum<G>(ss.x + ss.y) * inv_hd + a.eps));
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const float2 A = mul2(v.A[k], rstd), B = mul2(v.B[k], rstd);
@@ -361,7 +372,7 @@ __device__ __forceinline__ Pairs compute(const Args& a, const Factors<MODE>& f, 
       ss = ub::fma2(w.B[k], w.B[k], ss);
       dot = ub::fma2(y.B[k], w.B[k], dot);
     }
-    const float rstd = rsqrtf(team_sum<G>(ss.x + ss.y) * inv_hd + a.eps);
+    const float rstd = reciprocal_root<T>(team_sum<G>(ss.x + ss.y) * inv_hd + a.eps);
     const float2 m = both(-team_sum<G>(dot.x + dot.y) * rstd * inv_hd);
     // Rows that do not count: not 0 * x r, as their r may be infinite.
     const float2 rs = both(rstd), counts = both(live ? rstd : 0.f);
@@ -405,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, resident(LAYOUT, sizeof(T), MODE)) ro
   __shared__ double2 freqs[MAX_HD / 2];
   __shared__ float gamma[2][MODE != ROTATE ? MAX_HD : 1];
   // Pieces on their way, in two halves; at the end the sums for the weights' gradients.
-  __shared__ __align__(16) uint32_t ring[(LAYOUT == STAGED ? 1 : 2) * PIECES * PIECE];
+  __shared__ __align__(16) uint32_t ring[2 * PIECES * PIECE];
   static_assert(MODE != NORM_BACKWARD || sizeof(ring) >= THREADS * VEC * sizeof(float), "the sums use the ring");
   load_tables<T, MODE>(a, freqs, reinterpret_cast<float (*)[MAX_HD]>(gamma));
   const Place<T, LAYOUT> at(a, threadIdx.x % G);
@@ -446,140 +457,133 @@ __global__ void __launch_bounds__(THREADS, resident(LAYOUT, sizeof(T), MODE)) ro
 
   const long long stride = (long long)gridDim.x * TEAMS;
   const int per_round = U * a.split;
-  if constexpr (LAYOUT != STAGED) {
-    uint32_t* const mine = ring + threadIdx.x * 4;
-    int half = 0;
-    const auto fetch = [&](Source<T, MODE>& s) {  // the next heads into the other half
+  uint32_t* const mine = ring + threadIdx.x * 4;  // the thread's own pieces; STAGED: the team's rows
+  T* const rows = reinterpret_cast<T*>(ring) + (threadIdx.x / G) * (G * VEC);
+  constexpr int ROW = THREADS * VEC;  // elements from piece to piece
+  int half = 0;
+  const auto fetch = [&](Source<T, MODE>& s) {  // the next heads into the other half
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool on = s.on && at.has && u * a.split < s.left;
-        uint32_t* const to = mine + (half * PIECES + u) * PIECE;
-        Piece<T, LAYOUT>::fetch(to, on ? s.x + u * s.step : static_cast<const T*>(a.side[0].x), at.off0, at.off1, on);
+    for (int u = 0; u < U; ++u) {
+      const bool on = s.on && u * a.split < s.left;
+      const T* const x = on ? s.x + u * s.step : static_cast<const T*>(a.side[0].x);
+      [[maybe_unused]] const T* const x0 = on ? s.x0 + u * s.step0 : static_cast<const T*>(a.side[0].x0);
+      const int to = half * PIECES + u;
+      if constexpr (LAYOUT == STAGED) {
+        stage<T, G>(rows + to * ROW, x, at.c, a.hd, on, a.pieces);
+        if constexpr (MODE == NORM_BACKWARD) stage<T, G>(rows + (to + U) * ROW, x0, at.c, a.hd, on, a.pieces);
+      } else {
+        const bool has = on && at.has;
+        Piece<T, LAYOUT>::fetch(mine + to * PIECE, has ? x : static_cast<const T*>(a.side[0].x), at.off0, at.off1, has);
         if constexpr (MODE == NORM_BACKWARD)
-          Piece<T, LAYOUT>::fetch(to + U * PIECE, on ? s.x0 + u * s.step0 : static_cast<const T*>(a.side[0].x0), at.off0,
-                                  at.off1, on);
+          Piece<T, LAYOUT>::fetch(mine + (to + U) * PIECE, has ? x0 : static_cast<const T*>(a.side[0].x0), at.off0,
+                                  at.off1, has);
       }
-      cp_commit();
-      half ^= 1;
-      s.x += U * s.step;
-      if constexpr (MODE == NORM_BACKWARD) s.x0 += U * s.step0;
-      s.left -= per_round;
-    };
-    long long base = (long long)blockIdx.x * TEAMS;
-    Token t(a, (unsigned)base + threadIdx.x / G);
-    Source<T, MODE> src(a, a.side[0], t);
-    fetch(src);
-    for (; base < a.items; base += stride) {
-      cosines(t);
-      const Token next(a, base + stride < a.items ? (unsigned)(base + stride) + threadIdx.x / G : a.items);
-#pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const Side& sd = a.side[side];
-        const Factors<MODE> f = factors(side);
-        T* out = static_cast<T*>(sd.out) + ((long long)t.token * sd.heads + t.part) * a.hd;
-        int left = sd.heads - t.part;
-        // the same number of rounds for all parts
-        for (int rounds = (sd.heads + per_round - 1) / per_round; rounds > 0; --rounds) {
-          if (rounds == 1) {  // the next heads are the other side's, or the next token's
-            if (side == 0 && a.side[1].heads > 0)
-              src = Source<T, MODE>(a, a.side[1], t);
-            else
-              src = Source<T, MODE>(a, a.side[0], next);
-          }
-          fetch(src);
-          cp_wait<1>();
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const uint32_t* const from = mine + (half * PIECES + u) * PIECE;
-            Piece<T, LAYOUT> r, r0;
-            r.read(from);
-            Pairs w;
-            if constexpr (MODE == NORM_BACKWARD) {
-              r0.read(from + U * PIECE);
-              w = r0.get();
-            }
-            const bool row = t.active && u * a.split < left;
-            r.set(compute<G, MODE>(a, f, at.turned, inv_hd, r.get(), w, row && t.inside, d[side]));
-            if (row && at.has) {
-              if (MODE != ROTATE && !t.inside) {
-#pragma unroll
-                for (int k = 0; k < (int)(2 * sizeof(T)); ++k) r.w[k] = 0;
-              }
-              r.store(out + (long long)u * a.split * a.hd, at.off0, at.off1);
-            }
-          }
-          out += (long long)per_round * a.hd;
-          left -= per_round;
-        }
-      }
-      t = next;
     }
-    cp_wait<0>();
-  } else {
-    T* const buf = reinterpret_cast<T*>(ring) + (threadIdx.x / G) * (G * VEC);
-    constexpr int ROW = THREADS * VEC;  // from piece to piece
-    const auto pairs = [&](const T* from) {
+    cp_commit();
+    half ^= 1;
+    s.x += U * s.step;
+    if constexpr (MODE == NORM_BACKWARD) s.x0 += U * s.step0;
+    s.left -= per_round;
+  };
+  // A lane's pairs of a row in flight. STAGED: elements behind hd are zeros (hd is below G * VEC where it is odd).
+  const auto pairs = [&](int from) {
+    if constexpr (LAYOUT == STAGED) {
       Pairs v;
+      const T* const row = rows + from * ROW;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {  // elements behind hd are zeros: hd is below G * VEC where it is odd
+      for (int j = 0; j < 4; ++j) {
         const int ea = at.element(a, j, 0), eb = at.element(a, j, 1);
-        part_of(v.A, j) = at.has ? to_f(from[ea]) : 0.f;
-        part_of(v.B, j) = at.has ? to_f(from[eb]) : 0.f;
+        part_of(v.A, j) = at.has ? to_f(row[ea]) : 0.f;
+        part_of(v.B, j) = at.has ? to_f(row[eb]) : 0.f;
       }
       return v;
-    };
-    for (long long base = (long long)blockIdx.x * TEAMS; base < a.items; base += stride) {
-      const Token t(a, (unsigned)base + threadIdx.x / G);
-      cosines(t);
+    } else {
+      Piece<T, LAYOUT> r;
+      r.read(mine + from * PIECE);
+      return r.get();
+    }
+  };
+  const auto zeros = [](Pairs& y) {
 #pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const Side& sd = a.side[side];
-        const Factors<MODE> f = factors(side);
-        Source<T, MODE> src(a, sd, t);
-        T* out = static_cast<T*>(sd.out) + ((long long)t.token * sd.heads + t.part) * a.hd;
-        for (int rounds = (sd.heads + per_round - 1) / per_round; rounds > 0; --rounds) {
+    for (int k = 0; k < 2; ++k) y.A[k] = y.B[k] = both(0.f);
+  };
+
+  long long base = (long long)blockIdx.x * TEAMS;
+  Token t(a, (unsigned)base + threadIdx.x / G);
+  Source<T, MODE> src(a, a.side[0], t);
+  fetch(src);
+  for (; base < a.items; base += stride) {
+    cosines(t);
+    const Token next(a, base + stride < a.items ? (unsigned)(base + stride) + threadIdx.x / G : a.items);
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const bool on = src.on && u * a.split < src.left;
-            stage<T, G>(buf + u * ROW, src.x + u * src.step, at.c, a.hd, on, a.pieces);
-            if constexpr (MODE == NORM_BACKWARD)
-              stage<T, G>(buf + (U + u) * ROW, src.x0 + u * src.step0, at.c, a.hd, on, a.pieces);
-          }
+    for (int side = 0; side < 2; ++side) {
+      const Side& sd = a.side[side];
+      const Factors<MODE> f = factors(side);
+      T* out = static_cast<T*>(sd.out) + ((long long)t.token * sd.heads + t.part) * a.hd;
+      int left = sd.heads - t.part;
+      // the same number of rounds for all parts
+      for (int rounds = (sd.heads + per_round - 1) / per_round; rounds > 0; --rounds) {
+        if (rounds == 1) {  // the next heads are the other side's, or the next token's
+          if (side == 0 && a.side[1].heads > 0)
+            src = Source<T, MODE>(a, a.side[1], t);
+          else
+            src = Source<T, MODE>(a, a.side[0], next);
+        }
+        fetch(src);
+        cp_wait<1>();
+        const int from = half * PIECES;
+        if constexpr (LAYOUT == STAGED) {
           __syncwarp();
           Pairs v[U], w[U];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            v[u] = pairs(buf + u * ROW);
-            if constexpr (MODE == NORM_BACKWARD) w[u] = pairs(buf + (U + u) * ROW);
+            v[u] = pairs(from + u);
+            if constexpr (MODE == NORM_BACKWARD) w[u] = pairs(from + U + u);
           }
           __syncwarp();
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const bool row = t.active && u * a.split < src.left;
-            Pairs y = compute<G, MODE>(a, f, at.turned, inv_hd, v[u], w[u], row && t.inside, d[side]);
+            const bool row = t.active && u * a.split < left;
+            Pairs y = compute<T, G, MODE>(a, f, at.turned, inv_hd, v[u], w[u], row && t.inside, d[side]);
+            if (MODE != ROTATE && !t.inside) zeros(y);
+            T* const to = rows + (from + u) * ROW;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const bool zero = MODE != ROTATE && !t.inside;
               if (at.has) {
-                buf[u * ROW + at.element(a, j, 0)] = from_f<T>(zero ? 0.f : part_of(y.A, j));
-                buf[u * ROW + at.element(a, j, 1)] = from_f<T>(zero ? 0.f : part_of(y.B, j));
+                to[at.element(a, j, 0)] = from_f<T>(part_of(y.A, j));
+                to[at.element(a, j, 1)] = from_f<T>(part_of(y.B, j));
               }
             }
           }
           __syncwarp();
 #pragma unroll
           for (int u = 0; u < U; ++u)
-            if (t.active && u * a.split < src.left)
-              unstage<T, G>(buf + u * ROW, out + (long long)u * a.split * a.hd, at.c, a.hd, a.pieces);
+            if (t.active && u * a.split < left)
+              unstage<T, G>(rows + (from + u) * ROW, out + (long long)u * a.split * a.hd, at.c, a.hd, a.pieces);
           __syncwarp();
-          src.x += U * src.step;
-          if constexpr (MODE == NORM_BACKWARD) src.x0 += U * src.step0;
-          src.left -= per_round;
-          out += (long long)per_round * a.hd;
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const Pairs v = pairs(from + u);
+            Pairs w;
+            if constexpr (MODE == NORM_BACKWARD) w = pairs(from + U + u);
+            const bool row = t.active && u * a.split < left;
+            Pairs y = compute<T, G, MODE>(a, f, at.turned, inv_hd, v, w, row && t.inside, d[side]);
+            if (row && at.has) {
+              if (MODE != ROTATE && !t.inside) zeros(y);
+              Piece<T, LAYOUT> r;
+              r.set(y);
+              r.store(out + (long long)u * a.split * a.hd, at.off0, at.off1);
+            }
+          }
         }
+        out += (long long)per_round * a.hd;
+        left -= per_round;
       }
     }
+    t = next;
   }
+  cp_wait<0>();
   if constexpr (MODE == NORM_BACKWARD) {
     if (a.part == nullptr) return;
     float* const red = reinterpret_cast<float*>(ring);
