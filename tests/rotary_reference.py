@@ -12,6 +12,15 @@ from training_reference import U, acc, floor, half
 # An angle is reduced to a fraction of a turn, rounded to fp32 (at most 1/2, so pi U of the angle), and its sine and
 # cosine are off by at most 2 U of themselves and U for the factor: 6.2 U. Two products and a sum add 2 U to each term.
 TURN = 10 * U
+# For 16-bit tensors the functions are off by 2^-21.19 (7 U) in place of 2 U of themselves, and their argument rounds once
+# more (2 pi t: pi U) and carries 2 pi's own rounding (U / 2 of half a turn, 2 U): 10.2 U more.
+TURN16 = 21 * U
+
+
+def turn_error(t: torch.dtype) -> float:
+    return TURN if t == torch.float32 else TURN16
+
+
 # A head's sum of squares has at most 13 roundings in a row and one in each square, the mean two, eps one, the reciprocal
 # root 4 U, and the root halves what is before it: 13 U. x r gamma: two more.
 RSTD = 13 * U
@@ -60,7 +69,7 @@ def rotary_reference(x, freqs, positions, interleaved, scale, inverse):
     x = x.double()
     a = angles(x, freqs, positions)
     y = turned(x, -a if inverse else a, interleaved, scale)
-    return y, half(t) * y.abs() + TURN * pair_size(x, n, interleaved, scale) + floor(t) + 2.0**-149
+    return y, half(t) * y.abs() + turn_error(t) * pair_size(x, n, interleaved, scale) + floor(t) + 2.0**-149
 
 
 def qk_norm_reference(x, dy, gamma, freqs, positions, interleaved, scale, eps, lens):
@@ -86,10 +95,10 @@ def qk_norm_reference(x, dy, gamma, freqs, positions, interleaved, scale, eps, l
     n = f.shape[0]
     e_z = (RSTD + 2 * U) * z.abs()
     small = 2.0**-149
-    e_y = half(t) * y.abs() + TURN * pair_size(z, n, interleaved, scale) + turn_bound(e_z, n, interleaved, scale) + \
+    e_y = half(t) * y.abs() + turn_error(t) * pair_size(z, n, interleaved, scale) + turn_bound(e_z, n, interleaved, scale) + \
         floor(t) + small
     gr = turned(dy, -a, interleaved, scale)
-    e_g = TURN * pair_size(dy, n, interleaved, scale)
+    e_g = turn_error(t) * pair_size(dy, n, interleaved, scale)
     h = gr * g
     e_h = e_g * g.abs() + U * h.abs()
     m = (h * xhat).mean(-1, keepdim=True)

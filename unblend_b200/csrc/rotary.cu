@@ -49,6 +49,18 @@ struct Side {  // q or k
   int heads;
 };
 
+// n / d for n < 2^31 without a division (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+struct Divisor {
+  unsigned d, m, s;
+
+  Divisor() = default;
+  explicit Divisor(unsigned by) : d(by), s(0) {
+    while (s < 32 && (1ull << s) < by) ++s;
+    m = (unsigned)(((1ull << 32) * ((1ull << s) - by)) / by + 1);
+  }
+  __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
 struct Args {
   Side side[2];
   const void* freqs;
@@ -56,8 +68,9 @@ struct Args {
   const int* lens;
   float* part;  // backward of the norm: [gridDim.x][2 hd] sums for the weights' gradients, may be null
   long long pos_stride;  // of a sequence
-  unsigned length, inner, items;
-  int split;  // teams that share a token's heads
+  Divisor length, inner, parts;  // parts: teams that share a token's heads
+  unsigned items;
+  int split;  // parts again
   int hd, pairs, half;
   float scale, eps, sign;
   bool f64, pos64, w_is_t, pieces;
@@ -65,13 +78,18 @@ struct Args {
 
 // Cosine and sine of position p times a frequency, times scale. The frequency comes in turns, as the sum of two doubles,
 // and the whole turns are taken off the product before anything is rounded to fp32: the error is that of the final
-// functions for every integer below 2^53.
+// functions for every integer below 2^53. 16-bit tensors take the hardware's functions, off by 2^-21 within half a turn:
+// a 500th of what rounding the results to fp16 costs, and an eighth of the instructions.
+template <typename T>
 __device__ __forceinline__ void turn(double p, double2 f, float scale, float& c, float& s) {
   const double hi = p * f.x;
   const double lo = fma(p, f.y, fma(p, f.x, -hi));
   double t = (hi - rint(hi)) + lo;  // beyond 2^53 turns the low part has whole ones too
   t -= rint(t);
-  sincospif(2.f * (float)t, &s, &c);
+  if (sizeof(T) == 2)
+    __sincosf(6.283185307f * (float)t, &s, &c);
+  else
+    sincospif(2.f * (float)t, &s, &c);
   c *= scale;
   s *= scale;
 }
@@ -112,11 +130,11 @@ struct Token {
 
   __device__ __forceinline__ Token(const Args& a, unsigned item) {
     active = item < a.items;
-    token = active ? item / (unsigned)a.split : 0;
+    token = active ? a.parts(item) : 0;
     part = active ? (int)(item - token * a.split) : 0;
-    const unsigned seq = token / a.length;
-    l = token - seq * a.length;
-    o = seq / a.inner, i = seq - o * a.inner;
+    const unsigned seq = a.length(token);
+    l = token - seq * a.length.d;
+    o = a.inner(seq), i = seq - o * a.inner.d;
     inside = a.lens == nullptr || (int)l < a.lens[seq];
     p = (double)l;
     if (a.positions) {
@@ -449,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, resident(LAYOUT, sizeof(T), MODE)) ro
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float c = 1.f, s = 0.f;
-      if (at.turned >> j & 1) turn(t.p, freqs[at.pair(a, j)], a.scale, c, s);
+      if (at.turned >> j & 1) turn<T>(t.p, freqs[at.pair(a, j)], a.scale, c, s);
       part_of(C, j) = c;
       part_of(S, j) = s * a.sign;
     }
@@ -684,8 +702,9 @@ int run(Args& a, const UnblendRotaryParams* p, const void* q, const void* k, con
   a.positions = p->positions;
   a.lens = MODE != ROTATE ? p->lens : nullptr;
   a.pos_stride = p->positions_stride;
-  a.length = p->length;
-  a.inner = p->inner;
+  a.length = Divisor((unsigned)p->length);
+  a.inner = Divisor((unsigned)p->inner);
+  a.parts = Divisor((unsigned)pl.split);
   a.items = pl.items;
   a.split = pl.split;
   a.hd = p->hd;
