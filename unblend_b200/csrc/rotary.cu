@@ -47,6 +47,7 @@ struct Side {  // q or k
   UnblendHeadStrides s, s0;
   const void* gamma;
   int heads;
+  int rounds;  // of a team's batches, the same for all of a token's teams
 };
 
 // n / d for n < 2^31 without a division (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
@@ -302,7 +303,7 @@ __device__ __forceinline__ void stage(T* buf, const T* row, int c, int hd, bool 
       const int e = (i * G + c) * (16 / (int)sizeof(T));
       const bool has = on && e < hd;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(buf + e)),
-                   "l"(has ? row + e : row), "r"(has ? 16 : 0)
+                   "l"(row + e), "r"(has ? 16 : 0)
                    : "memory");
     }
   } else {
@@ -483,18 +484,17 @@ __global__ void __launch_bounds__(THREADS, resident(LAYOUT, sizeof(T), MODE)) ro
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool on = s.on && u * a.split < s.left;
-      const T* const x = on ? s.x + u * s.step : static_cast<const T*>(a.side[0].x);
-      [[maybe_unused]] const T* const x0 = on ? s.x0 + u * s.step0 : static_cast<const T*>(a.side[0].x0);
+      const T* const x = s.x + u * s.step;  // behind the last head nothing is read from it
+      [[maybe_unused]] const T* const x0 = s.x0 + u * s.step0;
       const int to = half * PIECES + u;
       if constexpr (LAYOUT == STAGED) {
         stage<T, G>(rows + to * ROW, x, at.c, a.hd, on, a.pieces);
         if constexpr (MODE == NORM_BACKWARD) stage<T, G>(rows + (to + U) * ROW, x0, at.c, a.hd, on, a.pieces);
       } else {
         const bool has = on && at.has;
-        Piece<T, LAYOUT>::fetch(mine + to * PIECE, has ? x : static_cast<const T*>(a.side[0].x), at.off0, at.off1, has);
+        Piece<T, LAYOUT>::fetch(mine + to * PIECE, x, at.off0, at.off1, has);
         if constexpr (MODE == NORM_BACKWARD)
-          Piece<T, LAYOUT>::fetch(mine + (to + U) * PIECE, has ? x0 : static_cast<const T*>(a.side[0].x0), at.off0,
-                                  at.off1, has);
+          Piece<T, LAYOUT>::fetch(mine + (to + U) * PIECE, x0, at.off0, at.off1, has);
       }
     }
     cp_commit();
@@ -539,8 +539,7 @@ __global__ void __launch_bounds__(THREADS, resident(LAYOUT, sizeof(T), MODE)) ro
       const Factors<MODE> f = factors(side);
       T* out = static_cast<T*>(sd.out) + ((long long)t.token * sd.heads + t.part) * a.hd;
       int left = sd.heads - t.part;
-      // the same number of rounds for all parts
-      for (int rounds = (sd.heads + per_round - 1) / per_round; rounds > 0; --rounds) {
+      for (int rounds = sd.rounds; rounds > 0; --rounds) {
         if (rounds == 1) {  // the next heads are the other side's, or the next token's
           if (side == 0 && a.side[1].heads > 0)
             src = Source<T, MODE>(a, a.side[1], t);
@@ -673,7 +672,9 @@ bool params_ok(const UnblendRotaryParams* p) {
 }
 
 template <typename T, int LAYOUT, int MODE>
-int launch_lanes(const Args& a, const Plan& pl, cudaStream_t st) {
+int launch_lanes(Args& a, const Plan& pl, cudaStream_t st) {
+  const int per_round = batch(LAYOUT, sizeof(T), MODE) * pl.split;
+  for (Side& s : a.side) s.rounds = (s.heads + per_round - 1) / per_round;
   switch (pl.lanes) {
     case 4: rotary_kernel<T, LAYOUT, 4, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
     case 8: rotary_kernel<T, LAYOUT, 8, MODE><<<pl.grid, THREADS, 0, st>>>(a); break;
@@ -685,7 +686,7 @@ int launch_lanes(const Args& a, const Plan& pl, cudaStream_t st) {
 }
 
 template <typename T, int MODE>
-int launch_layout(const Args& a, const Plan& pl, cudaStream_t st) {
+int launch_layout(Args& a, const Plan& pl, cudaStream_t st) {
   switch (pl.layout) {
     case ADJACENT: return launch_lanes<T, ADJACENT, MODE>(a, pl, st);
     case HALF: return launch_lanes<T, HALF, MODE>(a, pl, st);
@@ -696,8 +697,8 @@ int launch_layout(const Args& a, const Plan& pl, cudaStream_t st) {
 template <int MODE>
 int run(Args& a, const UnblendRotaryParams* p, const void* q, const void* k, const void* q0, const void* k0, void* qo,
         void* ko, bool inverse, Plan& pl, cudaStream_t st) {
-  a.side[0] = Side{q, q0, qo, p->q, p->q0, MODE != ROTATE ? p->gamma_q : nullptr, p->heads};
-  a.side[1] = Side{k, k0, ko, p->k, p->k0, MODE != ROTATE ? p->gamma_k : nullptr, p->k_heads};
+  a.side[0] = Side{q, q0, qo, p->q, p->q0, MODE != ROTATE ? p->gamma_q : nullptr, p->heads, 0};
+  a.side[1] = Side{k, k0, ko, p->k, p->k0, MODE != ROTATE ? p->gamma_k : nullptr, p->k_heads, 0};
   a.freqs = p->freqs;
   a.positions = p->positions;
   a.lens = MODE != ROTATE ? p->lens : nullptr;
