@@ -42,6 +42,16 @@ def test_state_layout():
     assert training.adamw_moments(s)[0] is s.exp_avg
 
 
+def test_states_are_saved_as_tuples(tmp_path):
+    for bits in (32, 8):
+        s = training.adamw_state([torch.zeros(300), torch.zeros(5)], bits)
+        s.exp_avg[7] = 3
+        torch.save(tuple(s), tmp_path / "state.pt")
+        back = training.AdamWState(*torch.load(tmp_path / "state.pt", weights_only=True))
+        assert all(a is b or torch.equal(a, b) for a, b in zip(s, back))
+        assert training._check_state(back) == 3
+
+
 def test_refuses():
     p, g = [torch.zeros(5), torch.zeros(2, 3)], [torch.zeros(5), torch.zeros(2, 3)]
     s = training.adamw_state(p)
@@ -56,7 +66,8 @@ def test_refuses():
                 lambda: step(p, g, s, 0), lambda: step(p, g, s, -1), lambda: step(p, g, s, 1.0),
                 lambda: step(p, g, s, True), lambda: step(p, g, s, one.int()), lambda: step(p, g, s, one.repeat(2)),
                 lambda: step(p, g, s, 1 << 62), lambda: step(p, g, s, 1, lr=-1.0), lambda: step(p, g, s, 1, lr=math.nan),
-                lambda: step(p, g, s, 1, lr=math.inf), lambda: step(p, g, s, 1, lr=torch.ones(1).double()),
+                lambda: step(p, g, s, 1, lr=math.inf), lambda: step(p, g, s, 1, lr=1e19),
+                lambda: step(p, g, s, 1, weight_decay=1e19), lambda: step(p, g, s, 1, lr=torch.ones(1).double()),
                 lambda: step(p, g, s, 1, betas=(1.0, 0.9)), lambda: step(p, g, s, 1, betas=(0.9, -0.1)),
                 lambda: step(p, g, s, 1, betas=0.9), lambda: step(p, g, s, 1, betas=(0.9,)),
                 lambda: step(p, g, s, 1, eps=-1e-8), lambda: step(p, g, s, 1, eps=1e-40),
@@ -121,7 +132,7 @@ def test_entry_points_refuse_before_they_launch():
                dict(args=None), dict(args=with_(beta1=1.0)), dict(args=with_(beta2=-0.5)),
                dict(args=with_(beta1=math.nan)), dict(args=with_(eps=-1.0)), dict(args=with_(eps=math.inf)),
                dict(args=with_(eps=1e-40)), dict(args=with_(eps=math.nan)),
-               dict(args=with_(lr=math.nan)), dict(args=with_(weight_decay=math.inf)), dict(args=with_(step=0)),
+               dict(args=with_(lr=math.nan)), dict(args=with_(lr=1e19)), dict(args=with_(weight_decay=math.inf)), dict(args=with_(step=0)),
                dict(args=with_(step_device=p + 4)), dict(args=with_(lr_device=p + 2)),
                dict(args=with_(grad_scale=p + 1)), dict(table=_table((0, p, 10, 0))), dict(table=_table((p, 0, 10, 0))),
                dict(table=_table((p, p + 4096, 0, 0))), dict(table=_table((p, p + 4096, 10, -1))),

@@ -391,6 +391,55 @@ def test_in_front_of_attention(t):
     assert _lib.error_flag() == 0
 
 
+def test_one_side_and_the_same_tensor_twice():
+    f, w = _rand(16, seed=1), _rand(32, seed=2, shift=1.0).requires_grad_()
+    q = _rand(2, 9, 4, 32, seed=3).requires_grad_()
+    d = _rand(2, 9, 4, 32, seed=4)
+    y, none = training.rotary(q, None, f)
+    assert none is None
+    assert torch.equal(torch.autograd.grad(y, q, d)[0], training.rotary_backward(d, None, f)[0])
+    y, none = training.qk_norm_rotary(q, None, w, None, f)
+    assert none is None
+    want = training.qk_norm_rotary_backward(d, None, q.detach(), None, w.detach(), None, f)
+    got = torch.autograd.grad(y, (q, w), d)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[2])
+    a, b = training.rotary(q, q, f)
+    assert torch.equal(a, b)
+    once = training.rotary_backward(d, None, f)[0]
+    assert torch.equal(torch.autograd.grad(a, q, d, retain_graph=True)[0], once)
+    assert torch.equal(torch.autograd.grad((a * d).sum() + (b * d).sum(), q)[0], once + once)
+
+
+def test_two_calls_at_once():
+    """Threads with streams of their own."""
+    import threading
+
+    f, w = training.rotary_freqs(64, device="cuda"), _rand(64, seed=1, shift=1.0)
+    data = [[_rand(3, 500, h, 64, seed=10 * i + h, t=BF16) for h in (4, 2)] for i in range(4)]
+
+    def run(q, k):
+        return training.qk_norm_rotary_backward(q, k, q, k, w, w, f)
+
+    want = [run(*d) for d in data]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got = run(*data[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_packed_parameters():
     """The parameters that a call passes: sizes, strides and addresses of what it was given."""
     q, k = torch.zeros(2, 3, 5, 4, 16, device="cuda")[:, 1:], torch.zeros(2, 2, 5, 2, 18, device="cuda")[..., :16]

@@ -716,7 +716,7 @@ extern "C" int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, 
   UB_REQUIRE(exp_avg && exp_avg_sq && aligned16(exp_avg) && aligned16(exp_avg_sq));
   UB_REQUIRE(bits == 32 || (scales && reinterpret_cast<uintptr_t>(scales) % 8 == 0));
   UB_REQUIRE(p->beta1 >= 0 && p->beta1 < 1 && p->beta2 >= 0 && p->beta2 < 1 && eps_ok(p->eps));
-  UB_REQUIRE(std::isfinite(p->weight_decay) && (p->lr_device || std::isfinite(p->lr)));
+  UB_REQUIRE(std::fabs(p->weight_decay) <= 1e18 && (p->lr_device || std::fabs(p->lr) <= 1e18));
   UB_REQUIRE(p->step_device || p->step >= 1);
   UB_REQUIRE(reinterpret_cast<uintptr_t>(p->step_device) % 8 == 0 && reinterpret_cast<uintptr_t>(p->lr_device) % 4 == 0 &&
              reinterpret_cast<uintptr_t>(p->grad_scale) % 4 == 0);

@@ -930,7 +930,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     if not (isinstance(betas, (tuple, list)) and len(betas) == 2):
         raise ValueError(f"betas must be two numbers, got {betas!r}")
     a = _lib.AdamWParams(0.0, _number("betas[0]", betas[0], 0, 1), _number("betas[1]", betas[1], 0, 1),
-                         _number("eps", eps, 0, 1e30), _number("weight_decay", weight_decay, 0))
+                         _number("eps", eps, 0, 1e30), _number("weight_decay", weight_decay, 0, 1e18))
     if 0 < eps < torch.finfo(torch.float32).smallest_normal:
         raise ValueError(f"eps must be 0 or a normal float32, got {eps!r}")
     if isinstance(step, torch.Tensor):
@@ -944,7 +944,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
         _check_scalar("lr", lr, torch.float32, device)
         a.lr_device = lr.data_ptr()
     else:
-        a.lr = _number("lr", lr, 0)
+        a.lr = _number("lr", lr, 0, 1e18)
     if grad_scale is not None:
         _check_scalar("grad_scale", grad_scale, torch.float32, device)
         a.grad_scale = grad_scale.data_ptr()
