@@ -446,8 +446,11 @@ def test_packed_parameters():
     f, pos = torch.ones(8, dtype=F64, device="cuda"), torch.zeros(2, 2, 5, dtype=torch.int64, device="cuda")
     w, lens = torch.ones(16, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
     dq, dk = torch.zeros(q.shape, device="cuda"), torch.zeros(k.shape, device="cuda")
-    q_out, k_out, at, p, _ = _lib.tensor_lists().heads(dq, dk, w, None, f, pos, False, 0.5, 1e-3, lens, q, k)
-    assert at == tuple(x.data_ptr() for x in (dq, dk, q, k, q_out, k_out))
+    args = (dq, dk, w, None, f, pos, False, 0.5, 1e-3, lens, q, k)
+    q_out, k_out, dgq, dgk, at, p, held = _lib.tensor_lists().heads(*args, True, training._norm_workspace())
+    assert at == tuple(x.data_ptr() for x in (dq, dk, q, k, q_out, k_out, dgq, dgk, held[-1]))
+    assert held[-1].numel() >= 2 * 16 * 4
+    assert _lib.tensor_lists().heads(*args, False, training._norm_workspace())[2:4] == (None, None)
     p = _lib.RotaryParams.from_buffer_copy(p)
     got = {n: getattr(p, n) for n, _ in p._fields_ if n not in ("q", "k", "q0", "k0")}
     assert got.pop("eps") == pytest.approx(1e-3)

@@ -133,8 +133,3 @@ def test_param_struct_layout(tmp_path):
     from test_capi import test_param_struct_layout_matches_c
 
     test_param_struct_layout_matches_c(tmp_path, _lib.RotaryParams, "UnblendRotaryParams")
-
-
-def test_workspace_by_the_sizes_alone():
-    p = bytes(_params(pairs=8, freqs=16))
-    assert training._rotary_workspace_bytes(p[:training._ROTARY_SIZES]) >= 2 * 64 * 4

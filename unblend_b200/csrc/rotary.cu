@@ -7,9 +7,18 @@
 // linear, so its backward pass is the transposed rotation of the gradients alone; the norm's backward pass reads x again
 // and takes r from it, as the row is in registers anyway.
 //
-// Bound: HBM (2 passes over the tensors per direction, 3 for the norm's backward pass). A team of lanes (the next power of
-// two of hd / 8) keeps a token and walks over its heads, so that cosines and sines are computed once per token and not
-// read from a table.
+// Bound: HBM (2 passes over the tensors per direction, 3 for the norm's backward pass) for many heads per token; issue slots
+// for few, as each token's angles and addresses are shared by fewer rows. A team of lanes (the next power of two of hd / 8)
+// keeps a token and walks over its heads, so that cosines and sines are computed once per token and lane and not read from
+// a table. Rows come through shared memory a batch of heads ahead (cp.async): with loads to registers alone too few bytes
+// were in flight (norm, 801 x 62 x 16 heads of 64: 119 us a step, now 100). Pairs are kept whole in a lane and worked on two
+// at a time in packed fp32; as single floats the arithmetic bound the kernels (142 us).
+//
+// Measured, bf16: 62 x 801 tokens x 16 heads of 64, rotation 29 us per direction (6.9 TB/s), norm 801 x 62 35 us forward
+// (5.8 TB/s) and 57 us backward (5.4); 20018 x 40 heads of 128 in half layout 68 us (6.0 TB/s) and 111 us (5.5). Forward and
+// backward of 3 x 16381 x 20 heads of 128, 64 dims turned, fp16: 174 us (5.8 TB/s). Rows that have to go through shared memory:
+// 32000 x 32 heads of 128 with 25 pairs in half layout 304 us (3.5 TB/s). Others would lose by it: the first two of these cases
+// 131 instead of 78 us and 206 instead of 100 (both directions), as elements are picked one by one.
 #include <cmath>
 
 #include "train_common.cuh"
@@ -639,8 +648,11 @@ bool heads_ok(const UnblendHeadStrides& s, const void* x, const UnblendRotaryPar
          (p->length <= 1 || s.row * elem % 16 == 0) && (heads <= 1 || s.head * elem % 16 == 0);
 }
 
-// Enough teams for all SMs come first: a token's heads are divided among teams, which compute its cosines each for
-// itself, until there are about 1024 threads per SM. Larger calls keep a token's heads together.
+// Enough teams for all SMs come first: a token's heads are divided among teams, which compute its cosines each for itself,
+// until there are 256 threads per SM; larger calls keep a token's heads together. Both sides, a forward and a backward call waited
+// for: 62 tokens x 16 heads of 64, fp32, divided 27 us, undivided 28; norm of 8058 padded tokens x 16 heads of 48, fp32, divided
+// by three 41 us among other calls, undivided 37; 1025 tokens x 64 heads of 96 by way of shared memory (16 lanes: by three) 68,
+// by ten 64.
 Plan make_plan(const UnblendRotaryParams* p, bool aligned, int mode) {
   Plan r;
   r.pieces = aligned && p->hd % VEC == 0;
@@ -649,7 +661,7 @@ Plan make_plan(const UnblendRotaryParams* p, bool aligned, int mode) {
   while (r.lanes * VEC < p->hd) r.lanes *= 2;
   const long long tokens = (long long)p->outer * p->inner * p->length;
   const int most = p->heads > p->k_heads ? p->heads : p->k_heads;
-  long long split = (ub::kNumSMs * 1024LL + tokens * r.lanes - 1) / (tokens * r.lanes);
+  long long split = (ub::kNumSMs * 256LL + tokens * r.lanes - 1) / (tokens * r.lanes);
   if (split > most) split = most;
   r.split = (int)split;
   r.items = (unsigned)(tokens * split);

@@ -337,13 +337,14 @@ UnblendHeadStrides strides(const at::Tensor& t) {
 
 long long pointer(const at::Tensor& t) { return (long long)reinterpret_cast<uintptr_t>(t.const_data_ptr()); }
 
-// heads(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens[, q0, k0])
+// heads(q, k, gamma_q, gamma_k, freqs, positions, interleaved, scale, eps, lens[, q0, k0, weights, workspace])
 //   -> None for a side without elements or tensors off the GPU, after the checks; else
-//      (q_out, k_out, (addresses of q, k, [q0, k0,] q_out, k_out), UnblendRotaryParams, tensors that it points to)
+//      (q_out, k_out, dgamma_q, dgamma_k, addresses for the entry point, UnblendRotaryParams, tensors that these point to)
 //
-// With q0 and k0, q and k are the gradients of the norm's outputs for those inputs.
+// With q0 and k0, q and k are the gradients of the norm's outputs for those inputs; weights: whether gradients of gamma_q and
+// gamma_k are wanted; workspace: address of unblend_qk_norm_rotary_grad_workspace.
 PyObject* heads(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
-  if (n_args != N_ARGS && n_args != N_ARGS + 2) return refuse("heads: wrong number of arguments");
+  if (n_args != N_ARGS && n_args != N_ARGS + 4) return refuse("heads: wrong number of arguments");
   try {
     Call c;
     const bool backward = n_args > N_ARGS;
@@ -407,12 +408,26 @@ PyObject* heads(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     const at::Tensor q_out = at::empty(q.sizes(), q.options());
     const at::Tensor k_out = c.k ? at::empty(k.sizes(), k.options()) : at::Tensor();
     const auto address = [](const at::Tensor& t) { return t.defined() ? pointer(t) : 0LL; };
-    PyObject* at_ = backward ? Py_BuildValue("(LLLLLL)", address(q), address(k), address(q0), address(k0),
-                                             address(q_out), address(k_out))
-                             : Py_BuildValue("(LLLL)", address(q), address(k), address(q_out), address(k_out));
-    return Py_BuildValue("(NNNy#(NNNNNNNNN))", wrap(q_out), wrap(k_out), at_, reinterpret_cast<const char*>(&p),
-                         (Py_ssize_t)sizeof(p), wrap(q), wrap(k), wrap(q0), wrap(k0), wrap(freqs), wrap(positions),
-                         wrap(gammas[0]), wrap(gammas[1]), wrap(lens));
+    at::Tensor dgamma[2], work;
+    PyObject* addresses;
+    if (backward) {
+      if (PyObject_IsTrue(o[N_ARGS + 2]) > 0 && (c.gamma[0] || c.gamma[1])) {
+        const auto workspace = reinterpret_cast<int (*)(const UnblendRotaryParams*, long long*)>(
+            PyLong_AsVoidPtr(o[N_ARGS + 3]));
+        long long bytes = 0;
+        if (!workspace || workspace(&p, &bytes) != 0) return refuse("heads: no workspace for these sizes");
+        for (at::Tensor& d : dgamma) d = at::empty({p.hd}, gammas[c.gamma[0] ? 0 : 1].options());
+        work = at::empty({bytes}, q.options().dtype(at::kByte));
+      }
+      addresses = Py_BuildValue("(LLLLLLLLL)", address(q), address(k), address(q0), address(k0), address(q_out),
+                                address(k_out), address(dgamma[0]), address(dgamma[1]), address(work));
+    } else {
+      addresses = Py_BuildValue("(LLLL)", address(q), address(k), address(q_out), address(k_out));
+    }
+    return Py_BuildValue("(NNNNNy#(NNNNNNNNNNNN))", wrap(q_out), wrap(k_out), wrap(dgamma[0]), wrap(dgamma[1]), addresses,
+                         reinterpret_cast<const char*>(&p), (Py_ssize_t)sizeof(p), wrap(q), wrap(k), wrap(q0), wrap(k0),
+                         wrap(freqs), wrap(positions), wrap(gammas[0]), wrap(gammas[1]), wrap(lens), wrap(dgamma[0]),
+                         wrap(dgamma[1]), wrap(work));
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());  // out of memory
     return nullptr;

@@ -36,7 +36,6 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 MAX_HEAD_DIM = 128
-_ROTARY_SIZES = _lib.RotaryParams.scale.offset  # bytes of the fields that say how large a call is
 ADAMW_BLOCK = 256  # elements of a moment that share a scale in 8 bits; each parameter starts a block of its own
 _TABLE, _TABLE_ROW = 896, 32  # tensors of one launch; bytes of UnblendAdamWTensor
 _FEW_RUNS = 1024  # runs of 1024 elements that the norm takes in one kernel
@@ -498,17 +497,6 @@ def rotary_freqs(dims: int, base: float = 10000.0, factor: float = 1.0, method: 
     return f.to(device) if device is not None else f
 
 
-@lru_cache(maxsize=4096)
-def _rotary_workspace_bytes(sizes: bytes) -> int:
-    """Workspace of the norm's backward pass, by the leading fields of ``UnblendRotaryParams``."""
-    p = _lib.RotaryParams.from_buffer_copy(sizes.ljust(ctypes.sizeof(_lib.RotaryParams), b"\0"))
-    p.pairs = 0  # the workspace does not depend on them, and their frequencies are not here
-    n = ctypes.c_longlong(0)
-    _lib.check("unblend_qk_norm_rotary_grad_workspace",
-               _lib.load().unblend_qk_norm_rotary_grad_workspace(ctypes.byref(p), ctypes.byref(n)))
-    return n.value
-
-
 def _heads(*args):
     """The checks of a call on heads, and its outputs and parameters (None for a side without elements, or on the CPU)."""
     return _lib.tensor_lists().heads(*args)
@@ -526,7 +514,7 @@ def _rotate(q, k, freqs, positions, interleaved: bool, scale: float, inverse: bo
         elif k is not None and k.numel():
             k_out = _rotate(k, None, freqs, positions, interleaved, scale, inverse)[0]
         return q_out, k_out
-    q_out, k_out, at, p, _held = got
+    q_out, k_out, _, _, at, p, _held = got
     _launch(q_out, "unblend_rotary", *at, p, inverse)
     return q_out, k_out
 
@@ -625,7 +613,7 @@ def _qk_norm_forward(q, k, gamma_q, gamma_k, *args):
         elif k is not None and k.numel():
             k_out = _qk_norm_forward(k, None, gamma_k, None, *args)[0]
         return q_out, k_out
-    q_out, k_out, at, p, _held = got
+    q_out, k_out, _, _, at, p, _held = got
     _launch(q_out, "unblend_qk_norm_rotary_forward", *at, p)
     return q_out, k_out
 
@@ -647,8 +635,7 @@ def qk_norm_rotary_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.
 
 def _qk_norm_backward(dq, dk, q, k, weight_grads: bool, gamma_q, gamma_k, *args):
     """``args``: freqs, positions, interleaved, scale, eps, lens."""
-    got = _heads(dq, dk, gamma_q, gamma_k, *args, q, k)
-    weights = [g for g in (gamma_q, gamma_k) if g is not None] if weight_grads else []
+    got = _heads(dq, dk, gamma_q, gamma_k, *args, q, k, weight_grads, _norm_workspace())
     if got is None:
         _check_cuda("q", q)
         dq_out, dk_out = _empty(q), None if k is None else _empty(k)
@@ -658,14 +645,15 @@ def _qk_norm_backward(dq, dk, q, k, weight_grads: bool, gamma_q, gamma_k, *args)
         elif k is not None and k.numel():
             dk_out, _, dgamma_k, _ = _qk_norm_backward(dk, None, k, None, weight_grads, gamma_k, None, *args)
         return dq_out, dk_out, dgamma_q, dgamma_k
-    dq_out, dk_out, at, p, _held = got
-    dgamma_q = dgamma_k = work = None
-    if weights:
-        dgamma_q, dgamma_k = (dq_out.new_empty(dq_out.shape[-1], dtype=weights[0].dtype) for _ in range(2))
-        work = _scratch(dq_out, _rotary_workspace_bytes(p[:_ROTARY_SIZES]))
-    _launch(dq_out, "unblend_qk_norm_rotary_backward", *at, _lib.ptr(dgamma_q), _lib.ptr(dgamma_k), _lib.ptr(work), p,
-            kernels=1 + bool(weights))
+    dq_out, dk_out, dgamma_q, dgamma_k, at, p, _held = got
+    _launch(dq_out, "unblend_qk_norm_rotary_backward", *at, p, kernels=1 + (dgamma_q is not None))
     return dq_out, dk_out, dgamma_q if gamma_q is not None else None, dgamma_k if gamma_k is not None else None
+
+
+@lru_cache(maxsize=1)
+def _norm_workspace() -> int:
+    """Address of the entry point that says how large the workspace is."""
+    return ctypes.cast(_lib.load().unblend_qk_norm_rotary_grad_workspace, ctypes.c_void_p).value
 
 
 class _QKNormRotary(torch.autograd.Function):
