@@ -5,7 +5,9 @@ Operators of the models' pre-norm block ``x + LayerScale * dropout(attention(lay
 keys in front of the attention, each as
 
 * a differentiable function (``layer_norm``, ``rotary``, ``qk_norm_rotary``, ``attention``, ``dropout_add``), and
-* its two passes as plain calls (``*_forward``, ``*_backward``) for callers that keep the saved tensors themselves.
+* its two passes as plain calls (``*_forward``, ``*_backward``) for callers that keep the saved tensors themselves;
+
+and what follows the gradients: their norm (``grad_norm``) and the update of all parameters (``adamw_step``), in place.
 
 All take CUDA tensors in fp32, bf16 or fp16 and run hand-written kernels on the current stream of the tensors' device;
 wrong arguments raise ``ValueError`` before anything is launched, and there is no CPU path. Statistics, softmax and
