@@ -8,6 +8,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -43,6 +44,12 @@ PyObject* wrap(const at::Tensor& t) {
   if (t.defined()) return THPVariable_Wrap(t);
   Py_RETURN_NONE;
 }
+
+// The interpreter is free meanwhile: an allocation can wait for the GPU.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
 
 int type_of(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -82,26 +89,24 @@ PyObject* sizes(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (n_args != 2 || !PyUnicode_Check(args[0]) || !listed(args[1])) return refuse("sizes(name, list of tensors)");
   const char* name = PyUnicode_AsUTF8(args[0]);
   if (!name) return nullptr;
-  try {
-    const Py_ssize_t n = PyList_GET_SIZE(args[1]);
-    PyObject* out = PyList_New(n);
-    if (!out) return nullptr;
-    at::Device room(at::kCPU);
-    const at::Device* device = nullptr;
-    for (Py_ssize_t i = 0; i < n; ++i) {
-      const at::Tensor* t = nullptr;
-      const bool ok = fine(name, i, PyList_GET_ITEM(args[1], i), t, device, room);
-      PyObject* x = ok ? PyLong_FromLongLong(t->numel()) : nullptr;
-      if (!x) {
-        Py_DECREF(out);
-        return nullptr;
-      }
-      PyList_SET_ITEM(out, i, x);
+  HANDLE_TH_ERRORS  // torch's exceptions as Python's: out of memory stays what it is
+  const Py_ssize_t n = PyList_GET_SIZE(args[1]);
+  PyObject* out = PyList_New(n);
+  if (!out) return nullptr;
+  at::Device room(at::kCPU);
+  const at::Device* device = nullptr;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor* t = nullptr;
+    const bool ok = fine(name, i, PyList_GET_ITEM(args[1], i), t, device, room);
+    PyObject* x = ok ? PyLong_FromLongLong(t->numel()) : nullptr;
+    if (!x) {
+      Py_DECREF(out);
+      return nullptr;
     }
-    return out;
-  } catch (const std::exception& e) {
-    return refuse(std::string(name) + ": " + e.what());
+    PyList_SET_ITEM(out, i, x);
   }
+  return out;
+  END_HANDLE_TH_ERRORS
 }
 
 // table(params or None, grads) -> (table, [(type of params, type of grads, tensors), ...], blocks, runs)
@@ -116,57 +121,55 @@ PyObject* table(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (with && PyList_GET_SIZE(args[0]) != n)
     return refuse("params and grads must be lists of one length, got " + std::to_string(PyList_GET_SIZE(args[0])) +
                   " and " + std::to_string(n));
-  try {
-    std::vector<UnblendAdamWTensor> rows[9];
-    at::Device room(at::kCPU);
-    const at::Device* device = nullptr;
-    int64_t blocks = 0, runs = 0;
-    for (Py_ssize_t i = 0; i < n; ++i) {
-      PyObject* go = PyList_GET_ITEM(args[1], i);
-      const at::Tensor *p = nullptr, *g = nullptr;
-      const int64_t first = blocks;
-      if (with) {
-        if (!fine("params", i, PyList_GET_ITEM(args[0], i), p, device, room)) return nullptr;
-        blocks += (p->numel() + BLOCK - 1) / BLOCK;
-      }
-      if (go == Py_None) continue;
-      if (!fine("grads", i, go, g, device, room)) return nullptr;
-      if (with && p->sizes() != g->sizes())
-        return refuse("grads[" + std::to_string(i) + "] must have its parameter's shape " + text(p->sizes()) + ", got " +
-                      text(g->sizes()));
-      if (g->numel() == 0) continue;
-      UnblendAdamWTensor row;
-      row.param = with ? p->data_ptr() : nullptr;
-      row.grad = g->const_data_ptr();
-      row.n = g->numel();
-      row.block = first;
-      runs += (row.n + RUN - 1) / RUN;
-      rows[(with ? 3 * type_of(*p) : 0) + type_of(*g)].push_back(row);
+  HANDLE_TH_ERRORS
+  std::vector<UnblendAdamWTensor> rows[9];
+  at::Device room(at::kCPU);
+  const at::Device* device = nullptr;
+  int64_t blocks = 0, runs = 0;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* go = PyList_GET_ITEM(args[1], i);
+    const at::Tensor *p = nullptr, *g = nullptr;
+    const int64_t first = blocks;
+    if (with) {
+      if (!fine("params", i, PyList_GET_ITEM(args[0], i), p, device, room)) return nullptr;
+      blocks += (p->numel() + BLOCK - 1) / BLOCK;
     }
-    size_t count = 0;
-    for (const auto& r : rows) count += r.size();
-    PyObject* bytes = PyBytes_FromStringAndSize(nullptr, (Py_ssize_t)(count * sizeof(UnblendAdamWTensor)));
-    PyObject* kinds = PyList_New(0);
-    char* to = bytes ? PyBytes_AS_STRING(bytes) : nullptr;
-    bool ok = bytes && kinds;
-    for (int k = 0; ok && k < 9; ++k) {
-      if (rows[k].empty()) continue;
-      const size_t len = rows[k].size() * sizeof(UnblendAdamWTensor);
-      std::memcpy(to, rows[k].data(), len);
-      to += len;
-      PyObject* kind = Py_BuildValue("(iin)", k / 3, k % 3, (Py_ssize_t)rows[k].size());
-      ok = kind && PyList_Append(kinds, kind) == 0;
-      Py_XDECREF(kind);
-    }
-    if (!ok) {
-      Py_XDECREF(bytes);
-      Py_XDECREF(kinds);
-      return nullptr;
-    }
-    return Py_BuildValue("(NNLL)", bytes, kinds, (long long)blocks, (long long)runs);
-  } catch (const std::exception& e) {
-    return refuse(std::string("params and grads: ") + e.what());
+    if (go == Py_None) continue;
+    if (!fine("grads", i, go, g, device, room)) return nullptr;
+    if (with && p->sizes() != g->sizes())
+      return refuse("grads[" + std::to_string(i) + "] must have its parameter's shape " + text(p->sizes()) + ", got " +
+                    text(g->sizes()));
+    if (g->numel() == 0) continue;
+    UnblendAdamWTensor row;
+    row.param = with ? p->data_ptr() : nullptr;
+    row.grad = g->const_data_ptr();
+    row.n = g->numel();
+    row.block = first;
+    runs += (row.n + RUN - 1) / RUN;
+    rows[(with ? 3 * type_of(*p) : 0) + type_of(*g)].push_back(row);
   }
+  size_t count = 0;
+  for (const auto& r : rows) count += r.size();
+  PyObject* bytes = PyBytes_FromStringAndSize(nullptr, (Py_ssize_t)(count * sizeof(UnblendAdamWTensor)));
+  PyObject* kinds = PyList_New(0);
+  char* to = bytes ? PyBytes_AS_STRING(bytes) : nullptr;
+  bool ok = bytes && kinds;
+  for (int k = 0; ok && k < 9; ++k) {
+    if (rows[k].empty()) continue;
+    const size_t len = rows[k].size() * sizeof(UnblendAdamWTensor);
+    std::memcpy(to, rows[k].data(), len);
+    to += len;
+    PyObject* kind = Py_BuildValue("(iin)", k / 3, k % 3, (Py_ssize_t)rows[k].size());
+    ok = kind && PyList_Append(kinds, kind) == 0;
+    Py_XDECREF(kind);
+  }
+  if (!ok) {
+    Py_XDECREF(bytes);
+    Py_XDECREF(kinds);
+    return nullptr;
+  }
+  return Py_BuildValue("(NNLL)", bytes, kinds, (long long)blocks, (long long)runs);
+  END_HANDLE_TH_ERRORS
 }
 
 // norm_outputs(like, with scale, bytes) -> (norm, scale or None, workspace) on like's device
@@ -174,16 +177,17 @@ PyObject* norm_outputs(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (n_args != 3 || !THPVariable_Check(args[0])) return refuse("norm_outputs(like, with scale, bytes)");
   const long long bytes = PyLong_AsLongLong(args[2]);
   if (bytes < 0) return PyErr_Occurred() ? nullptr : refuse("norm_outputs: bytes below 0");
-  try {
-    const at::TensorOptions options = at::TensorOptions().device(THPVariable_Unpack(args[0]).device());
-    const at::Tensor norm = at::empty({}, options.dtype(at::kFloat));
-    const at::Tensor scale = args[1] == Py_True ? at::empty({}, options.dtype(at::kFloat)) : at::Tensor();
-    const at::Tensor work = at::empty({bytes}, options.dtype(at::kByte));
-    return Py_BuildValue("(NNN)", wrap(norm), wrap(scale), wrap(work));
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());  // out of memory
-    return nullptr;
+  HANDLE_TH_ERRORS
+  const at::TensorOptions options = at::TensorOptions().device(THPVariable_Unpack(args[0]).device());
+  at::Tensor norm, scale, work;
+  {
+    const Unlocked unlocked;
+    norm = at::empty({}, options.dtype(at::kFloat));
+    if (args[1] == Py_True) scale = at::empty({}, options.dtype(at::kFloat));
+    work = at::empty({bytes}, options.dtype(at::kByte));
   }
+  return Py_BuildValue("(NNN)", wrap(norm), wrap(scale), wrap(work));
+  END_HANDLE_TH_ERRORS
 }
 
 // changed(params, grads): the parameters that have a gradient were written in place
@@ -345,93 +349,95 @@ long long pointer(const at::Tensor& t) { return (long long)reinterpret_cast<uint
 // gamma_k are wanted; workspace: address of unblend_qk_norm_rotary_grad_workspace.
 PyObject* heads(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   if (n_args != N_ARGS && n_args != N_ARGS + 4) return refuse("heads: wrong number of arguments");
-  try {
-    Call c;
-    const bool backward = n_args > N_ARGS;
-    const char* const names[2] = {backward ? "dq" : "q", backward ? "dk" : "k"};
-    if (!read(o, names, c)) return nullptr;
-    if (backward) {
-      for (int i = 0; i < 2; ++i) {
-        if ((o[N_ARGS + i] == Py_None) != (o[i] == Py_None))
-          return refuse(std::string(names[i]) + " must be given with its input, and only then");
-        if (o[i] == Py_None) continue;
-        if (!heads_ok(names[i] + 1, o[N_ARGS + i], c.q)) return nullptr;
-        if (THPVariable_Unpack(o[N_ARGS + i]).sizes() != THPVariable_Unpack(o[i]).sizes())
-          return refuse(std::string(names[i]) + " must have shape " + shape(THPVariable_Unpack(o[N_ARGS + i])) + ", got " +
-                        shape(THPVariable_Unpack(o[i])));
-      }
-    }
-    if (!c.q->is_cuda() || c.q->numel() == 0 || (c.k && c.k->numel() == 0)) Py_RETURN_NONE;
-    const at::NoGradGuard no_grad;
-    const int64_t d = c.q->dim();
-    const at::Tensor q = unit(*c.q), k = c.k ? unit(*c.k) : at::Tensor();
-    const at::Tensor q0 = backward ? unit(THPVariable_Unpack(o[N_ARGS])) : at::Tensor();
-    const at::Tensor k0 = backward && c.k ? unit(THPVariable_Unpack(o[N_ARGS + 1])) : at::Tensor();
-    at::Tensor freqs, positions, gammas[2], lens;
-    UnblendRotaryParams p{};
-    p.dtype = type_of(q);
-    p.outer = (int)q.size(0);
-    p.inner = d == 5 ? (int)q.size(1) : 1;
-    p.length = (int)q.size(d - 3);
-    p.heads = (int)q.size(d - 2);
-    p.k_heads = c.k ? (int)k.size(d - 2) : 0;
-    p.hd = (int)q.size(d - 1);
-    p.half = c.half;
-    p.scale = (float)c.scale;
-    p.eps = (float)c.eps;
-    if (c.freqs) {
-      freqs = c.freqs->contiguous();
-      p.pairs = (int)freqs.numel();
-      p.freqs = freqs.const_data_ptr();
-      p.freqs_f64 = freqs.scalar_type() == at::kDouble;
-    }
-    if (c.positions) {
-      positions = c.positions->contiguous();
-      p.positions = positions.const_data_ptr();
-      p.positions_i64 = positions.scalar_type() == at::kLong;
-      p.positions_stride = positions.dim() > 1 ? p.length : 0;
-    }
+  HANDLE_TH_ERRORS
+  Call c;
+  const bool backward = n_args > N_ARGS;
+  const char* const names[2] = {backward ? "dq" : "q", backward ? "dk" : "k"};
+  if (!read(o, names, c)) return nullptr;
+  if (backward) {
     for (int i = 0; i < 2; ++i) {
-      if (!c.gamma[i]) continue;
-      gammas[i] = c.gamma[i]->contiguous();
-      p.w_dtype = type_of(gammas[i]);
-      (i ? p.gamma_k : p.gamma_q) = gammas[i].const_data_ptr();
+      if ((o[N_ARGS + i] == Py_None) != (o[i] == Py_None))
+        return refuse(std::string(names[i]) + " must be given with its input, and only then");
+      if (o[i] == Py_None) continue;
+      if (!heads_ok(names[i] + 1, o[N_ARGS + i], c.q)) return nullptr;
+      if (THPVariable_Unpack(o[N_ARGS + i]).sizes() != THPVariable_Unpack(o[i]).sizes())
+        return refuse(std::string(names[i]) + " must have shape " + shape(THPVariable_Unpack(o[N_ARGS + i])) + ", got " +
+                      shape(THPVariable_Unpack(o[i])));
     }
-    if (c.lens) {
-      lens = c.lens->contiguous();
-      p.lens = lens.const_data_ptr<int>();
-    }
-    p.q = strides(q);
-    if (c.k) p.k = strides(k);
-    if (backward) p.q0 = strides(q0);
-    if (backward && c.k) p.k0 = strides(k0);
-    const at::Tensor q_out = at::empty(q.sizes(), q.options());
-    const at::Tensor k_out = c.k ? at::empty(k.sizes(), k.options()) : at::Tensor();
-    const auto address = [](const at::Tensor& t) { return t.defined() ? pointer(t) : 0LL; };
-    at::Tensor dgamma[2], work;
-    PyObject* addresses;
-    if (backward) {
-      if (PyObject_IsTrue(o[N_ARGS + 2]) > 0 && (c.gamma[0] || c.gamma[1])) {
-        const auto workspace = reinterpret_cast<int (*)(const UnblendRotaryParams*, long long*)>(
-            PyLong_AsVoidPtr(o[N_ARGS + 3]));
-        long long bytes = 0;
-        if (!workspace || workspace(&p, &bytes) != 0) return refuse("heads: no workspace for these sizes");
-        for (at::Tensor& d : dgamma) d = at::empty({p.hd}, gammas[c.gamma[0] ? 0 : 1].options());
-        work = at::empty({bytes}, q.options().dtype(at::kByte));
-      }
-      addresses = Py_BuildValue("(LLLLLLLLL)", address(q), address(k), address(q0), address(k0), address(q_out),
-                                address(k_out), address(dgamma[0]), address(dgamma[1]), address(work));
-    } else {
-      addresses = Py_BuildValue("(LLLL)", address(q), address(k), address(q_out), address(k_out));
-    }
-    return Py_BuildValue("(NNNNNy#(NNNNNNNNNNNN))", wrap(q_out), wrap(k_out), wrap(dgamma[0]), wrap(dgamma[1]), addresses,
-                         reinterpret_cast<const char*>(&p), (Py_ssize_t)sizeof(p), wrap(q), wrap(k), wrap(q0), wrap(k0),
-                         wrap(freqs), wrap(positions), wrap(gammas[0]), wrap(gammas[1]), wrap(lens), wrap(dgamma[0]),
-                         wrap(dgamma[1]), wrap(work));
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());  // out of memory
-    return nullptr;
   }
+  if (!c.q->is_cuda() || c.q->numel() == 0 || (c.k && c.k->numel() == 0)) Py_RETURN_NONE;
+  const at::NoGradGuard no_grad;
+  const int64_t d = c.q->dim();
+  const bool weights = backward && (c.gamma[0] || c.gamma[1]) && PyObject_IsTrue(o[N_ARGS + 2]) > 0;
+  int (*workspace)(const UnblendRotaryParams*, long long*) = nullptr;
+  if (weights) workspace = reinterpret_cast<decltype(workspace)>(PyLong_AsVoidPtr(o[N_ARGS + 3]));
+  const at::Tensor* const inputs[2] = {backward ? &THPVariable_Unpack(o[N_ARGS]) : nullptr,
+                                       backward && c.k ? &THPVariable_Unpack(o[N_ARGS + 1]) : nullptr};
+  at::Tensor q, k, q0, k0, freqs, positions, gammas[2], lens, q_out, k_out, dgamma[2], work;
+  {
+    const Unlocked unlocked;
+    q = unit(*c.q);
+    if (c.k) k = unit(*c.k);
+    if (inputs[0]) q0 = unit(*inputs[0]);
+    if (inputs[1]) k0 = unit(*inputs[1]);
+    if (c.freqs) freqs = c.freqs->contiguous();
+    if (c.positions) positions = c.positions->contiguous();
+    if (c.lens) lens = c.lens->contiguous();
+    for (int i = 0; i < 2; ++i)
+      if (c.gamma[i]) gammas[i] = c.gamma[i]->contiguous();
+    q_out = at::empty(q.sizes(), q.options());
+    if (c.k) k_out = at::empty(k.sizes(), k.options());
+    if (weights)
+      for (at::Tensor& g : dgamma) g = at::empty({q.size(d - 1)}, gammas[c.gamma[0] ? 0 : 1].options());
+  }
+  UnblendRotaryParams p{};
+  p.dtype = type_of(q);
+  p.outer = (int)q.size(0);
+  p.inner = d == 5 ? (int)q.size(1) : 1;
+  p.length = (int)q.size(d - 3);
+  p.heads = (int)q.size(d - 2);
+  p.k_heads = c.k ? (int)k.size(d - 2) : 0;
+  p.hd = (int)q.size(d - 1);
+  p.half = c.half;
+  p.scale = (float)c.scale;
+  p.eps = (float)c.eps;
+  if (c.freqs) {
+    p.pairs = (int)freqs.numel();
+    p.freqs = freqs.const_data_ptr();
+    p.freqs_f64 = freqs.scalar_type() == at::kDouble;
+  }
+  if (c.positions) {
+    p.positions = positions.const_data_ptr();
+    p.positions_i64 = positions.scalar_type() == at::kLong;
+    p.positions_stride = positions.dim() > 1 ? p.length : 0;
+  }
+  for (int i = 0; i < 2; ++i) {
+    if (!c.gamma[i]) continue;
+    p.w_dtype = type_of(gammas[i]);
+    (i ? p.gamma_k : p.gamma_q) = gammas[i].const_data_ptr();
+  }
+  if (c.lens) p.lens = lens.const_data_ptr<int>();
+  p.q = strides(q);
+  if (c.k) p.k = strides(k);
+  if (backward) p.q0 = strides(q0);
+  if (backward && c.k) p.k0 = strides(k0);
+  if (weights) {
+    long long bytes = 0;
+    if (!workspace || workspace(&p, &bytes) != 0) return refuse("heads: no workspace for these sizes");
+    const Unlocked unlocked;
+    work = at::empty({bytes}, q.options().dtype(at::kByte));
+  }
+  const auto address = [](const at::Tensor& t) { return t.defined() ? pointer(t) : 0LL; };
+  PyObject* addresses = backward
+                            ? Py_BuildValue("(LLLLLLLLL)", address(q), address(k), address(q0), address(k0),
+                                            address(q_out), address(k_out), address(dgamma[0]), address(dgamma[1]),
+                                            address(work))
+                            : Py_BuildValue("(LLLL)", address(q), address(k), address(q_out), address(k_out));
+  return Py_BuildValue("(NNNNNy#(NNNNNNNNNNNN))", wrap(q_out), wrap(k_out), wrap(dgamma[0]), wrap(dgamma[1]), addresses,
+                       reinterpret_cast<const char*>(&p), (Py_ssize_t)sizeof(p), wrap(q), wrap(k), wrap(q0), wrap(k0),
+                       wrap(freqs), wrap(positions), wrap(gammas[0]), wrap(gammas[1]), wrap(lens), wrap(dgamma[0]),
+                       wrap(dgamma[1]), wrap(work));
+  END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {
