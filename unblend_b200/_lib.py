@@ -207,11 +207,10 @@ _SIGNATURES = {
                                   ctypes.POINTER(AttnTrainParams), c_void_p],
     "unblend_attention_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_ll, ctypes.POINTER(AttnTrainParams), c_void_p],
-    "unblend_adamw_step": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
-                           ctypes.POINTER(AdamWParams), c_void_p],
+    # Parameters are a structure by reference or its bytes.
+    "unblend_adamw_step": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p],
     "unblend_adamw_values": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p],
     "unblend_grad_norm": [c_void_p, ctypes.POINTER(c_int), c_float, c_void_p, c_void_p, c_void_p, c_void_p],
-    # The parameters may be a RotaryParams by reference or its bytes.
     "unblend_rotary": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
     "unblend_qk_norm_rotary_forward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "unblend_qk_norm_rotary_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -13,6 +13,7 @@
 #include <torch/version.h>
 
 #include <cstdint>
+#include <cstdio>
 #include <cstring>
 #include <string>
 #include <vector>
@@ -190,16 +191,162 @@ PyObject* norm_outputs(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// changed(params, grads): the parameters that have a gradient were written in place
+// Whether x is a number in [low, high); its value.
+bool number(const char* name, PyObject* x, double low, double high, double& value) {
+  if (!PyBool_Check(x) && (PyFloat_Check(x) || PyLong_Check(x))) {
+    value = PyFloat_AsDouble(x);
+    if (value >= low && value < high) return true;
+    PyErr_Clear();  // an integer beyond all floats
+  }
+  char range[64];
+  std::snprintf(range, sizeof range, " must be a number in [%g, %g), got ", low, high);
+  PyObject* shown = PyObject_Repr(x);
+  if (!shown) return false;
+  const char* got = PyUnicode_AsUTF8(shown);
+  if (got) refuse(std::string(name) + range + got);
+  Py_DECREF(shown);
+  return false;
+}
+
+// Whether o is a tensor of one element on `device`.
+bool scalar_ok(const char* name, PyObject* o, at::ScalarType type, const at::Device& device) {
+  if (THPVariable_Check(o)) {
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (t.scalar_type() == type && t.device() == device && t.layout() == at::kStrided && t.numel() == 1 && !t.is_neg())
+      return true;
+  }
+  return raised(std::string(name) + " must be a " + (type == at::kLong ? "int64" : "float32") +
+                " tensor of one element on " + device.str());
+}
+
+// The blocks of a state's moments; -1 after a ValueError.
+int64_t state_blocks(PyObject* const* o) {
+  const bool eight = o[2] != Py_None;
+  static const char* const names[2] = {"exp_avg", "exp_avg_sq"};
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor* t = THPVariable_Check(o[i]) ? &THPVariable_Unpack(o[i]) : nullptr;
+    if (!t || t->layout() != at::kStrided || t->scalar_type() != (eight ? at::kByte : at::kFloat) || t->dim() != 1 ||
+        t->numel() % BLOCK || !t->is_contiguous() || t->is_neg() ||
+        reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16) {
+      refuse(std::string("state.") + names[i] + " must be contiguous " + (eight ? "uint8" : "float32") +
+             " from a 16-byte boundary on, whole blocks of " + std::to_string(BLOCK) +
+             (eight ? " (with scales)" : " (without scales)"));
+      return -1;
+    }
+  }
+  const at::Tensor &m = THPVariable_Unpack(o[0]), &v = THPVariable_Unpack(o[1]);
+  const int64_t blocks = m.numel() / BLOCK;
+  if (m.numel() != v.numel() || m.device() != v.device()) {
+    refuse("state.exp_avg and state.exp_avg_sq must have one shape and device");
+    return -1;
+  }
+  if (blocks && m.const_data_ptr() == v.const_data_ptr()) {
+    refuse("state.exp_avg and state.exp_avg_sq must be two tensors");
+    return -1;
+  }
+  if (eight) {
+    const at::Tensor* t = THPVariable_Check(o[2]) ? &THPVariable_Unpack(o[2]) : nullptr;
+    if (!t || t->layout() != at::kStrided || t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(0) != blocks ||
+        t->size(1) != 2 || !t->is_contiguous() || t->is_neg() || t->device() != m.device() ||
+        reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 8) {
+      refuse("state.scales must be contiguous float32 (" + std::to_string(blocks) + ", 2) on " + m.device().str());
+      return -1;
+    }
+  }
+  return blocks;
+}
+
+// state(exp_avg, exp_avg_sq, scales or None) -> blocks
+PyObject* state(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  if (n_args != 3) return refuse("state(exp_avg, exp_avg_sq, scales)");
+  HANDLE_TH_ERRORS
+  const int64_t blocks = state_blocks(args);
+  return blocks < 0 ? nullptr : PyLong_FromLongLong(blocks);
+  END_HANDLE_TH_ERRORS
+}
+
+// adamw(params, grads, exp_avg, exp_avg_sq, scales, step, lr, beta1, beta2, eps, weight_decay, grad_scale)
+//   -> (table, kinds, UnblendAdamWParams, addresses of the state's tensors)
+PyObject* adamw(PyObject* self, PyObject* const* args, Py_ssize_t n_args) {
+  if (n_args != 12) return refuse("adamw: wrong number of arguments");
+  HANDLE_TH_ERRORS
+  PyObject* got = table(self, args, 2);
+  if (!got) return nullptr;
+  const auto fail = [&] {
+    Py_DECREF(got);
+    return nullptr;
+  };
+  if (PyList_GET_SIZE(args[0]) == 0) {
+    refuse("params must hold at least one tensor");
+    return fail();
+  }
+  const at::Device device = THPVariable_Unpack(PyList_GET_ITEM(args[0], 0)).device();
+  const int64_t have = state_blocks(args + 2), want = PyLong_AsLongLong(PyTuple_GET_ITEM(got, 2));
+  if (have < 0) return fail();
+  if (have != want) {
+    refuse("state holds " + std::to_string(have) + " blocks of " + std::to_string(BLOCK) + " moments, params need " +
+           std::to_string(want));
+    return fail();
+  }
+  const at::Tensor& m = THPVariable_Unpack(args[2]);
+  if (m.device() != device) {
+    refuse("state is on " + m.device().str() + ", expected " + device.str());
+    return fail();
+  }
+  UnblendAdamWParams p{};
+  if (!number("betas[0]", args[7], 0, 1, p.beta1) || !number("betas[1]", args[8], 0, 1, p.beta2) ||
+      !number("eps", args[9], 0, 1e30, p.eps) || !number("weight_decay", args[10], 0, 1e18, p.weight_decay))
+    return fail();
+  if (p.eps > 0 && p.eps < 1.17549435e-38) {
+    refuse("eps must be 0 or a normal float32");
+    return fail();
+  }
+  PyObject* const step = args[5];
+  if (THPVariable_Check(step)) {
+    if (!scalar_ok("step", step, at::kLong, device)) return fail();
+    p.step_device = static_cast<const long long*>(THPVariable_Unpack(step).const_data_ptr());
+  } else {
+    p.step = PyLong_Check(step) && !PyBool_Check(step) ? PyLong_AsLongLong(step) : 0;
+    PyErr_Clear();
+    if (p.step < 1) {
+      refuse("step must be the update's number from 1 on, an int or an int64 tensor");
+      return fail();
+    }
+  }
+  if (THPVariable_Check(args[6])) {
+    if (!scalar_ok("lr", args[6], at::kFloat, device)) return fail();
+    p.lr_device = THPVariable_Unpack(args[6]).const_data_ptr<float>();
+  } else if (!number("lr", args[6], 0, 1e18, p.lr)) {
+    return fail();
+  }
+  if (args[11] != Py_None) {
+    if (!scalar_ok("grad_scale", args[11], at::kFloat, device)) return fail();
+    p.grad_scale = THPVariable_Unpack(args[11]).const_data_ptr<float>();
+  }
+  const auto address = [](PyObject* o) {
+    return o == Py_None ? 0LL : (long long)reinterpret_cast<uintptr_t>(THPVariable_Unpack(o).const_data_ptr());
+  };
+  PyObject* out = Py_BuildValue("(OOy#(LLL))", PyTuple_GET_ITEM(got, 0), PyTuple_GET_ITEM(got, 1),
+                                reinterpret_cast<const char*>(&p), (Py_ssize_t)sizeof(p), address(args[2]),
+                                address(args[3]), address(args[4]));
+  Py_DECREF(got);
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// changed(params, grads, state): the parameters that have a gradient, and the state's tensors, were written in place
 PyObject* changed(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
-  if (n_args != 2 || !listed(args[0]) || !listed(args[1]) || PyList_GET_SIZE(args[0]) != PyList_GET_SIZE(args[1]))
-    return refuse("changed(params, grads)");
-  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]); ++i) {
-    PyObject* o = PyList_GET_ITEM(args[0], i);
-    if (PyList_GET_ITEM(args[1], i) == Py_None || !THPVariable_Check(o)) continue;
+  if (n_args != 3 || !listed(args[0]) || !listed(args[1]) || PyList_GET_SIZE(args[0]) != PyList_GET_SIZE(args[1]) ||
+      !PyTuple_Check(args[2]))
+    return refuse("changed(params, grads, state)");
+  const auto bump = [](PyObject* o) {
+    if (!THPVariable_Check(o)) return;
     const at::Tensor& t = THPVariable_Unpack(o);
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  }
+  };
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]); ++i)
+    if (PyList_GET_ITEM(args[1], i) != Py_None) bump(PyList_GET_ITEM(args[0], i));
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(args[2]); ++i) bump(PyTuple_GET_ITEM(args[2], i));
   Py_RETURN_NONE;
 }
 
@@ -443,6 +590,8 @@ PyObject* heads(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
 PyMethodDef methods[] = {
     {"sizes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sizes)), METH_FASTCALL, nullptr},
     {"table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(table)), METH_FASTCALL, nullptr},
+    {"state", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(state)), METH_FASTCALL, nullptr},
+    {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw)), METH_FASTCALL, nullptr},
     {"norm_outputs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(norm_outputs)), METH_FASTCALL, nullptr},
     {"changed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(changed)), METH_FASTCALL, nullptr},
     {"heads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(heads)), METH_FASTCALL, nullptr},

@@ -858,28 +858,7 @@ def _check_state(state) -> int:
     """Blocks of a state's moments."""
     if not isinstance(state, AdamWState):
         raise ValueError(f"state must be an AdamWState, got {type(state).__name__}")
-    m, v, scales = state
-    t = torch.float32 if scales is None else torch.uint8
-    for name, x in (("exp_avg", m), ("exp_avg_sq", v)):
-        if not isinstance(x, torch.Tensor) or x.dtype != t or x.dim() != 1 or x.numel() % ADAMW_BLOCK or \
-                not x.is_contiguous() or x.data_ptr() % 16:
-            raise ValueError(f"state.{name} must be contiguous {t} from a 16-byte boundary on, whole blocks of "
-                             f"{ADAMW_BLOCK} ({'without' if scales is None else 'with'} scales)")
-    blocks = m.numel() // ADAMW_BLOCK
-    if m.shape != v.shape or m.device != v.device:
-        raise ValueError("state.exp_avg and state.exp_avg_sq must have one shape and device")
-    if blocks and m.data_ptr() == v.data_ptr():
-        raise ValueError("state.exp_avg and state.exp_avg_sq must be two tensors")
-    if scales is not None and (not isinstance(scales, torch.Tensor) or scales.dtype != torch.float32 or
-                               scales.shape != (blocks, 2) or not scales.is_contiguous() or
-                               scales.device != m.device or scales.data_ptr() % 8):
-        raise ValueError(f"state.scales must be contiguous float32 ({blocks}, 2) on {m.device}")
-    return blocks
-
-
-def _check_scalar(name: str, t, dtype: torch.dtype, device: torch.device) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.numel() != 1 or t.device != device or t.is_neg():
-        raise ValueError(f"{name} must be a {dtype} tensor of one element on {device}")
+    return _lib.tensor_lists().state(*state)
 
 
 def _number(name: str, x, low: float, high: float = math.inf) -> float:
@@ -908,47 +887,22 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     are rounded. A value that is not finite spoils its whole block.
     """
     params, grads = _check_list("params", params), _check_list("grads", grads)
-    table, kinds, blocks, _ = _lib.tensor_lists().table(params, grads)
-    if not params:
-        raise ValueError("params must hold at least one tensor")
-    have = _check_state(state)
-    if have != blocks:
-        raise ValueError(f"state holds {have} blocks of {ADAMW_BLOCK} moments, params need {blocks}")
-    device = params[0].device
-    if state.exp_avg.device != device:
-        raise ValueError(f"state is on {state.exp_avg.device}, expected {device}")
+    if not isinstance(state, AdamWState):
+        raise ValueError(f"state must be an AdamWState, got {type(state).__name__}")
     if not (isinstance(betas, (tuple, list)) and len(betas) == 2):
         raise ValueError(f"betas must be two numbers, got {betas!r}")
-    a = _lib.AdamWParams(0.0, _number("betas[0]", betas[0], 0, 1), _number("betas[1]", betas[1], 0, 1),
-                         _number("eps", eps, 0, 1e30), _number("weight_decay", weight_decay, 0, 1e18))
-    if 0 < eps < torch.finfo(torch.float32).smallest_normal:
-        raise ValueError(f"eps must be 0 or a normal float32, got {eps!r}")
-    if isinstance(step, torch.Tensor):
-        _check_scalar("step", step, torch.int64, device)
-        a.step_device = step.data_ptr()
-    elif isinstance(step, int) and not isinstance(step, bool) and 1 <= step < 1 << 62:
-        a.step = step
-    else:
-        raise ValueError(f"step must be the update's number from 1 on, got {step!r}")
-    if isinstance(lr, torch.Tensor):
-        _check_scalar("lr", lr, torch.float32, device)
-        a.lr_device = lr.data_ptr()
-    else:
-        a.lr = _number("lr", lr, 0, 1e18)
-    if grad_scale is not None:
-        _check_scalar("grad_scale", grad_scale, torch.float32, device)
-        a.grad_scale = grad_scale.data_ptr()
-    _check_cuda("params", state.exp_avg)
+    lists = _lib.tensor_lists()
+    table, kinds, p, moments = lists.adamw(params, grads, *state, step, lr, *betas, eps, weight_decay, grad_scale)
+    like = state.exp_avg
+    _check_cuda("params", like)
     if len(kinds) > 1:  # within a kind the entry point checks
         _check_apart(params, grads)
     bits = 32 if state.scales is None else 8
     at = ctypes.cast(ctypes.c_char_p(table), ctypes.c_void_p).value
     for t, tg, n in kinds:
-        _launch(state.exp_avg, "unblend_adamw_step", at, n, state.exp_avg.data_ptr(), state.exp_avg_sq.data_ptr(),
-                _lib.ptr(state.scales), bits, t, tg, ctypes.byref(a), kernels=-(-n // _TABLE))
+        _launch(like, "unblend_adamw_step", at, n, *moments, bits, t, tg, p, kernels=-(-n // _TABLE))
         at += n * _TABLE_ROW
-    _lib.tensor_lists().changed(params, grads)  # autograd refuses to use what it saved of them before
-    torch.autograd.graph.increment_version([t for t in state if t is not None])
+    lists.changed(params, grads, state)  # autograd refuses to use what it saved of them before
 
 
 def _check_apart(params: list, grads: list) -> None:
