@@ -87,6 +87,9 @@ def test_refuses():
                 lambda: training.adamw_views(p, torch.zeros(256)), lambda: training.adamw_moments(p)):
         with pytest.raises(ValueError):
             bad()
+    conv = torch.zeros(2, 3, 4, 4).to(memory_format=torch.channels_last)
+    with pytest.raises(ValueError, match="contiguous"):
+        training.adamw_state([conv])
     neg = torch.zeros(5, dtype=torch.complex64).conj().imag
     for bad in (lambda: step([neg, p[1]], g, s, 1), lambda: step(p, [neg, g[1]], s, 1)):
         with pytest.raises(ValueError):

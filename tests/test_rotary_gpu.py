@@ -193,6 +193,19 @@ def test_padded_batch(hd, pairs, t):
         assert not any(x[behind].any() for x in (*out2, *back2[:2]))
 
 
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_axial_lengths_and_scales(interleaved):
+    """Lengths of (outer, inner) sequences whose token axes are transposed; factors of 0 and below."""
+    f, w = _rand(9, seed=1), _rand(48, seed=2, shift=1.0)
+    axis = _rand(2, 21, 3, 2, 4, 48, seed=3, t=BF16)
+    q, k = (x.transpose(1, 2) for x in axis.unbind(3))
+    lens = torch.tensor([21, 0, 5, 20, 1, 13], device="cuda", dtype=torch.int32)
+    for scale in (0.0, -1.5, 1e-3):
+        _check_norm(q, k, w, w, f, None, interleaved, scale, lens=lens)
+        _check_norm(q, None, w, None, f, None, interleaved, scale, lens=lens)
+        _check_rotary(q, k, f, None, interleaved, scale)
+
+
 def test_norm_hard_rows():
     """Rows of zeros, tiny and huge rows; NaN and infinities stay in their row, but for the weights' gradient."""
     f, gq = _rand(32, seed=1), _rand(64, seed=2, shift=1.0)
@@ -383,7 +396,7 @@ def test_in_front_of_attention(t):
     z = torch.einsum("nihd,njhd->nhij", qd, kd) * hd**-0.5
     z = z.masked_fill(~see[:, None, None], -math.inf)
     o = torch.einsum("nhij,njhd->nihd", z.softmax(-1), vd) * see[..., None, None]
-    want = (o, *torch.autograd.grad(o, (x, a, b), dout.double()))
+    want = (o.detach(), *torch.autograd.grad(o, (x, a, b), dout.double()))
     for y, w in zip((x.detach() for x in got), want):
         # five stages, each rounding its operands and result to t; sums of many roundings average out
         rel = float((y.double() - w).norm() / w.norm())

@@ -357,7 +357,7 @@ __device__ __forceinline__ float reciprocal_root(float x) {
 
 // The arithmetic on a lane's pairs of one row: v the input (the output's gradient), w the forward's input for its gradient.
 // live: whether the row counts for the weights' gradients.
-template <typename T, int G, int MODE>
+template <typename T, int LAYOUT, int G, int MODE>
 __device__ __forceinline__ Pairs compute(const Args& a, const Factors<MODE>& f, unsigned turned, float inv_hd, Pairs v,
                                          const Pairs& w, bool live, Pairs& dgamma) {
   Pairs y;
@@ -381,11 +381,11 @@ __device__ __forceinline__ Pairs compute(const Args& a, const Factors<MODE>& f, 
     }
     if (2 * a.pairs != a.hd) {  // not 1 a - 0 b: b may be infinite
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (!(turned >> j & 1)) {
-          part_of(y.A, j) = part_of(v.A, j);
-          part_of(y.B, j) = part_of(v.B, j);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const bool turns = LAYOUT == HALF ? turned != 0 : turned >> j & 1;  // HALF: all of a lane's pairs or none
+        part_of(y.A, j) = turns ? part_of(y.A, j) : part_of(v.A, j);
+        part_of(y.B, j) = turns ? part_of(y.B, j) : part_of(v.B, j);
+      }
     }
   }
   if constexpr (MODE == NORM_BACKWARD) {
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(THREADS, resident(LAYOUT, sizeof(T), MODE)) ro
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const bool row = t.active && u * a.split < left;
-            Pairs y = compute<T, G, MODE>(a, f, at.turned, inv_hd, v[u], w[u], row && t.inside, d[side]);
+            Pairs y = compute<T, LAYOUT, G, MODE>(a, f, at.turned, inv_hd, v[u], w[u], row && t.inside, d[side]);
             if (MODE != ROTATE && !t.inside) zeros(y);
             T* const to = rows + (from + u) * ROW;
 #pragma unroll
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(THREADS, resident(LAYOUT, sizeof(T), MODE)) ro
             Pairs w;
             if constexpr (MODE == NORM_BACKWARD) w = pairs(from + U + u);
             const bool row = t.active && u * a.split < left;
-            Pairs y = compute<T, G, MODE>(a, f, at.turned, inv_hd, v, w, row && t.inside, d[side]);
+            Pairs y = compute<T, LAYOUT, G, MODE>(a, f, at.turned, inv_hd, v, w, row && t.inside, d[side]);
             if (row && at.has) {
               if (MODE != ROTATE && !t.inside) zeros(y);
               Piece<T, LAYOUT> r;
