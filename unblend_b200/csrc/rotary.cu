@@ -706,11 +706,20 @@ int launch_layout(Args& a, const Plan& pl, cudaStream_t st) {
   }
 }
 
+// Teams form the addresses of heads behind the last one too (and copy nothing from them), which have to be aligned like
+// the others. The stride of a single head is used for nothing else and may be any number: 0 in its place.
+UnblendHeadStrides steps(UnblendHeadStrides s, int heads) {
+  if (heads <= 1) s.head = 0;
+  return s;
+}
+
 template <int MODE>
 int run(Args& a, const UnblendRotaryParams* p, const void* q, const void* k, const void* q0, const void* k0, void* qo,
         void* ko, bool inverse, Plan& pl, cudaStream_t st) {
-  a.side[0] = Side{q, q0, qo, p->q, p->q0, MODE != ROTATE ? p->gamma_q : nullptr, p->heads, 0};
-  a.side[1] = Side{k, k0, ko, p->k, p->k0, MODE != ROTATE ? p->gamma_k : nullptr, p->k_heads, 0};
+  a.side[0] = Side{q, q0, qo, steps(p->q, p->heads), steps(p->q0, p->heads), MODE != ROTATE ? p->gamma_q : nullptr,
+                   p->heads, 0};
+  a.side[1] = Side{k, k0, ko, steps(p->k, p->k_heads), steps(p->k0, p->k_heads), MODE != ROTATE ? p->gamma_k : nullptr,
+                   p->k_heads, 0};
   a.freqs = p->freqs;
   a.positions = p->positions;
   a.lens = MODE != ROTATE ? p->lens : nullptr;
