@@ -1,0 +1,55 @@
+"""AdamW and the norm of gradients on the GPU at the edge of what they take."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from adamw_reference import M_TABLE, U_TABLE, codes
+from unblend_b200 import training
+
+pytestmark = pytest.mark.gpu
+
+F32 = torch.float32
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def test_every_ratio_gets_its_code():
+    """All fp32 numbers of 18 octaves as moments relative to a largest of 1, above, between and below the codes. With beta =
+    0 the step takes m = g, and u = sqrt(g^2) = g: the root of a rounded square is the number again in radix 2."""
+    n = 1 << 23
+    p = [torch.zeros((n + 254) // 255 * 256, device="cuda")]
+    state = training.adamw_state(p, 8)
+    for octave in range(18):
+        w = torch.arange(n, device="cuda", dtype=torch.int32) + ((127 - 1 - octave) << 23)
+        g = w.view(F32)
+        g = torch.nn.functional.pad(torch.where(w % 3 == 0, -g, g), (0, -n % 255)).view(-1, 255)
+        g = torch.nn.functional.pad(g, (1, 0), value=1.0).view(-1)
+        training.adamw_step(p, [g], state, 2, betas=(0.0, 0.0), eps=1.0)
+        assert bool((state.scales == 1).all())
+        m, _ = codes(g, M_TABLE)
+        same = (m == state.exp_avg) | ((m & 127 == 0) & (state.exp_avg & 127 == 0))
+        assert bool(same.all()), octave
+        u, _ = codes(g.abs(), U_TABLE)
+        assert torch.equal(u, state.exp_avg_sq), octave
+
+
+def test_roots_are_rounded_correctly():
+    """The scales of u are the roots of v, rounded once, for any size of v; zeros and NaN among them. One element
+    of each block has a moment, no gradient."""
+    n = 1 << 17
+    s = torch.exp2(torch.rand(n, device="cuda", generator=_gen(1)) * 136 - 73)  # s^2 from 2^-146 to 2^126
+    s[:4] = torch.tensor([0.0, 1.8e19, float("nan"), 1e-30], device="cuda")
+    p = [torch.zeros(n * 256, device="cuda")]
+    state = training.adamw_state(p, 8)
+    state.exp_avg_sq[77::256] = 255
+    state.scales[:, 1] = s
+    v = (s * s) * torch.tensor(0.9, dtype=F32, device="cuda")
+    training.adamw_step(p, [torch.zeros_like(p[0])], state, 2, betas=(0.5, 0.9))
+    want = v.double().sqrt().float()  # 53 bits are enough for the second rounding to change nothing
+    assert want[1].isfinite() and int(want.isnan().sum()) == 1
+    assert torch.equal(state.scales[:, 1].nan_to_num(-1.0), want.nan_to_num(-1.0))
+    assert not state.scales[:, 0].any()

@@ -8,11 +8,11 @@
 // device, and a captured graph keeps them) by bisection.
 //
 // In 32 bits HBM bounds it: 28 bytes per fp32 element, 6.5 TB/s (134 M parameters in 675 tensors: 575 us). In 8 bits 10 + 1/16
-// bytes per 16-bit element are few beside the codes' arithmetic, about 56 instructions per element of which half are the
-// integer pipe's (118 M bf16 parameters: 281 us, 4.0 TB/s, issue slots 71 % and integer pipe 56 % busy; 509 us with scalar
-// floats and 32-bit patterns for the codes). What helped: two floats, and two codes as bf16, per instruction; roots without a
-// branch for each; runs of consecutive blocks per warp, as the search took 10 instructions per element; the next block's
-// loads ahead of a block's arithmetic. Handing out the values: 180 us for the same (6.2 TB/s).
+// bytes per 16-bit element are few beside the codes' arithmetic, about 63 instructions per element of which half are the
+// integer pipe's (118 M bf16 parameters: 297 us, 3.8 TB/s, issue slots 73 % and integer pipe 54 % busy; 509 us with scalar
+// floats and 32-bit patterns for the codes). What helped: two floats, and two codes as bf16, per instruction; runs of
+// consecutive blocks per warp, as the search took 10 instructions per element; the next block's loads ahead of a block's
+// arithmetic. Handing out the values: 180 us for the same (6.2 TB/s).
 //
 // 8 bits: a block has two scales, the largest |m| and the largest u = sqrt(v). u is kept instead of v because its range is
 // half as many octaves. Codes are small floats relative to the scale, whose largest code is 1: m has a sign, 3 bits of
@@ -145,33 +145,6 @@ __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
-}
-
-// Correctly rounded roots of eight values (not below 0). An approximate reciprocal root y is off by 2^-22; s = v y and one
-// Newton step with the residual v - s^2, which an fma computes exactly, round as the true root does for every fp32 number
-// from 2^-80 on (compared with the library's for each of them). Zeros, smaller values, infinities and NaN take the library's
-// function, which tests each value for its own.
-__device__ __forceinline__ void roots(const float2 (&v)[4], float2 (&u)[4], float& top) {
-  float low = v[0].x;
-  top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 y;
-    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(v[i].x));
-    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(v[i].y));
-    const float2 s = mul2(v[i], y), h = mul2(y, both(0.5f));
-    u[i] = ub::fma2(ub::fma2(mul2(s, both(-1.f)), s, v[i]), h, s);
-    asm("min.f32 %0, %1, %2, %3;" : "=f"(low) : "f"(low), "f"(v[i].x), "f"(v[i].y));
-    top = top3(top, u[i].x, u[i].y);
-  }
-  if (!(low >= 0x1p-80f && top <= 3.402823466e38f)) {
-    top = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      u[i] = make_float2(__fsqrt_rn(v[i].x), __fsqrt_rn(v[i].y));
-      top = top3(top, u[i].x, u[i].y);
-    }
-  }
 }
 
 // 1 / top, 0 for a block of zeros (or below the normal range, where 1 / top could overflow).
@@ -337,7 +310,11 @@ __device__ __forceinline__ void update(Unit<T, TG, EIGHT, N>& x, const StepArgs&
       moments(i);
       top_m = top3(top_m, mv[i].x, mv[i].y);
     }
-    roots(uv, root_v, top_u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      root_v[i] = make_float2(__fsqrt_rn(uv[i].x), __fsqrt_rn(uv[i].y));
+      top_u = top3(top_u, root_v[i].x, root_v[i].y);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) param(i, root_v[i]);
   } else {
