@@ -5,7 +5,10 @@ from __future__ import annotations
 import pytest
 import torch
 
+from rotary_reference import TURN16
 from test_rotary_gpu import BF16, F16, F32, _check_norm, _check_rotary, _rand
+from training_reference import assert_within, half
+from unblend_b200 import training
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +31,24 @@ def test_one_head_of_any_stride(interleaved, t):
                 _check_rotary(q, k, f, None, interleaved)
                 _check_norm(q, k, w, None if k is None else w, f, None, interleaved,
                             dq=other if q.shape[-2] == 1 else many, dk=dk)
+
+
+@pytest.mark.parametrize("outer,inner,length,heads", [(3, 7, 999983, 1), (1, 1, 20000003, 1), (4194301, 5, 1, 1),
+                                                      (2, 4194305, 2, 1), (1, 3, 5, 1 << 20), (1, 1, 2, 999979),
+                                                      (32768, 1, 512, 1), (1, 65536, 255, 1)])
+def test_every_row_is_found(outer, inner, length, heads):
+    """Axes of many sizes around powers of two and primes: each row turns by the position given for it, an angle that is
+    its number. x = 1 + 0 i becomes its cosine and sine."""
+    x = torch.zeros(outer, inner, length, heads, 2, device="cuda", dtype=BF16)
+    x[..., 0] = 1
+    rows = outer * inner * length
+    number = torch.arange(rows, device="cuda").view(outer, inner, length)
+    f = torch.ones(1, device="cuda", dtype=torch.float64)
+    y = training.rotary_forward(x, None, f, number)[0].view(rows, heads, 2)
+    for first in range(0, rows, 1 << 21):  # not all in 64 bits at a time
+        part = slice(first, first + (1 << 21))
+        a = number.view(-1)[part, None].double()
+        want = torch.stack((a.cos(), a.sin()), -1)
+        assert_within("turned", y[part], want.expand(-1, heads, -1), half(BF16) * want.abs() + TURN16 + 2.0**-133)
+    y = training.rotary_forward(x, None, f)[0].view(-1, length, heads, 2)
+    assert torch.equal(y[:1].expand_as(y), y)  # rows counted from 0 in each sequence

@@ -59,16 +59,23 @@ struct Side {  // q or k
   int rounds;  // of a team's batches, the same for all of a token's teams
 };
 
-// n / d for n < 2^31 without a division (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+// n / d for n < 2^31 without a division, as a product with a rounded-up reciprocal of 31 + l bits behind the point, where
+// 2^l is the first power of two that is not below d:
+//
+//   m = floor(2^(31 + l) / d) + 1, so m d = 2^(31 + l) + e with 0 < e <= d <= 2^l, and
+//   n m / 2^(31 + l) = n / d + (n e / 2^(31 + l)) / d
+//
+// The last term is below 1 / d, as n e < 2^31 2^l: it never reaches the next integer. m is below 2^32, because d is above
+// 2^(l - 1) (m = 2^31 + 1 for powers of two). The upper half of 2 n m, which fits 64 bits, takes 32 of the 32 + l places.
 struct Divisor {
-  unsigned d, m, s;
+  unsigned d, m, l;
 
   Divisor() = default;
-  explicit Divisor(unsigned by) : d(by), s(0) {
-    while (s < 32 && (1ull << s) < by) ++s;
-    m = (unsigned)(((1ull << 32) * ((1ull << s) - by)) / by + 1);
+  explicit Divisor(unsigned by) : d(by), l(0) {
+    while ((1ull << l) < d) ++l;
+    m = (unsigned)((1ull << (31 + l)) / d + 1);
   }
-  __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(m, n) + n) >> s; }
+  __device__ __forceinline__ unsigned operator()(unsigned n) const { return __umulhi(2 * n, m) >> l; }
 };
 
 struct Args {
