@@ -53,3 +53,19 @@ def test_roots_are_rounded_correctly():
     assert want[1].isfinite() and int(want.isnan().sum()) == 1
     assert torch.equal(state.scales[:, 1].nan_to_num(-1.0), want.nan_to_num(-1.0))
     assert not state.scales[:, 0].any()
+
+
+@pytest.mark.parametrize("n", [1000, 3_000_000])  # one kernel, partial sums and a join
+def test_a_norm_beyond_fp32_skips_the_step(n):
+    """Finite gradients whose norm is no fp32 number: infinite, as it is handed out, and its factor NaN."""
+    grads = [torch.full((n,), 3e38, device="cuda")]
+    norm, scale = training.grad_norm(grads, 1.0)
+    assert norm.isinf() and scale.isnan()
+    p = [torch.ones(n, device="cuda")]
+    for bits in (32, 8):
+        state = training.adamw_state(p, bits)
+        training.adamw_step(p, grads, state, 1, grad_scale=scale)
+        assert bool((p[0] == 1).all()) and not any(bool(x.any()) for x in state if x is not None)
+    largest = torch.finfo(F32).max
+    norm, scale = training.grad_norm([torch.tensor([largest], device="cuda")], 1.0)  # the last one that is
+    assert float(norm) == largest and float(scale) == pytest.approx(1 / largest, rel=0, abs=2.0**-149)

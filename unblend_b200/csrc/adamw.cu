@@ -516,8 +516,9 @@ __device__ __forceinline__ double cta_squares(const Table<N>& tab) {
 
 __device__ __forceinline__ void norm_out(double sum, float max_norm, float* norm, float* scale) {
   const double r = sqrt(sum);
-  *norm = (float)r;
-  if (scale) *scale = !isfinite(r) ? (float)(r - r) : r > max_norm ? (float)(max_norm / r) : 1.f;
+  const float given = (float)r;  // infinite from half a step above the largest fp32 number on
+  *norm = given;
+  if (scale) *scale = !isfinite(given) ? given - given : r > max_norm ? (float)(max_norm / r) : 1.f;
 }
 
 template <typename T, int N>
