@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -52,3 +54,30 @@ def test_every_row_is_found(outer, inner, length, heads):
         assert_within("turned", y[part], want.expand(-1, heads, -1), half(BF16) * want.abs() + TURN16 + 2.0**-133)
     y = training.rotary_forward(x, None, f)[0].view(-1, length, heads, 2)
     assert torch.equal(y[:1].expand_as(y), y)  # rows counted from 0 in each sequence
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_norm_keeps_infinities_behind_the_pairs(interleaved, t):
+    """An infinity behind the pairs makes its row's reciprocal root 0: it becomes NaN itself, the other dims 0. Infinite and
+    NaN weights there reach no other dim either."""
+    for hd, pairs in ((64, 5), (64, 8), (64, 0), (50, 7), (128, 32), (33, 16)):
+        f, w = _rand(pairs, seed=1), _rand(hd, seed=2, shift=1.0)
+        for at in range(2 * pairs, hd, 3):
+            x = _rand(2, 9, 3, hd, seed=3, t=t)
+            clean = training.qk_norm_rotary_forward(x, None, w, None, f, None, interleaved)[0]
+            x[1, 4, 2, at], x[0, 8, 0, at] = math.inf, -math.inf
+            y = training.qk_norm_rotary_forward(x, None, w, None, f, None, interleaved)[0]
+            want = clean.clone()
+            for row in ((1, 4, 2), (0, 8, 0)):
+                want[row] = 0
+                want[(*row, at)] = math.nan
+            assert torch.equal(y.nan_to_num(7.0), want.nan_to_num(7.0)), (hd, pairs, at)
+            x = _rand(2, 9, 3, hd, seed=3, t=t)
+            for bad in (math.inf, math.nan):
+                g = w.clone()
+                g[at] = bad
+                y = training.qk_norm_rotary_forward(x, None, g, None, f, None, interleaved)[0]
+                assert not y[..., at].isfinite().any()
+                y[..., at] = clean[..., at]
+                assert torch.equal(y, clean), (hd, pairs, at)

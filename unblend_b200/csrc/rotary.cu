@@ -368,32 +368,38 @@ template <typename T, int LAYOUT, int G, int MODE>
 __device__ __forceinline__ Pairs compute(const Args& a, const Factors<MODE>& f, unsigned turned, float inv_hd, Pairs v,
                                          const Pairs& w, bool live, Pairs& dgamma) {
   Pairs y;
+  // What does not turn is x, not 1 a - 0 b: b may be infinite.
+  const auto keep = [&](Pairs x) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool turns = LAYOUT == HALF ? turned != 0 : turned >> j & 1;  // HALF: all of a lane's pairs or none
+      part_of(y.A, j) = turns ? part_of(y.A, j) : part_of(x.A, j);
+      part_of(y.B, j) = turns ? part_of(y.B, j) : part_of(x.B, j);
+    }
+  };
   if constexpr (MODE == NORM) {
     float2 ss = mul2(v.A[0], v.A[0]);
     ss = ub::fma2(v.A[1], v.A[1], ss);
     ss = ub::fma2(v.B[0], v.B[0], ss);
     ss = ub::fma2(v.B[1], v.B[1], ss);
     const float2 rstd = both(reciprocal_root<T>(team_sum<G>(ss.x + ss.y) * inv_hd + a.eps));
+    Pairs x;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const float2 A = mul2(v.A[k], rstd), B = mul2(v.B[k], rstd);
-      y.A[k] = ub::fma2(f.SB[k], B, mul2(f.CA[k], A));
-      y.B[k] = ub::fma2(f.SA[k], A, mul2(f.CB[k], B));
+      x.A[k] = mul2(f.CA[k], A);
+      x.B[k] = mul2(f.CB[k], B);
+      y.A[k] = ub::fma2(f.SB[k], B, x.A[k]);
+      y.B[k] = ub::fma2(f.SA[k], A, x.B[k]);
     }
+    if (2 * a.pairs != a.hd) keep(x);
   } else {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       y.A[k] = ub::fma2(f.SB[k], v.B[k], mul2(f.CA[k], v.A[k]));
       y.B[k] = ub::fma2(f.SA[k], v.A[k], mul2(f.CB[k], v.B[k]));
     }
-    if (2 * a.pairs != a.hd) {  // not 1 a - 0 b: b may be infinite
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool turns = LAYOUT == HALF ? turned != 0 : turned >> j & 1;  // HALF: all of a lane's pairs or none
-        part_of(y.A, j) = turns ? part_of(y.A, j) : part_of(v.A, j);
-        part_of(y.B, j) = turns ? part_of(y.B, j) : part_of(v.B, j);
-      }
-    }
+    if (2 * a.pairs != a.hd) keep(v);
   }
   if constexpr (MODE == NORM_BACKWARD) {
     const Pairs g = y;
