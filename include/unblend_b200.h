@@ -706,7 +706,7 @@ typedef struct {
   void* param;      /* n contiguous elements of dtype, updated in place (not read by unblend_grad_norm) */
   const void* grad; /* n contiguous elements of grad_dtype */
   long long n;      /* >= 1 */
-  long long block;  /* the tensor's moments start at element 256 * block of exp_avg and exp_avg_sq */
+  long long block;  /* < 2^31: the tensor's moments start at element 256 * block of exp_avg and exp_avg_sq */
 } UnblendAdamWTensor;
 
 typedef struct {
@@ -724,8 +724,9 @@ typedef struct {
  * bits 32: exp_avg and exp_avg_sq are float, whole blocks of 256 per tensor. bits 8: uint8 codes, and scales holds two
  * floats per block, the largest |m| and the largest u = sqrt(v). With c = code & 127 a code of exp_avg stands for the
  * float of the bit pattern (c + 889) << 20 (0 for c = 0) times the first scale, negative with bit 7; a code of exp_avg_sq
- * for the square of the pattern (code + 1777) << 19 (0 for 0) times the second. Parameters must not share memory with
- * one another or with a gradient (UNBLEND_ERR_OVERLAP).
+ * for the square of the pattern (code + 1777) << 19 (0 for 0) times the second. What the call writes
+ * (parameters, and the tensors' blocks of moments and scales) must not share memory within itself or with anything that
+ * the call reads (UNBLEND_ERR_OVERLAP).
  */
 int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, void* exp_avg, void* exp_avg_sq, float* scales,
                        int bits, int dtype, int grad_dtype, const UnblendAdamWParams* p, void* stream);

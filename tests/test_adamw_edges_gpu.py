@@ -6,15 +6,10 @@ import pytest
 import torch
 
 from adamw_reference import M_TABLE, U_TABLE, codes
+from test_adamw_gpu import BF16, F32, _gen, _model, _state
 from unblend_b200 import training
 
 pytestmark = pytest.mark.gpu
-
-F32 = torch.float32
-
-
-def _gen(seed):
-    return torch.Generator(device="cuda").manual_seed(seed)
 
 
 def test_every_ratio_gets_its_code():
@@ -69,3 +64,24 @@ def test_a_norm_beyond_fp32_skips_the_step(n):
     largest = torch.finfo(F32).max
     norm, scale = training.grad_norm([torch.tensor([largest], device="cuda")], 1.0)  # the last one that is
     assert float(norm) == largest and float(scale) == pytest.approx(1 / largest, rel=0, abs=2.0**-149)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_neighbours_in_one_buffer(bits):
+    """Parameters, gradients, moments, scales and the numbers of a step side by side in one allocation are apart."""
+    params, grads = _model(1, BF16)
+    state = _state(params, bits, 2)
+    parts = [*params, *grads, *(x for x in state if x is not None)]
+    size = [-(-x.nbytes // 16) * 16 for x in parts]
+    raw = torch.zeros(sum(size) + 32, device="cuda", dtype=torch.uint8)
+    inside = [x[:y.nbytes].view(y.dtype).view(y.shape) for x, y in zip(raw.split([*size, 32])[:-1], parts)]
+    for x, y in zip(inside, parts):
+        x.copy_(y)
+    n = len(params)
+    number, lr, gs = raw[-32:-24].view(torch.int64), raw[-24:-20].view(F32), raw[-16:-12].view(F32)
+    number.fill_(7), lr.fill_(1e-3), gs.fill_(0.5)
+    for p, g, s in ((params, grads, state), (inside[:n], inside[n:2 * n], training.AdamWState(*inside[2 * n:]))):
+        training.adamw_step(p, g, s, number, lr, grad_scale=gs)
+    for x, y in zip(inside, parts):
+        assert torch.equal(x, y)
+    assert int(number) == 7 and float(gs) == 0.5

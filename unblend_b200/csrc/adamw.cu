@@ -578,33 +578,87 @@ bool tensors_ok(const UnblendAdamWTensor* t, int count, bool params, int elem, i
   for (int i = 0; i < count; ++i) {
     if (t[i].n < 1 || t[i].n >= (1LL << 39) || !t[i].grad || reinterpret_cast<uintptr_t>(t[i].grad) % grad_elem)
       return false;
-    if (params && (!t[i].param || reinterpret_cast<uintptr_t>(t[i].param) % elem || t[i].block < 0)) return false;
+    if (params && (!t[i].param || reinterpret_cast<uintptr_t>(t[i].param) % elem || t[i].block < 0 ||
+                   t[i].block >= (1LL << 31)))
+      return false;
     units += (t[i].n + BLOCK - 1) / BLOCK;
   }
   return units < (1LL << 31);
 }
 
-// Whether no two parameters share memory with one another, nor a parameter with a gradient.
-bool apart(const UnblendAdamWTensor* t, int count, int elem, int grad_elem) {
-  struct Span {
-    uintptr_t from, to;
-  };
+struct Span {
+  uintptr_t from, to;
+};
+
+void in_order(Span* from, Span* to) {  // usually they are: allocated one after another
   const auto before = [](const Span& x, const Span& y) { return x.from < y.from; };
+  if (!std::is_sorted(from, to, before)) std::sort(from, to, before);
+}
+
+// The next of two lists in order.
+struct Merged {
+  const Span *a, *a_end, *b, *b_end;
+
+  bool empty() const { return a == a_end && b == b_end; }
+  bool first() const { return b == b_end || (a != a_end && a->from <= b->from); }
+  const Span& peek() const { return first() ? *a : *b; }
+  Span take() { return first() ? *a++ : *b++; }
+};
+
+// Whether what the call writes (parameters, moments, scales) shares memory neither within itself nor with what else it reads
+// (gradients, numbers on the device).
+bool apart(const UnblendAdamWTensor* t, int count, int elem, int grad_elem, int bits, const void* m, const void* v,
+           const void* scales, const UnblendAdamWParams* p) {
   std::vector<Span> spans(2 * (size_t)count);  // parameters, then gradients
+  std::vector<Span> blocks;                    // of the moments, joined where tensors follow one another
+  bool ordered = true;
   for (int i = 0; i < count; ++i) {
-    const uintptr_t p = reinterpret_cast<uintptr_t>(t[i].param), g = reinterpret_cast<uintptr_t>(t[i].grad);
-    spans[i] = Span{p, p + (uintptr_t)t[i].n * elem};
+    const uintptr_t w = reinterpret_cast<uintptr_t>(t[i].param), g = reinterpret_cast<uintptr_t>(t[i].grad);
+    spans[i] = Span{w, w + (uintptr_t)t[i].n * elem};
     spans[count + i] = Span{g, g + (uintptr_t)t[i].n * grad_elem};
+    const uintptr_t from = (uintptr_t)t[i].block, to = from + (uintptr_t)((t[i].n + BLOCK - 1) / BLOCK);
+    if (!blocks.empty() && from == blocks.back().to) {
+      blocks.back().to = to;
+    } else {
+      ordered &= blocks.empty() || from > blocks.back().to;
+      blocks.push_back(Span{from, to});
+    }
   }
-  for (Span* s : {spans.data(), spans.data() + count})  // usually they were allocated one after another
-    if (!std::is_sorted(s, s + count, before)) std::sort(s, s + count, before);
-  const Span *p = spans.data(), *p_end = p + count, *g = p_end, *g_end = g + count;
-  uintptr_t written = 0, seen = 0;  // ends of the parameters, and of both, so far
-  while (p < p_end || g < g_end) {
-    const bool param = g == g_end || (p < p_end && p->from <= g->from);
-    const Span& x = param ? *p++ : *g++;
-    if (x.from < (param ? seen : written)) return false;
-    if (param) written = std::max(written, x.to);
+  Span* const params = spans.data();
+  in_order(params, params + count);
+  in_order(params + count, params + 2 * count);
+  if (!ordered) {
+    in_order(blocks.data(), blocks.data() + blocks.size());
+    for (size_t i = 1; i < blocks.size(); ++i)
+      if (blocks[i].from < blocks[i - 1].to) return false;
+  }
+  std::vector<Span> moments, numbers;
+  moments.reserve(3 * blocks.size());
+  const auto add = [&](const void* base, uintptr_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base);
+    for (const Span& b : blocks) moments.push_back(Span{at + b.from * bytes, at + b.to * bytes});
+  };
+  add(m, BLOCK * bits / 8);
+  add(v, BLOCK * bits / 8);
+  if (bits == 8) add(scales, sizeof(float2));
+  in_order(moments.data(), moments.data() + moments.size());
+  numbers.reserve(3);
+  const auto number = [&](const void* x, uintptr_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+    if (x) numbers.push_back(Span{at, at + bytes});
+  };
+  number(p->step_device, sizeof(long long));
+  number(p->lr_device, sizeof(float));
+  number(p->grad_scale, sizeof(float));
+  in_order(numbers.data(), numbers.data() + numbers.size());
+  Merged written{params, params + count, moments.data(), moments.data() + moments.size()};
+  Merged only_read{params + count, params + 2 * count, numbers.data(), numbers.data() + numbers.size()};
+  uintptr_t end = 0, seen = 0;  // of what is written, and of all, so far
+  while (!written.empty() || !only_read.empty()) {
+    const bool write = only_read.empty() || (!written.empty() && written.peek().from <= only_read.peek().from);
+    const Span x = write ? written.take() : only_read.take();
+    if (x.from < (write ? seen : end)) return false;
+    if (write) end = std::max(end, x.to);
     seen = std::max(seen, x.to);
   }
   return true;
@@ -706,7 +760,8 @@ extern "C" int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, 
              reinterpret_cast<uintptr_t>(p->grad_scale) % 4 == 0);
   UB_REQUIRE(tensors_ok(tensors, count, true, elem_size(dtype), elem_size(grad_dtype)));
   try {
-    if (!apart(tensors, count, elem_size(dtype), elem_size(grad_dtype))) return UNBLEND_ERR_OVERLAP;
+    if (!apart(tensors, count, elem_size(dtype), elem_size(grad_dtype), bits, exp_avg, exp_avg_sq, scales, p))
+      return UNBLEND_ERR_OVERLAP;
   } catch (const std::bad_alloc&) {
     return (int)cudaErrorMemoryAllocation;
   }

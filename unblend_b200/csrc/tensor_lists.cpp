@@ -219,6 +219,17 @@ bool scalar_ok(const char* name, PyObject* o, at::ScalarType type, const at::Dev
                 " tensor of one element on " + device.str());
 }
 
+// Memory from one address up to another.
+struct Span {
+  uintptr_t from, to;
+  bool meets(const Span& o) const { return from < o.to && o.from < to && from < to && o.from < o.to; }
+};
+
+Span span_of(const at::Tensor& t) {  // of a contiguous tensor
+  const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  return Span{at, at + (uintptr_t)t.numel() * t.element_size()};
+}
+
 // The blocks of a state's moments; -1 after a ValueError.
 int64_t state_blocks(PyObject* const* o) {
   const bool eight = o[2] != Py_None;
@@ -240,8 +251,8 @@ int64_t state_blocks(PyObject* const* o) {
     refuse("state.exp_avg and state.exp_avg_sq must have one shape and device");
     return -1;
   }
-  if (blocks && m.const_data_ptr() == v.const_data_ptr()) {
-    refuse("state.exp_avg and state.exp_avg_sq must be two tensors");
+  if (span_of(m).meets(span_of(v))) {
+    refuse("state.exp_avg and state.exp_avg_sq must not share memory");
     return -1;
   }
   if (eight) {
@@ -250,6 +261,10 @@ int64_t state_blocks(PyObject* const* o) {
         t->size(1) != 2 || !t->is_contiguous() || t->is_neg() || t->device() != m.device() ||
         reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 8) {
       refuse("state.scales must be contiguous float32 (" + std::to_string(blocks) + ", 2) on " + m.device().str());
+      return -1;
+    }
+    if (span_of(*t).meets(span_of(m)) || span_of(*t).meets(span_of(v))) {
+      refuse("state.scales must not share memory with the moments");
       return -1;
     }
   }
@@ -263,6 +278,41 @@ PyObject* state(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const int64_t blocks = state_blocks(args);
   return blocks < 0 ? nullptr : PyLong_FromLongLong(blocks);
   END_HANDLE_TH_ERRORS
+}
+
+// Whether a step's tensors, the state and the numbers on the device (null: not given) share no memory: the state with any
+// tensor, a parameter or the state with a number. Parameters and gradients among themselves are left to the entry point.
+bool state_apart(PyObject* table, PyObject* kinds, PyObject* const* state, const UnblendAdamWParams& p) {
+  static const uintptr_t SIZE[3] = {4, 2, 2};  // by UnblendDtype
+  static_assert(UNBLEND_F32 == 0 && UNBLEND_BF16 < 3 && UNBLEND_F16 < 3, "SIZE");
+  Span moments[3] = {};
+  for (int i = 0; i < 3; ++i)
+    if (state[i] != Py_None) moments[i] = span_of(THPVariable_Unpack(state[i]));
+  Span numbers[3] = {};
+  const void* const at[3] = {p.step_device, p.lr_device, p.grad_scale};
+  for (int i = 0; i < 3; ++i) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(at[i]);
+    if (a) numbers[i] = Span{a, a + (i == 0 ? 8 : 4)};
+    for (const Span& m : moments)
+      if (numbers[i].meets(m)) return raised("step, lr and grad_scale must not share memory with the state");
+  }
+  const char* row_at = PyBytes_AS_STRING(table);
+  for (Py_ssize_t k = 0; k < PyList_GET_SIZE(kinds); ++k) {
+    PyObject* const kind = PyList_GET_ITEM(kinds, k);
+    const long types[2] = {PyLong_AsLong(PyTuple_GET_ITEM(kind, 0)), PyLong_AsLong(PyTuple_GET_ITEM(kind, 1))};
+    const Py_ssize_t n = PyLong_AsSsize_t(PyTuple_GET_ITEM(kind, 2));
+    for (Py_ssize_t i = 0; i < n; ++i, row_at += sizeof(UnblendAdamWTensor)) {
+      UnblendAdamWTensor row;
+      std::memcpy(&row, row_at, sizeof row);
+      const uintptr_t w = reinterpret_cast<uintptr_t>(row.param), g = reinterpret_cast<uintptr_t>(row.grad);
+      const Span param{w, w + (uintptr_t)row.n * SIZE[types[0]]}, grad{g, g + (uintptr_t)row.n * SIZE[types[1]]};
+      for (const Span& m : moments)
+        if (param.meets(m) || grad.meets(m)) return raised("params and grads must not share memory with the state");
+      for (const Span& x : numbers)
+        if (param.meets(x)) return raised("step, lr and grad_scale must not share memory with params");
+    }
+  }
+  return true;
 }
 
 // adamw(params, grads, exp_avg, exp_avg_sq, scales, step, lr, beta1, beta2, eps, weight_decay, grad_scale)
@@ -323,6 +373,7 @@ PyObject* adamw(PyObject* self, PyObject* const* args, Py_ssize_t n_args) {
     if (!scalar_ok("grad_scale", args[11], at::kFloat, device)) return fail();
     p.grad_scale = THPVariable_Unpack(args[11]).const_data_ptr<float>();
   }
+  if (!state_apart(PyTuple_GET_ITEM(got, 0), PyTuple_GET_ITEM(got, 1), args + 2, p)) return fail();
   const auto address = [](PyObject* o) {
     return o == Py_None ? 0LL : (long long)reinterpret_cast<uintptr_t>(THPVariable_Unpack(o).const_data_ptr());
   };

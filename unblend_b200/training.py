@@ -876,7 +876,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     ``p = (1 - lr weight_decay) p - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)``, in fp32, rounded once
     to the parameter's type. Parameters are contiguous fp32, bf16 or fp16 in any mixture, gradients likewise with a type of
     their own (fp32 parameters may be given 16-bit gradients). A gradient of None leaves its parameter and moments as
-    they are. Parameters that share memory are refused.
+    they are. Whatever the call writes, parameters and ``state``, must not share memory within itself or with another
+    argument.
 
     ``step`` is the number of this update, from 1: an int, or an int64 tensor on the device that the caller advances (for
     captured graphs, as ``lr`` may be an fp32 tensor). ``grad_scale`` (fp32 tensor, one element, such as the second result
