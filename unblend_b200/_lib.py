@@ -284,12 +284,19 @@ def tensor_lists():
     if _tensor_lists is None:
         import importlib.util
 
-        from .build import EXTENSION
+        from .build import EXTENSION, STAMP_SUFFIX, extension_stamp
 
         path = os.path.join(os.path.dirname(LIB_PATH), EXTENSION + ".so")
         load()
         if not os.path.exists(path):
-            raise RuntimeError(f"unblend_b200 extension not built ({path}); run `python -m unblend_b200.build`")
+            raise RuntimeError(f"unblend_b200 extension not built ({path}); run `python -m unblend_b200.build` with torch, "
+                               "g++ and Python's headers installed")
+        # Before it is loaded: what was built for another torch or Python may end in an undefined symbol.
+        if os.path.exists(path + STAMP_SUFFIX):
+            built = open(path + STAMP_SUFFIX).read()
+            if built != extension_stamp():
+                raise RuntimeError(f"{path} was built for {built}, this is {extension_stamp()}; run "
+                                   "`python -m unblend_b200.build`")
         spec = importlib.util.spec_from_file_location(EXTENSION, path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)

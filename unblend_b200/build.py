@@ -2,9 +2,11 @@
 
 Every ``csrc/*.cu`` file is compiled with ``nvcc -gencode
 arch=compute_100a,code=sm_100a`` and linked into one C-ABI shared library that
-the host code loads with ctypes, and ``csrc/tensor_lists.cpp`` into a Python extension
-beside it. Objects are rebuilt only when a source or header is newer. The FFT twiddle table (``csrc/twiddle4096.inc``) is generated
-here in double precision, so the kernels hold it as static module data.
+the host code loads with ctypes. That needs nvcc alone; where torch, g++ and Python's
+headers are installed, ``csrc/tensor_lists.cpp`` becomes a Python extension beside it.
+Objects are rebuilt only when a source or header is newer. The FFT twiddle table
+(``csrc/twiddle4096.inc``) is generated here in double precision, so the kernels hold
+it as static module data.
 
 Usage: ``python -m unblend_b200.build [-j N] [--force]``.
 """
@@ -78,30 +80,55 @@ def source_digest() -> str:
 
 
 EXTENSION = "tensor_lists"
+STAMP_SUFFIX = ".torch"
 
 
-def _extension(force: bool) -> None:
-    """The Python extension, against the headers of the installed torch."""
+def extension_stamp() -> str:
+    """What the extension is built for: another torch or Python needs another build."""
     import sysconfig
 
     import torch
-    from torch.utils.cpp_extension import include_paths, library_paths
+
+    return f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _extension(force: bool) -> str | None:
+    """Build the Python extension against the headers of the installed torch; on a machine that lacks what this needs,
+    return what that is (the library and its C interface need none of it)."""
+    import sysconfig
 
     src, out = os.path.join(CSRC, EXTENSION + ".cpp"), os.path.join(LIBDIR, EXTENSION + ".so")
-    stamp = out + ".torch"  # another torch needs another build
-    if not force and os.path.exists(out) and os.path.exists(stamp) and open(stamp).read() == torch.__version__ and \
-            os.path.getmtime(out) >= max(os.path.getmtime(src), _deps()):
-        return
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+    stamp = out + STAMP_SUFFIX
+    cxx = os.environ.get("CXX", "g++")
+    try:
+        from torch.utils.cpp_extension import include_paths, library_paths
+
+        import torch
+    except ImportError as e:
+        lacking: str | None = f"torch ({e})"
+    else:
+        lacking = cxx if shutil.which(cxx) is None else None
+        if not os.path.exists(os.path.join(sysconfig.get_path("include"), "Python.h")):
+            lacking = "Python.h"
+    if lacking is None and not force and os.path.exists(out) and os.path.exists(stamp) and \
+            open(stamp).read() == extension_stamp() and os.path.getmtime(out) >= max(os.path.getmtime(src), _deps()):
+        return None
+    for f in (out, stamp):  # from here on it does not belong to the library
+        if os.path.exists(f):
+            os.remove(f)
+    if lacking is not None:
+        return lacking
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f for p in include_paths() for f in ("-isystem", p)), "-isystem", sysconfig.get_path("include"),
            src, "-o", out + ".tmp", *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-lc10"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"g++ failed for {src}:\n{res.stderr}")
+        raise RuntimeError(f"{cxx} failed for {src}:\n{res.stderr}")
     os.replace(out + ".tmp", out)
     with open(stamp, "w") as f:
-        f.write(torch.__version__)
+        f.write(extension_stamp())
+    return None
 
 
 DIGEST_NAME = "libunblend_b200.digest"
@@ -126,7 +153,8 @@ def _compile(src: str, force: bool, log: list) -> str:
 
 
 def build(force: bool = False, jobs: int = 8, verbose: bool = False) -> str:
-    """Compile and link the library; return its path."""
+    """Compile and link the library, and build the extension beside it where torch, its compiler and Python's headers
+    are there; return the library's path."""
     os.makedirs(OBJDIR, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
     write_twiddles()
@@ -135,7 +163,6 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         extension = ex.submit(_extension, force)
         objs = list(ex.map(lambda s: _compile(s, force, log), sources))
-        extension.result()
     lib = os.path.join(LIBDIR, LIBNAME)
     if force or not os.path.exists(lib) or os.path.getmtime(lib) < max(os.path.getmtime(o) for o in objs):
         cmd = [nvcc(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", *objs, "-o", lib + ".tmp", "-lcuda"]
@@ -147,6 +174,10 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False) -> str:
     # library whose stamp differs from the sources next to it.
     with open(os.path.join(LIBDIR, DIGEST_NAME), "w") as f:
         f.write(source_digest() + "\n")
+    lacking = extension.result()  # raises after the library is in place
+    if lacking is not None:
+        print(f"{EXTENSION} not built, {lacking} is missing: the library and its C interface work without it, the rotary "
+              "operators, AdamW and the gradient norm of unblend_b200.training do not", file=sys.stderr)
     if verbose:
         for src, text in log:
             print(f"== {os.path.basename(src)}\n{text}")
