@@ -475,8 +475,9 @@ bool read(PyObject* const* o, const char* const (&names)[2], Call& c) {
   c.freqs = c.positions = c.lens = nullptr;
   if (o[FREQS] != Py_None) {
     c.freqs = THPVariable_Check(o[FREQS]) ? tensor(o[FREQS]) : nullptr;
-    if (!c.freqs || (c.freqs->scalar_type() != at::kFloat && c.freqs->scalar_type() != at::kDouble) ||
-        c.freqs->dim() != 1 || c.freqs->device() != q.device())
+    if (!c.freqs || c.freqs->layout() != at::kStrided ||
+        (c.freqs->scalar_type() != at::kFloat && c.freqs->scalar_type() != at::kDouble) || c.freqs->dim() != 1 ||
+        c.freqs->device() != q.device())
       return raised("freqs must be a float32 or float64 tensor [pairs] on " + q.device().str());
     if (2 * c.freqs->numel() > hd)
       return raised(std::to_string(c.freqs->numel()) + " pairs do not fit into head_dim " + std::to_string(hd));
@@ -486,7 +487,8 @@ bool read(PyObject* const* o, const char* const (&names)[2], Call& c) {
   }
   if (o[POSITIONS] != Py_None) {
     c.positions = THPVariable_Check(o[POSITIONS]) ? tensor(o[POSITIONS]) : nullptr;
-    if (!c.positions || (c.positions->scalar_type() != at::kInt && c.positions->scalar_type() != at::kLong) ||
+    if (!c.positions || c.positions->layout() != at::kStrided ||
+        (c.positions->scalar_type() != at::kInt && c.positions->scalar_type() != at::kLong) ||
         c.positions->device() != q.device())
       return raised("positions must be an int32 or int64 tensor on " + q.device().str());
     const auto all = q.sizes().slice(0, dims - 2), row = q.sizes().slice(dims - 3, 1);
@@ -497,8 +499,14 @@ bool read(PyObject* const* o, const char* const (&names)[2], Call& c) {
     PyErr_Clear();
     return raised("eps must be >= 0");
   }
+  if (THPVariable_Check(o[SCALE]) && THPVariable_Unpack(o[SCALE]).numel() != 1)
+    return raised("scale must be a number, got a tensor of shape " + shape(THPVariable_Unpack(o[SCALE])));
   c.scale = PyFloat_AsDouble(o[SCALE]);
-  if (c.scale == -1.0 && PyErr_Occurred()) return false;
+  if (c.scale == -1.0 && PyErr_Occurred()) {
+    if (!PyErr_ExceptionMatches(PyExc_TypeError) && !PyErr_ExceptionMatches(PyExc_OverflowError)) return false;
+    PyErr_Clear();
+    return raised(std::string("scale must be a number that fp32 holds, got ") + Py_TYPE(o[SCALE])->tp_name);
+  }
   if (!(c.scale >= -F32_MAX && c.scale <= F32_MAX))
     return raised("scale must be finite in float32, got " + std::to_string(c.scale));
   if (q.numel() >= MOST_ROWS * hd || (c.k && c.k->numel() >= MOST_ROWS * hd))
@@ -517,7 +525,8 @@ bool read(PyObject* const* o, const char* const (&names)[2], Call& c) {
   if (o[LENS] != Py_None) {
     c.lens = THPVariable_Check(o[LENS]) ? tensor(o[LENS]) : nullptr;
     const int64_t seqs = q.size(0) * (dims == 5 ? q.size(1) : 1);
-    if (!c.lens || c.lens->scalar_type() != at::kInt || c.lens->device() != q.device())
+    if (!c.lens || c.lens->layout() != at::kStrided || c.lens->scalar_type() != at::kInt ||
+        c.lens->device() != q.device())
       return raised("lens must be an int32 tensor on " + q.device().str());
     if (c.lens->numel() != seqs)
       return raised("lens must hold one length for each of " + std::to_string(seqs) + " sequences, got " +
