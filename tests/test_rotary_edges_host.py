@@ -33,3 +33,15 @@ def test_kinds_of_arguments(call):
 def test_sparse_lengths():
     with pytest.raises(ValueError, match="lens"):
         training.qk_norm_rotary(Q, K, None, None, F, lens=torch.ones(2, dtype=torch.int32).to_sparse())
+
+
+def test_frequencies_refuse_what_is_no_number():
+    for bad in (dict(base="10"), dict(base=None), dict(base=10**400), dict(factor="2"), dict(factor=None), dict(factor=[2.0]),
+                dict(method="parts", trained_length=9, slow="1"), dict(method="parts", trained_length=9, fast=None),
+                dict(method="parts", trained_length=9, slow=math.nan), dict(method=None)):
+        with pytest.raises(ValueError):
+            training.rotary_freqs(4, **bad)
+    same = training.rotary_freqs(4, 100.0, 2.0)
+    assert torch.equal(training.rotary_freqs(4, np.float32(100), torch.tensor(2.0)), same)
+    f = training.rotary_freqs(4, factor=2.0, method="parts", trained_length=9, fast=math.inf)
+    assert torch.equal(f, training.rotary_freqs(4, factor=2.0))  # nothing turns fast enough to be kept

@@ -475,6 +475,11 @@ def rotary_freqs(dims: int, base: float = 10000.0, factor: float = 1.0, method: 
     """
     if not isinstance(dims, int) or dims < 2 or dims % 2:
         raise ValueError(f"dims must be even and positive, got {dims!r}")
+    for name, x in (("base", base), ("factor", factor), ("slow", slow), ("fast", fast)):
+        try:
+            math.isfinite(x)
+        except (TypeError, OverflowError):
+            raise ValueError(f"{name} must be a number, got {x!r}") from None
     if not (base > 0 and math.isfinite(base)):
         raise ValueError(f"base must be positive, got {base!r}")
     if not (factor >= 1 and math.isfinite(factor)):
