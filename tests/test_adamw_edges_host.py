@@ -99,3 +99,14 @@ def test_entry_point_refuses_shared_moments():
             assert call(one, far, far + 65536, **{n: at}) == _lib.ERR_OVERLAP
         assert call(one, far, far + 512, far + 4096, 8, **{n: far + 4096 + 8}) == _lib.ERR_OVERLAP
     assert call([(p, p + 4096, 300, 1 << 31)], far, far + 65536) == _lib.ERR_INVALID
+
+
+def test_clipping_to_what_fp32_does_not_hold():
+    """Below the smallest fp32 number a largest norm would be 0."""
+    g = [torch.ones(5)]
+    for bad in (1e-46, 5e-324, -1e-50):
+        with pytest.raises(ValueError, match="max_norm must be"):
+            training.grad_norm(g, bad)
+    for good in (1e-45, 3e38, 1):
+        with pytest.raises(ValueError, match="CUDA devices only"):
+            training.grad_norm(g, good)

@@ -956,8 +956,8 @@ def grad_norm(grads: Sequence[torch.Tensor | None], max_norm: float | None = Non
     like = next((g for g in grads if g is not None), None)
     if like is None:
         raise ValueError("grads must hold at least one tensor")
-    if max_norm is not None and not (_number("max_norm", max_norm, 0) > 0 and max_norm <= _F32_MAX):
-        raise ValueError(f"max_norm must be positive, got {max_norm!r}")
+    if max_norm is not None and not (_number("max_norm", max_norm, 0) > 2.0**-150 and max_norm <= _F32_MAX):  # 0 in fp32
+        raise ValueError(f"max_norm must be positive in float32, got {max_norm!r}")
     _check_cuda("grads", like)
     counts = (ctypes.c_int * 3)()
     for _, t, n in kinds:
