@@ -81,3 +81,23 @@ def test_norm_keeps_infinities_behind_the_pairs(interleaved, t):
                 assert not y[..., at].isfinite().any()
                 y[..., at] = clean[..., at]
                 assert torch.equal(y, clean), (hd, pairs, at)
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_bits_behind_the_pairs(interleaved, t):
+    """What does not turn comes through bit for bit, signs of zeros and subnormal numbers too; NaN stay NaN."""
+    whole = torch.int32 if t == F32 else torch.int16
+    tiny, most = torch.finfo(t).smallest_normal, torch.finfo(t).max
+    values = torch.tensor([-0.0, math.inf, 0.0, -math.inf, math.nan, tiny / 4, -tiny / 2, most, -most, 1.0], device="cuda")
+    for hd, pairs in ((64, 5), (64, 8), (64, 0), (50, 7), (128, 32), (33, 16), (256, 100)):
+        f = _rand(pairs, seed=1)
+        q = _rand(2, 9, 3, hd, seed=2, t=t)
+        behind = q[..., 2 * pairs:]
+        behind.copy_(values.to(t).repeat(behind.numel() // 10 + 1)[:behind.numel()].view(behind.shape))
+        for call in (training.rotary_forward, training.rotary_backward):
+            y = call(q, None, f, None, interleaved, 3.0)[0]
+            got, nan = y[..., 2 * pairs:], behind.isnan()
+            assert nan.any() and torch.equal(got.isnan(), nan)
+            assert torch.equal(got.contiguous().view(whole)[~nan], behind.contiguous().view(whole)[~nan]), (hd, pairs)
+            assert y[..., :2 * pairs].isfinite().all()
