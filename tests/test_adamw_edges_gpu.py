@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from adamw_reference import M_TABLE, U_TABLE, codes
-from test_adamw_gpu import BF16, F32, _gen, _model, _state
+from test_adamw_gpu import BF16, F32, _check_step, _gen, _model, _state
 from unblend_b200 import training
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +85,55 @@ def test_neighbours_in_one_buffer(bits):
     for x, y in zip(inside, parts):
         assert torch.equal(x, y)
     assert int(number) == 7 and float(gs) == 0.5
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_steps(bits):
+    """Each of 150 steps from the state that the one before left, gradients of changing sizes."""
+    sizes = [(300,), (64, 5), (7,)]
+    params, grads = _model(3, BF16, sizes=sizes)
+    state = training.adamw_state(params, bits)
+    for n in range(1, 151):
+        for i, g in enumerate(grads):
+            g.copy_(torch.randn(g.shape, device="cuda", generator=_gen(10 * n + i)) * 10.0 ** (i - 3 - n // 50))
+        _check_step(params, grads, state, n, betas=(0.9, 0.999))
+
+
+def test_second_moments_in_8_bits_beside_a_larger_one():
+    """A root that shrinks by 0.05 % per step beside a steady one stays where it is, one that shrinks by 5 % (more than
+    half a code, at most 1/32) moves on with each step, and a block that shrinks as a whole does so by its scale."""
+    p, zero = [torch.zeros(256, device="cuda")], torch.zeros(256, device="cuda")
+    steady = zero.clone()
+    steady[0] = 1.0
+    for beta2, grad, steps in ((0.999, steady, 400), (0.999, zero, 400), (0.9, steady, 50)):
+        state = training.adamw_state(p, 8)
+        state.exp_avg_sq.copy_(torch.arange(255, -1, -1, device="cuda").clamp(min=100))
+        state.scales[:, 1] = 1.0
+        before = state.exp_avg_sq.clone()
+        for n in range(steps):
+            training.adamw_step(p, [grad], state, n + 1, betas=(0.9, beta2))
+        if beta2 == 0.9:
+            assert state.exp_avg_sq[0] == 255
+            assert bool((before[1:].int() - state.exp_avg_sq[1:].int() >= steps).all())
+        else:
+            assert torch.equal(state.exp_avg_sq, before)
+        # each step rounds its products and the root: 4 U
+        want = 1.0 if grad is steady else 0.999 ** (steps / 2)
+        assert abs(float(state.scales[0, 1]) - want) <= steps * 4 * 2.0**-24 * want + 3e-8 * steps * (grad is steady)
+
+
+def test_moments_behind_2_to_31():
+    """The last elements of a large tensor, over two steps, are those of a small one bit for bit; nothing else changes."""
+    n = (1 << 31) + 1001
+    start = (n - 3000) // 256 * 256
+    p, g = torch.zeros(n, device="cuda", dtype=BF16), torch.zeros(n, device="cuda", dtype=BF16)
+    small = [(torch.randn(n - start, device="cuda", generator=_gen(s)) * 0.1).to(BF16) for s in (1, 2)]
+    p[start:], g[start:] = small
+    state, little = training.adamw_state([p], 8), training.adamw_state(small[:1], 8)
+    for step in (1, 2):
+        training.adamw_step([p], [g], state, step)
+        _check_step(small[:1], small[1:], little, step, 1.0, lr=1e-3, betas=(0.9, 0.999), weight_decay=0.01)
+        for big, x, at in ((p, small[0], start), (state.exp_avg, little.exp_avg, start),
+                           (state.exp_avg_sq, little.exp_avg_sq, start), (state.scales, little.scales, start // 256)):
+            assert torch.equal(big[at:], x) and bool(x.any())
+            assert not big[:at].any()
