@@ -589,33 +589,31 @@ bool tensors_ok(const UnblendAdamWTensor* t, int count, bool params, int elem, i
 struct Span {
   uintptr_t from, to;
 };
+bool before(const Span& x, const Span& y) { return x.from < y.from; }
 
-void in_order(Span* from, Span* to) {  // usually they are: allocated one after another
-  const auto before = [](const Span& x, const Span& y) { return x.from < y.from; };
-  if (!std::is_sorted(from, to, before)) std::sort(from, to, before);
+// The spans of `list` in order, those up to `mid` and those from there each usually being so already.
+void in_order(std::vector<Span>& list, size_t mid) {
+  const auto parts = {list.begin(), list.begin() + mid, list.end()};
+  for (auto p = parts.begin(); p + 1 != parts.end(); ++p)
+    if (!std::is_sorted(p[0], p[1], before)) std::sort(p[0], p[1], before);
+  std::inplace_merge(list.begin(), list.begin() + mid, list.end(), before);
 }
-
-// The next of two lists in order.
-struct Merged {
-  const Span *a, *a_end, *b, *b_end;
-
-  bool empty() const { return a == a_end && b == b_end; }
-  bool first() const { return b == b_end || (a != a_end && a->from <= b->from); }
-  const Span& peek() const { return first() ? *a : *b; }
-  Span take() { return first() ? *a++ : *b++; }
-};
 
 // Whether what the call writes (parameters, moments, scales) shares memory neither within itself nor with what else it reads
 // (gradients, numbers on the device).
 bool apart(const UnblendAdamWTensor* t, int count, int elem, int grad_elem, int bits, const void* m, const void* v,
            const void* scales, const UnblendAdamWParams* p) {
-  std::vector<Span> spans(2 * (size_t)count);  // parameters, then gradients
-  std::vector<Span> blocks;                    // of the moments, joined where tensors follow one another
+  std::vector<Span> written, only_read, blocks;  // blocks: of the moments, joined where tensors follow one another
+  written.reserve((size_t)count + 3);
+  only_read.reserve((size_t)count + 3);
+  const auto span = [](const void* x, uintptr_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+    return Span{at, at + bytes};
+  };
   bool ordered = true;
   for (int i = 0; i < count; ++i) {
-    const uintptr_t w = reinterpret_cast<uintptr_t>(t[i].param), g = reinterpret_cast<uintptr_t>(t[i].grad);
-    spans[i] = Span{w, w + (uintptr_t)t[i].n * elem};
-    spans[count + i] = Span{g, g + (uintptr_t)t[i].n * grad_elem};
+    written.push_back(span(t[i].param, (uintptr_t)t[i].n * elem));
+    only_read.push_back(span(t[i].grad, (uintptr_t)t[i].n * grad_elem));
     const uintptr_t from = (uintptr_t)t[i].block, to = from + (uintptr_t)((t[i].n + BLOCK - 1) / BLOCK);
     if (!blocks.empty() && from == blocks.back().to) {
       blocks.back().to = to;
@@ -624,39 +622,28 @@ bool apart(const UnblendAdamWTensor* t, int count, int elem, int grad_elem, int 
       blocks.push_back(Span{from, to});
     }
   }
-  Span* const params = spans.data();
-  in_order(params, params + count);
-  in_order(params + count, params + 2 * count);
   if (!ordered) {
-    in_order(blocks.data(), blocks.data() + blocks.size());
+    std::sort(blocks.begin(), blocks.end(), before);
     for (size_t i = 1; i < blocks.size(); ++i)
       if (blocks[i].from < blocks[i - 1].to) return false;
   }
-  std::vector<Span> moments, numbers;
-  moments.reserve(3 * blocks.size());
-  const auto add = [&](const void* base, uintptr_t bytes) {
+  const auto moments = [&](const void* base, uintptr_t bytes) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(base);
-    for (const Span& b : blocks) moments.push_back(Span{at + b.from * bytes, at + b.to * bytes});
+    for (const Span& b : blocks) written.push_back(Span{at + b.from * bytes, at + b.to * bytes});
   };
-  add(m, BLOCK * bits / 8);
-  add(v, BLOCK * bits / 8);
-  if (bits == 8) add(scales, sizeof(float2));
-  in_order(moments.data(), moments.data() + moments.size());
-  numbers.reserve(3);
-  const auto number = [&](const void* x, uintptr_t bytes) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(x);
-    if (x) numbers.push_back(Span{at, at + bytes});
-  };
-  number(p->step_device, sizeof(long long));
-  number(p->lr_device, sizeof(float));
-  number(p->grad_scale, sizeof(float));
-  in_order(numbers.data(), numbers.data() + numbers.size());
-  Merged written{params, params + count, moments.data(), moments.data() + moments.size()};
-  Merged only_read{params + count, params + 2 * count, numbers.data(), numbers.data() + numbers.size()};
+  moments(m, BLOCK * bits / 8);
+  moments(v, BLOCK * bits / 8);
+  if (bits == 8) moments(scales, sizeof(float2));
+  if (p->step_device) only_read.push_back(span(p->step_device, sizeof(long long)));
+  if (p->lr_device) only_read.push_back(span(p->lr_device, sizeof(float)));
+  if (p->grad_scale) only_read.push_back(span(p->grad_scale, sizeof(float)));
+  in_order(written, count);
+  in_order(only_read, count);
+  const Span *w = written.data(), *w_end = w + written.size(), *r = only_read.data(), *r_end = r + only_read.size();
   uintptr_t end = 0, seen = 0;  // of what is written, and of all, so far
-  while (!written.empty() || !only_read.empty()) {
-    const bool write = only_read.empty() || (!written.empty() && written.peek().from <= only_read.peek().from);
-    const Span x = write ? written.take() : only_read.take();
+  while (w < w_end || r < r_end) {
+    const bool write = r == r_end || (w < w_end && w->from <= r->from);
+    const Span& x = write ? *w++ : *r++;
     if (x.from < (write ? seen : end)) return false;
     if (write) end = std::max(end, x.to);
     seen = std::max(seen, x.to);
@@ -742,10 +729,10 @@ int launch_squares(const UnblendAdamWTensor* t, int count, bool few, float max_n
   return 0;
 }
 
-}  // namespace
-
 // The update multiplies by an approximate reciprocal, which takes normal numbers only; the root of v is 0 or above 2^-75.
 bool eps_ok(double eps) { return eps == 0 || (eps >= 1.17549435e-38 && eps <= 1e30); }
+
+}  // namespace
 
 extern "C" int unblend_adamw_step(const UnblendAdamWTensor* tensors, int count, void* exp_avg, void* exp_avg_sq,
                                   float* scales, int bits, int dtype, int grad_dtype, const UnblendAdamWParams* p,

@@ -219,10 +219,10 @@ bool scalar_ok(const char* name, PyObject* o, at::ScalarType type, const at::Dev
                 " tensor of one element on " + device.str());
 }
 
-// Memory from one address up to another.
+// Memory from one address up to another, which is above it where two are compared.
 struct Span {
   uintptr_t from, to;
-  bool meets(const Span& o) const { return from < o.to && o.from < to && from < to && o.from < o.to; }
+  bool meets(const Span& o) const { return (from < o.to) & (o.from < to); }
 };
 
 Span span_of(const at::Tensor& t) {  // of a contiguous tensor
@@ -251,7 +251,7 @@ int64_t state_blocks(PyObject* const* o) {
     refuse("state.exp_avg and state.exp_avg_sq must have one shape and device");
     return -1;
   }
-  if (span_of(m).meets(span_of(v))) {
+  if (blocks && span_of(m).meets(span_of(v))) {
     refuse("state.exp_avg and state.exp_avg_sq must not share memory");
     return -1;
   }
@@ -263,7 +263,7 @@ int64_t state_blocks(PyObject* const* o) {
       refuse("state.scales must be contiguous float32 (" + std::to_string(blocks) + ", 2) on " + m.device().str());
       return -1;
     }
-    if (span_of(*t).meets(span_of(m)) || span_of(*t).meets(span_of(v))) {
+    if (blocks && (span_of(*t).meets(span_of(m)) || span_of(*t).meets(span_of(v)))) {
       refuse("state.scales must not share memory with the moments");
       return -1;
     }
@@ -285,17 +285,21 @@ PyObject* state(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 bool state_apart(PyObject* table, PyObject* kinds, PyObject* const* state, const UnblendAdamWParams& p) {
   static const uintptr_t SIZE[3] = {4, 2, 2};  // by UnblendDtype
   static_assert(UNBLEND_F32 == 0 && UNBLEND_BF16 < 3 && UNBLEND_F16 < 3, "SIZE");
-  Span moments[3] = {};
+  Span held[3], number[3];
+  int n_held = 0, n_number = 0;
   for (int i = 0; i < 3; ++i)
-    if (state[i] != Py_None) moments[i] = span_of(THPVariable_Unpack(state[i]));
-  Span numbers[3] = {};
-  const void* const at[3] = {p.step_device, p.lr_device, p.grad_scale};
-  for (int i = 0; i < 3; ++i) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(at[i]);
-    if (a) numbers[i] = Span{a, a + (i == 0 ? 8 : 4)};
-    for (const Span& m : moments)
-      if (numbers[i].meets(m)) return raised("step, lr and grad_scale must not share memory with the state");
-  }
+    if (state[i] != Py_None) held[n_held++] = span_of(THPVariable_Unpack(state[i]));
+  if (held[0].from == held[0].to) return true;  // nothing is written
+  const auto add = [&](const void* x, uintptr_t bytes) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x);
+    if (a) number[n_number++] = Span{a, a + bytes};
+  };
+  add(p.step_device, sizeof(long long));
+  add(p.lr_device, sizeof(float));
+  add(p.grad_scale, sizeof(float));
+  for (int i = 0; i < n_number; ++i)
+    for (int j = 0; j < n_held; ++j)
+      if (number[i].meets(held[j])) return raised("step, lr and grad_scale must not share memory with the state");
   const char* row_at = PyBytes_AS_STRING(table);
   for (Py_ssize_t k = 0; k < PyList_GET_SIZE(kinds); ++k) {
     PyObject* const kind = PyList_GET_ITEM(kinds, k);
@@ -306,10 +310,11 @@ bool state_apart(PyObject* table, PyObject* kinds, PyObject* const* state, const
       std::memcpy(&row, row_at, sizeof row);
       const uintptr_t w = reinterpret_cast<uintptr_t>(row.param), g = reinterpret_cast<uintptr_t>(row.grad);
       const Span param{w, w + (uintptr_t)row.n * SIZE[types[0]]}, grad{g, g + (uintptr_t)row.n * SIZE[types[1]]};
-      for (const Span& m : moments)
-        if (param.meets(m) || grad.meets(m)) return raised("params and grads must not share memory with the state");
-      for (const Span& x : numbers)
-        if (param.meets(x)) return raised("step, lr and grad_scale must not share memory with params");
+      bool meet = false, meet_number = false;
+      for (int j = 0; j < n_held; ++j) meet |= param.meets(held[j]) | grad.meets(held[j]);
+      for (int j = 0; j < n_number; ++j) meet_number |= param.meets(number[j]);
+      if (meet) return raised("params and grads must not share memory with the state");
+      if (meet_number) return raised("step, lr and grad_scale must not share memory with params");
     }
   }
   return true;
