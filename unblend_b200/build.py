@@ -104,7 +104,7 @@ def _extension(force: bool) -> str | None:
         from torch.utils.cpp_extension import include_paths, library_paths
 
         import torch
-    except ImportError as e:
+    except (ImportError, OSError) as e:  # OSError: a library of its own that does not load
         lacking: str | None = f"torch ({e})"
     else:
         lacking = cxx if shutil.which(cxx) is None else None

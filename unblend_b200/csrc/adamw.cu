@@ -37,7 +37,7 @@ using namespace ub::train;
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int BLOCK = 256;            // elements that share scales
 // CTAs per SM that the registers allow: in 8 bits a warp has two blocks in flight, for fp32 tensors of twice the size (134 M fp32
-// parameters with values: 616 us with two CTAs, 690 with three and spills).
+// parameters with values: 616 us with two CTAs, 658 with three and spills).
 constexpr int FULL_CTAS = 4;
 constexpr int eight_ctas(int elem, int grad_elem) { return elem + grad_elem > 4 ? 2 : 3; }
 constexpr int SMALL = 64, MIDDLE = 256, LARGE = 896;  // tensors of a launch: 2.3, 9 or 32 KB of kernel parameters
